@@ -1002,6 +1002,98 @@ int mlcg_sum_arrays(const float* const* arrays, int count, int64_t n, float* out
 int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
                     const int64_t* bytes, int count, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Sequence encoder: attention, group norm and dropout over chains of beads */
+/* ---------------------------------------------------------------------- */
+
+/* No counterparts in the reference.  Shared conventions: the beads of all
+ * chains lie one after the other; `dtype` is 0 fp32, 1 fp16, 2 bf16, the type
+ * of every `void*` array; sums, statistics and logits are fp32.  `tiles` holds
+ * n_tiles records of 4 int32 (16-byte aligned): a chain's first row, its
+ * length, the tile's first row within the chain (a multiple of the tile's
+ * rows) and the chain's number, one record for each tile of each chain, a
+ * chain's tiles one after the other; a chain of length 0 has none. */
+
+/* Attention of every bead to the present beads of its chain, with a bias by
+ * clipped relative position:
+ *   l_ij = scale q_i.k_j + table[bucket_of[clip(p_j - p_i, -reach, reach) + reach], h]
+ *   out_i = sum_j softmax_j(l_ij) v_j,  zeros where no bead is present.
+ * q is [beads, heads, dim], k and v [beads, kv_heads, dim] with the last axis
+ * contiguous and strides (row, head) in elements in host memory; heads is a
+ * multiple of kv_heads, head h reads key/value head h / (heads / kv_heads).
+ * table [buckets, heads]; bucket_of [2 reach + 1] with entries in
+ * [0, buckets); 1 <= reach <= 1024, 1 <= dim <= 128.  keep [beads]: 0 marks an
+ * absent bead, whose key and value are not read as numbers (NULL: all are
+ * present); positions [beads]: p, any int32 (NULL: the index in the chain).
+ * out [beads, heads, dim]; lse [heads, beads] (may be NULL): the base-2 log of
+ * the row's sum, +inf for a row without keys, which the backward pass takes.
+ * tile_rows, 32 or 128: the rows of the tiles in `tiles`.
+ *
+ * The backward pass gives the gradients of q, k, v (contiguous) and table.
+ * bucket_order [2 reach + 1] lists the offsets 0 .. 2 reach by bucket,
+ * bucket_first [buckets + 1] where each bucket's begin. */
+int64_t mlcg_chain_attention_workspace_floats(int64_t beads, int heads,
+                                              int64_t n_tiles, int buckets);
+int mlcg_chain_attention(const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, int64_t beads, int heads,
+                         int kv_heads, int dim, int dtype, const void* table,
+                         int buckets, const int32_t* bucket_of, int reach,
+                         float scale, const int32_t* tiles, int64_t n_tiles,
+                         int tile_rows, const uint8_t* keep,
+                         const int32_t* positions, void* out, float* lse,
+                         void* stream);
+int mlcg_chain_attention_backward(
+    const void* q, const int64_t* q_strides, const void* k,
+    const int64_t* k_strides, const void* v, const int64_t* v_strides,
+    int64_t beads, int heads, int kv_heads, int dim, int dtype,
+    const void* table, int buckets, const int32_t* bucket_of,
+    const int32_t* bucket_order, const int32_t* bucket_first, int reach,
+    float scale, const int32_t* tiles, int64_t n_tiles, int tile_rows,
+    const uint8_t* keep, const int32_t* positions, const void* out,
+    const float* lse, const void* grad_out, void* grad_q, void* grad_k,
+    void* grad_v, void* grad_table, float* workspace,
+    int64_t workspace_floats, void* stream);
+
+/* Group norm of every chain and activation, channels last: mean and biased
+ * variance over a chain's beads and the width / groups channels of a group,
+ * y = act((x - mean) / sqrt(var + eps) * weight + bias), act 0 tanh,
+ * 1 shifted softplus, 2 x sigmoid(x), 3 none.  x [rows, width] with row
+ * stride ld, y, grad_y and grad_x contiguous, width <= 1024.  stats
+ * [3, chains, groups] is kept for the backward pass: the mean, what its
+ * rounding left out, and 1 / sqrt(var + eps) (not written for a chain of
+ * length 0).  `size`: the rows of the tiles in `tiles`, at most
+ * mlcg_group_norm_slab_rows; first_tile [chains]: a chain's first tile, -1
+ * for a chain of length 0.  grad_bias_weight [2, width]: the gradient of bias,
+ * then of weight. */
+int mlcg_group_norm_slab_rows(int width, int dtype);
+int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t chains,
+                                         int width, int groups, int backward);
+int mlcg_group_norm_act(const void* x, int64_t ld, int64_t rows, int dtype,
+                        const void* weight, const void* bias, int width,
+                        int groups, const int32_t* tiles,
+                        const int32_t* first_tile, int64_t n_tiles, int size,
+                        int64_t chains, float eps, int act, void* y,
+                        float* stats, float* workspace,
+                        int64_t workspace_floats, void* stream);
+int mlcg_group_norm_act_backward(
+    const void* x, int64_t ld, const void* grad_y, int64_t rows, int dtype,
+    const void* weight, const void* bias, int width, int groups,
+    const int32_t* tiles, const int32_t* first_tile, int64_t n_tiles, int size,
+    int64_t chains, int act, const float* stats, void* grad_x, void* grad_bias_weight, float* workspace,
+    int64_t workspace_floats, void* stream);
+
+/* out[e] = residual[e] + (u16(e) >= threshold ? x[e] * 65536 /
+ * (65536 - threshold) : 0), u16(e) the half-word e % 8 (the low half of the
+ * first word first) of Philox4x32-10 with the key `seed` and the counter
+ * (e / 8, step); residual may be NULL.  threshold = round(65536 p) < 65536.
+ * step_dev, if not NULL, is read on the device in place of `step`, so that a
+ * recorded graph draws a new mask on every replay.  The gradient of x is the
+ * same call on the gradient of out without a residual. */
+int mlcg_dropout_add(const void* x, const void* residual, int64_t n, int dtype,
+                     int threshold, uint64_t seed, const int64_t* step_dev,
+                     int64_t step, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -151,6 +151,19 @@ _SIGNATURES = {
     "mlcg_mse_workspace_floats": [_I64],
     "mlcg_mse_mean": [_P, _P, _I64, _P, _P, _I64, _P],
     "mlcg_mse_mean_backward": [_P, _P, _P, _I64, _P, _P],
+    "mlcg_chain_attention_workspace_floats": [_I64, _I32, _I64, _I32],
+    "mlcg_chain_attention": [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I32, _P,
+        _I32, _F32, _P, _I64, _I32, _P, _P, _P, _P, _P],
+    "mlcg_chain_attention_backward": [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P,
+        _I32, _P, _P, _P, _I32, _F32, _P, _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+        _I64, _P],
+    "mlcg_group_norm_slab_rows": [_I32, _I32],
+    "mlcg_group_norm_workspace_floats": [_I64, _I64, _I32, _I32, _I32],
+    "mlcg_group_norm_act": [_P, _I64, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64, _I32, _I64,
+        _F32, _I32, _P, _P, _P, _I64, _P],
+    "mlcg_group_norm_act_backward": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64,
+        _I32, _I64, _I32, _P, _P, _P, _P, _I64, _P],
+    "mlcg_dropout_add": [_P, _P, _I64, _I32, _I32, _U64, _P, _I64, _P, _P],
 }
 _RESTYPES = {"mlcg_version": _c.c_char_p, "mlcg_scan_workspace_ints": _I64,
              "mlcg_radius_workspace_bytes": _I64,
@@ -164,6 +177,8 @@ _RESTYPES = {"mlcg_version": _c.c_char_p, "mlcg_scan_workspace_ints": _I64,
              "mlcg_out_rev2_workspace_floats": _I64,
              "mlcg_rbf_param_grad_workspace_floats": _I64,
              "mlcg_type_sum_workspace_floats": _I64, "mlcg_node_weight_image_bytes": _I64,
+             "mlcg_chain_attention_workspace_floats": _I64,
+             "mlcg_group_norm_workspace_floats": _I64,
              "mlcg_mse_workspace_floats": _I64, "mlcg_prior_pair_records_ints": _I64,
              "mlcg_mfma_loop_flops_per_wave_iter": _I64}
 

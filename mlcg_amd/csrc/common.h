@@ -57,6 +57,10 @@ __device__ __forceinline__ float mlcg_wave_sum(float v) {
 // Activation ids shared by the filter network, the interaction block and the
 // output network (they are one module instance in StandardSchNet).
 enum { MLCG_ACT_TANH = 0, MLCG_ACT_SSP = 1 };
+// ... and two that only the group norm has: x sigmoid(x), and none.
+enum { MLCG_ACT_SILU = 2, MLCG_ACT_NONE = 3 };
+// Element types of the entry points that take more than one.
+enum { MLCG_DTYPE_F32 = 0, MLCG_DTYPE_F16 = 1, MLCG_DTYPE_BF16 = 2 };
 // Cutoff ids for the RBF envelope and the CFConv envelope.
 enum { MLCG_CUT_IDENTITY = 0, MLCG_CUT_COSINE = 1 };
 

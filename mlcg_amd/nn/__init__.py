@@ -9,7 +9,9 @@ from .prior import (Dihedral, FourierSeries, Harmonic, HarmonicAngles, HarmonicB
 from .radial_basis import ExpNormalBasis, GaussianBasis
 from .schnet import CFConv, InteractionBlock, SchNet, StandardSchNet
 
-__all__ = ["ShiftedSoftplus", "CosineCutoff", "IdentityCutoff", "EnergyOut", "GradientsOut",
+from .chain import chain_attention, dropout_add, group_norm_act
+
+__all__ = ["chain_attention", "dropout_add", "group_norm_act", "ShiftedSoftplus", "CosineCutoff", "IdentityCutoff", "EnergyOut", "GradientsOut",
            "SumOut", "EnergyMSE", "ForceMSE", "ForceRMSE", "Loss", "MLP",
            "init_xavier_uniform", "GaussianBasis", "ExpNormalBasis", "CFConv",
            "InteractionBlock", "SchNet", "StandardSchNet", "Harmonic", "HarmonicBonds",

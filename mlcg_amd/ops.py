@@ -13,6 +13,7 @@ import math
 from dataclasses import dataclass
 from typing import List, Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -1751,4 +1752,395 @@ def philox_normals(seed: int, step: int, n: int, device) -> torch.Tensor:
     out = torch.empty(n, 3, dtype=torch.float32, device=device)
     call("mlcg_philox_normals", int(seed) & ((1 << 64) - 1), int(step), n, ptr(out),
          stream_handle(torch.device(device)))
+    return out
+
+
+# --------------------------------------------------------------------------
+# Sequence encoder: attention, group norm and dropout over chains of beads
+
+DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CHAIN_TILE_ROWS = (32, 64, 128, 256)  # the tiles a ChainLayout lists
+CHAIN_ACTS = {"tanh": 0, "ssp": 1, "silu": 2, "none": 3}
+MAX_ATTENTION_DIM = 128
+MAX_ATTENTION_REACH = 1024
+MAX_NORM_WIDTH = 1024
+
+
+@dataclass(eq=False)
+class ChainLayout:
+    """Where the chains of a packed [S, ...] array begin and end, and the
+    tiles that the kernels go through (built once by chain_layout, on the
+    device).
+
+    lengths : beads of every chain, on the host
+    ptr     : [n_chains + 1] int64, each chain's first bead
+    tiles   : {rows: [n, 4] int32}, for tiles of 32, 64, 128 and 256 beads the
+              records (chain's first bead, its length, the tile's first bead in
+              it, chain), the longest chains first
+    first   : {rows: [n_chains] int32}, a chain's first tile, -1 without beads
+    """
+
+    lengths: Tuple[int, ...]
+    n_chains: int
+    n_beads: int
+    max_len: int
+    device: torch.device
+    ptr: torch.Tensor
+    tiles: dict
+    first: dict
+
+
+def chain_layout(lengths, device) -> ChainLayout:
+    """ChainLayout of chains with these numbers of beads (a sequence or a
+    tensor; a tensor on the GPU is read back once).  Lengths may be zero."""
+    if isinstance(lengths, torch.Tensor):
+        _check(not lengths.is_floating_point() and lengths.dtype != torch.bool,
+               "chain lengths must be integers")
+        lengths = lengths.detach().cpu().numpy()
+    lens = np.asarray(lengths)
+    _check(lens.ndim == 1 and (lens.size == 0 or np.issubdtype(lens.dtype, np.integer)),
+           "chain lengths must be a 1-D sequence of integers")
+    lens = lens.astype(np.int64)
+    _check(lens.size < 2 ** 31 and bool((lens >= 0).all()),
+           "chain lengths must not be negative")
+    total = int(lens.sum())
+    _check(total < 2 ** 31 - 256, "a ChainLayout holds less than 2^31 - 256 beads")
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    start = np.concatenate([[0], np.cumsum(lens)])
+    order = np.argsort(-lens, kind="stable")  # long chains begin first
+    parts, sizes = [], []
+    for rows in CHAIN_TILE_ROWS:
+        count = (lens[order] + rows - 1) // rows
+        chain = np.repeat(order, count)
+        begin = np.concatenate([[0], np.cumsum(count)])
+        within = (np.arange(begin[-1]) - np.repeat(begin[:-1], count)) * rows
+        parts.append(np.stack([start[chain], lens[chain], within, chain], 1).reshape(-1))
+        first = np.full(lens.size, -1, dtype=np.int64)
+        first[order] = np.where(count > 0, begin[:-1], -1)
+        sizes.append((int(begin[-1]), first))
+    firsts = [f for _, f in sizes]
+    packed = torch.from_numpy(np.concatenate(parts + firsts).astype(np.int32)).to(device)
+    tiles, first, at = {}, {}, 0
+    for rows, (n, _) in zip(CHAIN_TILE_ROWS, sizes):
+        tiles[rows] = packed[at:at + 4 * n].view(n, 4)
+        at += 4 * n
+    for rows in CHAIN_TILE_ROWS:
+        first[rows] = packed[at:at + lens.size]
+        at += lens.size
+    return ChainLayout(lengths=tuple(lens.tolist()), n_chains=int(lens.size), n_beads=total,
+                       max_len=int(lens.max()) if lens.size else 0, device=device,
+                       ptr=torch.from_numpy(start).to(device), tiles=tiles, first=first)
+
+
+@dataclass(eq=False)
+class RelativeBuckets:
+    """The buckets of relative positions (built by relative_buckets).
+
+    bucket_of : [2 reach + 1] int32, the bucket of the offset d - reach,
+                -reach <= d <= reach; offsets beyond belong to the ends'
+    order     : [2 reach + 1] int32, the offsets' indices by bucket
+    first     : [num_buckets + 1] int32, where each bucket's begin in order
+    """
+
+    num_buckets: int
+    reach: int
+    bucket_of: torch.Tensor
+    order: torch.Tensor
+    first: torch.Tensor
+
+
+def relative_bucket_table(num_buckets: int, reach: int, kind: str = "log") -> List[int]:
+    """The bucket of every offset -reach .. reach.
+
+    "clip": one bucket an offset (num_buckets = 2 reach + 1).  "log": half of
+    the buckets serve offsets up to 0 (0, -1, ...), half the positive ones; of
+    the n buckets of a direction the first n // 2 hold one offset each and
+    the others offsets in equal ratios up to `reach`."""
+    _check(isinstance(num_buckets, int) and isinstance(reach, int),
+           "num_buckets and reach must be integers")
+    _check(1 <= reach <= MAX_ATTENTION_REACH,
+           f"reach must lie in 1 .. {MAX_ATTENTION_REACH}, got {reach}")
+    if kind == "clip":
+        _check(num_buckets == 2 * reach + 1,
+               f"one bucket an offset: num_buckets must be 2 reach + 1 = {2 * reach + 1}")
+        return list(range(num_buckets))
+    _check(kind == "log", f"kind must be 'log' or 'clip', got {kind!r}")
+    _check(num_buckets >= 2, "num_buckets must be at least 2")
+    side = num_buckets // 2
+    exact = max(1, side // 2)
+    table = []
+    for d in range(-reach, reach + 1):
+        n = abs(d)
+        if n >= exact:
+            share = 1.0
+            if reach > exact:
+                share = math.log(n / exact) / math.log(reach / exact)
+            # the small addend keeps offsets whose exact share is a whole
+            # number in the bucket that begins there
+            n = exact + int(share * (side - exact) + 1e-9)
+        table.append(min(n, side - 1) + (side if d > 0 else 0))
+    return table
+
+
+def relative_buckets(num_buckets: int, reach: int, kind="log", device="cuda") -> RelativeBuckets:
+    """RelativeBuckets of a scheme of relative_bucket_table, or of a table of
+    one's own: `kind` may be the 2 reach + 1 buckets themselves."""
+    if isinstance(kind, str):
+        table = relative_bucket_table(num_buckets, reach, kind)
+    else:
+        table = [int(b) for b in kind]
+        _check(1 <= reach <= MAX_ATTENTION_REACH,
+               f"reach must lie in 1 .. {MAX_ATTENTION_REACH}, got {reach}")
+        _check(len(table) == 2 * reach + 1, f"a table of buckets has 2 reach + 1 = "
+                                            f"{2 * reach + 1} entries, got {len(table)}")
+        _check(num_buckets >= 1 and all(0 <= b < num_buckets for b in table),
+               f"buckets must lie in 0 .. {num_buckets - 1}")
+    bucket = np.asarray(table, dtype=np.int64)
+    order = np.argsort(bucket, kind="stable")
+    first = np.searchsorted(bucket[order], np.arange(num_buckets + 1))
+    packed = torch.from_numpy(np.concatenate([bucket, order, first]).astype(np.int32)).to(device)
+    n = len(table)
+    return RelativeBuckets(num_buckets=num_buckets, reach=reach, bucket_of=packed[:n],
+                           order=packed[n:2 * n], first=packed[2 * n:])
+
+
+def _chain_dtype(t: torch.Tensor, what: str) -> int:
+    dt = DTYPE_IDS.get(t.dtype)
+    _check(dt is not None, lambda: f"{what} takes float32, float16 or bfloat16, got {t.dtype}")
+    return dt
+
+
+def _attention_heads(t: torch.Tensor, name: str, chains: ChainLayout, like: torch.Tensor):
+    """t as [S, heads, dim] with a contiguous last axis, and its strides."""
+    _check(t.dim() == 3 and t.shape[0] == chains.n_beads and t.dtype == like.dtype
+           and t.device == like.device,
+           lambda: f"{name} must be [{chains.n_beads}, heads, dim] {like.dtype} on "
+                   f"{like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        t = t.contiguous()
+    return t, (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+
+
+def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions):
+    require_device(q, k, v, table, keep, positions)
+    dt = _chain_dtype(q, "chain_attention")
+    _check(isinstance(chains, ChainLayout) and chains.device == q.device,
+           "chains must be a ChainLayout on the queries' device")
+    q, qs = _attention_heads(q, "q", chains, q)
+    k, ks = _attention_heads(k, "k", chains, q)
+    v, vs = _attention_heads(v, "v", chains, q)
+    n, heads, dim = q.shape
+    kv = k.shape[1]
+    _check(k.shape == v.shape and k.shape[2] == dim,
+           lambda: f"k and v must be [{n}, kv_heads, {dim}], got {tuple(k.shape)} and "
+                   f"{tuple(v.shape)}")
+    _check(1 <= kv <= heads <= 1024 and heads % kv == 0,
+           lambda: f"{heads} query heads cannot share {kv} key/value heads")
+    _check(1 <= dim <= MAX_ATTENTION_DIM,
+           lambda: f"the head dimension must lie in 1 .. {MAX_ATTENTION_DIM}, got {dim}")
+    _check(isinstance(buckets, RelativeBuckets) and buckets.bucket_of.device == q.device,
+           "buckets must be RelativeBuckets on the queries' device")
+    _check(tuple(table.shape) == (buckets.num_buckets, heads) and table.dtype == q.dtype
+           and table.device == q.device,
+           lambda: f"table must be [{buckets.num_buckets}, {heads}] {q.dtype} on {q.device}, "
+                   f"got {tuple(table.shape)} {table.dtype} on {table.device}")
+    if keep is not None:
+        _check(keep.dtype == torch.bool and tuple(keep.shape) == (n,) and keep.device == q.device,
+               lambda: f"keep must be [{n}] bool on {q.device}")
+        keep = keep.contiguous()
+    if positions is not None:
+        _check(positions.dtype == torch.int32 and tuple(positions.shape) == (n,)
+               and positions.device == q.device, lambda: f"positions must be [{n}] int32 on "
+                                                         f"{q.device}")
+        positions = positions.contiguous()
+    scale = dim ** -0.5 if scale is None else float(scale)
+    rows = 32 if chains.max_len <= 32 else 128
+    return (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table.contiguous(), scale, keep,
+            positions, rows)
+
+
+def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                    buckets: RelativeBuckets, chains: ChainLayout, scale: Optional[float] = None,
+                    keep: Optional[torch.Tensor] = None,
+                    positions: Optional[torch.Tensor] = None, want_lse: bool = False
+                    ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(out [S, H, D], lse [H, S] | None): attention of every bead to the
+    present beads of its chain with a bias by relative position
+    (mlcg_chain_attention): logits scale q_i.k_j + table[bucket(p_j - p_i), h].
+
+    q [S, H, D], k and v [S, KV, D] (H a multiple of KV; views with any row
+    and head stride, e.g. slices of one projection), table
+    [num_buckets, H]; scale defaults to 1 / sqrt(D).  keep [S] bool: absent
+    beads (False) are no keys, whatever their rows hold; a chain without a
+    present bead gives zeros.  positions [S] int32 (residue numbers; the index
+    in the chain by default) give the offsets, clipped at the reach."""
+    (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
+     rows) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
+    out = torch.empty(n, heads, dim, dtype=q.dtype, device=q.device)
+    lse = torch.empty(heads, n, dtype=torch.float32, device=q.device) if want_lse else None
+    tiles = chains.tiles[rows]
+    call("mlcg_chain_attention", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim, dt,
+         ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), buckets.reach, scale,
+         ptr(tiles), tiles.shape[0], rows, ptr(keep), ptr(positions), ptr(out), ptr(lse),
+         stream_handle(q.device))
+    return out, lse
+
+
+def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: ChainLayout,
+                             out: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor,
+                             scale: Optional[float] = None,
+                             keep: Optional[torch.Tensor] = None,
+                             positions: Optional[torch.Tensor] = None):
+    """(grad q, grad k, grad v, grad table) of chain_attention for the gradient
+    of its output (mlcg_chain_attention_backward); out and lse are the
+    forward's.  Every sum has a fixed order."""
+    (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
+     rows) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
+    dev = q.device
+    for t, name, shape, dtype in ((out, "out", (n, heads, dim), q.dtype),
+                                  (grad, "grad", (n, heads, dim), q.dtype),
+                                  (lse, "lse", (heads, n), torch.float32)):
+        _check(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype
+               and t.device == dev, lambda: f"{name} must be {shape} {dtype} on {dev}")
+    out, lse, grad = out.contiguous(), lse.contiguous(), grad.contiguous()
+    dq = torch.empty(n, heads, dim, dtype=q.dtype, device=dev)
+    dk = torch.empty(n, kv, dim, dtype=q.dtype, device=dev)
+    dv = torch.empty(n, kv, dim, dtype=q.dtype, device=dev)
+    if n == 0:
+        return dq, dk, dv, torch.zeros_like(table)
+    dtable = torch.empty_like(table)
+    tiles = chains.tiles[rows]
+    nws = heads * (n + tiles.shape[0] * buckets.num_buckets)
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    call("mlcg_chain_attention_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim,
+         dt, ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), ptr(buckets.order),
+         ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, ptr(keep),
+         ptr(positions), ptr(out), ptr(lse), ptr(grad), ptr(dq), ptr(dk), ptr(dv), ptr(dtable),
+         ptr(ws), nws, stream_handle(dev))
+    return dq, dk, dv, dtable
+
+
+def _norm_args(x, weight, bias, groups, chains, act):
+    require_device(x, weight, bias)
+    dt = _chain_dtype(x, "group_norm_act")
+    _check(isinstance(chains, ChainLayout) and chains.device == x.device,
+           "chains must be a ChainLayout on the rows' device")
+    _check(x.dim() == 2 and x.shape[0] == chains.n_beads,
+           lambda: f"x must be [{chains.n_beads}, width], got {tuple(x.shape)}")
+    n, width = x.shape
+    _check(1 <= width <= MAX_NORM_WIDTH and 1 <= groups <= width and width % groups == 0,
+           lambda: f"group_norm_act takes 1 .. {MAX_NORM_WIDTH} channels in equal groups, got "
+                   f"{width} in {groups}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        _check(tuple(t.shape) == (width,) and t.dtype == x.dtype and t.device == x.device,
+               lambda: f"{name} must be [{width}] {x.dtype} on {x.device}")
+    _check(act in CHAIN_ACTS, lambda: f"act must be one of {sorted(CHAIN_ACTS)}, got {act!r}")
+    if (width > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < width):
+        x = x.contiguous()
+    ld = x.stride(0) if n > 1 else width
+    rows = _norm_slab_rows(width, dt)
+    return x, ld, n, width, dt, weight.contiguous(), bias.contiguous(), CHAIN_ACTS[act], rows
+
+
+_NORM_ROWS: dict = {}
+
+
+def _norm_slab_rows(width: int, dt: int) -> int:
+    rows = _NORM_ROWS.get((width, dt))
+    if rows is None:
+        rows = _NORM_ROWS[width, dt] = int(_lib.load().mlcg_group_norm_slab_rows(width, dt))
+    return rows
+
+
+def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, groups: int,
+                   chains: ChainLayout, eps: float = 1e-5, act: str = "none"
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y [S, C], stats [3, B, G]): group norm of every chain with an
+    affine map and an activation, channels last (mlcg_group_norm_act).
+
+    The statistics of a chain and group are those of all its beads and the
+    C / groups channels of the group (biased variance, formed from deviations
+    in fp32); y = act((x - mean) rstd weight + bias) with act "none", "tanh",
+    "ssp" (shifted softplus) or "silu".  x may have any row stride; weight and
+    bias [C] have its type.  stats holds the mean, what its rounding left out
+    and 1 / sqrt(var + eps), undefined for an empty chain."""
+    x, ld, n, width, dt, weight, bias, act_id, rows = _norm_args(x, weight, bias, groups, chains,
+                                                                 act)
+    dev = x.device
+    y = torch.empty(n, width, dtype=x.dtype, device=dev)
+    tiles = chains.tiles[rows]
+    stats = torch.empty(3, chains.n_chains, groups, dtype=torch.float32, device=dev)
+    nws = 4 * tiles.shape[0] * groups
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    call("mlcg_group_norm_act", ptr(x), ld, n, dt, ptr(weight), ptr(bias), width, groups,
+         ptr(tiles), ptr(chains.first[rows]), tiles.shape[0], rows, chains.n_chains, float(eps),
+         act_id, ptr(y), ptr(stats), ptr(ws), nws, stream_handle(dev))
+    return y, stats
+
+
+def group_norm_act_backward(x, weight, bias, groups: int, chains: ChainLayout,
+                            stats: torch.Tensor, grad: torch.Tensor, act: str = "none"):
+    """(grad x, grad weight, grad bias) of group_norm_act for the gradient of y
+    (mlcg_group_norm_act_backward); stats are the forward's."""
+    x, ld, n, width, dt, weight, bias, act_id, rows = _norm_args(x, weight, bias, groups, chains,
+                                                                 act)
+    dev = x.device
+    _check(tuple(grad.shape) == (n, width) and grad.dtype == x.dtype and grad.device == dev,
+           lambda: f"grad must be [{n}, {width}] {x.dtype} on {dev}")
+    _check(tuple(stats.shape) == (3, chains.n_chains, groups) and stats.dtype == torch.float32
+           and stats.device == dev,
+           lambda: f"stats must be [3, {chains.n_chains}, {groups}] float32 on {dev}")
+    grad, stats = grad.contiguous(), stats.contiguous()
+    dx = torch.empty(n, width, dtype=x.dtype, device=dev)
+    if n == 0:
+        return dx, torch.zeros_like(weight), torch.zeros_like(bias)
+    dbw = torch.empty(2, width, dtype=x.dtype, device=dev)
+    tiles = chains.tiles[rows]
+    nws = 2 * (tiles.shape[0] + chains.n_chains) * width
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    call("mlcg_group_norm_act_backward", ptr(x), ld, ptr(grad), n, dt, ptr(weight), ptr(bias),
+         width, groups, ptr(tiles), ptr(chains.first[rows]), tiles.shape[0], rows,
+         chains.n_chains, act_id, ptr(stats), ptr(dx), ptr(dbw), ptr(ws), nws,
+         stream_handle(dev))
+    return dx, dbw[1], dbw[0]
+
+
+def dropout_threshold(p: float) -> int:
+    """The drop probability in 1/65536ths, as dropout_add draws it."""
+    _check(isinstance(p, (int, float)) and 0.0 <= p < 1.0,
+           lambda: f"the drop probability must lie in [0, 1), got {p!r}")
+    return min(65535, int(round(p * 65536)))
+
+
+def dropout_add(x: torch.Tensor, p: float, seed: int, step,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + dropout(x) with a mask that is drawn from a counter and never
+    stored (mlcg_dropout_add): element e (in row-major order) is kept, and
+    scaled by 65536 / (65536 - t), t = round(65536 p), where the half-word
+    e % 8 of Philox4x32-10(key seed, counter (e // 8, step)) is at least t.
+
+    step: an integer, or a one-element int64 tensor on the device that the
+    kernel reads (a recorded graph then draws a new mask on every replay).
+    The gradient of x is dropout_add(grad, p, seed, step)."""
+    require_device(x, residual)
+    dt = _chain_dtype(x, "dropout_add")
+    if residual is not None:
+        _check(residual.shape == x.shape and residual.dtype == x.dtype
+               and residual.device == x.device,
+               lambda: f"residual must be {tuple(x.shape)} {x.dtype} on {x.device}")
+        residual = residual.contiguous()
+    t = dropout_threshold(p)
+    _check(isinstance(seed, int) and 0 <= seed < 2 ** 64, "seed must be an integer in [0, 2^64)")
+    step_dev = None
+    if isinstance(step, torch.Tensor):
+        _check(step.dtype == torch.int64 and step.numel() == 1 and step.device == x.device,
+               lambda: f"step must be an integer or one int64 on {x.device}")
+        step_dev, step = step, 0
+    _check(isinstance(step, int) and 0 <= step < 2 ** 63, "step must be an integer in [0, 2^63)")
+    x = x.contiguous()
+    out = torch.empty_like(x)
+    call("mlcg_dropout_add", ptr(x), ptr(residual), x.numel(), dt, t, seed, ptr(step_dev), step,
+         ptr(out), stream_handle(x.device))
     return out
