@@ -1027,7 +1027,9 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * present); positions [beads]: p, any int32 (NULL: the index in the chain).
  * out [beads, heads, dim]; lse [heads, beads] (may be NULL): the base-2 log of
  * the row's sum, +inf for a row without keys, which the backward pass takes.
- * tile_rows, 32 or 128: the rows of the tiles in `tiles`.
+ * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or (with
+ * tile_rows 64 and dim <= 64) 2: parts of the keys (backward: of the queries)
+ * that a workgroup's waves share and join.
  *
  * The backward pass gives the gradients of q, k, v (contiguous) and table.
  * bucket_order [2 reach + 1] lists the offsets 0 .. 2 reach by bucket,
@@ -1040,7 +1042,7 @@ int mlcg_chain_attention(const void* q, const int64_t* q_strides, const void* k,
                          int kv_heads, int dim, int dtype, const void* table,
                          int buckets, const int32_t* bucket_of, int reach,
                          float scale, const int32_t* tiles, int64_t n_tiles,
-                         int tile_rows, const uint8_t* keep,
+                         int tile_rows, int splits, const uint8_t* keep,
                          const int32_t* positions, void* out, float* lse,
                          void* stream);
 int mlcg_chain_attention_backward(
@@ -1050,7 +1052,7 @@ int mlcg_chain_attention_backward(
     const void* table, int buckets, const int32_t* bucket_of,
     const int32_t* bucket_order, const int32_t* bucket_first, int reach,
     float scale, const int32_t* tiles, int64_t n_tiles, int tile_rows,
-    const uint8_t* keep, const int32_t* positions, const void* out,
+    int splits, const uint8_t* keep, const int32_t* positions, const void* out,
     const float* lse, const void* grad_out, void* grad_q, void* grad_k,
     void* grad_v, void* grad_table, float* workspace,
     int64_t workspace_floats, void* stream);

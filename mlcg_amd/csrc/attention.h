@@ -1,0 +1,1120 @@
+// Attention of the beads of a chain to each other with a learned bias by
+// relative position (gfx950): the kernels, one file of instantiations for
+// each element type (attention_f32.hip, attention_f16.hip,
+// attention_bf16.hip), the entry points in attention.hip.
+//
+// For query bead i and key bead j of one chain, head h (R = reach):
+//   l_ij = scale q_i.k_j + table[bucket_of[clip(p_j - p_i, -R, R) + R], h]
+//   P_ij = exp(l_ij) / sum_j exp(l_ij)  over the present keys,   o_i = sum_j P_ij v_j
+// (a row without any present key gives zeros), p the bead's index in its
+// chain or a residue number; backward, with dP_ij = do_i . v_j,
+//   delta_i = sum_j P_ij dP_ij = do_i . o_i,   dS_ij = P_ij (dP_ij - delta_i),
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
+//   dv_j = sum_i P_ij do_i,  dtable[b, h] = sum of dS_ij over the pairs in b.
+// Neither the bias nor the probabilities are ever stored: the forward pass
+// keeps the running maximum and sum of every row (base-2 exponents) and the
+// log of the sum, from which the backward passes form P again.
+//
+// Tiles: a wave owns 32 queries (forward, dq) or 32 keys (dk, dv) as the
+// columns of 32 x 32 MFMA tiles, so a lane is one query (key) and the softmax
+// statistics are lane values; the other side comes in tiles of KT rows
+// through LDS.  The 16 accumulators of a lane are rows 8 a + 4 g + c (g the
+// lane's half): as the contraction over them is free to be permuted, they are
+// used as the B operand of the next product as they are, and the A operand's
+// tile is stored transposed with its rows in that order.  In 16 bits a step
+// of 16 is one v_mfma_f32_32x32x16, in 32 bits eight v_mfma_f32_32x32x2.
+//
+// A workgroup is NQ x NK waves: NQ blocks of 32 columns, and NK parts of the
+// rows, each wave its own KT rows of a staged tile of NK KT; the parts are
+// joined through LDS at the end.  The next tile's rows are loaded into
+// registers while the present one is used.
+//
+// LDS rows hold 16-byte chunks, exchanged by row (xor), so that the 16-byte
+// reads of 8 consecutive rows fall on all banks.
+//
+// The bias of an offset is one LDS value a head: an array over the offsets
+// from -(R + M) to R + M, M beyond the largest span of a tile, so that a tile
+// that touches the band |offset| < R needs no clipping; a block of 32 rows
+// outside of it has one value.  The table's gradient is summed by offset into
+// the same kind of array, one a wave:
+//   index positions: the block of 32 x 32 dS goes through LDS, [query][key]
+//   with a gap of zeros behind each row, and lane n adds the diagonal
+//   offset n - 31 (32 reads a lane, no test: past an end stand zeros);
+//   given positions: LDS adds of integers, dS scaled by a power of two and cut
+//   in two parts of 15 bits (LDS adds of floats take about 200 cycles a wave
+//   against 6, and their order would change the last bits);
+// then by bucket, then over the workgroups in a fixed order.
+#pragma once
+
+#include <type_traits>
+
+#include "chain.h"
+
+constexpr int kAttnQ = 32;               // columns of a wave
+constexpr int kAttnSpan = 96;            // offsets beyond the reach that a block can touch
+constexpr float kAttnLog2e = 1.4426950408889634f;
+constexpr float kAttnLazy = 8.0f;        // the running maximum may lag by this many powers of two
+
+struct AttnArgs {
+  const void *q, *k, *v, *table, *out, *grad;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  int64_t beads;
+  const int32_t* bucket_of;  // [2 reach + 1]
+  const int4* tiles;         // (chain's first row, its length, tile's first row in it, chain)
+  const uint8_t* keep;
+  const int32_t* pos;
+  float* lse;  // [heads][beads], base 2; +inf for a row without keys
+  int n_tiles, heads, group, dim, reach, buckets, vec;
+  float scale;
+};
+
+struct AttnGrads {
+  void *dq, *dk, *dv, *dtable;
+  float* ws;
+  const int32_t *order, *first;
+};
+
+// shape: waves of columns and of rows, 10 NQ + NK
+template <typename T>
+int attn_forward(AttnArgs a, int shape, void* out, hipStream_t s);
+template <typename T>
+int attn_backward(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s);
+
+#ifdef MLCG_ATTENTION_TYPE
+
+namespace {
+
+template <typename T>
+constexpr int key_tile() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+
+// element offset of (row, el) in an LDS tile of LEN elements a row
+template <typename T, int LEN>
+__device__ __forceinline__ int tile_at(int row, int el) {
+  constexpr int EPC = 16 / sizeof(T), NCH = LEN / EPC;
+  static_assert(NCH >= 4, "a row holds at least four chunks");
+  const int sw = NCH >= 8 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
+  return row * LEN + (((el / EPC) ^ sw) * EPC) + el % EPC;
+}
+
+// 8 consecutive elements of a row, from a multiple of 8
+template <typename T, int LEN>
+__device__ __forceinline__ v8<T> tile_frag(const T* tile, int row, int el) {
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const v8<T>*>(tile + tile_at<T, LEN>(row, el));
+  } else {
+    const v4<T> a = *reinterpret_cast<const v4<T>*>(tile + tile_at<T, LEN>(row, el));
+    const v4<T> b = *reinterpret_cast<const v4<T>*>(tile + tile_at<T, LEN>(row, el + 4));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// where a row of the contraction stands in a transposed tile's row
+__device__ __forceinline__ int row_place(int r) {
+  return (r & ~15) + ((r >> 2) & 1) * 8 + ((r >> 3) & 1) * 4 + (r & 3);
+}
+
+// the row, within its block of 32, of a lane's accumulator i
+__device__ __forceinline__ constexpr int acc_row(int i, int g) {
+  return 8 * (i / 4) + 4 * g + i % 4;
+}
+
+__device__ __forceinline__ void mma(f32x16& c, v8<__bf16> a, v8<__bf16> b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& c, v8<_Float16> a, v8<_Float16> b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& c, v8<float> a, v8<float> b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+}
+
+// 4 elements from p, zero where !ok or past `left`
+template <typename T>
+__device__ __forceinline__ v4<T> load4(const T* p, bool ok, int left, int vec) {
+  v4<T> r{};
+  if (!ok || left <= 0) return r;
+  if (vec) return *reinterpret_cast<const v4<T>*>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < left) r[j] = p[j];
+  return r;
+}
+
+// 8 elements of a row at el: a B operand's fragment
+template <typename T>
+__device__ __forceinline__ v8<T> load8(const T* row, int el, bool ok, int dim, int vec) {
+  const v4<T> a = load4<T>(row + el, ok, dim - el, vec);
+  const v4<T> b = load4<T>(row + el + 4, ok, dim - el - 4, vec);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// ROWS rows on their way from memory to LDS: every thread holds blocks of 4
+// rows x 4 columns, written as they are and / or transposed.
+template <typename T, int DP, int ROWS, int NT>
+struct Stage {
+  static constexpr int NJ = DP / 4, BLOCKS = ROWS / 4 * NJ, PER = (BLOCKS + NT - 1) / NT;
+  v4<T> x[PER][4];
+
+  // rows at or past `rows` become zeros
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int dim, int vec) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * NT;
+      const int j = i % NJ, r0 = i / NJ * 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[p][r] = load4<T>(src + (r0 + r) * stride + 4 * j,
+                           (BLOCKS % NT == 0 || i < BLOCKS) && r0 + r < rows, dim - 4 * j, vec);
+    }
+  }
+  // zeros in the rows that are absent (present: one byte a row), or NULL
+  __device__ __forceinline__ void drop(const uint32_t (&absent)[PER]) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (absent[p] >> r & 1) x[p][r] = v4<T>{};
+  }
+  __device__ __forceinline__ void find_absent(const uint8_t* keep, int rows,
+                                              uint32_t (&absent)[PER]) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * NT, r0 = i / NJ * 4;
+      absent[p] = 0;
+      if (keep && (BLOCKS % NT == 0 || i < BLOCKS))
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r0 + r < rows && !keep[r0 + r]) absent[p] |= 1u << r;
+    }
+  }
+  __device__ __forceinline__ void put_rows(T* tile) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * NT;
+      const int j = i % NJ, r0 = i / NJ * 4;
+      if (BLOCKS % NT && i >= BLOCKS) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<v4<T>*>(tile + tile_at<T, DP>(r0 + r, 4 * j)) = x[p][r];
+    }
+  }
+  // a wave's KT rows are a transposed tile of its own
+  template <int KT>
+  __device__ __forceinline__ void put_trans(T* trans) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * NT;
+      const int j = i % NJ, r0 = i / NJ * 4;
+      if (BLOCKS % NT && i >= BLOCKS) continue;
+      T* mine = trans + (r0 / KT) * (KT * DP);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const v4<T> c = {x[p][0][d], x[p][1][d], x[p][2][d], x[p][3][d]};
+        *reinterpret_cast<v4<T>*>(mine + tile_at<T, KT>(4 * j + d, row_place(r0 % KT))) = c;
+      }
+    }
+  }
+};
+
+// ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped; only
+// the offsets that a chain of `len` beads can touch, and the ends
+template <typename T>
+__device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, float* ext) {
+  const int n = 2 * (a.reach + kAttnSpan) + 1;
+  const T* table = (const T*)a.table;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int d = min(max(i - kAttnSpan, 0), 2 * a.reach);
+    ext[i] = kAttnLog2e * (float)table[(int64_t)a.bucket_of[d] * a.heads + head];
+  }
+}
+
+// clipped offset p_j - p_i as an index of ext, for any int32 positions
+__device__ __forceinline__ int offset_cell(int pj, int pi, int reach) {
+  return min(max(__builtin_elementwise_sub_sat(pj, pi), -reach), reach) + reach + kAttnSpan;
+}
+
+template <typename T>
+__device__ __forceinline__ v8<T> pack8(const float* p) {
+  v8<T> r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)p[e];
+  return r;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// the wave's 32 columns of  tile . B  for all KT rows of its tile
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void tile_product(const T* tile, const v8<T> (&b)[DP / 16],
+                                             f32x16 (&s)[KT / 32]) {
+  const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int n = 0; n < KT / 32; ++n) {
+    s[n] = f32x16{};
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+      mma(s[n], tile_frag<T, DP>(tile, 32 * n + col, 16 * k + 8 * g), b[k]);
+  }
+}
+
+// acc += trans . P  with P the KT rows of a lane's column
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void trans_product(const T* trans, const float (&p)[KT / 2],
+                                              f32x16 (&acc)[DP / 32]) {
+  const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int u = 0; u < KT / 16; ++u) {
+    const v8<T> b = pack8<T>(p + 8 * u);
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+      mma(acc[n], tile_frag<T, KT>(trans, 32 * n + col, 16 * u + 8 * g), b);
+  }
+}
+
+// a lane's column (the accumulators of DP rows) as a row of dst
+template <typename T, int DP>
+__device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32], float f,
+                                             int dim, int vec) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int d = 32 * n + 8 * a + 4 * g;
+      v4<T> o;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = (T)(acc[n][4 * a + c] * f);
+      if (vec) {
+        if (d < dim) *reinterpret_cast<v4<T>*>(dst + d) = o;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (d + c < dim) dst[d + c] = o[c];
+      }
+    }
+}
+
+// acc of the NK waves of a column block, joined in the order of the parts;
+// the sums are part 0's.  buf: (NK - 1) NQ 64 values for each accumulator.
+template <int DP, int NQ, int NK>
+__device__ __forceinline__ void join_parts(f32x16 (&acc)[DP / 32], float* buf) {
+  if constexpr (NK > 1) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % NQ, wk = wave / NQ;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) {
+      __syncthreads();
+      if (wk > 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          buf[(((wk - 1) * NQ + wq) * 16 + r) * 64 + lane] = acc[n][r];
+      __syncthreads();
+      if (wk == 0)
+#pragma unroll
+        for (int p = 1; p < NK; ++p)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[n][r] += buf[(((p - 1) * NQ + wq) * 16 + r) * 64 + lane];
+    }
+  }
+}
+
+// Where a block of 32 rows lies to the wave's columns: all offsets at or past
+// the reach (1), at or before its negative (-1), or neither (0).
+__device__ __forceinline__ int block_side(int d_min, int d_max, int R) {
+  return d_min >= R ? 1 : d_max <= -R ? -1 : 0;
+}
+
+// The logits (base 2) of a tile whose lanes are queries and whose rows are
+// keys, and each block's side.
+template <int KT>
+__device__ __forceinline__ void query_logits(const AttnArgs& a, const f32x16 (&s)[KT / 32],
+                                             const float* ext, const int* kpos, int k0, int qw,
+                                             int qi, int qp, int qlo, int qhi, bool valid,
+                                             float (&x)[KT / 2], int (&side)[KT / 32]) {
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+  const float c = a.scale * kAttnLog2e;
+  const int R = a.reach;
+  if (a.pos) {
+    const int kp = kpos[lane % KT];
+    const uint64_t hi = __ballot(!valid || __builtin_elementwise_sub_sat(kp, qhi) >= R);
+    const uint64_t lo = __ballot(!valid || __builtin_elementwise_sub_sat(kp, qlo) <= -R);
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n)
+      side[n] = (uint32_t)(hi >> (32 * n)) == ~0u ? 1 : (uint32_t)(lo >> (32 * n)) == ~0u ? -1 : 0;
+  } else {
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n)
+      side[n] = block_side(k0 + 32 * n - (qw + 31), k0 + 32 * n + 31 - qw, R);
+  }
+#pragma unroll
+  for (int n = 0; n < KT / 32; ++n) {
+    if (side[n]) {
+      const float b = side[n] > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, b);
+    } else if (a.pos) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        x[16 * n + i] = fmaf(s[n][i], c, ext[offset_cell(kpos[32 * n + acc_row(i, g)], qp, R)]);
+    } else {
+      const float* e = ext + (k0 + 32 * n - qi + 4 * g + R + kAttnSpan);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[acc_row(i, 0)]);
+    }
+  }
+}
+
+// -inf for the absent keys of a tile (cap: +inf for a present one); a NaN
+// there becomes -inf, too
+template <int KT>
+__device__ __forceinline__ void mask_logits(const float* cap, float (&x)[KT / 2]) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < KT / 2; i += 4) {
+    const float4 c = *reinterpret_cast<const float4*>(cap + 32 * (i / 16) + acc_row(i % 16, g));
+    x[i] = c.x < 0.0f ? c.x : x[i];
+    x[i + 1] = c.y < 0.0f ? c.y : x[i + 1];
+    x[i + 2] = c.z < 0.0f ? c.z : x[i + 2];
+    x[i + 3] = c.w < 0.0f ? c.w : x[i + 3];
+  }
+}
+
+// the keys' caps and positions of a tile: thread i loads row i's
+struct KeyInfo {
+  float cap;
+  int pos;
+  __device__ __forceinline__ void load(const AttnArgs& a, const int4& t, int k0, int rows) {
+    const int i = threadIdx.x;
+    cap = -INFINITY;
+    pos = 0;
+    if (i < rows && k0 + i < t.y) {
+      const int64_t row = (int64_t)t.x + k0 + i;
+      if (!a.keep || a.keep[row]) cap = INFINITY;
+      if (a.pos) pos = a.pos[row];
+    }
+  }
+  __device__ __forceinline__ void put(int rows, float* caps, int* kpos) const {
+    if ((int)threadIdx.x < rows) {
+      caps[threadIdx.x] = cap;
+      kpos[threadIdx.x] = pos;
+    }
+  }
+};
+
+template <typename T, int DP, int NQ, int NK>
+struct FwdLds {
+  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  T tile[2][KS * DP];
+  T trans[2][KS * DP];
+  float cap[2][KS];
+  int kpos[2][KS];
+  float ext[1];  // 2 (reach + kAttnSpan) + 1
+};
+
+template <typename T, int DP, int NQ, int NK>
+__global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* __restrict__ out) {
+  constexpr int KT = key_tile<T>(), KS = KT * NK, NT = 64 * NQ * NK;
+  using Lds = FwdLds<T, DP, NQ, NK>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Lds& L = *reinterpret_cast<Lds*>(smem);
+  float* ext = L.ext;
+
+  const int head = blockIdx.x % a.heads, kv = head / a.group;
+  const int4 t = a.tiles[blockIdx.x / a.heads];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int wq = wave % NQ, wk = wave / NQ;
+  const int qw = t.z + kAttnQ * wq, qi = qw + (lane & 31);
+  const bool q_ok = qi < t.y;
+  const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
+  const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
+  const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
+  Stage<T, DP, KS, NT> ks, vs;
+  uint32_t absent[Stage<T, DP, KS, NT>::PER];
+  KeyInfo info;
+  ks.load(kbase, a.k_row, t.y, a.dim, a.vec);
+  vs.load(vbase, a.v_row, t.y, a.dim, a.vec);
+  vs.find_absent(keep, t.y, absent);
+  info.load(a, t, 0, KS);
+
+  const T* q = (const T*)a.q + ((int64_t)t.x + qi) * a.q_row + head * a.q_head;
+  v8<T> qf[DP / 16];
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T>(q, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+  int qp = 0, qlo = 0, qhi = 0;
+  if (a.pos) {
+    qp = a.pos[(int64_t)t.x + min(qi, t.y - 1)];
+    qlo = wave_min(qp);
+    qhi = wave_max(qp);
+  }
+  fill_bias<T>(a, head, ext);
+
+  f32x16 acc[DP / 32] = {};
+  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  int buf = 0;
+  for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+    if (keep) {  // an absent key's row may hold anything: no number may come from it
+      ks.drop(absent);
+      vs.drop(absent);
+    }
+    ks.put_rows(L.tile[buf]);
+    vs.template put_trans<KT>(L.trans[buf]);
+    info.put(KS, L.cap[buf], L.kpos[buf]);
+    const int kn = k0 + KS;
+    if (kn < t.y) {
+      ks.load(kbase + kn * a.k_row, a.k_row, t.y - kn, a.dim, a.vec);
+      vs.load(vbase + kn * a.v_row, a.v_row, t.y - kn, a.dim, a.vec);
+      if (keep) vs.find_absent(keep + kn, t.y - kn, absent);
+      info.load(a, t, kn, KS);
+    }
+    __syncthreads();
+    const int kw = k0 + KT * wk;
+    if (qw >= t.y || kw >= t.y) continue;
+    const T* tile = L.tile[buf] + wk * KT * DP;
+    const float* cap = L.cap[buf] + wk * KT;
+    f32x16 s[KT / 32];
+    tile_product<T, DP, KT>(tile, qf, s);
+    float x[KT / 2];
+    int side[KT / 32];
+    query_logits<KT>(a, s, ext, L.kpos[buf] + wk * KT, kw, qw, qi, qp, qlo, qhi,
+                     a.pos && cap[lane % KT] > 0.0f, x, side);
+    if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < KT / 2; ++i) top = fmaxf(top, x[i]);
+    top = fmaxf(top, other_half(top));
+    // the maximum follows only where it has grown by more than 2^kAttnLazy:
+    // the exponentials then stay below 2^kAttnLazy, and most tiles leave the
+    // sums alone
+    if (__any(top > m + kAttnLazy)) {
+      const float m_new = fmaxf(m, top);
+      base = m_new == -INFINITY ? 0.0f : m_new;  // no key so far: exp2(-inf) = 0
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+    }
+    float sum[4] = {};
+#pragma unroll
+    for (int i = 0; i < KT / 2; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+      sum[i % 4] += x[i];
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    trans_product<T, DP, KT>(L.trans[buf] + wk * KT * DP, x, acc);
+  }
+  l += other_half(l);
+  if constexpr (NK > 1) {
+    // the parts on one maximum, then summed
+    __shared__ float ms[NK][NQ][kAttnQ], ls[NK][NQ][kAttnQ];
+    if (g == 0) {
+      ms[wk][wq][lane] = m;
+      ls[wk][wq][lane] = l;
+    }
+    __syncthreads();
+    const int c = lane & 31;
+    float top = ms[0][wq][c];
+#pragma unroll
+    for (int p = 1; p < NK; ++p) top = fmaxf(top, ms[p][wq][c]);
+    base = top == -INFINITY ? 0.0f : top;
+    l = 0.0f;
+#pragma unroll
+    for (int p = 0; p < NK; ++p)
+      l = fmaf(ls[p][wq][c], __builtin_amdgcn_exp2f(ms[p][wq][c] - base), l);
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    m = top;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] *= f;
+    join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
+  }
+  if (wk > 0 || !q_ok) return;
+  const int64_t row = (int64_t)t.x + qi;
+  store_column<T, DP>(out + (row * a.heads + head) * a.dim, acc, l == 0.0f ? 0.0f : 1.0f / l,
+                      a.dim, a.vec);
+  if (a.lse && g == 0)
+    a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// ---------------------------------------------------------------------------
+// The table's gradient
+
+constexpr int kDiagPitch = 68;  // 32 values and the gap of zeros; 16-byte rows
+constexpr int kDiagFloats = 32 + 32 * kDiagPitch;
+
+// mine[cell of offset d0 + n - 31] += diagonal n of the block whose lanes are
+// queries 0..31 and whose rows are keys 0..31, d0 = first key - first query.
+__device__ __forceinline__ void add_diagonals(const float* x, float* scratch, float* at_d0) {
+  const int lane = threadIdx.x & 63, q = lane & 31, g = lane >> 5;
+  float* row = scratch + 32 + q * kDiagPitch + 4 * g;
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+    *reinterpret_cast<float4*>(row + 8 * a) =
+        make_float4(x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const float* d = scratch + 32 + lane - 31;
+  float t[4] = {};
+#pragma unroll
+  for (int r = 0; r < 32; ++r) t[r % 4] += d[r * (kDiagPitch + 1)];
+  at_d0[lane - 31] += (t[0] + t[1]) + (t[2] + t[3]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Sums by offset for given positions: integers of dS 2^e, a high part of at
+// most 2^15 and 15 bits below it, 16 tiles (2^11 values each) at most before
+// they are moved to the wave's float array.
+struct OffsetInts {
+  int *hi, *lo;
+  float scale, inverse;  // 2^e, or 0 before the first tile
+  int tiles;
+  bool poison;
+  int cells;
+  float* mine;  // of the offset -reach
+
+  __device__ __forceinline__ void init(int* space, int reach, float* at) {
+    cells = 2 * reach + 1;
+    hi = space;
+    lo = space + cells;
+    scale = inverse = 0.0f;
+    tiles = 0;
+    poison = false;
+    mine = at;
+    for (int i = threadIdx.x & 63; i < 2 * cells; i += 64) space[i] = 0;
+  }
+  __device__ __forceinline__ void flush() {
+    for (int i = threadIdx.x & 63; i < cells; i += 64) {
+      float v = ((float)hi[i] + (float)lo[i] * 0x1p-15f) * inverse;
+      if (poison) v = NAN;
+      mine[i] += v;
+      hi[i] = lo[i] = 0;
+    }
+    tiles = 0;
+  }
+  // makes room for a tile of values up to `top`
+  __device__ __forceinline__ void prepare(float top) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (!(top <= 3.0e38f)) {
+      poison = true;
+      top = 0.0f;
+    }
+    if (tiles == 16 || !(top * scale <= 32768.0f) || (scale == 0.0f && top > 0.0f)) {
+      if (scale != 0.0f) flush();
+      if (top > 0.0f) {
+        int e;
+        (void)frexpf(top, &e);  // top < 2^e
+        e = max(e, -100);
+        scale = ldexpf(1.0f, 15 - e);
+        inverse = ldexpf(1.0f, e - 15);
+      }
+      tiles = 0;
+    }
+    ++tiles;
+  }
+  __device__ __forceinline__ void add(int cell, float v) {
+    const float y = v * scale, h = rintf(y);
+    atomicAdd(hi + cell, (int)h);
+    atomicAdd(lo + cell, (int)rintf((y - h) * 32768.0f));
+  }
+};
+
+// The waves' sums by offset (dd, one array of `cells` a wave) to buckets.
+template <int NT>
+__device__ __forceinline__ void flush_offsets(const AttnArgs& a, float* dd, int cells,
+                                              const int32_t* order, const int32_t* first,
+                                              float* out) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < cells; i += NT) {
+    float t = dd[i];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) t += dd[w * cells + i];
+    dd[i] = t;
+  }
+  __syncthreads();
+  if (tid < 64) {  // the cells beyond the reach belong to its ends
+    float lo = 0.0f, hi = 0.0f;
+    for (int i = tid; i <= kAttnSpan; i += 64) {
+      lo += dd[i];
+      hi += dd[cells - 1 - i];
+    }
+    lo = mlcg_wave_sum(lo);
+    hi = mlcg_wave_sum(hi);
+    if (tid == 0) {
+      dd[kAttnSpan] = lo;
+      dd[cells - 1 - kAttnSpan] = hi;
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < a.buckets; b += NT) {
+    float t = 0.0f;
+    for (int i = first[b]; i < first[b + 1]; ++i) t += dd[kAttnSpan + order[i]];
+    out[b] = t;
+  }
+}
+
+// floats of a wave's scratch: the diagonals' block or the integers
+__host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions) {
+  const int ints = (2 * (2 * reach + 1) + 3) & ~3;
+  return positions && ints > kDiagFloats ? ints : kDiagFloats;
+}
+
+template <typename T, int DP, int NQ, int NK>
+struct DqLds {
+  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  T kt[KS * DP], ktr[KS * DP], vt[KS * DP];
+  float cap[KS];
+  int kpos[KS];
+  float rest[4];  // scratch of the waves, ext, dd of the waves
+};
+
+// dq, delta and the workgroup's part of the table's gradient; lanes are
+// queries as in the forward pass.
+template <typename T, int DP, int NQ, int NK>
+__global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
+    AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
+    const int32_t* __restrict__ order, const int32_t* __restrict__ first,
+    float* __restrict__ dtable_part) {
+  constexpr int KT = key_tile<T>(), KS = KT * NK, NW = NQ * NK, NT = 64 * NW;
+  using Lds = DqLds<T, DP, NQ, NK>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Lds& L = *reinterpret_cast<Lds*>(smem);
+  const int R = a.reach, cells = 2 * (R + kAttnSpan) + 1;
+  const int sf = scratch_floats(R, a.pos != nullptr);
+  float* ext = L.rest + NW * sf;
+  float* dd = ext + cells;
+
+  const int head = blockIdx.x % a.heads, kv = head / a.group, tile = blockIdx.x / a.heads;
+  const int4 t = a.tiles[tile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int wq = wave % NQ, wk = wave / NQ;
+  const int qw = t.z + kAttnQ * wq, qi = qw + (lane & 31);
+  const bool q_ok = qi < t.y;
+  const int64_t row = (int64_t)t.x + qi;
+  const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
+  const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
+  const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
+  Stage<T, DP, KS, NT> ks, vs;
+  uint32_t absent[Stage<T, DP, KS, NT>::PER];
+  KeyInfo info;
+  ks.load(kbase, a.k_row, t.y, a.dim, a.vec);
+  vs.load(vbase, a.v_row, t.y, a.dim, a.vec);
+  vs.find_absent(keep, t.y, absent);
+  info.load(a, t, 0, KS);
+
+  const T* q = (const T*)a.q + row * a.q_row + head * a.q_head;
+  const int64_t flat = (row * a.heads + head) * a.dim;
+  v8<T> qf[DP / 16], gf[DP / 16];
+  float delta = 0.0f;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    qf[k] = load8<T>(q, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+    gf[k] = load8<T>((const T*)a.grad + flat, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+    const v8<T> of = load8<T>((const T*)a.out + flat, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[k][e], (float)of[e], delta);
+  }
+  delta += other_half(delta);
+  const float lse = q_ok ? a.lse[head * a.beads + row] : INFINITY;
+  int qp = 0, qlo = 0, qhi = 0;
+  if (a.pos) {
+    qp = a.pos[(int64_t)t.x + min(qi, t.y - 1)];
+    qlo = wave_min(qp);
+    qhi = wave_max(qp);
+  }
+  fill_bias<T>(a, head, ext);
+  for (int i = threadIdx.x; i < NW * cells; i += NT) dd[i] = 0.0f;
+  float* mine = dd + wave * cells;
+  float* scratch = L.rest + wave * sf;
+  OffsetInts ints;
+  if (a.pos)
+    ints.init(reinterpret_cast<int*>(scratch), R, mine + kAttnSpan);
+  else
+    for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
+  float far_lo = 0.0f, far_hi = 0.0f;
+
+  f32x16 acc[DP / 32] = {};
+  for (int k0 = 0; k0 < t.y; k0 += KS) {
+    __syncthreads();
+    if (keep) {
+      ks.drop(absent);
+      vs.drop(absent);
+    }
+    ks.put_rows(L.kt);
+    ks.template put_trans<KT>(L.ktr);
+    vs.put_rows(L.vt);
+    info.put(KS, L.cap, L.kpos);
+    const int kn = k0 + KS;
+    if (kn < t.y) {
+      ks.load(kbase + kn * a.k_row, a.k_row, t.y - kn, a.dim, a.vec);
+      vs.load(vbase + kn * a.v_row, a.v_row, t.y - kn, a.dim, a.vec);
+      if (keep) vs.find_absent(keep + kn, t.y - kn, absent);
+      info.load(a, t, kn, KS);
+    }
+    __syncthreads();
+    const int kw = k0 + KT * wk;
+    if (qw >= t.y || kw >= t.y) continue;
+    const float* cap = L.cap + wk * KT;
+    const int* kpos = L.kpos + wk * KT;
+    f32x16 s[KT / 32];
+    tile_product<T, DP, KT>(L.kt + wk * KT * DP, qf, s);
+    float x[KT / 2];
+    int side[KT / 32];
+    query_logits<KT>(a, s, ext, kpos, kw, qw, qi, qp, qlo, qhi,
+                     a.pos && cap[lane % KT] > 0.0f, x, side);
+    if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
+#pragma unroll
+    for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - lse);
+    tile_product<T, DP, KT>(L.vt + wk * KT * DP, gf, s);  // dP
+    if (t.y <= KT) {
+      // a chain of one tile: delta from P and dP themselves, so that a row
+      // of one key has dS = 0 exactly
+      delta = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) delta = fmaf(x[i], s[i / 16][i % 16], delta);
+      delta += other_half(delta);
+    }
+#pragma unroll
+    for (int i = 0; i < KT / 2; ++i) x[i] *= s[i / 16][i % 16] - delta;
+    bool near = false;
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n) {
+      if (side[n]) {
+        float sum[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i % 4] += x[16 * n + i];
+        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (side[n] > 0)
+          far_hi += all;
+        else
+          far_lo += all;
+      } else if (a.pos) {
+        near = true;
+      } else {
+        add_diagonals(x + 16 * n, scratch, mine + (kw + 32 * n - qw + R + kAttnSpan));
+      }
+    }
+    if (near) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) top = fmaxf(top, fabsf(x[i]));
+      // NaN does not survive the maximum
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) top = x[i] != x[i] ? INFINITY : top;
+      ints.prepare(top);
+#pragma unroll
+      for (int n = 0; n < KT / 32; ++n)
+        if (!side[n])
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            ints.add(offset_cell(kpos[32 * n + acc_row(i, g)], qp, R) - kAttnSpan, x[16 * n + i]);
+    }
+    trans_product<T, DP, KT>(L.ktr + wk * KT * DP, x, acc);
+  }
+  if (a.pos) ints.flush();
+  far_lo = mlcg_wave_sum(far_lo);
+  far_hi = mlcg_wave_sum(far_hi);
+  if (lane == 0) {
+    mine[0] += far_lo;
+    mine[cells - 1] += far_hi;
+  }
+  join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
+  if (q_ok && wk == 0) {
+    store_column<T, DP>(dq + flat, acc, a.scale, a.dim, a.vec);
+    if (g == 0) delta_out[head * a.beads + row] = delta;
+  }
+  flush_offsets<NT>(a, dd, cells, order, first,
+                    dtable_part + ((int64_t)head * a.n_tiles + tile) * a.buckets);
+}
+
+template <typename T, int DP, int NQ, int NK>
+struct DkvLds {
+  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  T qt[2][KS * DP], qtr[2][KS * DP], gt[2][KS * DP], gtr[2][KS * DP];
+  float lse[2][KS], delta[2][KS];
+  int qpos[2][KS];
+  float ext[1];
+};
+
+// dk and dv; lanes are keys, the tiles hold queries.  The query heads that
+// share a key/value head are taken one after the other.
+template <typename T, int DP, int NQ, int NK>
+__global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
+                                                                const float* __restrict__ delta,
+                                                                T* __restrict__ dk,
+                                                                T* __restrict__ dv) {
+  constexpr int KT = key_tile<T>(), KS = KT * NK, NT = 64 * NQ * NK;
+  using Lds = DkvLds<T, DP, NQ, NK>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Lds& L = *reinterpret_cast<Lds*>(smem);
+  float* ext = L.ext;
+
+  const int kv_heads = a.heads / a.group;
+  const int kv = blockIdx.x % kv_heads;
+  const int4 t = a.tiles[blockIdx.x / kv_heads];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int wq = wave % NQ, wk = wave / NQ;
+  const int kw = t.z + kAttnQ * wq, ki = kw + (lane & 31);
+  const int64_t row = (int64_t)t.x + ki;
+  const bool in = ki < t.y, k_ok = in && (!a.keep || a.keep[row]);
+
+  Stage<T, DP, KS, NT> qs, gs;
+  float lse_n = INFINITY, delta_n = 0.0f;
+  int pos_n = 0;
+  auto load = [&](int head, int q0) {
+    const int64_t row0 = (int64_t)t.x + q0;
+    qs.load((const T*)a.q + row0 * a.q_row + head * a.q_head, a.q_row, t.y - q0, a.dim, a.vec);
+    gs.load((const T*)a.grad + (row0 * a.heads + head) * a.dim, (int64_t)a.heads * a.dim,
+            t.y - q0, a.dim, a.vec);
+    const int i = threadIdx.x;
+    lse_n = INFINITY;  // exp2(-inf) = 0 for the rows past the end
+    delta_n = 0.0f;
+    if (i < KS && q0 + i < t.y) {
+      lse_n = a.lse[head * a.beads + row0 + i];
+      delta_n = delta[head * a.beads + row0 + i];
+      if (a.pos) pos_n = a.pos[row0 + i];
+    }
+  };
+  load(kv * a.group, 0);
+
+  const T* k = (const T*)a.k + row * a.k_row + kv * a.k_head;
+  const T* v = (const T*)a.v + row * a.v_row + kv * a.v_head;
+  v8<T> kf[DP / 16], vf[DP / 16];
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) {
+    kf[i] = load8<T>(k, 16 * i + 8 * g, k_ok, a.dim, a.vec);
+    vf[i] = load8<T>(v, 16 * i + 8 * g, k_ok, a.dim, a.vec);
+  }
+  int kp = 0, klo = 0, khi = 0;
+  if (a.pos) {
+    kp = a.pos[(int64_t)t.x + min(ki, t.y - 1)];
+    klo = wave_min(kp);
+    khi = wave_max(kp);
+  }
+  const float c = a.scale * kAttnLog2e;
+  const int R = a.reach;
+
+  f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
+  int buf = 0;
+  for (int h = 0; h < a.group; ++h) {
+    const int head = kv * a.group + h;
+    if (h > 0) __syncthreads();
+    fill_bias<T>(a, head, ext);
+    for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
+      qs.put_rows(L.qt[buf]);
+      qs.template put_trans<KT>(L.qtr[buf]);
+      gs.put_rows(L.gt[buf]);
+      gs.template put_trans<KT>(L.gtr[buf]);
+      if ((int)threadIdx.x < KS) {
+        L.lse[buf][threadIdx.x] = lse_n;
+        L.delta[buf][threadIdx.x] = delta_n;
+        L.qpos[buf][threadIdx.x] = pos_n;
+      }
+      if (q0 + KS < t.y)
+        load(head, q0 + KS);
+      else if (h + 1 < a.group)
+        load(head + 1, 0);
+      __syncthreads();
+      const int qw = q0 + KT * wk;
+      if (kw >= t.y || qw >= t.y) continue;
+      const float* lses = L.lse[buf] + wk * KT;
+      const float* dels = L.delta[buf] + wk * KT;
+      const int* qpos = L.qpos[buf] + wk * KT;
+      f32x16 s[KT / 32];
+      tile_product<T, DP, KT>(L.qt[buf] + wk * KT * DP, kf, s);
+      float x[KT / 2];
+      uint64_t hi = 0, lo = 0;
+      if (a.pos) {
+        const int qp = qpos[lane % KT];
+        const bool past = qw + lane % KT >= t.y;
+        hi = __ballot(past || __builtin_elementwise_sub_sat(klo, qp) >= R);
+        lo = __ballot(past || __builtin_elementwise_sub_sat(khi, qp) <= -R);
+      }
+#pragma unroll
+      for (int n = 0; n < KT / 32; ++n) {
+        const int q_n = qw + 32 * n;
+        const int side = a.pos ? ((uint32_t)(hi >> (32 * n)) == ~0u   ? 1
+                                  : (uint32_t)(lo >> (32 * n)) == ~0u ? -1
+                                                                      : 0)
+                               : block_side(kw - (q_n + 31), kw + 31 - q_n, R);
+        if (side) {
+          const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, b);
+        } else if (a.pos) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[16 * n + i] = fmaf(s[n][i], c, ext[offset_cell(kp, qpos[32 * n + acc_row(i, g)], R)]);
+        } else {
+          const float* e = ext + (ki - q_n - 4 * g + R + kAttnSpan);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[-acc_row(i, 0)]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KT / 2; i += 4) {
+        const float4 ls =
+            *reinterpret_cast<const float4*>(lses + 32 * (i / 16) + acc_row(i % 16, g));
+        x[i] = __builtin_amdgcn_exp2f(x[i] - ls.x);
+        x[i + 1] = __builtin_amdgcn_exp2f(x[i + 1] - ls.y);
+        x[i + 2] = __builtin_amdgcn_exp2f(x[i + 2] - ls.z);
+        x[i + 3] = __builtin_amdgcn_exp2f(x[i + 3] - ls.w);
+      }
+      trans_product<T, DP, KT>(L.gtr[buf] + wk * KT * DP, x, dva);
+      tile_product<T, DP, KT>(L.gt[buf] + wk * KT * DP, vf, s);  // dP
+#pragma unroll
+      for (int i = 0; i < KT / 2; i += 4) {
+        const float4 de =
+            *reinterpret_cast<const float4*>(dels + 32 * (i / 16) + acc_row(i % 16, g));
+        x[i] *= s[i / 16][i % 16] - de.x;
+        x[i + 1] *= s[i / 16][i % 16 + 1] - de.y;
+        x[i + 2] *= s[i / 16][i % 16 + 2] - de.z;
+        x[i + 3] *= s[i / 16][i % 16 + 3] - de.w;
+      }
+      trans_product<T, DP, KT>(L.qtr[buf] + wk * KT * DP, x, dka);
+    }
+  }
+  join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
+  join_parts<DP, NQ, NK>(dva, reinterpret_cast<float*>(smem));
+  if (!in || wk > 0) return;
+  const int64_t flat = (row * kv_heads + kv) * a.dim;
+  if (!k_ok) {  // an absent key takes part in nothing
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) dka[n] = dva[n] = f32x16{};
+  }
+  store_column<T, DP>(dk + flat, dka, a.scale, a.dim, a.vec);
+  store_column<T, DP>(dv + flat, dva, 1.0f, a.dim, a.vec);
+}
+
+// dtable[b][head] = sum of the workgroups' parts [head][tile][b]: 8 buckets x
+// 32 slices of the tiles a workgroup, joined in order.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_dtable_kernel(const float* __restrict__ part,
+                                                          int n_tiles, int buckets, int heads,
+                                                          T* __restrict__ dtable) {
+  __shared__ float red[32][9];
+  const int b = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3, head = blockIdx.y;
+  float s = 0.0f;
+  if (b < buckets)
+    for (int i = slice; i < n_tiles; i += 32) s += part[((int64_t)head * n_tiles + i) * buckets + b];
+  red[slice][threadIdx.x & 7] = s;
+  __syncthreads();
+  if (slice == 0 && b < buckets) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += red[i][threadIdx.x];
+    dtable[(int64_t)b * heads + head] = (T)t;
+  }
+}
+
+// LDS above 64 KiB has to be asked for.
+int allow_lds(const void* f, unsigned bytes) {
+  if (bytes > 163840u) return MLCG_ERR_UNSUPPORTED;
+  if (bytes <= 65536u) return MLCG_OK;
+  return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) ==
+                 hipSuccess
+             ? MLCG_OK
+             : MLCG_ERR_LAUNCH;
+}
+
+template <typename T, int DP, int NQ, int NK>
+int launch_fwd(const AttnArgs& a, void* out, hipStream_t s) {
+  const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
+  const unsigned lds = sizeof(FwdLds<T, DP, NQ, NK>) + 4 * cells;
+  auto f = attn_fwd_kernel<T, DP, NQ, NK>;
+  if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
+  hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NQ * NK), lds, s, a,
+                     (T*)out);
+  return mlcg_launch_status();
+}
+
+template <typename T, int DP, int NQ, int NK>
+int launch_bwd(const AttnArgs& a, const AttnGrads& o, hipStream_t s) {
+  constexpr unsigned NW = NQ * NK;
+  const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
+  const unsigned lds1 = sizeof(DqLds<T, DP, NQ, NK>) +
+                        4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 1) * cells);
+  const unsigned lds2 = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
+  auto f1 = attn_dq_kernel<T, DP, NQ, NK>;
+  auto f2 = attn_dkv_kernel<T, DP, NQ, NK>;
+  if (int e = allow_lds(reinterpret_cast<const void*>(f1), lds1)) return e;
+  if (int e = allow_lds(reinterpret_cast<const void*>(f2), lds2)) return e;
+  float* delta = o.ws;
+  float* part = o.ws + a.heads * a.beads;
+  hipLaunchKernelGGL(f1, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NW), lds1, s, a,
+                     (T*)o.dq, delta, o.order, o.first, part);
+  hipLaunchKernelGGL(f2, dim3((unsigned)(a.n_tiles * (a.heads / a.group))), dim3(64 * NW), lds2, s,
+                     a, delta, (T*)o.dk, (T*)o.dv);
+  hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(mlcg_div_up(a.buckets, 8), a.heads), dim3(256), 0,
+                     s, part, a.n_tiles, a.buckets, a.heads, (T*)o.dtable);
+  return mlcg_launch_status();
+}
+
+// vector loads and stores of four elements: every row and head starts at a
+// multiple of four
+bool attn_vec(const AttnArgs& a, int size) {
+  const void* p[] = {a.q, a.k, a.v, a.out, a.grad};
+  for (const void* x : p)
+    if (reinterpret_cast<uintptr_t>(x) % (4 * size)) return false;
+  const int64_t st[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.dim};
+  for (int64_t x : st)
+    if (x % 4) return false;
+  return true;
+}
+
+template <typename F>
+int by_shape(int dim, int shape, F f) {
+  using std::integral_constant;
+  auto with = [&](auto dp) {
+    switch (shape) {
+      case 11: return f(dp, integral_constant<int, 1>(), integral_constant<int, 1>());
+      case 21: return f(dp, integral_constant<int, 2>(), integral_constant<int, 1>());
+      case 41: return f(dp, integral_constant<int, 4>(), integral_constant<int, 1>());
+      case 22:
+        if constexpr (decltype(dp)::value <= 64)
+          return f(dp, integral_constant<int, 2>(), integral_constant<int, 2>());
+    }
+    return (int)MLCG_ERR_UNSUPPORTED;
+  };
+  if (dim <= 32) return with(integral_constant<int, 32>());
+  if (dim <= 64) return with(integral_constant<int, 64>());
+  return with(integral_constant<int, 128>());
+}
+
+}  // namespace
+
+template <>
+int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStream_t s) {
+  using T = MLCG_ATTENTION_TYPE;
+  a.vec = attn_vec(a, sizeof(T));
+  return by_shape(a.dim, shape, [&](auto dp, auto nq, auto nk) {
+    return launch_fwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value>(a, out, s);
+  });
+}
+
+template <>
+int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s) {
+  using T = MLCG_ATTENTION_TYPE;
+  a.vec = attn_vec(a, sizeof(T));
+  return by_shape(a.dim, shape, [&](auto dp, auto nq, auto nk) {
+    return launch_bwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value>(a, o, s);
+  });
+}
+
+#endif  // MLCG_ATTENTION_TYPE

@@ -1956,9 +1956,16 @@ def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions):
                                                          f"{q.device}")
         positions = positions.contiguous()
     scale = dim ** -0.5 if scale is None else float(scale)
-    rows = 32 if chains.max_len <= 32 else 128
+    rows, splits = _attention_shape(chains, heads, dim)
     return (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table.contiguous(), scale, keep,
-            positions, rows)
+            positions, rows, splits)
+
+
+def _attention_shape(chains: ChainLayout, heads: int, dim: int) -> Tuple[int, int]:
+    """(beads of a tile, parts of the other side) of the attention kernels."""
+    if chains.max_len <= 32:
+        return 32, 1
+    return (64, 1) if chains.max_len <= 64 else (128, 1)
 
 
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -1977,13 +1984,13 @@ def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: to
     present bead gives zeros.  positions [S] int32 (residue numbers; the index
     in the chain by default) give the offsets, clipped at the reach."""
     (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
-     rows) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
+     rows, splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
     out = torch.empty(n, heads, dim, dtype=q.dtype, device=q.device)
     lse = torch.empty(heads, n, dtype=torch.float32, device=q.device) if want_lse else None
     tiles = chains.tiles[rows]
     call("mlcg_chain_attention", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim, dt,
          ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), buckets.reach, scale,
-         ptr(tiles), tiles.shape[0], rows, ptr(keep), ptr(positions), ptr(out), ptr(lse),
+         ptr(tiles), tiles.shape[0], rows, splits, ptr(keep), ptr(positions), ptr(out), ptr(lse),
          stream_handle(q.device))
     return out, lse
 
@@ -1997,7 +2004,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     of its output (mlcg_chain_attention_backward); out and lse are the
     forward's.  Every sum has a fixed order."""
     (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
-     rows) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
+     rows, splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
     dev = q.device
     for t, name, shape, dtype in ((out, "out", (n, heads, dim), q.dtype),
                                   (grad, "grad", (n, heads, dim), q.dtype),
@@ -2016,7 +2023,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     call("mlcg_chain_attention_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim,
          dt, ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), ptr(buckets.order),
-         ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, ptr(keep),
+         ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, splits, ptr(keep),
          ptr(positions), ptr(out), ptr(lse), ptr(grad), ptr(dq), ptr(dk), ptr(dv), ptr(dtable),
          ptr(ws), nws, stream_handle(dev))
     return dq, dk, dv, dtable
