@@ -1019,7 +1019,8 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  *   l_ij = scale q_i.k_j + table[bucket_of[clip(p_j - p_i, -reach, reach) + reach], h]
  *   out_i = sum_j softmax_j(l_ij) v_j,  zeros where no bead is present.
  * q is [beads, heads, dim], k and v [beads, kv_heads, dim] with the last axis
- * contiguous and strides (row, head) in elements in host memory; heads is a
+ * contiguous and strides (row, head) in elements in host memory, a row's from
+ * 0 to below 2^22; heads is a
  * multiple of kv_heads, head h reads key/value head h / (heads / kv_heads).
  * table [buckets, heads]; bucket_of [2 reach + 1] with entries in
  * [0, buckets); 1 <= reach <= 1024, 1 <= dim <= 128.  keep [beads]: 0 marks an

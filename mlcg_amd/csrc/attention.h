@@ -20,17 +20,21 @@
 // statistics are lane values; the other side comes in tiles of KT rows
 // through LDS.  The 16 accumulators of a lane are rows 8 a + 4 g + c (g the
 // lane's half): as the contraction over them is free to be permuted, they are
-// used as the B operand of the next product as they are, and the A operand's
-// tile is stored transposed with its rows in that order.  In 16 bits a step
-// of 16 is one v_mfma_f32_32x32x16, in 32 bits eight v_mfma_f32_32x32x2.
+// used as the B operand of the next product as they are, and the A operand
+// takes the tile's columns with its rows in that order: in 16 bits by the
+// transposing LDS read (4 rows of a column a lane), in 32 bits by single
+// values.  So every operand has one LDS tile, row by row, for both products.
+// In 16 bits a step of 16 is one v_mfma_f32_32x32x16, in 32 bits eight
+// v_mfma_f32_32x32x2.
 //
 // A workgroup is NQ x NK waves: NQ blocks of 32 columns, and NK parts of the
 // rows, each wave its own KT rows of a staged tile of NK KT; the parts are
 // joined through LDS at the end.  The next tile's rows are loaded into
-// registers while the present one is used.
+// registers while the present one is used, and written to the other of two
+// buffers: one barrier a tile.
 //
 // LDS rows hold 16-byte chunks, exchanged by row (xor), so that the 16-byte
-// reads of 8 consecutive rows fall on all banks.
+// reads of 8 consecutive rows and the transposing reads fall on all banks.
 //
 // The bias of an offset is one LDS value a head: an array over the offsets
 // from -(R + M) to R + M, M beyond the largest span of a tile, so that a tile
@@ -64,7 +68,7 @@ struct AttnArgs {
   const uint8_t* keep;
   const int32_t* pos;
   float* lse;  // [heads][beads], base 2; +inf for a row without keys
-  int n_tiles, heads, group, dim, reach, buckets, vec;
+  int n_tiles, heads, group, dim, reach, buckets;
   float scale;
 };
 
@@ -89,18 +93,26 @@ constexpr int key_tile() {
   return sizeof(T) == 2 ? 64 : 32;
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// what row r's chunks are exchanged by, in a tile of N chunks a row
+template <int N>
+__device__ __forceinline__ constexpr int chunk_swap(int r) {
+  static_assert(N >= 4, "a row holds at least four chunks");
+  return N >= 8 ? r & 7 : (r >> 1) & 3;
+}
+
 // element offset of (row, el) in an LDS tile of LEN elements a row
 template <typename T, int LEN>
 __device__ __forceinline__ int tile_at(int row, int el) {
-  constexpr int EPC = 16 / sizeof(T), NCH = LEN / EPC;
-  static_assert(NCH >= 4, "a row holds at least four chunks");
-  const int sw = NCH >= 8 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
-  return row * LEN + (((el / EPC) ^ sw) * EPC) + el % EPC;
+  constexpr int EPC = 16 / sizeof(T);
+  return row * LEN + (((el / EPC) ^ chunk_swap<LEN / EPC>(row)) * EPC) + el % EPC;
 }
 
-// 8 consecutive elements of a row, from a multiple of 8
+// A operand of a step over the columns: row `row`, elements 16 k + 8 g ..
 template <typename T, int LEN>
-__device__ __forceinline__ v8<T> tile_frag(const T* tile, int row, int el) {
+__device__ __forceinline__ v8<T> row_frag(const T* tile, int row, int el) {
   if constexpr (sizeof(T) == 2) {
     return *reinterpret_cast<const v8<T>*>(tile + tile_at<T, LEN>(row, el));
   } else {
@@ -110,9 +122,30 @@ __device__ __forceinline__ v8<T> tile_frag(const T* tile, int row, int el) {
   }
 }
 
-// where a row of the contraction stands in a transposed tile's row
-__device__ __forceinline__ int row_place(int r) {
-  return (r & ~15) + ((r >> 2) & 1) * 8 + ((r >> 3) & 1) * 4 + (r & 3);
+// A operand of a step over the rows: column 32 n + (lane & 31), rows 16 u +
+// 4 g + 0..3 and 16 u + 8 + 4 g + 0..3
+template <typename T, int LEN>
+__device__ __forceinline__ v8<T> column_frag(const T* tile, int u, int n) {
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    // 16 lanes give the places of 4 rows x 16 columns, lane i those of row
+    // i / 4, and get a column's 4 rows each
+    const int el = 32 * n + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int row = 16 * u + 4 * g + ((lane & 15) >> 2);
+    s16x4 x[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+      x[a] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)(tile + tile_at<T, LEN>(row + 8 * a, el)));
+    const auto both = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(v8<T>, both);
+  } else {
+    v8<T> r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r[e] = tile[tile_at<T, LEN>(16 * u + 8 * (e / 4) + 4 * g + e % 4, 32 * n + (lane & 31))];
+    return r;
+  }
 }
 
 // the row, within its block of 32, of a lane's accumulator i
@@ -131,96 +164,91 @@ __device__ __forceinline__ void mma(f32x16& c, v8<float> a, v8<float> b) {
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
 }
 
-// 4 elements from p, zero where !ok or past `left`
-template <typename T>
-__device__ __forceinline__ v4<T> load4(const T* p, bool ok, int left, int vec) {
-  v4<T> r{};
-  if (!ok || left <= 0) return r;
-  if (vec) return *reinterpret_cast<const v4<T>*>(p);
+// 8 elements of a row at el: a B operand's fragment, zeros where !ok and past
+// dim.  VEC: rows begin at multiples of 16 bytes and dim is one.
+template <typename T, bool VEC>
+__device__ __forceinline__ v8<T> load8(const T* row, int el, bool ok, int dim) {
+  v8<T> r{};
+  if (!ok) return r;
+  if constexpr (VEC) {
+    v4<T> a{}, b{};
+    if (el < dim) a = *reinterpret_cast<const v4<T>*>(row + el);
+    if (el + 4 < dim) b = *reinterpret_cast<const v4<T>*>(row + el + 4);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < left) r[j] = p[j];
-  return r;
-}
-
-// 8 elements of a row at el: a B operand's fragment
-template <typename T>
-__device__ __forceinline__ v8<T> load8(const T* row, int el, bool ok, int dim, int vec) {
-  const v4<T> a = load4<T>(row + el, ok, dim - el, vec);
-  const v4<T> b = load4<T>(row + el + 4, ok, dim - el - 4, vec);
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// ROWS rows on their way from memory to LDS: every thread holds blocks of 4
-// rows x 4 columns, written as they are and / or transposed.
-template <typename T, int DP, int ROWS, int NT>
-struct Stage {
-  static constexpr int NJ = DP / 4, BLOCKS = ROWS / 4 * NJ, PER = (BLOCKS + NT - 1) / NT;
-  v4<T> x[PER][4];
-
-  // rows at or past `rows` become zeros
-  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int dim, int vec) {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int i = threadIdx.x + p * NT;
-      const int j = i % NJ, r0 = i / NJ * 4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        x[p][r] = load4<T>(src + (r0 + r) * stride + 4 * j,
-                           (BLOCKS % NT == 0 || i < BLOCKS) && r0 + r < rows, dim - 4 * j, vec);
-    }
+    for (int e = 0; e < 8; ++e)
+      if (el + e < dim) r[e] = row[el + e];
+    return r;
   }
-  // zeros in the rows that are absent (present: one byte a row), or NULL
-  __device__ __forceinline__ void drop(const uint32_t (&absent)[PER]) {
+}
+
+// ROWS rows on their way from memory to LDS, a thread PER chunks of 16 bytes.
+// A chunk's place is the tile's first row plus an offset that stays the same
+// from tile to tile.  Rows past the chain's end are read as its last one; like
+// absent ones they are replaced by zeros (0 P would not be 0 where they hold
+// no number).  Columns past dim repeat the last ones: they meet zeros of the
+// other operand or accumulators that nothing reads.
+template <typename T, int DP, int ROWS, int NT, bool VEC>
+struct Stage {
+  static constexpr int EPC = 16 / sizeof(T), NCH = DP / EPC, PER = ROWS * NCH / NT;
+  static_assert(ROWS * NCH % NT == 0, "whole chunks a thread");
+  typedef T chunk __attribute__((ext_vector_type(EPC)));
+  chunk x[PER];
+  uint32_t off[PER];  // bytes
+  int stride;
+
+  __device__ __forceinline__ static int row(int p) { return (threadIdx.x + p * NT) / NCH; }
+  __device__ __forceinline__ static int column(int p) { return threadIdx.x % NCH * EPC; }
+
+  __device__ __forceinline__ void init(int row_stride, int dim) {
+    static_assert(NT % NCH == 0, "a thread's chunks stand in one column");
+    stride = row_stride;
 #pragma unroll
     for (int p = 0; p < PER; ++p)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (absent[p] >> r & 1) x[p][r] = v4<T>{};
+      off[p] = (uint32_t)(row(p) * stride + min(column(p), dim - (VEC ? EPC : 1))) * sizeof(T);
   }
-  __device__ __forceinline__ void find_absent(const uint8_t* keep, int rows,
-                                              uint32_t (&absent)[PER]) {
+  // src: the tile's first row; rows: those of the chain from there on
+  __device__ __forceinline__ void load(const T* src, int rows, int dim) {
+    const char* at = reinterpret_cast<const char*>(src);
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int i = threadIdx.x + p * NT, r0 = i / NJ * 4;
-      absent[p] = 0;
-      if (keep && (BLOCKS % NT == 0 || i < BLOCKS))
+      uint32_t o = off[p];
+      if (rows < ROWS) o -= (uint32_t)max(row(p) - (rows - 1), 0) * stride * sizeof(T);
+      if constexpr (VEC) {
+        x[p] = *reinterpret_cast<const chunk*>(at + o);
+      } else {
+        const T* e = reinterpret_cast<const T*>(at + o);
+        x[p] = chunk{};
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r0 + r < rows && !keep[r0 + r]) absent[p] |= 1u << r;
-    }
-  }
-  __device__ __forceinline__ void put_rows(T* tile) const {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int i = threadIdx.x + p * NT;
-      const int j = i % NJ, r0 = i / NJ * 4;
-      if (BLOCKS % NT && i >= BLOCKS) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<v4<T>*>(tile + tile_at<T, DP>(r0 + r, 4 * j)) = x[p][r];
-    }
-  }
-  // a wave's KT rows are a transposed tile of its own
-  template <int KT>
-  __device__ __forceinline__ void put_trans(T* trans) const {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int i = threadIdx.x + p * NT;
-      const int j = i % NJ, r0 = i / NJ * 4;
-      if (BLOCKS % NT && i >= BLOCKS) continue;
-      T* mine = trans + (r0 / KT) * (KT * DP);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const v4<T> c = {x[p][0][d], x[p][1][d], x[p][2][d], x[p][3][d]};
-        *reinterpret_cast<v4<T>*>(mine + tile_at<T, KT>(4 * j + d, row_place(r0 % KT))) = c;
+        for (int j = 0; j < EPC; ++j)
+          if (column(p) + j < dim) x[p][j] = e[j];
       }
     }
   }
+  // the rows of the thread's chunks that are past the end or absent
+  __device__ __forceinline__ static uint32_t find_absent(const uint8_t* keep, int rows) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int r = min(row(p), rows - 1);
+      if (row(p) >= rows || (keep && !keep[r])) bits |= 1u << p;
+    }
+    return bits;
+  }
+  __device__ __forceinline__ void drop(uint32_t absent) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (absent >> p & 1) x[p] = chunk{};
+  }
+  __device__ __forceinline__ void put(T* tile) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      *reinterpret_cast<chunk*>(tile + tile_at<T, DP>(row(p), column(p))) = x[p];
+  }
 };
 
-// ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped; only
-// the offsets that a chain of `len` beads can touch, and the ends
+// ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped
 template <typename T>
 __device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, float* ext) {
   const int n = 2 * (a.reach + kAttnSpan) + 1;
@@ -267,28 +295,26 @@ __device__ __forceinline__ void tile_product(const T* tile, const v8<T> (&b)[DP 
     s[n] = f32x16{};
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)
-      mma(s[n], tile_frag<T, DP>(tile, 32 * n + col, 16 * k + 8 * g), b[k]);
+      mma(s[n], row_frag<T, DP>(tile, 32 * n + col, 16 * k + 8 * g), b[k]);
   }
 }
 
-// acc += trans . P  with P the KT rows of a lane's column
+// acc += tile^T . P  with P the KT rows of a lane's column
 template <typename T, int DP, int KT>
-__device__ __forceinline__ void trans_product(const T* trans, const float (&p)[KT / 2],
-                                              f32x16 (&acc)[DP / 32]) {
-  const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
+__device__ __forceinline__ void column_product(const T* tile, const float (&p)[KT / 2],
+                                               f32x16 (&acc)[DP / 32]) {
 #pragma unroll
   for (int u = 0; u < KT / 16; ++u) {
     const v8<T> b = pack8<T>(p + 8 * u);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-      mma(acc[n], tile_frag<T, KT>(trans, 32 * n + col, 16 * u + 8 * g), b);
+    for (int n = 0; n < DP / 32; ++n) mma(acc[n], column_frag<T, DP>(tile, u, n), b);
   }
 }
 
 // a lane's column (the accumulators of DP rows) as a row of dst
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 __device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32], float f,
-                                             int dim, int vec) {
+                                             int dim) {
   const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
@@ -298,7 +324,7 @@ __device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32
       v4<T> o;
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[c] = (T)(acc[n][4 * a + c] * f);
-      if (vec) {
+      if constexpr (VEC) {
         if (d < dim) *reinterpret_cast<v4<T>*>(dst + d) = o;
       } else {
 #pragma unroll
@@ -377,18 +403,25 @@ __device__ __forceinline__ void query_logits(const AttnArgs& a, const f32x16 (&s
   }
 }
 
-// -inf for the absent keys of a tile (cap: +inf for a present one); a NaN
-// there becomes -inf, too
+// min(x, cap) as the instruction has it: the smaller number where x is NaN
+__device__ __forceinline__ float min_number(float x, float cap) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(cap));
+  return r;
+}
+
+// -inf for the absent keys of a tile (cap -inf), whatever stands there; a NaN
+// of a present key (cap +inf) becomes +inf, and the row NaN all the same
 template <int KT>
 __device__ __forceinline__ void mask_logits(const float* cap, float (&x)[KT / 2]) {
   const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
   for (int i = 0; i < KT / 2; i += 4) {
     const float4 c = *reinterpret_cast<const float4*>(cap + 32 * (i / 16) + acc_row(i % 16, g));
-    x[i] = c.x < 0.0f ? c.x : x[i];
-    x[i + 1] = c.y < 0.0f ? c.y : x[i + 1];
-    x[i + 2] = c.z < 0.0f ? c.z : x[i + 2];
-    x[i + 3] = c.w < 0.0f ? c.w : x[i + 3];
+    x[i] = min_number(x[i], c.x);
+    x[i + 1] = min_number(x[i + 1], c.y);
+    x[i + 2] = min_number(x[i + 2], c.z);
+    x[i + 3] = min_number(x[i + 3], c.w);
   }
 }
 
@@ -417,15 +450,14 @@ struct KeyInfo {
 template <typename T, int DP, int NQ, int NK>
 struct FwdLds {
   static constexpr int KT = key_tile<T>(), KS = KT * NK;
-  T tile[2][KS * DP];
-  T trans[2][KS * DP];
+  T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
   float ext[1];  // 2 (reach + kAttnSpan) + 1
 };
 
-template <typename T, int DP, int NQ, int NK>
-__global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* __restrict__ out) {
+template <typename T, int DP, int NQ, int NK, bool VEC>
+__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T* __restrict__ out) {
   constexpr int KT = key_tile<T>(), KS = KT * NK, NT = 64 * NQ * NK;
   using Lds = FwdLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -441,18 +473,19 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* _
   const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
   const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
-  Stage<T, DP, KS, NT> ks, vs;
-  uint32_t absent[Stage<T, DP, KS, NT>::PER];
+  Stage<T, DP, KS, NT, VEC> ks, vs;
   KeyInfo info;
-  ks.load(kbase, a.k_row, t.y, a.dim, a.vec);
-  vs.load(vbase, a.v_row, t.y, a.dim, a.vec);
-  vs.find_absent(keep, t.y, absent);
+  ks.init((int)a.k_row, a.dim);
+  vs.init((int)a.v_row, a.dim);
+  ks.load(kbase, t.y, a.dim);
+  vs.load(vbase, t.y, a.dim);
+  uint32_t absent = ks.find_absent(keep, t.y);
   info.load(a, t, 0, KS);
 
   const T* q = (const T*)a.q + ((int64_t)t.x + qi) * a.q_row + head * a.q_head;
   v8<T> qf[DP / 16];
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T>(q, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+  for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, q_ok, a.dim);
   int qp = 0, qlo = 0, qhi = 0;
   if (a.pos) {
     qp = a.pos[(int64_t)t.x + min(qi, t.y - 1)];
@@ -465,27 +498,26 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* _
   float m = -INFINITY, base = 0.0f, l = 0.0f;
   int buf = 0;
   for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
-    if (keep) {  // an absent key's row may hold anything: no number may come from it
+    if (keep || k0 + KS > t.y) {
       ks.drop(absent);
       vs.drop(absent);
     }
-    ks.put_rows(L.tile[buf]);
-    vs.template put_trans<KT>(L.trans[buf]);
+    ks.put(L.k[buf]);
+    vs.put(L.v[buf]);
     info.put(KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
-      ks.load(kbase + kn * a.k_row, a.k_row, t.y - kn, a.dim, a.vec);
-      vs.load(vbase + kn * a.v_row, a.v_row, t.y - kn, a.dim, a.vec);
-      if (keep) vs.find_absent(keep + kn, t.y - kn, absent);
+      ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
+      vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
+      if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
       info.load(a, t, kn, KS);
     }
     __syncthreads();
     const int kw = k0 + KT * wk;
     if (qw >= t.y || kw >= t.y) continue;
-    const T* tile = L.tile[buf] + wk * KT * DP;
     const float* cap = L.cap[buf] + wk * KT;
     f32x16 s[KT / 32];
-    tile_product<T, DP, KT>(tile, qf, s);
+    tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
     float x[KT / 2];
     int side[KT / 32];
     query_logits<KT>(a, s, ext, L.kpos[buf] + wk * KT, kw, qw, qi, qp, qlo, qhi,
@@ -516,7 +548,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* _
       sum[i % 4] += x[i];
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    trans_product<T, DP, KT>(L.trans[buf] + wk * KT * DP, x, acc);
+    column_product<T, DP, KT>(L.v[buf] + wk * KT * DP, x, acc);
   }
   l += other_half(l);
   if constexpr (NK > 1) {
@@ -546,8 +578,8 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_fwd_kernel(AttnArgs a, T* _
   }
   if (wk > 0 || !q_ok) return;
   const int64_t row = (int64_t)t.x + qi;
-  store_column<T, DP>(out + (row * a.heads + head) * a.dim, acc, l == 0.0f ? 0.0f : 1.0f / l,
-                      a.dim, a.vec);
+  store_column<T, DP, VEC>(out + (row * a.heads + head) * a.dim, acc, l == 0.0f ? 0.0f : 1.0f / l,
+                      a.dim);
   if (a.lse && g == 0)
     a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -678,16 +710,16 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
 template <typename T, int DP, int NQ, int NK>
 struct DqLds {
   static constexpr int KT = key_tile<T>(), KS = KT * NK;
-  T kt[KS * DP], ktr[KS * DP], vt[KS * DP];
-  float cap[KS];
-  int kpos[KS];
+  T k[2][KS * DP], v[2][KS * DP];
+  float cap[2][KS];
+  int kpos[2][KS];
   float rest[4];  // scratch of the waves, ext, dd of the waves
 };
 
 // dq, delta and the workgroup's part of the table's gradient; lanes are
 // queries as in the forward pass.
-template <typename T, int DP, int NQ, int NK>
-__global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
+template <typename T, int DP, int NQ, int NK, bool VEC>
+__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
     const int32_t* __restrict__ order, const int32_t* __restrict__ first,
     float* __restrict__ dtable_part) {
@@ -710,12 +742,13 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
   const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
   const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
-  Stage<T, DP, KS, NT> ks, vs;
-  uint32_t absent[Stage<T, DP, KS, NT>::PER];
+  Stage<T, DP, KS, NT, VEC> ks, vs;
   KeyInfo info;
-  ks.load(kbase, a.k_row, t.y, a.dim, a.vec);
-  vs.load(vbase, a.v_row, t.y, a.dim, a.vec);
-  vs.find_absent(keep, t.y, absent);
+  ks.init((int)a.k_row, a.dim);
+  vs.init((int)a.v_row, a.dim);
+  ks.load(kbase, t.y, a.dim);
+  vs.load(vbase, t.y, a.dim);
+  uint32_t absent = ks.find_absent(keep, t.y);
   info.load(a, t, 0, KS);
 
   const T* q = (const T*)a.q + row * a.q_row + head * a.q_head;
@@ -724,9 +757,9 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
   float delta = 0.0f;
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
-    qf[k] = load8<T>(q, 16 * k + 8 * g, q_ok, a.dim, a.vec);
-    gf[k] = load8<T>((const T*)a.grad + flat, 16 * k + 8 * g, q_ok, a.dim, a.vec);
-    const v8<T> of = load8<T>((const T*)a.out + flat, 16 * k + 8 * g, q_ok, a.dim, a.vec);
+    qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, q_ok, a.dim);
+    gf[k] = load8<T, VEC>((const T*)a.grad + flat, 16 * k + 8 * g, q_ok, a.dim);
+    const v8<T> of = load8<T, VEC>((const T*)a.out + flat, 16 * k + 8 * g, q_ok, a.dim);
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[k][e], (float)of[e], delta);
   }
@@ -750,30 +783,29 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
   float far_lo = 0.0f, far_hi = 0.0f;
 
   f32x16 acc[DP / 32] = {};
-  for (int k0 = 0; k0 < t.y; k0 += KS) {
-    __syncthreads();
-    if (keep) {
+  int buf = 0;
+  for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+    if (keep || k0 + KS > t.y) {
       ks.drop(absent);
       vs.drop(absent);
     }
-    ks.put_rows(L.kt);
-    ks.template put_trans<KT>(L.ktr);
-    vs.put_rows(L.vt);
-    info.put(KS, L.cap, L.kpos);
+    ks.put(L.k[buf]);
+    vs.put(L.v[buf]);
+    info.put(KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
-      ks.load(kbase + kn * a.k_row, a.k_row, t.y - kn, a.dim, a.vec);
-      vs.load(vbase + kn * a.v_row, a.v_row, t.y - kn, a.dim, a.vec);
-      if (keep) vs.find_absent(keep + kn, t.y - kn, absent);
+      ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
+      vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
+      if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
       info.load(a, t, kn, KS);
     }
     __syncthreads();
     const int kw = k0 + KT * wk;
     if (qw >= t.y || kw >= t.y) continue;
-    const float* cap = L.cap + wk * KT;
-    const int* kpos = L.kpos + wk * KT;
+    const float* cap = L.cap[buf] + wk * KT;
+    const int* kpos = L.kpos[buf] + wk * KT;
     f32x16 s[KT / 32];
-    tile_product<T, DP, KT>(L.kt + wk * KT * DP, qf, s);
+    tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
     float x[KT / 2];
     int side[KT / 32];
     query_logits<KT>(a, s, ext, kpos, kw, qw, qi, qp, qlo, qhi,
@@ -781,7 +813,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
     if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
 #pragma unroll
     for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - lse);
-    tile_product<T, DP, KT>(L.vt + wk * KT * DP, gf, s);  // dP
+    tile_product<T, DP, KT>(L.v[buf] + wk * KT * DP, gf, s);  // dP
     if (t.y <= KT) {
       // a chain of one tile: delta from P and dP themselves, so that a row
       // of one key has dS = 0 exactly
@@ -825,7 +857,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
           for (int i = 0; i < 16; ++i)
             ints.add(offset_cell(kpos[32 * n + acc_row(i, g)], qp, R) - kAttnSpan, x[16 * n + i]);
     }
-    trans_product<T, DP, KT>(L.ktr + wk * KT * DP, x, acc);
+    column_product<T, DP, KT>(L.k[buf] + wk * KT * DP, x, acc);
   }
   if (a.pos) ints.flush();
   far_lo = mlcg_wave_sum(far_lo);
@@ -836,7 +868,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
   }
   join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
   if (q_ok && wk == 0) {
-    store_column<T, DP>(dq + flat, acc, a.scale, a.dim, a.vec);
+    store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
     if (g == 0) delta_out[head * a.beads + row] = delta;
   }
   flush_offsets<NT>(a, dd, cells, order, first,
@@ -846,7 +878,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dq_kernel(
 template <typename T, int DP, int NQ, int NK>
 struct DkvLds {
   static constexpr int KT = key_tile<T>(), KS = KT * NK;
-  T qt[2][KS * DP], qtr[2][KS * DP], gt[2][KS * DP], gtr[2][KS * DP];
+  T q[2][KS * DP], g[2][KS * DP];
   float lse[2][KS], delta[2][KS];
   int qpos[2][KS];
   float ext[1];
@@ -854,8 +886,8 @@ struct DkvLds {
 
 // dk and dv; lanes are keys, the tiles hold queries.  The query heads that
 // share a key/value head are taken one after the other.
-template <typename T, int DP, int NQ, int NK>
-__global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
+template <typename T, int DP, int NQ, int NK, bool VEC>
+__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
                                                                 const float* __restrict__ delta,
                                                                 T* __restrict__ dk,
                                                                 T* __restrict__ dv) {
@@ -874,14 +906,17 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
   const int64_t row = (int64_t)t.x + ki;
   const bool in = ki < t.y, k_ok = in && (!a.keep || a.keep[row]);
 
-  Stage<T, DP, KS, NT> qs, gs;
+  Stage<T, DP, KS, NT, VEC> qs, gs;
+  qs.init((int)a.q_row, a.dim);
+  gs.init(a.heads * a.dim, a.dim);
+  uint32_t absent = 0;
   float lse_n = INFINITY, delta_n = 0.0f;
   int pos_n = 0;
   auto load = [&](int head, int q0) {
     const int64_t row0 = (int64_t)t.x + q0;
-    qs.load((const T*)a.q + row0 * a.q_row + head * a.q_head, a.q_row, t.y - q0, a.dim, a.vec);
-    gs.load((const T*)a.grad + (row0 * a.heads + head) * a.dim, (int64_t)a.heads * a.dim,
-            t.y - q0, a.dim, a.vec);
+    qs.load((const T*)a.q + row0 * a.q_row + head * a.q_head, t.y - q0, a.dim);
+    gs.load((const T*)a.grad + (row0 * a.heads + head) * a.dim, t.y - q0, a.dim);
+    if (q0 + KS > t.y) absent = qs.find_absent(nullptr, t.y - q0);
     const int i = threadIdx.x;
     lse_n = INFINITY;  // exp2(-inf) = 0 for the rows past the end
     delta_n = 0.0f;
@@ -898,8 +933,8 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
   v8<T> kf[DP / 16], vf[DP / 16];
 #pragma unroll
   for (int i = 0; i < DP / 16; ++i) {
-    kf[i] = load8<T>(k, 16 * i + 8 * g, k_ok, a.dim, a.vec);
-    vf[i] = load8<T>(v, 16 * i + 8 * g, k_ok, a.dim, a.vec);
+    kf[i] = load8<T, VEC>(k, 16 * i + 8 * g, k_ok, a.dim);
+    vf[i] = load8<T, VEC>(v, 16 * i + 8 * g, k_ok, a.dim);
   }
   int kp = 0, klo = 0, khi = 0;
   if (a.pos) {
@@ -917,10 +952,12 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
     if (h > 0) __syncthreads();
     fill_bias<T>(a, head, ext);
     for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
-      qs.put_rows(L.qt[buf]);
-      qs.template put_trans<KT>(L.qtr[buf]);
-      gs.put_rows(L.gt[buf]);
-      gs.template put_trans<KT>(L.gtr[buf]);
+      if (q0 + KS > t.y) {
+        qs.drop(absent);
+        gs.drop(absent);
+      }
+      qs.put(L.q[buf]);
+      gs.put(L.g[buf]);
       if ((int)threadIdx.x < KS) {
         L.lse[buf][threadIdx.x] = lse_n;
         L.delta[buf][threadIdx.x] = delta_n;
@@ -937,7 +974,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
       const float* dels = L.delta[buf] + wk * KT;
       const int* qpos = L.qpos[buf] + wk * KT;
       f32x16 s[KT / 32];
-      tile_product<T, DP, KT>(L.qt[buf] + wk * KT * DP, kf, s);
+      tile_product<T, DP, KT>(L.q[buf] + wk * KT * DP, kf, s);
       float x[KT / 2];
       uint64_t hi = 0, lo = 0;
       if (a.pos) {
@@ -976,8 +1013,8 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
         x[i + 2] = __builtin_amdgcn_exp2f(x[i + 2] - ls.z);
         x[i + 3] = __builtin_amdgcn_exp2f(x[i + 3] - ls.w);
       }
-      trans_product<T, DP, KT>(L.gtr[buf] + wk * KT * DP, x, dva);
-      tile_product<T, DP, KT>(L.gt[buf] + wk * KT * DP, vf, s);  // dP
+      column_product<T, DP, KT>(L.g[buf] + wk * KT * DP, x, dva);
+      tile_product<T, DP, KT>(L.g[buf] + wk * KT * DP, vf, s);  // dP
 #pragma unroll
       for (int i = 0; i < KT / 2; i += 4) {
         const float4 de =
@@ -987,7 +1024,7 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
         x[i + 2] *= s[i / 16][i % 16 + 2] - de.z;
         x[i + 3] *= s[i / 16][i % 16 + 3] - de.w;
       }
-      trans_product<T, DP, KT>(L.qtr[buf] + wk * KT * DP, x, dka);
+      column_product<T, DP, KT>(L.q[buf] + wk * KT * DP, x, dka);
     }
   }
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
@@ -998,8 +1035,8 @@ __global__ __launch_bounds__(64 * NQ * NK) void attn_dkv_kernel(AttnArgs a,
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) dka[n] = dva[n] = f32x16{};
   }
-  store_column<T, DP>(dk + flat, dka, a.scale, a.dim, a.vec);
-  store_column<T, DP>(dv + flat, dva, 1.0f, a.dim, a.vec);
+  store_column<T, DP, VEC>(dk + flat, dka, a.scale, a.dim);
+  store_column<T, DP, VEC>(dv + flat, dva, 1.0f, a.dim);
 }
 
 // dtable[b][head] = sum of the workgroups' parts [head][tile][b]: 8 buckets x
@@ -1033,26 +1070,26 @@ int allow_lds(const void* f, unsigned bytes) {
              : MLCG_ERR_LAUNCH;
 }
 
-template <typename T, int DP, int NQ, int NK>
+template <typename T, int DP, int NQ, int NK, bool VEC>
 int launch_fwd(const AttnArgs& a, void* out, hipStream_t s) {
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds = sizeof(FwdLds<T, DP, NQ, NK>) + 4 * cells;
-  auto f = attn_fwd_kernel<T, DP, NQ, NK>;
+  auto f = attn_fwd_kernel<T, DP, NQ, NK, VEC>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
   hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NQ * NK), lds, s, a,
                      (T*)out);
   return mlcg_launch_status();
 }
 
-template <typename T, int DP, int NQ, int NK>
+template <typename T, int DP, int NQ, int NK, bool VEC>
 int launch_bwd(const AttnArgs& a, const AttnGrads& o, hipStream_t s) {
   constexpr unsigned NW = NQ * NK;
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds1 = sizeof(DqLds<T, DP, NQ, NK>) +
                         4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 1) * cells);
   const unsigned lds2 = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
-  auto f1 = attn_dq_kernel<T, DP, NQ, NK>;
-  auto f2 = attn_dkv_kernel<T, DP, NQ, NK>;
+  auto f1 = attn_dq_kernel<T, DP, NQ, NK, VEC>;
+  auto f2 = attn_dkv_kernel<T, DP, NQ, NK, VEC>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f1), lds1)) return e;
   if (int e = allow_lds(reinterpret_cast<const void*>(f2), lds2)) return e;
   float* delta = o.ws;
@@ -1066,35 +1103,39 @@ int launch_bwd(const AttnArgs& a, const AttnGrads& o, hipStream_t s) {
   return mlcg_launch_status();
 }
 
-// vector loads and stores of four elements: every row and head starts at a
-// multiple of four
+// 16-byte loads and stores: every row and head starts at a multiple of them
 bool attn_vec(const AttnArgs& a, int size) {
   const void* p[] = {a.q, a.k, a.v, a.out, a.grad};
   for (const void* x : p)
-    if (reinterpret_cast<uintptr_t>(x) % (4 * size)) return false;
+    if (!chain_aligned16(x)) return false;
   const int64_t st[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.dim};
   for (int64_t x : st)
-    if (x % 4) return false;
+    if (x * size % 16) return false;
   return true;
 }
 
 template <typename F>
-int by_shape(int dim, int shape, F f) {
+int by_shape(const AttnArgs& a, int shape, int size, F f) {
+  using std::bool_constant;
   using std::integral_constant;
-  auto with = [&](auto dp) {
+  auto with = [&](auto dp, auto vec) {
+    using One = integral_constant<int, 1>;
     switch (shape) {
-      case 11: return f(dp, integral_constant<int, 1>(), integral_constant<int, 1>());
-      case 21: return f(dp, integral_constant<int, 2>(), integral_constant<int, 1>());
-      case 41: return f(dp, integral_constant<int, 4>(), integral_constant<int, 1>());
+      case 11: return f(dp, One(), One(), vec);
+      case 21: return f(dp, integral_constant<int, 2>(), One(), vec);
+      case 41: return f(dp, integral_constant<int, 4>(), One(), vec);
       case 22:
         if constexpr (decltype(dp)::value <= 64)
-          return f(dp, integral_constant<int, 2>(), integral_constant<int, 2>());
+          return f(dp, integral_constant<int, 2>(), integral_constant<int, 2>(), vec);
     }
     return (int)MLCG_ERR_UNSUPPORTED;
   };
-  if (dim <= 32) return with(integral_constant<int, 32>());
-  if (dim <= 64) return with(integral_constant<int, 64>());
-  return with(integral_constant<int, 128>());
+  auto either = [&](auto dp) {
+    return attn_vec(a, size) ? with(dp, bool_constant<true>()) : with(dp, bool_constant<false>());
+  };
+  if (a.dim <= 32) return either(integral_constant<int, 32>());
+  if (a.dim <= 64) return either(integral_constant<int, 64>());
+  return either(integral_constant<int, 128>());
 }
 
 }  // namespace
@@ -1102,18 +1143,18 @@ int by_shape(int dim, int shape, F f) {
 template <>
 int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  a.vec = attn_vec(a, sizeof(T));
-  return by_shape(a.dim, shape, [&](auto dp, auto nq, auto nk) {
-    return launch_fwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value>(a, out, s);
+  return by_shape(a, shape, sizeof(T), [&](auto dp, auto nq, auto nk, auto vec) {
+    return launch_fwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
+                      decltype(vec)::value>(a, out, s);
   });
 }
 
 template <>
 int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  a.vec = attn_vec(a, sizeof(T));
-  return by_shape(a.dim, shape, [&](auto dp, auto nq, auto nk) {
-    return launch_bwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value>(a, o, s);
+  return by_shape(a, shape, sizeof(T), [&](auto dp, auto nq, auto nk, auto vec) {
+    return launch_bwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
+                      decltype(vec)::value>(a, o, s);
   });
 }
 

@@ -4,6 +4,8 @@
 namespace {
 
 bool attn_ok(const AttnArgs& a, int tile_rows, int splits, int dtype) {
+  for (int64_t row : {a.q_row, a.k_row, a.v_row})
+    if (row < 0 || row >= (int64_t(1) << 22)) return false;
   return a.beads >= 0 && a.beads < (int64_t(1) << 31) - 256 && a.heads >= 1 && a.heads <= 1024 &&
          a.dim >= 1 && a.dim <= 128 && a.reach >= 1 && a.reach <= 1024 && a.buckets >= 1 &&
          (int64_t)a.n_tiles * a.heads < (int64_t(1) << 31) &&
@@ -33,7 +35,7 @@ extern "C" int mlcg_chain_attention(const void* q, const int64_t* q_strides, con
   AttnArgs a{q, k, v, table, out, nullptr, q_strides[0], q_strides[1], k_strides[0],
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, lse, (int)n_tiles, heads,
-             heads / kv_heads, dim, reach, buckets, 0, scale};
+             heads / kv_heads, dim, reach, buckets, scale};
   MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype));
   if (beads == 0 || n_tiles == 0) return MLCG_OK;
   MLCG_REQUIRE(q && k && v && table && bucket_of && tiles && out);
@@ -58,7 +60,7 @@ extern "C" int mlcg_chain_attention_backward(
   AttnArgs a{q, k, v, table, out, grad_out, q_strides[0], q_strides[1], k_strides[0],
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, const_cast<float*>(lse),
-             (int)n_tiles, heads, heads / kv_heads, dim, reach, buckets, 0, scale};
+             (int)n_tiles, heads, heads / kv_heads, dim, reach, buckets, scale};
   MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype) && beads >= 1);
   MLCG_REQUIRE(q && k && v && table && bucket_of && bucket_order && bucket_first && tiles && out &&
                lse && grad_out && grad_q && grad_k && grad_v && grad_table && workspace);

@@ -1918,7 +1918,7 @@ def _attention_heads(t: torch.Tensor, name: str, chains: ChainLayout, like: torc
            and t.device == like.device,
            lambda: f"{name} must be [{chains.n_beads}, heads, dim] {like.dtype} on "
                    f"{like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    if (t.stride(2) != 1 and t.shape[2] > 1) or t.stride(0) >= 2 ** 22:
         t = t.contiguous()
     return t, (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
 
