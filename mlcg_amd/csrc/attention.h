@@ -248,14 +248,17 @@ struct Stage {
   }
 };
 
-// ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped
+// ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped; a bias
+// of the type's lowest or highest value stays a number
 template <typename T>
 __device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, float* ext) {
   const int n = 2 * (a.reach + kAttnSpan) + 1;
   const T* table = (const T*)a.table;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int d = min(max(i - kAttnSpan, 0), 2 * a.reach);
-    ext[i] = kAttnLog2e * (float)table[(int64_t)a.bucket_of[d] * a.heads + head];
+    const float b = (float)table[(int64_t)a.bucket_of[d] * a.heads + head];
+    const float e = kAttnLog2e * b;
+    ext[i] = fabsf(e) > 3.0e38f && fabsf(b) != INFINITY ? copysignf(3.0e38f, b) : e;
   }
 }
 
@@ -285,17 +288,30 @@ __device__ __forceinline__ int wave_max(int v) {
   return v;
 }
 
-// the wave's 32 columns of  tile . B  for all KT rows of its tile
+// s += the wave's 32 columns of  tile . B  for all KT rows of its tile
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void tile_product(const T* tile, const v8<T> (&b)[DP / 16],
                                              f32x16 (&s)[KT / 32]) {
   const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
 #pragma unroll
   for (int n = 0; n < KT / 32; ++n) {
-    s[n] = f32x16{};
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)
       mma(s[n], row_frag<T, DP>(tile, 32 * n + col, 16 * k + 8 * g), b[k]);
+  }
+}
+
+// a lane's rows of one value a row
+template <int KT>
+__device__ __forceinline__ void load_rows(const float* rows, f32x16 (&s)[KT / 32]) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < KT / 2; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(rows + 32 * (i / 16) + acc_row(i % 16, g));
+    s[i / 16][i % 16] = v.x;
+    s[i / 16][i % 16 + 1] = v.y;
+    s[i / 16][i % 16 + 2] = v.z;
+    s[i / 16][i % 16 + 3] = v.w;
   }
 }
 
@@ -363,13 +379,14 @@ __device__ __forceinline__ int block_side(int d_min, int d_max, int R) {
   return d_min >= R ? 1 : d_max <= -R ? -1 : 0;
 }
 
-// The logits (base 2) of a tile whose lanes are queries and whose rows are
-// keys, and each block's side.
+// The logits (base 2) less `shift` of a tile whose lanes are queries and whose
+// rows are keys, and each block's side.
 template <int KT>
 __device__ __forceinline__ void query_logits(const AttnArgs& a, const f32x16 (&s)[KT / 32],
                                              const float* ext, const int* kpos, int k0, int qw,
                                              int qi, int qp, int qlo, int qhi, bool valid,
-                                             float (&x)[KT / 2], int (&side)[KT / 32]) {
+                                             float shift, float (&x)[KT / 2],
+                                             int (&side)[KT / 32]) {
   const int lane = threadIdx.x & 63, g = lane >> 5;
   const float c = a.scale * kAttnLog2e;
   const int R = a.reach;
@@ -388,17 +405,18 @@ __device__ __forceinline__ void query_logits(const AttnArgs& a, const f32x16 (&s
 #pragma unroll
   for (int n = 0; n < KT / 32; ++n) {
     if (side[n]) {
-      const float b = side[n] > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+      const float b = (side[n] > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, b);
     } else if (a.pos) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        x[16 * n + i] = fmaf(s[n][i], c, ext[offset_cell(kpos[32 * n + acc_row(i, g)], qp, R)]);
+        x[16 * n + i] =
+            fmaf(s[n][i], c, ext[offset_cell(kpos[32 * n + acc_row(i, g)], qp, R)] - shift);
     } else {
       const float* e = ext + (k0 + 32 * n - qi + 4 * g + R + kAttnSpan);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[acc_row(i, 0)]);
+      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[acc_row(i, 0)] - shift);
     }
   }
 }
@@ -516,26 +534,29 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
     const int kw = k0 + KT * wk;
     if (qw >= t.y || kw >= t.y) continue;
     const float* cap = L.cap[buf] + wk * KT;
-    f32x16 s[KT / 32];
+    f32x16 s[KT / 32] = {};
     tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
     float x[KT / 2];
     int side[KT / 32];
     query_logits<KT>(a, s, ext, L.kpos[buf] + wk * KT, kw, qw, qi, qp, qlo, qhi,
-                     a.pos && cap[lane % KT] > 0.0f, x, side);
+                     a.pos && cap[lane % KT] > 0.0f, base, x, side);
     if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < KT / 2; ++i) top = fmaxf(top, x[i]);
-    top = fmaxf(top, other_half(top));
-    // the maximum follows only where it has grown by more than 2^kAttnLazy:
-    // the exponentials then stay below 2^kAttnLazy, and most tiles leave the
-    // sums alone
-    if (__any(top > m + kAttnLazy)) {
-      const float m_new = fmaxf(m, top);
-      base = m_new == -INFINITY ? 0.0f : m_new;  // no key so far: exp2(-inf) = 0
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
-      m = m_new;
+    // the maximum follows only where it has grown by more than 2^kAttnLazy
+    // (or there was none): the exponentials stay below 2^kAttnLazy, and most
+    // tiles leave the sums alone
+    if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
+      top = fmaxf(top, other_half(top)) + base;
+      m = fmaxf(m, top);
+      const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
+      base += grown;
+      // nothing to scale before the first key, where the base may have to fall
+      const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
       l *= alpha;
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) x[i] -= grown;
 #pragma unroll
       for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -544,7 +565,7 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
     float sum[4] = {};
 #pragma unroll
     for (int i = 0; i < KT / 2; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+      x[i] = __builtin_amdgcn_exp2f(x[i]);
       sum[i % 4] += x[i];
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -582,6 +603,16 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
                       a.dim);
   if (a.lse && g == 0)
     a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// Whether a chain of one tile has one present key at most.  The softmax over
+// one key is constant: the backward passes then take P = 1 and dS = 0, not
+// what the roundings of the sums would leave of them.
+template <int KT>
+__device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
+  if (len > KT) return false;
+  const int lane = threadIdx.x & 63;
+  return __popcll(__ballot(lane < len && (!keep || keep[lane]))) <= 1;
 }
 
 // ---------------------------------------------------------------------------
@@ -781,6 +812,10 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
   else
     for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
+  const bool lone = lone_key<KT>(keep, t.y);
+  f32x16 minus_delta;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
 
   f32x16 acc[DP / 32] = {};
   int buf = 0;
@@ -804,26 +839,22 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
     if (qw >= t.y || kw >= t.y) continue;
     const float* cap = L.cap[buf] + wk * KT;
     const int* kpos = L.kpos[buf] + wk * KT;
-    f32x16 s[KT / 32];
+    f32x16 s[KT / 32] = {};
     tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
     float x[KT / 2];
     int side[KT / 32];
     query_logits<KT>(a, s, ext, kpos, kw, qw, qi, qp, qlo, qhi,
-                     a.pos && cap[lane % KT] > 0.0f, x, side);
+                     a.pos && cap[lane % KT] > 0.0f, lse, x, side);
     if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
 #pragma unroll
-    for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - lse);
-    tile_product<T, DP, KT>(L.v[buf] + wk * KT * DP, gf, s);  // dP
-    if (t.y <= KT) {
-      // a chain of one tile: delta from P and dP themselves, so that a row
-      // of one key has dS = 0 exactly
-      delta = 0.0f;
+    for (int n = 0; n < KT / 32; ++n) s[n] = minus_delta;
+    tile_product<T, DP, KT>(L.v[buf] + wk * KT * DP, gf, s);  // dP - delta
 #pragma unroll
-      for (int i = 0; i < KT / 2; ++i) delta = fmaf(x[i], s[i / 16][i % 16], delta);
-      delta += other_half(delta);
+    for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i / 16][i % 16];
+    if (lone) {
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) x[i] = 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < KT / 2; ++i) x[i] *= s[i / 16][i % 16] - delta;
     bool near = false;
 #pragma unroll
     for (int n = 0; n < KT / 32; ++n) {
@@ -942,7 +973,10 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
     klo = wave_min(kp);
     khi = wave_max(kp);
   }
-  const float c = a.scale * kAttnLog2e;
+  // The sums of the logits begin with -lse / c and those of dP with -delta.  A
+  // scale of 0 is one that leaves nothing of the products.
+  const bool lone = lone_key<KT>(a.keep ? a.keep + t.x : nullptr, t.y);
+  const float c = fabsf(a.scale) < 1e-30f ? 1e-30f : a.scale * kAttnLog2e;
   const int R = a.reach;
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
@@ -959,8 +993,8 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
       qs.put(L.q[buf]);
       gs.put(L.g[buf]);
       if ((int)threadIdx.x < KS) {
-        L.lse[buf][threadIdx.x] = lse_n;
-        L.delta[buf][threadIdx.x] = delta_n;
+        L.lse[buf][threadIdx.x] = -lse_n / c;
+        L.delta[buf][threadIdx.x] = -delta_n;
         L.qpos[buf][threadIdx.x] = pos_n;
       }
       if (q0 + KS < t.y)
@@ -974,6 +1008,7 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
       const float* dels = L.delta[buf] + wk * KT;
       const int* qpos = L.qpos[buf] + wk * KT;
       f32x16 s[KT / 32];
+      load_rows<KT>(lses, s);
       tile_product<T, DP, KT>(L.q[buf] + wk * KT * DP, kf, s);
       float x[KT / 2];
       uint64_t hi = 0, lo = 0;
@@ -1005,25 +1040,17 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
         }
       }
 #pragma unroll
-      for (int i = 0; i < KT / 2; i += 4) {
-        const float4 ls =
-            *reinterpret_cast<const float4*>(lses + 32 * (i / 16) + acc_row(i % 16, g));
-        x[i] = __builtin_amdgcn_exp2f(x[i] - ls.x);
-        x[i + 1] = __builtin_amdgcn_exp2f(x[i + 1] - ls.y);
-        x[i + 2] = __builtin_amdgcn_exp2f(x[i + 2] - ls.z);
-        x[i + 3] = __builtin_amdgcn_exp2f(x[i + 3] - ls.w);
+      for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
+      if (lone) {
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i)
+          x[i] = k_ok && qw + 32 * (i / 16) + acc_row(i % 16, g) < t.y ? 1.0f : 0.0f;
       }
       column_product<T, DP, KT>(L.g[buf] + wk * KT * DP, x, dva);
-      tile_product<T, DP, KT>(L.g[buf] + wk * KT * DP, vf, s);  // dP
+      load_rows<KT>(dels, s);
+      tile_product<T, DP, KT>(L.g[buf] + wk * KT * DP, vf, s);  // dP - delta
 #pragma unroll
-      for (int i = 0; i < KT / 2; i += 4) {
-        const float4 de =
-            *reinterpret_cast<const float4*>(dels + 32 * (i / 16) + acc_row(i % 16, g));
-        x[i] *= s[i / 16][i % 16] - de.x;
-        x[i + 1] *= s[i / 16][i % 16 + 1] - de.y;
-        x[i + 2] *= s[i / 16][i % 16 + 2] - de.z;
-        x[i + 3] *= s[i / 16][i % 16 + 3] - de.w;
-      }
+      for (int i = 0; i < KT / 2; ++i) x[i] = lone ? 0.0f : x[i] * s[i / 16][i % 16];
       column_product<T, DP, KT>(L.q[buf] + wk * KT * DP, x, dka);
     }
   }
