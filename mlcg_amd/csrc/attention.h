@@ -88,19 +88,22 @@ int attn_backward(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s);
 
 namespace {
 
+// rows of a part of a staged tile; they are used 32 at a time
 template <typename T>
-constexpr int key_tile() {
+constexpr int part_rows() {
   return sizeof(T) == 2 ? 64 : 32;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// what row r's chunks are exchanged by, in a tile of N chunks a row
+// what row r's chunks are exchanged by, in a tile of N chunks a row: the 16
+// bytes of 8 consecutive rows, and the 32 bytes of 4 that 16 lanes of the
+// transposing read take, fall on all banks
 template <int N>
 __device__ __forceinline__ constexpr int chunk_swap(int r) {
   static_assert(N >= 4, "a row holds at least four chunks");
-  return N >= 8 ? r & 7 : (r >> 1) & 3;
+  return N >= 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
 }
 
 // element offset of (row, el) in an LDS tile of LEN elements a row
@@ -146,6 +149,11 @@ __device__ __forceinline__ v8<T> column_frag(const T* tile, int u, int n) {
       r[e] = tile[tile_at<T, LEN>(16 * u + 8 * (e / 4) + 4 * g + e % 4, 32 * n + (lane & 31))];
     return r;
   }
+}
+
+// the wave's number in its workgroup, as the one value that it is
+__device__ __forceinline__ int wave_number() {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 }
 
 // the row, within its block of 32, of a lane's accumulator i
@@ -288,42 +296,37 @@ __device__ __forceinline__ int wave_max(int v) {
   return v;
 }
 
-// s += the wave's 32 columns of  tile . B  for all KT rows of its tile
-template <typename T, int DP, int KT>
-__device__ __forceinline__ void tile_product(const T* tile, const v8<T> (&b)[DP / 16],
-                                             f32x16 (&s)[KT / 32]) {
+// s += the wave's 32 columns of  tile . B  for the tile's rows r0 .. r0 + 31
+template <typename T, int DP>
+__device__ __forceinline__ void row_product(const T* tile, int r0, const v8<T> (&b)[DP / 16],
+                                            f32x16& s) {
   const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
 #pragma unroll
-  for (int n = 0; n < KT / 32; ++n) {
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-      mma(s[n], row_frag<T, DP>(tile, 32 * n + col, 16 * k + 8 * g), b[k]);
-  }
+  for (int k = 0; k < DP / 16; ++k) mma(s, row_frag<T, DP>(tile + r0 * DP, col, 16 * k + 8 * g), b[k]);
 }
 
-// a lane's rows of one value a row
-template <int KT>
-__device__ __forceinline__ void load_rows(const float* rows, f32x16 (&s)[KT / 32]) {
-  const int g = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int i = 0; i < KT / 2; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(rows + 32 * (i / 16) + acc_row(i % 16, g));
-    s[i / 16][i % 16] = v.x;
-    s[i / 16][i % 16 + 1] = v.y;
-    s[i / 16][i % 16 + 2] = v.z;
-    s[i / 16][i % 16 + 3] = v.w;
-  }
-}
-
-// acc += tile^T . P  with P the KT rows of a lane's column
-template <typename T, int DP, int KT>
-__device__ __forceinline__ void column_product(const T* tile, const float (&p)[KT / 2],
+// acc += tile^T . P  with P the rows r0 .. r0 + 31 of a lane's column
+template <typename T, int DP>
+__device__ __forceinline__ void column_product(const T* tile, int r0, const float (&p)[16],
                                                f32x16 (&acc)[DP / 32]) {
 #pragma unroll
-  for (int u = 0; u < KT / 16; ++u) {
+  for (int u = 0; u < 2; ++u) {
     const v8<T> b = pack8<T>(p + 8 * u);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) mma(acc[n], column_frag<T, DP>(tile, u, n), b);
+    for (int n = 0; n < DP / 32; ++n) mma(acc[n], column_frag<T, DP>(tile + r0 * DP, u, n), b);
+  }
+}
+
+// a lane's 16 rows of one value a row
+__device__ __forceinline__ void load_rows(const float* rows, f32x16& s) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(rows + acc_row(i, g));
+    s[i] = v.x;
+    s[i + 1] = v.y;
+    s[i + 2] = v.z;
+    s[i + 3] = v.w;
   }
 }
 
@@ -355,7 +358,7 @@ __device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32
 template <int DP, int NQ, int NK>
 __device__ __forceinline__ void join_parts(f32x16 (&acc)[DP / 32], float* buf) {
   if constexpr (NK > 1) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % NQ, wk = wave / NQ;
+    const int lane = threadIdx.x & 63, wave = wave_number(), wq = wave % NQ, wk = wave / NQ;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) {
       __syncthreads();
@@ -373,87 +376,31 @@ __device__ __forceinline__ void join_parts(f32x16 (&acc)[DP / 32], float* buf) {
   }
 }
 
+// scale log2(e); a scale of 0 is one that leaves nothing of the products (sums
+// begin with values divided by it)
+__device__ __forceinline__ float logit_factor(const AttnArgs& a) {
+  return fabsf(a.scale) < 1e-30f ? 1e-30f : a.scale * kAttnLog2e;
+}
+
 // Where a block of 32 rows lies to the wave's columns: all offsets at or past
 // the reach (1), at or before its negative (-1), or neither (0).
 __device__ __forceinline__ int block_side(int d_min, int d_max, int R) {
   return d_min >= R ? 1 : d_max <= -R ? -1 : 0;
 }
 
-// The logits (base 2) less `shift` of a tile whose lanes are queries and whose
-// rows are keys, and each block's side.
-template <int KT>
-__device__ __forceinline__ void query_logits(const AttnArgs& a, const f32x16 (&s)[KT / 32],
-                                             const float* ext, const int* kpos, int k0, int qw,
-                                             int qi, int qp, int qlo, int qhi, bool valid,
-                                             float shift, float (&x)[KT / 2],
-                                             int (&side)[KT / 32]) {
-  const int lane = threadIdx.x & 63, g = lane >> 5;
-  const float c = a.scale * kAttnLog2e;
-  const int R = a.reach;
-  if (a.pos) {
-    const int kp = kpos[lane % KT];
-    const uint64_t hi = __ballot(!valid || __builtin_elementwise_sub_sat(kp, qhi) >= R);
-    const uint64_t lo = __ballot(!valid || __builtin_elementwise_sub_sat(kp, qlo) <= -R);
-#pragma unroll
-    for (int n = 0; n < KT / 32; ++n)
-      side[n] = (uint32_t)(hi >> (32 * n)) == ~0u ? 1 : (uint32_t)(lo >> (32 * n)) == ~0u ? -1 : 0;
-  } else {
-#pragma unroll
-    for (int n = 0; n < KT / 32; ++n)
-      side[n] = block_side(k0 + 32 * n - (qw + 31), k0 + 32 * n + 31 - qw, R);
-  }
-#pragma unroll
-  for (int n = 0; n < KT / 32; ++n) {
-    if (side[n]) {
-      const float b = (side[n] > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, b);
-    } else if (a.pos) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        x[16 * n + i] =
-            fmaf(s[n][i], c, ext[offset_cell(kpos[32 * n + acc_row(i, g)], qp, R)] - shift);
-    } else {
-      const float* e = ext + (k0 + 32 * n - qi + 4 * g + R + kAttnSpan);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[acc_row(i, 0)] - shift);
-    }
-  }
-}
-
-// min(x, cap) as the instruction has it: the smaller number where x is NaN
-__device__ __forceinline__ float min_number(float x, float cap) {
-  float r;
-  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(cap));
-  return r;
-}
-
-// -inf for the absent keys of a tile (cap -inf), whatever stands there; a NaN
-// of a present key (cap +inf) becomes +inf, and the row NaN all the same
-template <int KT>
-__device__ __forceinline__ void mask_logits(const float* cap, float (&x)[KT / 2]) {
-  const int g = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int i = 0; i < KT / 2; i += 4) {
-    const float4 c = *reinterpret_cast<const float4*>(cap + 32 * (i / 16) + acc_row(i % 16, g));
-    x[i] = min_number(x[i], c.x);
-    x[i + 1] = min_number(x[i + 1], c.y);
-    x[i + 2] = min_number(x[i + 2], c.z);
-    x[i + 3] = min_number(x[i + 3], c.w);
-  }
-}
-
-// the keys' caps and positions of a tile: thread i loads row i's
+// What stands for the keys of a tile in LDS: the value that their products'
+// sums begin with (0, or for an absent key what makes the logit -inf), and
+// their positions.  Thread i loads row i's.
 struct KeyInfo {
   float cap;
   int pos;
   __device__ __forceinline__ void load(const AttnArgs& a, const int4& t, int k0, int rows) {
     const int i = threadIdx.x;
-    cap = -INFINITY;
+    cap = logit_factor(a) > 0.0f ? -INFINITY : INFINITY;
     pos = 0;
     if (i < rows && k0 + i < t.y) {
       const int64_t row = (int64_t)t.x + k0 + i;
-      if (!a.keep || a.keep[row]) cap = INFINITY;
+      if (!a.keep || a.keep[row]) cap = 0.0f;
       if (a.pos) pos = a.pos[row];
     }
   }
@@ -465,18 +412,81 @@ struct KeyInfo {
   }
 };
 
+// A wave of queries: its first one, the lane's, and the positions of the
+// lane's and of the wave's ends.
+struct QueryPlace {
+  int first, mine, pos, lo, hi;
+  bool ok;
+  __device__ __forceinline__ QueryPlace(const AttnArgs& a, const int4& t, int begin)
+      : first(begin), mine(begin + (threadIdx.x & 31)), pos(0), lo(0), hi(0) {
+    ok = mine < t.y;
+    if (a.pos) {
+      pos = a.pos[(int64_t)t.x + min(mine, t.y - 1)];
+      lo = wave_min(pos);
+      hi = wave_max(pos);
+    }
+  }
+};
+
+// The logits (base 2) less `shift` of a block whose lanes are queries and
+// whose rows are the keys kb .. kb + 31; returns the block's side.
+__device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16& s, const float* ext,
+                                            const float* cap, const int* kpos, int kb,
+                                            const QueryPlace& q, float shift, float (&x)[16]) {
+  const int g = (threadIdx.x >> 5) & 1;
+  const float c = logit_factor(a);
+  const int R = a.reach;
+  int side;
+  if (a.pos) {
+    const int kp = kpos[threadIdx.x & 31];
+    const bool absent = cap[threadIdx.x & 31] != 0.0f;
+    side = __all(absent || __builtin_elementwise_sub_sat(kp, q.hi) >= R)    ? 1
+           : __all(absent || __builtin_elementwise_sub_sat(kp, q.lo) <= -R) ? -1
+                                                                            : 0;
+  } else {
+    side = block_side(kb - (q.first + 31), kb + 31 - q.first, R);
+  }
+  if (side) {
+    const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, b);
+  } else if (a.pos) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      x[i] = fmaf(s[i], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - shift);
+  } else {
+    const float* e = ext + (kb - q.mine + 4 * g + R + kAttnSpan);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, e[acc_row(i, 0)] - shift);
+  }
+  return side;
+}
+
+// Waves a SIMD that the registers of a kernel are limited for: `values` 32-bit
+// values of fragments and accumulators, and about 70 more.
+constexpr int waves_for(int values) {
+  return values <= 24 ? 4 : values <= 64 ? 3 : 2;
+}
+
 template <typename T, int DP, int NQ, int NK>
 struct FwdLds {
-  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  static constexpr int KS = part_rows<T>() * NK;
   T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
   float ext[1];  // 2 (reach + kAttnSpan) + 1
 };
 
+// a query's fragments, an accumulator of DP rows, a block of logits
+template <typename T, int DP>
+constexpr int fwd_waves() {
+  return waves_for(DP * (int)sizeof(T) / 8 + DP / 2);
+}
+
 template <typename T, int DP, int NQ, int NK, bool VEC>
-__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T* __restrict__ out) {
-  constexpr int KT = key_tile<T>(), KS = KT * NK, NT = 64 * NQ * NK;
+__global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_kernel(
+    AttnArgs a, T* __restrict__ out) {
+  constexpr int RT = part_rows<T>(), KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = FwdLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -484,10 +494,8 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
 
   const int head = blockIdx.x % a.heads, kv = head / a.group;
   const int4 t = a.tiles[blockIdx.x / a.heads];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int lane = threadIdx.x & 63, g = lane >> 5, wave = wave_number();
   const int wq = wave % NQ, wk = wave / NQ;
-  const int qw = t.z + kAttnQ * wq, qi = qw + (lane & 31);
-  const bool q_ok = qi < t.y;
   const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
   const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
@@ -500,22 +508,18 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
   uint32_t absent = ks.find_absent(keep, t.y);
   info.load(a, t, 0, KS);
 
-  const T* q = (const T*)a.q + ((int64_t)t.x + qi) * a.q_row + head * a.q_head;
+  const QueryPlace qi(a, t, t.z + kAttnQ * wq);
+  const T* q = (const T*)a.q + ((int64_t)t.x + qi.mine) * a.q_row + head * a.q_head;
   v8<T> qf[DP / 16];
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, q_ok, a.dim);
-  int qp = 0, qlo = 0, qhi = 0;
-  if (a.pos) {
-    qp = a.pos[(int64_t)t.x + min(qi, t.y - 1)];
-    qlo = wave_min(qp);
-    qhi = wave_max(qp);
-  }
+  for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, qi.ok, a.dim);
   fill_bias<T>(a, head, ext);
 
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, base = 0.0f, l = 0.0f;
   int buf = 0;
-  for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+  // puts the tile of k0 into LDS and sends for the next one
+  auto next_tile = [&](int k0) {
     if (keep || k0 + KS > t.y) {
       ks.drop(absent);
       vs.drop(absent);
@@ -531,45 +535,54 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
       info.load(a, t, kn, KS);
     }
     __syncthreads();
-    const int kw = k0 + KT * wk;
-    if (qw >= t.y || kw >= t.y) continue;
-    const float* cap = L.cap[buf] + wk * KT;
-    f32x16 s[KT / 32] = {};
-    tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
-    float x[KT / 2];
-    int side[KT / 32];
-    query_logits<KT>(a, s, ext, L.kpos[buf] + wk * KT, kw, qw, qi, qp, qlo, qhi,
-                     a.pos && cap[lane % KT] > 0.0f, base, x, side);
-    if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
-    float top = x[0];
+  };
+  if (qi.first >= t.y)  // no queries: this wave only loads
+    for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) next_tile(k0);
+  else for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+    next_tile(k0);
+#pragma unroll RT / 32
+    for (int r0 = RT * wk; r0 < RT * wk + RT && k0 + r0 < t.y; r0 += 32) {
+      const int kb = k0 + r0;
+      f32x16 s;
+      if (keep || kb + 32 > t.y) {
+        load_rows(L.cap[buf] + r0, s);
+        row_product<T, DP>(L.k[buf], r0, qf, s);
+      } else {
+        s = f32x16{};
+        row_product<T, DP>(L.k[buf], r0, qf, s);
+      }
+      float x[16];
+      query_logits(a, s, ext, L.cap[buf] + r0, L.kpos[buf] + r0, kb, qi, base, x);
+      float top = x[0];
 #pragma unroll
-    for (int i = 1; i < KT / 2; ++i) top = fmaxf(top, x[i]);
-    // the maximum follows only where it has grown by more than 2^kAttnLazy
-    // (or there was none): the exponentials stay below 2^kAttnLazy, and most
-    // tiles leave the sums alone
-    if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
-      top = fmaxf(top, other_half(top)) + base;
-      m = fmaxf(m, top);
-      const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
-      base += grown;
-      // nothing to scale before the first key, where the base may have to fall
-      const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
-      l *= alpha;
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+      // the maximum follows only where it has grown by more than 2^kAttnLazy
+      // (or there was none): the exponentials stay below 2^kAttnLazy, and most
+      // blocks leave the sums alone
+      if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
+        top = fmaxf(top, other_half(top)) + base;
+        m = fmaxf(m, top);
+        const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
+        base += grown;
+        // nothing to scale before the first key, where the base may have to fall
+        const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
+        l *= alpha;
 #pragma unroll
-      for (int i = 0; i < KT / 2; ++i) x[i] -= grown;
+        for (int i = 0; i < 16; ++i) x[i] -= grown;
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n)
+        for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+          for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+      }
+      float sum[4] = {};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i]);
+        sum[i % 4] += x[i];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      column_product<T, DP>(L.v[buf], r0, x, acc);
     }
-    float sum[4] = {};
-#pragma unroll
-    for (int i = 0; i < KT / 2; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i]);
-      sum[i % 4] += x[i];
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    column_product<T, DP, KT>(L.v[buf] + wk * KT * DP, x, acc);
   }
   l += other_half(l);
   if constexpr (NK > 1) {
@@ -597,20 +610,20 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_fwd_kernel(AttnArgs a, T
       for (int r = 0; r < 16; ++r) acc[n][r] *= f;
     join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
   }
-  if (wk > 0 || !q_ok) return;
-  const int64_t row = (int64_t)t.x + qi;
-  store_column<T, DP, VEC>(out + (row * a.heads + head) * a.dim, acc, l == 0.0f ? 0.0f : 1.0f / l,
-                      a.dim);
+  if (wk > 0 || !qi.ok) return;
+  const int64_t row = (int64_t)t.x + qi.mine;
+  store_column<T, DP, VEC>(out + (row * a.heads + head) * a.dim, acc,
+                           l == 0.0f ? 0.0f : 1.0f / l, a.dim);
   if (a.lse && g == 0)
     a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// Whether a chain of one tile has one present key at most.  The softmax over
+// Whether a chain of one part has one present key at most.  The softmax over
 // one key is constant: the backward passes then take P = 1 and dS = 0, not
 // what the roundings of the sums would leave of them.
-template <int KT>
+template <int RT>
 __device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
-  if (len > KT) return false;
+  if (len > RT) return false;
   const int lane = threadIdx.x & 63;
   return __popcll(__ballot(lane < len && (!keep || keep[lane]))) <= 1;
 }
@@ -640,12 +653,12 @@ __device__ __forceinline__ void add_diagonals(const float* x, float* scratch, fl
 }
 
 // Sums by offset for given positions: integers of dS 2^e, a high part of at
-// most 2^15 and 15 bits below it, 16 tiles (2^11 values each) at most before
+// most 2^15 and 15 bits below it, 32 blocks (2^10 values each) at most before
 // they are moved to the wave's float array.
 struct OffsetInts {
   int *hi, *lo;
-  float scale, inverse;  // 2^e, or 0 before the first tile
-  int tiles;
+  float scale, inverse;  // 2^e, or 0 before the first block
+  int blocks;
   bool poison;
   int cells;
   float* mine;  // of the offset -reach
@@ -655,7 +668,7 @@ struct OffsetInts {
     hi = space;
     lo = space + cells;
     scale = inverse = 0.0f;
-    tiles = 0;
+    blocks = 0;
     poison = false;
     mine = at;
     for (int i = threadIdx.x & 63; i < 2 * cells; i += 64) space[i] = 0;
@@ -667,9 +680,9 @@ struct OffsetInts {
       mine[i] += v;
       hi[i] = lo[i] = 0;
     }
-    tiles = 0;
+    blocks = 0;
   }
-  // makes room for a tile of values up to `top`
+  // makes room for a block of values up to `top`
   __device__ __forceinline__ void prepare(float top) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -677,7 +690,7 @@ struct OffsetInts {
       poison = true;
       top = 0.0f;
     }
-    if (tiles == 16 || !(top * scale <= 32768.0f) || (scale == 0.0f && top > 0.0f)) {
+    if (blocks == 32 || !(top * scale <= 32768.0f) || (scale == 0.0f && top > 0.0f)) {
       if (scale != 0.0f) flush();
       if (top > 0.0f) {
         int e;
@@ -686,9 +699,9 @@ struct OffsetInts {
         scale = ldexpf(1.0f, 15 - e);
         inverse = ldexpf(1.0f, e - 15);
       }
-      tiles = 0;
+      blocks = 0;
     }
-    ++tiles;
+    ++blocks;
   }
   __device__ __forceinline__ void add(int cell, float v) {
     const float y = v * scale, h = rintf(y);
@@ -740,21 +753,27 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
 
 template <typename T, int DP, int NQ, int NK>
 struct DqLds {
-  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  static constexpr int KS = part_rows<T>() * NK;
   T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
   float rest[4];  // scratch of the waves, ext, dd of the waves
 };
 
+// fragments of q and do, an accumulator, -delta
+template <typename T, int DP>
+constexpr int dq_waves() {
+  return waves_for(2 * (DP * (int)sizeof(T) / 8) + DP / 2 + 16);
+}
+
 // dq, delta and the workgroup's part of the table's gradient; lanes are
 // queries as in the forward pass.
 template <typename T, int DP, int NQ, int NK, bool VEC>
-__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
+__global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
     const int32_t* __restrict__ order, const int32_t* __restrict__ first,
     float* __restrict__ dtable_part) {
-  constexpr int KT = key_tile<T>(), KS = KT * NK, NW = NQ * NK, NT = 64 * NW;
+  constexpr int RT = part_rows<T>(), KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
   using Lds = DqLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -765,11 +784,8 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
 
   const int head = blockIdx.x % a.heads, kv = head / a.group, tile = blockIdx.x / a.heads;
   const int4 t = a.tiles[tile];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int lane = threadIdx.x & 63, g = lane >> 5, wave = wave_number();
   const int wq = wave % NQ, wk = wave / NQ;
-  const int qw = t.z + kAttnQ * wq, qi = qw + (lane & 31);
-  const bool q_ok = qi < t.y;
-  const int64_t row = (int64_t)t.x + qi;
   const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
   const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
@@ -782,26 +798,22 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
   uint32_t absent = ks.find_absent(keep, t.y);
   info.load(a, t, 0, KS);
 
+  const QueryPlace qi(a, t, t.z + kAttnQ * wq);
+  const int64_t row = (int64_t)t.x + qi.mine;
   const T* q = (const T*)a.q + row * a.q_row + head * a.q_head;
   const int64_t flat = (row * a.heads + head) * a.dim;
   v8<T> qf[DP / 16], gf[DP / 16];
   float delta = 0.0f;
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
-    qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, q_ok, a.dim);
-    gf[k] = load8<T, VEC>((const T*)a.grad + flat, 16 * k + 8 * g, q_ok, a.dim);
-    const v8<T> of = load8<T, VEC>((const T*)a.out + flat, 16 * k + 8 * g, q_ok, a.dim);
+    qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, qi.ok, a.dim);
+    gf[k] = load8<T, VEC>((const T*)a.grad + flat, 16 * k + 8 * g, qi.ok, a.dim);
+    const v8<T> of = load8<T, VEC>((const T*)a.out + flat, 16 * k + 8 * g, qi.ok, a.dim);
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[k][e], (float)of[e], delta);
   }
   delta += other_half(delta);
-  const float lse = q_ok ? a.lse[head * a.beads + row] : INFINITY;
-  int qp = 0, qlo = 0, qhi = 0;
-  if (a.pos) {
-    qp = a.pos[(int64_t)t.x + min(qi, t.y - 1)];
-    qlo = wave_min(qp);
-    qhi = wave_max(qp);
-  }
+  const float lse = qi.ok ? a.lse[head * a.beads + row] : INFINITY;
   fill_bias<T>(a, head, ext);
   for (int i = threadIdx.x; i < NW * cells; i += NT) dd[i] = 0.0f;
   float* mine = dd + wave * cells;
@@ -812,14 +824,15 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
   else
     for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
-  const bool lone = lone_key<KT>(keep, t.y);
+  const bool lone = lone_key<RT>(keep, t.y);
   f32x16 minus_delta;
 #pragma unroll
   for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
 
   f32x16 acc[DP / 32] = {};
   int buf = 0;
-  for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+  // puts the tile of k0 into LDS and sends for the next one
+  auto next_tile = [&](int k0) {
     if (keep || k0 + KS > t.y) {
       ks.drop(absent);
       vs.drop(absent);
@@ -835,60 +848,58 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
       info.load(a, t, kn, KS);
     }
     __syncthreads();
-    const int kw = k0 + KT * wk;
-    if (qw >= t.y || kw >= t.y) continue;
-    const float* cap = L.cap[buf] + wk * KT;
-    const int* kpos = L.kpos[buf] + wk * KT;
-    f32x16 s[KT / 32] = {};
-    tile_product<T, DP, KT>(L.k[buf] + wk * KT * DP, qf, s);
-    float x[KT / 2];
-    int side[KT / 32];
-    query_logits<KT>(a, s, ext, kpos, kw, qw, qi, qp, qlo, qhi,
-                     a.pos && cap[lane % KT] > 0.0f, lse, x, side);
-    if (keep || kw + KT > t.y) mask_logits<KT>(cap, x);
+  };
+  if (qi.first >= t.y)  // no queries: this wave only loads
+    for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) next_tile(k0);
+  else for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
+    next_tile(k0);
+#pragma unroll RT / 32
+    for (int r0 = RT * wk; r0 < RT * wk + RT && k0 + r0 < t.y; r0 += 32) {
+      const int kb = k0 + r0;
+      const int* kpos = L.kpos[buf] + r0;
+      f32x16 s;
+      if (keep || kb + 32 > t.y) {
+        load_rows(L.cap[buf] + r0, s);
+        row_product<T, DP>(L.k[buf], r0, qf, s);
+      } else {
+        s = f32x16{};
+        row_product<T, DP>(L.k[buf], r0, qf, s);
+      }
+      float x[16];
+      const int side = query_logits(a, s, ext, L.cap[buf] + r0, kpos, kb, qi, lse, x);
+      s = minus_delta;
+      row_product<T, DP>(L.v[buf], r0, gf, s);  // dP - delta
 #pragma unroll
-    for (int n = 0; n < KT / 32; ++n) s[n] = minus_delta;
-    tile_product<T, DP, KT>(L.v[buf] + wk * KT * DP, gf, s);  // dP - delta
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i];
+      if (lone) {
 #pragma unroll
-    for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i / 16][i % 16];
-    if (lone) {
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) x[i] = 0.0f;
-    }
-    bool near = false;
-#pragma unroll
-    for (int n = 0; n < KT / 32; ++n) {
-      if (side[n]) {
+        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+      }
+      if (side) {
         float sum[4] = {};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i % 4] += x[16 * n + i];
+        for (int i = 0; i < 16; ++i) sum[i % 4] += x[i];
         const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (side[n] > 0)
+        if (side > 0)
           far_hi += all;
         else
           far_lo += all;
-      } else if (a.pos) {
-        near = true;
+      } else if (!a.pos) {
+        add_diagonals(x, scratch, mine + (kb - qi.first + R + kAttnSpan));
       } else {
-        add_diagonals(x + 16 * n, scratch, mine + (kw + 32 * n - qw + R + kAttnSpan));
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+        // NaN does not survive the maximum
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = x[i] != x[i] ? INFINITY : top;
+        ints.prepare(top);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          ints.add(offset_cell(kpos[acc_row(i, g)], qi.pos, R) - kAttnSpan, x[i]);
       }
+      column_product<T, DP>(L.k[buf], r0, x, acc);
     }
-    if (near) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) top = fmaxf(top, fabsf(x[i]));
-      // NaN does not survive the maximum
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) top = x[i] != x[i] ? INFINITY : top;
-      ints.prepare(top);
-#pragma unroll
-      for (int n = 0; n < KT / 32; ++n)
-        if (!side[n])
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            ints.add(offset_cell(kpos[32 * n + acc_row(i, g)], qp, R) - kAttnSpan, x[16 * n + i]);
-    }
-    column_product<T, DP, KT>(L.k[buf] + wk * KT * DP, x, acc);
   }
   if (a.pos) ints.flush();
   far_lo = mlcg_wave_sum(far_lo);
@@ -898,7 +909,7 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
     mine[cells - 1] += far_hi;
   }
   join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
-  if (q_ok && wk == 0) {
+  if (qi.ok && wk == 0) {
     store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
     if (g == 0) delta_out[head * a.beads + row] = delta;
   }
@@ -908,21 +919,25 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dq_kernel(
 
 template <typename T, int DP, int NQ, int NK>
 struct DkvLds {
-  static constexpr int KT = key_tile<T>(), KS = KT * NK;
+  static constexpr int KS = part_rows<T>() * NK;
   T q[2][KS * DP], g[2][KS * DP];
   float lse[2][KS], delta[2][KS];
   int qpos[2][KS];
   float ext[1];
 };
 
+// fragments of k and v and two accumulators
+template <typename T, int DP>
+constexpr int dkv_waves() {
+  return waves_for(2 * (DP * (int)sizeof(T) / 8) + DP);
+}
+
 // dk and dv; lanes are keys, the tiles hold queries.  The query heads that
 // share a key/value head are taken one after the other.
 template <typename T, int DP, int NQ, int NK, bool VEC>
-__global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
-                                                                const float* __restrict__ delta,
-                                                                T* __restrict__ dk,
-                                                                T* __restrict__ dv) {
-  constexpr int KT = key_tile<T>(), KS = KT * NK, NT = 64 * NQ * NK;
+__global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
+    AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
+  constexpr int RT = part_rows<T>(), KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = DkvLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -931,11 +946,14 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
   const int kv_heads = a.heads / a.group;
   const int kv = blockIdx.x % kv_heads;
   const int4 t = a.tiles[blockIdx.x / kv_heads];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 5;
+  const int lane = threadIdx.x & 63, g = lane >> 5, wave = wave_number();
   const int wq = wave % NQ, wk = wave / NQ;
   const int kw = t.z + kAttnQ * wq, ki = kw + (lane & 31);
   const int64_t row = (int64_t)t.x + ki;
   const bool in = ki < t.y, k_ok = in && (!a.keep || a.keep[row]);
+  // the sums of the logits begin with -lse / c, those of dP with -delta
+  const float c = logit_factor(a);
+  const int R = a.reach;
 
   Stage<T, DP, KS, NT, VEC> qs, gs;
   qs.init((int)a.q_row, a.dim);
@@ -973,85 +991,85 @@ __global__ __launch_bounds__(64 * NQ * NK, 2) void attn_dkv_kernel(AttnArgs a,
     klo = wave_min(kp);
     khi = wave_max(kp);
   }
-  // The sums of the logits begin with -lse / c and those of dP with -delta.  A
-  // scale of 0 is one that leaves nothing of the products.
-  const bool lone = lone_key<KT>(a.keep ? a.keep + t.x : nullptr, t.y);
-  const float c = fabsf(a.scale) < 1e-30f ? 1e-30f : a.scale * kAttnLog2e;
-  const int R = a.reach;
+  const bool lone = lone_key<RT>(a.keep ? a.keep + t.x : nullptr, t.y);
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
   int buf = 0;
+  // puts the tile of q0 into LDS and sends for the next one
+  auto next_tile = [&](int h, int q0) {
+    if (q0 + KS > t.y) {
+      qs.drop(absent);
+      gs.drop(absent);
+    }
+    qs.put(L.q[buf]);
+    gs.put(L.g[buf]);
+    if ((int)threadIdx.x < KS) {
+      L.lse[buf][threadIdx.x] = -lse_n / c;
+      L.delta[buf][threadIdx.x] = -delta_n;
+      L.qpos[buf][threadIdx.x] = pos_n;
+    }
+    if (q0 + KS < t.y)
+      load(kv * a.group + h, q0 + KS);
+    else if (h + 1 < a.group)
+      load(kv * a.group + h + 1, 0);
+    __syncthreads();
+  };
   for (int h = 0; h < a.group; ++h) {
     const int head = kv * a.group + h;
     if (h > 0) __syncthreads();
     fill_bias<T>(a, head, ext);
-    for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
-      if (q0 + KS > t.y) {
-        qs.drop(absent);
-        gs.drop(absent);
-      }
-      qs.put(L.q[buf]);
-      gs.put(L.g[buf]);
-      if ((int)threadIdx.x < KS) {
-        L.lse[buf][threadIdx.x] = -lse_n / c;
-        L.delta[buf][threadIdx.x] = -delta_n;
-        L.qpos[buf][threadIdx.x] = pos_n;
-      }
-      if (q0 + KS < t.y)
-        load(head, q0 + KS);
-      else if (h + 1 < a.group)
-        load(head + 1, 0);
-      __syncthreads();
-      const int qw = q0 + KT * wk;
-      if (kw >= t.y || qw >= t.y) continue;
-      const float* lses = L.lse[buf] + wk * KT;
-      const float* dels = L.delta[buf] + wk * KT;
-      const int* qpos = L.qpos[buf] + wk * KT;
-      f32x16 s[KT / 32];
-      load_rows<KT>(lses, s);
-      tile_product<T, DP, KT>(L.q[buf] + wk * KT * DP, kf, s);
-      float x[KT / 2];
-      uint64_t hi = 0, lo = 0;
-      if (a.pos) {
-        const int qp = qpos[lane % KT];
-        const bool past = qw + lane % KT >= t.y;
-        hi = __ballot(past || __builtin_elementwise_sub_sat(klo, qp) >= R);
-        lo = __ballot(past || __builtin_elementwise_sub_sat(khi, qp) <= -R);
-      }
-#pragma unroll
-      for (int n = 0; n < KT / 32; ++n) {
-        const int q_n = qw + 32 * n;
-        const int side = a.pos ? ((uint32_t)(hi >> (32 * n)) == ~0u   ? 1
-                                  : (uint32_t)(lo >> (32 * n)) == ~0u ? -1
-                                                                      : 0)
-                               : block_side(kw - (q_n + 31), kw + 31 - q_n, R);
+    if (kw >= t.y)  // no keys: this wave only loads
+      for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) next_tile(h, q0);
+    else for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
+      next_tile(h, q0);
+#pragma unroll RT / 32
+      for (int r0 = RT * wk; r0 < RT * wk + RT && q0 + r0 < t.y; r0 += 32) {
+        const int qb = q0 + r0;
+        const int* qpos = L.qpos[buf] + r0;
+        f32x16 s;
+        load_rows(L.lse[buf] + r0, s);
+        row_product<T, DP>(L.q[buf], r0, kf, s);
+        float x[16];
+        int side;
+        if (a.pos) {
+          const int qp = qpos[lane & 31];
+          const bool past = qb + (lane & 31) >= t.y;
+          side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
+                 : __all(past || __builtin_elementwise_sub_sat(khi, qp) <= -R) ? -1
+                                                                               : 0;
+        } else {
+          side = block_side(kw - (qb + 31), kw + 31 - qb, R);
+        }
         if (side) {
           const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, b);
+          for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, b);
         } else if (a.pos) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            x[16 * n + i] = fmaf(s[n][i], c, ext[offset_cell(kp, qpos[32 * n + acc_row(i, g)], R)]);
+            x[i] = fmaf(s[i], c, ext[offset_cell(kp, qpos[acc_row(i, g)], R)]);
         } else {
-          const float* e = ext + (ki - q_n - 4 * g + R + kAttnSpan);
+          const float* e = ext + (ki - qb - 4 * g + R + kAttnSpan);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[16 * n + i] = fmaf(s[n][i], c, e[-acc_row(i, 0)]);
+          for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, e[-acc_row(i, 0)]);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
+        if (lone) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = k_ok && qb + acc_row(i, g) < t.y ? 1.0f : 0.0f;
+        }
+        column_product<T, DP>(L.g[buf], r0, x, dva);
+        load_rows(L.delta[buf] + r0, s);
+        row_product<T, DP>(L.g[buf], r0, vf, s);  // dP - delta
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= s[i];
+        if (lone) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+        }
+        column_product<T, DP>(L.q[buf], r0, x, dka);
       }
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
-      if (lone) {
-#pragma unroll
-        for (int i = 0; i < KT / 2; ++i)
-          x[i] = k_ok && qw + 32 * (i / 16) + acc_row(i % 16, g) < t.y ? 1.0f : 0.0f;
-      }
-      column_product<T, DP, KT>(L.g[buf] + wk * KT * DP, x, dva);
-      load_rows<KT>(dels, s);
-      tile_product<T, DP, KT>(L.g[buf] + wk * KT * DP, vf, s);  // dP - delta
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) x[i] = lone ? 0.0f : x[i] * s[i / 16][i % 16];
-      column_product<T, DP, KT>(L.q[buf] + wk * KT * DP, x, dka);
     }
   }
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
@@ -1154,6 +1172,10 @@ int by_shape(const AttnArgs& a, int shape, int size, F f) {
       case 22:
         if constexpr (decltype(dp)::value <= 64)
           return f(dp, integral_constant<int, 2>(), integral_constant<int, 2>(), vec);
+        break;
+      case 42:
+        if constexpr (decltype(dp)::value <= 64)
+          return f(dp, integral_constant<int, 4>(), integral_constant<int, 2>(), vec);
     }
     return (int)MLCG_ERR_UNSUPPORTED;
   };

@@ -10,7 +10,7 @@ bool attn_ok(const AttnArgs& a, int tile_rows, int splits, int dtype) {
          a.dim >= 1 && a.dim <= 128 && a.reach >= 1 && a.reach <= 1024 && a.buckets >= 1 &&
          (int64_t)a.n_tiles * a.heads < (int64_t(1) << 31) &&
          (tile_rows == 32 || tile_rows == 64 || tile_rows == 128) &&
-         (splits == 1 || (splits == 2 && tile_rows == 64)) && dtype >= MLCG_DTYPE_F32 &&
+         (splits == 1 || (splits == 2 && tile_rows >= 64)) && dtype >= MLCG_DTYPE_F32 &&
          dtype <= MLCG_DTYPE_BF16;
 }
 
