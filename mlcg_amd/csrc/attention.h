@@ -156,9 +156,9 @@ __device__ __forceinline__ int wave_number() {
   return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 }
 
-// the row, within its block of 32, of a lane's accumulator i
+// the row of a lane's accumulator i % 16 of block i / 16
 __device__ __forceinline__ constexpr int acc_row(int i, int g) {
-  return 8 * (i / 4) + 4 * g + i % 4;
+  return 8 * (i / 4) + 4 * g + i % 4;  // 32 a block
 }
 
 __device__ __forceinline__ void mma(f32x16& c, v8<__bf16> a, v8<__bf16> b) {
@@ -296,37 +296,41 @@ __device__ __forceinline__ int wave_max(int v) {
   return v;
 }
 
-// s += the wave's 32 columns of  tile . B  for the tile's rows r0 .. r0 + 31
-template <typename T, int DP>
-__device__ __forceinline__ void row_product(const T* tile, int r0, const v8<T> (&b)[DP / 16],
-                                            f32x16& s) {
+// s[n] += the wave's 32 columns of  tile . B  for the rows 32 n .. 32 n + 31
+template <typename T, int DP, int N>
+__device__ __forceinline__ void row_product(const T* tile, const v8<T> (&b)[DP / 16],
+                                            f32x16 (&s)[N]) {
   const int col = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1;
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) mma(s, row_frag<T, DP>(tile + r0 * DP, col, 16 * k + 8 * g), b[k]);
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+      mma(s[n], row_frag<T, DP>(tile + 32 * n * DP, col, 16 * k + 8 * g), b[k]);
 }
 
-// acc += tile^T . P  with P the rows r0 .. r0 + 31 of a lane's column
-template <typename T, int DP>
-__device__ __forceinline__ void column_product(const T* tile, int r0, const float (&p)[16],
+// acc += tile^T . P  with P the 32 N rows of a lane's column
+template <typename T, int DP, int N>
+__device__ __forceinline__ void column_product(const T* tile, const float (&p)[16 * N],
                                                f32x16 (&acc)[DP / 32]) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < 2 * N; ++u) {
     const v8<T> b = pack8<T>(p + 8 * u);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) mma(acc[n], column_frag<T, DP>(tile + r0 * DP, u, n), b);
+    for (int n = 0; n < DP / 32; ++n) mma(acc[n], column_frag<T, DP>(tile, u, n), b);
   }
 }
 
-// a lane's 16 rows of one value a row
-__device__ __forceinline__ void load_rows(const float* rows, f32x16& s) {
+// a lane's rows of one value a row
+template <int N>
+__device__ __forceinline__ void load_rows(const float* rows, f32x16 (&s)[N]) {
   const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) {
+  for (int i = 0; i < 16 * N; i += 4) {
     const float4 v = *reinterpret_cast<const float4*>(rows + acc_row(i, g));
-    s[i] = v.x;
-    s[i + 1] = v.y;
-    s[i + 2] = v.z;
-    s[i + 3] = v.w;
+    s[i / 16][i % 16] = v.x;
+    s[i / 16][i % 16 + 1] = v.y;
+    s[i / 16][i % 16 + 2] = v.z;
+    s[i / 16][i % 16 + 3] = v.w;
   }
 }
 
@@ -382,8 +386,8 @@ __device__ __forceinline__ float logit_factor(const AttnArgs& a) {
   return fabsf(a.scale) < 1e-30f ? 1e-30f : a.scale * kAttnLog2e;
 }
 
-// Where a block of 32 rows lies to the wave's columns: all offsets at or past
-// the reach (1), at or before its negative (-1), or neither (0).
+// Where `rows` rows lie to the wave's 32 columns: all offsets at or past the
+// reach (1), at or before its negative (-1), or neither (0).
 __device__ __forceinline__ int block_side(int d_min, int d_max, int R) {
   return d_min >= R ? 1 : d_max <= -R ? -1 : 0;
 }
@@ -428,36 +432,38 @@ struct QueryPlace {
   }
 };
 
-// The logits (base 2) less `shift` of a block whose lanes are queries and
-// whose rows are the keys kb .. kb + 31; returns the block's side.
-__device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16& s, const float* ext,
-                                            const float* cap, const int* kpos, int kb,
-                                            const QueryPlace& q, float shift, float (&x)[16]) {
-  const int g = (threadIdx.x >> 5) & 1;
+// The logits (base 2) less `shift` of 32 N keys from kb on (rows) and the
+// wave's queries (lanes); returns the keys' side.
+template <int N>
+__device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)[N],
+                                            const float* ext, const float* cap, const int* kpos,
+                                            int kb, const QueryPlace& q, float shift,
+                                            float (&x)[16 * N]) {
+  const int lane = threadIdx.x & 63, g = lane >> 5;
   const float c = logit_factor(a);
   const int R = a.reach;
   int side;
   if (a.pos) {
-    const int kp = kpos[threadIdx.x & 31];
-    const bool absent = cap[threadIdx.x & 31] != 0.0f;
+    const int kp = kpos[lane % (32 * N)];
+    const bool absent = cap[lane % (32 * N)] != 0.0f;
     side = __all(absent || __builtin_elementwise_sub_sat(kp, q.hi) >= R)    ? 1
            : __all(absent || __builtin_elementwise_sub_sat(kp, q.lo) <= -R) ? -1
                                                                             : 0;
   } else {
-    side = block_side(kb - (q.first + 31), kb + 31 - q.first, R);
+    side = block_side(kb - (q.first + 31), kb + 32 * N - 1 - q.first, R);
   }
   if (side) {
     const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, b);
+    for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
   } else if (a.pos) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      x[i] = fmaf(s[i], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - shift);
+    for (int i = 0; i < 16 * N; ++i)
+      x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - shift);
   } else {
     const float* e = ext + (kb - q.mine + 4 * g + R + kAttnSpan);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, e[acc_row(i, 0)] - shift);
+    for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, e[acc_row(i, 0)] - shift);
   }
   return side;
 }
@@ -465,7 +471,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16& s, 
 // Waves a SIMD that the registers of a kernel are limited for: `values` 32-bit
 // values of fragments and accumulators, and about 70 more.
 constexpr int waves_for(int values) {
-  return values <= 24 ? 4 : values <= 64 ? 3 : 2;
+  return values <= 24 ? 3 : 2;
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -486,7 +492,7 @@ constexpr int fwd_waves() {
 template <typename T, int DP, int NQ, int NK, bool VEC>
 __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_kernel(
     AttnArgs a, T* __restrict__ out) {
-  constexpr int RT = part_rows<T>(), KS = RT * NK, NT = 64 * NQ * NK;
+  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = FwdLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -540,49 +546,44 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_k
     for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) next_tile(k0);
   else for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
     next_tile(k0);
-#pragma unroll RT / 32
-    for (int r0 = RT * wk; r0 < RT * wk + RT && k0 + r0 < t.y; r0 += 32) {
-      const int kb = k0 + r0;
-      f32x16 s;
-      if (keep || kb + 32 > t.y) {
-        load_rows(L.cap[buf] + r0, s);
-        row_product<T, DP>(L.k[buf], r0, qf, s);
-      } else {
-        s = f32x16{};
-        row_product<T, DP>(L.k[buf], r0, qf, s);
-      }
-      float x[16];
-      query_logits(a, s, ext, L.cap[buf] + r0, L.kpos[buf] + r0, kb, qi, base, x);
-      float top = x[0];
+    const int kb = k0 + RT * wk;
+    if (kb >= t.y) continue;
+    const T* vt = L.v[buf] + RT * wk * DP;
+    const float* cap = L.cap[buf] + RT * wk;
+    f32x16 s[N];
+    load_rows<N>(cap, s);
+    row_product<T, DP, N>(L.k[buf] + RT * wk * DP, qf, s);
+    float x[16 * N];
+    query_logits<N>(a, s, ext, cap, L.kpos[buf] + RT * wk, kb, qi, base, x);
+    float top = x[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-      // the maximum follows only where it has grown by more than 2^kAttnLazy
-      // (or there was none): the exponentials stay below 2^kAttnLazy, and most
-      // blocks leave the sums alone
-      if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
-        top = fmaxf(top, other_half(top)) + base;
-        m = fmaxf(m, top);
-        const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
-        base += grown;
-        // nothing to scale before the first key, where the base may have to fall
-        const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
-        l *= alpha;
+    for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, x[i]);
+    // the maximum follows only where it has grown by more than 2^kAttnLazy
+    // (or there was none): the exponentials stay below 2^kAttnLazy, and most
+    // tiles leave the sums alone
+    if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
+      top = fmaxf(top, other_half(top)) + base;
+      m = fmaxf(m, top);
+      const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
+      base += grown;
+      // nothing to scale before the first key, where the base may have to fall
+      const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
+      l *= alpha;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] -= grown;
+      for (int i = 0; i < 16 * N; ++i) x[i] -= grown;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
+      for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
-      }
-      float sum[4] = {};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i]);
-        sum[i % 4] += x[i];
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      column_product<T, DP>(L.v[buf], r0, x, acc);
+        for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
     }
+    float sum[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16 * N; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i]);
+      sum[i % 4] += x[i];
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    column_product<T, DP, N>(vt, x, acc);
   }
   l += other_half(l);
   if constexpr (NK > 1) {
@@ -618,12 +619,11 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_k
     a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// Whether a chain of one part has one present key at most.  The softmax over
-// one key is constant: the backward passes then take P = 1 and dS = 0, not
-// what the roundings of the sums would leave of them.
-template <int RT>
+// Whether a chain has one present key at most, of up to 64 beads.  The softmax
+// over one key is constant: the backward passes then write dq = dk = 0 and dv
+// the sum of do, not what the roundings of their sums would leave of them.
 __device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
-  if (len > RT) return false;
+  if (len > 64) return false;
   const int lane = threadIdx.x & 63;
   return __popcll(__ballot(lane < len && (!keep || keep[lane]))) <= 1;
 }
@@ -653,12 +653,12 @@ __device__ __forceinline__ void add_diagonals(const float* x, float* scratch, fl
 }
 
 // Sums by offset for given positions: integers of dS 2^e, a high part of at
-// most 2^15 and 15 bits below it, 32 blocks (2^10 values each) at most before
+// most 2^15 and 15 bits below it, 16 tiles (up to 2^11 values each) before
 // they are moved to the wave's float array.
 struct OffsetInts {
   int *hi, *lo;
-  float scale, inverse;  // 2^e, or 0 before the first block
-  int blocks;
+  float scale, inverse;  // 2^e, or 0 before the first tile
+  int tiles;
   bool poison;
   int cells;
   float* mine;  // of the offset -reach
@@ -668,7 +668,7 @@ struct OffsetInts {
     hi = space;
     lo = space + cells;
     scale = inverse = 0.0f;
-    blocks = 0;
+    tiles = 0;
     poison = false;
     mine = at;
     for (int i = threadIdx.x & 63; i < 2 * cells; i += 64) space[i] = 0;
@@ -680,9 +680,9 @@ struct OffsetInts {
       mine[i] += v;
       hi[i] = lo[i] = 0;
     }
-    blocks = 0;
+    tiles = 0;
   }
-  // makes room for a block of values up to `top`
+  // makes room for a tile of values up to `top`
   __device__ __forceinline__ void prepare(float top) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -690,7 +690,7 @@ struct OffsetInts {
       poison = true;
       top = 0.0f;
     }
-    if (blocks == 32 || !(top * scale <= 32768.0f) || (scale == 0.0f && top > 0.0f)) {
+    if (tiles == 16 || !(top * scale <= 32768.0f) || (scale == 0.0f && top > 0.0f)) {
       if (scale != 0.0f) flush();
       if (top > 0.0f) {
         int e;
@@ -699,9 +699,9 @@ struct OffsetInts {
         scale = ldexpf(1.0f, 15 - e);
         inverse = ldexpf(1.0f, e - 15);
       }
-      blocks = 0;
+      tiles = 0;
     }
-    ++blocks;
+    ++tiles;
   }
   __device__ __forceinline__ void add(int cell, float v) {
     const float y = v * scale, h = rintf(y);
@@ -773,7 +773,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
     const int32_t* __restrict__ order, const int32_t* __restrict__ first,
     float* __restrict__ dtable_part) {
-  constexpr int RT = part_rows<T>(), KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
+  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
   using Lds = DqLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -789,6 +789,13 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   const T* kbase = (const T*)a.k + (int64_t)t.x * a.k_row + kv * a.k_head;
   const T* vbase = (const T*)a.v + (int64_t)t.x * a.v_row + kv * a.v_head;
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
+  float* part = dtable_part + ((int64_t)head * a.n_tiles + tile) * a.buckets;
+  if (lone_key(keep, t.y)) {
+    for (int i = threadIdx.x; i < min(kAttnQ * NQ, t.y - t.z) * a.dim; i += NT)
+      dq[((int64_t)(t.x + t.z + i / a.dim) * a.heads + head) * a.dim + i % a.dim] = (T)0.0f;
+    for (int i = threadIdx.x; i < a.buckets; i += NT) part[i] = 0.0f;
+    return;
+  }
   Stage<T, DP, KS, NT, VEC> ks, vs;
   KeyInfo info;
   ks.init((int)a.k_row, a.dim);
@@ -824,7 +831,6 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   else
     for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
-  const bool lone = lone_key<RT>(keep, t.y);
   f32x16 minus_delta;
 #pragma unroll
   for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
@@ -853,53 +859,48 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) next_tile(k0);
   else for (int k0 = 0; k0 < t.y; k0 += KS, buf ^= 1) {
     next_tile(k0);
-#pragma unroll RT / 32
-    for (int r0 = RT * wk; r0 < RT * wk + RT && k0 + r0 < t.y; r0 += 32) {
-      const int kb = k0 + r0;
-      const int* kpos = L.kpos[buf] + r0;
-      f32x16 s;
-      if (keep || kb + 32 > t.y) {
-        load_rows(L.cap[buf] + r0, s);
-        row_product<T, DP>(L.k[buf], r0, qf, s);
-      } else {
-        s = f32x16{};
-        row_product<T, DP>(L.k[buf], r0, qf, s);
-      }
-      float x[16];
-      const int side = query_logits(a, s, ext, L.cap[buf] + r0, kpos, kb, qi, lse, x);
-      s = minus_delta;
-      row_product<T, DP>(L.v[buf], r0, gf, s);  // dP - delta
+    const int kb = k0 + RT * wk;
+    if (kb >= t.y) continue;
+    const T* kt = L.k[buf] + RT * wk * DP;
+    const float* cap = L.cap[buf] + RT * wk;
+    const int* kpos = L.kpos[buf] + RT * wk;
+    f32x16 s[N];
+    load_rows<N>(cap, s);
+    row_product<T, DP, N>(kt, qf, s);
+    float x[16 * N];
+    const int side = query_logits<N>(a, s, ext, cap, kpos, kb, qi, lse, x);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i];
-      if (lone) {
+    for (int n = 0; n < N; ++n) s[n] = minus_delta;
+    row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, s);  // dP - delta
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-      }
-      if (side) {
-        float sum[4] = {};
+    for (int i = 0; i < 16 * N; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i / 16][i % 16];
+    if (side) {
+      float sum[4] = {};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i % 4] += x[i];
-        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (side > 0)
-          far_hi += all;
-        else
-          far_lo += all;
-      } else if (!a.pos) {
-        add_diagonals(x, scratch, mine + (kb - qi.first + R + kAttnSpan));
-      } else {
-        float top = 0.0f;
+      for (int i = 0; i < 16 * N; ++i) sum[i % 4] += x[i];
+      const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (side > 0)
+        far_hi += all;
+      else
+        far_lo += all;
+    } else if (!a.pos) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
-        // NaN does not survive the maximum
+      for (int n = 0; n < N; ++n)
+        if (kb + 32 * n < t.y)
+          add_diagonals(x + 16 * n, scratch, mine + (kb + 32 * n - qi.first + R + kAttnSpan));
+    } else {
+      float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = x[i] != x[i] ? INFINITY : top;
-        ints.prepare(top);
+      for (int i = 0; i < 16 * N; ++i) top = fmaxf(top, fabsf(x[i]));
+      // NaN does not survive the maximum
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          ints.add(offset_cell(kpos[acc_row(i, g)], qi.pos, R) - kAttnSpan, x[i]);
-      }
-      column_product<T, DP>(L.k[buf], r0, x, acc);
+      for (int i = 0; i < 16 * N; ++i) top = x[i] != x[i] ? INFINITY : top;
+      ints.prepare(top);
+#pragma unroll
+      for (int i = 0; i < 16 * N; ++i)
+        ints.add(offset_cell(kpos[acc_row(i, g)], qi.pos, R) - kAttnSpan, x[i]);
     }
+    column_product<T, DP, N>(kt, x, acc);
   }
   if (a.pos) ints.flush();
   far_lo = mlcg_wave_sum(far_lo);
@@ -913,8 +914,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
     if (g == 0) delta_out[head * a.beads + row] = delta;
   }
-  flush_offsets<NT>(a, dd, cells, order, first,
-                    dtable_part + ((int64_t)head * a.n_tiles + tile) * a.buckets);
+  flush_offsets<NT>(a, dd, cells, order, first, part);
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -937,7 +937,7 @@ constexpr int dkv_waves() {
 template <typename T, int DP, int NQ, int NK, bool VEC>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
     AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
-  constexpr int RT = part_rows<T>(), KS = RT * NK, NT = 64 * NQ * NK;
+  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = DkvLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -951,6 +951,21 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
   const int kw = t.z + kAttnQ * wq, ki = kw + (lane & 31);
   const int64_t row = (int64_t)t.x + ki;
   const bool in = ki < t.y, k_ok = in && (!a.keep || a.keep[row]);
+  if (lone_key(a.keep ? a.keep + t.x : nullptr, t.y)) {
+    for (int i = threadIdx.x; i < min(kAttnQ * NQ, t.y - t.z) * a.dim; i += NT) {
+      const int64_t r = t.x + t.z + i / a.dim;
+      const int d = i % a.dim;
+      float sum = 0.0f;
+      if (!a.keep || a.keep[r])
+        for (int j = 0; j < t.y; ++j)
+          for (int h = 0; h < a.group; ++h)
+            sum += (float)((const T*)a.grad)[((int64_t)(t.x + j) * a.heads + kv * a.group + h) *
+                                                 a.dim + d];
+      dk[(r * kv_heads + kv) * a.dim + d] = (T)0.0f;
+      dv[(r * kv_heads + kv) * a.dim + d] = (T)sum;
+    }
+    return;
+  }
   // the sums of the logits begin with -lse / c, those of dP with -delta
   const float c = logit_factor(a);
   const int R = a.reach;
@@ -991,7 +1006,6 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     klo = wave_min(kp);
     khi = wave_max(kp);
   }
-  const bool lone = lone_key<RT>(a.keep ? a.keep + t.x : nullptr, t.y);
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
   int buf = 0;
@@ -1022,54 +1036,46 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
       for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) next_tile(h, q0);
     else for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
       next_tile(h, q0);
-#pragma unroll RT / 32
-      for (int r0 = RT * wk; r0 < RT * wk + RT && q0 + r0 < t.y; r0 += 32) {
-        const int qb = q0 + r0;
-        const int* qpos = L.qpos[buf] + r0;
-        f32x16 s;
-        load_rows(L.lse[buf] + r0, s);
-        row_product<T, DP>(L.q[buf], r0, kf, s);
-        float x[16];
-        int side;
-        if (a.pos) {
-          const int qp = qpos[lane & 31];
-          const bool past = qb + (lane & 31) >= t.y;
-          side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
-                 : __all(past || __builtin_elementwise_sub_sat(khi, qp) <= -R) ? -1
-                                                                               : 0;
-        } else {
-          side = block_side(kw - (qb + 31), kw + 31 - qb, R);
-        }
-        if (side) {
-          const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, b);
-        } else if (a.pos) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[i] = fmaf(s[i], c, ext[offset_cell(kp, qpos[acc_row(i, g)], R)]);
-        } else {
-          const float* e = ext + (ki - qb - 4 * g + R + kAttnSpan);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = fmaf(s[i], c, e[-acc_row(i, 0)]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
-        if (lone) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = k_ok && qb + acc_row(i, g) < t.y ? 1.0f : 0.0f;
-        }
-        column_product<T, DP>(L.g[buf], r0, x, dva);
-        load_rows(L.delta[buf] + r0, s);
-        row_product<T, DP>(L.g[buf], r0, vf, s);  // dP - delta
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= s[i];
-        if (lone) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-        }
-        column_product<T, DP>(L.q[buf], r0, x, dka);
+      const int qb = q0 + RT * wk;
+      if (qb >= t.y) continue;
+      const T* qt = L.q[buf] + RT * wk * DP;
+      const T* gt = L.g[buf] + RT * wk * DP;
+      const int* qpos = L.qpos[buf] + RT * wk;
+      f32x16 s[N];
+      load_rows<N>(L.lse[buf] + RT * wk, s);
+      row_product<T, DP, N>(qt, kf, s);
+      float x[16 * N];
+      int side;
+      if (a.pos) {
+        const int qp = qpos[lane % RT];
+        const bool past = qb + lane % RT >= t.y;
+        side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
+               : __all(past || __builtin_elementwise_sub_sat(khi, qp) <= -R) ? -1
+                                                                             : 0;
+      } else {
+        side = block_side(kw - (qb + RT - 1), kw + 31 - qb, R);
       }
+      if (side) {
+        const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+#pragma unroll
+        for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
+      } else if (a.pos) {
+#pragma unroll
+        for (int i = 0; i < 16 * N; ++i)
+          x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kp, qpos[acc_row(i, g)], R)]);
+      } else {
+        const float* e = ext + (ki - qb - 4 * g + R + kAttnSpan);
+#pragma unroll
+        for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, e[-acc_row(i, 0)]);
+      }
+      load_rows<N>(L.delta[buf] + RT * wk, s);
+      row_product<T, DP, N>(gt, vf, s);  // dP - delta
+#pragma unroll
+      for (int i = 0; i < 16 * N; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
+      column_product<T, DP, N>(gt, x, dva);
+#pragma unroll
+      for (int i = 0; i < 16 * N; ++i) x[i] *= s[i / 16][i % 16];
+      column_product<T, DP, N>(qt, x, dka);
     }
   }
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));

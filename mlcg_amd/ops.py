@@ -1923,7 +1923,7 @@ def _attention_heads(t: torch.Tensor, name: str, chains: ChainLayout, like: torc
     return t, (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
 
 
-def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions):
+def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, backward=False):
     require_device(q, k, v, table, keep, positions)
     dt = _chain_dtype(q, "chain_attention")
     _check(isinstance(chains, ChainLayout) and chains.device == q.device,
@@ -1956,16 +1956,23 @@ def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions):
                                                          f"{q.device}")
         positions = positions.contiguous()
     scale = dim ** -0.5 if scale is None else float(scale)
-    rows, splits = _attention_shape(chains, heads, dim)
+    rows, splits = _attention_shape(chains, heads, dim, backward)
     return (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table.contiguous(), scale, keep,
             positions, rows, splits)
 
 
-def _attention_shape(chains: ChainLayout, heads: int, dim: int) -> Tuple[int, int]:
+def _attention_shape(chains: ChainLayout, heads: int, dim: int, backward: bool
+                     ) -> Tuple[int, int]:
     """(beads of a tile, parts of the other side) of the attention kernels."""
     if chains.max_len <= 32:
         return 32, 1
-    return (64, 1) if chains.max_len <= 64 else (128, 1)
+    if chains.max_len <= 64:
+        return 64, 1
+    groups = chains.tiles[128].shape[0] * heads
+    long = chains.n_beads >= 400 * chains.n_chains
+    if dim <= 64 and long and (backward or groups < 1024):
+        return 128, 2
+    return 128, 1
 
 
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -2003,8 +2010,8 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     """(grad q, grad k, grad v, grad table) of chain_attention for the gradient
     of its output (mlcg_chain_attention_backward); out and lse are the
     forward's.  Every sum has a fixed order."""
-    (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
-     rows, splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
+    (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions, rows,
+     splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, True)
     dev = q.device
     for t, name, shape, dtype in ((out, "out", (n, heads, dim), q.dtype),
                                   (grad, "grad", (n, heads, dim), q.dtype),
