@@ -1065,25 +1065,27 @@ int mlcg_chain_attention_backward(
  * stride ld, y, grad_y and grad_x contiguous, width <= 1024.  stats
  * [3, chains, groups] is kept for the backward pass: the mean, what its
  * rounding left out, and 1 / sqrt(var + eps) (not written for a chain of
- * length 0).  `size`: the rows of the tiles in `tiles`, at most
- * mlcg_group_norm_slab_rows; first_tile [chains]: a chain's first tile, -1
- * for a chain of length 0.  grad_bias_weight [2, width]: the gradient of bias,
+ * length 0).  `tiles` have 256 rows; first_tile [chains]: a chain's first tile, -1
+ * for a chain of length 0; whole: the n_whole chains that have beads as one
+ * tile each, max_len the longest one's length.  grad_bias_weight [2, width]: the gradient of bias,
  * then of weight. */
-int mlcg_group_norm_slab_rows(int width, int dtype);
 int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t chains,
+                                         int64_t n_whole, int64_t max_len,
                                          int width, int groups, int backward);
 int mlcg_group_norm_act(const void* x, int64_t ld, int64_t rows, int dtype,
                         const void* weight, const void* bias, int width,
                         int groups, const int32_t* tiles,
-                        const int32_t* first_tile, int64_t n_tiles, int size,
+                        const int32_t* first_tile, int64_t n_tiles,
+                        const int32_t* whole, int64_t n_whole, int64_t max_len,
                         int64_t chains, float eps, int act, void* y,
                         float* stats, float* workspace,
                         int64_t workspace_floats, void* stream);
 int mlcg_group_norm_act_backward(
     const void* x, int64_t ld, const void* grad_y, int64_t rows, int dtype,
     const void* weight, const void* bias, int width, int groups,
-    const int32_t* tiles, const int32_t* first_tile, int64_t n_tiles, int size,
-    int64_t chains, int act, const float* stats, void* grad_x, void* grad_bias_weight, float* workspace,
+    const int32_t* tiles, const int32_t* first_tile, int64_t n_tiles,
+    const int32_t* whole, int64_t n_whole, int64_t max_len, int64_t chains,
+    int act, const float* stats, void* grad_x, void* grad_bias_weight, float* workspace,
     int64_t workspace_floats, void* stream);
 
 /* out[e] = residual[e] + (u16(e) >= threshold ? x[e] * 65536 /

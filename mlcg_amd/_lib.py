@@ -157,12 +157,10 @@ _SIGNATURES = {
     "mlcg_chain_attention_backward": [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P,
         _I32, _P, _P, _P, _I32, _F32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P,
         _P, _I64, _P],
-    "mlcg_group_norm_slab_rows": [_I32, _I32],
-    "mlcg_group_norm_workspace_floats": [_I64, _I64, _I32, _I32, _I32],
-    "mlcg_group_norm_act": [_P, _I64, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64, _I32, _I64,
-        _F32, _I32, _P, _P, _P, _I64, _P],
+    "mlcg_group_norm_workspace_floats": [_I64, _I64, _I64, _I64, _I32, _I32, _I32],
+    "mlcg_group_norm_act": [_P, _I64, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64, _P, _I64, _I64, _I64, _F32, _I32, _P, _P, _P, _I64, _P],
     "mlcg_group_norm_act_backward": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64,
-        _I32, _I64, _I32, _P, _P, _P, _P, _I64, _P],
+        _P, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P],
     "mlcg_dropout_add": [_P, _P, _I64, _I32, _I32, _U64, _P, _I64, _P, _P],
 }
 _RESTYPES = {"mlcg_version": _c.c_char_p, "mlcg_scan_workspace_ints": _I64,

@@ -8,24 +8,38 @@
 // chain's beads (summed over the chains: the gradients of b_c and w_c),
 //   dx = (dz w_c - sum_g w_c A_c / n - hat sum_g w_c B_c / n) / sqrt(var + eps).
 //
-// A workgroup holds a slab of a chain's rows in registers: its threads form
-// TR rows x TC columns, a column one vector of W channels, and every thread
-// has the rows tr, tr + TR, ... of its column.  The mean and the sum of
-// squared deviations from it are two passes over the registers, so neither
-// is formed from a difference of large sums; the second pass also gives what
-// the rounding of the mean left out, which is kept beside it (a deviation of a
-// value far from zero is then as exact as the value).  Slabs of one chain are
-// joined from theirs in slab order; every sum has a fixed order.
+// A workgroup's threads form TR rows x TC columns, a column one vector of W
+// channels (16 bytes), and go down a chain or a slab of it NV rows of a thread
+// at a time, with all loads of such a step in flight.
+//
+// Statistics: the mean of the first step's values, rounded, is the pivot p;
+// s = sum (x - p) and q = sum (x - p)^2 give mean = p + s / n and var =
+// (q - s^2 / n) / n.  As p is the mean of n1 of the n values, (p - mean)^2 <=
+// var n / n1: the difference loses a factor of 1 + n / n1 at most (for a
+// chain of one step nothing).  What the rounding of the mean leaves out is
+// kept beside it, so that a deviation of a value far from zero is as exact as
+// the value.  Every sum has a fixed order.
+//
+// Chains of up to kOneRows beads, or many chains: a workgroup takes a whole
+// chain, twice over its rows, the second time from the cache; one launch
+// forward, and backward one that writes dx and each workgroup's sums by
+// channel over the chains it takes, and one that joins these.  Few long
+// chains: slabs of them, joined in slab order, then a second reading.
+#include <algorithm>
+
 #include "chain.h"
 
 namespace {
 
 constexpr int kMaxWidth = 1024;
+constexpr int kSlabRows = 256;
+constexpr int kNV = 4;
 
 struct NormShape {
   const int4* tiles;  // (chain's first row, chain's length, slab's first row in it, chain)
   int n_tiles, size;  // slabs, and rows of a slab
-  int C, G, TC, TR, cols, per;  // cols columns of sums, per of them a group
+  int C, G, TC, TR;
+  int64_t chains;
 };
 
 __device__ __forceinline__ void act_z(int act, float z, float& y, float& d) {
@@ -42,6 +56,12 @@ __device__ __forceinline__ void act_z(int act, float z, float& y, float& d) {
   }
 }
 
+__device__ __forceinline__ float act_value(int act, float z) {
+  if (act == MLCG_ACT_NONE) return z;
+  if (act == MLCG_ACT_SILU) return z * mlcg_sigmoid(z);
+  return mlcg_act_value(act, z);
+}
+
 template <typename T, int W>
 struct Vec {
   typedef T type __attribute__((ext_vector_type(W)));
@@ -55,9 +75,35 @@ struct Vec<T, 1> {
   };
 };
 
+// A thread's place among the rows and columns of a workgroup.
+struct Place {
+  int row, col;
+  bool in;
+  __device__ __forceinline__ Place(const NormShape& sh)
+      : row(threadIdx.x / sh.TC), col(threadIdx.x % sh.TC), in(row < sh.TR) {}
+};
+
+// the rows r0 + row + v TR, v < NV, of a column; those at or past `rows` are
+// loaded as the last one
+template <typename T, int W>
+__device__ __forceinline__ void load_step(const NormShape& sh, const Place& at, const T* x,
+                                          int64_t ld, int r0, int rows,
+                                          typename Vec<T, W>::type (&out)[kNV]) {
+#pragma unroll
+  for (int v = 0; v < kNV; ++v) {
+    const int r = min(r0 + at.row + v * sh.TR, rows - 1);
+    out[v] = *reinterpret_cast<const typename Vec<T, W>::type*>(x + r * ld + at.col * W);
+  }
+}
+
+__device__ __forceinline__ bool step_row(const NormShape& sh, const Place& at, int r0, int v,
+                                         int rows) {
+  return at.in && r0 + at.row + v * sh.TR < rows;
+}
+
 // Sums of K values a thread over the rows of its column: the rows that lie
-// in one wave by a butterfly (TC divides 64), the rest through LDS.  sums[c]
-// for c < TC K, valid for every thread on return.
+// in one wave by a butterfly (TC divides 64), the rest through LDS.
+// sums[col K + k], valid for every thread on return.
 template <int K>
 __device__ void column_sums(const NormShape& sh, const float (&v)[K], float* red, float* sums) {
   const int tid = threadIdx.x, nt = blockDim.x;
@@ -89,136 +135,92 @@ __device__ void column_sums(const NormShape& sh, const float (&v)[K], float* red
   __syncthreads();
 }
 
-// out[g] = f times the sum of the group's `per` columns of in, a wave a group.
-__device__ void group_sums(const float* in, int groups, int per, float* out, float f = 1.0f) {
+// a = the sum of the group's columns' first (of two, second) values, a wave a
+// group: f(group, a, b) on its first lane.
+template <typename F>
+__device__ __forceinline__ void group_sums(const float* sums, int groups, int per, int values,
+                                           F f) {
   const int lane = threadIdx.x & 63;
   for (int g = threadIdx.x >> 6; g < groups; g += blockDim.x >> 6) {
-    float t = 0.0f;
-    for (int c = lane; c < per; c += 64) t += in[g * per + c];
-    t = mlcg_wave_sum(t);
-    if (lane == 0) out[g] = t * f;
+    float a = 0.0f, b = 0.0f;
+    for (int c = lane; c < per; c += 64) {
+      a += sums[values * (g * per + c)];
+      if (values > 1) b += sums[values * (g * per + c) + 1];
+    }
+    a = mlcg_wave_sum(a);
+    if (values > 1) b = mlcg_wave_sum(b);
+    if (lane == 0) f(g, a, b);
   }
   __syncthreads();
 }
 
-template <typename T, int W, int NV>
-__device__ __forceinline__ void load_slab(const NormShape& sh, const T* x, int64_t ld,
-                                          int64_t first, int rows, int row, int col,
-                                          typename Vec<T, W>::type (&out)[NV]) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int r = row + v * sh.TR;
-    if (row < sh.TR && r < rows)
-      out[v] = *reinterpret_cast<const typename Vec<T, W>::type*>(x + (first + r) * ld + col * W);
-    else
-      out[v] = typename Vec<T, W>::type{};
-  }
-}
-
-// (mean, its remainder, M2) of every group of a slab -> part[g][tile]
-template <typename T, int W, int NV, bool GROUPED>
-__global__ __launch_bounds__(1024) void norm_part_kernel(NormShape sh, const T* __restrict__ x,
-                                                         int64_t ld, float4* __restrict__ part) {
-  extern __shared__ float lds[];
-  float* red = lds;                                  // blockDim * W
-  float* sums = red + blockDim.x * W;                // C
-  float* mean = sums + sh.C;                         // G
-  float* rest = mean + sh.G;                         // G
-  float* m2 = rest + sh.G;                           // G
-  const int4 t = sh.tiles[blockIdx.x];
-  const int rows = min(sh.size, t.y - t.z);
-  const int col = threadIdx.x % sh.TC, row = threadIdx.x / sh.TC;
-  typename Vec<T, W>::type xv[NV];
-  load_slab<T, W, NV>(sh, x, ld, (int64_t)t.x + t.z, rows, row, col, xv);
+// The statistics of `rows` rows from x on, by group, into LDS: the mean, its
+// remainder and the sum of squared deviations.  GROUPED: a vector lies in one
+// group, and its values are summed first.
+template <typename T, int W, bool GROUPED>
+__device__ __forceinline__ void row_stats(const NormShape& sh, const Place& at, const T* x,
+                                          int64_t ld, int rows, float* lds, float* mean,
+                                          float* rest, float* m2) {
   constexpr int K = GROUPED ? 1 : W;
-  const float inv = 1.0f / ((float)rows * (float)(sh.C / sh.G));
+  float* red = lds;                         // blockDim 2 K
+  float* sums = red + blockDim.x * 2 * K;   // TC 2 K
+  const int P = sh.C / sh.G, per = GROUPED ? P / W : P;
+  typename Vec<T, W>::type xv[kNV];
+  load_step<T, W>(sh, at, x, ld, 0, rows, xv);
   float s[K] = {};
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < kNV; ++v)
+    if (step_row(sh, at, 0, v, rows))
 #pragma unroll
-    for (int j = 0; j < W; ++j) s[GROUPED ? 0 : j] += (float)xv[v][j];
+      for (int j = 0; j < W; ++j) s[GROUPED ? 0 : j] += (float)xv[v][j];
   column_sums<K>(sh, s, red, sums);
-  // the mean comes back from LDS: rounded, as it is kept
-  group_sums(sums, sh.G, sh.per, mean, inv);
-  float mu[W];
+  const float first = 1.0f / ((float)min(rows, kNV * sh.TR) * (float)P);
+  // the pivot comes back from LDS: rounded, as it is used
+  group_sums(sums, sh.G, per, 1, [&](int g, float a, float) { mean[g] = a * first; });
+  float p[W], d2[2 * K] = {};
 #pragma unroll
-  for (int j = 0; j < W; ++j) mu[j] = mean[(col * W + j) / (sh.C / sh.G)];
-  float c[K] = {};
+  for (int j = 0; j < W; ++j) p[j] = mean[(at.col * W + j) / P];
+  for (int r0 = 0;;) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) s[k] = 0.0f;
+    for (int v = 0; v < kNV; ++v) {
+      const bool ok = step_row(sh, at, r0, v, rows);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const bool ok = row < sh.TR && row + v * sh.TR < rows;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float d = ok ? (float)xv[v][j] - mu[j] : 0.0f;
-      c[GROUPED ? 0 : j] += d;
-      s[GROUPED ? 0 : j] = fmaf(d, d, s[GROUPED ? 0 : j]);
+      for (int j = 0; j < W; ++j) {
+        const float d = ok ? (float)xv[v][j] - p[j] : 0.0f;
+        const int k = GROUPED ? 0 : j;
+        d2[2 * k] += d;
+        d2[2 * k + 1] = fmaf(d, d, d2[2 * k + 1]);
+      }
     }
+    r0 += kNV * sh.TR;
+    if (r0 >= rows) break;
+    load_step<T, W>(sh, at, x, ld, r0, rows, xv);
   }
-  column_sums<K>(sh, c, red, sums);
-  group_sums(sums, sh.G, sh.per, rest);
-  column_sums<K>(sh, s, red, sums);
-  group_sums(sums, sh.G, sh.per, m2);
-  for (int g = threadIdx.x; g < sh.G; g += blockDim.x) {
-    const float lo = rest[g] * inv;
-    part[(int64_t)g * sh.n_tiles + blockIdx.x] =
-        make_float4(mean[g], lo, fmaxf(0.0f, m2[g] - lo * rest[g]), 0.0f);
-  }
-}
-
-// A chain's statistics from its slabs': with n_t values of mean m_t and sum of
-// squares M_t,  mean = sum n_t m_t / n  and  M = sum M_t + n_t (m_t - mean)^2.
-// stats: the mean, its remainder and 1 / sqrt(var + eps), [3][chains][G].
-__global__ __launch_bounds__(256) void norm_join_kernel(NormShape sh,
-                                                        const int32_t* __restrict__ first_tile,
-                                                        const float4* __restrict__ part,
-                                                        float eps, float* __restrict__ stats) {
-  const int chain = blockIdx.x, g = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int t0 = first_tile[chain];
-  if (g >= sh.G || t0 < 0) return;  // an empty chain has no slab and no statistics
-  const int len = sh.tiles[t0].y;
-  const int count = (len + sh.size - 1) / sh.size;
-  const float4* p = part + (int64_t)g * sh.n_tiles + t0;
-  const float n = (float)len;
-  float s = 0.0f;
-  for (int t = lane; t < count; t += 64)
-    s = fmaf((float)min(sh.size, len - t * sh.size), p[t].x, s);
-  const float mu = mlcg_wave_sum(s) / n;
-  float c = 0.0f;
-  for (int t = lane; t < count; t += 64)
-    c = fmaf((float)min(sh.size, len - t * sh.size), (p[t].x - mu) + p[t].y, c);
-  const float lo = mlcg_wave_sum(c) / n;
-  const float P = (float)(sh.C / sh.G);
-  float m2 = 0.0f;
-  for (int t = lane; t < count; t += 64) {
-    const float d = (p[t].x - mu) + (p[t].y - lo);
-    m2 += fmaf((float)min(sh.size, len - t * sh.size) * P * d, d, p[t].z);
-  }
-  m2 = mlcg_wave_sum(m2);
-  if (lane == 0) {
-    const int64_t at = (int64_t)chain * sh.G + g, all = (int64_t)gridDim.x * sh.G;
-    stats[at] = mu;
-    stats[all + at] = lo;
-    stats[2 * all + at] = 1.0f / sqrtf(m2 / (n * P) + eps);
-  }
+  column_sums<2 * K>(sh, d2, red, sums);
+  const float inv = 1.0f / ((float)rows * (float)P);
+  group_sums(sums, sh.G, per, 2, [&](int g, float a, float q) {
+    const float pivot = mean[g], step = a * inv;
+    float hi = pivot + step;
+    asm("" : "+v"(hi));  // the rounded sum, as it is kept
+    mean[g] = hi;
+    rest[g] = (pivot - hi) + step;
+    m2[g] = fmaxf(0.0f, q - step * a);
+  });
 }
 
 // What the elementwise passes need of a thread's channels.
 template <typename T, int W>
 struct Channels {
   float mu[W], lo[W], rs[W], w[W], b[W];
-  __device__ __forceinline__ Channels(const NormShape& sh, const float* stats, int64_t chain,
-                                      int64_t chains, int col, const T* weight, const T* bias) {
-    const int P = sh.C / sh.G;
-    const int64_t all = chains * sh.G;
+  __device__ __forceinline__ Channels(int P, const Place& at, const float* mean,
+                                      const float* rest, const float* rstd, const T* weight,
+                                      const T* bias) {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      const int c = col * W + j;
-      const int64_t at = chain * sh.G + c / P;
-      mu[j] = stats[at];
-      lo[j] = stats[all + at];
-      rs[j] = stats[2 * all + at];
+      const int c = at.col * W + j;
+      mu[j] = mean[c / P];
+      lo[j] = rest[c / P];
+      rs[j] = rstd[c / P];
       w[j] = (float)weight[c];
       b[j] = (float)bias[c];
     }
@@ -229,26 +231,244 @@ struct Channels {
 };
 
 template <typename T, int W>
+__device__ __forceinline__ void apply_rows(const NormShape& sh, const Place& at,
+                                           const Channels<T, W>& ch, const T* x, int64_t ld,
+                                           int rows, int act, T* y) {
+  for (int r0 = 0; r0 < rows; r0 += kNV * sh.TR) {
+    typename Vec<T, W>::type xv[kNV];
+    load_step<T, W>(sh, at, x, ld, r0, rows, xv);
+#pragma unroll
+    for (int v = 0; v < kNV; ++v) {
+      typename Vec<T, W>::type out;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        out[j] = (T)act_value(act, fmaf(ch.hat(j, (float)xv[v][j]), ch.w[j], ch.b[j]));
+      if (step_row(sh, at, r0, v, rows))
+        *reinterpret_cast<typename Vec<T, W>::type*>(
+            y + (int64_t)(r0 + at.row + v * sh.TR) * sh.C + at.col * W) = out;
+    }
+  }
+}
+
+// One chain a workgroup.
+template <typename T, int W, bool GROUPED>
+__global__ __launch_bounds__(1024) void norm_chain_kernel(NormShape sh, const T* __restrict__ x,
+                                                          int64_t ld, const T* __restrict__ w,
+                                                          const T* __restrict__ b, float eps,
+                                                          int act, T* __restrict__ y,
+                                                          float* __restrict__ stats) {
+  extern __shared__ float lds[];
+  float* mean = lds;  // G each
+  float* rest = mean + sh.G;
+  float* rstd = rest + sh.G;
+  const int4 t = sh.tiles[blockIdx.x];
+  const Place at(sh);
+  const int P = sh.C / sh.G;
+  const T* xt = x + (int64_t)t.x * ld;
+  row_stats<T, W, GROUPED>(sh, at, xt, ld, t.y, rstd + sh.G, mean, rest, rstd);
+  const float inv = 1.0f / ((float)t.y * (float)P);
+  for (int g = threadIdx.x; g < sh.G; g += blockDim.x) {
+    const float rs = 1.0f / sqrtf(rstd[g] * inv + eps);
+    rstd[g] = rs;
+    const int64_t k = (int64_t)t.w * sh.G + g, all = sh.chains * sh.G;
+    stats[k] = mean[g];
+    stats[all + k] = rest[g];
+    stats[2 * all + k] = rs;
+  }
+  __syncthreads();
+  const Channels<T, W> ch(P, at, mean, rest, rstd, w, b);
+  apply_rows<T, W>(sh, at, ch, xt, ld, t.y, act, y + (int64_t)t.x * sh.C);
+}
+
+// (mean, its remainder, M2) of every group of a slab -> part[g][tile]
+template <typename T, int W, bool GROUPED>
+__global__ __launch_bounds__(1024) void norm_part_kernel(NormShape sh, const T* __restrict__ x,
+                                                         int64_t ld, float4* __restrict__ part) {
+  extern __shared__ float lds[];
+  float* mean = lds;  // G each
+  float* rest = mean + sh.G;
+  float* m2 = rest + sh.G;
+  const int4 t = sh.tiles[blockIdx.x];
+  const Place at(sh);
+  row_stats<T, W, GROUPED>(sh, at, x + ((int64_t)t.x + t.z) * ld, ld, min(sh.size, t.y - t.z),
+                           m2 + sh.G, mean, rest, m2);
+  for (int g = threadIdx.x; g < sh.G; g += blockDim.x)
+    part[(int64_t)g * sh.n_tiles + blockIdx.x] = make_float4(mean[g], rest[g], m2[g], 0.0f);
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = mlcg_wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// A chain's statistics from its slabs', a workgroup a group: with n_t values of
+// mean m_t and sum of squares M_t,  mean = sum n_t m_t / n  and  M = sum M_t +
+// n_t (m_t - mean)^2.  stats: the mean, its remainder and 1 / sqrt(var + eps),
+// [3][chains][G].
+__global__ __launch_bounds__(256) void norm_join_kernel(NormShape sh,
+                                                        const int32_t* __restrict__ first_tile,
+                                                        const float4* __restrict__ part,
+                                                        float eps, float* __restrict__ stats) {
+  __shared__ float red[4];
+  const int chain = blockIdx.x, g = blockIdx.y;
+  const int t0 = first_tile[chain];
+  if (t0 < 0) return;  // an empty chain has no slab and no statistics
+  const int len = sh.tiles[t0].y;
+  const int count = (len + sh.size - 1) / sh.size;
+  const float4* p = part + (int64_t)g * sh.n_tiles + t0;
+  const float n = (float)len;
+  float s = 0.0f;
+  for (int t = threadIdx.x; t < count; t += 256)
+    s = fmaf((float)min(sh.size, len - t * sh.size), p[t].x, s);
+  const float mu = block_sum(s, red) / n;
+  float c = 0.0f;
+  for (int t = threadIdx.x; t < count; t += 256)
+    c = fmaf((float)min(sh.size, len - t * sh.size), (p[t].x - mu) + p[t].y, c);
+  const float lo = block_sum(c, red) / n;
+  const float P = (float)(sh.C / sh.G);
+  float m2 = 0.0f;
+  for (int t = threadIdx.x; t < count; t += 256) {
+    const float d = (p[t].x - mu) + (p[t].y - lo);
+    m2 += fmaf((float)min(sh.size, len - t * sh.size) * P * d, d, p[t].z);
+  }
+  m2 = block_sum(m2, red);
+  if (threadIdx.x == 0) {
+    const int64_t at = (int64_t)chain * sh.G + g, all = sh.chains * sh.G;
+    stats[at] = mu;
+    stats[all + at] = lo;
+    stats[2 * all + at] = 1.0f / sqrtf(m2 / (n * P) + eps);
+  }
+}
+
+template <typename T, int W>
 __global__ __launch_bounds__(1024) void norm_apply_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ w,
-    const T* __restrict__ b, const float* __restrict__ stats, int64_t chains, int act,
-    T* __restrict__ y) {
+    const T* __restrict__ b, const float* __restrict__ stats, int act, T* __restrict__ y) {
   const int4 t = sh.tiles[blockIdx.x];
-  const int rows = min(sh.size, t.y - t.z);
-  const int col = threadIdx.x % sh.TC, row = threadIdx.x / sh.TC;
-  if (row >= sh.TR) return;
-  const Channels<T, W> ch(sh, stats, t.w, chains, col, w, b);
-  for (int r = row; r < rows; r += sh.TR) {
-    const int64_t at = (int64_t)t.x + t.z + r;
-    const auto xv = *reinterpret_cast<const typename Vec<T, W>::type*>(x + at * ld + col * W);
-    typename Vec<T, W>::type out;
+  const Place at(sh);
+  if (!at.in) return;
+  const float* st = stats + (int64_t)t.w * sh.G;
+  const int64_t all = sh.chains * sh.G;
+  const Channels<T, W> ch(sh.C / sh.G, at, st, st + all, st + 2 * all, w, b);
+  const int64_t first = (int64_t)t.x + t.z;
+  apply_rows<T, W>(sh, at, ch, x + first * ld, ld, min(sh.size, t.y - t.z), act,
+                   y + first * sh.C);
+}
+
+// ---------------------------------------------------------------------------
+// Backward
+
+// (A_c, B_c) of rows from x, dy on -> sums[2 c], sums[2 c + 1]
+template <typename T, int W>
+__device__ __forceinline__ void row_grads(const NormShape& sh, const Place& at,
+                                          const Channels<T, W>& ch, const T* x, int64_t ld,
+                                          const T* dy, int rows, int act, float* red,
+                                          float* sums) {
+  float ab[2 * W] = {};
+  for (int r0 = 0; r0 < rows; r0 += kNV * sh.TR) {
+    typename Vec<T, W>::type xv[kNV], gv[kNV];
+    load_step<T, W>(sh, at, x, ld, r0, rows, xv);
+    load_step<T, W>(sh, at, dy, sh.C, r0, rows, gv);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float yv, d;
-      act_z(act, fmaf(ch.hat(j, (float)xv[j]), ch.w[j], ch.b[j]), yv, d);
-      out[j] = (T)yv;
+    for (int v = 0; v < kNV; ++v) {
+      const bool ok = step_row(sh, at, r0, v, rows);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float hat = ch.hat(j, (float)xv[v][j]);
+        float yv, d;
+        act_z(act, fmaf(hat, ch.w[j], ch.b[j]), yv, d);
+        const float dz = ok ? (float)gv[v][j] * d : 0.0f;
+        ab[2 * j] += dz;
+        ab[2 * j + 1] = fmaf(dz, hat, ab[2 * j + 1]);
+      }
     }
-    *reinterpret_cast<typename Vec<T, W>::type*>(y + at * sh.C + col * W) = out;
+  }
+  column_sums<2 * W>(sh, ab, red, sums);
+}
+
+// dx of rows from x, dy on, with the groups' sums of w A and w B
+template <typename T, int W>
+__device__ __forceinline__ void row_dx(const NormShape& sh, const Place& at,
+                                       const Channels<T, W>& ch, const T* x, int64_t ld,
+                                       const T* dy, int rows, int act, const float* s1,
+                                       const float* s2, float inv, T* dx) {
+  const int P = sh.C / sh.G;
+  float m1[W], m2[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    m1[j] = s1[(at.col * W + j) / P] * inv;
+    m2[j] = s2[(at.col * W + j) / P] * inv;
+  }
+  for (int r0 = 0; r0 < rows; r0 += kNV * sh.TR) {
+    typename Vec<T, W>::type xv[kNV], gv[kNV];
+    load_step<T, W>(sh, at, x, ld, r0, rows, xv);
+    load_step<T, W>(sh, at, dy, sh.C, r0, rows, gv);
+#pragma unroll
+    for (int v = 0; v < kNV; ++v) {
+      typename Vec<T, W>::type out;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float hat = ch.hat(j, (float)xv[v][j]);
+        float yv, d;
+        act_z(act, fmaf(hat, ch.w[j], ch.b[j]), yv, d);
+        // rounded as in the sums, not fused with the difference: the gradient
+        // of a group of one value is then 0, not its rounding error times up
+        // to 1 / sqrt(eps)
+        float dh = (float)gv[v][j] * d * ch.w[j];
+        asm("" : "+v"(dh));
+        out[j] = (T)((dh - m1[j] - hat * m2[j]) * ch.rs[j]);
+      }
+      if (step_row(sh, at, r0, v, rows))
+        *reinterpret_cast<typename Vec<T, W>::type*>(
+            dx + (int64_t)(r0 + at.row + v * sh.TR) * sh.C + at.col * W) = out;
+    }
+  }
+}
+
+// dx of the chains blockIdx.x, blockIdx.x + gridDim.x, ... and the sums of A_c
+// and B_c over them -> part[workgroup][2][C]
+template <typename T, int W>
+__global__ __launch_bounds__(1024) void norm_chain_bwd_kernel(
+    NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
+    const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats, int act,
+    T* __restrict__ dx, float* __restrict__ part) {
+  extern __shared__ float lds[];
+  float* red = lds;                        // blockDim 2 W
+  float* sums = red + blockDim.x * 2 * W;  // 2 C: (A, B) by channel
+  float* total = sums + 2 * sh.C;          // 2 C
+  float* s1 = total + 2 * sh.C;            // G each
+  float* s2 = s1 + sh.G;
+  const Place at(sh);
+  const int P = sh.C / sh.G;
+  const int64_t all = sh.chains * sh.G;
+  for (int c = threadIdx.x; c < 2 * sh.C; c += blockDim.x) total[c] = 0.0f;
+  for (int tile = blockIdx.x; tile < sh.n_tiles; tile += gridDim.x) {
+    const int4 t = sh.tiles[tile];
+    const float* st = stats + (int64_t)t.w * sh.G;
+    const Channels<T, W> ch(P, at, st, st + all, st + 2 * all, w, b);
+    const T* xt = x + (int64_t)t.x * ld;
+    const T* dt = dy + (int64_t)t.x * sh.C;
+    row_grads<T, W>(sh, at, ch, xt, ld, dt, t.y, act, red, sums);
+    for (int c = threadIdx.x; c < 2 * sh.C; c += blockDim.x) {
+      const float a = sums[c];
+      total[c] += a;
+      sums[c] = (float)w[c >> 1] * a;
+    }
+    __syncthreads();
+    group_sums(sums, sh.G, P, 2, [&](int g, float a, float q) {
+      s1[g] = a;
+      s2[g] = q;
+    });
+    row_dx<T, W>(sh, at, ch, xt, ld, dt, t.y, act, s1, s2, 1.0f / ((float)t.y * (float)P),
+                 dx + (int64_t)t.x * sh.C);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < sh.C; c += blockDim.x) {
+    part[(int64_t)blockIdx.x * 2 * sh.C + c] = total[2 * c];
+    part[(int64_t)blockIdx.x * 2 * sh.C + sh.C + c] = total[2 * c + 1];
   }
 }
 
@@ -256,50 +476,34 @@ __global__ __launch_bounds__(1024) void norm_apply_kernel(
 template <typename T, int W>
 __global__ __launch_bounds__(1024) void norm_bwd_part_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
-    const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats,
-    int64_t chains, int act, float* __restrict__ part) {
+    const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats, int act,
+    float* __restrict__ part) {
   extern __shared__ float lds[];
-  float* red = lds;                    // blockDim * W
-  float* sums = red + blockDim.x * W;  // C
+  float* red = lds;                        // blockDim 2 W
+  float* sums = red + blockDim.x * 2 * W;  // 2 C
   const int4 t = sh.tiles[blockIdx.x];
-  const int rows = min(sh.size, t.y - t.z);
-  const int col = threadIdx.x % sh.TC, row = threadIdx.x / sh.TC;
-  float A[W] = {}, B[W] = {};
-  const Channels<T, W> ch(sh, stats, t.w, chains, col, w, b);
-  if (row < sh.TR) {
-    for (int r = row; r < rows; r += sh.TR) {
-      const int64_t at = (int64_t)t.x + t.z + r;
-      const auto xv = *reinterpret_cast<const typename Vec<T, W>::type*>(x + at * ld + col * W);
-      const auto gv = *reinterpret_cast<const typename Vec<T, W>::type*>(dy + at * sh.C + col * W);
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const float hat = ch.hat(j, (float)xv[j]);
-        float yv, d;
-        act_z(act, fmaf(hat, ch.w[j], ch.b[j]), yv, d);
-        const float dz = (float)gv[j] * d;
-        A[j] += dz;
-        B[j] = fmaf(dz, hat, B[j]);
-      }
-    }
+  const Place at(sh);
+  const int64_t all = sh.chains * sh.G, first = (int64_t)t.x + t.z;
+  const float* st = stats + (int64_t)t.w * sh.G;
+  const Channels<T, W> ch(sh.C / sh.G, at, st, st + all, st + 2 * all, w, b);
+  row_grads<T, W>(sh, at, ch, x + first * ld, ld, dy + first * sh.C, min(sh.size, t.y - t.z), act,
+                  red, sums);
+  for (int c = threadIdx.x; c < sh.C; c += blockDim.x) {
+    part[(int64_t)blockIdx.x * 2 * sh.C + c] = sums[2 * c];
+    part[(int64_t)blockIdx.x * 2 * sh.C + sh.C + c] = sums[2 * c + 1];
   }
-  column_sums<W>(sh, A, red, sums);
-  for (int c = threadIdx.x; c < sh.C; c += blockDim.x)
-    part[(int64_t)blockIdx.x * 2 * sh.C + c] = sums[c];
-  column_sums<W>(sh, B, red, sums);
-  for (int c = threadIdx.x; c < sh.C; c += blockDim.x)
-    part[(int64_t)blockIdx.x * 2 * sh.C + sh.C + c] = sums[c];
 }
 
 // out[seg][col] = sum over the segment's rows of in[row][col], `cols` columns:
-// 32 columns x 32 slices of the rows a workgroup, the slices joined in order.
+// 8 columns x 128 slices of the rows a workgroup, the slices joined in order.
 // Segments are the slabs of a chain (first_tile, tiles), or all `rows` rows.
 template <typename O>
 __global__ __launch_bounds__(1024) void norm_rows_kernel(const float* __restrict__ in, int cols,
                                                          const int32_t* __restrict__ first_tile,
                                                          const int4* __restrict__ tiles, int size,
                                                          int rows, O* __restrict__ out) {
-  __shared__ float red[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  __shared__ float red[128][9];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3;
   int64_t r0 = 0;
   int n = rows;
   if (first_tile) {
@@ -308,15 +512,21 @@ __global__ __launch_bounds__(1024) void norm_rows_kernel(const float* __restrict
     n = t0 < 0 ? 0 : (tiles[t0].y + size - 1) / size;
   }
   float s = 0.0f;
-  if (col < cols)
-    for (int r = slice; r < n; r += 32) s += in[(r0 + r) * cols + col];
-  red[slice][threadIdx.x & 31] = s;
+  if (col < cols) {
+#pragma unroll 8
+    for (int r = slice; r < n; r += 128) s += in[(r0 + r) * cols + col];
+  }
+  red[slice][threadIdx.x & 7] = s;
   __syncthreads();
-  if (slice == 0 && col < cols) {
+  if (threadIdx.x < 64) {  // 8 lanes a column: 16 slices each, then a butterfly
+    const int c = threadIdx.x & 7;
     float t = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) t += red[k][threadIdx.x];
-    out[(int64_t)blockIdx.y * cols + col] = (O)t;
+    for (int k = 0; k < 16; ++k) t += red[(threadIdx.x >> 3) * 16 + k][c];
+    t += __shfl_xor(t, 8, 64);
+    t += __shfl_xor(t, 16, 64);
+    t += __shfl_xor(t, 32, 64);
+    if (threadIdx.x < 8 && col < cols) out[(int64_t)blockIdx.y * cols + col] = (O)t;
   }
 }
 
@@ -324,216 +534,214 @@ template <typename T, int W>
 __global__ __launch_bounds__(1024) void norm_bwd_apply_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
     const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats,
-    int64_t chains, const float* __restrict__ chain_sums, int act, T* __restrict__ dx) {
+    const float* __restrict__ chain_sums, int act, T* __restrict__ dx) {
   extern __shared__ float lds[];
-  float* wa = lds;          // C: w_c A_c, then w_c B_c
-  float* s1 = wa + sh.C;    // G
-  float* s2 = s1 + sh.G;    // G
+  float* wa = lds;              // 2 C: (w A, w B) by channel
+  float* s1 = wa + 2 * sh.C;    // G each
+  float* s2 = s1 + sh.G;
   const int4 t = sh.tiles[blockIdx.x];
-  const int rows = min(sh.size, t.y - t.z);
-  const int col = threadIdx.x % sh.TC, row = threadIdx.x / sh.TC;
+  const Place at(sh);
   const int P = sh.C / sh.G;
-  for (int k = 0; k < 2; ++k) {
-    const float* a = chain_sums + ((int64_t)t.w * 2 + k) * sh.C;
-    for (int c = threadIdx.x; c < sh.C; c += blockDim.x) wa[c] = (float)w[c] * a[c];
-    __syncthreads();
-    group_sums(wa, sh.G, P, k == 0 ? s1 : s2);
+  const float* a = chain_sums + (int64_t)t.w * 2 * sh.C;
+  for (int c = threadIdx.x; c < sh.C; c += blockDim.x) {
+    wa[2 * c] = (float)w[c] * a[c];
+    wa[2 * c + 1] = (float)w[c] * a[sh.C + c];
   }
-  if (row >= sh.TR) return;
-  const float inv = 1.0f / ((float)t.y * (float)P);
-  const Channels<T, W> ch(sh, stats, t.w, chains, col, w, b);
-  float m1[W], m2[W];
-#pragma unroll
-  for (int j = 0; j < W; ++j) {
-    m1[j] = s1[(col * W + j) / P] * inv;
-    m2[j] = s2[(col * W + j) / P] * inv;
-  }
-  for (int r = row; r < rows; r += sh.TR) {
-    const int64_t at = (int64_t)t.x + t.z + r;
-    const auto xv = *reinterpret_cast<const typename Vec<T, W>::type*>(x + at * ld + col * W);
-    const auto gv = *reinterpret_cast<const typename Vec<T, W>::type*>(dy + at * sh.C + col * W);
-    typename Vec<T, W>::type out;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float hat = ch.hat(j, (float)xv[j]);
-      float yv, d;
-      act_z(act, fmaf(hat, ch.w[j], ch.b[j]), yv, d);
-      // rounded as in the sums, not fused with the difference: the gradient of a
-      // group of one value is then 0, not its rounding error times up to 1 / sqrt(eps)
-      float dh = (float)gv[j] * d * ch.w[j];
-      asm("" : "+v"(dh));
-      out[j] = (T)((dh - m1[j] - hat * m2[j]) * ch.rs[j]);
-    }
-    *reinterpret_cast<typename Vec<T, W>::type*>(dx + at * sh.C + col * W) = out;
-  }
+  __syncthreads();
+  group_sums(wa, sh.G, P, 2, [&](int g, float p, float q) {
+    s1[g] = p;
+    s2[g] = q;
+  });
+  const int64_t all = sh.chains * sh.G, first = (int64_t)t.x + t.z;
+  const float* st = stats + (int64_t)t.w * sh.G;
+  const Channels<T, W> ch(P, at, st, st + all, st + 2 * all, w, b);
+  row_dx<T, W>(sh, at, ch, x + first * ld, ld, dy + first * sh.C, min(sh.size, t.y - t.z), act, s1,
+               s2, 1.0f / ((float)t.y * (float)P), dx + first * sh.C);
 }
 
-constexpr int kNV = 16, kNV1 = 32;  // rows of a thread: vectors, and single channels
+// ---------------------------------------------------------------------------
+// Launches
+
+struct NormArgs {
+  const void *x, *dy, *w, *b;
+  int64_t ld, chains;
+  const int4 *tiles, *whole;
+  const int32_t* first_tile;
+  int n_tiles, n_whole, max_len, C, G, act;
+  float eps;
+};
+
+constexpr int kOneRows = 1024, kOneChains = 512;
+
+bool by_chain(int max_len, int n_whole) { return max_len <= kOneRows || n_whole >= kOneChains; }
 
 // Threads of a workgroup: a column of every vector of a row, and at least 4
 // rows of them where a row has no more than 256 vectors.
 int norm_threads(int tc) { return tc <= 64 ? 256 : 1024; }
 
-template <typename T, int W>
-NormShape norm_shape(const int32_t* tiles, int n_tiles, int size, int C, int G) {
+template <int W>
+NormShape norm_shape(const NormArgs& a, bool one) {
   NormShape sh;
-  sh.tiles = reinterpret_cast<const int4*>(tiles);
-  sh.n_tiles = n_tiles;
-  sh.size = size;
-  sh.C = C;
-  sh.G = G;
-  sh.TC = C / W;
+  sh.tiles = one ? a.whole : a.tiles;
+  sh.n_tiles = one ? a.n_whole : a.n_tiles;
+  sh.size = one ? a.max_len : kSlabRows;
+  sh.C = a.C;
+  sh.G = a.G;
+  sh.TC = a.C / W;
   sh.TR = norm_threads(sh.TC) / sh.TC;
-  sh.cols = 0;
-  sh.per = 0;
+  sh.chains = a.chains;
   return sh;
 }
 
+// LDS above 64 KiB has to be asked for.
+template <typename F>
+int allow(F f, unsigned lds) {
+  if (lds > 65536u &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(f),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+    return MLCG_ERR_LAUNCH;
+  return MLCG_OK;
+}
+
 template <typename T, int W>
-int norm_fwd(NormShape sh, const T* x, int64_t ld, const T* w, const T* b,
-             const int32_t* first_tile, int64_t chains, float eps, int act, T* y,
-             float* stats, float* ws, hipStream_t s) {
-  const int nt = norm_threads(sh.TC);
-  constexpr int NV = W == 1 ? kNV1 : kNV;
-  const int P = sh.C / sh.G;
-  const unsigned lds = (unsigned)((nt * W + sh.C + 3 * sh.G) * sizeof(float));
-  float4* part = reinterpret_cast<float4*>(ws);
-  if (P % W == 0) {
-    sh.per = P / W;
-    hipLaunchKernelGGL((norm_part_kernel<T, W, NV, true>), dim3(sh.n_tiles), dim3(nt), lds, s, sh,
-                       x, ld, part);
-  } else {
-    sh.per = P;
-    hipLaunchKernelGGL((norm_part_kernel<T, W, NV, false>), dim3(sh.n_tiles), dim3(nt), lds, s,
-                       sh, x, ld, part);
+int norm_fwd(const NormArgs& a, void* y, float* stats, float* ws, hipStream_t s) {
+  const bool one = by_chain(a.max_len, a.n_whole), grouped = (a.C / a.G) % W == 0;
+  const NormShape sh = norm_shape<W>(a, one);
+  const int nt = norm_threads(sh.TC), k = grouped ? 1 : W;
+  const unsigned lds = (unsigned)((3 * sh.G + (nt + sh.TC) * 2 * k) * sizeof(float));
+  const T *x = (const T*)a.x, *w = (const T*)a.w, *b = (const T*)a.b;
+  if (one) {
+    auto f = grouped ? norm_chain_kernel<T, W, true> : norm_chain_kernel<T, W, false>;
+    if (int e = allow(f, lds)) return e;
+    hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, w, b, a.eps, a.act,
+                       (T*)y, stats);
+    return mlcg_launch_status();
   }
-  hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)chains, mlcg_div_up(sh.G, 4)), dim3(256), 0,
-                     s, sh, first_tile, part, eps, stats);
-  hipLaunchKernelGGL((norm_apply_kernel<T, W>), dim3(sh.n_tiles), dim3(nt), 0, s, sh, x, ld, w, b,
-                     stats, chains, act, y);
+  float4* part = reinterpret_cast<float4*>(ws);
+  auto f = grouped ? norm_part_kernel<T, W, true> : norm_part_kernel<T, W, false>;
+  if (int e = allow(f, lds)) return e;
+  hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, part);
+  hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)sh.chains, sh.G), dim3(256), 0, s, sh,
+                     a.first_tile, part, a.eps, stats);
+  hipLaunchKernelGGL((norm_apply_kernel<T, W>), dim3(sh.n_tiles), dim3(nt), 0, s, sh, x, a.ld, w,
+                     b, stats, a.act, (T*)y);
   return mlcg_launch_status();
 }
 
 template <typename T, int W>
-int norm_bwd(NormShape sh, const T* x, int64_t ld, const T* dy, const T* w, const T* b,
-             const float* stats, const int32_t* first_tile, int64_t chains, int act, T* dx, T* dw_db, float* ws, hipStream_t s) {
+int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* ws,
+             hipStream_t s) {
+  const bool one = by_chain(a.max_len, a.n_whole);
+  const NormShape sh = norm_shape<W>(a, one);
   const int nt = norm_threads(sh.TC);
-  const unsigned lds = (unsigned)((nt * W + sh.C) * sizeof(float));
+  const T *x = (const T*)a.x, *dy = (const T*)a.dy, *w = (const T*)a.w, *b = (const T*)a.b;
+  const unsigned cols = mlcg_div_up(2 * sh.C, 8);
+  if (one) {
+    const unsigned lds = (unsigned)((nt * 2 * W + 4 * sh.C + 2 * sh.G) * sizeof(float));
+    auto f = norm_chain_bwd_kernel<T, W>;
+    if (int e = allow(f, lds)) return e;
+    const int groups = std::min(sh.n_tiles, 1024);
+    hipLaunchKernelGGL(f, dim3(groups), dim3(nt), lds, s, sh, x, a.ld, dy, w, b, stats, a.act,
+                       (T*)dx, ws);
+    hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, ws, 2 * sh.C, nullptr,
+                       nullptr, 1, groups, (T*)dbw);
+    return mlcg_launch_status();
+  }
+  const unsigned lds = (unsigned)((nt * 2 * W + 2 * sh.C) * sizeof(float));
+  auto f = norm_bwd_part_kernel<T, W>;
+  if (int e = allow(f, lds)) return e;
   float* part = ws;
   float* chain_sums = ws + (int64_t)sh.n_tiles * 2 * sh.C;
-  hipLaunchKernelGGL((norm_bwd_part_kernel<T, W>), dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, ld,
-                     dy, w, b, stats, chains, act, part);
-  hipLaunchKernelGGL(norm_rows_kernel<float>, dim3(mlcg_div_up(2 * sh.C, 32), (unsigned)chains),
-                     dim3(1024), 0, s, part, 2 * sh.C, first_tile, sh.tiles, sh.size, 0,
-                     chain_sums);
+  hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, dy, w, b, stats, a.act,
+                     part);
+  hipLaunchKernelGGL(norm_rows_kernel<float>, dim3(cols, (unsigned)sh.chains), dim3(1024), 0, s,
+                     part, 2 * sh.C, a.first_tile, sh.tiles, sh.size, 0, chain_sums);
   hipLaunchKernelGGL((norm_bwd_apply_kernel<T, W>), dim3(sh.n_tiles), dim3(nt),
-                     (unsigned)((sh.C + 2 * sh.G) * sizeof(float)), s, sh, x, ld, dy, w, b, stats,
-                     chains, chain_sums, act, dx);
-  hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(mlcg_div_up(2 * sh.C, 32), 1), dim3(1024), 0, s,
-                     chain_sums, 2 * sh.C, nullptr, nullptr, 1, (int)chains, dw_db);
+                     (unsigned)((2 * sh.C + 2 * sh.G) * sizeof(float)), s, sh, x, a.ld, dy, w, b,
+                     stats, chain_sums, a.act, (T*)dx);
+  hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, chain_sums, 2 * sh.C,
+                     nullptr, nullptr, 1, (int)sh.chains, (T*)dbw);
   return mlcg_launch_status();
 }
 
+// 16-byte vectors of channels, where every row begins at a multiple of them
 template <typename T>
-constexpr int vec_width() {
-  return 16 / sizeof(T);
+bool norm_vec(const NormArgs& a, const void* out) {
+  constexpr int W = 16 / sizeof(T);
+  return a.C % W == 0 && a.ld % W == 0 && chain_aligned16(a.x) && chain_aligned16(a.dy) &&
+         chain_aligned16(out);
 }
 
-template <typename T>
-bool norm_vec(const void* x, int64_t ld, const void* o1, const void* o2, int C) {
-  constexpr int W = vec_width<T>();
-  return C % W == 0 && ld % W == 0 && chain_aligned16(x) && chain_aligned16(o1) &&
-         chain_aligned16(o2);
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == MLCG_DTYPE_F32) return f(float{});
+  if (dtype == MLCG_DTYPE_F16) return f(_Float16{});
+  return f(__bf16{});
 }
 
-bool norm_args_ok(int64_t rows, int64_t chains, int64_t n_tiles, int size, int width, int groups,
-                  int64_t ld, int act, int dtype) {
-  return rows >= 0 && rows < (int64_t(1) << 31) && chains >= 0 && chains < (int64_t(1) << 31) &&
-         n_tiles >= 0 && n_tiles < (int64_t(1) << 31) && size >= 1 && width >= 1 &&
-         width <= kMaxWidth && groups >= 1 && width % groups == 0 && ld >= width &&
-         act >= MLCG_ACT_TANH && act <= MLCG_ACT_NONE && dtype >= MLCG_DTYPE_F32 &&
-         dtype <= MLCG_DTYPE_BF16;
+bool norm_args_ok(const NormArgs& a, int64_t rows, int64_t n_tiles, int64_t n_whole,
+                  int64_t max_len, int dtype) {
+  const int64_t most = int64_t(1) << 31;
+  return rows >= 1 && rows < most && a.chains >= 1 && a.chains < most && n_tiles >= 1 &&
+         n_tiles < most && n_whole >= 1 && n_whole <= n_tiles && max_len >= 1 && max_len <= rows &&
+         a.C >= 1 && a.C <= kMaxWidth && a.G >= 1 && a.C % a.G == 0 && a.ld >= a.C &&
+         a.act >= MLCG_ACT_TANH && a.act <= MLCG_ACT_NONE && dtype >= MLCG_DTYPE_F32 &&
+         dtype <= MLCG_DTYPE_BF16 && a.x && a.w && a.b && a.tiles && a.whole && a.first_tile;
 }
 
 }  // namespace
 
-// Rows of a slab that fit the registers, a power of two of 32 to 256.
-extern "C" int mlcg_group_norm_slab_rows(int width, int dtype) {
-  if (width < 1 || width > kMaxWidth || dtype < MLCG_DTYPE_F32 || dtype > MLCG_DTYPE_BF16)
-    return -1;
-  const int W = dtype == MLCG_DTYPE_F32 ? 4 : 8;
-  // the vector form's and the single-channel form's: the call decides which
-  // runs, so a slab has to fit both
-  int rows = 256;
-  const int t1 = norm_threads(width), tv = norm_threads(width / W);
-  while (rows > 32 && (rows > kNV1 * (t1 / width) ||
-                       (width % W == 0 && rows > kNV * (tv / (width / W)))))
-    rows >>= 1;
-  return rows;
-}
-
-extern "C" int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t chains, int width,
+extern "C" int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t chains,
+                                                    int64_t n_whole, int64_t max_len, int width,
                                                     int groups, int backward) {
-  if (n_tiles < 0 || chains < 0 || width < 1 || groups < 1) return -1;
+  if (n_tiles < 0 || chains < 0 || n_whole < 0 || max_len < 0 || width < 1 || groups < 1)
+    return -1;
+  if (max_len <= kOneRows || n_whole >= kOneChains)
+    return backward ? 2 * std::min<int64_t>(n_whole, 1024) * width : 0;
   return backward ? 2 * (n_tiles + chains) * width : 4 * n_tiles * groups;
 }
 
 extern "C" int mlcg_group_norm_act(const void* x, int64_t ld, int64_t rows, int dtype,
                                    const void* weight, const void* bias, int width, int groups,
                                    const int32_t* tiles, const int32_t* first_tile,
-                                   int64_t n_tiles, int size, int64_t chains, float eps, int act,
-                                   void* y, float* stats, float* workspace,
-                                   int64_t workspace_floats, void* stream) {
-  MLCG_REQUIRE(norm_args_ok(rows, chains, n_tiles, size, width, groups, ld, act, dtype));
-  MLCG_REQUIRE(size <= mlcg_group_norm_slab_rows(width, dtype));
-  if (rows == 0 || n_tiles == 0) return MLCG_OK;
-  MLCG_REQUIRE(x && weight && bias && tiles && first_tile && y && stats && workspace);
-  MLCG_REQUIRE(workspace_floats >=
-               mlcg_group_norm_workspace_floats(n_tiles, chains, width, groups, 0));
+                                   int64_t n_tiles, const int32_t* whole, int64_t n_whole,
+                                   int64_t max_len, int64_t chains, float eps, int act, void* y,
+                                   float* stats, float* workspace, int64_t workspace_floats,
+                                   void* stream) {
+  if (rows == 0) return MLCG_OK;
+  const NormArgs a{x, nullptr, weight, bias, ld, chains, reinterpret_cast<const int4*>(tiles),
+                   reinterpret_cast<const int4*>(whole), first_tile, (int)n_tiles, (int)n_whole,
+                   (int)max_len, width, groups, act, eps};
+  MLCG_REQUIRE(norm_args_ok(a, rows, n_tiles, n_whole, max_len, dtype) && y && stats);
+  const int64_t need = mlcg_group_norm_workspace_floats(n_tiles, chains, n_whole, max_len, width,
+                                                        groups, 0);
+  MLCG_REQUIRE(workspace_floats >= need && (need == 0 || workspace));
   hipStream_t s = mlcg_stream(stream);
-#define NORM_FWD(T)                                                                              \
-  if (norm_vec<T>(x, ld, y, nullptr, width))                                                     \
-    return norm_fwd<T, vec_width<T>()>(                                                          \
-        norm_shape<T, vec_width<T>()>(tiles, (int)n_tiles, size, width, groups), (const T*)x,    \
-        ld, (const T*)weight, (const T*)bias, first_tile, chains, eps, act, (T*)y, stats, workspace, s);                                                                           \
-  return norm_fwd<T, 1>(norm_shape<T, 1>(tiles, (int)n_tiles, size, width, groups), (const T*)x, \
-                        ld, (const T*)weight, (const T*)bias, first_tile, chains, eps, act,      \
-                        (T*)y, stats, workspace, s);
-  if (dtype == MLCG_DTYPE_F32) {
-    NORM_FWD(float)
-  } else if (dtype == MLCG_DTYPE_F16) {
-    NORM_FWD(_Float16)
-  }
-  NORM_FWD(__bf16)
-#undef NORM_FWD
+  return by_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return norm_vec<T>(a, y) ? norm_fwd<T, 16 / (int)sizeof(T)>(a, y, stats, workspace, s)
+                             : norm_fwd<T, 1>(a, y, stats, workspace, s);
+  });
 }
 
 extern "C" int mlcg_group_norm_act_backward(
     const void* x, int64_t ld, const void* grad_y, int64_t rows, int dtype, const void* weight,
     const void* bias, int width, int groups, const int32_t* tiles, const int32_t* first_tile,
-    int64_t n_tiles, int size, int64_t chains, int act, const float* stats, void* grad_x, void* grad_weight_bias, float* workspace, int64_t workspace_floats,
-    void* stream) {
-  MLCG_REQUIRE(norm_args_ok(rows, chains, n_tiles, size, width, groups, ld, act, dtype));
-  MLCG_REQUIRE(rows > 0 && n_tiles > 0 && size <= mlcg_group_norm_slab_rows(width, dtype));
-  MLCG_REQUIRE(x && grad_y && weight && bias && tiles && first_tile && stats && grad_x &&
-               grad_weight_bias && workspace);
-  MLCG_REQUIRE(workspace_floats >=
-               mlcg_group_norm_workspace_floats(n_tiles, chains, width, groups, 1));
+    int64_t n_tiles, const int32_t* whole, int64_t n_whole, int64_t max_len, int64_t chains,
+    int act, const float* stats, void* grad_x, void* grad_bias_weight, float* workspace,
+    int64_t workspace_floats, void* stream) {
+  const NormArgs a{x, grad_y, weight, bias, ld, chains, reinterpret_cast<const int4*>(tiles),
+                   reinterpret_cast<const int4*>(whole), first_tile, (int)n_tiles, (int)n_whole,
+                   (int)max_len, width, groups, act, 0.0f};
+  MLCG_REQUIRE(norm_args_ok(a, rows, n_tiles, n_whole, max_len, dtype) && grad_y && stats &&
+               grad_x && grad_bias_weight && workspace);
+  MLCG_REQUIRE(workspace_floats >= mlcg_group_norm_workspace_floats(
+                                       n_tiles, chains, n_whole, max_len, width, groups, 1));
   hipStream_t s = mlcg_stream(stream);
-#define NORM_BWD(T)                                                                              \
-  if (norm_vec<T>(x, ld, grad_y, grad_x, width))                                                 \
-    return norm_bwd<T, vec_width<T>()>(                                                          \
-        norm_shape<T, vec_width<T>()>(tiles, (int)n_tiles, size, width, groups), (const T*)x,    \
-        ld, (const T*)grad_y, (const T*)weight, (const T*)bias, stats, first_tile, chains,  \
-        act, (T*)grad_x, (T*)grad_weight_bias, workspace, s);                                    \
-  return norm_bwd<T, 1>(norm_shape<T, 1>(tiles, (int)n_tiles, size, width, groups), (const T*)x, \
-                        ld, (const T*)grad_y, (const T*)weight, (const T*)bias, stats,      \
-                        first_tile, chains, act, (T*)grad_x, (T*)grad_weight_bias, workspace, s);
-  if (dtype == MLCG_DTYPE_F32) {
-    NORM_BWD(float)
-  } else if (dtype == MLCG_DTYPE_F16) {
-    NORM_BWD(_Float16)
-  }
-  NORM_BWD(__bf16)
-#undef NORM_BWD
+  return by_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return norm_vec<T>(a, grad_x)
+               ? norm_bwd<T, 16 / (int)sizeof(T)>(a, stats, grad_x, grad_bias_weight, workspace, s)
+               : norm_bwd<T, 1>(a, stats, grad_x, grad_bias_weight, workspace, s);
+  });
 }

@@ -1778,6 +1778,7 @@ class ChainLayout:
               records (chain's first bead, its length, the tile's first bead in
               it, chain), the longest chains first
     first   : {rows: [n_chains] int32}, a chain's first tile, -1 without beads
+    whole   : [n, 4] int32, the chains that have beads as one tile each
     """
 
     lengths: Tuple[int, ...]
@@ -1788,6 +1789,7 @@ class ChainLayout:
     ptr: torch.Tensor
     tiles: dict
     first: dict
+    whole: torch.Tensor
 
 
 def chain_layout(lengths, device) -> ChainLayout:
@@ -1811,7 +1813,8 @@ def chain_layout(lengths, device) -> ChainLayout:
     start = np.concatenate([[0], np.cumsum(lens)])
     order = np.argsort(-lens, kind="stable")  # long chains begin first
     parts, sizes = [], []
-    for rows in CHAIN_TILE_ROWS:
+    max_len = int(lens.max()) if lens.size else 0
+    for rows in (*CHAIN_TILE_ROWS, max(1, max_len)):
         count = (lens[order] + rows - 1) // rows
         chain = np.repeat(order, count)
         begin = np.concatenate([[0], np.cumsum(count)])
@@ -1820,18 +1823,20 @@ def chain_layout(lengths, device) -> ChainLayout:
         first = np.full(lens.size, -1, dtype=np.int64)
         first[order] = np.where(count > 0, begin[:-1], -1)
         sizes.append((int(begin[-1]), first))
-    firsts = [f for _, f in sizes]
+    firsts = [f for _, f in sizes[:-1]]
     packed = torch.from_numpy(np.concatenate(parts + firsts).astype(np.int32)).to(device)
     tiles, first, at = {}, {}, 0
     for rows, (n, _) in zip(CHAIN_TILE_ROWS, sizes):
         tiles[rows] = packed[at:at + 4 * n].view(n, 4)
         at += 4 * n
+    whole = packed[at:at + 4 * sizes[-1][0]].view(-1, 4)
+    at += 4 * sizes[-1][0]
     for rows in CHAIN_TILE_ROWS:
         first[rows] = packed[at:at + lens.size]
         at += lens.size
     return ChainLayout(lengths=tuple(lens.tolist()), n_chains=int(lens.size), n_beads=total,
-                       max_len=int(lens.max()) if lens.size else 0, device=device,
-                       ptr=torch.from_numpy(start).to(device), tiles=tiles, first=first)
+                       max_len=max_len, device=device, ptr=torch.from_numpy(start).to(device),
+                       tiles=tiles, first=first, whole=whole)
 
 
 @dataclass(eq=False)
@@ -2054,18 +2059,23 @@ def _norm_args(x, weight, bias, groups, chains, act):
     if (width > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < width):
         x = x.contiguous()
     ld = x.stride(0) if n > 1 else width
-    rows = _norm_slab_rows(width, dt)
-    return x, ld, n, width, dt, weight.contiguous(), bias.contiguous(), CHAIN_ACTS[act], rows
+    return x, ld, n, width, dt, weight.contiguous(), bias.contiguous(), CHAIN_ACTS[act]
 
 
-_NORM_ROWS: dict = {}
+NORM_SLAB_ROWS = 256
 
 
-def _norm_slab_rows(width: int, dt: int) -> int:
-    rows = _NORM_ROWS.get((width, dt))
-    if rows is None:
-        rows = _NORM_ROWS[width, dt] = int(_lib.load().mlcg_group_norm_slab_rows(width, dt))
-    return rows
+def _norm_workspace(chains: ChainLayout, width: int, groups: int, backward: int, dev):
+    nws = int(_lib.load().mlcg_group_norm_workspace_floats(
+        chains.tiles[NORM_SLAB_ROWS].shape[0], chains.n_chains, chains.whole.shape[0],
+        chains.max_len, width, groups, backward))
+    return (torch.empty(nws, dtype=torch.float32, device=dev) if nws > 0 else None), nws
+
+
+def _norm_chains(chains: ChainLayout):
+    tiles, whole = chains.tiles[NORM_SLAB_ROWS], chains.whole
+    return (ptr(tiles), ptr(chains.first[NORM_SLAB_ROWS]), tiles.shape[0], ptr(whole),
+            whole.shape[0], chains.max_len, chains.n_chains)
 
 
 def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, groups: int,
@@ -2080,17 +2090,14 @@ def group_norm_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, gr
     "ssp" (shifted softplus) or "silu".  x may have any row stride; weight and
     bias [C] have its type.  stats holds the mean, what its rounding left out
     and 1 / sqrt(var + eps), undefined for an empty chain."""
-    x, ld, n, width, dt, weight, bias, act_id, rows = _norm_args(x, weight, bias, groups, chains,
-                                                                 act)
+    x, ld, n, width, dt, weight, bias, act_id = _norm_args(x, weight, bias, groups, chains, act)
     dev = x.device
     y = torch.empty(n, width, dtype=x.dtype, device=dev)
-    tiles = chains.tiles[rows]
     stats = torch.empty(3, chains.n_chains, groups, dtype=torch.float32, device=dev)
-    nws = 4 * tiles.shape[0] * groups
-    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    ws, nws = _norm_workspace(chains, width, groups, 0, dev)
     call("mlcg_group_norm_act", ptr(x), ld, n, dt, ptr(weight), ptr(bias), width, groups,
-         ptr(tiles), ptr(chains.first[rows]), tiles.shape[0], rows, chains.n_chains, float(eps),
-         act_id, ptr(y), ptr(stats), ptr(ws), nws, stream_handle(dev))
+         *_norm_chains(chains), float(eps), act_id, ptr(y), ptr(stats), ptr(ws), nws,
+         stream_handle(dev))
     return y, stats
 
 
@@ -2098,8 +2105,7 @@ def group_norm_act_backward(x, weight, bias, groups: int, chains: ChainLayout,
                             stats: torch.Tensor, grad: torch.Tensor, act: str = "none"):
     """(grad x, grad weight, grad bias) of group_norm_act for the gradient of y
     (mlcg_group_norm_act_backward); stats are the forward's."""
-    x, ld, n, width, dt, weight, bias, act_id, rows = _norm_args(x, weight, bias, groups, chains,
-                                                                 act)
+    x, ld, n, width, dt, weight, bias, act_id = _norm_args(x, weight, bias, groups, chains, act)
     dev = x.device
     _check(tuple(grad.shape) == (n, width) and grad.dtype == x.dtype and grad.device == dev,
            lambda: f"grad must be [{n}, {width}] {x.dtype} on {dev}")
@@ -2111,13 +2117,10 @@ def group_norm_act_backward(x, weight, bias, groups: int, chains: ChainLayout,
     if n == 0:
         return dx, torch.zeros_like(weight), torch.zeros_like(bias)
     dbw = torch.empty(2, width, dtype=x.dtype, device=dev)
-    tiles = chains.tiles[rows]
-    nws = 2 * (tiles.shape[0] + chains.n_chains) * width
-    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    ws, nws = _norm_workspace(chains, width, groups, 1, dev)
     call("mlcg_group_norm_act_backward", ptr(x), ld, ptr(grad), n, dt, ptr(weight), ptr(bias),
-         width, groups, ptr(tiles), ptr(chains.first[rows]), tiles.shape[0], rows,
-         chains.n_chains, act_id, ptr(stats), ptr(dx), ptr(dbw), ptr(ws), nws,
-         stream_handle(dev))
+         width, groups, *_norm_chains(chains), act_id, ptr(stats), ptr(dx), ptr(dbw), ptr(ws),
+         nws, stream_handle(dev))
     return dx, dbw[1], dbw[0]
 
 
