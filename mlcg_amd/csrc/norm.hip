@@ -26,6 +26,7 @@
 // channel over the chains it takes, and one that joins these.  Few long
 // chains: slabs of them, joined in slab order, then a second reading.
 #include <algorithm>
+#include <type_traits>
 
 #include "chain.h"
 
@@ -33,7 +34,6 @@ namespace {
 
 constexpr int kMaxWidth = 1024;
 constexpr int kSlabRows = 256;
-constexpr int kNV = 4;
 
 struct NormShape {
   const int4* tiles;  // (chain's first row, chain's length, slab's first row in it, chain)
@@ -83,12 +83,20 @@ struct Place {
       : row(threadIdx.x / sh.TC), col(threadIdx.x % sh.TC), in(row < sh.TR) {}
 };
 
+// Rows of a thread's step: 16 channels of 16 bits, or 16 of 32 bits, in flight
+// for each array; more would cost the waves that hide the latency.
+template <int W>
+constexpr int step_rows() {
+  return W == 8 ? 2 : 4;
+}
+
 // the rows r0 + row + v TR, v < NV, of a column; those at or past `rows` are
 // loaded as the last one
 template <typename T, int W>
 __device__ __forceinline__ void load_step(const NormShape& sh, const Place& at, const T* x,
                                           int64_t ld, int r0, int rows,
-                                          typename Vec<T, W>::type (&out)[kNV]) {
+                                          typename Vec<T, W>::type (&out)[step_rows<W>()]) {
+  constexpr int kNV = step_rows<W>();
 #pragma unroll
   for (int v = 0; v < kNV; ++v) {
     const int r = min(r0 + at.row + v * sh.TR, rows - 1);
@@ -155,16 +163,16 @@ __device__ __forceinline__ void group_sums(const float* sums, int groups, int pe
 }
 
 // The statistics of `rows` rows from x on, by group, into LDS: the mean, its
-// remainder and the sum of squared deviations.  GROUPED: a vector lies in one
-// group, and its values are summed first.
-template <typename T, int W, bool GROUPED>
+// remainder and the sum of squared deviations.  K sums a vector, of W / K
+// channels of one group each.
+template <typename T, int W, int K>
 __device__ __forceinline__ void row_stats(const NormShape& sh, const Place& at, const T* x,
                                           int64_t ld, int rows, float* lds, float* mean,
                                           float* rest, float* m2) {
-  constexpr int K = GROUPED ? 1 : W;
+  constexpr int kNV = step_rows<W>();
   float* red = lds;                         // blockDim 2 K
   float* sums = red + blockDim.x * 2 * K;   // TC 2 K
-  const int P = sh.C / sh.G, per = GROUPED ? P / W : P;
+  const int P = sh.C / sh.G, per = P / (W / K);
   typename Vec<T, W>::type xv[kNV];
   load_step<T, W>(sh, at, x, ld, 0, rows, xv);
   float s[K] = {};
@@ -172,7 +180,7 @@ __device__ __forceinline__ void row_stats(const NormShape& sh, const Place& at, 
   for (int v = 0; v < kNV; ++v)
     if (step_row(sh, at, 0, v, rows))
 #pragma unroll
-      for (int j = 0; j < W; ++j) s[GROUPED ? 0 : j] += (float)xv[v][j];
+      for (int j = 0; j < W; ++j) s[j / (W / K)] += (float)xv[v][j];
   column_sums<K>(sh, s, red, sums);
   const float first = 1.0f / ((float)min(rows, kNV * sh.TR) * (float)P);
   // the pivot comes back from LDS: rounded, as it is used
@@ -187,7 +195,7 @@ __device__ __forceinline__ void row_stats(const NormShape& sh, const Place& at, 
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const float d = ok ? (float)xv[v][j] - p[j] : 0.0f;
-        const int k = GROUPED ? 0 : j;
+        const int k = j / (W / K);
         d2[2 * k] += d;
         d2[2 * k + 1] = fmaf(d, d, d2[2 * k + 1]);
       }
@@ -225,8 +233,9 @@ struct Channels {
       b[j] = (float)bias[c];
     }
   }
+  // the remainder of the mean is below what 16 bits hold of a value
   __device__ __forceinline__ float hat(int j, float x) const {
-    return ((x - mu[j]) - lo[j]) * rs[j];
+    return sizeof(T) == 4 ? ((x - mu[j]) - lo[j]) * rs[j] : (x - mu[j]) * rs[j];
   }
 };
 
@@ -234,6 +243,7 @@ template <typename T, int W>
 __device__ __forceinline__ void apply_rows(const NormShape& sh, const Place& at,
                                            const Channels<T, W>& ch, const T* x, int64_t ld,
                                            int rows, int act, T* y) {
+  constexpr int kNV = step_rows<W>();
   for (int r0 = 0; r0 < rows; r0 += kNV * sh.TR) {
     typename Vec<T, W>::type xv[kNV];
     load_step<T, W>(sh, at, x, ld, r0, rows, xv);
@@ -251,8 +261,8 @@ __device__ __forceinline__ void apply_rows(const NormShape& sh, const Place& at,
 }
 
 // One chain a workgroup.
-template <typename T, int W, bool GROUPED>
-__global__ __launch_bounds__(1024) void norm_chain_kernel(NormShape sh, const T* __restrict__ x,
+template <typename T, int W, int K, int NT>
+__global__ __launch_bounds__(NT) void norm_chain_kernel(NormShape sh, const T* __restrict__ x,
                                                           int64_t ld, const T* __restrict__ w,
                                                           const T* __restrict__ b, float eps,
                                                           int act, T* __restrict__ y,
@@ -265,7 +275,7 @@ __global__ __launch_bounds__(1024) void norm_chain_kernel(NormShape sh, const T*
   const Place at(sh);
   const int P = sh.C / sh.G;
   const T* xt = x + (int64_t)t.x * ld;
-  row_stats<T, W, GROUPED>(sh, at, xt, ld, t.y, rstd + sh.G, mean, rest, rstd);
+  row_stats<T, W, K>(sh, at, xt, ld, t.y, rstd + sh.G, mean, rest, rstd);
   const float inv = 1.0f / ((float)t.y * (float)P);
   for (int g = threadIdx.x; g < sh.G; g += blockDim.x) {
     const float rs = 1.0f / sqrtf(rstd[g] * inv + eps);
@@ -281,8 +291,8 @@ __global__ __launch_bounds__(1024) void norm_chain_kernel(NormShape sh, const T*
 }
 
 // (mean, its remainder, M2) of every group of a slab -> part[g][tile]
-template <typename T, int W, bool GROUPED>
-__global__ __launch_bounds__(1024) void norm_part_kernel(NormShape sh, const T* __restrict__ x,
+template <typename T, int W, int K, int NT>
+__global__ __launch_bounds__(NT) void norm_part_kernel(NormShape sh, const T* __restrict__ x,
                                                          int64_t ld, float4* __restrict__ part) {
   extern __shared__ float lds[];
   float* mean = lds;  // G each
@@ -290,7 +300,7 @@ __global__ __launch_bounds__(1024) void norm_part_kernel(NormShape sh, const T* 
   float* m2 = rest + sh.G;
   const int4 t = sh.tiles[blockIdx.x];
   const Place at(sh);
-  row_stats<T, W, GROUPED>(sh, at, x + ((int64_t)t.x + t.z) * ld, ld, min(sh.size, t.y - t.z),
+  row_stats<T, W, K>(sh, at, x + ((int64_t)t.x + t.z) * ld, ld, min(sh.size, t.y - t.z),
                            m2 + sh.G, mean, rest, m2);
   for (int g = threadIdx.x; g < sh.G; g += blockDim.x)
     part[(int64_t)g * sh.n_tiles + blockIdx.x] = make_float4(mean[g], rest[g], m2[g], 0.0f);
@@ -343,8 +353,8 @@ __global__ __launch_bounds__(256) void norm_join_kernel(NormShape sh,
   }
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(1024) void norm_apply_kernel(
+template <typename T, int W, int NT>
+__global__ __launch_bounds__(NT) void norm_apply_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ w,
     const T* __restrict__ b, const float* __restrict__ stats, int act, T* __restrict__ y) {
   const int4 t = sh.tiles[blockIdx.x];
@@ -367,6 +377,7 @@ __device__ __forceinline__ void row_grads(const NormShape& sh, const Place& at,
                                           const Channels<T, W>& ch, const T* x, int64_t ld,
                                           const T* dy, int rows, int act, float* red,
                                           float* sums) {
+  constexpr int kNV = step_rows<W>();
   float ab[2 * W] = {};
   for (int r0 = 0; r0 < rows; r0 += kNV * sh.TR) {
     typename Vec<T, W>::type xv[kNV], gv[kNV];
@@ -395,6 +406,7 @@ __device__ __forceinline__ void row_dx(const NormShape& sh, const Place& at,
                                        const Channels<T, W>& ch, const T* x, int64_t ld,
                                        const T* dy, int rows, int act, const float* s1,
                                        const float* s2, float inv, T* dx) {
+  constexpr int kNV = step_rows<W>();
   const int P = sh.C / sh.G;
   float m1[W], m2[W];
 #pragma unroll
@@ -429,52 +441,72 @@ __device__ __forceinline__ void row_dx(const NormShape& sh, const Place& at,
 }
 
 // dx of the chains blockIdx.x, blockIdx.x + gridDim.x, ... and the sums of A_c
-// and B_c over them -> part[workgroup][2][C]
-template <typename T, int W>
-__global__ __launch_bounds__(1024) void norm_chain_bwd_kernel(
+// and B_c over them -> part[workgroup][2][C].  A chain needs the groups' sums
+// alone (K of w A and of w B a vector); the channels' stay in the threads'
+// registers until the last chain.
+template <typename T, int W, int K, int NT>
+__global__ __launch_bounds__(NT) void norm_chain_bwd_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
     const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats, int act,
     T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int kNV = step_rows<W>();
   extern __shared__ float lds[];
-  float* red = lds;                        // blockDim 2 W
-  float* sums = red + blockDim.x * 2 * W;  // 2 C: (A, B) by channel
-  float* total = sums + 2 * sh.C;          // 2 C
-  float* s1 = total + 2 * sh.C;            // G each
+  float* red = lds;              // NT 2 W
+  float* sums = red + NT * 2 * W;  // 2 C
+  float* s1 = sums + 2 * sh.C;   // G each
   float* s2 = s1 + sh.G;
   const Place at(sh);
   const int P = sh.C / sh.G;
   const int64_t all = sh.chains * sh.G;
-  for (int c = threadIdx.x; c < 2 * sh.C; c += blockDim.x) total[c] = 0.0f;
+  float ab[2 * W] = {};
   for (int tile = blockIdx.x; tile < sh.n_tiles; tile += gridDim.x) {
     const int4 t = sh.tiles[tile];
     const float* st = stats + (int64_t)t.w * sh.G;
     const Channels<T, W> ch(P, at, st, st + all, st + 2 * all, w, b);
     const T* xt = x + (int64_t)t.x * ld;
     const T* dt = dy + (int64_t)t.x * sh.C;
-    row_grads<T, W>(sh, at, ch, xt, ld, dt, t.y, act, red, sums);
-    for (int c = threadIdx.x; c < 2 * sh.C; c += blockDim.x) {
-      const float a = sums[c];
-      total[c] += a;
-      sums[c] = (float)w[c >> 1] * a;
+    float wab[2 * K] = {};
+    for (int r0 = 0; r0 < t.y; r0 += kNV * sh.TR) {
+      typename Vec<T, W>::type xv[kNV], gv[kNV];
+      load_step<T, W>(sh, at, xt, ld, r0, t.y, xv);
+      load_step<T, W>(sh, at, dt, sh.C, r0, t.y, gv);
+#pragma unroll
+      for (int v = 0; v < kNV; ++v) {
+        const bool ok = step_row(sh, at, r0, v, t.y);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const float hat = ch.hat(j, (float)xv[v][j]);
+          float yv, d;
+          act_z(act, fmaf(hat, ch.w[j], ch.b[j]), yv, d);
+          const float dz = ok ? (float)gv[v][j] * d : 0.0f;
+          ab[2 * j] += dz;
+          ab[2 * j + 1] = fmaf(dz, hat, ab[2 * j + 1]);
+          float dh = dz * ch.w[j];
+          asm("" : "+v"(dh));  // rounded, as in row_dx
+          const int k = j / (W / K);
+          wab[2 * k] += dh;
+          wab[2 * k + 1] = fmaf(dh, hat, wab[2 * k + 1]);
+        }
+      }
     }
-    __syncthreads();
-    group_sums(sums, sh.G, P, 2, [&](int g, float a, float q) {
+    column_sums<2 * K>(sh, wab, red, sums);
+    group_sums(sums, sh.G, P / (W / K), 2, [&](int g, float a, float q) {
       s1[g] = a;
       s2[g] = q;
     });
     row_dx<T, W>(sh, at, ch, xt, ld, dt, t.y, act, s1, s2, 1.0f / ((float)t.y * (float)P),
                  dx + (int64_t)t.x * sh.C);
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < sh.C; c += blockDim.x) {
-    part[(int64_t)blockIdx.x * 2 * sh.C + c] = total[2 * c];
-    part[(int64_t)blockIdx.x * 2 * sh.C + sh.C + c] = total[2 * c + 1];
+  column_sums<2 * W>(sh, ab, red, sums);
+  for (int c = threadIdx.x; c < sh.C; c += NT) {
+    part[(int64_t)blockIdx.x * 2 * sh.C + c] = sums[2 * c];
+    part[(int64_t)blockIdx.x * 2 * sh.C + sh.C + c] = sums[2 * c + 1];
   }
 }
 
 // (A_c, B_c) of a slab -> part[tile][2][C]
-template <typename T, int W>
-__global__ __launch_bounds__(1024) void norm_bwd_part_kernel(
+template <typename T, int W, int NT>
+__global__ __launch_bounds__(NT) void norm_bwd_part_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
     const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats, int act,
     float* __restrict__ part) {
@@ -530,8 +562,8 @@ __global__ __launch_bounds__(1024) void norm_rows_kernel(const float* __restrict
   }
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(1024) void norm_bwd_apply_kernel(
+template <typename T, int W, int NT>
+__global__ __launch_bounds__(NT) void norm_bwd_apply_kernel(
     NormShape sh, const T* __restrict__ x, int64_t ld, const T* __restrict__ dy,
     const T* __restrict__ w, const T* __restrict__ b, const float* __restrict__ stats,
     const float* __restrict__ chain_sums, int act, T* __restrict__ dx) {
@@ -576,11 +608,24 @@ constexpr int kOneRows = 1024, kOneChains = 512;
 bool by_chain(int max_len, int n_whole) { return max_len <= kOneRows || n_whole >= kOneChains; }
 
 // Threads of a workgroup: a column of every vector of a row, and at least 4
-// rows of them where a row has no more than 256 vectors.
-int norm_threads(int tc) { return tc <= 64 ? 256 : 1024; }
+// rows of them where a row has no more than 256 vectors; twice as many where
+// few chains leave compute units idle and one takes more than a step (192
+// chains of up to 80 beads x 128 in fp32, both directions: 25 us against 31;
+// 2048 of up to 268 in bf16: 257 against 199).
+int norm_threads(const NormArgs& a, int W) {
+  const int tc = a.C / W;
+  if (tc > 64) return 1024;
+  return by_chain(a.max_len, a.n_whole) && a.n_whole <= 256 && a.max_len > 4 * (256 / tc)
+             ? 512
+             : 256;
+}
+
+// Sums a vector of W channels: one for each of its groups where they divide
+// it, or one where it lies in one, or else one a channel.
+int vector_sums(int W, int P) { return P % W == 0 ? 1 : W % P == 0 ? W / P : W; }
 
 template <int W>
-NormShape norm_shape(const NormArgs& a, bool one) {
+NormShape norm_shape(const NormArgs& a, bool one, int nt) {
   NormShape sh;
   sh.tiles = one ? a.whole : a.tiles;
   sh.n_tiles = one ? a.n_whole : a.n_tiles;
@@ -588,7 +633,7 @@ NormShape norm_shape(const NormArgs& a, bool one) {
   sh.C = a.C;
   sh.G = a.G;
   sh.TC = a.C / W;
-  sh.TR = norm_threads(sh.TC) / sh.TC;
+  sh.TR = nt / sh.TC;
   sh.chains = a.chains;
   return sh;
 }
@@ -603,44 +648,44 @@ int allow(F f, unsigned lds) {
   return MLCG_OK;
 }
 
-template <typename T, int W>
+template <typename T, int W, int K, int NT>
 int norm_fwd(const NormArgs& a, void* y, float* stats, float* ws, hipStream_t s) {
-  const bool one = by_chain(a.max_len, a.n_whole), grouped = (a.C / a.G) % W == 0;
-  const NormShape sh = norm_shape<W>(a, one);
-  const int nt = norm_threads(sh.TC), k = grouped ? 1 : W;
-  const unsigned lds = (unsigned)((3 * sh.G + (nt + sh.TC) * 2 * k) * sizeof(float));
+  const bool one = by_chain(a.max_len, a.n_whole);
+  const NormShape sh = norm_shape<W>(a, one, NT);
+  constexpr int nt = NT;
+  const unsigned lds = (unsigned)((3 * sh.G + (nt + sh.TC) * 2 * K) * sizeof(float));
   const T *x = (const T*)a.x, *w = (const T*)a.w, *b = (const T*)a.b;
   if (one) {
-    auto f = grouped ? norm_chain_kernel<T, W, true> : norm_chain_kernel<T, W, false>;
+    auto f = norm_chain_kernel<T, W, K, NT>;
     if (int e = allow(f, lds)) return e;
     hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, w, b, a.eps, a.act,
                        (T*)y, stats);
     return mlcg_launch_status();
   }
   float4* part = reinterpret_cast<float4*>(ws);
-  auto f = grouped ? norm_part_kernel<T, W, true> : norm_part_kernel<T, W, false>;
+  auto f = norm_part_kernel<T, W, K, NT>;
   if (int e = allow(f, lds)) return e;
   hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, part);
   hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)sh.chains, sh.G), dim3(256), 0, s, sh,
                      a.first_tile, part, a.eps, stats);
-  hipLaunchKernelGGL((norm_apply_kernel<T, W>), dim3(sh.n_tiles), dim3(nt), 0, s, sh, x, a.ld, w,
+  hipLaunchKernelGGL((norm_apply_kernel<T, W, NT>), dim3(sh.n_tiles), dim3(nt), 0, s, sh, x, a.ld, w,
                      b, stats, a.act, (T*)y);
   return mlcg_launch_status();
 }
 
-template <typename T, int W>
+template <typename T, int W, int K, int NT>
 int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* ws,
              hipStream_t s) {
   const bool one = by_chain(a.max_len, a.n_whole);
-  const NormShape sh = norm_shape<W>(a, one);
-  const int nt = norm_threads(sh.TC);
+  const NormShape sh = norm_shape<W>(a, one, NT);
+  constexpr int nt = NT;
   const T *x = (const T*)a.x, *dy = (const T*)a.dy, *w = (const T*)a.w, *b = (const T*)a.b;
   const unsigned cols = mlcg_div_up(2 * sh.C, 8);
   if (one) {
-    const unsigned lds = (unsigned)((nt * 2 * W + 4 * sh.C + 2 * sh.G) * sizeof(float));
-    auto f = norm_chain_bwd_kernel<T, W>;
+    const unsigned lds = (unsigned)((nt * 2 * W + 2 * sh.C + 2 * sh.G) * sizeof(float));
+    auto f = norm_chain_bwd_kernel<T, W, K, NT>;
     if (int e = allow(f, lds)) return e;
-    const int groups = std::min(sh.n_tiles, 1024);
+    const int groups = std::min(sh.n_tiles, 2048);
     hipLaunchKernelGGL(f, dim3(groups), dim3(nt), lds, s, sh, x, a.ld, dy, w, b, stats, a.act,
                        (T*)dx, ws);
     hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, ws, 2 * sh.C, nullptr,
@@ -648,7 +693,7 @@ int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* 
     return mlcg_launch_status();
   }
   const unsigned lds = (unsigned)((nt * 2 * W + 2 * sh.C) * sizeof(float));
-  auto f = norm_bwd_part_kernel<T, W>;
+  auto f = norm_bwd_part_kernel<T, W, NT>;
   if (int e = allow(f, lds)) return e;
   float* part = ws;
   float* chain_sums = ws + (int64_t)sh.n_tiles * 2 * sh.C;
@@ -656,7 +701,7 @@ int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* 
                      part);
   hipLaunchKernelGGL(norm_rows_kernel<float>, dim3(cols, (unsigned)sh.chains), dim3(1024), 0, s,
                      part, 2 * sh.C, a.first_tile, sh.tiles, sh.size, 0, chain_sums);
-  hipLaunchKernelGGL((norm_bwd_apply_kernel<T, W>), dim3(sh.n_tiles), dim3(nt),
+  hipLaunchKernelGGL((norm_bwd_apply_kernel<T, W, NT>), dim3(sh.n_tiles), dim3(nt),
                      (unsigned)((2 * sh.C + 2 * sh.G) * sizeof(float)), s, sh, x, a.ld, dy, w, b,
                      stats, chain_sums, a.act, (T*)dx);
   hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, chain_sums, 2 * sh.C,
@@ -679,6 +724,23 @@ int by_type(int dtype, F f) {
   return f(__bf16{});
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+template <int W, typename F>
+int by_shape(const NormArgs& a, bool vec, F f) {
+  auto threads = [&](auto w, auto k) {
+    const int nt = norm_threads(a, decltype(w)::value);
+    return nt == 256 ? f(w, k, Int<256>()) : nt == 512 ? f(w, k, Int<512>()) : f(w, k, Int<1024>());
+  };
+  if (!vec) return threads(Int<1>(), Int<1>());
+  const int k = vector_sums(W, a.C / a.G);
+  if (k == 1) return threads(Int<W>(), Int<1>());
+  if (k == 2) return threads(Int<W>(), Int<2>());
+  if (W == 8 && k == 4) return threads(Int<W>(), Int<4>());
+  return threads(Int<W>(), Int<W>());
+}
+
 bool norm_args_ok(const NormArgs& a, int64_t rows, int64_t n_tiles, int64_t n_whole,
                   int64_t max_len, int dtype) {
   const int64_t most = int64_t(1) << 31;
@@ -697,7 +759,7 @@ extern "C" int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t cha
   if (n_tiles < 0 || chains < 0 || n_whole < 0 || max_len < 0 || width < 1 || groups < 1)
     return -1;
   if (max_len <= kOneRows || n_whole >= kOneChains)
-    return backward ? 2 * std::min<int64_t>(n_whole, 1024) * width : 0;
+    return backward ? 2 * std::min<int64_t>(n_whole, 2048) * width : 0;
   return backward ? 2 * (n_tiles + chains) * width : 4 * n_tiles * groups;
 }
 
@@ -719,8 +781,12 @@ extern "C" int mlcg_group_norm_act(const void* x, int64_t ld, int64_t rows, int 
   hipStream_t s = mlcg_stream(stream);
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    return norm_vec<T>(a, y) ? norm_fwd<T, 16 / (int)sizeof(T)>(a, y, stats, workspace, s)
-                             : norm_fwd<T, 1>(a, y, stats, workspace, s);
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool vec = norm_vec<T>(a, y);
+    return by_shape<W>(a, vec, [&](auto w, auto k, auto nt) {
+      return norm_fwd<T, decltype(w)::value, decltype(k)::value, decltype(nt)::value>(
+          a, y, stats, workspace, s);
+    });
   });
 }
 
@@ -740,8 +806,11 @@ extern "C" int mlcg_group_norm_act_backward(
   hipStream_t s = mlcg_stream(stream);
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    return norm_vec<T>(a, grad_x)
-               ? norm_bwd<T, 16 / (int)sizeof(T)>(a, stats, grad_x, grad_bias_weight, workspace, s)
-               : norm_bwd<T, 1>(a, stats, grad_x, grad_bias_weight, workspace, s);
+    constexpr int W = 16 / (int)sizeof(T);
+    const bool vec = norm_vec<T>(a, grad_x);
+    return by_shape<W>(a, vec, [&](auto w, auto k, auto nt) {
+      return norm_bwd<T, decltype(w)::value, decltype(k)::value, decltype(nt)::value>(
+          a, stats, grad_x, grad_bias_weight, workspace, s);
+    });
   });
 }
