@@ -1,4 +1,6 @@
 from .activations import ShiftedSoftplus
+from .chain import (ChainAttention, ChainEmbedding, ChainEncoder, ChainEncoderLayer,
+                    CounterDropout, GroupNormAct, chain_attention, dropout_add, group_norm_act)
 from .cutoff import CosineCutoff, IdentityCutoff
 from .gradients import EnergyOut, GradientsOut, SumOut
 from .losses import EnergyMSE, ForceMSE, ForceRMSE, Loss
@@ -9,11 +11,12 @@ from .prior import (Dihedral, FourierSeries, Harmonic, HarmonicAngles, HarmonicB
 from .radial_basis import ExpNormalBasis, GaussianBasis
 from .schnet import CFConv, InteractionBlock, SchNet, StandardSchNet
 
-from .chain import chain_attention, dropout_add, group_norm_act
-
-__all__ = ["chain_attention", "dropout_add", "group_norm_act", "ShiftedSoftplus", "CosineCutoff", "IdentityCutoff", "EnergyOut", "GradientsOut",
+__all__ = ["ShiftedSoftplus", "CosineCutoff", "IdentityCutoff", "EnergyOut", "GradientsOut",
            "SumOut", "EnergyMSE", "ForceMSE", "ForceRMSE", "Loss", "MLP",
            "init_xavier_uniform", "GaussianBasis", "ExpNormalBasis", "CFConv",
            "InteractionBlock", "SchNet", "StandardSchNet", "Harmonic", "HarmonicBonds",
            "HarmonicAngles", "FourierSeries", "Dihedral", "Repulsion", "StaticHarmonicBonds",
-           "StaticHarmonicAngles", "StaticDihedral", "StaticRepulsion"]
+           "StaticHarmonicAngles", "StaticDihedral", "StaticRepulsion",
+           "ChainAttention", "ChainEmbedding", "ChainEncoder", "ChainEncoderLayer",
+           "CounterDropout", "GroupNormAct", "chain_attention", "dropout_add",
+           "group_norm_act"]

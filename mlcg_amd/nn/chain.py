@@ -16,7 +16,6 @@ take GPU tensors only, and they are differentiable once.
 
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -112,3 +111,208 @@ def dropout_add(x: torch.Tensor, p: float, seed: int, step,
     if not _needs_grad(x, residual):
         return ops.dropout_add(x, p, seed, step, residual)
     return _Dropout.apply(x, residual, p, seed, step)
+
+
+class ChainAttention(torch.nn.Module):
+    """Attention of every bead to the present beads of its chain: a projection
+    to queries, keys and values (``kv_heads`` of the latter serve ``heads``
+    query heads), a learned bias by relative position, a projection back.
+
+    forward(x [S, width], chains, keep=None, positions=None) -> [S, width]."""
+
+    def __init__(self, width: int, heads: int, kv_heads: Optional[int] = None,
+                 num_buckets: int = 32, reach: int = 128, kind: str = "log"):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if width % heads != 0 or not 1 <= kv_heads <= heads or heads % kv_heads != 0:
+            raise ValueError(f"{width} channels cannot be split into {heads} heads with "
+                             f"{kv_heads} key/value heads")
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, width // heads
+        self.qkv = torch.nn.Linear(width, (heads + 2 * kv_heads) * self.dim)
+        self.out = torch.nn.Linear(width, width)
+        self.bias_table = torch.nn.Parameter(torch.zeros(num_buckets, heads))
+        buckets = ops.relative_buckets(num_buckets, reach, kind, device="cpu")
+        self.num_buckets, self.reach = num_buckets, reach
+        for name in ("bucket_of", "order", "first"):
+            self.register_buffer(name, getattr(buckets, name), persistent=False)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        init_xavier_uniform(self.qkv)
+        init_xavier_uniform(self.out)
+        torch.nn.init.zeros_(self.bias_table)
+
+    @property
+    def buckets(self) -> ops.RelativeBuckets:
+        return ops.RelativeBuckets(num_buckets=self.num_buckets, reach=self.reach,
+                                   bucket_of=self.bucket_of, order=self.order, first=self.first)
+
+    def forward(self, x, chains, keep=None, positions=None):
+        h, kv, d = self.heads, self.kv_heads, self.dim
+        qkv = self.qkv(x).view(-1, h + 2 * kv, d)
+        y = chain_attention(qkv[:, :h], qkv[:, h:h + kv], qkv[:, h + kv:], self.bias_table,
+                            self.buckets, chains, keep=keep, positions=positions)
+        return self.out(y.reshape(-1, h * d))
+
+
+class GroupNormAct(torch.nn.Module):
+    """Group norm of every chain with an affine map by channel and an
+    activation: forward(x [S, width], chains) -> [S, width]."""
+
+    def __init__(self, groups: int, width: int, act: str = "none", eps: float = 1e-5):
+        super().__init__()
+        if width % groups != 0 or act not in ops.CHAIN_ACTS:
+            raise ValueError(f"GroupNormAct: {width} channels in {groups} groups, act {act!r}")
+        self.groups, self.act, self.eps = groups, act, eps
+        self.weight = torch.nn.Parameter(torch.ones(width))
+        self.bias = torch.nn.Parameter(torch.zeros(width))
+
+    def reset_parameters(self):
+        torch.nn.init.ones_(self.weight)
+        torch.nn.init.zeros_(self.bias)
+
+    def forward(self, x, chains):
+        return group_norm_act(x, self.weight, self.bias, self.groups, chains, self.eps, self.act)
+
+
+class CounterDropout(torch.nn.Module):
+    """residual + dropout(x), the mask drawn from (seed, step) and never
+    stored.  The step is a buffer that every training call moves on, on the
+    device: a recorded training step draws a new mask on every replay, and a
+    run resumed from a checkpoint goes on with the next one.  Modules of one
+    model need seeds of their own.  In eval mode: residual + x."""
+
+    def __init__(self, p: float, seed: int):
+        super().__init__()
+        ops.dropout_threshold(p)
+        self.p, self.seed = p, seed
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x
+        # the backward pass reads the value that this call used
+        step = self.step.add_(1).clone()
+        return dropout_add(x, self.p, self.seed, step, residual)
+
+
+class ChainEncoderLayer(torch.nn.Module):
+    """x + drop(attention(norm(x))), then x + drop(lin(act(norm(lin(x)))))."""
+
+    def __init__(self, width: int, heads: int, kv_heads: Optional[int] = None,
+                 hidden: Optional[int] = None, norm_groups: int = 8, act: str = "silu",
+                 dropout: float = 0.0, seed: int = 0, num_buckets: int = 32, reach: int = 128,
+                 kind: str = "log"):
+        super().__init__()
+        hidden = 2 * width if hidden is None else hidden
+        self.norm1 = GroupNormAct(norm_groups, width)
+        self.attention = ChainAttention(width, heads, kv_heads, num_buckets, reach, kind)
+        self.drop1 = CounterDropout(dropout, 2 * seed)
+        self.lin1 = torch.nn.Linear(width, hidden)
+        self.norm2 = GroupNormAct(norm_groups, hidden, act)
+        self.lin2 = torch.nn.Linear(hidden, width)
+        self.drop2 = CounterDropout(dropout, 2 * seed + 1)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        for m in (self.norm1, self.attention, self.norm2):
+            m.reset_parameters()
+        init_xavier_uniform(self.lin1)
+        init_xavier_uniform(self.lin2)
+
+    def forward(self, x, chains, keep=None, positions=None):
+        y = self.attention(self.norm1(x, chains), chains, keep, positions)
+        x = self.drop1(y, residual=x)
+        y = self.lin2(self.norm2(self.lin1(x), chains))
+        return self.drop2(y, residual=x)
+
+
+class ChainEncoder(torch.nn.Module):
+    """ChainEncoderLayers in a row: features [S, width] of the beads of all
+    chains to features that depend on their place in the sequence.  ``seed``
+    begins the layers' dropout streams."""
+
+    def __init__(self, width: int, layers: int, heads: int, seed: int = 0, **layer_options):
+        super().__init__()
+        if layers < 1:
+            raise ValueError("At least one encoder layer must be specified")
+        self.layers = torch.nn.ModuleList(
+            ChainEncoderLayer(width, heads, seed=seed + i, **layer_options)
+            for i in range(layers))
+
+    def reset_parameters(self):
+        for layer in self.layers:
+            layer.reset_parameters()
+
+    def forward(self, x, chains, keep=None, positions=None):
+        for layer in self.layers:
+            x = layer(x, chains, keep, positions)
+        return x
+
+
+class ChainEmbedding(torch.nn.Module):
+    """An embedding layer for SchNet whose rows are the beads (sites) of given
+    molecules in place of bead types: row s is the encoder's feature of site s
+    in its chain, made from the embeddings of the sites' types.  A batch's
+    ``atom_types`` then holds the sites (0 .. S - 1) its beads are.
+
+    types [S]: the sites' bead types, chain after chain; lengths: the beads of
+    every chain; keep [S] bool: sites without a resolved structure; positions
+    [S]: residue numbers (the index in the chain by default).
+
+    The table is made anew in every forward pass, as training needs it;
+    ``as_embedding()`` gives it as a plain Embedding for simulations."""
+
+    def __init__(self, embedding_size: int, width: int, encoder: torch.nn.Module, types, lengths,
+                 keep=None, positions=None):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.empty(embedding_size, width))
+        self.encoder = encoder
+        self.register_buffer("types", torch.as_tensor(types, dtype=torch.int64))
+        self.register_buffer("keep", None if keep is None else
+                             torch.as_tensor(keep, dtype=torch.bool))
+        self.register_buffer("positions", None if positions is None else
+                             torch.as_tensor(positions, dtype=torch.int32))
+        self.lengths = tuple(int(n) for n in lengths)
+        n = self.types.numel()
+        if self.types.dim() != 1 or sum(self.lengths) != n or any(
+                t is not None and tuple(t.shape) != (n,) for t in (self.keep, self.positions)):
+            raise ValueError("types, keep and positions hold one value for every bead of the "
+                             "chains")
+        if n and not 0 <= int(self.types.min()) <= int(self.types.max()) < embedding_size:
+            raise ValueError("a site's type lies outside the embedding table")
+        torch.nn.init.normal_(self.weight)
+
+    def reset_parameters(self):
+        torch.nn.init.normal_(self.weight)
+        self.encoder.reset_parameters()
+
+    @property
+    def chains(self) -> ops.ChainLayout:
+        """The chains' layout, on the device of the weights."""
+        made = self.__dict__.get("_layout")
+        if made is None or made.device != self.weight.device:
+            made = self.__dict__["_layout"] = ops.chain_layout(self.lengths, self.weight.device)
+        return made
+
+    def __getstate__(self):
+        state = dict(self.__dict__)
+        state.pop("_layout", None)  # of one device, and made again where it is needed
+        return state
+
+    def table(self) -> torch.Tensor:
+        x = torch.nn.functional.embedding(self.types, self.weight)
+        return self.encoder(x, self.chains, self.keep, self.positions)
+
+    def forward(self, sites: torch.Tensor) -> torch.Tensor:
+        return self.table().index_select(0, sites)
+
+    @torch.no_grad()
+    def as_embedding(self) -> torch.nn.Embedding:
+        """The present table as a plain embedding layer (without dropout)."""
+        training = self.training
+        try:
+            return torch.nn.Embedding.from_pretrained(self.eval().table().detach().clone(),
+                                                      freeze=False)
+        finally:
+            self.train(training)

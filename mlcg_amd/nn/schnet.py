@@ -22,6 +22,7 @@ from ..data._keys import ENERGY_KEY
 from ..neighbor_list.neighbor_list import atomic_data2neighbor_list, validate_neighborlist
 from . import _fused
 from .activations import activation_id
+from .chain import ChainEmbedding
 from .cutoff import CosineCutoff, IdentityCutoff
 from .mlp import MLP, init_xavier_uniform
 from .radial_basis import ExpNormalBasis, GaussianBasis
@@ -250,7 +251,7 @@ class SchNet(torch.nn.Module):
         if bt is None or bt[1].numel() != (bt[0].numel() if isinstance(rbf, ExpNormalBasis)
                                            else 1):
             return None
-        if not isinstance(self.embedding_layer, torch.nn.Embedding):
+        if not isinstance(self.embedding_layer, (torch.nn.Embedding, ChainEmbedding)):
             return None
         rc = rbf.cutoff
         if not isinstance(rc, (IdentityCutoff, CosineCutoff)):
@@ -323,7 +324,9 @@ class SchNet(torch.nn.Module):
         lins = self.output_network.linears()
         rbf = self.rbf_layer
         basis = list(_basis_tensors(rbf)) if getattr(rbf, "trainable", False) else []
-        return _fused.Params(emb=self.embedding_layer.weight, blocks=blocks,
+        emb = self.embedding_layer
+        table = emb.table() if isinstance(emb, ChainEmbedding) else emb.weight
+        return _fused.Params(emb=table, blocks=blocks,
                              out_w=[lin.weight for lin in lins],
                              out_b=[lin.bias for lin in lins], basis=basis)
 
