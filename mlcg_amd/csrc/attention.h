@@ -72,6 +72,10 @@ struct AttnArgs {
   float scale;
 };
 
+// Whether positions are given: known when the kernel is built, or (kEither, in
+// the form without 16-byte loads) when it runs.
+enum { kIndex = 0, kGiven = 1, kEither = 2 };
+
 struct AttnGrads {
   void *dq, *dk, *dv, *dtable;
   float* ws;
@@ -88,10 +92,10 @@ int attn_backward(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s);
 
 namespace {
 
-// rows of a part of a staged tile; they are used 32 at a time
-template <typename T>
+// rows of a part of a staged tile: 64, or 32 of the widest
+template <typename T, int DP>
 constexpr int part_rows() {
-  return sizeof(T) == 2 ? 64 : 32;
+  return sizeof(T) * DP <= 128 ? 64 : 32;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -275,11 +279,20 @@ __device__ __forceinline__ int offset_cell(int pj, int pi, int reach) {
   return min(max(__builtin_elementwise_sub_sat(pj, pi), -reach), reach) + reach + kAttnSpan;
 }
 
+// v, rounded to fp32 where it is a product, as T.  hipcc may otherwise fold a
+// product into the conversion to fp16 (one rounding in place of two) in one
+// form of a kernel and not in another, and equal calls differ by a bit.
+template <typename T>
+__device__ __forceinline__ T round_to(float v) {
+  if constexpr (std::is_same<T, _Float16>::value) asm("" : "+v"(v));
+  return (T)v;
+}
+
 template <typename T>
 __device__ __forceinline__ v8<T> pack8(const float* p) {
   v8<T> r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = (T)p[e];
+  for (int e = 0; e < 8; ++e) r[e] = round_to<T>(p[e]);
   return r;
 }
 
@@ -346,7 +359,7 @@ __device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32
       const int d = 32 * n + 8 * a + 4 * g;
       v4<T> o;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = (T)(acc[n][4 * a + c] * f);
+      for (int c = 0; c < 4; ++c) o[c] = round_to<T>(acc[n][4 * a + c] * f);
       if constexpr (VEC) {
         if (d < dim) *reinterpret_cast<v4<T>*>(dst + d) = o;
       } else {
@@ -392,12 +405,18 @@ __device__ __forceinline__ int block_side(int d_min, int d_max, int R) {
   return d_min >= R ? 1 : d_max <= -R ? -1 : 0;
 }
 
+template <int POS>
+__device__ __forceinline__ bool given_positions(const AttnArgs& a) {
+  return POS == kEither ? a.pos != nullptr : POS == kGiven;
+}
+
 // What stands for the keys of a tile in LDS: the value that their products'
 // sums begin with (0, or for an absent key what makes the logit -inf), and
 // their positions.  Thread i loads row i's.
 struct KeyInfo {
   float cap;
   int pos;
+  template <int POS>
   __device__ __forceinline__ void load(const AttnArgs& a, const int4& t, int k0, int rows) {
     const int i = threadIdx.x;
     cap = logit_factor(a) > 0.0f ? -INFINITY : INFINITY;
@@ -405,13 +424,14 @@ struct KeyInfo {
     if (i < rows && k0 + i < t.y) {
       const int64_t row = (int64_t)t.x + k0 + i;
       if (!a.keep || a.keep[row]) cap = 0.0f;
-      if (a.pos) pos = a.pos[row];
+      if (given_positions<POS>(a)) pos = a.pos[row];
     }
   }
+  template <int POS>
   __device__ __forceinline__ void put(int rows, float* caps, int* kpos) const {
     if ((int)threadIdx.x < rows) {
       caps[threadIdx.x] = cap;
-      kpos[threadIdx.x] = pos;
+      if (POS != kIndex) kpos[threadIdx.x] = pos;
     }
   }
 };
@@ -421,10 +441,10 @@ struct KeyInfo {
 struct QueryPlace {
   int first, mine, pos, lo, hi;
   bool ok;
-  __device__ __forceinline__ QueryPlace(const AttnArgs& a, const int4& t, int begin)
+  __device__ __forceinline__ QueryPlace(const AttnArgs& a, bool given, const int4& t, int begin)
       : first(begin), mine(begin + (threadIdx.x & 31)), pos(0), lo(0), hi(0) {
     ok = mine < t.y;
-    if (a.pos) {
+    if (given) {
       pos = a.pos[(int64_t)t.x + min(mine, t.y - 1)];
       lo = wave_min(pos);
       hi = wave_max(pos);
@@ -434,7 +454,7 @@ struct QueryPlace {
 
 // The logits (base 2) less `shift` of 32 N keys from kb on (rows) and the
 // wave's queries (lanes); returns the keys' side.
-template <int N>
+template <int N, int POS>
 __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)[N],
                                             const float* ext, const float* cap, const int* kpos,
                                             int kb, const QueryPlace& q, float shift,
@@ -443,7 +463,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
   const float c = logit_factor(a);
   const int R = a.reach;
   int side;
-  if (a.pos) {
+  if (given_positions<POS>(a)) {
     const int kp = kpos[lane % (32 * N)];
     const bool absent = cap[lane % (32 * N)] != 0.0f;
     side = __all(absent || __builtin_elementwise_sub_sat(kp, q.hi) >= R)    ? 1
@@ -456,7 +476,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
     const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
-  } else if (a.pos) {
+  } else if (given_positions<POS>(a)) {
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i)
       x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - shift);
@@ -476,7 +496,7 @@ constexpr int waves_for(int values) {
 
 template <typename T, int DP, int NQ, int NK>
 struct FwdLds {
-  static constexpr int KS = part_rows<T>() * NK;
+  static constexpr int KS = part_rows<T, DP>() * NK;
   T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
@@ -489,10 +509,10 @@ constexpr int fwd_waves() {
   return waves_for(DP * (int)sizeof(T) / 8 + DP / 2);
 }
 
-template <typename T, int DP, int NQ, int NK, bool VEC>
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_kernel(
     AttnArgs a, T* __restrict__ out) {
-  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
+  constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = FwdLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -512,9 +532,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_k
   ks.load(kbase, t.y, a.dim);
   vs.load(vbase, t.y, a.dim);
   uint32_t absent = ks.find_absent(keep, t.y);
-  info.load(a, t, 0, KS);
+  info.template load<POS>(a, t, 0, KS);
 
-  const QueryPlace qi(a, t, t.z + kAttnQ * wq);
+  const bool given = given_positions<POS>(a);
+  const QueryPlace qi(a, given, t, t.z + kAttnQ * wq);
   const T* q = (const T*)a.q + ((int64_t)t.x + qi.mine) * a.q_row + head * a.q_head;
   v8<T> qf[DP / 16];
 #pragma unroll
@@ -532,13 +553,13 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_k
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.put(KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
       vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
       if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
-      info.load(a, t, kn, KS);
+      info.template load<POS>(a, t, kn, KS);
     }
     __syncthreads();
   };
@@ -554,7 +575,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_k
     load_rows<N>(cap, s);
     row_product<T, DP, N>(L.k[buf] + RT * wk * DP, qf, s);
     float x[16 * N];
-    query_logits<N>(a, s, ext, cap, L.kpos[buf] + RT * wk, kb, qi, base, x);
+    query_logits<N, POS>(a, s, ext, cap, L.kpos[buf] + RT * wk, kb, qi, base, x);
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, x[i]);
@@ -710,7 +731,8 @@ struct OffsetInts {
   }
 };
 
-// The waves' sums by offset (dd, one array of `cells` a wave) to buckets.
+// The waves' sums by offset (dd, one array of `cells` a wave and one more) to
+// buckets.
 template <int NT>
 __device__ __forceinline__ void flush_offsets(const AttnArgs& a, float* dd, int cells,
                                               const int32_t* order, const int32_t* first,
@@ -738,10 +760,20 @@ __device__ __forceinline__ void flush_offsets(const AttnArgs& a, float* dd, int 
     }
   }
   __syncthreads();
-  for (int b = tid; b < a.buckets; b += NT) {
+  // by bucket in the second array (the ends' cells are free now), all loads of
+  // the order at once; then 8 lanes a bucket
+  const int n = 2 * a.reach + 1;
+  float* sorted = dd + cells;
+  for (int i = tid; i < n; i += NT) sorted[i] = dd[kAttnSpan + order[i]];
+  __syncthreads();
+  for (int b = tid >> 3; b < a.buckets; b += NT / 8) {
+    const int end = first[b + 1];
     float t = 0.0f;
-    for (int i = first[b]; i < first[b + 1]; ++i) t += dd[kAttnSpan + order[i]];
-    out[b] = t;
+    for (int i = first[b] + (tid & 7); i < end; i += 8) t += sorted[i];
+    t += __shfl_xor(t, 1, 64);
+    t += __shfl_xor(t, 2, 64);
+    t += __shfl_xor(t, 4, 64);
+    if ((tid & 7) == 0) out[b] = t;
   }
 }
 
@@ -753,7 +785,7 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
 
 template <typename T, int DP, int NQ, int NK>
 struct DqLds {
-  static constexpr int KS = part_rows<T>() * NK;
+  static constexpr int KS = part_rows<T, DP>() * NK;
   T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
@@ -768,17 +800,17 @@ constexpr int dq_waves() {
 
 // dq, delta and the workgroup's part of the table's gradient; lanes are
 // queries as in the forward pass.
-template <typename T, int DP, int NQ, int NK, bool VEC>
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
     const int32_t* __restrict__ order, const int32_t* __restrict__ first,
     float* __restrict__ dtable_part) {
-  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
+  constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
   using Lds = DqLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
   const int R = a.reach, cells = 2 * (R + kAttnSpan) + 1;
-  const int sf = scratch_floats(R, a.pos != nullptr);
+  const int sf = scratch_floats(R, given_positions<POS>(a));
   float* ext = L.rest + NW * sf;
   float* dd = ext + cells;
 
@@ -803,9 +835,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   ks.load(kbase, t.y, a.dim);
   vs.load(vbase, t.y, a.dim);
   uint32_t absent = ks.find_absent(keep, t.y);
-  info.load(a, t, 0, KS);
+  info.template load<POS>(a, t, 0, KS);
 
-  const QueryPlace qi(a, t, t.z + kAttnQ * wq);
+  const bool given = given_positions<POS>(a);
+  const QueryPlace qi(a, given, t, t.z + kAttnQ * wq);
   const int64_t row = (int64_t)t.x + qi.mine;
   const T* q = (const T*)a.q + row * a.q_row + head * a.q_head;
   const int64_t flat = (row * a.heads + head) * a.dim;
@@ -826,7 +859,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   float* mine = dd + wave * cells;
   float* scratch = L.rest + wave * sf;
   OffsetInts ints;
-  if (a.pos)
+  if (given)
     ints.init(reinterpret_cast<int*>(scratch), R, mine + kAttnSpan);
   else
     for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
@@ -845,13 +878,13 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.put(KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
       vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
       if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
-      info.load(a, t, kn, KS);
+      info.template load<POS>(a, t, kn, KS);
     }
     __syncthreads();
   };
@@ -868,7 +901,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     load_rows<N>(cap, s);
     row_product<T, DP, N>(kt, qf, s);
     float x[16 * N];
-    const int side = query_logits<N>(a, s, ext, cap, kpos, kb, qi, lse, x);
+    const int side = query_logits<N, POS>(a, s, ext, cap, kpos, kb, qi, lse, x);
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] = minus_delta;
     row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, s);  // dP - delta
@@ -883,7 +916,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
         far_hi += all;
       else
         far_lo += all;
-    } else if (!a.pos) {
+    } else if (!given) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
         if (kb + 32 * n < t.y)
@@ -902,7 +935,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     }
     column_product<T, DP, N>(kt, x, acc);
   }
-  if (a.pos) ints.flush();
+  if (given) ints.flush();
   far_lo = mlcg_wave_sum(far_lo);
   far_hi = mlcg_wave_sum(far_hi);
   if (lane == 0) {
@@ -919,7 +952,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
 
 template <typename T, int DP, int NQ, int NK>
 struct DkvLds {
-  static constexpr int KS = part_rows<T>() * NK;
+  static constexpr int KS = part_rows<T, DP>() * NK;
   T q[2][KS * DP], g[2][KS * DP];
   float lse[2][KS], delta[2][KS];
   int qpos[2][KS];
@@ -934,10 +967,10 @@ constexpr int dkv_waves() {
 
 // dk and dv; lanes are keys, the tiles hold queries.  The query heads that
 // share a key/value head are taken one after the other.
-template <typename T, int DP, int NQ, int NK, bool VEC>
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
     AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
-  constexpr int RT = part_rows<T>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
+  constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = DkvLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -974,6 +1007,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
   qs.init((int)a.q_row, a.dim);
   gs.init(a.heads * a.dim, a.dim);
   uint32_t absent = 0;
+  const bool given = given_positions<POS>(a);
   float lse_n = INFINITY, delta_n = 0.0f;
   int pos_n = 0;
   auto load = [&](int head, int q0) {
@@ -987,7 +1021,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     if (i < KS && q0 + i < t.y) {
       lse_n = a.lse[head * a.beads + row0 + i];
       delta_n = delta[head * a.beads + row0 + i];
-      if (a.pos) pos_n = a.pos[row0 + i];
+      if (given) pos_n = a.pos[row0 + i];
     }
   };
   load(kv * a.group, 0);
@@ -1001,7 +1035,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     vf[i] = load8<T, VEC>(v, 16 * i + 8 * g, k_ok, a.dim);
   }
   int kp = 0, klo = 0, khi = 0;
-  if (a.pos) {
+  if (given) {
     kp = a.pos[(int64_t)t.x + min(ki, t.y - 1)];
     klo = wave_min(kp);
     khi = wave_max(kp);
@@ -1020,7 +1054,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     if ((int)threadIdx.x < KS) {
       L.lse[buf][threadIdx.x] = -lse_n / c;
       L.delta[buf][threadIdx.x] = -delta_n;
-      L.qpos[buf][threadIdx.x] = pos_n;
+      if (POS != kIndex) L.qpos[buf][threadIdx.x] = pos_n;
     }
     if (q0 + KS < t.y)
       load(kv * a.group + h, q0 + KS);
@@ -1046,7 +1080,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
       row_product<T, DP, N>(qt, kf, s);
       float x[16 * N];
       int side;
-      if (a.pos) {
+      if (given) {
         const int qp = qpos[lane % RT];
         const bool past = qb + lane % RT >= t.y;
         side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
@@ -1059,7 +1093,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
         const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
 #pragma unroll
         for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
-      } else if (a.pos) {
+      } else if (given) {
 #pragma unroll
         for (int i = 0; i < 16 * N; ++i)
           x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kp, qpos[acc_row(i, g)], R)]);
@@ -1121,26 +1155,26 @@ int allow_lds(const void* f, unsigned bytes) {
              : MLCG_ERR_LAUNCH;
 }
 
-template <typename T, int DP, int NQ, int NK, bool VEC>
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 int launch_fwd(const AttnArgs& a, void* out, hipStream_t s) {
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds = sizeof(FwdLds<T, DP, NQ, NK>) + 4 * cells;
-  auto f = attn_fwd_kernel<T, DP, NQ, NK, VEC>;
+  auto f = attn_fwd_kernel<T, DP, NQ, NK, VEC, POS>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
   hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NQ * NK), lds, s, a,
                      (T*)out);
   return mlcg_launch_status();
 }
 
-template <typename T, int DP, int NQ, int NK, bool VEC>
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 int launch_bwd(const AttnArgs& a, const AttnGrads& o, hipStream_t s) {
   constexpr unsigned NW = NQ * NK;
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds1 = sizeof(DqLds<T, DP, NQ, NK>) +
-                        4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 1) * cells);
+                        4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 2) * cells);
   const unsigned lds2 = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
-  auto f1 = attn_dq_kernel<T, DP, NQ, NK, VEC>;
-  auto f2 = attn_dkv_kernel<T, DP, NQ, NK, VEC>;
+  auto f1 = attn_dq_kernel<T, DP, NQ, NK, VEC, POS>;
+  auto f2 = attn_dkv_kernel<T, DP, NQ, NK, VEC, POS>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f1), lds1)) return e;
   if (int e = allow_lds(reinterpret_cast<const void*>(f2), lds2)) return e;
   float* delta = o.ws;
@@ -1165,28 +1199,31 @@ bool attn_vec(const AttnArgs& a, int size) {
   return true;
 }
 
-template <typename F>
-int by_shape(const AttnArgs& a, int shape, int size, F f) {
-  using std::bool_constant;
+template <int size_of, typename F>
+int by_shape(const AttnArgs& a, int shape, F f) {
   using std::integral_constant;
-  auto with = [&](auto dp, auto vec) {
-    using One = integral_constant<int, 1>;
-    switch (shape) {
-      case 11: return f(dp, One(), One(), vec);
-      case 21: return f(dp, integral_constant<int, 2>(), One(), vec);
-      case 41: return f(dp, integral_constant<int, 4>(), One(), vec);
-      case 22:
-        if constexpr (decltype(dp)::value <= 64)
-          return f(dp, integral_constant<int, 2>(), integral_constant<int, 2>(), vec);
-        break;
-      case 42:
-        if constexpr (decltype(dp)::value <= 64)
-          return f(dp, integral_constant<int, 4>(), integral_constant<int, 2>(), vec);
+  using One = integral_constant<int, 1>;
+  using Two = integral_constant<int, 2>;
+  using Four = integral_constant<int, 4>;
+  auto with = [&](auto dp, auto vec, auto pos) {
+    constexpr bool split = decltype(dp)::value <= 64;
+    const int nk = split ? shape % 10 : 1, nq = shape / 10;
+    if (nk == 2) {
+      if constexpr (split) {
+        if (nq == 2) return f(dp, Two(), Two(), vec, pos);
+        if (nq == 4) return f(dp, Four(), Two(), vec, pos);
+      }
     }
-    return (int)MLCG_ERR_UNSUPPORTED;
+    if (nq == 1) return f(dp, One(), One(), vec, pos);
+    if (nq == 2) return f(dp, Two(), One(), vec, pos);
+    return f(dp, Four(), One(), vec, pos);
   };
   auto either = [&](auto dp) {
-    return attn_vec(a, size) ? with(dp, bool_constant<true>()) : with(dp, bool_constant<false>());
+    using std::bool_constant;
+    if (!attn_vec(a, size_of))
+      return with(dp, bool_constant<false>(), integral_constant<int, kEither>());
+    return a.pos ? with(dp, bool_constant<true>(), integral_constant<int, kGiven>())
+                 : with(dp, bool_constant<true>(), integral_constant<int, kIndex>());
   };
   if (a.dim <= 32) return either(integral_constant<int, 32>());
   if (a.dim <= 64) return either(integral_constant<int, 64>());
@@ -1198,18 +1235,18 @@ int by_shape(const AttnArgs& a, int shape, int size, F f) {
 template <>
 int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  return by_shape(a, shape, sizeof(T), [&](auto dp, auto nq, auto nk, auto vec) {
+  return by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec, auto pos) {
     return launch_fwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
-                      decltype(vec)::value>(a, out, s);
+                      decltype(vec)::value, decltype(pos)::value>(a, out, s);
   });
 }
 
 template <>
 int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  return by_shape(a, shape, sizeof(T), [&](auto dp, auto nq, auto nk, auto vec) {
+  return by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec, auto pos) {
     return launch_bwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
-                      decltype(vec)::value>(a, o, s);
+                      decltype(vec)::value, decltype(pos)::value>(a, o, s);
   });
 }
 

@@ -1968,14 +1968,21 @@ def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, bac
 
 def _attention_shape(chains: ChainLayout, heads: int, dim: int, backward: bool
                      ) -> Tuple[int, int]:
-    """(beads of a tile, parts of the other side) of the attention kernels."""
-    if chains.max_len <= 32:
+    """(beads of a tile, parts of the other side that a workgroup's waves share)
+    of the attention kernels, by the chains' lengths and the number of
+    workgroups of 128 beads.  Measured (us, forward / backward): 512 chains of
+    35 beads in bf16 25 / 76 with tiles of 64, 27 / 83 with 128; one of 2048
+    (128 workgroups) 42 / 106 in two parts of 64, 53 / 145 whole; 4 of 1031 in
+    fp32 58 / 168 in two parts of 128, 64 / 185 whole; one of 8191 in bf16
+    282 / 896 and 262 / 1245; 16 of 500 40 / 113 and 35 / 92."""
+    if chains.max_len <= 32 and backward:
         return 32, 1
     if chains.max_len <= 64:
         return 64, 1
     groups = chains.tiles[128].shape[0] * heads
-    long = chains.n_beads >= 400 * chains.n_chains
-    if dim <= 64 and long and (backward or groups < 1024):
+    if dim <= 64 and groups <= 128:
+        return 64, 2
+    if dim <= 64 and chains.n_beads >= 1000 * chains.n_chains and (backward or groups < 512):
         return 128, 2
     return 128, 1
 
