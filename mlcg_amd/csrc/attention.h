@@ -92,10 +92,15 @@ int attn_backward(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s);
 
 namespace {
 
-// rows of a part of a staged tile: 64, or 32 of the widest
+// rows of a part of a staged tile: 64, or 32 of the widest and, backward, of
+// 32-bit elements (the accumulators and blocks of 64 leave two waves a SIMD)
 template <typename T, int DP>
 constexpr int part_rows() {
   return sizeof(T) * DP <= 128 ? 64 : 32;
+}
+template <typename T, int DP>
+constexpr int part_rows_bwd() {
+  return sizeof(T) == 2 ? part_rows<T, DP>() : 32;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -491,7 +496,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
 // Waves a SIMD that the registers of a kernel are limited for: `values` 32-bit
 // values of fragments and accumulators, and about 70 more.
 constexpr int waves_for(int values) {
-  return values <= 24 ? 3 : 2;
+  return values <= 24 ? 3 : values <= 200 ? 2 : 1;
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -785,7 +790,7 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
 
 template <typename T, int DP, int NQ, int NK>
 struct DqLds {
-  static constexpr int KS = part_rows<T, DP>() * NK;
+  static constexpr int KS = part_rows_bwd<T, DP>() * NK;
   T k[2][KS * DP], v[2][KS * DP];
   float cap[2][KS];
   int kpos[2][KS];
@@ -805,7 +810,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
     const int32_t* __restrict__ order, const int32_t* __restrict__ first,
     float* __restrict__ dtable_part) {
-  constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
+  constexpr int RT = part_rows_bwd<T, DP>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
   using Lds = DqLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
@@ -952,7 +957,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
 
 template <typename T, int DP, int NQ, int NK>
 struct DkvLds {
-  static constexpr int KS = part_rows<T, DP>() * NK;
+  static constexpr int KS = part_rows_bwd<T, DP>() * NK;
   T q[2][KS * DP], g[2][KS * DP];
   float lse[2][KS], delta[2][KS];
   int qpos[2][KS];
@@ -970,7 +975,7 @@ constexpr int dkv_waves() {
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
     AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
-  constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
+  constexpr int RT = part_rows_bwd<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = DkvLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
