@@ -496,7 +496,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
 // Waves a SIMD that the registers of a kernel are limited for: `values` 32-bit
 // values of fragments and accumulators, and about 70 more.
 constexpr int waves_for(int values) {
-  return values <= 24 ? 3 : values <= 200 ? 2 : 1;
+  return values <= 24 ? 3 : values < 192 ? 2 : 1;
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -508,14 +508,17 @@ struct FwdLds {
   float ext[1];  // 2 (reach + kAttnSpan) + 1
 };
 
-// a query's fragments, an accumulator of DP rows, a block of logits
-template <typename T, int DP>
+// a query's fragments and an accumulator of DP rows; one wave more where a
+// workgroup of four waves has few chunks to hold (2 x 4099 beads of 64 channels
+// in bf16: 160 us against 218, as all workgroups then run at once)
+template <typename T, int DP, int NQ, int NK>
 constexpr int fwd_waves() {
-  return waves_for(DP * (int)sizeof(T) / 8 + DP / 2);
+  constexpr int values = DP * (int)sizeof(T) / 8 + DP / 2;
+  return waves_for(values) + (NQ == 4 && NK == 1 && values <= 48 ? 1 : 0);
 }
 
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
-__global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP>())) void attn_fwd_kernel(
+__global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void attn_fwd_kernel(
     AttnArgs a, T* __restrict__ out) {
   constexpr int RT = part_rows<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = FwdLds<T, DP, NQ, NK>;
@@ -797,10 +800,10 @@ struct DqLds {
   float rest[4];  // scratch of the waves, ext, dd of the waves
 };
 
-// fragments of q and do, an accumulator, -delta
+// fragments of q and do, an accumulator
 template <typename T, int DP>
 constexpr int dq_waves() {
-  return waves_for(2 * (DP * (int)sizeof(T) / 8) + DP / 2 + 16);
+  return waves_for(2 * (DP * (int)sizeof(T) / 8) + DP / 2);
 }
 
 // dq, delta and the workgroup's part of the table's gradient; lanes are
@@ -869,10 +872,6 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   else
     for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
-  f32x16 minus_delta;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
-
   f32x16 acc[DP / 32] = {};
   int buf = 0;
   // puts the tile of k0 into LDS and sends for the next one
@@ -908,10 +907,11 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     float x[16 * N];
     const int side = query_logits<N, POS>(a, s, ext, cap, kpos, kb, qi, lse, x);
 #pragma unroll
-    for (int n = 0; n < N; ++n) s[n] = minus_delta;
-    row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, s);  // dP - delta
+    for (int n = 0; n < N; ++n) s[n] = f32x16{};
+    row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, s);  // dP
 #pragma unroll
-    for (int i = 0; i < 16 * N; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]) * s[i / 16][i % 16];
+    for (int i = 0; i < 16 * N; ++i)
+      x[i] = __builtin_amdgcn_exp2f(x[i]) * (s[i / 16][i % 16] - delta);
     if (side) {
       float sum[4] = {};
 #pragma unroll
