@@ -243,20 +243,23 @@ struct Stage {
       }
     }
   }
-  // the rows of the thread's chunks that are past the end or absent
-  __device__ __forceinline__ static uint32_t find_absent(const uint8_t* keep, int rows) {
-    uint32_t bits = 0;
+  // The rows of the thread's chunks that are past the end or absent, in two
+  // steps: the bytes of `keep` (may be NULL) are sent for with a tile's rows
+  // and looked at with them, as loads return in order.
+  struct Rows {
+    uint8_t keep[PER];
+    int rows;
+    __device__ __forceinline__ void load(const uint8_t* bytes, int n) {
+      rows = n;
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int r = min(row(p), rows - 1);
-      if (row(p) >= rows || (keep && !keep[r])) bits |= 1u << p;
+      for (int p = 0; p < PER; ++p) keep[p] = bytes ? bytes[min(row(p), n - 1)] : 1;
     }
-    return bits;
-  }
-  __device__ __forceinline__ void drop(uint32_t absent) {
+    __device__ __forceinline__ bool absent(int p) const { return row(p) >= rows || !keep[p]; }
+  };
+  __device__ __forceinline__ void drop(const Rows& r) {
 #pragma unroll
     for (int p = 0; p < PER; ++p)
-      if (absent >> p & 1) x[p] = chunk{};
+      if (r.absent(p)) x[p] = chunk{};
   }
   __device__ __forceinline__ void put(T* tile) const {
 #pragma unroll
@@ -419,23 +422,26 @@ __device__ __forceinline__ bool given_positions(const AttnArgs& a) {
 // sums begin with (0, or for an absent key what makes the logit -inf), and
 // their positions.  Thread i loads row i's.
 struct KeyInfo {
-  float cap;
+  bool in;
+  uint8_t keep;
   int pos;
   template <int POS>
   __device__ __forceinline__ void load(const AttnArgs& a, const int4& t, int k0, int rows) {
     const int i = threadIdx.x;
-    cap = logit_factor(a) > 0.0f ? -INFINITY : INFINITY;
+    in = i < rows && k0 + i < t.y;
+    keep = 1;
     pos = 0;
-    if (i < rows && k0 + i < t.y) {
+    if (in) {
       const int64_t row = (int64_t)t.x + k0 + i;
-      if (!a.keep || a.keep[row]) cap = 0.0f;
+      if (a.keep) keep = a.keep[row];
       if (given_positions<POS>(a)) pos = a.pos[row];
     }
   }
   template <int POS>
-  __device__ __forceinline__ void put(int rows, float* caps, int* kpos) const {
+  __device__ __forceinline__ void put(const AttnArgs& a, int rows, float* caps, int* kpos) const {
     if ((int)threadIdx.x < rows) {
-      caps[threadIdx.x] = cap;
+      const float none = logit_factor(a) > 0.0f ? -INFINITY : INFINITY;
+      caps[threadIdx.x] = in && keep ? 0.0f : none;
       if (POS != kIndex) kpos[threadIdx.x] = pos;
     }
   }
@@ -539,7 +545,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   vs.init((int)a.v_row, a.dim);
   ks.load(kbase, t.y, a.dim);
   vs.load(vbase, t.y, a.dim);
-  uint32_t absent = ks.find_absent(keep, t.y);
+  typename Stage<T, DP, KS, NT, VEC>::Rows absent;
+  absent.load(keep, t.y);
   info.template load<POS>(a, t, 0, KS);
 
   const bool given = given_positions<POS>(a);
@@ -561,12 +568,12 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.template put<POS>(KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(a, KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
       vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
-      if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
+      if (keep || kn + KS > t.y) absent.load(keep ? keep + kn : keep, t.y - kn);
       info.template load<POS>(a, t, kn, KS);
     }
     __syncthreads();
@@ -842,7 +849,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   vs.init((int)a.v_row, a.dim);
   ks.load(kbase, t.y, a.dim);
   vs.load(vbase, t.y, a.dim);
-  uint32_t absent = ks.find_absent(keep, t.y);
+  typename Stage<T, DP, KS, NT, VEC>::Rows absent;
+  absent.load(keep, t.y);
   info.template load<POS>(a, t, 0, KS);
 
   const bool given = given_positions<POS>(a);
@@ -882,12 +890,12 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.template put<POS>(KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(a, KS, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
       vs.load(vbase + kn * a.v_row, t.y - kn, a.dim);
-      if (keep || kn + KS > t.y) absent = ks.find_absent(keep ? keep + kn : keep, t.y - kn);
+      if (keep || kn + KS > t.y) absent.load(keep ? keep + kn : keep, t.y - kn);
       info.template load<POS>(a, t, kn, KS);
     }
     __syncthreads();
@@ -1011,7 +1019,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
   Stage<T, DP, KS, NT, VEC> qs, gs;
   qs.init((int)a.q_row, a.dim);
   gs.init(a.heads * a.dim, a.dim);
-  uint32_t absent = 0;
+  typename Stage<T, DP, KS, NT, VEC>::Rows absent;
   const bool given = given_positions<POS>(a);
   float lse_n = INFINITY, delta_n = 0.0f;
   int pos_n = 0;
@@ -1019,7 +1027,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     const int64_t row0 = (int64_t)t.x + q0;
     qs.load((const T*)a.q + row0 * a.q_row + head * a.q_head, t.y - q0, a.dim);
     gs.load((const T*)a.grad + (row0 * a.heads + head) * a.dim, t.y - q0, a.dim);
-    if (q0 + KS > t.y) absent = qs.find_absent(nullptr, t.y - q0);
+    if (q0 + KS > t.y) absent.load(nullptr, t.y - q0);
     const int i = threadIdx.x;
     lse_n = INFINITY;  // exp2(-inf) = 0 for the rows past the end
     delta_n = 0.0f;
@@ -1172,24 +1180,26 @@ int launch_fwd(const AttnArgs& a, void* out, hipStream_t s) {
 }
 
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
-int launch_bwd(const AttnArgs& a, const AttnGrads& o, hipStream_t s) {
+int launch_dq(const AttnArgs& a, const AttnGrads& o, float* delta, float* part, hipStream_t s) {
   constexpr unsigned NW = NQ * NK;
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
-  const unsigned lds1 = sizeof(DqLds<T, DP, NQ, NK>) +
-                        4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 2) * cells);
-  const unsigned lds2 = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
-  auto f1 = attn_dq_kernel<T, DP, NQ, NK, VEC, POS>;
-  auto f2 = attn_dkv_kernel<T, DP, NQ, NK, VEC, POS>;
-  if (int e = allow_lds(reinterpret_cast<const void*>(f1), lds1)) return e;
-  if (int e = allow_lds(reinterpret_cast<const void*>(f2), lds2)) return e;
-  float* delta = o.ws;
-  float* part = o.ws + a.heads * a.beads;
-  hipLaunchKernelGGL(f1, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NW), lds1, s, a,
+  const unsigned lds = sizeof(DqLds<T, DP, NQ, NK>) +
+                       4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 2) * cells);
+  auto f = attn_dq_kernel<T, DP, NQ, NK, VEC, POS>;
+  if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
+  hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NW), lds, s, a,
                      (T*)o.dq, delta, o.order, o.first, part);
-  hipLaunchKernelGGL(f2, dim3((unsigned)(a.n_tiles * (a.heads / a.group))), dim3(64 * NW), lds2, s,
-                     a, delta, (T*)o.dk, (T*)o.dv);
-  hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(mlcg_div_up(a.buckets, 8), a.heads), dim3(256), 0,
-                     s, part, a.n_tiles, a.buckets, a.heads, (T*)o.dtable);
+  return mlcg_launch_status();
+}
+
+template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
+int launch_dkv(const AttnArgs& a, const AttnGrads& o, const float* delta, hipStream_t s) {
+  const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
+  const unsigned lds = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
+  auto f = attn_dkv_kernel<T, DP, NQ, NK, VEC, POS>;
+  if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
+  hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * (a.heads / a.group))), dim3(64 * NQ * NK), lds,
+                     s, a, delta, (T*)o.dk, (T*)o.dv);
   return mlcg_launch_status();
 }
 
@@ -1249,10 +1259,28 @@ int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStrea
 template <>
 int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  return by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec, auto pos) {
-    return launch_bwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
-                      decltype(vec)::value, decltype(pos)::value>(a, o, s);
-  });
+  float* delta = o.ws;
+  float* part = o.ws + a.heads * a.beads;
+  if (int e = by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec,
+                                                      auto pos) {
+        return launch_dq<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
+                         decltype(vec)::value, decltype(pos)::value>(a, o, delta, part, s);
+      }))
+    return e;
+  // keys of shared heads give fewer workgroups than queries: where they are no
+  // more than the compute units, two waves share a block of keys (8191 beads,
+  // 8 heads on 2 key heads in bf16: both passes 793 us against 1048)
+  const int64_t groups = (int64_t)a.n_tiles * (a.heads / a.group);
+  const int kv_shape = shape >= 20 && groups <= 256 ? shape / 10 * 10 + 2 : shape;
+  if (int e = by_shape<(int)sizeof(T)>(a, kv_shape, [&](auto dp, auto nq, auto nk, auto vec,
+                                                         auto pos) {
+        return launch_dkv<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
+                          decltype(vec)::value, decltype(pos)::value>(a, o, delta, s);
+      }))
+    return e;
+  hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(mlcg_div_up(a.buckets, 8), a.heads), dim3(256), 0,
+                     s, part, a.n_tiles, a.buckets, a.heads, (T*)o.dtable);
+  return mlcg_launch_status();
 }
 
 #endif  // MLCG_ATTENTION_TYPE

@@ -1973,8 +1973,8 @@ def _attention_shape(chains: ChainLayout, heads: int, dim: int, backward: bool
     workgroups of 128 beads.  Measured (us, forward / backward): 512 chains of
     35 beads in bf16 25 / 76 with tiles of 64, 27 / 83 with 128; one of 2048
     (128 workgroups) 42 / 106 in two parts of 64, 53 / 145 whole; 4 of 1031 in
-    fp32 58 / 168 in two parts of 128, 64 / 185 whole; one of 8191 in bf16
-    282 / 896 and 262 / 1245; 16 of 500 40 / 113 and 35 / 92."""
+    fp32 (144) 58 / 168 in two parts of 128, 64 / 185 whole; 2 of 4096 (512)
+    137 / 358 and 139 / 344; 2 of 3000 96 / 253 and 87 / 227."""
     if chains.max_len <= 32 and backward:
         return 32, 1
     if chains.max_len <= 64:
@@ -1982,9 +1982,7 @@ def _attention_shape(chains: ChainLayout, heads: int, dim: int, backward: bool
     groups = chains.tiles[128].shape[0] * heads
     if dim <= 64 and groups <= 128:
         return 64, 2
-    if dim <= 64 and chains.n_beads >= 1000 * chains.n_chains and (backward or groups < 512):
-        return 128, 2
-    return 128, 1
+    return 128, 2 if dim <= 64 and groups <= 256 else 1
 
 
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
