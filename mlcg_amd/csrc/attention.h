@@ -296,6 +296,12 @@ __device__ __forceinline__ T round_to(float v) {
   return (T)v;
 }
 
+// The probabilities and dS, in fp32 until here, take the elements' type as
+// operands of the products with v, do, k and q, as the matrix instructions ask
+// for: below 2^kAttnLazy relative to the row's base (forward) or at most 1
+// (backward), each is off by half a unit of that type, as its other factor is.
+// The sums that follow, of the row, of o, dq, dk, dv and of the table, stay in
+// fp32, and the row's sum and the table take the values before this rounding.
 template <typename T>
 __device__ __forceinline__ v8<T> pack8(const float* p) {
   v8<T> r;
@@ -526,6 +532,15 @@ constexpr int fwd_waves() {
   return waves_for(values) + (NQ == 4 && NK == 1 && values <= 48 ? 1 : 0);
 }
 
+// Forward; lanes are queries, the tiles hold keys.  Bound by the issue of its
+// matrix and vector instructions, which overlap between the waves of a SIMD
+// alone: at 8191 beads, 8 heads of 64 on 2 in bf16 a logit costs 6.8 vector
+// instructions (one of them exp2, at a quarter of the rate), so that they take
+// 57 % of the SIMDs' cycles and the products 24 %.  224 us, 613 TFLOP/s, 53 %
+// of a large library product's rate.  4 chains of 1031, 4 heads of 32 in fp32:
+// 47 us (46 TFLOP/s), 144 workgroups of 128 queries on 256 compute units.
+// 512 chains of up to 100, 4 heads of 32 in bf16: 20 us, one or two tiles a
+// workgroup, bound by the latency of its first loads.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void attn_fwd_kernel(
     AttnArgs a, T* __restrict__ out) {
@@ -817,7 +832,12 @@ constexpr int dq_waves() {
 }
 
 // dq, delta and the workgroup's part of the table's gradient; lanes are
-// queries as in the forward pass.
+// queries as in the forward pass.  2 chains of 4099 beads, 8 heads of 64 in
+// bf16: 228 us (452 TFLOP/s over three products), vector instructions 36 % of
+// the SIMDs' cycles, products 18 %, the diagonals' LDS round trips in the band
+// and the waits at the tiles' barrier the rest.  48 chains of up to 268, 8
+// heads of 16 in fp32, positions given: 77 us, of which the sums by offset
+// about 40.  4 chains of 1031, 4 heads of 32 in fp32: 74 us.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
@@ -996,7 +1016,12 @@ constexpr int dkv_waves() {
 }
 
 // dk and dv; lanes are keys, the tiles hold queries.  The query heads that
-// share a key/value head are taken one after the other.
+// share a key/value head are taken one after the other, so their gradients are
+// summed in one wave's registers, in order.  2 chains of 4099 beads, 8 heads
+// of 64 in bf16: 214 us (643 TFLOP/s over four products), products 26 % of
+// the SIMDs' cycles, vector instructions 25 %; two waves a SIMD (128 fragments
+// and accumulators a lane) do not cover the LDS reads between them.  4 chains
+// of 1031, 4 heads of 32 in fp32: 81 us (54 TFLOP/s; 144 workgroups).
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
     AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
@@ -1155,7 +1180,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 }
 
 // dtable[b][head] = sum of the workgroups' parts [head][tile][b]: 8 buckets x
-// 32 slices of the tiles a workgroup, joined in order.
+// 32 slices of the tiles a workgroup, joined in order.  5 us, a launch's own
+// latency; a last workgroup that joins them would need an ordered counter.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_dtable_kernel(const float* __restrict__ part,
                                                           int n_tiles, int buckets, int heads,
@@ -1164,7 +1190,8 @@ __global__ __launch_bounds__(256) void attn_dtable_kernel(const float* __restric
   const int b = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3, head = blockIdx.y;
   float s = 0.0f;
   if (b < buckets)
-    for (int i = slice; i < n_tiles; i += 32) s += part[((int64_t)head * n_tiles + i) * buckets + b];
+    for (int i = slice; i < n_tiles; i += 32)
+      s += part[((int64_t)head * n_tiles + i) * buckets + b];
   red[slice][threadIdx.x & 7] = s;
   __syncthreads();
   if (slice == 0 && b < buckets) {

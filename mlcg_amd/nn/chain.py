@@ -310,9 +310,10 @@ class ChainEmbedding(torch.nn.Module):
     @torch.no_grad()
     def as_embedding(self) -> torch.nn.Embedding:
         """The present table as a plain embedding layer (without dropout)."""
-        training = self.training
+        modes = [(m, m.training) for m in self.modules()]
         try:
             return torch.nn.Embedding.from_pretrained(self.eval().table().detach().clone(),
                                                       freeze=False)
         finally:
-            self.train(training)
+            for m, training in modes:
+                m.training = training

@@ -2040,9 +2040,9 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     call("mlcg_chain_attention_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim,
          dt, ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), ptr(buckets.order),
-         ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, splits, ptr(keep),
-         ptr(positions), ptr(out), ptr(lse), ptr(grad), ptr(dq), ptr(dk), ptr(dv), ptr(dtable),
-         ptr(ws), nws, stream_handle(dev))
+         ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, splits,
+         ptr(keep), ptr(positions), ptr(out), ptr(lse), ptr(grad), ptr(dq), ptr(dk), ptr(dv),
+         ptr(dtable), ptr(ws), nws, stream_handle(dev))
     return dq, dk, dv, dtable
 
 
