@@ -1028,9 +1028,9 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * present); positions [beads]: p, any int32 (NULL: the index in the chain).
  * out [beads, heads, dim]; lse [heads, beads] (may be NULL): the base-2 log of
  * the row's sum, +inf for a row without keys, which the backward pass takes.
- * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or (with
- * tile_rows 64 and dim <= 64) 2: parts of the keys (backward: of the queries)
- * that a workgroup's waves share and join.
+ * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or, with
+ * dim <= 64, 2 (tile_rows 64 or 128) or 4 (tile_rows 64, forward alone): parts of
+ * the keys (backward: of the queries) that a workgroup's waves share and join.
  *
  * The backward pass gives the gradients of q, k, v (contiguous) and table.
  * bucket_order [2 reach + 1] lists the offsets 0 .. 2 reach by bucket,

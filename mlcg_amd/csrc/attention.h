@@ -1258,7 +1258,9 @@ bool attn_vec(const AttnArgs& a, int size) {
   return true;
 }
 
-template <int size_of, typename F>
+// four parts: of the forward pass alone (the backward's tiles and sums by
+// offset of eight waves would not fit the LDS)
+template <int size_of, bool FORWARD, typename F>
 int by_shape(const AttnArgs& a, int shape, F f) {
   using std::integral_constant;
   using One = integral_constant<int, 1>;
@@ -1267,6 +1269,8 @@ int by_shape(const AttnArgs& a, int shape, F f) {
   auto with = [&](auto dp, auto vec, auto pos) {
     constexpr bool split = decltype(dp)::value <= 64;
     const int nk = split ? shape % 10 : 1, nq = shape / 10;
+    if constexpr (split && FORWARD)
+      if (nk == 4) return f(dp, Two(), Four(), vec, pos);
     if (nk == 2) {
       if constexpr (split) {
         if (nq == 2) return f(dp, Two(), Two(), vec, pos);
@@ -1294,7 +1298,8 @@ int by_shape(const AttnArgs& a, int shape, F f) {
 template <>
 int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  return by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec, auto pos) {
+  return by_shape<(int)sizeof(T), true>(a, shape, [&](auto dp, auto nq, auto nk, auto vec,
+                                                       auto pos) {
     return launch_fwd<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
                       decltype(vec)::value, decltype(pos)::value>(a, out, s);
   });
@@ -1305,8 +1310,8 @@ int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o
   using T = MLCG_ATTENTION_TYPE;
   float* delta = o.ws;
   float* part = o.ws + a.heads * a.beads;
-  if (int e = by_shape<(int)sizeof(T)>(a, shape, [&](auto dp, auto nq, auto nk, auto vec,
-                                                      auto pos) {
+  if (int e = by_shape<(int)sizeof(T), false>(a, shape, [&](auto dp, auto nq, auto nk, auto vec,
+                                                            auto pos) {
         return launch_dq<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
                          decltype(vec)::value, decltype(pos)::value>(a, o, delta, part, s);
       }))
@@ -1316,8 +1321,8 @@ int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o
   // 8 heads on 2 key heads in bf16: both passes 793 us against 1048)
   const int64_t groups = (int64_t)a.n_tiles * (a.heads / a.group);
   const int kv_shape = shape >= 20 && groups <= 256 ? shape / 10 * 10 + 2 : shape;
-  if (int e = by_shape<(int)sizeof(T)>(a, kv_shape, [&](auto dp, auto nq, auto nk, auto vec,
-                                                         auto pos) {
+  if (int e = by_shape<(int)sizeof(T), false>(a, kv_shape, [&](auto dp, auto nq, auto nk,
+                                                               auto vec, auto pos) {
         return launch_dkv<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
                           decltype(vec)::value, decltype(pos)::value>(a, o, delta, s);
       }))

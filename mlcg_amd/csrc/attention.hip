@@ -3,15 +3,16 @@
 
 namespace {
 
-bool attn_ok(const AttnArgs& a, int tile_rows, int splits, int dtype) {
+bool attn_ok(const AttnArgs& a, int tile_rows, int splits, int dtype, bool backward) {
   for (int64_t row : {a.q_row, a.k_row, a.v_row})
     if (row < 0 || row >= (int64_t(1) << 22)) return false;
   return a.beads >= 0 && a.beads < (int64_t(1) << 31) - 256 && a.heads >= 1 && a.heads <= 1024 &&
          a.dim >= 1 && a.dim <= 128 && a.reach >= 1 && a.reach <= 1024 && a.buckets >= 1 &&
          (int64_t)a.n_tiles * a.heads < (int64_t(1) << 31) &&
          (tile_rows == 32 || tile_rows == 64 || tile_rows == 128) &&
-         (splits == 1 || (splits == 2 && tile_rows >= 64)) && dtype >= MLCG_DTYPE_F32 &&
-         dtype <= MLCG_DTYPE_BF16;
+         (splits == 1 || (splits == 2 && tile_rows >= 64) ||
+          (splits == 4 && tile_rows == 64 && a.dim <= 64 && !backward)) &&
+         dtype >= MLCG_DTYPE_F32 && dtype <= MLCG_DTYPE_BF16;
 }
 
 }  // namespace
@@ -36,7 +37,7 @@ extern "C" int mlcg_chain_attention(const void* q, const int64_t* q_strides, con
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, lse, (int)n_tiles, heads,
              heads / kv_heads, dim, reach, buckets, scale};
-  MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype));
+  MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype, false));
   if (beads == 0 || n_tiles == 0) return MLCG_OK;
   MLCG_REQUIRE(q && k && v && table && bucket_of && tiles && out);
   const int shape = 10 * (tile_rows / 32) + splits;
@@ -61,7 +62,7 @@ extern "C" int mlcg_chain_attention_backward(
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, const_cast<float*>(lse),
              (int)n_tiles, heads, heads / kv_heads, dim, reach, buckets, scale};
-  MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype) && beads >= 1);
+  MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype, true) && beads >= 1);
   MLCG_REQUIRE(q && k && v && table && bucket_of && bucket_order && bucket_first && tiles && out &&
                lse && grad_out && grad_q && grad_k && grad_v && grad_table && workspace);
   MLCG_REQUIRE(workspace_floats >=

@@ -1961,28 +1961,56 @@ def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, bac
                                                          f"{q.device}")
         positions = positions.contiguous()
     scale = dim ** -0.5 if scale is None else float(scale)
-    rows, splits = _attention_shape(chains, heads, dim, backward)
+    rows, splits = _attention_shape(chains, heads, dim, q.dtype, buckets.reach, backward)
     return (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table.contiguous(), scale, keep,
             positions, rows, splits)
 
 
-def _attention_shape(chains: ChainLayout, heads: int, dim: int, backward: bool
-                     ) -> Tuple[int, int]:
+def _attention_reach(rows: int, splits: int, dim: int) -> int:
+    """The reach up to which a workgroup of the backward pass fits the 160 KiB
+    of LDS: its tiles and, for every wave, two to three arrays over the offsets
+    (rounded down over the element types)."""
+    if (rows, splits) == (128, 2):
+        return 512 if dim <= 32 else 192
+    if ((rows, splits) == (64, 2) and dim > 32) or (rows == 128 and dim > 64):
+        return 768
+    return 1024
+
+
+def _attention_shape(chains: ChainLayout, heads: int, dim: int, dtype: torch.dtype, reach: int,
+                     backward: bool) -> Tuple[int, int]:
+    """_attention_shape_rule, or fewer waves where a long reach leaves no room."""
+    shape = _attention_shape_rule(chains, heads, dim, dtype, backward)
+    if backward and reach > _attention_reach(*shape, dim):
+        shape = (128, 1) if shape[0] == 128 and reach <= _attention_reach(128, 1, dim) else (64, 1)
+    return shape
+
+
+def _attention_shape_rule(chains: ChainLayout, heads: int, dim: int, dtype: torch.dtype,
+                          backward: bool) -> Tuple[int, int]:
     """(beads of a tile, parts of the other side that a workgroup's waves share)
-    of the attention kernels, by the chains' lengths and the number of
-    workgroups of 128 beads.  Measured (us, forward / backward): 512 chains of
-    35 beads in bf16 25 / 76 with tiles of 64, 27 / 83 with 128; one of 2048
-    (128 workgroups) 42 / 106 in two parts of 64, 53 / 145 whole; 4 of 1031 in
-    fp32 (144) 58 / 168 in two parts of 128, 64 / 185 whole; 2 of 4096 (512)
-    137 / 358 and 139 / 344; 2 of 3000 96 / 253 and 87 / 227."""
+    of the attention kernels, by the chains' lengths and the workgroups of 128
+    beads that there are for 256 compute units.  Measured (us, forward /
+    backward): 512 chains of 35 beads in bf16 25 / 76 with tiles of 64, 27 / 83
+    with 128.  One of 2048, 8 heads of 64 in bf16 (128 workgroups): 27 / 106 in
+    two parts of 64, 23 / - in four, 53 / 145 whole.  6 of 1000, 4 heads of 32
+    in fp32 (192): 44 / 149 in two parts of 128, 47 / 151 of 64, 48 / 159 whole.
+    10 of these (320, a second round of a quarter): 69 / 232 in two parts of
+    64, 80 / 275 whole, and 16 (512) 87 / 291 and 82 / 279; in bf16 10 take
+    33 / 124 and 31 / 90.  2 of 4096 in bf16 (512): 137 / 358 in two parts of
+    128, 139 / 344 whole."""
     if chains.max_len <= 32 and backward:
         return 32, 1
     if chains.max_len <= 64:
         return 64, 1
+    if dim > 64:
+        return 128, 1
     groups = chains.tiles[128].shape[0] * heads
-    if dim <= 64 and groups <= 128:
+    if not backward and chains.max_len > 256 and chains.tiles[64].shape[0] * heads <= 256:
+        return 64, 4
+    if groups <= 128 or (dtype == torch.float32 and 256 < groups <= 384):
         return 64, 2
-    return 128, 2 if dim <= 64 and groups <= 256 else 1
+    return 128, 2 if groups <= 256 else 1
 
 
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,

@@ -115,6 +115,58 @@ def test_attention_shared_heads(heads, kv, dtype):
     _check_attention(*_attention_case([90, 140], heads, kv, 16, dtype, seed=heads))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [16, 40, 64])
+def test_attention_few_long_chains(dim, dtype):
+    """The keys of a tile in four parts: absent beads (whole parts of them, too)
+    and residue numbers, a reach that takes the most LDS, unaligned rows."""
+    from mlcg_amd import nn
+
+    print(f"attention few long {dim} {dtype}", flush=True)
+    lens = [611, 258]
+    q, k, v, table, b, chains, grad = _attention_case(lens, 2, 1, dim, dtype, seed=dim,
+                                                      reach=1024)
+    g = torch.Generator().manual_seed(dim)
+    keep = torch.rand(sum(lens), generator=g) < 0.8
+    keep[64:330] = False
+    keep[611:] = False
+    keep[700] = True
+    pos = torch.cumsum((torch.rand(sum(lens), generator=g) < 0.4).int(), 0).to(torch.int32)
+    for kp, ps in ((None, None), (keep.cuda(), None), (keep.cuda(), pos.cuda())):
+        _check_attention(q, k, v, table, b, chains, grad, keep=kp, positions=ps)
+    odd = torch.empty(sum(lens), 4, dim + 1, dtype=dtype, device="cuda")[:, :, :dim]
+    odd[:, :2], odd[:, 2:3], odd[:, 3:] = q, k, v
+    a = nn.chain_attention(q, k, v, table, b, chains, keep=keep.cuda())
+    o = nn.chain_attention(odd[:, :2], odd[:, 2:3], odd[:, 3:], table, b, chains,
+                           keep=keep.cuda())
+    assert torch.equal(a, o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("chains_of_130", [20, 40, 50])
+def test_attention_many_middling_chains(chains_of_130, dtype):
+    """Workgroup counts on both sides of the compute units and of half as many
+    again, where the shapes change."""
+    print(f"attention middling {chains_of_130} {dtype}", flush=True)
+    _check_attention(*_attention_case([130] * chains_of_130, 4, 2, 16, dtype,
+                                      seed=chains_of_130))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("reach", [192, 193, 512, 513, 768, 769, 1024])
+def test_attention_reach(reach, dim, dtype):
+    """A reach that leaves little room beside the tiles, at every shape of the
+    backward pass, positions given or not."""
+    print(f"attention reach {reach} {dim} {dtype}", flush=True)
+    for lens in ([33, 20], [60], [300], [130] * 40):
+        q, k, v, table, b, chains, grad = _attention_case(lens, 4, 4, dim, dtype, seed=reach,
+                                                          reach=reach)
+        pos = 3 * torch.arange(sum(lens), dtype=torch.int32, device="cuda")
+        for ps in (None, pos):
+            _check_attention(q, k, v, table, b, chains, grad, positions=ps)
+
+
 @pytest.mark.parametrize("kind,buckets,reach", [
     ("clip", 3, 1), ("clip", 65, 32), ("clip", 257, 128), ("log", 2, 5), ("log", 47, 100),
     ("log", 32, 1024), ("log", 16, 3)])
