@@ -122,11 +122,12 @@ def philox4x32(counter, key, rounds=10):
     return x
 
 
-def dropout_kept(n, p, seed, step):
-    """[n] bool: the elements that dropout_add keeps, in Python integers."""
+def dropout_kept(n, p, seed, step, first=0):
+    """[n] bool: which of the elements from `first` (a multiple of 8) on
+    dropout_add keeps, in Python integers."""
     t = min(65535, int(round(65536 * p)))
     kept = []
-    for c in range((n + 7) // 8):
+    for c in range(first // 8, first // 8 + (n + 7) // 8):
         words = philox4x32([c & 0xFFFFFFFF, c >> 32, step & 0xFFFFFFFF, step >> 32],
                            [seed & 0xFFFFFFFF, seed >> 32])
         for w in words:

@@ -539,6 +539,57 @@ def test_dropout_layouts_and_graph():
     assert not any(torch.equal(a, c) for a, c in zip(seen, seen[1:]))
 
 
+def test_offsets_past_32_bits():
+    """Rows so far apart that their offsets pass 2^31 elements give what
+    contiguous ones give, and so do rows past 2^31 elements of a long x."""
+    from mlcg_amd import nn, ops
+
+    print("offsets past 32 bits: views", flush=True)
+    lens = [500, 90, 1]
+    s = sum(lens)
+    q, k, v, table, b, chains, grad = _attention_case(lens, 2, 1, 64, torch.bfloat16, views=False)
+    far = torch.empty(s, 2 ** 22 - 8, dtype=torch.bfloat16, device="cuda")  # 5 GB
+    assert far.stride(0) * (s - 1) > 2 ** 31
+    wide = far[:, :256].unflatten(1, (4, 64))
+    wide[:, :2], wide[:, 2:3], wide[:, 3:] = q, k, v
+    near = [q, k, v]
+    apart = [wide[:, :2], wide[:, 2:3], wide[:, 3:]]
+    outs = []
+    for args in (near, apart):
+        leaves = [t.detach().requires_grad_(True) for t in args]
+        out = nn.chain_attention(*leaves, table, b, chains)
+        outs.append((out.detach(), *torch.autograd.grad(out, leaves, grad)))
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    x = _randn((s, 128), torch.bfloat16, 5)
+    far[:, 300 * 8:300 * 8 + 128] = x
+    y0, st0 = ops.group_norm_act(x, w, w, 8, chains)
+    y1, st1 = ops.group_norm_act(far[:, 300 * 8:300 * 8 + 128], w, w, 8, chains)
+    assert torch.equal(y0, y1) and torch.equal(st0, st1)
+    del far, wide, apart
+    print("offsets past 32 bits: a long x", flush=True)
+    n, c = 2 ** 23 + 256, 256
+    x = torch.empty(n, c, dtype=torch.bfloat16, device="cuda").normal_()
+    assert x.numel() > 2 ** 31
+    lens = [256] * (n // 256)
+    chains = ops.chain_layout(lens, "cuda")
+    w = torch.ones(c, dtype=torch.bfloat16, device="cuda")
+    y, st = ops.group_norm_act(x, w, w, 8, chains)
+    dx, _, _ = ops.group_norm_act_backward(x, w, w, 8, chains, st, y)
+    last = ops.chain_layout([256] * 512, "cuda")
+    rows = slice(n - 512 * 256, n)
+    y1, st1 = ops.group_norm_act(x[rows], w, w, 8, last)
+    dx1, _, _ = ops.group_norm_act_backward(x[rows], w, w, 8, last, st1, y1)
+    assert torch.equal(y[rows], y1) and torch.equal(dx[rows], dx1)
+    del y, dx
+    z = ops.dropout_add(x, 0.5, 11, 3).view(-1)
+    e = 2 ** 31 + 8
+    kept, scale = R.dropout_kept(4096, 0.5, 11, 3, first=e)
+    want = torch.where(kept, x.view(-1)[e:e + 4096].cpu() * scale, 0.0)  # scale 2: exact
+    assert torch.equal(z[e:e + 4096].cpu(), want)
+
+
 def test_empty_inputs():
     from mlcg_amd import nn, ops
 
