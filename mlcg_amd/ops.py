@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import List, Optional, Tuple
 
 import numpy as np
@@ -1779,6 +1779,8 @@ class ChainLayout:
               it, chain), the longest chains first
     first   : {rows: [n_chains] int32}, a chain's first tile, -1 without beads
     whole   : [n, 4] int32, the chains that have beads as one tile each
+    plans   : what the operators have derived from the lengths: the shapes of
+              the attention's workgroups, the sizes of workspaces
     """
 
     lengths: Tuple[int, ...]
@@ -1790,6 +1792,7 @@ class ChainLayout:
     tiles: dict
     first: dict
     whole: torch.Tensor
+    plans: dict = field(default_factory=dict, repr=False)
 
 
 def chain_layout(lengths, device) -> ChainLayout:
@@ -1917,51 +1920,58 @@ def _chain_dtype(t: torch.Tensor, what: str) -> int:
     return dt
 
 
-def _attention_heads(t: torch.Tensor, name: str, chains: ChainLayout, like: torch.Tensor):
+_Strides = ctypes.c_int64 * 2
+
+
+def _attention_heads(t: torch.Tensor, name: str, n: int, dtype: torch.dtype,
+                     device: torch.device):
     """t as [S, heads, dim] with a contiguous last axis, and its strides."""
-    _check(t.dim() == 3 and t.shape[0] == chains.n_beads and t.dtype == like.dtype
-           and t.device == like.device,
-           lambda: f"{name} must be [{chains.n_beads}, heads, dim] {like.dtype} on "
-                   f"{like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if (t.stride(2) != 1 and t.shape[2] > 1) or t.stride(0) >= 2 ** 22:
+    shape, stride = t.shape, t.stride()
+    _check(len(shape) == 3 and shape[0] == n and t.dtype == dtype and t.device == device,
+           lambda: f"{name} must be [{n}, heads, dim] {dtype} on {device}, got "
+                   f"{tuple(shape)} {t.dtype} on {t.device}")
+    if (stride[2] != 1 and shape[2] > 1) or stride[0] >= 2 ** 22:
         t = t.contiguous()
-    return t, (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+        stride = t.stride()
+    return t, _Strides(stride[0], stride[1])
 
 
 def _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, backward=False):
     require_device(q, k, v, table, keep, positions)
     dt = _chain_dtype(q, "chain_attention")
-    _check(isinstance(chains, ChainLayout) and chains.device == q.device,
+    dtype, device = q.dtype, q.device
+    _check(isinstance(chains, ChainLayout) and chains.device == device,
            "chains must be a ChainLayout on the queries' device")
-    q, qs = _attention_heads(q, "q", chains, q)
-    k, ks = _attention_heads(k, "k", chains, q)
-    v, vs = _attention_heads(v, "v", chains, q)
-    n, heads, dim = q.shape
-    kv = k.shape[1]
-    _check(k.shape == v.shape and k.shape[2] == dim,
+    n = chains.n_beads
+    q, qs = _attention_heads(q, "q", n, dtype, device)
+    k, ks = _attention_heads(k, "k", n, dtype, device)
+    v, vs = _attention_heads(v, "v", n, dtype, device)
+    _, heads, dim = q.shape
+    _, kv, k_dim = k.shape
+    _check(k_dim == dim and v.shape == k.shape,
            lambda: f"k and v must be [{n}, kv_heads, {dim}], got {tuple(k.shape)} and "
                    f"{tuple(v.shape)}")
     _check(1 <= kv <= heads <= 1024 and heads % kv == 0,
            lambda: f"{heads} query heads cannot share {kv} key/value heads")
     _check(1 <= dim <= MAX_ATTENTION_DIM,
            lambda: f"the head dimension must lie in 1 .. {MAX_ATTENTION_DIM}, got {dim}")
-    _check(isinstance(buckets, RelativeBuckets) and buckets.bucket_of.device == q.device,
+    _check(isinstance(buckets, RelativeBuckets) and buckets.bucket_of.device == device,
            "buckets must be RelativeBuckets on the queries' device")
-    _check(tuple(table.shape) == (buckets.num_buckets, heads) and table.dtype == q.dtype
-           and table.device == q.device,
-           lambda: f"table must be [{buckets.num_buckets}, {heads}] {q.dtype} on {q.device}, "
+    _check(table.shape == (buckets.num_buckets, heads) and table.dtype == dtype
+           and table.device == device,
+           lambda: f"table must be [{buckets.num_buckets}, {heads}] {dtype} on {device}, "
                    f"got {tuple(table.shape)} {table.dtype} on {table.device}")
     if keep is not None:
-        _check(keep.dtype == torch.bool and tuple(keep.shape) == (n,) and keep.device == q.device,
-               lambda: f"keep must be [{n}] bool on {q.device}")
+        _check(keep.dtype == torch.bool and keep.shape == (n,) and keep.device == device,
+               lambda: f"keep must be [{n}] bool on {device}")
         keep = keep.contiguous()
     if positions is not None:
-        _check(positions.dtype == torch.int32 and tuple(positions.shape) == (n,)
-               and positions.device == q.device, lambda: f"positions must be [{n}] int32 on "
-                                                         f"{q.device}")
+        _check(positions.dtype == torch.int32 and positions.shape == (n,)
+               and positions.device == device,
+               lambda: f"positions must be [{n}] int32 on {device}")
         positions = positions.contiguous()
     scale = dim ** -0.5 if scale is None else float(scale)
-    rows, splits = _attention_shape(chains, heads, dim, q.dtype, buckets.reach, backward)
+    rows, splits = _attention_shape(chains, heads, dim, dtype, buckets.reach, backward)
     return (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table.contiguous(), scale, keep,
             positions, rows, splits)
 
@@ -1980,9 +1990,14 @@ def _attention_reach(rows: int, splits: int, dim: int) -> int:
 def _attention_shape(chains: ChainLayout, heads: int, dim: int, dtype: torch.dtype, reach: int,
                      backward: bool) -> Tuple[int, int]:
     """_attention_shape_rule, or fewer waves where a long reach leaves no room."""
-    shape = _attention_shape_rule(chains, heads, dim, dtype, backward)
-    if backward and reach > _attention_reach(*shape, dim):
-        shape = (128, 1) if shape[0] == 128 and reach <= _attention_reach(128, 1, dim) else (64, 1)
+    plan = (heads, dim, dtype, reach, backward)
+    shape = chains.plans.get(plan)
+    if shape is None:
+        shape = _attention_shape_rule(chains, heads, dim, dtype, backward)
+        if backward and reach > _attention_reach(*shape, dim):
+            fits = shape[0] == 128 and reach <= _attention_reach(128, 1, dim)
+            shape = (128 if fits else 64, 1)
+        chains.plans[plan] = shape
     return shape
 
 
@@ -2054,7 +2069,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     for t, name, shape, dtype in ((out, "out", (n, heads, dim), q.dtype),
                                   (grad, "grad", (n, heads, dim), q.dtype),
                                   (lse, "lse", (heads, n), torch.float32)):
-        _check(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype
+        _check(isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype
                and t.device == dev, lambda: f"{name} must be {shape} {dtype} on {dev}")
     out, lse, grad = out.contiguous(), lse.contiguous(), grad.contiguous()
     dq = torch.empty(n, heads, dim, dtype=q.dtype, device=dev)
@@ -2077,7 +2092,8 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
 def _norm_args(x, weight, bias, groups, chains, act):
     require_device(x, weight, bias)
     dt = _chain_dtype(x, "group_norm_act")
-    _check(isinstance(chains, ChainLayout) and chains.device == x.device,
+    dtype, device = x.dtype, x.device
+    _check(isinstance(chains, ChainLayout) and chains.device == device,
            "chains must be a ChainLayout on the rows' device")
     _check(x.dim() == 2 and x.shape[0] == chains.n_beads,
            lambda: f"x must be [{chains.n_beads}, width], got {tuple(x.shape)}")
@@ -2086,12 +2102,14 @@ def _norm_args(x, weight, bias, groups, chains, act):
            lambda: f"group_norm_act takes 1 .. {MAX_NORM_WIDTH} channels in equal groups, got "
                    f"{width} in {groups}")
     for t, name in ((weight, "weight"), (bias, "bias")):
-        _check(tuple(t.shape) == (width,) and t.dtype == x.dtype and t.device == x.device,
-               lambda: f"{name} must be [{width}] {x.dtype} on {x.device}")
+        _check(t.shape == (width,) and t.dtype == dtype and t.device == device,
+               lambda: f"{name} must be [{width}] {dtype} on {device}")
     _check(act in CHAIN_ACTS, lambda: f"act must be one of {sorted(CHAIN_ACTS)}, got {act!r}")
-    if (width > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < width):
-        x = x.contiguous()
-    ld = x.stride(0) if n > 1 else width
+    ld, step = x.stride()
+    if (width > 1 and step != 1) or (n > 1 and ld < width):
+        x, ld = x.contiguous(), width
+    if n <= 1:
+        ld = width
     return x, ld, n, width, dt, weight.contiguous(), bias.contiguous(), CHAIN_ACTS[act]
 
 
@@ -2099,9 +2117,13 @@ NORM_SLAB_ROWS = 256
 
 
 def _norm_workspace(chains: ChainLayout, width: int, groups: int, backward: int, dev):
-    nws = int(_lib.load().mlcg_group_norm_workspace_floats(
-        chains.tiles[NORM_SLAB_ROWS].shape[0], chains.n_chains, chains.whole.shape[0],
-        chains.max_len, width, groups, backward))
+    plan = (width, groups, backward)
+    nws = chains.plans.get(plan)
+    if nws is None:
+        nws = chains.plans[plan] = int(
+            _lib.load().mlcg_group_norm_workspace_floats(
+                chains.tiles[NORM_SLAB_ROWS].shape[0], chains.n_chains, chains.whole.shape[0],
+                chains.max_len, width, groups, backward))
     return (torch.empty(nws, dtype=torch.float32, device=dev) if nws > 0 else None), nws
 
 
@@ -2140,9 +2162,9 @@ def group_norm_act_backward(x, weight, bias, groups: int, chains: ChainLayout,
     (mlcg_group_norm_act_backward); stats are the forward's."""
     x, ld, n, width, dt, weight, bias, act_id = _norm_args(x, weight, bias, groups, chains, act)
     dev = x.device
-    _check(tuple(grad.shape) == (n, width) and grad.dtype == x.dtype and grad.device == dev,
+    _check(grad.shape == (n, width) and grad.dtype == x.dtype and grad.device == dev,
            lambda: f"grad must be [{n}, {width}] {x.dtype} on {dev}")
-    _check(tuple(stats.shape) == (3, chains.n_chains, groups) and stats.dtype == torch.float32
+    _check(stats.shape == (3, chains.n_chains, groups) and stats.dtype == torch.float32
            and stats.device == dev,
            lambda: f"stats must be [3, {chains.n_chains}, {groups}] float32 on {dev}")
     grad, stats = grad.contiguous(), stats.contiguous()
@@ -2154,7 +2176,8 @@ def group_norm_act_backward(x, weight, bias, groups: int, chains: ChainLayout,
     call("mlcg_group_norm_act_backward", ptr(x), ld, ptr(grad), n, dt, ptr(weight), ptr(bias),
          width, groups, *_norm_chains(chains), act_id, ptr(stats), ptr(dx), ptr(dbw), ptr(ws),
          nws, stream_handle(dev))
-    return dx, dbw[1], dbw[0]
+    db, dw = dbw.unbind()
+    return dx, dw, db
 
 
 def dropout_threshold(p: float) -> int:
