@@ -1031,6 +1031,10 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or, with
  * dim <= 64, 2 (tile_rows 64 or 128) or 4 (tile_rows 64, forward alone): parts of
  * the keys (backward: of the queries) that a workgroup's waves share and join.
+ * Backward, a long reach leaves no room for the sums by offset of many waves:
+ * MLCG_ERR_UNSUPPORTED above a reach of 192 (tile_rows 128 with splits 2; 512
+ * with dim <= 32) or 768 (tile_rows 64 with splits 2 and dim > 32, 128 with
+ * dim > 64) or a little more; the other shapes take every reach.
  *
  * The backward pass gives the gradients of q, k, v (contiguous) and table.
  * bucket_order [2 reach + 1] lists the offsets 0 .. 2 reach by bucket,
