@@ -812,8 +812,7 @@ __device__ __forceinline__ void flush_offsets(const AttnArgs& a, float* dd, int 
 
 // floats of a wave's scratch: the diagonals' block or the integers
 __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions) {
-  const int ints = (2 * (2 * reach + 1) + 3) & ~3;
-  return positions && ints > kDiagFloats ? ints : kDiagFloats;
+  return positions ? (2 * (2 * reach + 1) + 3) & ~3 : kDiagFloats;
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -836,8 +835,9 @@ constexpr int dq_waves() {
 // bf16: 228 us (452 TFLOP/s over three products), vector instructions 36 % of
 // the SIMDs' cycles, products 18 %, the diagonals' LDS round trips in the band
 // and the waits at the tiles' barrier the rest.  48 chains of up to 268, 8
-// heads of 16 in fp32, positions given: 77 us, of which the sums by offset
-// about 40.  4 chains of 1031, 4 heads of 32 in fp32: 74 us.
+// heads of 16 in fp32, positions given: 63 us, of which the sums by offset
+// about 30 (77 with the diagonals' block kept beside the integers: two
+// workgroups a compute unit instead of three).  4 chains of 1031, 4 heads of 32 in fp32: 74 us.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
@@ -966,8 +966,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
       for (int i = 0; i < 16 * N; ++i) top = x[i] != x[i] ? INFINITY : top;
       ints.prepare(top);
       // beads of one residue follow each other: one sum for equal neighbours (48
-      // chains of up to 268 beads, 2.5 to a residue, 8 heads of 16: 79 us against
-      // about 97)
+      // chains of up to 268 beads, 2.5 to a residue, 8 heads of 16: about 18 us
+      // less)
 #pragma unroll
       for (int i = 0; i < 16 * N; i += 4) {
         const int4 p = *reinterpret_cast<const int4*>(kpos + acc_row(i, g));
