@@ -42,8 +42,9 @@
 // outside of it has one value.  The table's gradient is summed by offset into
 // the same kind of array, one a wave:
 //   index positions: the block of 32 x 32 dS goes through LDS, [query][key]
-//   with a gap of zeros behind each row, and lane n adds the diagonal
-//   offset n - 31 (32 reads a lane, no test: past an end stand zeros);
+//   with a gap of zeros behind each row, at once or in two halves, and lane n
+//   adds the diagonal offset n - 31 (32 reads a lane, no test: past an end
+//   stand zeros);
 //   given positions: LDS adds of integers, dS scaled by a power of two and cut
 //   in two parts of 15 bits (LDS adds of floats take about 200 cycles a wave
 //   against 6, and their order would change the last bits);
@@ -686,24 +687,40 @@ __device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
 // The table's gradient
 
 constexpr int kDiagPitch = 68;  // 32 values and the gap of zeros; 16-byte rows
-constexpr int kDiagFloats = 32 + 32 * kDiagPitch;
+// queries that pass through the block at a time: half of them where the
+// registers allow three waves a SIMD, which the whole block's LDS would not
+// (512 chains of up to 100 beads, 4 heads of 32 in bf16: dq 35 us against 43)
+template <int DP>
+constexpr int diag_rows() {
+  return DP == 32 ? 16 : 32;
+}
+template <int DP>
+constexpr int diag_floats() {
+  return 32 + diag_rows<DP>() * kDiagPitch;
+}
 
 // mine[cell of offset d0 + n - 31] += diagonal n of the block whose lanes are
 // queries 0..31 and whose rows are keys 0..31, d0 = first key - first query.
+template <int DP>
 __device__ __forceinline__ void add_diagonals(const float* x, float* scratch, float* at_d0) {
+  constexpr int QR = diag_rows<DP>();
   const int lane = threadIdx.x & 63, q = lane & 31, g = lane >> 5;
-  float* row = scratch + 32 + q * kDiagPitch + 4 * g;
-#pragma unroll
-  for (int a = 0; a < 4; ++a)
-    *reinterpret_cast<float4*>(row + 8 * a) =
-        make_float4(x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  const float* d = scratch + 32 + lane - 31;
+  float* row = scratch + 32 + (q % QR) * kDiagPitch + 4 * g;
   float t[4] = {};
 #pragma unroll
-  for (int r = 0; r < 32; ++r) t[r % 4] += d[r * (kDiagPitch + 1)];
+  for (int q0 = 0; q0 < 32; q0 += QR) {
+    if (q / QR == q0 / QR)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *reinterpret_cast<float4*>(row + 8 * a) =
+            make_float4(x[4 * a], x[4 * a + 1], x[4 * a + 2], x[4 * a + 3]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float* d = scratch + 32 + lane - 31 + q0;
+#pragma unroll
+    for (int r = 0; r < QR; ++r) t[r % 4] += d[r * (kDiagPitch + 1)];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
   at_d0[lane - 31] += (t[0] + t[1]) + (t[2] + t[3]);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Sums by offset for given positions: integers of dS 2^e, a high part of at
@@ -811,8 +828,9 @@ __device__ __forceinline__ void flush_offsets(const AttnArgs& a, float* dd, int 
 }
 
 // floats of a wave's scratch: the diagonals' block or the integers
+template <int DP>
 __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions) {
-  return positions ? (2 * (2 * reach + 1) + 3) & ~3 : kDiagFloats;
+  return positions ? (2 * (2 * reach + 1) + 3) & ~3 : diag_floats<DP>();
 }
 
 template <typename T, int DP, int NQ, int NK>
@@ -848,7 +866,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   extern __shared__ __align__(16) unsigned char smem[];
   Lds& L = *reinterpret_cast<Lds*>(smem);
   const int R = a.reach, cells = 2 * (R + kAttnSpan) + 1;
-  const int sf = scratch_floats(R, given_positions<POS>(a));
+  const int sf = scratch_floats<DP>(R, given_positions<POS>(a));
   float* ext = L.rest + NW * sf;
   float* dd = ext + cells;
 
@@ -901,7 +919,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   if (given)
     ints.init(reinterpret_cast<int*>(scratch), R, mine + kAttnSpan);
   else
-    for (int i = lane; i < kDiagFloats; i += 64) scratch[i] = 0.0f;
+    for (int i = lane; i < diag_floats<DP>(); i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
   f32x16 acc[DP / 32] = {};
   int buf = 0;
@@ -956,7 +974,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
 #pragma unroll
       for (int n = 0; n < N; ++n)
         if (kb + 32 * n < t.y)
-          add_diagonals(x + 16 * n, scratch, mine + (kb + 32 * n - qi.first + R + kAttnSpan));
+          add_diagonals<DP>(x + 16 * n, scratch,
+                            mine + (kb + 32 * n - qi.first + R + kAttnSpan));
     } else {
       float top = 0.0f;
 #pragma unroll
@@ -1228,7 +1247,7 @@ int launch_dq(const AttnArgs& a, const AttnGrads& o, float* delta, float* part, 
   constexpr unsigned NW = NQ * NK;
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds = sizeof(DqLds<T, DP, NQ, NK>) +
-                       4 * (NW * scratch_floats(a.reach, a.pos != nullptr) + (NW + 2) * cells);
+                       4 * (NW * scratch_floats<DP>(a.reach, a.pos != nullptr) + (NW + 2) * cells);
   auto f = attn_dq_kernel<T, DP, NQ, NK, VEC, POS>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
   hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NW), lds, s, a,
