@@ -1028,6 +1028,8 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * present); positions [beads]: p, any int32 (NULL: the index in the chain).
  * out [beads, heads, dim]; lse [heads, beads] (may be NULL): the base-2 log of
  * the row's sum, +inf for a row without keys, which the backward pass takes.
+ * rest [beads, heads, dim] (16-bit types; may be NULL): what the rounding of out
+ * leaves out, from which the backward pass has its row sums in full.
  * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or, with
  * dim <= 64, 2 (tile_rows 64 or 128) or 4 (tile_rows 64, forward alone): parts of
  * the keys (backward: of the queries) that a workgroup's waves share and join.
@@ -1048,8 +1050,8 @@ int mlcg_chain_attention(const void* q, const int64_t* q_strides, const void* k,
                          int buckets, const int32_t* bucket_of, int reach,
                          float scale, const int32_t* tiles, int64_t n_tiles,
                          int tile_rows, int splits, const uint8_t* keep,
-                         const int32_t* positions, void* out, float* lse,
-                         void* stream);
+                         const int32_t* positions, void* out, void* rest,
+                         float* lse, void* stream);
 int mlcg_chain_attention_backward(
     const void* q, const int64_t* q_strides, const void* k,
     const int64_t* k_strides, const void* v, const int64_t* v_strides,
@@ -1058,8 +1060,8 @@ int mlcg_chain_attention_backward(
     const int32_t* bucket_order, const int32_t* bucket_first, int reach,
     float scale, const int32_t* tiles, int64_t n_tiles, int tile_rows,
     int splits, const uint8_t* keep, const int32_t* positions, const void* out,
-    const float* lse, const void* grad_out, void* grad_q, void* grad_k,
-    void* grad_v, void* grad_table, float* workspace,
+    const void* rest, const float* lse, const void* grad_out, void* grad_q,
+    void* grad_k, void* grad_v, void* grad_table, float* workspace,
     int64_t workspace_floats, void* stream);
 
 /* Group norm of every chain and activation, channels last: mean and biased

@@ -153,10 +153,10 @@ _SIGNATURES = {
     "mlcg_mse_mean_backward": [_P, _P, _P, _I64, _P, _P],
     "mlcg_chain_attention_workspace_floats": [_I64, _I32, _I64, _I32],
     "mlcg_chain_attention": [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I32, _P,
-        _I32, _F32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P],
+        _I32, _F32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P],
     "mlcg_chain_attention_backward": [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P,
         _I32, _P, _P, _P, _I32, _F32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P,
-        _P, _I64, _P],
+        _P, _P, _I64, _P],
     "mlcg_group_norm_workspace_floats": [_I64, _I64, _I64, _I64, _I32, _I32, _I32],
     "mlcg_group_norm_act": [_P, _I64, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64, _P, _I64, _I64, _I64, _F32, _I32, _P, _P, _P, _I64, _P],
     "mlcg_group_norm_act_backward": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64,

@@ -71,6 +71,7 @@ struct AttnArgs {
   float* lse;  // [heads][beads], base 2; +inf for a row without keys
   int n_tiles, heads, group, dim, reach, buckets;
   float scale;
+  void* rest;  // what the rounding of out leaves out, or NULL
 };
 
 // Whether positions are given: known when the kernel is built, or (kEither, in
@@ -388,6 +389,33 @@ __device__ __forceinline__ void store_column(T* dst, const f32x16 (&acc)[DP / 32
     }
 }
 
+// what the rounding of a column leaves out, rounded itself
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void store_rest(T* dst, const f32x16 (&acc)[DP / 32], float f,
+                                           int dim) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int d = 32 * n + 8 * a + 4 * g;
+      v4<T> o;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v = acc[n][4 * a + c] * f;
+        asm("" : "+v"(v));  // as store_column rounds it
+        o[c] = (T)(v - (float)(T)v);
+      }
+      if constexpr (VEC) {
+        if (d < dim) *reinterpret_cast<v4<T>*>(dst + d) = o;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (d + c < dim) dst[d + c] = o[c];
+      }
+    }
+}
+
 // acc of the NK waves of a column block, joined in the order of the parts;
 // the sums are part 0's.  buf: (NK - 1) NQ 64 values for each accumulator.
 template <int DP, int NQ, int NK>
@@ -668,8 +696,14 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   }
   if (wk > 0 || !qi.ok) return;
   const int64_t row = (int64_t)t.x + qi.mine;
-  store_column<T, DP, VEC>(out + (row * a.heads + head) * a.dim, acc,
-                           l == 0.0f ? 0.0f : 1.0f / l, a.dim);
+  const int64_t flat = (row * a.heads + head) * a.dim;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  store_column<T, DP, VEC>(out + flat, acc, inv, a.dim);
+  // a row's dS sum to what delta = do . o is off, so that the rounding of o
+  // would be the table's largest error (2 chains of 4099 beads in bf16: 4.3e-3
+  // of its gradient against 1.7e-3)
+  if constexpr (sizeof(T) == 2)
+    if (a.rest) store_rest<T, DP, VEC>((T*)a.rest + flat, acc, inv, a.dim);
   if (a.lse && g == 0)
     a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -906,8 +940,12 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, qi.ok, a.dim);
     gf[k] = load8<T, VEC>((const T*)a.grad + flat, 16 * k + 8 * g, qi.ok, a.dim);
     const v8<T> of = load8<T, VEC>((const T*)a.out + flat, 16 * k + 8 * g, qi.ok, a.dim);
+    v8<T> rf = {};
+    if (sizeof(T) == 2 && a.rest)
+      rf = load8<T, VEC>((const T*)a.rest + flat, 16 * k + 8 * g, qi.ok, a.dim);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[k][e], (float)of[e], delta);
+    for (int e = 0; e < 8; ++e)
+      delta = fmaf((float)gf[k][e], (float)of[e] + (float)rf[e], delta);
   }
   delta += other_half(delta);
   const float lse = qi.ok ? a.lse[head * a.beads + row] : INFINITY;
@@ -1268,7 +1306,7 @@ int launch_dkv(const AttnArgs& a, const AttnGrads& o, const float* delta, hipStr
 
 // 16-byte loads and stores: every row and head starts at a multiple of them
 bool attn_vec(const AttnArgs& a, int size) {
-  const void* p[] = {a.q, a.k, a.v, a.out, a.grad};
+  const void* p[] = {a.q, a.k, a.v, a.out, a.grad, a.rest};
   for (const void* x : p)
     if (!chain_aligned16(x)) return false;
   const int64_t st[] = {a.q_row, a.q_head, a.k_row, a.k_head, a.v_row, a.v_head, a.dim};

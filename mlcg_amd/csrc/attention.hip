@@ -30,13 +30,13 @@ extern "C" int mlcg_chain_attention(const void* q, const int64_t* q_strides, con
                                     int buckets, const int32_t* bucket_of, int reach, float scale,
                                     const int32_t* tiles, int64_t n_tiles, int tile_rows,
                                     int splits, const uint8_t* keep, const int32_t* positions,
-                                    void* out, float* lse, void* stream) {
+                                    void* out, void* rest, float* lse, void* stream) {
   MLCG_REQUIRE(q_strides && k_strides && v_strides && kv_heads >= 1 && heads >= 1 &&
                heads % kv_heads == 0 && n_tiles >= 0 && n_tiles < (int64_t(1) << 31));
   AttnArgs a{q, k, v, table, out, nullptr, q_strides[0], q_strides[1], k_strides[0],
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, lse, (int)n_tiles, heads,
-             heads / kv_heads, dim, reach, buckets, scale};
+             heads / kv_heads, dim, reach, buckets, scale, rest};
   MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype, false));
   if (beads == 0 || n_tiles == 0) return MLCG_OK;
   MLCG_REQUIRE(q && k && v && table && bucket_of && tiles && out);
@@ -53,15 +53,16 @@ extern "C" int mlcg_chain_attention_backward(
     int dtype, const void* table, int buckets, const int32_t* bucket_of,
     const int32_t* bucket_order, const int32_t* bucket_first, int reach, float scale,
     const int32_t* tiles, int64_t n_tiles, int tile_rows, int splits, const uint8_t* keep,
-    const int32_t* positions, const void* out, const float* lse, const void* grad_out,
-    void* grad_q, void* grad_k, void* grad_v, void* grad_table, float* workspace,
+    const int32_t* positions, const void* out, const void* rest, const float* lse,
+    const void* grad_out, void* grad_q, void* grad_k, void* grad_v, void* grad_table, float* workspace,
     int64_t workspace_floats, void* stream) {
   MLCG_REQUIRE(q_strides && k_strides && v_strides && kv_heads >= 1 && heads >= 1 &&
                heads % kv_heads == 0 && n_tiles >= 1 && n_tiles < (int64_t(1) << 31));
   AttnArgs a{q, k, v, table, out, grad_out, q_strides[0], q_strides[1], k_strides[0],
              k_strides[1], v_strides[0], v_strides[1], beads, bucket_of,
              reinterpret_cast<const int4*>(tiles), keep, positions, const_cast<float*>(lse),
-             (int)n_tiles, heads, heads / kv_heads, dim, reach, buckets, scale};
+             (int)n_tiles, heads, heads / kv_heads, dim, reach, buckets, scale,
+             const_cast<void*>(rest)};
   MLCG_REQUIRE(attn_ok(a, tile_rows, splits, dtype, true) && beads >= 1);
   MLCG_REQUIRE(q && k && v && table && bucket_of && bucket_order && bucket_first && tiles && out &&
                lse && grad_out && grad_q && grad_k && grad_v && grad_table && workspace);

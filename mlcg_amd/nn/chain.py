@@ -28,19 +28,21 @@ from .mlp import init_xavier_uniform
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, chains, scale, keep, positions):
+        rest = None if q.dtype == torch.float32 else torch.empty(q.shape, dtype=q.dtype,
+                                                                 device=q.device)
         out, lse = ops.chain_attention(q, k, v, table, buckets, chains, scale, keep, positions,
-                                       want_lse=True)
-        ctx.save_for_backward(q, k, v, table, out, lse, keep, positions)
+                                       want_lse=True, rest=rest)
+        ctx.save_for_backward(q, k, v, table, out, lse, keep, positions, rest)
         ctx.plan = (buckets, chains, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, table, out, lse, keep, positions = ctx.saved_tensors
+        q, k, v, table, out, lse, keep, positions, rest = ctx.saved_tensors
         buckets, chains, scale = ctx.plan
         dq, dk, dv, dt = ops.chain_attention_backward(q, k, v, table, buckets, chains, out, lse,
-                                                      grad, scale, keep, positions)
+                                                      grad, scale, keep, positions, rest)
         return dq, dk, dv, dt, None, None, None, None, None
 
 

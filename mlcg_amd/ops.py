@@ -2028,10 +2028,19 @@ def _attention_shape_rule(chains: ChainLayout, heads: int, dim: int, dtype: torc
     return 128, 2 if groups <= 256 else 1
 
 
+def _check_rest(rest: Optional[torch.Tensor], out: torch.Tensor) -> None:
+    _check(rest is None or (rest.shape == out.shape and rest.dtype == out.dtype
+                            and rest.device == out.device and rest.is_contiguous()
+                            and out.dtype != torch.float32),
+           lambda: f"rest must be a contiguous {tuple(out.shape)} {out.dtype} on {out.device}, of "
+                   "a 16-bit type")
+
+
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
                     buckets: RelativeBuckets, chains: ChainLayout, scale: Optional[float] = None,
                     keep: Optional[torch.Tensor] = None,
-                    positions: Optional[torch.Tensor] = None, want_lse: bool = False
+                    positions: Optional[torch.Tensor] = None, want_lse: bool = False,
+                    rest: Optional[torch.Tensor] = None
                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(out [S, H, D], lse [H, S] | None): attention of every bead to the
     present beads of its chain with a bias by relative position
@@ -2042,16 +2051,19 @@ def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: to
     [num_buckets, H]; scale defaults to 1 / sqrt(D).  keep [S] bool: absent
     beads (False) are no keys, whatever their rows hold; a chain without a
     present bead gives zeros.  positions [S] int32 (residue numbers; the index
-    in the chain by default) give the offsets, clipped at the reach."""
+    in the chain by default) give the offsets, clipped at the reach.  rest
+    (like out; 16-bit types) takes what out's rounding leaves out, for a
+    backward pass whose table's gradient is as exact as the others."""
     (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions,
      rows, splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
     out = torch.empty(n, heads, dim, dtype=q.dtype, device=q.device)
+    _check_rest(rest, out)
     lse = torch.empty(heads, n, dtype=torch.float32, device=q.device) if want_lse else None
     tiles = chains.tiles[rows]
     call("mlcg_chain_attention", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim, dt,
          ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), buckets.reach, scale,
-         ptr(tiles), tiles.shape[0], rows, splits, ptr(keep), ptr(positions), ptr(out), ptr(lse),
-         stream_handle(q.device))
+         ptr(tiles), tiles.shape[0], rows, splits, ptr(keep), ptr(positions), ptr(out),
+         ptr(rest), ptr(lse), stream_handle(q.device))
     return out, lse
 
 
@@ -2059,9 +2071,10 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
                              out: torch.Tensor, lse: torch.Tensor, grad: torch.Tensor,
                              scale: Optional[float] = None,
                              keep: Optional[torch.Tensor] = None,
-                             positions: Optional[torch.Tensor] = None):
+                             positions: Optional[torch.Tensor] = None,
+                             rest: Optional[torch.Tensor] = None):
     """(grad q, grad k, grad v, grad table) of chain_attention for the gradient
-    of its output (mlcg_chain_attention_backward); out and lse are the
+    of its output (mlcg_chain_attention_backward); out, lse and rest are the
     forward's.  Every sum has a fixed order."""
     (q, qs, k, ks, v, vs, n, heads, kv, dim, dt, table, scale, keep, positions, rows,
      splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions, True)
@@ -2072,6 +2085,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
         _check(isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype
                and t.device == dev, lambda: f"{name} must be {shape} {dtype} on {dev}")
     out, lse, grad = out.contiguous(), lse.contiguous(), grad.contiguous()
+    _check_rest(rest, out)
     dq = torch.empty(n, heads, dim, dtype=q.dtype, device=dev)
     dk = torch.empty(n, kv, dim, dtype=q.dtype, device=dev)
     dv = torch.empty(n, kv, dim, dtype=q.dtype, device=dev)
@@ -2084,8 +2098,8 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     call("mlcg_chain_attention_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim,
          dt, ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), ptr(buckets.order),
          ptr(buckets.first), buckets.reach, scale, ptr(tiles), tiles.shape[0], rows, splits,
-         ptr(keep), ptr(positions), ptr(out), ptr(lse), ptr(grad), ptr(dq), ptr(dk), ptr(dv),
-         ptr(dtable), ptr(ws), nws, stream_handle(dev))
+         ptr(keep), ptr(positions), ptr(out), ptr(rest), ptr(lse), ptr(grad), ptr(dq), ptr(dk),
+         ptr(dv), ptr(dtable), ptr(ws), nws, stream_handle(dev))
     return dq, dk, dv, dtable
 
 

@@ -167,6 +167,22 @@ def test_attention_reach(reach, dim, dtype):
             _check_attention(q, k, v, table, b, chains, grad, positions=ps)
 
 
+def test_attention_table_gradient_of_a_long_chain():
+    """The table's gradient sums dS of millions of pairs, which nearly cancel:
+    it is off by its own rounding alone, at most u / sqrt(3) in the mean over a
+    binade, and by what the 32-bit sums leave (u / 16)."""
+    print("attention table gradient", flush=True)
+    q, k, v, table, b, chains, grad = _attention_case([2000], 2, 2, 64, torch.bfloat16, seed=4)
+    leaf = table.clone().requires_grad_(True)
+    from mlcg_amd import nn
+
+    got, = torch.autograd.grad(nn.chain_attention(q, k, v, leaf, b, chains), leaf, grad)
+    ref, _ = R.attention(q, k, v, table, b.bucket_of, chains.lengths, None, None, None, grad)
+    d = (got.cpu().double() - ref["table"]).norm() / ref["table"].norm()
+    u = U[torch.bfloat16]
+    assert float(d) <= u / math.sqrt(3.0) + u / 16.0, float(d)
+
+
 @pytest.mark.parametrize("kind,buckets,reach", [
     ("clip", 3, 1), ("clip", 65, 32), ("clip", 257, 128), ("log", 2, 5), ("log", 47, 100),
     ("log", 32, 1024), ("log", 16, 3)])
@@ -639,6 +655,10 @@ def test_refusals():
         args = dict(dict(q=q, k=k, v=k, table=table, buckets=b, chains=chains), **change)
         with pytest.raises(RuntimeError, match=match):
             nn.chain_attention(**args)
+    h = torch.float16
+    for rest in (q.to(h)[:9], q, q.to(h).transpose(0, 1)):
+        with pytest.raises(RuntimeError, match="rest must"):
+            ops.chain_attention(q.to(h), k.to(h), k.to(h), table.to(h), b, chains, rest=rest)
     x = torch.zeros(10, 12, device="cuda")
     w = torch.zeros(12, device="cuda")
     for args, match in (((x, w, w, 5, chains), "equal groups"), ((x[:9], w, w, 3, chains), "x must"),
