@@ -568,7 +568,8 @@ constexpr int fwd_waves() {
 // 57 % of the SIMDs' cycles and the products 24 %.  224 us, 613 TFLOP/s, 53 %
 // of a large library product's rate.  4 chains of 1031, 4 heads of 32 in fp32:
 // 47 us (46 TFLOP/s), 144 workgroups of 128 queries on 256 compute units.
-// 512 chains of up to 100, 4 heads of 32 in bf16: 20 us, one or two tiles a
+// 512 chains of up to 100, 4 heads of 32 in bf16: 20 us (25 with rest, 8-byte
+// stores of separate rows), one or two tiles a
 // workgroup, bound by the latency of its first loads.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void attn_fwd_kernel(
