@@ -59,6 +59,11 @@ constexpr int kAttnQ = 32;               // columns of a wave
 constexpr int kAttnSpan = 96;            // offsets beyond the reach that a block can touch
 constexpr float kAttnLog2e = 1.4426950408889634f;
 constexpr float kAttnLazy = 8.0f;        // the running maximum may lag by this many powers of two
+// A tile whose logits exceed the running maximum by more than this, or lie as
+// far below 0 when there was none, is formed once more about the new one: a
+// difference of 2^6 is rounded by 2^-18, as logits of that size are themselves,
+// but from a bias of -1e9 to an ordinary key nothing of the key would be left.
+constexpr float kAttnJump = 64.0f;
 
 struct AttnArgs {
   const void *q, *k, *v, *table, *out, *grad;
@@ -340,6 +345,22 @@ __device__ __forceinline__ void row_product(const T* tile, const v8<T> (&b)[DP /
         mma(s[n], row_frag<T, DP>(tile + 32 * n * DP, col, 16 * k + 8 * g), b[k]);
 }
 
+// Keeps the reads of the above two ahead of the products that take them (in 16
+// bits, where a product is shorter than the read's latency): hipcc otherwise
+// orders them read, wait, product.  READS: the 16-byte reads before the first.
+template <typename T, int DP, int N, int READS>
+__device__ __forceinline__ void reads_ahead() {
+  if constexpr (sizeof(T) == 2) {
+    constexpr int products = DP / 16 * N;
+    __builtin_amdgcn_sched_group_barrier(0x100, READS + 2, 0);  // LDS reads
+#pragma unroll
+    for (int i = 0; i < products; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+  }
+}
+
 // acc += tile^T . P  with P the 32 N rows of a lane's column
 template <typename T, int DP, int N>
 __device__ __forceinline__ void column_product(const T* tile, const float (&p)[16 * N],
@@ -501,16 +522,33 @@ struct QueryPlace {
   }
 };
 
+// The size of a row's shift from which on the logits are rounded before it is
+// taken off.  Below, it is taken off the bias first, so that a large bias that
+// all keys of a row have in common cancels and the products stay (the logits
+// then lie within half a spacing of the shift of 0: 2^6 in 32 bits, 1 in
+// fp16, whose probabilities have to fit it); beyond, the products vanish beside
+// a bias, or are themselves that large.
+template <typename T>
+constexpr float kAttnFar = std::is_same<T, _Float16>::value ? 0x1p24f : 0x1p31f;
+
+template <typename T>
+__device__ __forceinline__ bool far_shift(float shift) {
+  return fabsf(shift) >= kAttnFar<T> && fabsf(shift) < INFINITY;
+}
+
 // The logits (base 2) less `shift` of 32 N keys from kb on (rows) and the
-// wave's queries (lanes); returns the keys' side.
-template <int N, int POS>
+// wave's queries (lanes); returns the keys' side.  A shift of +inf: -inf.
+// any_far: whether far_shift holds for any of the wave's rows.
+template <typename T, int N, int POS>
 __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)[N],
                                             const float* ext, const float* cap, const int* kpos,
                                             int kb, const QueryPlace& q, float shift,
-                                            float (&x)[16 * N]) {
+                                            bool any_far, float (&x)[16 * N]) {
   const int lane = threadIdx.x & 63, g = lane >> 5;
   const float c = logit_factor(a);
   const int R = a.reach;
+  float near = shift;
+  if (__builtin_expect(any_far, 0)) near = far_shift<T>(shift) ? 0.0f : shift;
   int side;
   if (given_positions<POS>(a)) {
     const int kp = kpos[lane % (32 * N)];
@@ -522,17 +560,22 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
     side = block_side(kb - (q.first + 31), kb + 32 * N - 1 - q.first, R);
   }
   if (side) {
-    const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - shift;
+    const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - near;
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
   } else if (given_positions<POS>(a)) {
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i)
-      x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - shift);
+      x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kpos[acc_row(i, g)], q.pos, R)] - near);
   } else {
     const float* e = ext + (kb - q.mine + 4 * g + R + kAttnSpan);
 #pragma unroll
-    for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, e[acc_row(i, 0)] - shift);
+    for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, e[acc_row(i, 0)] - near);
+  }
+  if (__builtin_expect(any_far, 0)) {
+    const float rest = far_shift<T>(shift) ? shift : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16 * N; ++i) x[i] -= rest;
   }
   return side;
 }
@@ -606,7 +649,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   fill_bias<T>(a, head, ext);
 
   f32x16 acc[DP / 32] = {};
-  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  // the exponents are relative to base, the row's maximum so far or up to
+  // kAttnLazy below it; 0 before the row's first key
+  bool first = true, any_far = false;
+  float base = 0.0f, l = 0.0f;
   int buf = 0;
   // puts the tile of k0 into LDS and sends for the next one
   auto next_tile = [&](int k0) {
@@ -634,31 +680,47 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
     if (kb >= t.y) continue;
     const T* vt = L.v[buf] + RT * wk * DP;
     const float* cap = L.cap[buf] + RT * wk;
-    f32x16 s[N];
-    load_rows<N>(cap, s);
-    row_product<T, DP, N>(L.k[buf] + RT * wk * DP, qf, a.dim, s);
     float x[16 * N];
-    query_logits<N, POS>(a, s, ext, cap, L.kpos[buf] + RT * wk, kb, qi, base, x);
-    float top = x[0];
+    // a jump is known to a spacing of its larger end, at the second turn to a
+    // spacing of what is left, and at the third it is gone
+    constexpr int kAttnTurns = 3;
+#pragma unroll 1
+    for (int turn = 1;; ++turn) {
+      // nothing of the tile is kept in registers for another turn (hipcc would,
+      // and spill: 1053 us in place of 216 at 8191 beads)
+      asm volatile("" ::: "memory");
+      f32x16 s[N];
+      load_rows<N>(cap, s);
+      row_product<T, DP, N>(L.k[buf] + RT * wk * DP, qf, a.dim, s);
+      reads_ahead<T, DP, N, 4 * N>();
+      query_logits<T, N, POS>(a, s, ext, cap, L.kpos[buf] + RT * wk, kb, qi, base,
+                              any_far, x);
+      float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, x[i]);
-    // the maximum follows only where it has grown by more than 2^kAttnLazy
-    // (or there was none): the exponentials stay below 2^kAttnLazy, and most
-    // tiles leave the sums alone
-    if (__any(top > kAttnLazy || (m == -INFINITY && top > -INFINITY))) {
-      top = fmaxf(top, other_half(top)) + base;
-      m = fmaxf(m, top);
-      const float grown = m == -INFINITY ? 0.0f : m - base;  // no key so far: exp2(-inf) = 0
-      base += grown;
+      for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, x[i]);
+      // the base follows only where the maximum has grown by more than
+      // 2^kAttnLazy (or there was none): the exponentials stay below
+      // 2^kAttnLazy, and most tiles leave the sums alone
+      if (__builtin_expect(!__any(top > kAttnLazy || (first && top > -INFINITY)), 1)) break;
+      top = fmaxf(top, other_half(top));
+      const bool none = top == -INFINITY;  // no key so far: exp2(-inf) = 0
+      const float next = none ? base : first ? top : fmaxf(base, base + top);
+      // the difference of the two as they are kept, which the next tiles see
+      const float grown = next - base;
+      base = next;
+      any_far = __any(far_shift<T>(base));
       // nothing to scale before the first key, where the base may have to fall
       const float alpha = grown < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-grown);
+      first = first && none;
       l *= alpha;
-#pragma unroll
-      for (int i = 0; i < 16 * N; ++i) x[i] -= grown;
 #pragma unroll
       for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+      if (__builtin_expect(turn < kAttnTurns && __any(fabsf(grown) > kAttnJump), 0)) continue;
+#pragma unroll
+      for (int i = 0; i < 16 * N; ++i) x[i] -= grown;
+      break;
     }
     float sum[4] = {};
 #pragma unroll
@@ -674,7 +736,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
     // the parts on one maximum, then summed
     __shared__ float ms[NK][NQ][kAttnQ], ls[NK][NQ][kAttnQ];
     if (g == 0) {
-      ms[wk][wq][lane] = m;
+      ms[wk][wq][lane] = first ? -INFINITY : base;
       ls[wk][wq][lane] = l;
     }
     __syncthreads();
@@ -682,13 +744,13 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
     float top = ms[0][wq][c];
 #pragma unroll
     for (int p = 1; p < NK; ++p) top = fmaxf(top, ms[p][wq][c]);
+    const float mine = base;
     base = top == -INFINITY ? 0.0f : top;
     l = 0.0f;
 #pragma unroll
     for (int p = 0; p < NK; ++p)
       l = fmaf(ls[p][wq][c], __builtin_amdgcn_exp2f(ms[p][wq][c] - base), l);
-    const float f = __builtin_amdgcn_exp2f(m - base);
-    m = top;
+    const float f = first ? 0.0f : __builtin_amdgcn_exp2f(mine - base);
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -706,7 +768,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   if constexpr (sizeof(T) == 2)
     if (a.rest) store_rest<T, DP, VEC>((T*)a.rest + flat, acc, inv, a.dim);
   if (a.lse && g == 0)
-    a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : base + __builtin_amdgcn_logf(l);
 }
 
 // Whether a chain has one present key at most, of up to 64 beads.  The softmax
@@ -950,6 +1012,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   }
   delta += other_half(delta);
   const float lse = qi.ok ? a.lse[head * a.beads + row] : INFINITY;
+  const bool any_far = __any(far_shift<T>(lse));
   fill_bias<T>(a, head, ext);
   for (int i = threadIdx.x; i < NW * cells; i += NT) dd[i] = 0.0f;
   float* mine = dd + wave * cells;
@@ -993,7 +1056,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     load_rows<N>(cap, s);
     row_product<T, DP, N>(kt, qf, a.dim, s);
     float x[16 * N];
-    const int side = query_logits<N, POS>(a, s, ext, cap, kpos, kb, qi, lse, x);
+    const int side = query_logits<T, N, POS>(a, s, ext, cap, kpos, kb, qi, lse, any_far, x);
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] = f32x16{};
     row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, a.dim, s);  // dP

@@ -38,10 +38,9 @@ def attention(q, k, v, table, bucket_of, lengths, scale=None, keep=None, positio
             vv = torch.where(ok[:, None], v[r, s], 0.0)
             logit = (q[r, h] @ kk.T) * scale + table[cell, h]
             logit = logit.masked_fill(~ok[None, :], -math.inf)
-            if bool(ok.any()):
-                p = torch.softmax(logit, 1)
-            else:
-                p = torch.zeros_like(logit)
+            # a row that nothing is left of (no key, or biases of -inf alone) is 0
+            empty = (logit == -math.inf).all(1, keepdim=True)
+            p = torch.softmax(logit.masked_fill(empty, 0.0), 1).masked_fill(empty, 0.0)
             o = p @ vv
             val["out"][r, h] = o
             size["out"][r, h] = o.abs() + p @ vv.abs()
@@ -53,9 +52,9 @@ def attention(q, k, v, table, bucket_of, lengths, scale=None, keep=None, positio
             # delta is formed from the rounded output
             e = p * (g.abs() * o.abs()).sum(1, keepdim=True)
             val["q"][r, h] = ds @ kk * scale
-            size["q"][r, h] = (ds.abs() + e) @ kk.abs() * scale
+            size["q"][r, h] = (ds.abs() + e) @ kk.abs() * abs(scale)
             val["k"][r, s] += ds.T @ q[r, h] * scale
-            size["k"][r, s] += (ds.abs() + e).T @ q[r, h].abs() * scale
+            size["k"][r, s] += (ds.abs() + e).T @ q[r, h].abs() * abs(scale)
             val["v"][r, s] += p.T @ g
             size["v"][r, s] += p.T @ g.abs()
             flat = cell.reshape(-1).numpy()

@@ -1,0 +1,62 @@
+"""The attention over chains where its numbers are large, small or absent:
+biases that mask, common to a row or not, of the type's ends and infinite, and
+the accuracy of what the gradients are formed from.  The bounds are those of
+test_gpu_chain.py (the logits' roundings are of the products' size, whatever
+the size of the biases that cancel) unless a test derives its own."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import chain_ref as R
+from tests.test_gpu_chain import TYPES, U, _attention_case
+
+pytestmark = pytest.mark.gpu
+
+
+def _masked_case(lens, heads, kv, dim, dtype, bias, seed=0):
+    """A band of 8 beads of ordinary biases, `bias` beyond it."""
+    q, k, v, table, b, chains, grad = _attention_case(lens, heads, kv, dim, dtype, seed=seed,
+                                                      kind="clip", buckets=17, reach=8)
+    table = table.clone()
+    table[0] = table[-1] = bias
+    return q, k, v, table, b, chains, grad
+
+
+def _biases(dtype):
+    info = torch.finfo(dtype)
+    common = [-1e4, info.min, info.max, -math.inf]
+    return common if dtype == torch.float16 else [*common, -1e8, -1e9, 1e9]
+
+
+RANGE = [(t, b) for t in TYPES for b in _biases(t)]
+
+
+@pytest.mark.parametrize("dtype,bias", RANGE)
+@pytest.mark.parametrize("lens", [[40, 33], [300, 90], [300] * 12, [130] * 70])
+def test_forward_of_masking_biases(lens, dtype, bias):
+    """Keys beyond the band come before and after ordinary ones, and the bias is
+    the same for all keys of some rows: it cancels, or leaves nothing."""
+    from mlcg_amd import nn
+
+    print(f"masking biases {lens[0]} {dtype} {bias}", flush=True)
+    q, k, v, table, b, chains, _ = _masked_case(lens, 2, 1, 32, dtype, bias)
+    s = sum(lens)
+    keep = torch.ones(s, dtype=torch.bool)
+    keep[:lens[0]] = False
+    keep[lens[0] - 20:lens[0] - 3] = True
+    pos = torch.cumsum((torch.rand(s, generator=torch.Generator().manual_seed(1)) < 0.4).int(),
+                       0).to(torch.int32).cuda()
+    u = U[dtype]
+    parts = 64.0 if dtype == torch.float32 else 1.25
+    for kp in (None, keep.cuda()):
+        for ps in (None, pos):
+            out = nn.chain_attention(q, k, v, table, b, chains, keep=kp, positions=ps)
+            ref, size = R.attention(q, k, v, table, b.bucket_of, lens, None, kp, ps)
+            floor = (4.0 * u if dtype == torch.float32 else 64 * 2.0 ** -24) * float(
+                size["out"].max())
+            d = (out.cpu().double() - ref["out"]).abs()
+            bad = ~(d <= parts * u * size["out"] + floor + 2.0 ** -24)
+            assert not bool(bad.any()), (
+                f"{int(bad.sum())} of {bad.numel()} off, worst {float(d.max())}")
