@@ -1026,8 +1026,9 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * [0, buckets); 1 <= reach <= 1024, 1 <= dim <= 128.  keep [beads]: 0 marks an
  * absent bead, whose key and value are not read as numbers (NULL: all are
  * present); positions [beads]: p, any int32 (NULL: the index in the chain).
- * out [beads, heads, dim]; lse [heads, beads] (may be NULL): the base-2 log of
- * the row's sum, +inf for a row without keys, which the backward pass takes.
+ * out [beads, heads, dim]; lse [2, heads, beads] (may be NULL): m and l of the
+ * row's log-sum m + log2 l in base 2, +inf and 0 for a row without keys, which
+ * the backward pass takes.
  * rest [beads, heads, dim] (16-bit types; may be NULL): what the rounding of out
  * leaves out, from which the backward pass has its row sums in full.
  * tile_rows, 32, 64 or 128: the rows of the tiles in `tiles`; splits, 1 or, with

@@ -12,8 +12,10 @@
 //   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
 //   dv_j = sum_i P_ij do_i,  dtable[b, h] = sum of dS_ij over the pairs in b.
 // Neither the bias nor the probabilities are ever stored: the forward pass
-// keeps the running maximum and sum of every row (base-2 exponents) and the
-// log of the sum, from which the backward passes form P again.
+// keeps a running maximum m and sum l of every row (base-2 exponents), apart,
+// from which the backward passes form P = exp2(l_ij log2(e) - m) / l again: in
+// one number with m, log2 l would be lost beside a large bias that all of a
+// row's keys have in common.
 //
 // Tiles: a wave owns 32 queries (forward, dq) or 32 keys (dk, dv) as the
 // columns of 32 x 32 MFMA tiles, so a lane is one query (key) and the softmax
@@ -56,6 +58,7 @@
 #include "chain.h"
 
 constexpr int kAttnQ = 32;               // columns of a wave
+constexpr int kAttnWaves = 4;            // waves of columns of a workgroup, at most
 constexpr int kAttnSpan = 96;            // offsets beyond the reach that a block can touch
 constexpr float kAttnLog2e = 1.4426950408889634f;
 constexpr float kAttnLazy = 8.0f;        // the running maximum may lag by this many powers of two
@@ -73,7 +76,7 @@ struct AttnArgs {
   const int4* tiles;         // (chain's first row, its length, tile's first row in it, chain)
   const uint8_t* keep;
   const int32_t* pos;
-  float* lse;  // [heads][beads], base 2; +inf for a row without keys
+  float* lse;  // [2][heads][beads]: m, +inf for a row without keys, and l
   int n_tiles, heads, group, dim, reach, buckets;
   float scale;
   void* rest;  // what the rounding of out leaves out, or NULL
@@ -82,6 +85,13 @@ struct AttnArgs {
 // Whether positions are given: known when the kernel is built, or (kEither, in
 // the form without 16-byte loads) when it runs.
 enum { kIndex = 0, kGiven = 1, kEither = 2 };
+
+// What dq leaves for dk and dv of every row [heads][beads], and of every wave of
+// queries [heads][tiles][waves].
+struct AttnRows {
+  float *delta, *start;  // do . o;  -(m + log2 l) / c
+  float* apart;          // whether m is too large for start to take its place
+};
 
 struct AttnGrads {
   void *dq, *dk, *dv, *dtable;
@@ -767,8 +777,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   // of its gradient against 1.7e-3)
   if constexpr (sizeof(T) == 2)
     if (a.rest) store_rest<T, DP, VEC>((T*)a.rest + flat, acc, inv, a.dim);
-  if (a.lse && g == 0)
-    a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : base + __builtin_amdgcn_logf(l);
+  if (a.lse && g == 0) {
+    a.lse[head * a.beads + row] = l == 0.0f ? INFINITY : base;
+    a.lse[(a.heads + head) * a.beads + row] = l;
+  }
 }
 
 // Whether a chain has one present key at most, of up to 64 beads.  The softmax
@@ -930,6 +942,11 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
   return positions ? (2 * (2 * reach + 1) + 3) & ~3 : diag_floats<DP>();
 }
 
+// Up to this |m| the sums that dk and dv form a row's logits from begin with
+// -(m + log2 l) / c, so that they leave nothing to subtract (rounded by 2^-16
+// there, below a 16-bit factor's 2^-12).
+constexpr float kAttnFold = 512.0f;
+
 template <typename T, int DP, int NQ, int NK>
 struct DqLds {
   static constexpr int KS = part_rows_bwd<T, DP>() * NK;
@@ -955,9 +972,8 @@ constexpr int dq_waves() {
 // workgroups a compute unit instead of three).  4 chains of 1031, 4 heads of 32 in fp32: 74 us.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
-    AttnArgs a, T* __restrict__ dq, float* __restrict__ delta_out,
-    const int32_t* __restrict__ order, const int32_t* __restrict__ first,
-    float* __restrict__ dtable_part) {
+    AttnArgs a, T* __restrict__ dq, AttnRows rows_out, const int32_t* __restrict__ order,
+    const int32_t* __restrict__ first, float* __restrict__ dtable_part) {
   constexpr int RT = part_rows_bwd<T, DP>(), N = RT / 32, KS = RT * NK, NW = NQ * NK, NT = 64 * NW;
   using Lds = DqLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -1011,8 +1027,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
       delta = fmaf((float)gf[k][e], (float)of[e] + (float)rf[e], delta);
   }
   delta += other_half(delta);
-  const float lse = qi.ok ? a.lse[head * a.beads + row] : INFINITY;
-  const bool any_far = __any(far_shift<T>(lse));
+  const float m = qi.ok ? a.lse[head * a.beads + row] : INFINITY;
+  const float l = qi.ok ? a.lse[(a.heads + head) * a.beads + row] : 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, delta_inv = delta * inv;
+  const bool any_far = __any(far_shift<T>(m));
   fill_bias<T>(a, head, ext);
   for (int i = threadIdx.x; i < NW * cells; i += NT) dd[i] = 0.0f;
   float* mine = dd + wave * cells;
@@ -1056,13 +1074,13 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     load_rows<N>(cap, s);
     row_product<T, DP, N>(kt, qf, a.dim, s);
     float x[16 * N];
-    const int side = query_logits<T, N, POS>(a, s, ext, cap, kpos, kb, qi, lse, any_far, x);
+    const int side = query_logits<T, N, POS>(a, s, ext, cap, kpos, kb, qi, m, any_far, x);
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] = f32x16{};
     row_product<T, DP, N>(L.v[buf] + RT * wk * DP, gf, a.dim, s);  // dP
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i)
-      x[i] = __builtin_amdgcn_exp2f(x[i]) * (s[i / 16][i % 16] - delta);
+      x[i] = __builtin_amdgcn_exp2f(x[i]) * fmaf(s[i / 16][i % 16], inv, -delta_inv);
     if (side) {
       float sum[4] = {};
 #pragma unroll
@@ -1116,7 +1134,17 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
   if (qi.ok && wk == 0) {
     store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
-    if (g == 0) delta_out[head * a.beads + row] = delta;
+    if (g == 0) {
+      rows_out.delta[head * a.beads + row] = delta;
+      // -inf logits for a row without keys
+      const float sum = l == 0.0f ? -INFINITY : -(m + __builtin_amdgcn_logf(l));
+      rows_out.start[head * a.beads + row] = sum / logit_factor(a);
+    }
+  }
+  if (wk == 0) {
+    const bool any = __any(fabsf(m) >= kAttnFold && m < INFINITY);
+    if (lane == 0)
+      rows_out.apart[((int64_t)head * a.n_tiles + tile) * NQ + wq] = any ? 1.0f : 0.0f;
   }
   flush_offsets<NT>(a, dd, cells, order, first, part);
 }
@@ -1125,7 +1153,9 @@ template <typename T, int DP, int NQ, int NK>
 struct DkvLds {
   static constexpr int KS = part_rows_bwd<T, DP>() * NK;
   T q[2][KS * DP], g[2][KS * DP];
-  float lse[2][KS], delta[2][KS];
+  float start[2][KS];             // of the sums, or
+  float m[2][KS], inv[2][KS];     // m and 1 / l
+  float delta[2][KS];
   int qpos[2][KS];
   float ext[1];
 };
@@ -1145,7 +1175,7 @@ constexpr int dkv_waves() {
 // of 1031, 4 heads of 32 in fp32: 81 us (54 TFLOP/s; 144 workgroups).
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
-    AttnArgs a, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv) {
+    AttnArgs a, AttnRows rows_in, T* __restrict__ dk, T* __restrict__ dv) {
   constexpr int RT = part_rows_bwd<T, DP>(), N = RT / 32, KS = RT * NK, NT = 64 * NQ * NK;
   using Lds = DkvLds<T, DP, NQ, NK>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -1154,7 +1184,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 
   const int kv_heads = a.heads / a.group;
   const int kv = blockIdx.x % kv_heads;
-  const int4 t = a.tiles[blockIdx.x / kv_heads];
+  const int tile = blockIdx.x / kv_heads;
+  const int4 t = a.tiles[tile];
   const int lane = threadIdx.x & 63, g = lane >> 5, wave = wave_number();
   const int wq = wave % NQ, wk = wave / NQ;
   const int kw = t.z + kAttnQ * wq, ki = kw + (lane & 31);
@@ -1175,7 +1206,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     }
     return;
   }
-  // the sums of the logits begin with -lse / c, those of dP with -delta
+  // the sums of dP begin with -delta
   const float c = logit_factor(a);
   const int R = a.reach;
 
@@ -1184,23 +1215,37 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
   gs.init(a.heads * a.dim, a.dim);
   typename Stage<T, DP, KS, NT, VEC>::Rows absent;
   const bool given = given_positions<POS>(a);
-  float lse_n = INFINITY, delta_n = 0.0f;
+  float start_n = 0.0f, m_n = 0.0f, l_n = 0.0f, delta_n = 0.0f;
   int pos_n = 0;
-  auto load = [&](int head, int q0) {
+  auto load = [&](int head, int q0, bool folded, bool apart) {
     const int64_t row0 = (int64_t)t.x + q0;
     qs.load((const T*)a.q + row0 * a.q_row + head * a.q_head, t.y - q0, a.dim);
     gs.load((const T*)a.grad + (row0 * a.heads + head) * a.dim, t.y - q0, a.dim);
     if (q0 + KS > t.y) absent.load(nullptr, t.y - q0);
     const int i = threadIdx.x;
-    lse_n = INFINITY;  // exp2(-inf) = 0 for the rows past the end
-    delta_n = 0.0f;
+    // exp2(-inf) = 0 for the rows past the end
+    start_n = c > 0.0f ? -INFINITY : INFINITY;
+    m_n = INFINITY;
+    l_n = delta_n = 0.0f;
     if (i < KS && q0 + i < t.y) {
-      lse_n = a.lse[head * a.beads + row0 + i];
-      delta_n = delta[head * a.beads + row0 + i];
+      const int64_t at = head * a.beads + row0 + i;
+      if (folded) start_n = rows_in.start[at];
+      if (apart) {
+        m_n = a.lse[at];
+        l_n = a.lse[a.heads * a.beads + at];
+      }
+      delta_n = rows_in.delta[at];
       if (given) pos_n = a.pos[row0 + i];
     }
   };
-  load(kv * a.group, 0);
+  load(kv * a.group, 0, true, true);
+  // any large m among the chain's queries of these heads
+  float large = 0.0f;
+  for (int h = 0; h < a.group; ++h) {
+    const int64_t at = (int64_t)(kv * a.group + h) * a.n_tiles + tile - t.z / (kAttnQ * NQ);
+    for (int i = lane; i < (t.y + kAttnQ - 1) / kAttnQ; i += 64)
+      large = fmaxf(large, rows_in.apart[at * NQ + i]);
+  }
 
   const T* k = (const T*)a.k + row * a.k_row + kv * a.k_head;
   const T* v = (const T*)a.v + row * a.v_row + kv * a.v_head;
@@ -1219,75 +1264,102 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
   int buf = 0;
-  // puts the tile of q0 into LDS and sends for the next one
-  auto next_tile = [&](int h, int q0) {
-    if (q0 + KS > t.y) {
-      qs.drop(absent);
-      gs.drop(absent);
+  auto all_queries = [&](auto fold) {
+    constexpr bool FOLD = decltype(fold)::value;
+    // puts the tile of q0 into LDS and sends for the next one
+    auto next_tile = [&](int h, int q0) {
+      if (q0 + KS > t.y) {
+        qs.drop(absent);
+        gs.drop(absent);
+      }
+      qs.put(L.q[buf]);
+      gs.put(L.g[buf]);
+      if ((int)threadIdx.x < KS) {
+        if (FOLD) {
+          L.start[buf][threadIdx.x] = start_n;
+        } else {
+          L.m[buf][threadIdx.x] = m_n;
+          L.inv[buf][threadIdx.x] = l_n == 0.0f ? 0.0f : 1.0f / l_n;
+        }
+        L.delta[buf][threadIdx.x] = -delta_n;
+        if (POS != kIndex) L.qpos[buf][threadIdx.x] = pos_n;
+      }
+      if (q0 + KS < t.y)
+        load(kv * a.group + h, q0 + KS, FOLD, !FOLD);
+      else if (h + 1 < a.group)
+        load(kv * a.group + h + 1, 0, FOLD, !FOLD);
+      __syncthreads();
+    };
+    for (int h = 0; h < a.group; ++h) {
+      const int head = kv * a.group + h;
+      if (h > 0) __syncthreads();
+      fill_bias<T>(a, head, ext);
+      if (kw >= t.y)  // no keys: this wave only loads
+        for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) next_tile(h, q0);
+      else for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
+        next_tile(h, q0);
+        const int qb = q0 + RT * wk;
+        if (qb >= t.y) continue;
+        const T* qt = L.q[buf] + RT * wk * DP;
+        const T* gt = L.g[buf] + RT * wk * DP;
+        const int* qpos = L.qpos[buf] + RT * wk;
+        const float* mrow = L.m[buf] + RT * wk;
+        f32x16 s[N] = {};
+        if constexpr (FOLD) load_rows<N>(L.start[buf] + RT * wk, s);
+        row_product<T, DP, N>(qt, kf, a.dim, s);
+        float x[16 * N];
+        // from the bias of row i
+        auto logits = [&](auto bias) {
+          if constexpr (FOLD) {
+#pragma unroll
+            for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, bias(i));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16 * N; ++i) {
+              const float m = mrow[acc_row(i, g)], b = bias(i);
+              x[i] = far_shift<T>(m) ? fmaf(s[i / 16][i % 16], c, b) - m
+                                     : fmaf(s[i / 16][i % 16], c, b - m);
+            }
+          }
+        };
+        int side;
+        if (given) {
+          const int qp = qpos[lane % RT];
+          const bool past = qb + lane % RT >= t.y;
+          side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
+                 : __all(past || __builtin_elementwise_sub_sat(khi, qp) <= -R) ? -1
+                                                                               : 0;
+        } else {
+          side = block_side(kw - (qb + RT - 1), kw + 31 - qb, R);
+        }
+        if (side) {
+          const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+          logits([=](int) { return b; });
+        } else if (given) {
+          logits([=](int i) { return ext[offset_cell(kp, qpos[acc_row(i, g)], R)]; });
+        } else {
+          const float* e = ext + (ki - qb - 4 * g + R + kAttnSpan);
+          logits([=](int i) { return e[-acc_row(i, 0)]; });
+        }
+        load_rows<N>(L.delta[buf] + RT * wk, s);
+        row_product<T, DP, N>(gt, vf, a.dim, s);  // dP - delta
+#pragma unroll
+        for (int i = 0; i < 16 * N; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
+        if constexpr (!FOLD) {
+#pragma unroll
+          for (int i = 0; i < 16 * N; ++i) x[i] *= L.inv[buf][RT * wk + acc_row(i, g)];
+        }
+        column_product<T, DP, N>(gt, x, dva);
+#pragma unroll
+        for (int i = 0; i < 16 * N; ++i) x[i] *= s[i / 16][i % 16];
+        column_product<T, DP, N>(qt, x, dka);
+      }
     }
-    qs.put(L.q[buf]);
-    gs.put(L.g[buf]);
-    if ((int)threadIdx.x < KS) {
-      L.lse[buf][threadIdx.x] = -lse_n / c;
-      L.delta[buf][threadIdx.x] = -delta_n;
-      if (POS != kIndex) L.qpos[buf][threadIdx.x] = pos_n;
-    }
-    if (q0 + KS < t.y)
-      load(kv * a.group + h, q0 + KS);
-    else if (h + 1 < a.group)
-      load(kv * a.group + h + 1, 0);
-    __syncthreads();
   };
-  for (int h = 0; h < a.group; ++h) {
-    const int head = kv * a.group + h;
-    if (h > 0) __syncthreads();
-    fill_bias<T>(a, head, ext);
-    if (kw >= t.y)  // no keys: this wave only loads
-      for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) next_tile(h, q0);
-    else for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
-      next_tile(h, q0);
-      const int qb = q0 + RT * wk;
-      if (qb >= t.y) continue;
-      const T* qt = L.q[buf] + RT * wk * DP;
-      const T* gt = L.g[buf] + RT * wk * DP;
-      const int* qpos = L.qpos[buf] + RT * wk;
-      f32x16 s[N];
-      load_rows<N>(L.lse[buf] + RT * wk, s);
-      row_product<T, DP, N>(qt, kf, a.dim, s);
-      float x[16 * N];
-      int side;
-      if (given) {
-        const int qp = qpos[lane % RT];
-        const bool past = qb + lane % RT >= t.y;
-        side = __all(past || __builtin_elementwise_sub_sat(klo, qp) >= R)    ? 1
-               : __all(past || __builtin_elementwise_sub_sat(khi, qp) <= -R) ? -1
-                                                                             : 0;
-      } else {
-        side = block_side(kw - (qb + RT - 1), kw + 31 - qb, R);
-      }
-      if (side) {
-        const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
-#pragma unroll
-        for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
-      } else if (given) {
-#pragma unroll
-        for (int i = 0; i < 16 * N; ++i)
-          x[i] = fmaf(s[i / 16][i % 16], c, ext[offset_cell(kp, qpos[acc_row(i, g)], R)]);
-      } else {
-        const float* e = ext + (ki - qb - 4 * g + R + kAttnSpan);
-#pragma unroll
-        for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, e[-acc_row(i, 0)]);
-      }
-      load_rows<N>(L.delta[buf] + RT * wk, s);
-      row_product<T, DP, N>(gt, vf, a.dim, s);  // dP - delta
-#pragma unroll
-      for (int i = 0; i < 16 * N; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
-      column_product<T, DP, N>(gt, x, dva);
-#pragma unroll
-      for (int i = 0; i < 16 * N; ++i) x[i] *= s[i / 16][i % 16];
-      column_product<T, DP, N>(qt, x, dka);
-    }
-  }
+  if (__any(large != 0.0f))
+    all_queries(std::false_type());
+  else
+    all_queries(std::true_type());
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
   join_parts<DP, NQ, NK>(dva, reinterpret_cast<float*>(smem));
   if (!in || wk > 0) return;
@@ -1345,7 +1417,8 @@ int launch_fwd(const AttnArgs& a, void* out, hipStream_t s) {
 }
 
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
-int launch_dq(const AttnArgs& a, const AttnGrads& o, float* delta, float* part, hipStream_t s) {
+int launch_dq(const AttnArgs& a, const AttnGrads& o, const AttnRows& rows, float* part,
+              hipStream_t s) {
   constexpr unsigned NW = NQ * NK;
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds = sizeof(DqLds<T, DP, NQ, NK>) +
@@ -1353,18 +1426,18 @@ int launch_dq(const AttnArgs& a, const AttnGrads& o, float* delta, float* part, 
   auto f = attn_dq_kernel<T, DP, NQ, NK, VEC, POS>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
   hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * a.heads)), dim3(64 * NW), lds, s, a,
-                     (T*)o.dq, delta, o.order, o.first, part);
+                     (T*)o.dq, rows, o.order, o.first, part);
   return mlcg_launch_status();
 }
 
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
-int launch_dkv(const AttnArgs& a, const AttnGrads& o, const float* delta, hipStream_t s) {
+int launch_dkv(const AttnArgs& a, const AttnGrads& o, const AttnRows& rows, hipStream_t s) {
   const unsigned cells = 2 * (a.reach + kAttnSpan) + 1;
   const unsigned lds = sizeof(DkvLds<T, DP, NQ, NK>) + 4 * cells;
   auto f = attn_dkv_kernel<T, DP, NQ, NK, VEC, POS>;
   if (int e = allow_lds(reinterpret_cast<const void*>(f), lds)) return e;
   hipLaunchKernelGGL(f, dim3((unsigned)(a.n_tiles * (a.heads / a.group))), dim3(64 * NQ * NK), lds,
-                     s, a, delta, (T*)o.dk, (T*)o.dv);
+                     s, a, rows, (T*)o.dk, (T*)o.dv);
   return mlcg_launch_status();
 }
 
@@ -1429,12 +1502,13 @@ int attn_forward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, void* out, hipStrea
 template <>
 int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o, hipStream_t s) {
   using T = MLCG_ATTENTION_TYPE;
-  float* delta = o.ws;
-  float* part = o.ws + a.heads * a.beads;
+  const int64_t n = a.heads * a.beads, tiles = (int64_t)a.heads * a.n_tiles;
+  const AttnRows rows{o.ws, o.ws + n, o.ws + 2 * n};
+  float* part = rows.apart + kAttnWaves * tiles;
   if (int e = by_shape<(int)sizeof(T), false>(a, shape, [&](auto dp, auto nq, auto nk, auto vec,
                                                             auto pos) {
         return launch_dq<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
-                         decltype(vec)::value, decltype(pos)::value>(a, o, delta, part, s);
+                         decltype(vec)::value, decltype(pos)::value>(a, o, rows, part, s);
       }))
     return e;
   // keys of shared heads give fewer workgroups than queries: where they are no
@@ -1445,7 +1519,7 @@ int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o
   if (int e = by_shape<(int)sizeof(T), false>(a, kv_shape, [&](auto dp, auto nq, auto nk,
                                                                auto vec, auto pos) {
         return launch_dkv<T, decltype(dp)::value, decltype(nq)::value, decltype(nk)::value,
-                          decltype(vec)::value, decltype(pos)::value>(a, o, delta, s);
+                          decltype(vec)::value, decltype(pos)::value>(a, o, rows, s);
       }))
     return e;
   hipLaunchKernelGGL(attn_dtable_kernel<T>, dim3(mlcg_div_up(a.buckets, 8), a.heads), dim3(256), 0,

@@ -20,7 +20,7 @@ bool attn_ok(const AttnArgs& a, int tile_rows, int splits, int dtype, bool backw
 extern "C" int64_t mlcg_chain_attention_workspace_floats(int64_t beads, int heads,
                                                          int64_t n_tiles, int buckets) {
   if (beads < 0 || heads < 1 || n_tiles < 0 || buckets < 1) return -1;
-  return heads * (beads + n_tiles * buckets);
+  return heads * (2 * beads + n_tiles * (kAttnWaves + buckets));
 }
 
 extern "C" int mlcg_chain_attention(const void* q, const int64_t* q_strides, const void* k,

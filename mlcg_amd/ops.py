@@ -2042,9 +2042,11 @@ def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: to
                     positions: Optional[torch.Tensor] = None, want_lse: bool = False,
                     rest: Optional[torch.Tensor] = None
                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """(out [S, H, D], lse [H, S] | None): attention of every bead to the
+    """(out [S, H, D], lse [2, H, S] | None): attention of every bead to the
     present beads of its chain with a bias by relative position
     (mlcg_chain_attention): logits scale q_i.k_j + table[bucket(p_j - p_i), h].
+    lse, for the backward pass, is the row's log-sum in two parts, m and l of
+    m + log2 l in base 2 (m = +inf and l = 0 for a row without keys).
 
     q [S, H, D], k and v [S, KV, D] (H a multiple of KV; views with any row
     and head stride, e.g. slices of one projection), table
@@ -2058,7 +2060,7 @@ def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: to
      rows, splits) = _attention_args(q, k, v, table, buckets, chains, scale, keep, positions)
     out = torch.empty(n, heads, dim, dtype=q.dtype, device=q.device)
     _check_rest(rest, out)
-    lse = torch.empty(heads, n, dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty(2, heads, n, dtype=torch.float32, device=q.device) if want_lse else None
     tiles = chains.tiles[rows]
     call("mlcg_chain_attention", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim, dt,
          ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), buckets.reach, scale,
@@ -2081,7 +2083,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
     dev = q.device
     for t, name, shape, dtype in ((out, "out", (n, heads, dim), q.dtype),
                                   (grad, "grad", (n, heads, dim), q.dtype),
-                                  (lse, "lse", (heads, n), torch.float32)):
+                                  (lse, "lse", (2, heads, n), torch.float32)):
         _check(isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype
                and t.device == dev, lambda: f"{name} must be {shape} {dtype} on {dev}")
     out, lse, grad = out.contiguous(), lse.contiguous(), grad.contiguous()
@@ -2093,7 +2095,7 @@ def chain_attention_backward(q, k, v, table, buckets: RelativeBuckets, chains: C
         return dq, dk, dv, torch.zeros_like(table)
     dtable = torch.empty_like(table)
     tiles = chains.tiles[rows]
-    nws = heads * (n + tiles.shape[0] * buckets.num_buckets)
+    nws = heads * (2 * n + tiles.shape[0] * (4 + buckets.num_buckets))
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     call("mlcg_chain_attention_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, n, heads, kv, dim,
          dt, ptr(table), buckets.num_buckets, ptr(buckets.bucket_of), ptr(buckets.order),

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import chain_ref as R
-from tests.test_gpu_chain import TYPES, U, _attention_case
+from tests.test_gpu_chain import TYPES, U, _attention_case, _check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,21 @@ def test_forward_of_masking_biases(lens, dtype, bias):
             bad = ~(d <= parts * u * size["out"] + floor + 2.0 ** -24)
             assert not bool(bad.any()), (
                 f"{int(bad.sum())} of {bad.numel()} off, worst {float(d.max())}")
+
+
+@pytest.mark.parametrize("dtype,bias", RANGE)
+@pytest.mark.parametrize("lens,dim,scale", [([40, 33], 32, None), ([300, 90], 32, None),
+                                            ([300, 90], 64, -0.2), ([300, 90], 128, None),
+                                            ([300] * 12, 32, None), ([130] * 70, 24, None)])
+def test_gradients_of_masking_biases(lens, dim, scale, dtype, bias):
+    print(f"gradients, masking biases {lens[0]} {dim} {dtype} {bias}", flush=True)
+    q, k, v, table, b, chains, grad = _masked_case(lens, 2, 1, dim, dtype, bias, seed=dim)
+    s = sum(lens)
+    keep = torch.ones(s, dtype=torch.bool)
+    keep[:lens[0]] = False
+    keep[lens[0] - 20:lens[0] - 3] = True
+    pos = torch.cumsum((torch.rand(s, generator=torch.Generator().manual_seed(1)) < 0.4).int(),
+                       0).to(torch.int32).cuda()
+    for kp in (None, keep.cuda()):
+        for ps in (None, pos):
+            _check_attention(q, k, v, table, b, chains, grad, scale, kp, ps)
