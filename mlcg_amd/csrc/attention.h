@@ -785,7 +785,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
 
 // Whether a chain has one present key at most, of up to 64 beads.  The softmax
 // over one key is constant: the backward passes then write dq = dk = 0 and dv
-// the sum of do, not what the roundings of their sums would leave of them.
+// the sum of do over the rows that have the key (a bias of -inf may take it from
+// a row: l = 0), not what the roundings of their sums would leave of them.  A
+// row whose l is no number makes them none, too: l - l.
 __device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
   if (len > 64) return false;
   const int lane = threadIdx.x & 63;
@@ -992,8 +994,11 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   const uint8_t* keep = a.keep ? a.keep + t.x : nullptr;
   float* part = dtable_part + ((int64_t)head * a.n_tiles + tile) * a.buckets;
   if (lone_key(keep, t.y)) {
-    for (int i = threadIdx.x; i < min(kAttnQ * NQ, t.y - t.z) * a.dim; i += NT)
-      dq[((int64_t)(t.x + t.z + i / a.dim) * a.heads + head) * a.dim + i % a.dim] = (T)0.0f;
+    for (int i = threadIdx.x; i < min(kAttnQ * NQ, t.y - t.z) * a.dim; i += NT) {
+      const int64_t r = t.x + t.z + i / a.dim;
+      const float l = a.lse[(a.heads + head) * a.beads + r];
+      dq[(r * a.heads + head) * a.dim + i % a.dim] = (T)(l - l);
+    }
     for (int i = threadIdx.x; i < a.buckets; i += NT) part[i] = 0.0f;
     return;
   }
@@ -1195,14 +1200,18 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     for (int i = threadIdx.x; i < min(kAttnQ * NQ, t.y - t.z) * a.dim; i += NT) {
       const int64_t r = t.x + t.z + i / a.dim;
       const int d = i % a.dim;
-      float sum = 0.0f;
+      float sum = 0.0f, zero = 0.0f;
       if (!a.keep || a.keep[r])
         for (int j = 0; j < t.y; ++j)
-          for (int h = 0; h < a.group; ++h)
-            sum += (float)((const T*)a.grad)[((int64_t)(t.x + j) * a.heads + kv * a.group + h) *
-                                                 a.dim + d];
-      dk[(r * kv_heads + kv) * a.dim + d] = (T)0.0f;
-      dv[(r * kv_heads + kv) * a.dim + d] = (T)sum;
+          for (int h = 0; h < a.group; ++h) {
+            const int head = kv * a.group + h;
+            const float l = a.lse[(a.heads + head) * a.beads + t.x + j];
+            zero += l - l;
+            if (l != 0.0f)
+              sum += (float)((const T*)a.grad)[((int64_t)(t.x + j) * a.heads + head) * a.dim + d];
+          }
+      dk[(r * kv_heads + kv) * a.dim + d] = (T)zero;
+      dv[(r * kv_heads + kv) * a.dim + d] = (T)(sum + zero);
     }
     return;
   }

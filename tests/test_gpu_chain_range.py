@@ -78,3 +78,29 @@ def test_gradients_of_masking_biases(lens, dim, scale, dtype, bias):
     for kp in (None, keep.cuda()):
         for ps in (None, pos):
             _check_attention(q, k, v, table, b, chains, grad, scale, kp, ps)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_single_key_that_a_bias_takes_away(n, dtype):
+    """One present key, which the bias of some offsets takes away: these rows
+    are empty and give dv nothing; a logit that is no number stays one."""
+    from mlcg_amd import nn, ops
+
+    print(f"single key {n} {dtype}", flush=True)
+    q, k, v, _, _, chains, grad = _attention_case([n, 3], 2, 1, 16, dtype)
+    b = ops.relative_buckets(3, 1, "clip")
+    table = torch.zeros(3, 2, dtype=dtype, device="cuda")
+    table[0, 0] = table[1, 1] = -math.inf  # head 0 later rows, head 1 the key's own
+    keep = torch.zeros(n + 3, dtype=torch.bool, device="cuda")
+    keep[0] = True
+    keep[n:] = True
+    _check_attention(q, k, v, table, b, chains, grad, keep=keep)
+    q = q.clone()
+    q[n - 1, 0] = math.nan
+    table = torch.zeros_like(table)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    out = nn.chain_attention(*leaves, b, chains, keep=keep)
+    dq, dk, dv, _ = torch.autograd.grad(out, leaves, grad)
+    for t in (out[n - 1, 0], dq[n - 1, 0], dk[0, 0], dv[0, 0]):
+        assert bool(torch.isnan(t).all())
