@@ -89,7 +89,7 @@ enum { kIndex = 0, kGiven = 1, kEither = 2 };
 // What dq leaves for dk and dv of every row [heads][beads], and of every wave of
 // queries [heads][tiles][waves].
 struct AttnRows {
-  float *delta, *start;  // do . o;  -(m + log2 l) / c
+  float *delta, *start;  // do . o;  -(m + log2 l) / c, in 16 bits
   float* apart;          // whether m is too large for start to take its place
 };
 
@@ -944,9 +944,11 @@ __host__ __device__ __forceinline__ int scratch_floats(int reach, bool positions
   return positions ? (2 * (2 * reach + 1) + 3) & ~3 : diag_floats<DP>();
 }
 
-// Up to this |m| the sums that dk and dv form a row's logits from begin with
-// -(m + log2 l) / c, so that they leave nothing to subtract (rounded by 2^-16
-// there, below a 16-bit factor's 2^-12).
+// In 16 bits, up to this |m|, the sums that dk and dv form a row's logits from
+// begin with -(m + log2 l) / c, so that they leave nothing to subtract (rounded
+// by 2^-16 there, below a factor's 2^-12).  In 32 bits every step of these sums
+// would be rounded at that size (1031 beads of 32 channels: P off by 1.0e-6
+// against 2.2e-7), and the products bound the kernel, not the subtraction.
 constexpr float kAttnFold = 512.0f;
 
 template <typename T, int DP, int NQ, int NK>
@@ -1141,9 +1143,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
     if (g == 0) {
       rows_out.delta[head * a.beads + row] = delta;
-      // -inf logits for a row without keys
-      const float sum = l == 0.0f ? -INFINITY : -(m + __builtin_amdgcn_logf(l));
-      rows_out.start[head * a.beads + row] = sum / logit_factor(a);
+      if constexpr (sizeof(T) == 2) {  // -inf logits for a row without keys
+        const float sum = l == 0.0f ? -INFINITY : -(m + __builtin_amdgcn_logf(l));
+        rows_out.start[head * a.beads + row] = sum / logit_factor(a);
+      }
     }
   }
   if (wk == 0) {
@@ -1247,7 +1250,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
       if (given) pos_n = a.pos[row0 + i];
     }
   };
-  load(kv * a.group, 0, true, true);
+  load(kv * a.group, 0, sizeof(T) == 2, true);
   // any large m among the chain's queries of these heads
   float large = 0.0f;
   for (int h = 0; h < a.group; ++h) {
@@ -1273,8 +1276,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
   int buf = 0;
-  auto all_queries = [&](auto fold) {
-    constexpr bool FOLD = decltype(fold)::value;
+  // FOLD: sums that begin with start.  FAR: some m may be far_shift's.
+  auto all_queries = [&](auto fold, auto far) {
+    constexpr bool FOLD = decltype(fold)::value, FAR = decltype(far)::value;
     // puts the tile of q0 into LDS and sends for the next one
     auto next_tile = [&](int h, int q0) {
       if (q0 + KS > t.y) {
@@ -1326,8 +1330,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 #pragma unroll
             for (int i = 0; i < 16 * N; ++i) {
               const float m = mrow[acc_row(i, g)], b = bias(i);
-              x[i] = far_shift<T>(m) ? fmaf(s[i / 16][i % 16], c, b) - m
-                                     : fmaf(s[i / 16][i % 16], c, b - m);
+              x[i] = FAR && far_shift<T>(m) ? fmaf(s[i / 16][i % 16], c, b) - m
+                                            : fmaf(s[i / 16][i % 16], c, b - m);
             }
           }
         };
@@ -1366,9 +1370,9 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     }
   };
   if (__any(large != 0.0f))
-    all_queries(std::false_type());
+    all_queries(std::false_type(), std::true_type());
   else
-    all_queries(std::true_type());
+    all_queries(std::bool_constant<sizeof(T) == 2>(), std::false_type());
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
   join_parts<DP, NQ, NK>(dva, reinterpret_cast<float*>(smem));
   if (!in || wk > 0) return;

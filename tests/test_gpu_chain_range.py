@@ -104,3 +104,28 @@ def test_single_key_that_a_bias_takes_away(n, dtype):
     dq, dk, dv, _ = torch.autograd.grad(out, leaves, grad)
     for t in (out[n - 1, 0], dq[n - 1, 0], dk[0, 0], dv[0, 0]):
         assert bool(torch.isnan(t).all())
+
+
+def test_fp32_gradients_are_as_exact_as_their_logits():
+    """P is off by the roundings of its logit, exp2 and the row's sum alone.  A
+    model of these steps in 32 bits (1031 keys, 32 channels) gives P 2.2e-7,
+    normwise; the sums of dk and dv over the 33 queries that have a gradient
+    here add 2^-24 / sqrt(3) sqrt(33 / 2) = 1.4e-7: 2.6e-7, and twice that is
+    allowed.  With the sums begun at the row's logarithm in place of 0 the
+    same model gives 1.0e-6.  dq and out sum 1031 keys, two a step: 2^-24 /
+    sqrt(3) sqrt(516 / 2) = 5.5e-7, with P's 6.0e-7."""
+    from mlcg_amd import nn
+
+    print("fp32 gradients", flush=True)
+    lens = [1031] * 4
+    q, k, v, table, b, chains, grad = _attention_case(lens, 4, 4, 32, torch.float32, seed=6)
+    few = torch.zeros_like(grad)
+    few[::32] = grad[::32]
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    out = nn.chain_attention(*leaves, b, chains)
+    got = dict(zip("qkv", torch.autograd.grad(out, leaves[:3], few)), out=out.detach())
+    ref, _ = R.attention(q, k, v, table, b.bucket_of, lens, None, None, None, few)
+    for name, bound in (("k", 5.2e-7), ("v", 5.2e-7), ("q", 1.2e-6), ("out", 1.2e-6)):
+        d = (got[name].cpu().double() - ref[name]).norm() / ref[name].norm()
+        print(name, float(d), flush=True)
+        assert float(d) <= bound, (name, float(d))
