@@ -315,10 +315,12 @@ __device__ __forceinline__ T round_to(float v) {
 
 // The probabilities and dS, in fp32 until here, take the elements' type as
 // operands of the products with v, do, k and q, as the matrix instructions ask
-// for: below 2^kAttnLazy relative to the row's base (forward) or at most 1
-// (backward), each is off by half a unit of that type, as its other factor is.
-// The sums that follow, of the row, of o, dq, dk, dv and of the table, stay in
-// fp32, and the row's sum and the table take the values before this rounding.
+// for, and are each off by half a unit of that type, as their other factor is:
+// the probabilities below 2^kAttnLazy relative to the row's base (forward) or at
+// most 1 (backward), dS, which has the size of the gradients, in fp16 times a
+// power of two (OperandScale).  The sums that follow, of the row, of o, dq, dk,
+// dv and of the table, stay in fp32, and the row's sum and the table take the
+// values before this rounding.
 template <typename T>
 __device__ __forceinline__ v8<T> pack8(const float* p) {
   v8<T> r;
@@ -446,6 +448,68 @@ __device__ __forceinline__ void store_rest(T* dst, const f32x16 (&acc)[DP / 32],
       }
     }
 }
+
+// The power of two that a lane's column of dS is multiplied by before it becomes
+// an operand in fp16, whose range the gradients of a scaled loss, or of a long
+// chain, leave at either end: the largest value so far lies between 2^13 and
+// 2^15, so that values down to 2^-28 of it keep their bits.  It is taken out of
+// the accumulators where they are stored.  The other types need none.
+template <typename T>
+struct OperandScale {
+  static constexpr bool kOn = std::is_same<T, _Float16>::value;
+  float up = 0.0f;  // 0 before the first value
+
+  template <int M, int NA>
+  __device__ __forceinline__ void fit(float (&x)[M], f32x16 (&acc)[NA]) {
+    if constexpr (kOn) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < M; ++i) top = fmaxf(top, fabsf(x[i]));
+      if (__any(top * up > 32768.0f || (up == 0.0f && top > 0.0f))) {
+        top = fmaxf(top, other_half(top));
+        float alpha = 1.0f;
+        if (!(top <= 3.0e38f)) {  // infinite: it may as well be so in fp16
+          up = up == 0.0f ? 1.0f : up;
+        } else if (top * up > 32768.0f || (up == 0.0f && top > 0.0f)) {
+          int e;
+          (void)frexpf(top, &e);  // top < 2^e
+          const float next = ldexpf(1.0f, 14 - max(e, -100));
+          alpha = up == 0.0f ? 1.0f : next / up;
+          up = next;
+        }
+#pragma unroll
+        for (int n = 0; n < NA; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < M; ++i) x[i] *= up;
+    }
+  }
+  // the NK parts on the smallest of their scales; buf: 32 NQ NK values
+  template <int NQ, int NK, int NA>
+  __device__ __forceinline__ void join(f32x16 (&acc)[NA], float* buf) {
+    if constexpr (kOn && NK > 1) {
+      const int lane = threadIdx.x & 63, wave = wave_number(), wq = wave % NQ;
+      __syncthreads();
+      if (lane < 32) buf[32 * wave + lane] = up;
+      __syncthreads();
+      float least = 0.0f;
+#pragma unroll
+      for (int p = 0; p < NK; ++p) {
+        const float u = buf[32 * (p * NQ + wq) + (lane & 31)];
+        if (u != 0.0f) least = least == 0.0f ? u : fminf(least, u);
+      }
+      const float alpha = up == 0.0f ? 1.0f : least / up;
+      up = least;
+#pragma unroll
+      for (int n = 0; n < NA; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[n][r] *= alpha;
+    }
+  }
+  __device__ __forceinline__ float undo() const { return kOn && up != 0.0f ? 1.0f / up : 1.0f; }
+};
 
 // acc of the NK waves of a column block, joined in the order of the parts;
 // the sums are part 0's.  buf: (NK - 1) NQ 64 values for each accumulator.
@@ -1049,6 +1113,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     for (int i = lane; i < diag_floats<DP>(); i += 64) scratch[i] = 0.0f;
   float far_lo = 0.0f, far_hi = 0.0f;
   f32x16 acc[DP / 32] = {};
+  OperandScale<T> up;
   int buf = 0;
   // puts the tile of k0 into LDS and sends for the next one
   auto next_tile = [&](int k0) {
@@ -1129,6 +1194,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
         }
       }
     }
+    up.fit(x, acc);
     column_product<T, DP, N>(kt, x, acc);
   }
   if (given) ints.flush();
@@ -1138,9 +1204,10 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     mine[0] += far_lo;
     mine[cells - 1] += far_hi;
   }
+  up.template join<NQ, NK>(acc, reinterpret_cast<float*>(smem));
   join_parts<DP, NQ, NK>(acc, reinterpret_cast<float*>(smem));
   if (qi.ok && wk == 0) {
-    store_column<T, DP, VEC>(dq + flat, acc, a.scale, a.dim);
+    store_column<T, DP, VEC>(dq + flat, acc, a.scale * up.undo(), a.dim);
     if (g == 0) {
       rows_out.delta[head * a.beads + row] = delta;
       if constexpr (sizeof(T) == 2) {  // -inf logits for a row without keys
@@ -1275,6 +1342,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
   }
 
   f32x16 dka[DP / 32] = {}, dva[DP / 32] = {};
+  OperandScale<T> up;
   int buf = 0;
   // FOLD: sums that begin with start.  FAR: some m may be far_shift's.
   auto all_queries = [&](auto fold, auto far) {
@@ -1365,6 +1433,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
         column_product<T, DP, N>(gt, x, dva);
 #pragma unroll
         for (int i = 0; i < 16 * N; ++i) x[i] *= s[i / 16][i % 16];
+        up.fit(x, dka);
         column_product<T, DP, N>(qt, x, dka);
       }
     }
@@ -1373,6 +1442,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     all_queries(std::false_type(), std::true_type());
   else
     all_queries(std::bool_constant<sizeof(T) == 2>(), std::false_type());
+  up.template join<NQ, NK>(dka, reinterpret_cast<float*>(smem));
   join_parts<DP, NQ, NK>(dka, reinterpret_cast<float*>(smem));
   join_parts<DP, NQ, NK>(dva, reinterpret_cast<float*>(smem));
   if (!in || wk > 0) return;
@@ -1381,7 +1451,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) dka[n] = dva[n] = f32x16{};
   }
-  store_column<T, DP, VEC>(dk + flat, dka, a.scale, a.dim);
+  store_column<T, DP, VEC>(dk + flat, dka, a.scale * up.undo(), a.dim);
   store_column<T, DP, VEC>(dv + flat, dva, 1.0f, a.dim);
 }
 

@@ -129,3 +129,53 @@ def test_fp32_gradients_are_as_exact_as_their_logits():
         d = (got[name].cpu().double() - ref[name]).norm() / ref[name].norm()
         print(name, float(d), flush=True)
         assert float(d) <= bound, (name, float(d))
+
+
+def _normwise(got, ref, name, relative):
+    """Relative roundings, and half a spacing of fp16's subnormal numbers."""
+    d = float((got.detach().cpu().double() - ref).norm())
+    bound = relative * float(ref.norm()) + 2.0 ** -25 * math.sqrt(ref.numel())
+    assert d <= bound, f"{name}: {d / max(float(ref.norm()), 1e-300)} of its norm, bound " \
+                       f"{bound / max(float(ref.norm()), 1e-300)}"
+
+
+@pytest.mark.parametrize("lens", [[60, 45], [2000], [130] * 40])
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e2])
+def test_fp16_gradients_of_any_size(size, lens):
+    """Gradients of a loss that is scaled down or up: dS passes through 16 bits
+    relative to its row, not to 1.  P, dS and the output each round by 2^-11 /
+    sqrt(3) in the mean: 2^-11 for the three."""
+    from mlcg_amd import nn
+
+    print(f"fp16 gradients {lens[0]} {size}", flush=True)
+    q, k, v, table, b, chains, grad = _attention_case(lens, 2, 1, 64, torch.float16, seed=8)
+    grad = grad * size
+    pos = torch.cumsum((torch.rand(sum(lens), generator=torch.Generator().manual_seed(1)) < 0.4)
+                       .int(), 0).to(torch.int32).cuda()
+    for ps in (None, pos):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+        out = nn.chain_attention(*leaves, b, chains, positions=ps)
+        grads = torch.autograd.grad(out, leaves, grad)
+        ref, _ = R.attention(q, k, v, table, b.bucket_of, lens, None, None, ps, grad)
+        for name, got in zip(("q", "k", "v", "table"), grads):
+            _normwise(got, ref[name], name, 2.0 ** -11)
+
+
+def test_fp16_gradients_beyond_the_type_inside():
+    """dS passes fp16's largest number, the gradients do not."""
+    from mlcg_amd import nn
+
+    print("fp16 gradients, large dS", flush=True)
+    lens = [4, 70, 200]
+    q, k, v, table, b, chains, grad = _attention_case(lens, 2, 1, 64, torch.float16, seed=9,
+                                                      views=False)
+    k, q = k * 0.01, q * 0.01
+    v = v * 4.0
+    grad = (grad * 2e4).clamp(-6e4, 6e4)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    out = nn.chain_attention(*leaves, b, chains)
+    grads = torch.autograd.grad(out, leaves, grad)
+    ref, _ = R.attention(q, k, v, table, b.bucket_of, lens, None, None, None, grad)
+    for name, got in zip(("q", "k"), grads):
+        assert float(ref[name].abs().max()) < 6e4
+        _normwise(got, ref[name], name, 2.0 ** -11)
