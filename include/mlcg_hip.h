@@ -1026,6 +1026,8 @@ int mlcg_copy_batch(const void* const* srcs, void* const* dsts,
  * [0, buckets); 1 <= reach <= 1024, 1 <= dim <= 128.  keep [beads]: 0 marks an
  * absent bead, whose key and value are not read as numbers (NULL: all are
  * present); positions [beads]: p, any int32 (NULL: the index in the chain).
+ * A bias may be -inf (no key at that offset) or of any size; +inf or no number
+ * counts where a bead of the chain, present or not, has its offset to a query.
  * out [beads, heads, dim]; lse [2, heads, beads] (may be NULL): m and l of the
  * row's log-sum m + log2 l in base 2, +inf and 0 for a row without keys, which
  * the backward pass takes.

@@ -286,9 +286,12 @@ struct Stage {
 };
 
 // ext[n] = log2(e) bias of the offset n - (reach + kAttnSpan), clipped; a bias
-// of the type's lowest or highest value stays a number
+// of the type's lowest or highest value stays a number.  Of index positions in a
+// chain of `len`, offsets that no pair has, but rows past the end do, have 0:
+// the table may hold anything there, and -inf + inf is not -inf.
 template <typename T>
-__device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, float* ext) {
+__device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, int len, bool given,
+                                          float* ext) {
   const int n = 2 * (a.reach + kAttnSpan) + 1;
   const T* table = (const T*)a.table;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -296,6 +299,7 @@ __device__ __forceinline__ void fill_bias(const AttnArgs& a, int head, float* ex
     const float b = (float)table[(int64_t)a.bucket_of[d] * a.heads + head];
     const float e = kAttnLog2e * b;
     ext[i] = fabsf(e) > 3.0e38f && fabsf(b) != INFINITY ? copysignf(3.0e38f, b) : e;
+    if (!given && abs(i - (a.reach + kAttnSpan)) >= len) ext[i] = 0.0f;
   }
 }
 
@@ -553,7 +557,8 @@ __device__ __forceinline__ bool given_positions(const AttnArgs& a) {
 
 // What stands for the keys of a tile in LDS: the value that their products'
 // sums begin with (0, or for an absent key what makes the logit -inf), and
-// their positions.  Thread i loads row i's.
+// their positions (past the end another bead's, so that their offsets are
+// pairs').  Thread i loads row i's.
 struct KeyInfo {
   bool in;
   uint8_t keep;
@@ -571,11 +576,12 @@ struct KeyInfo {
     }
   }
   template <int POS>
-  __device__ __forceinline__ void put(const AttnArgs& a, int rows, float* caps, int* kpos) const {
+  __device__ __forceinline__ void put(const AttnArgs& a, int rows, int other, float* caps,
+                                      int* kpos) const {
     if ((int)threadIdx.x < rows) {
       const float none = logit_factor(a) > 0.0f ? -INFINITY : INFINITY;
       caps[threadIdx.x] = in && keep ? 0.0f : none;
-      if (POS != kIndex) kpos[threadIdx.x] = pos;
+      if (POS != kIndex) kpos[threadIdx.x] = in ? pos : other;
     }
   }
 };
@@ -634,7 +640,7 @@ __device__ __forceinline__ int query_logits(const AttnArgs& a, const f32x16 (&s)
     side = block_side(kb - (q.first + 31), kb + 32 * N - 1 - q.first, R);
   }
   if (side) {
-    const float b = (side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0]) - near;
+    const float b = ext[side > 0 ? 2 * R + kAttnSpan : kAttnSpan] - near;
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i) x[i] = fmaf(s[i / 16][i % 16], c, b);
   } else if (given_positions<POS>(a)) {
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
   v8<T> qf[DP / 16];
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) qf[k] = load8<T, VEC>(q, 16 * k + 8 * g, qi.ok, a.dim);
-  fill_bias<T>(a, head, ext);
+  fill_bias<T>(a, head, t.y, given, ext);
 
   f32x16 acc[DP / 32] = {};
   // the exponents are relative to base, the row's maximum so far or up to
@@ -736,7 +742,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.template put<POS>(a, KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(a, KS, qi.lo, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
@@ -1102,7 +1108,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
   const float l = qi.ok ? a.lse[(a.heads + head) * a.beads + row] : 0.0f;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l, delta_inv = delta * inv;
   const bool any_far = __any(far_shift<T>(m));
-  fill_bias<T>(a, head, ext);
+  fill_bias<T>(a, head, t.y, given, ext);
   for (int i = threadIdx.x; i < NW * cells; i += NT) dd[i] = 0.0f;
   float* mine = dd + wave * cells;
   float* scratch = L.rest + wave * sf;
@@ -1123,7 +1129,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_ker
     }
     ks.put(L.k[buf]);
     vs.put(L.v[buf]);
-    info.template put<POS>(a, KS, L.cap[buf], L.kpos[buf]);
+    info.template put<POS>(a, KS, qi.lo, L.cap[buf], L.kpos[buf]);
     const int kn = k0 + KS;
     if (kn < t.y) {
       ks.load(kbase + kn * a.k_row, t.y - kn, a.dim);
@@ -1363,7 +1369,8 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
           L.inv[buf][threadIdx.x] = l_n == 0.0f ? 0.0f : 1.0f / l_n;
         }
         L.delta[buf][threadIdx.x] = -delta_n;
-        if (POS != kIndex) L.qpos[buf][threadIdx.x] = pos_n;
+        // past the end a bead's of the chain, so that the offsets are pairs'
+        if (POS != kIndex) L.qpos[buf][threadIdx.x] = q0 + (int)threadIdx.x < t.y ? pos_n : klo;
       }
       if (q0 + KS < t.y)
         load(kv * a.group + h, q0 + KS, FOLD, !FOLD);
@@ -1374,7 +1381,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
     for (int h = 0; h < a.group; ++h) {
       const int head = kv * a.group + h;
       if (h > 0) __syncthreads();
-      fill_bias<T>(a, head, ext);
+      fill_bias<T>(a, head, t.y, given, ext);
       if (kw >= t.y)  // no keys: this wave only loads
         for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) next_tile(h, q0);
       else for (int q0 = 0; q0 < t.y; q0 += KS, buf ^= 1) {
@@ -1414,7 +1421,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_k
           side = block_side(kw - (qb + RT - 1), kw + 31 - qb, R);
         }
         if (side) {
-          const float b = side > 0 ? ext[2 * (R + kAttnSpan)] : ext[0];
+          const float b = ext[side > 0 ? 2 * R + kAttnSpan : kAttnSpan];
           logits([=](int) { return b; });
         } else if (given) {
           logits([=](int i) { return ext[offset_cell(kp, qpos[acc_row(i, g)], R)]; });

@@ -179,3 +179,55 @@ def test_fp16_gradients_beyond_the_type_inside():
     for name, got in zip(("q", "k"), grads):
         assert float(ref[name].abs().max()) < 6e4
         _normwise(got, ref[name], name, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_biases_that_no_pair_has(bad, dtype):
+    """Table entries of offsets that occur in no chain do not matter, whatever they
+    hold."""
+    from mlcg_amd import nn
+
+    print(f"unused biases {dtype} {bad}", flush=True)
+    odd = torch.cat([2 * torch.arange(n) + 1 for n in (40, 35, 1, 200)]).to(torch.int32)
+    for lens, ps, unused in (([40, 35], None, lambda d: abs(d) >= 40),
+                             ([120, 7], None, lambda d: abs(d) >= 120),
+                             ([40, 35, 1, 200], odd, lambda d: d % 2 == 1)):
+        q, k, v, table, b, chains, grad = _attention_case(lens, 2, 1, 32, dtype, kind="clip",
+                                                          buckets=257, reach=128)
+        mask = torch.tensor([unused(d) for d in range(-128, 129)], device="cuda")
+        outs = []
+        for fill in (0.0, bad):
+            t = table.clone()
+            t[mask] = fill
+            leaves = [x.detach().requires_grad_(True) for x in (q, k, v, t)]
+            out = nn.chain_attention(*leaves, b, chains,
+                                     positions=None if ps is None else ps.cuda())
+            outs.append((out.detach(), *torch.autograd.grad(out, leaves, grad)))
+        for x, y in zip(*outs):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_table_gradient_of_a_long_chain(dtype, given):
+    """As test_attention_table_gradient_of_a_long_chain, whose bound this is, in
+    both 16-bit types and with sums along diagonals or by residue numbers: the
+    table's gradient is off by its own rounding, u / sqrt(3) in the mean at most,
+    and u / 16 for what comes before it."""
+    from mlcg_amd import nn
+
+    print(f"table gradient {dtype} {given}", flush=True)
+    q, k, v, table, b, chains, grad = _attention_case([2000], 2, 2, 64, dtype, seed=4)
+    pos = None
+    if given:
+        pos = torch.cumsum((torch.rand(2000, generator=torch.Generator().manual_seed(1)) < 0.4)
+                           .int(), 0).to(torch.int32).cuda()
+    leaf = table.clone().requires_grad_(True)
+    got, = torch.autograd.grad(nn.chain_attention(q, k, v, leaf, b, chains, positions=pos), leaf,
+                               grad)
+    ref, _ = R.attention(q, k, v, table, b.bucket_of, chains.lengths, None, None, pos, grad)
+    d = (got.cpu().double() - ref["table"]).norm() / ref["table"].norm()
+    u = U[dtype]
+    print(float(d) / u, flush=True)
+    assert float(d) <= u / math.sqrt(3.0) + u / 16.0, float(d)
