@@ -11,7 +11,7 @@ from the table's gradient, and a simulation evaluates it once
 
 ``chain_attention``, ``group_norm_act`` and ``dropout_add`` are the operators
 with their gradients, on the HIP kernels; like the rest of the package they
-take GPU tensors only, and they are differentiable once.
+take GPU tensors only, and they are differentiable once, in reverse mode.
 """
 
 from __future__ import annotations
@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -47,7 +48,11 @@ class _Attention(torch.autograd.Function):
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its autograd function: for a gradient, or to be
+    refused there where a tangent asks for a forward-mode derivative."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def chain_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
