@@ -125,7 +125,8 @@ class ChainAttention(torch.nn.Module):
     to queries, keys and values (``kv_heads`` of the latter serve ``heads``
     query heads), a learned bias by relative position, a projection back.
 
-    forward(x [S, width], chains, keep=None, positions=None) -> [S, width]."""
+    forward(x [S, width], chains, keep=None, positions=None) -> [S, width].
+    The bias table takes the type of the projection, under autocast 16 bits."""
 
     def __init__(self, width: int, heads: int, kv_heads: Optional[int] = None,
                  num_buckets: int = 32, reach: int = 128, kind: str = "log"):
@@ -157,14 +158,15 @@ class ChainAttention(torch.nn.Module):
     def forward(self, x, chains, keep=None, positions=None):
         h, kv, d = self.heads, self.kv_heads, self.dim
         qkv = self.qkv(x).view(-1, h + 2 * kv, d)
-        y = chain_attention(qkv[:, :h], qkv[:, h:h + kv], qkv[:, h + kv:], self.bias_table,
-                            self.buckets, chains, keep=keep, positions=positions)
+        y = chain_attention(qkv[:, :h], qkv[:, h:h + kv], qkv[:, h + kv:],
+                            self.bias_table.to(qkv.dtype), self.buckets, chains, keep=keep,
+                            positions=positions)
         return self.out(y.reshape(-1, h * d))
 
 
 class GroupNormAct(torch.nn.Module):
     """Group norm of every chain with an affine map by channel and an
-    activation: forward(x [S, width], chains) -> [S, width]."""
+    activation: forward(x [S, width], chains) -> [S, width], in x's type."""
 
     def __init__(self, groups: int, width: int, act: str = "none", eps: float = 1e-5):
         super().__init__()
@@ -179,7 +181,8 @@ class GroupNormAct(torch.nn.Module):
         torch.nn.init.zeros_(self.bias)
 
     def forward(self, x, chains):
-        return group_norm_act(x, self.weight, self.bias, self.groups, chains, self.eps, self.act)
+        return group_norm_act(x, self.weight.to(x.dtype), self.bias.to(x.dtype), self.groups,
+                              chains, self.eps, self.act)
 
 
 class CounterDropout(torch.nn.Module):
@@ -187,7 +190,8 @@ class CounterDropout(torch.nn.Module):
     stored.  The step is a buffer that every training call moves on, on the
     device: a recorded training step draws a new mask on every replay, and a
     run resumed from a checkpoint goes on with the next one.  Modules of one
-    model need seeds of their own.  In eval mode: residual + x."""
+    model need seeds of their own.  In eval mode: residual + x.  x may be in 16
+    bits beside an fp32 residual, as under autocast."""
 
     def __init__(self, p: float, seed: int):
         super().__init__()
@@ -200,6 +204,8 @@ class CounterDropout(torch.nn.Module):
             return x if residual is None else residual + x
         # the backward pass reads the value that this call used
         step = self.step.add_(1).clone()
+        if residual is not None:
+            x = x.to(residual.dtype)
         return dropout_add(x, self.p, self.seed, step, residual)
 
 
