@@ -759,6 +759,13 @@ int mlcg_type_sum(const float* x, const int64_t* types, int64_t rows, int featur
                   int num_types, float* out, int* bad, float* workspace,
                   int64_t workspace_floats, void* stream);
 
+/* The same for tables of up to 2^24 - 1 rows (a row a bead of the molecules,
+ * mlcg_group_norm_act and below), whose workgroups serve a share of the sites
+ * each; rows < 2^31, no workspace, the same bits on every run.  Sites outside
+ * the table as in mlcg_type_sum. */
+int mlcg_site_sum(const float* x, const int64_t* sites, int64_t rows, int features,
+                  int num_sites, float* out, int* bad, void* stream);
+
 /* ---------------------------------------------------------------------- */
 /* Output network MLP([128, HH, 1]) with its reverse and tangent sweeps    */
 /* ---------------------------------------------------------------------- */

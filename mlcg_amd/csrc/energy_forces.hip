@@ -239,6 +239,9 @@ extern "C" int mlcg_energy_forces_grad(
                           stream);
   }
   if (st != MLCG_OK) return st;
+  if (mlcg_type_sum_workspace_floats(n_nodes, num_types) < 0)  // more types than it takes
+    return mlcg_site_sum(arr2(at2.xbar2(0)), types, n_nodes, kF, num_types, gr(0), nullptr,
+                         stream);
   return mlcg_type_sum(arr2(at2.xbar2(0)), types, n_nodes, kF, num_types, gr(0), nullptr,
                        workspace, workspace_floats, stream);
 }

@@ -930,6 +930,127 @@ __global__ __launch_bounds__(kF) void type_sum_combine_kernel(const float* __res
   out[(int64_t)t * kF + c] = sum;
 }
 
+// site_sum: the same for any T, tables whose rows are the beads of molecules.
+// Workgroup b serves the types t = b mod 256 (a molecule's beads spread over all)
+// and lists their rows, in row order, over as many chunks as the list holds;
+// then each of its waves takes every 16th of the types, picks its rows from
+// the list by ballots, and adds them, 16 loads of a row's 128 columns in flight,
+// with a compensated sum.  A list that is full is summed into out before the
+// next one begins.  No atomics: the same bits on every run.
+// Bound by its 256 scans of the types, and by the latency of the loads where a
+// type has many rows: 17152 rows of 268 types 11 us, 35000 of 1000 17, 32764
+// of 8191 15 and 131056 74 (one workgroup a type: 14, 48, 348, 1072; atomic adds, whose
+// order changes: 12, 19, 18, 57).
+constexpr int kSiteGroups = 256;
+constexpr int kSiteSteps = 8;
+constexpr int kSiteWaveRows = kSiteSteps * MLCG_WAVE;
+constexpr int kSiteChunk = kTypeWaves * kSiteWaveRows;  // 8192 rows
+constexpr int kSiteList = 12288;
+constexpr int kSiteBatch = 16;
+constexpr int kSiteMax = 1 << 24;                  // a type's number in its group has 16 bits
+
+__global__ __launch_bounds__(kTypeThreads) void site_sum_kernel(const float* __restrict__ x,
+                                                                 const int64_t* __restrict__ types,
+                                                                 int64_t rows, int T,
+                                                                 float* __restrict__ out,
+                                                                 int* __restrict__ bad,
+                                                                 unsigned* __restrict__ flags) {
+  __shared__ int list[kSiteList];  // rows of the group's types, in ascending order
+  __shared__ uint16_t local[kSiteList];
+  __shared__ int cnt[kTypeWaves];
+  __shared__ int mine[kTypeWaves][2 * MLCG_WAVE];  // a wave's rows of one type
+  const int b = blockIdx.x, w = threadIdx.x / MLCG_WAVE, l = mlcg_lane();
+  const uint64_t below = (l == 0) ? 0ull : (~0ull >> (MLCG_WAVE - l));  // lanes < l
+  int n = 0;          // listed
+  bool first = true;  // out holds nothing yet
+  for (int64_t r0 = 0; r0 == 0 || r0 < rows; r0 += kSiteChunk) {
+    const int64_t base = r0 + (int64_t)w * kSiteWaveRows;
+    int64_t tt[kSiteSteps];
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < kSiteSteps; ++i) {
+      const int64_t r = base + MLCG_WAVE * i + l;
+      tt[i] = r < rows ? types[r] : b;
+      const bool outside = tt[i] < 0 || tt[i] >= T;
+      if (b == 0 && outside) {  // as in type_sum_kernel
+        if (bad)
+          bad[0] = 1;
+        else
+          atomicOr(flags, kFlagTypeRange);
+      }
+      if (r >= rows || outside || tt[i] % kSiteGroups != b) tt[i] = -1;
+      found += __popcll(__ballot(tt[i] >= 0));
+    }
+    if (l == 0) cnt[w] = found;
+    __syncthreads();
+    int off = n, total = 0;
+#pragma unroll
+    for (int v = 0; v < kTypeWaves; ++v) {
+      off += v < w ? cnt[v] : 0;
+      total += cnt[v];
+    }
+#pragma unroll
+    for (int i = 0; i < kSiteSteps; ++i) {
+      const bool m = tt[i] >= 0;
+      const uint64_t bal = __ballot(m);
+      if (m) {
+        const int at = off + __popcll(bal & below);
+        list[at] = (int)(base + MLCG_WAVE * i + l);
+        local[at] = (uint16_t)(tt[i] / kSiteGroups);
+      }
+      off += __popcll(bal);
+    }
+    n += total;
+    __syncthreads();
+    if (r0 + kSiteChunk < rows && n <= kSiteList - kSiteChunk) continue;
+    for (int t = b + kSiteGroups * w; t < T; t += kSiteGroups * kTypeWaves) {
+      float2* const o = reinterpret_cast<float2*>(out + (int64_t)t * kF) + l;
+      float2 acc = make_float2(0.f, 0.f), comp = acc;
+      if (!first) acc = *o;
+      int p = 0;  // rows waiting in mine
+      const auto add = [&](int count) {
+        for (int m0 = 0; m0 < count; m0 += kSiteBatch) {
+          float2 xv[kSiteBatch];
+#pragma unroll
+          for (int u = 0; u < kSiteBatch; ++u)
+            xv[u] = m0 + u < count
+                        ? reinterpret_cast<const float2*>(x + (int64_t)mine[w][m0 + u] * kF)[l]
+                        : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int u = 0; u < kSiteBatch; ++u)
+            if (m0 + u < count) {
+              const float yx = xv[u].x - comp.x, yy = xv[u].y - comp.y;
+              const float sx = acc.x + yx, sy = acc.y + yy;
+              comp = make_float2((sx - acc.x) - yx, (sy - acc.y) - yy);
+              acc = make_float2(sx, sy);
+            }
+        }
+      };
+      for (int i = 0; i < n; i += MLCG_WAVE) {
+        const bool m = i + l < n && local[i + l] == t / kSiteGroups;
+        const uint64_t bal = __ballot(m);
+        if (m) mine[w][p + __popcll(bal & below)] = list[i + l];
+        p += __popcll(bal);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (p >= MLCG_WAVE) {
+          add(MLCG_WAVE);
+          p -= MLCG_WAVE;
+          const int next = l < p ? mine[w][MLCG_WAVE + l] : 0;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          if (l < p) mine[w][l] = next;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+      }
+      add(p);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      *o = acc;
+    }
+    first = false;
+    n = 0;
+    __syncthreads();  // the list is written again
+  }
+}
+
 // Workgroups per type: enough to give the chip about 256 workgroups, at most
 // one per chunk of rows.
 int type_groups(int64_t rows, int T) {
@@ -1217,5 +1338,19 @@ extern "C" int mlcg_type_sum(const float* x, const int64_t* types, int64_t rows,
   if (G > 1)
     hipLaunchKernelGGL(type_sum_combine_kernel, dim3((unsigned)num_types), dim3(kF), 0,
                        mlcg_stream(stream), workspace, G, num_types, out);
+  return mlcg_launch_status();
+}
+
+extern "C" int mlcg_site_sum(const float* x, const int64_t* sites, int64_t rows, int features,
+                             int num_sites, float* out, int* bad, void* stream) {
+  if (features != kF) return MLCG_ERR_UNSUPPORTED;
+  MLCG_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && num_sites >= 1 &&
+               num_sites < kSiteMax && out);
+  MLCG_REQUIRE(rows == 0 || (x && sites));
+  unsigned* const flags = bad ? nullptr : mlcg_numerics_word_ptr();
+  if (bad == nullptr && flags == nullptr) return MLCG_ERR_LAUNCH;
+  const int groups = num_sites < kSiteGroups ? num_sites : kSiteGroups;
+  hipLaunchKernelGGL(site_sum_kernel, dim3((unsigned)groups), dim3(kTypeThreads), 0,
+                     mlcg_stream(stream), x, sites, rows, num_sites, out, bad, flags);
   return mlcg_launch_status();
 }

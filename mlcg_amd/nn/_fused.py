@@ -519,7 +519,8 @@ _SWEEP = ("mlcg_embedding_gather", "mlcg_node_weight_images", "mlcg_node_gemm",
           "mlcg_node_gemm2", "mlcg_cfconv_gather", "mlcg_out_forward", "mlcg_segment_sum",
           "mlcg_cfconv_gather_bwd", "mlcg_pair_forces")
 _SWEEP2 = ("mlcg_pair_ddot", "mlcg_node_gemm", "mlcg_node_gemm2", "mlcg_cfconv_gather_tangent",
-           "mlcg_out_rev2", "mlcg_cfconv_gather_rev2", "mlcg_node_tmm_batch", "mlcg_type_sum")
+           "mlcg_out_rev2", "mlcg_cfconv_gather_rev2", "mlcg_node_tmm_batch", "mlcg_type_sum",
+           "mlcg_site_sum")
 
 
 @dataclass
@@ -586,7 +587,7 @@ def force_gradients(spec: FusedSpec, P: Params, st: State, u: Optional[torch.Ten
                     ) -> List[torch.Tensor]:
     """tangent(u, scale) and reverse2(tw, pw) after energy_forces(seed=tw): by one
     native call and the filters' gradients where energy_forces was one, too."""
-    if st.kept is None or u is None or P.emb.shape[0] > 128 or _TMM_SIDE or _lib.timed(_SWEEP2):
+    if st.kept is None or u is None or _TMM_SIDE or _lib.timed(_SWEEP2):
         if st.kept is not None:
             _unpack(spec, P, st)
         if u is not None:
@@ -883,9 +884,10 @@ def _blocks_reverse2(spec, P, st, tw, xbar2, g_out_w, g_out_b):
         filters.add(k, gagg2, g1, yd, dd)
         g_blocks[k] = [gA1, gA2, gc2, gA3, gc3]
     g_filters, g_basis = filters.finish()
-    if P.emb.shape[0] <= 128 and P.emb.shape[1] == 128 and st.types.dtype == torch.int64:
+    if P.emb.shape[1] == 128 and st.types.dtype == torch.int64:
         # fixed summation order; an out-of-table type raises a numerics flag
-        g_emb = ops.type_sum(xbar2, st.types, P.emb.shape[0], want_bad=False)[0]
+        row_sum = ops.type_sum if P.emb.shape[0] <= ops.MAX_TYPES else ops.site_sum
+        g_emb = row_sum(xbar2, st.types, P.emb.shape[0], want_bad=False)[0]
     else:
         g_emb = torch.zeros_like(P.emb).index_add_(0, st.types, xbar2)
     side.join()

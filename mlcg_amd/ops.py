@@ -750,6 +750,18 @@ def embedding_gather(table: torch.Tensor, types: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _sum_args(x: torch.Tensor, types: torch.Tensor, name: str):
+    require_device(x, types)
+    _check(x.dim() == 2 and x.shape[1] == NUM_FILTERS and x.dtype == torch.float32,
+           f"{name} takes [N, {NUM_FILTERS}] float32 rows")
+    _check(types.dtype == torch.int64 and types.shape == (x.shape[0],)
+           and types.device == x.device, "types must be int64 [N] on the rows' device")
+    return x.contiguous(), types.contiguous()
+
+
+MAX_TYPES = 128  # of type_sum
+
+
 def type_sum(x: torch.Tensor, types: torch.Tensor, num_types: int, want_bad: bool = True
              ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(out [num_types, 128], bad [1] int32): out[t] = sum of the rows of x
@@ -757,19 +769,28 @@ def type_sum(x: torch.Tensor, types: torch.Tensor, num_types: int, want_bad: boo
     (mlcg_type_sum); bad[0] = 1 when a type lies outside [0, num_types).
     With want_bad=False bad is None and such a type raises bit 2 of the
     numerics flags instead (check_numerics reports it)."""
-    require_device(x, types)
-    _check(x.dim() == 2 and x.shape[1] == NUM_FILTERS and x.dtype == torch.float32,
-           f"type_sum takes [N, {NUM_FILTERS}] float32 rows")
-    _check(types.dtype == torch.int64 and types.shape == (x.shape[0],)
-           and types.device == x.device, "types must be int64 [N] on the rows' device")
-    _check(1 <= num_types <= 128, "type_sum supports 1..128 types")
-    x, types = x.contiguous(), types.contiguous()
+    x, types = _sum_args(x, types, "type_sum")
+    _check(1 <= num_types <= MAX_TYPES, f"type_sum supports 1..{MAX_TYPES} types")
     out = torch.empty(num_types, NUM_FILTERS, dtype=torch.float32, device=x.device)
     bad = torch.zeros(1, dtype=torch.int32, device=x.device) if want_bad else None
     nws = int(_lib.load().mlcg_type_sum_workspace_floats(x.shape[0], num_types))
     ws = torch.empty(nws, dtype=torch.float32, device=x.device) if nws > 0 else None
     call("mlcg_type_sum", ptr(x), ptr(types), x.shape[0], NUM_FILTERS, num_types, ptr(out),
          ptr(bad), ptr(ws), nws, stream_handle(x.device))
+    return out, bad
+
+
+def site_sum(x: torch.Tensor, sites: torch.Tensor, num_sites: int, want_bad: bool = True
+             ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """type_sum for tables of any size, such as a ChainEmbedding's
+    (mlcg_site_sum): the same results, bits included, on every run."""
+    x, sites = _sum_args(x, sites, "site_sum")
+    _check(1 <= num_sites < 2 ** 24 and x.shape[0] < 2 ** 31,
+           "site_sum takes 1 .. 2^24 - 1 sites and less than 2^31 rows")
+    out = torch.empty(num_sites, NUM_FILTERS, dtype=torch.float32, device=x.device)
+    bad = torch.zeros(1, dtype=torch.int32, device=x.device) if want_bad else None
+    call("mlcg_site_sum", ptr(x), ptr(sites), x.shape[0], NUM_FILTERS, num_sites, ptr(out),
+         ptr(bad), stream_handle(x.device))
     return out, bad
 
 
@@ -1344,7 +1365,7 @@ def energy_forces_grad(pos: torch.Tensor, types: torch.Tensor, graph: PairGraph,
     seed = tw: the gradients of <pw, o> + <tw, odot> by every entry of weights
     (None for a None), odot along scale * u, and what the gradients of the
     filters read, per block (mlcg_energy_forces_grad)."""
-    _check(energy_forces_ok(pos, types, graph, weights, hidden) and weights[0].shape[0] <= 128,
+    _check(energy_forces_ok(pos, types, graph, weights, hidden),
            "energy_forces_grad: unsupported shapes, types or layouts")
     pos, (arrays, images, rows) = _validate_pos(pos), kept
     n, dev, L, cap = pos.shape[0], pos.device, len(filters), graph.pair_capacity
