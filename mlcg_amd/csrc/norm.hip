@@ -547,11 +547,11 @@ __global__ __launch_bounds__(1024) void norm_rows_kernel(const float* __restrict
                                                          const int4* __restrict__ tiles, int size,
                                                          int rows, O* __restrict__ out) {
   __shared__ float red[128][9];
-  const int col = blockIdx.x * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3;
+  const int col = blockIdx.y * 8 + (threadIdx.x & 7), slice = threadIdx.x >> 3;
   int64_t r0 = 0;
   int n = rows;
   if (first_tile) {
-    const int t0 = first_tile[blockIdx.y];
+    const int t0 = first_tile[blockIdx.x];
     r0 = t0 < 0 ? 0 : t0;
     n = t0 < 0 ? 0 : (tiles[t0].y + size - 1) / size;
   }
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(1024) void norm_rows_kernel(const float* __restrict
     t += __shfl_xor(t, 8, 64);
     t += __shfl_xor(t, 16, 64);
     t += __shfl_xor(t, 32, 64);
-    if (threadIdx.x < 8 && col < cols) out[(int64_t)blockIdx.y * cols + col] = (O)t;
+    if (threadIdx.x < 8 && col < cols) out[(int64_t)blockIdx.x * cols + col] = (O)t;
   }
 }
 
@@ -700,8 +700,8 @@ int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* 
     const int groups = std::min(sh.n_tiles, 2048);
     hipLaunchKernelGGL(f, dim3(groups), dim3(nt), lds, s, sh, x, a.ld, dy, w, b, stats, a.act,
                        (T*)dx, ws);
-    hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, ws, 2 * sh.C, nullptr,
-                       nullptr, 1, groups, (T*)dbw);
+    hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(1, cols), dim3(1024), 0, s, ws, 2 * sh.C,
+                       nullptr, nullptr, 1, groups, (T*)dbw);
     return mlcg_launch_status();
   }
   const unsigned lds = (unsigned)((nt * 2 * W + 2 * sh.C) * sizeof(float));
@@ -711,12 +711,13 @@ int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* 
   float* chain_sums = ws + (int64_t)sh.n_tiles * 2 * sh.C;
   hipLaunchKernelGGL(f, dim3(sh.n_tiles), dim3(nt), lds, s, sh, x, a.ld, dy, w, b, stats, a.act,
                      part);
-  hipLaunchKernelGGL(norm_rows_kernel<float>, dim3(cols, (unsigned)sh.chains), dim3(1024), 0, s,
+  // chains on the grid's first axis: the second one ends at 65535
+  hipLaunchKernelGGL(norm_rows_kernel<float>, dim3((unsigned)sh.chains, cols), dim3(1024), 0, s,
                      part, 2 * sh.C, a.first_tile, sh.tiles, sh.size, 0, chain_sums);
   hipLaunchKernelGGL((norm_bwd_apply_kernel<T, W, NT>), dim3(sh.n_tiles), dim3(nt),
                      (unsigned)((2 * sh.C + 2 * sh.G) * sizeof(float)), s, sh, x, a.ld, dy, w, b,
                      stats, chain_sums, a.act, (T*)dx);
-  hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(cols), dim3(1024), 0, s, chain_sums, 2 * sh.C,
+  hipLaunchKernelGGL(norm_rows_kernel<T>, dim3(1, cols), dim3(1024), 0, s, chain_sums, 2 * sh.C,
                      nullptr, nullptr, 1, (int)sh.chains, (T*)dbw);
   return mlcg_launch_status();
 }
