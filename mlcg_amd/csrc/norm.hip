@@ -615,9 +615,21 @@ struct NormArgs {
   float eps;
 };
 
+// A chain a workgroup where chains are short, or many of like lengths.  A longer
+// one among many is one workgroup's work, about 50 us for each of its slabs
+// forward and backward, so that it is slabs for all where it has more of them
+// than a compute unit's share of the slabs or chains (a chain's joins cost 0.14
+// us).  128 channels in fp32, forward and backward, a chain a workgroup / slabs:
+// 600 chains of 100 and one of 3000 609 / 136 us, 512 of 100 and one of 50000
+// 10060 / 139, 20000 of 30 and one of 50000 10857 / 2198; of like lengths, 512 of
+// 5000 2032 / 2039, 600 of 1500 792 / 789.
 constexpr int kOneRows = 1024, kOneChains = 512;
 
-bool by_chain(int max_len, int n_whole) { return max_len <= kOneRows || n_whole >= kOneChains; }
+bool by_chain(int64_t max_len, int64_t n_whole, int64_t n_tiles, int64_t chains) {
+  const int64_t longest = (max_len + kSlabRows - 1) / kSlabRows;
+  return max_len <= kOneRows ||
+         (n_whole >= kOneChains && longest <= std::max(n_tiles, chains) / 256);
+}
 
 // Threads of a workgroup: a column of every vector of a row, and at least 4
 // rows of them where a row has no more than 256 vectors; twice as many where
@@ -627,7 +639,7 @@ bool by_chain(int max_len, int n_whole) { return max_len <= kOneRows || n_whole 
 int norm_threads(const NormArgs& a, int W) {
   const int tc = a.C / W;
   if (tc > 64) return 1024;
-  return by_chain(a.max_len, a.n_whole) && a.n_whole <= 256 && a.max_len > 4 * (256 / tc)
+  return by_chain(a.max_len, a.n_whole, a.n_tiles, a.chains) && a.n_whole <= 256 && a.max_len > 4 * (256 / tc)
              ? 512
              : 256;
 }
@@ -662,7 +674,7 @@ int allow(F f, unsigned lds) {
 
 template <typename T, int W, int K, int NT>
 int norm_fwd(const NormArgs& a, void* y, float* stats, float* ws, hipStream_t s) {
-  const bool one = by_chain(a.max_len, a.n_whole);
+  const bool one = by_chain(a.max_len, a.n_whole, a.n_tiles, a.chains);
   const NormShape sh = norm_shape<W>(a, one, NT);
   constexpr int nt = NT;
   const unsigned lds = (unsigned)((3 * sh.G + (nt + sh.TC) * 2 * K) * sizeof(float));
@@ -688,7 +700,7 @@ int norm_fwd(const NormArgs& a, void* y, float* stats, float* ws, hipStream_t s)
 template <typename T, int W, int K, int NT>
 int norm_bwd(const NormArgs& a, const float* stats, void* dx, void* dbw, float* ws,
              hipStream_t s) {
-  const bool one = by_chain(a.max_len, a.n_whole);
+  const bool one = by_chain(a.max_len, a.n_whole, a.n_tiles, a.chains);
   const NormShape sh = norm_shape<W>(a, one, NT);
   constexpr int nt = NT;
   const T *x = (const T*)a.x, *dy = (const T*)a.dy, *w = (const T*)a.w, *b = (const T*)a.b;
@@ -771,7 +783,7 @@ extern "C" int64_t mlcg_group_norm_workspace_floats(int64_t n_tiles, int64_t cha
                                                     int groups, int backward) {
   if (n_tiles < 0 || chains < 0 || n_whole < 0 || max_len < 0 || width < 1 || groups < 1)
     return -1;
-  if (max_len <= kOneRows || n_whole >= kOneChains)
+  if (by_chain(max_len, n_whole, n_tiles, chains))
     return backward ? 2 * std::min<int64_t>(n_whole, 2048) * width : 0;
   return backward ? 2 * (n_tiles + chains) * width : 4 * n_tiles * groups;
 }

@@ -37,6 +37,24 @@ def test_gradients_over_many_chains(act, dtype):
     _check_norm(_randn((sum(lens), 32), dtype, 1) + 0.5, lens, 4, act)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_long_chain_among_many(dtype):
+    """600 short chains and one of 50000 beads, whose first beads lie far from
+    the others: its workgroups are many, and its deviations are taken from means
+    of neighbours."""
+    from mlcg_amd import _lib, ops
+
+    print(f"one long chain {dtype}", flush=True)
+    lens = [20] * 300 + [50000] + [35] * 300
+    x = _randn((sum(lens), 64), dtype, 1)
+    x[6000:6064] += 1000.0
+    _check_norm(x, lens, 4, "none")
+    chains = ops.chain_layout(lens, "cuda")
+    assert _lib.load().mlcg_group_norm_workspace_floats(
+        chains.tiles[256].shape[0], chains.n_chains, chains.whole.shape[0], chains.max_len, 64, 4,
+        0) > 0
+
+
 def test_more_chains_than_a_grid_axis():
     """70000 chains, most of them empty or short, and a long one."""
     print("70000 chains", flush=True)
