@@ -36,7 +36,9 @@
 // buffers: one barrier a tile.
 //
 // LDS rows hold 16-byte chunks, exchanged by row (xor), so that the 16-byte
-// reads of 8 consecutive rows and the transposing reads fall on all banks.
+// reads of 8 consecutive rows and the transposing reads fall on all banks (of
+// all LDS instructions, the writes among them, 0.8 to 1.2 conflict cycles each
+// are counted in 16 bits, of 4 to 5 that they take).
 //
 // The bias of an offset is one LDS value a head: an array over the offsets
 // from -(R + M) to R + M, M beyond the largest span of a tile, so that a tile
@@ -348,7 +350,7 @@ __device__ __forceinline__ int wave_max(int v) {
 
 // s[n] += the wave's 32 columns of  tile . B  for the rows 32 n .. 32 n + 31.
 // Of 16 channels in 32 bits the padding is passed over (48 chains of up to 268
-// beads, 8 heads: dk and dv 56 us against 66).
+// beads, 8 heads: dq 59 us against 72, dk and dv 54 against 69).
 template <typename T, int DP, int N>
 __device__ __forceinline__ void row_product(const T* tile, const v8<T> (&b)[DP / 16], int dim,
                                             f32x16 (&s)[N]) {
@@ -677,7 +679,7 @@ struct FwdLds {
 
 // a query's fragments and an accumulator of DP rows; one wave more where a
 // workgroup of four waves has few chunks to hold (2 x 4099 beads of 64 channels
-// in bf16: 160 us against 218, as all workgroups then run at once)
+// in bf16: 133 us against 167, as all workgroups then run at once)
 template <typename T, int DP, int NQ, int NK>
 constexpr int fwd_waves() {
   constexpr int values = DP * (int)sizeof(T) / 8 + DP / 2;
@@ -686,14 +688,13 @@ constexpr int fwd_waves() {
 
 // Forward; lanes are queries, the tiles hold keys.  Bound by the issue of its
 // matrix and vector instructions, which overlap between the waves of a SIMD
-// alone: at 8191 beads, 8 heads of 64 on 2 in bf16 a logit costs 6.8 vector
+// alone: at 8191 beads, 8 heads of 64 on 2 in bf16 a logit costs 6.9 vector
 // instructions (one of them exp2, at a quarter of the rate), so that they take
-// 57 % of the SIMDs' cycles and the products 24 %.  224 us, 613 TFLOP/s, 53 %
-// of a large library product's rate.  4 chains of 1031, 4 heads of 32 in fp32:
-// 47 us (46 TFLOP/s), 144 workgroups of 128 queries on 256 compute units.
-// 512 chains of up to 100, 4 heads of 32 in bf16: 20 us (25 with rest, 8-byte
-// stores of separate rows), one or two tiles a
-// workgroup, bound by the latency of its first loads.
+// about 60 % of the SIMDs' cycles and the products 25 %.  211 us, 652 TFLOP/s,
+// 56 % of a large library product's rate.  4 chains of 1031, 4 heads of 32 in
+// fp32: 47 us (46 TFLOP/s), 144 workgroups of 128 queries on 256 compute units.
+// 512 chains of up to 100, 4 heads of 32 in bf16, with rest: 19 us, one or two
+// tiles a workgroup, bound by the latency of its first loads.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void attn_fwd_kernel(
     AttnArgs a, T* __restrict__ out) {
@@ -767,7 +768,7 @@ __global__ __launch_bounds__(64 * NQ * NK, (fwd_waves<T, DP, NQ, NK>())) void at
 #pragma unroll 1
     for (int turn = 1;; ++turn) {
       // nothing of the tile is kept in registers for another turn (hipcc would,
-      // and spill: 1053 us in place of 216 at 8191 beads)
+      // and spill: 1053 us in place of 211 at 8191 beads)
       asm volatile("" ::: "memory");
       f32x16 s[N];
       load_rows<N>(cap, s);
@@ -870,7 +871,7 @@ __device__ __forceinline__ bool lone_key(const uint8_t* keep, int len) {
 constexpr int kDiagPitch = 68;  // 32 values and the gap of zeros; 16-byte rows
 // queries that pass through the block at a time: half of them where the
 // registers allow three waves a SIMD, which the whole block's LDS would not
-// (512 chains of up to 100 beads, 4 heads of 32 in bf16: dq 35 us against 43)
+// (512 chains of up to 100 beads, 4 heads of 32 in bf16: dq 37 us against 47)
 template <int DP>
 constexpr int diag_rows() {
   return DP == 32 ? 16 : 32;
@@ -1038,12 +1039,13 @@ constexpr int dq_waves() {
 
 // dq, delta and the workgroup's part of the table's gradient; lanes are
 // queries as in the forward pass.  2 chains of 4099 beads, 8 heads of 64 in
-// bf16: 228 us (452 TFLOP/s over three products), vector instructions 36 % of
-// the SIMDs' cycles, products 18 %, the diagonals' LDS round trips in the band
+// bf16: 220 us (469 TFLOP/s over three products), vector instructions 39 % of
+// the SIMDs' cycles, products 19 %, the diagonals' LDS round trips in the band
 // and the waits at the tiles' barrier the rest.  48 chains of up to 268, 8
-// heads of 16 in fp32, positions given: 63 us, of which the sums by offset
-// about 30 (77 with the diagonals' block kept beside the integers: two
-// workgroups a compute unit instead of three).  4 chains of 1031, 4 heads of 32 in fp32: 74 us.
+// heads of 16 in fp32, positions given: 59 us, of which the sums by offset
+// about 30 (14 more with the diagonals' block kept beside the integers: two
+// workgroups a compute unit instead of three).  4 chains of 1031, 4 heads of 32
+// in fp32: 71 us.
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dq_waves<T, DP>())) void attn_dq_kernel(
     AttnArgs a, T* __restrict__ dq, AttnRows rows_out, const int32_t* __restrict__ order,
@@ -1250,10 +1252,10 @@ constexpr int dkv_waves() {
 // dk and dv; lanes are keys, the tiles hold queries.  The query heads that
 // share a key/value head are taken one after the other, so their gradients are
 // summed in one wave's registers, in order.  2 chains of 4099 beads, 8 heads
-// of 64 in bf16: 214 us (643 TFLOP/s over four products), products 26 % of
-// the SIMDs' cycles, vector instructions 25 %; two waves a SIMD (128 fragments
+// of 64 in bf16: 209 us (658 TFLOP/s over four products), products 27 % of
+// the SIMDs' cycles, vector instructions 31 %; two waves a SIMD (128 fragments
 // and accumulators a lane) do not cover the LDS reads between them.  4 chains
-// of 1031, 4 heads of 32 in fp32: 81 us (54 TFLOP/s; 144 workgroups).
+// of 1031, 4 heads of 32 in fp32: 80 us (54 TFLOP/s; 144 workgroups).
 template <typename T, int DP, int NQ, int NK, bool VEC, int POS>
 __global__ __launch_bounds__(64 * NQ * NK, (dkv_waves<T, DP>())) void attn_dkv_kernel(
     AttnArgs a, AttnRows rows_in, T* __restrict__ dk, T* __restrict__ dv) {
@@ -1603,7 +1605,7 @@ int attn_backward<MLCG_ATTENTION_TYPE>(AttnArgs a, int shape, const AttnGrads& o
     return e;
   // keys of shared heads give fewer workgroups than queries: where they are no
   // more than the compute units, two waves share a block of keys (8191 beads,
-  // 8 heads on 2 key heads in bf16: both passes 793 us against 1048)
+  // 8 heads on 2 key heads in bf16: both passes 735 us against 1009)
   const int64_t groups = (int64_t)a.n_tiles * (a.heads / a.group);
   const int kv_shape = shape >= 20 && groups <= 256 ? shape / 10 * 10 + 2 : shape;
   if (int e = by_shape<(int)sizeof(T), false>(a, kv_shape, [&](auto dp, auto nq, auto nk,

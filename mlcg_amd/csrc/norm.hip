@@ -27,16 +27,17 @@
 // chains: slabs of them, joined in slab order, then a second reading.
 //
 // Measured: 2048 chains of up to 268 beads, 128 channels, bf16, silu: forward
-// 47 us, backward 106 + 6; three and five passes over 64 MB, the second
-// readings from the last cache: 4.1 and 3.0 TB/s against the 5.2 of a large
+// 47 us, backward 106 + 6; three and five passes over 79.5 MB, the second
+// readings from the last cache: 5.0 and 3.75 TB/s against the 5.2 of a large
 // copy.  The backward's vector instructions (the activation's derivative in
 // both passes) take half of the SIMDs' cycles.  With the chain kept in
 // registers (20 rows of a thread, two waves a SIMD) in place of the second
 // reading: 57 and 244 us, as too few waves are left to hide the loads; 192
 // chains of up to 80 in fp32 gained 2 us of 12 and of 15, less than such
-// calls' launches cost.  One chain of 120001 beads, fp32: statistics 22 us,
-// application 38, backward 45 and 63, all at 2.7 to 3.3 TB/s, and as much with
-// slabs of 128 and of 64 rows.
+// calls' launches cost.  One chain of 120001 beads of 256 channels, fp32, 123 MB
+// a pass: statistics 22 us, application 38, backward 45 and 63, 5.4 to 6.5 TB/s
+// over their one, two, two and three passes, whose number is what bounds it; as
+// much with slabs of 128 and of 64 rows.
 #include <algorithm>
 #include <type_traits>
 

@@ -2027,14 +2027,14 @@ def _attention_shape_rule(chains: ChainLayout, heads: int, dim: int, dtype: torc
     """(beads of a tile, parts of the other side that a workgroup's waves share)
     of the attention kernels, by the chains' lengths and the workgroups of 128
     beads that there are for 256 compute units.  Measured (us, forward /
-    backward): 512 chains of 35 beads in bf16 25 / 76 with tiles of 64, 27 / 83
-    with 128.  One of 2048, 8 heads of 64 in bf16 (128 workgroups): 27 / 106 in
-    two parts of 64, 23 / - in four, 53 / 145 whole.  6 of 1000, 4 heads of 32
-    in fp32 (192): 44 / 149 in two parts of 128, 47 / 151 of 64, 48 / 159 whole.
-    10 of these (320, a second round of a quarter): 69 / 232 in two parts of
-    64, 80 / 275 whole, and 16 (512) 87 / 291 and 82 / 279; in bf16 10 take
-    33 / 124 and 31 / 90.  2 of 4096 in bf16 (512): 137 / 358 in two parts of
-    128, 139 / 344 whole."""
+    backward): 512 chains of 35 beads in bf16 15 / 59 with tiles of 64, 15 / 60
+    with 128.  One of 2048, 8 heads of 64 in bf16 (128 workgroups): 29 / 83 in
+    two parts of 64, 23 / - in four, 42 / 101 whole.  6 of 1000, 4 heads of 32
+    in fp32 (192): 47 / 149 in two parts of 128, 45 / 151 of 64, 48 / 162 whole.
+    10 of these (320, a second round of a quarter): 69 / 235 in two parts of
+    64, 81 / 278 whole, and 16 (512) 88 / 296 and 82 / 282; in bf16 10 take
+    22 / 76 and 26 / 71.  2 of 4096 in bf16 (512): 117 / 308 in two parts of
+    128, 106 / 286 whole."""
     if chains.max_len <= 32 and backward:
         return 32, 1
     if chains.max_len <= 64:
