@@ -759,10 +759,10 @@ int mlcg_type_sum(const float* x, const int64_t* types, int64_t rows, int featur
                   int num_types, float* out, int* bad, float* workspace,
                   int64_t workspace_floats, void* stream);
 
-/* The same for tables of up to 2^24 - 1 rows (a row a bead of the molecules,
- * mlcg_group_norm_act and below), whose workgroups serve a share of the sites
- * each; rows < 2^31, no workspace, the same bits on every run.  Sites outside
- * the table as in mlcg_type_sum. */
+/* The same for tables of up to 2^24 - 1 rows (one for every bead of a set of
+ * molecules): each workgroup serves a share of the sites.  rows < 2^31, no
+ * workspace, the same bits on every run.  Sites outside the table as in
+ * mlcg_type_sum. */
 int mlcg_site_sum(const float* x, const int64_t* sites, int64_t rows, int features,
                   int num_sites, float* out, int* bad, void* stream);
 

@@ -640,7 +640,8 @@ bool by_chain(int64_t max_len, int64_t n_whole, int64_t n_tiles, int64_t chains)
 int norm_threads(const NormArgs& a, int W) {
   const int tc = a.C / W;
   if (tc > 64) return 1024;
-  return by_chain(a.max_len, a.n_whole, a.n_tiles, a.chains) && a.n_whole <= 256 && a.max_len > 4 * (256 / tc)
+  return by_chain(a.max_len, a.n_whole, a.n_tiles, a.chains) && a.n_whole <= 256 &&
+                 a.max_len > 4 * (256 / tc)
              ? 512
              : 256;
 }

@@ -66,7 +66,7 @@ def test_autocast(dropout, dtype):
     """fp32 parameters under autocast: the 16-bit kernels run, the parameters'
     gradients are fp32.  About twenty roundings of 2^-8 (2^-11) follow each
     other in two layers, forward and backward: 2^-8 sqrt(20) = 1.7e-2 in the
-    mean, of which some meet differences: 5e-2 (2^-11: a eighth)."""
+    mean, of which some meet differences: 5e-2 (2^-11: an eighth)."""
     g = torch.Generator().manual_seed(1)
     x = torch.randn(sum(LENS), 128, generator=g).cuda()
     grad = torch.randn(sum(LENS), 128, generator=g).cuda()
