@@ -1,10 +1,10 @@
 // Dropout with a residual sum, the mask from a counter (gfx950):
 //   out[e] = residual[e] + (u16(e) >= t ? x[e] * 65536 / (65536 - t) : 0)
 // The mask is never stored: u16(e) is half-word e % 8 of the 128 bits that
-// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC 2011) gives for the key
-// `seed` and the counter (e / 8, step), so the backward pass is the same
-// kernel on the gradient, without a residual.  The step may live in device
-// memory: a recorded graph then draws a new mask on every replay.
+// Philox4x32-10 (philox.h) gives for the key `seed` and the counter (e / 8,
+// step), so the backward pass is the same kernel on the gradient, without a
+// residual.  The step may live in device memory: a recorded graph then draws a
+// new mask on every replay.
 //
 // The drop probability is held in 16 bits (t = round(65536 p)), and the kept
 // values are scaled by the probability that is drawn, so the expectation is
@@ -16,35 +16,15 @@
 // 133 us for 703 MB (5.3 TB/s, the rate of a large copy); 17920 x 128 in fp32
 // 5.8 us a pass.
 #include "chain.h"
+#include "philox.h"
 
 namespace {
 
 constexpr int kDropThreads = 256;
 
-// keep[j] of the elements 8 c .. 8 c + 7
-struct Halves {
-  uint32_t w[4];
-  __device__ __forceinline__ uint32_t get(int j) const {
-    return (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-  }
-};
-
-__device__ __forceinline__ Halves drop_halves(uint64_t c, uint64_t step, uint64_t seed) {
-  uint32_t x0 = (uint32_t)c, x1 = (uint32_t)(c >> 32);
-  uint32_t x2 = (uint32_t)step, x3 = (uint32_t)(step >> 32);
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = (uint64_t)0xD2511F53u * x0;
-    const uint64_t b = (uint64_t)0xCD9E8D57u * x2;
-    x0 = (uint32_t)(b >> 32) ^ x1 ^ k0;
-    x1 = (uint32_t)b;
-    x2 = (uint32_t)(a >> 32) ^ x3 ^ k1;
-    x3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return Halves{{x0, x1, x2, x3}};
+// the half-word of element j of the eight that a counter serves
+__device__ __forceinline__ uint32_t half_word(const Philox& r, int j) {
+  return (j & 1) ? r.w[j >> 1] >> 16 : r.w[j >> 1] & 0xFFFFu;
 }
 
 template <typename T>
@@ -61,17 +41,17 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(
       const v8<T> xv = *reinterpret_cast<const v8<T>*>(x + e);
       v8<T> rv{};
       if (residual) rv = *reinterpret_cast<const v8<T>*>(residual + e);
-      const Halves h = drop_halves((uint64_t)c, step, seed);
+      const Philox h = mlcg_philox(seed, (uint64_t)c, step);
       v8<T> y;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        y[j] = (T)((float)rv[j] + (h.get(j) >= t ? (float)xv[j] * scale : 0.0f));
+        y[j] = (T)((float)rv[j] + (half_word(h, j) >= t ? (float)xv[j] * scale : 0.0f));
       *reinterpret_cast<v8<T>*>(out + e) = y;
     } else {
-      const Halves h = drop_halves((uint64_t)c, step, seed);
+      const Philox h = mlcg_philox(seed, (uint64_t)c, step);
       for (int j = 0; j < 8 && e + j < n; ++j)
         out[e + j] = (T)((residual ? (float)residual[e + j] : 0.0f) +
-                         (h.get(j) >= t ? (float)x[e + j] * scale : 0.0f));
+                         (half_word(h, j) >= t ? (float)x[e + j] * scale : 0.0f));
     }
   }
 }

@@ -17,29 +17,9 @@
 // lives in device memory and the final B kernel advances it, so a captured
 // graph of one step draws fresh noise on every replay.  Callers may instead
 // pass explicit noise (a [N, 3] array), which the parity tests use.
-#include "common.h"
+#include "philox.h"
 
 namespace {
-
-struct U4 {
-  uint32_t a, b, c, d;
-};
-
-__device__ __forceinline__ U4 philox4x32_10(U4 ctr, uint32_t k0, uint32_t k1) {
-  const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u;
-  const uint32_t W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p0 = (uint64_t)M0 * ctr.a;
-    const uint64_t p1 = (uint64_t)M1 * ctr.c;
-    const uint32_t hi0 = (uint32_t)(p0 >> 32), lo0 = (uint32_t)p0;
-    const uint32_t hi1 = (uint32_t)(p1 >> 32), lo1 = (uint32_t)p1;
-    ctr = U4{hi1 ^ ctr.b ^ k0, lo1, hi0 ^ ctr.d ^ k1, lo0};
-    k0 += W0;
-    k1 += W1;
-  }
-  return ctr;
-}
 
 // uniform in (0, 1]
 __device__ __forceinline__ float u01(uint32_t x) {
@@ -48,17 +28,15 @@ __device__ __forceinline__ float u01(uint32_t x) {
 
 __device__ __forceinline__ void normals3(uint64_t seed, int64_t bead, int64_t step, float& n0,
                                          float& n1, float& n2) {
-  const U4 r = philox4x32_10(U4{(uint32_t)bead, (uint32_t)((uint64_t)bead >> 32),
-                                (uint32_t)step, (uint32_t)((uint64_t)step >> 32)},
-                             (uint32_t)seed, (uint32_t)(seed >> 32));
+  const Philox r = mlcg_philox(seed, (uint64_t)bead, (uint64_t)step);
   const float two_pi = 6.283185307179586f;
-  const float ra = sqrtf(-2.0f * logf(u01(r.a)));
-  const float rb = sqrtf(-2.0f * logf(u01(r.c)));
+  const float ra = sqrtf(-2.0f * logf(u01(r.w[0])));
+  const float rb = sqrtf(-2.0f * logf(u01(r.w[2])));
   float s, c;
-  sincosf(two_pi * u01(r.b), &s, &c);
+  sincosf(two_pi * u01(r.w[1]), &s, &c);
   n0 = ra * c;
   n1 = ra * s;
-  sincosf(two_pi * u01(r.d), &s, &c);
+  sincosf(two_pi * u01(r.w[3]), &s, &c);
   n2 = rb * c;
 }
 
