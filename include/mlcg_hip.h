@@ -1115,6 +1115,112 @@ int mlcg_dropout_add(const void* x, const void* residual, int64_t n, int dtype,
                      int threshold, uint64_t seed, const int64_t* step_dev,
                      int64_t step, void* out, void* stream);
 
+/* The gated delta rule along chains.  A head's state S [dk, dv] goes from bead
+ * to bead of a chain, forwards or (reverse) from the last bead to the first,
+ *   S <- e^decay S,  S <- S + beta k (v - S^T k)^T,  out = scale S^T q,
+ * q and k, with normalize, brought to length one before (x / sqrt(x.x + 1e-6)).
+ * A bead that `keep` [beads] marks with 0 leaves the state as it is: its k, v,
+ * decay and beta are not read as numbers; its q still reads the state.
+ * q, k [beads, key_heads, dk] and v [beads, heads, dv] have the strides
+ * {row, head} in elements; head h reads key head h / (heads / key_heads); dk and
+ * dv lie in 1 .. 128.  decay, beta [beads, heads] are fp32, decay (the logarithm
+ * of the factor) at most 0 for a state that does not grow, -inf included.
+ * state and last_state [chains, heads, dk, dv], fp32, may be NULL (zeros; not
+ * wanted); last_state is not written for a chain without beads.
+ * `tiles` have 64 rows; segments [n_segments, 4]: (chain, its first tile there,
+ * tiles, 1 for a chain's first | 2 for its last), those of a chain one after the
+ * other; segment_first [n_whole + 1]: where the segments of each of the n_whole
+ * chains with beads begin.  With split = 0 every chain is one segment; else the
+ * segments run at the same time and are joined.
+ * kept and workspace have the sizes that mlcg_gated_delta_floats gives (n_split:
+ * n_segments, 0 without split): which 0, kept; 1, kept for the backward pass
+ * (train); 2, workspace of the forward and 3 of the backward pass.  Both begin
+ * at multiples of 32 bytes.
+ * The backward pass gives the gradients of q, k, v (contiguous), decay, beta
+ * and, unless grad_state is NULL, of state; grad_last_state may be NULL.
+ * mlcg_gated_delta_step: one bead each for `batch` states [batch, heads, dk, dv];
+ * next_state may be state. */
+int64_t mlcg_gated_delta_floats(int64_t beads, int64_t n_tiles, int64_t n_split,
+                                int heads, int dk, int dv, int dtype,
+                                int which);
+int mlcg_gated_delta(const void* q, const int64_t* q_strides, const void* k,
+                     const int64_t* k_strides, const void* v,
+                     const int64_t* v_strides, const float* decay,
+                     const float* beta, int64_t beads, int heads, int key_heads,
+                     int dk, int dv, int dtype, const int32_t* tiles,
+                     int64_t n_tiles, const int32_t* segments,
+                     int64_t n_segments, const int32_t* segment_first,
+                     int64_t n_whole, int split, const uint8_t* keep,
+                     const float* state, float scale, int normalize,
+                     int reverse, void* out, float* last_state, float* kept,
+                     int64_t kept_floats, int train, float* workspace,
+                     int64_t workspace_floats, void* stream);
+int mlcg_gated_delta_backward(
+    const void* q, const int64_t* q_strides, const void* k,
+    const int64_t* k_strides, const void* v, const int64_t* v_strides,
+    const float* decay, const float* beta, int64_t beads, int heads,
+    int key_heads, int dk, int dv, int dtype, const int32_t* tiles,
+    int64_t n_tiles, const int32_t* segments, int64_t n_segments,
+    const int32_t* segment_first, int64_t n_whole, int split,
+    const uint8_t* keep, float scale, int normalize, int reverse,
+    const float* kept, int64_t kept_floats, const void* grad_out,
+    const float* grad_last_state, void* grad_q, void* grad_k, void* grad_v,
+    float* grad_decay, float* grad_beta, float* grad_state, float* workspace,
+    int64_t workspace_floats, void* stream);
+int mlcg_gated_delta_step(const void* q, const int64_t* q_strides,
+                          const void* k, const int64_t* k_strides,
+                          const void* v, const int64_t* v_strides,
+                          const float* decay, const float* beta, int64_t batch,
+                          int heads, int key_heads, int dk, int dv, int dtype,
+                          const float* state, float scale, int normalize,
+                          void* out, float* next_state, void* stream);
+
+/* RMS norm of rows with the residual's addition: t = x + residual,
+ * y = t / sqrt(mean t^2 + eps) weight over a row's channels.  x, weight and y
+ * have the type dtype, residual and t residual_dtype, the same or fp32; the norm
+ * is that of the sum before it is rounded to t.  residual NULL: t = x, and t is
+ * not written.  x and residual have row strides; y, t and the gradients are
+ * contiguous; 1 <= width <= 8192; rstd [rows] is kept for the backward pass.
+ * Backward, with t as it was stored (x, of type residual_dtype = dtype, without
+ * a residual): grad_x = grad_residual in the types of x and t, either may be
+ * NULL, and so may grad_t (zeros). */
+int mlcg_rms_norm_add(const void* x, int64_t x_ld, const void* residual,
+                      int64_t r_ld, const void* weight, int64_t rows, int width,
+                      int dtype, int residual_dtype, float eps, void* y,
+                      void* t, float* rstd, void* stream);
+int64_t mlcg_rms_norm_add_workspace_floats(int64_t rows, int width);
+int mlcg_rms_norm_add_backward(const void* grad_y, const void* grad_t,
+                               const void* t, int64_t t_ld, const void* weight,
+                               const float* rstd, int64_t rows, int width,
+                               int dtype, int residual_dtype, void* grad_x,
+                               void* grad_residual, void* grad_weight,
+                               float* workspace, int64_t workspace_floats,
+                               void* stream);
+
+/* Embedding lookup with a factor: out[i] = scale table[tokens[i]], table
+ * [rows, width] and out contiguous, rows < 2^30, width <= 8192, fewer than 2^31
+ * tokens.  A token outside the table gives a zero row and raises bit 2 of the
+ * numerics flags.
+ * mlcg_token_order: the rows' order by token, rows of one token in their order:
+ * keys [n], the tokens in order (`rows` for those outside the table, which come
+ * last), and index [n], the rows.
+ * mlcg_scaled_embedding_backward: grad_table[v] = scale times the sum of the
+ * rows of grad whose token is v, in a fixed order; grad_table begins at a
+ * multiple of 16 bytes. */
+int mlcg_scaled_embedding(const void* table, int64_t rows,
+                          const int64_t* tokens, int64_t n, int width,
+                          int dtype, float scale, void* out, void* stream);
+int64_t mlcg_token_order_workspace_ints(int64_t n, int64_t rows);
+int mlcg_token_order(const int64_t* tokens, int64_t n, int64_t rows, int* keys,
+                     int* index, int* workspace, int64_t workspace_ints,
+                     void* stream);
+int64_t mlcg_scaled_embedding_workspace_floats(int64_t n, int width);
+int mlcg_scaled_embedding_backward(const void* grad, const int* keys,
+                                   const int* index, int64_t n, int64_t rows,
+                                   int width, int dtype, float scale,
+                                   void* grad_table, float* workspace,
+                                   int64_t workspace_floats, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

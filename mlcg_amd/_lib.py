@@ -163,6 +163,26 @@ _SIGNATURES = {
     "mlcg_group_norm_act_backward": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64,
         _P, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P],
     "mlcg_dropout_add": [_P, _P, _I64, _I32, _I32, _U64, _P, _I64, _P, _P],
+    "mlcg_gated_delta_floats": [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32],
+    "mlcg_gated_delta": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32,
+        _P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _F32, _I32, _I32, _P, _P, _P, _I64, _I32,
+        _P, _I64, _P],
+    "mlcg_gated_delta_backward": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32,
+        _I32, _P, _I64, _P, _I64, _P, _I64, _I32, _P, _F32, _I32, _I32, _P, _I64, _P, _P, _P,
+        _P, _P, _P, _P, _P, _P, _I64, _P],
+    "mlcg_gated_delta_step": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32,
+        _I32, _P, _F32, _I32, _P, _P, _P],
+    "mlcg_rms_norm_add": [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _F32, _P, _P, _P,
+        _P],
+    "mlcg_rms_norm_add_workspace_floats": [_I64, _I32],
+    "mlcg_rms_norm_add_backward": [_P, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _P,
+        _P, _P, _I64, _P],
+    "mlcg_scaled_embedding": [_P, _I64, _P, _I64, _I32, _I32, _F32, _P, _P],
+    "mlcg_token_order_workspace_ints": [_I64, _I64],
+    "mlcg_token_order": [_P, _I64, _I64, _P, _P, _P, _I64, _P],
+    "mlcg_scaled_embedding_workspace_floats": [_I64, _I32],
+    "mlcg_scaled_embedding_backward": [_P, _P, _P, _I64, _I64, _I32, _I32, _F32, _P, _P, _I64,
+        _P],
 }
 _RESTYPES = {"mlcg_version": _c.c_char_p, "mlcg_scan_workspace_ints": _I64,
              "mlcg_radius_workspace_bytes": _I64,
@@ -178,6 +198,10 @@ _RESTYPES = {"mlcg_version": _c.c_char_p, "mlcg_scan_workspace_ints": _I64,
              "mlcg_type_sum_workspace_floats": _I64, "mlcg_node_weight_image_bytes": _I64,
              "mlcg_chain_attention_workspace_floats": _I64,
              "mlcg_group_norm_workspace_floats": _I64,
+             "mlcg_gated_delta_floats": _I64,
+             "mlcg_rms_norm_add_workspace_floats": _I64,
+             "mlcg_token_order_workspace_ints": _I64,
+             "mlcg_scaled_embedding_workspace_floats": _I64,
              "mlcg_mse_workspace_floats": _I64, "mlcg_prior_pair_records_ints": _I64,
              "mlcg_mfma_loop_flops_per_wave_iter": _I64}
 

@@ -2,6 +2,8 @@ from .activations import ShiftedSoftplus
 from .chain import (ChainAttention, ChainEmbedding, ChainEncoder, ChainEncoderLayer,
                     CounterDropout, GroupNormAct, chain_attention, dropout_add, group_norm_act)
 from .cutoff import CosineCutoff, IdentityCutoff
+from .delta import (ChainDelta, ChainDeltaEncoder, ChainDeltaLayer, RMSNormAdd, gated_delta,
+                    rms_norm_add, scaled_embedding)
 from .gradients import EnergyOut, GradientsOut, SumOut
 from .losses import EnergyMSE, ForceMSE, ForceRMSE, Loss
 from .mlp import MLP, init_xavier_uniform
@@ -19,4 +21,5 @@ __all__ = ["ShiftedSoftplus", "CosineCutoff", "IdentityCutoff", "EnergyOut", "Gr
            "StaticHarmonicAngles", "StaticDihedral", "StaticRepulsion",
            "ChainAttention", "ChainEmbedding", "ChainEncoder", "ChainEncoderLayer",
            "CounterDropout", "GroupNormAct", "chain_attention", "dropout_add",
-           "group_norm_act"]
+           "group_norm_act", "ChainDelta", "ChainDeltaEncoder", "ChainDeltaLayer",
+           "RMSNormAdd", "gated_delta", "rms_norm_add", "scaled_embedding"]

@@ -271,14 +271,18 @@ class ChainEmbedding(torch.nn.Module):
 
     types [S]: the sites' bead types, chain after chain; lengths: the beads of
     every chain; keep [S] bool: sites without a resolved structure; positions
-    [S]: residue numbers (the index in the chain by default).
+    [S]: residue numbers (the index in the chain by default).  encoder: a
+    ChainEncoder or a ChainDeltaEncoder.  scale: a factor on the types' embeddings;
+    given, the look-up and its gradient go by scaled_embedding, which sums the
+    sites of a type in a fixed order (None: torch's look-up, no factor).
 
     The table is made anew in every forward pass, as training needs it;
     ``as_embedding()`` gives it as a plain Embedding for simulations."""
 
     def __init__(self, embedding_size: int, width: int, encoder: torch.nn.Module, types, lengths,
-                 keep=None, positions=None):
+                 keep=None, positions=None, scale: Optional[float] = None):
         super().__init__()
+        self.scale = None if scale is None else float(scale)
         self.weight = torch.nn.Parameter(torch.empty(embedding_size, width))
         self.encoder = encoder
         self.register_buffer("types", torch.as_tensor(types, dtype=torch.int64))
@@ -314,7 +318,12 @@ class ChainEmbedding(torch.nn.Module):
         return state
 
     def table(self) -> torch.Tensor:
-        x = torch.nn.functional.embedding(self.types, self.weight)
+        if self.scale is None:
+            x = torch.nn.functional.embedding(self.types, self.weight)
+        else:
+            from .delta import scaled_embedding
+
+            x = scaled_embedding(self.weight, self.types, self.scale)
         return self.encoder(x, self.chains, self.keep, self.positions)
 
     def forward(self, sites: torch.Tensor) -> torch.Tensor:

@@ -2254,3 +2254,379 @@ def dropout_add(x: torch.Tensor, p: float, seed: int, step,
     call("mlcg_dropout_add", ptr(x), ptr(residual), x.numel(), dt, t, seed, ptr(step_dev), step,
          ptr(out), stream_handle(x.device))
     return out
+
+
+# --------------------------------------------------------------------------
+# The sequence encoder of linear cost
+
+MAX_DELTA_DIM = 128
+DELTA_ROWS = 64  # beads of a chunk
+MAX_RMS_WIDTH = 8192
+
+
+def _delta_heads(q, k, v, decay, beta, n: int, what: str):
+    """The checked arguments that gated_delta and its step share."""
+    require_device(q, k, v, decay, beta)
+    dt = _chain_dtype(q, what)
+    dev = q.device
+    q, qs = _attention_heads(q, "q", n, q.dtype, dev)
+    k, ks = _attention_heads(k, "k", n, q.dtype, dev)
+    v, vs = _attention_heads(v, "v", n, q.dtype, dev)
+    keys, dk, heads, dv = q.shape[1], q.shape[2], v.shape[1], v.shape[2]
+    _check(k.shape == q.shape, lambda: f"k must be {tuple(q.shape)} like q, got {tuple(k.shape)}")
+    _check(1 <= dk <= MAX_DELTA_DIM and 1 <= dv <= MAX_DELTA_DIM,
+           lambda: f"{what} takes heads of 1 .. {MAX_DELTA_DIM} channels, got {dk} and {dv}")
+    _check(1 <= keys <= heads <= 1024 and heads % keys == 0,
+           lambda: f"the heads of v must be a multiple of those of q and k and at most 1024, got "
+                   f"{heads} and {keys}")
+    for t, name in ((decay, "decay"), (beta, "beta")):
+        _check(t.shape == (n, heads) and t.dtype == torch.float32 and t.device == dev,
+               lambda: f"{name} must be [{n}, {heads}] float32 on {dev}, got {tuple(t.shape)} "
+                       f"{t.dtype} on {t.device}")
+    return (q, qs, k, ks, v, vs, decay.contiguous(), beta.contiguous(), heads, keys, dk, dv, dt)
+
+
+def _check_delta_state(state: Optional[torch.Tensor], name: str, shape, dev):
+    if state is None:
+        return None
+    require_device(state)
+    _check(state.shape == shape and state.dtype == torch.float32 and state.device == dev,
+           lambda: f"{name} must be {tuple(shape)} float32 on {dev}, got {tuple(state.shape)} "
+                   f"{state.dtype} on {state.device}")
+    return state.contiguous()
+
+
+@dataclass(eq=False)
+class _DeltaPlan:
+    segments: torch.Tensor  # [n, 4] int32
+    first: torch.Tensor     # [chains with beads + 1] int32
+    split: int
+
+
+def _delta_segment_tiles(chains: ChainLayout, heads: int, dv: int) -> int:
+    """Chunks of a segment, 0 for whole chains."""
+    return 0
+
+
+def _delta_plan(chains: ChainLayout, heads: int, dv: int) -> _DeltaPlan:
+    rows = _delta_segment_tiles(chains, heads, dv)
+    plan = chains.plans.get(("delta", rows))
+    if plan is None:
+        lens = np.asarray(chains.lengths, dtype=np.int64)
+        order = np.argsort(-lens, kind="stable")
+        order = order[lens[order] > 0]
+        count = -(-lens[order] // DELTA_ROWS)
+        begin = np.concatenate([[0], np.cumsum(count)])
+        segs, first = [], [0]
+        for chain, n, at in zip(order.tolist(), count.tolist(), begin.tolist()):
+            step = rows or n
+            for a in range(0, n, step):
+                segs.append((chain, at + a, min(step, n - a),
+                             (1 if a == 0 else 0) | (2 if a + step >= n else 0)))
+            first.append(len(segs))
+        packed = torch.from_numpy(np.concatenate(
+            [np.asarray(segs, dtype=np.int32).reshape(-1), np.asarray(first, dtype=np.int32)])
+        ).to(chains.device)
+        plan = chains.plans[("delta", rows)] = _DeltaPlan(
+            segments=packed[:4 * len(segs)].view(-1, 4), first=packed[4 * len(segs):],
+            split=int(rows > 0))
+    return plan
+
+
+def _delta_floats(chains: ChainLayout, plan: _DeltaPlan, heads, dk, dv, dt, which: int) -> int:
+    key = ("delta floats", plan.split, plan.segments.shape[0], heads, dk, dv, dt, which)
+    n = chains.plans.get(key)
+    if n is None:
+        n = chains.plans[key] = int(_lib.load().mlcg_gated_delta_floats(
+            chains.n_beads, chains.tiles[DELTA_ROWS].shape[0],
+            plan.segments.shape[0] if plan.split else 0, heads, dk, dv, dt, which))
+    return n
+
+
+def _delta_args(q, k, v, decay, beta, chains, scale, keep):
+    _check(isinstance(chains, ChainLayout), "chains must be a ChainLayout")
+    args = _delta_heads(q, k, v, decay, beta, chains.n_beads, "gated_delta")
+    dev, dk = args[0].device, args[10]
+    _check(chains.device == dev, "chains must be a ChainLayout on the rows' device")
+    if keep is not None:
+        _check(keep.shape == (chains.n_beads,) and keep.dtype == torch.bool
+               and keep.device == dev, lambda: f"keep must be [{chains.n_beads}] bool on {dev}")
+        keep = keep.contiguous()
+    return args, float(dk ** -0.5 if scale is None else scale), keep
+
+
+def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+                beta: torch.Tensor, chains: ChainLayout, scale: Optional[float] = None,
+                keep: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                reverse: bool = False, normalize: bool = True, train: bool = False
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(out [S, H, DV], last [B, H, DK, DV], kept): the gated delta rule along
+    every chain (mlcg_gated_delta).  A head's state goes from bead to bead,
+
+        S <- exp(decay) S,  S <- S + beta k (v - S^T k)^T,  out = scale S^T q,
+
+    forwards or, with reverse, from the last bead to the first; normalize brings
+    q and k to length one (x / sqrt(x.x + 1e-6)) before.
+
+    q and k [S, HK, DK], v [S, H, DV] (H a multiple of HK; views with any row
+    and head stride), decay (the factor's logarithm, at most 0 where states must
+    not grow; -inf empties the state) and beta [S, H] in float32; scale defaults
+    to 1 / sqrt(DK).  keep [S] bool: an absent bead (False) leaves the state as
+    it is, whatever its k, v, decay and beta hold; its q reads the state.  state
+    [B, H, DK, DV] float32: where each chain begins (zeros by default); last is
+    where it ends.  kept is what the backward pass takes (train=True)."""
+    (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
+        q, k, v, decay, beta, chains, scale, keep)
+    n, dev = chains.n_beads, q.device
+    state = _check_delta_state(state, "state", (chains.n_chains, heads, dk, dv), dev)
+    out = torch.empty(n, heads, dv, dtype=q.dtype, device=dev)
+    last = torch.empty(chains.n_chains, heads, dk, dv, dtype=torch.float32, device=dev)
+    if chains.whole.shape[0] < chains.n_chains:  # chains without beads end as they begin
+        last.zero_() if state is None else last.copy_(state)
+    if n == 0:
+        return out, last, torch.empty(0, dtype=torch.float32, device=dev)
+    plan = _delta_plan(chains, heads, dv)
+    size = _delta_floats(chains, plan, heads, dk, dv, dt, 1 if train else 0)
+    kept = torch.empty(size, dtype=torch.float32, device=dev)
+    nws = _delta_floats(chains, plan, heads, dk, dv, dt, 2)
+    ws = torch.empty(nws, dtype=torch.float32, device=dev) if nws > 0 else None
+    tiles = chains.tiles[DELTA_ROWS]
+    call("mlcg_gated_delta", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), n, heads,
+         keys, dk, dv, dt, ptr(tiles), tiles.shape[0], ptr(plan.segments), plan.segments.shape[0],
+         ptr(plan.first), plan.first.shape[0] - 1, plan.split, ptr(keep), ptr(state), scale,
+         int(normalize), int(reverse), ptr(out), ptr(last), ptr(kept), size, int(train), ptr(ws),
+         nws, stream_handle(dev))
+    return out, last, kept
+
+
+def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.Tensor,
+                         grad: torch.Tensor, grad_last: Optional[torch.Tensor] = None,
+                         scale: Optional[float] = None, keep: Optional[torch.Tensor] = None,
+                         reverse: bool = False, normalize: bool = True, want_state: bool = False):
+    """(grad q, grad k, grad v, grad decay, grad beta, grad state | None) of
+    gated_delta for the gradients of its outputs (mlcg_gated_delta_backward);
+    kept is the forward's, with train=True.  Every sum has a fixed order."""
+    (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
+        q, k, v, decay, beta, chains, scale, keep)
+    n, dev = chains.n_beads, q.device
+    _check(grad.shape == (n, heads, dv) and grad.dtype == q.dtype and grad.device == dev,
+           lambda: f"grad must be [{n}, {heads}, {dv}] {q.dtype} on {dev}")
+    grad = grad.contiguous()
+    shape = (chains.n_chains, heads, dk, dv)
+    grad_last = _check_delta_state(grad_last, "grad_last", shape, dev)
+    dq = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
+    dkk = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
+    dvv = torch.empty(n, heads, dv, dtype=q.dtype, device=dev)
+    ddecay = torch.empty(n, heads, dtype=torch.float32, device=dev)
+    dbeta = torch.empty(n, heads, dtype=torch.float32, device=dev)
+    dstate = torch.empty(shape, dtype=torch.float32, device=dev) if want_state else None
+    if want_state and chains.whole.shape[0] < chains.n_chains:
+        dstate.zero_() if grad_last is None else dstate.copy_(grad_last)
+    if n == 0:
+        return dq, dkk, dvv, ddecay, dbeta, dstate
+    plan = _delta_plan(chains, heads, dv)
+    size = _delta_floats(chains, plan, heads, dk, dv, dt, 1)
+    _check(kept.shape == (size,) and kept.dtype == torch.float32 and kept.device == dev,
+           "kept must be what gated_delta gave with train=True for the same chains")
+    nws = _delta_floats(chains, plan, heads, dk, dv, dt, 3)
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    tiles = chains.tiles[DELTA_ROWS]
+    call("mlcg_gated_delta_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta),
+         n, heads, keys, dk, dv, dt, ptr(tiles), tiles.shape[0], ptr(plan.segments),
+         plan.segments.shape[0], ptr(plan.first), plan.first.shape[0] - 1, plan.split, ptr(keep),
+         scale, int(normalize), int(reverse), ptr(kept), size, ptr(grad), ptr(grad_last), ptr(dq),
+         ptr(dkk), ptr(dvv), ptr(ddecay), ptr(dbeta), ptr(dstate), ptr(ws), nws,
+         stream_handle(dev))
+    return dq, dkk, dvv, ddecay, dbeta, dstate
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    first, second = a.data_ptr(), b.data_ptr()
+    return (first < second + b.numel() * b.element_size()
+            and second < first + a.numel() * a.element_size())
+
+
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+                     beta: torch.Tensor, state: torch.Tensor, scale: Optional[float] = None,
+                     normalize: bool = True, into: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out [B, H, DV]: one more bead for each of B chains (mlcg_gated_delta_step),
+    the rule of gated_delta on states that lie in memory: q and k [B, HK, DK], v
+    [B, H, DV], decay and beta [B, H] float32, state [B, H, DK, DV] float32.  The
+    new states take the old ones' place or, given `into`, go there.  No
+    gradients."""
+    _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [B, heads, dim]")
+    _check(not (torch.is_grad_enabled()
+                and any(t.requires_grad for t in (q, k, v, decay, beta, state))),
+           "gated_delta_step has no gradients: call it under torch.no_grad()")
+    batch = q.shape[0]
+    q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = _delta_heads(
+        q, k, v, decay, beta, batch, "gated_delta_step")
+    dev, shape = q.device, (batch, heads, dk, dv)
+    into = state if into is None else into
+    for t, name in ((state, "state"), (into, "into")):
+        require_device(t)
+        _check(t.shape == shape and t.dtype == torch.float32 and t.device == dev
+               and t.is_contiguous(),
+               lambda: f"{name} must be a contiguous {shape} float32 on {dev}")
+    _check(state.data_ptr() == into.data_ptr() or not _overlap(state, into),
+           "into must be the state itself or not overlap it")
+    out = torch.empty(batch, heads, dv, dtype=q.dtype, device=dev)
+    call("mlcg_gated_delta_step", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), batch,
+         heads, keys, dk, dv, dt, ptr(state), float(dk ** -0.5 if scale is None else scale),
+         int(normalize), ptr(out), ptr(into), stream_handle(dev))
+    return out
+
+
+def _rms_rows(t: torch.Tensor, width: int):
+    """t with channels that lie next to each other, and its row stride."""
+    ld, step = t.stride()
+    if (width > 1 and step != 1) or ld < 0:
+        t, ld = t.contiguous(), width
+    return t, ld
+
+
+def _rms_types(x, residual, weight):
+    require_device(x, residual, weight)
+    dt = _chain_dtype(x, "rms_norm_add")
+    _check(x.dim() == 2 and 1 <= x.shape[1] <= MAX_RMS_WIDTH and x.shape[0] < 2 ** 31,
+           lambda: f"x must be [rows, 1 .. {MAX_RMS_WIDTH} channels], got {tuple(x.shape)}")
+    _check(weight.shape == x.shape[1:] and weight.dtype == x.dtype and weight.device == x.device,
+           lambda: f"weight must be [{x.shape[1]}] {x.dtype} on {x.device}")
+    if residual is not None:
+        _check(residual.shape == x.shape and residual.device == x.device
+               and residual.dtype in (x.dtype, torch.float32),
+               lambda: f"residual must be {tuple(x.shape)} {x.dtype} or float32 on {x.device}, "
+                       f"got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+    return dt
+
+
+def rms_norm_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y [N, C], t [N, C], rstd [N]): t = x + residual and its RMS norm,
+    y = t / sqrt(mean t^2 + eps) weight, over the channels of a row
+    (mlcg_rms_norm_add).  y has x's and weight's type, t the residual's: the same
+    or float32 (a residual stream in 32 bits beside 16-bit layers); the norm is
+    that of the sum before t is rounded.  residual None: t is x itself.  x and
+    residual may have any row stride."""
+    dt = _rms_types(x, residual, weight)
+    n, width = x.shape
+    dev = x.device
+    x, ld = _rms_rows(x, width)
+    y = torch.empty(n, width, dtype=x.dtype, device=dev)
+    rstd = torch.empty(n, dtype=torch.float32, device=dev)
+    t, rld, rdt = x, 0, dt
+    if residual is not None:
+        residual, rld = _rms_rows(residual, width)
+        t = torch.empty(n, width, dtype=residual.dtype, device=dev)
+        rdt = DTYPE_IDS[residual.dtype]
+    call("mlcg_rms_norm_add", ptr(x), ld, ptr(residual), rld, ptr(weight.contiguous()), n, width,
+         dt, rdt, float(eps), ptr(y), None if residual is None else ptr(t), ptr(rstd),
+         stream_handle(dev))
+    return y, t, rstd
+
+
+def rms_norm_add_backward(grad: torch.Tensor, grad_t: Optional[torch.Tensor], t: torch.Tensor,
+                          weight: torch.Tensor, rstd: torch.Tensor
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(grad x, grad residual, grad weight) of rms_norm_add for the gradients of
+    y and t (None: zeros); t and rstd are the forward's.  The first two are one
+    tensor where x and the residual have one type."""
+    dt = _rms_types(grad, t, weight)
+    n, width = t.shape
+    dev = t.device
+    _check(rstd.shape == (n,) and rstd.dtype == torch.float32 and rstd.device == dev,
+           lambda: f"rstd must be [{n}] float32 on {dev}")
+    if grad_t is not None:
+        _check(grad_t.shape == t.shape and grad_t.dtype == t.dtype and grad_t.device == dev,
+               lambda: f"grad_t must be {tuple(t.shape)} {t.dtype} on {dev}")
+        grad_t = grad_t.contiguous()
+    grad, rstd = grad.contiguous(), rstd.contiguous()
+    t, ld = _rms_rows(t, width)
+    dx = torch.empty(n, width, dtype=grad.dtype, device=dev)
+    dr = dx if t.dtype == grad.dtype else torch.empty(n, width, dtype=t.dtype, device=dev)
+    if n == 0:
+        return dx, dr, torch.zeros_like(weight)
+    dw = torch.empty(width, dtype=weight.dtype, device=dev)
+    nws = int(_lib.load().mlcg_rms_norm_add_workspace_floats(n, width))
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    call("mlcg_rms_norm_add_backward", ptr(grad), ptr(grad_t), ptr(t), ld,
+         ptr(weight.contiguous()), ptr(rstd), n, width, dt, DTYPE_IDS[t.dtype], ptr(dx),
+         None if dr is dx else ptr(dr), ptr(dw), ptr(ws), nws, stream_handle(dev))
+    return dx, dr, dw
+
+
+@dataclass(eq=False)
+class TokenOrder:
+    """The rows of an array of tokens in the order of their tokens (built by
+    token_order), rows of one token in their own order.
+
+    keys  : [N] int32, the tokens in order (`rows` for one outside the table)
+    index : [N] int32, the rows
+    rows  : rows of the table
+    """
+
+    keys: torch.Tensor
+    index: torch.Tensor
+    rows: int
+
+
+def _check_tokens(tokens: torch.Tensor) -> torch.Tensor:
+    require_device(tokens)
+    _check(tokens.dim() == 1 and tokens.dtype == torch.int64 and tokens.shape[0] < 2 ** 31,
+           lambda: f"tokens must be 1-D int64, got {tuple(tokens.shape)} {tokens.dtype}")
+    return tokens.contiguous()
+
+
+def token_order(tokens: torch.Tensor, rows: int) -> TokenOrder:
+    """TokenOrder of tokens [N] int64 for a table of `rows` rows, made on the
+    device (mlcg_token_order).  A token outside the table sets
+    NUMERICS_TYPE_RANGE (check_numerics raises)."""
+    tokens = _check_tokens(tokens)
+    _check(1 <= rows < 2 ** 30, "a table has 1 .. 2^30 - 1 rows")
+    n, dev = tokens.shape[0], tokens.device
+    keys, index = torch.empty(2, n, dtype=torch.int32, device=dev).unbind()
+    nws = int(_lib.load().mlcg_token_order_workspace_ints(n, rows))
+    ws = torch.empty(nws, dtype=torch.int32, device=dev)
+    call("mlcg_token_order", ptr(tokens), n, rows, ptr(keys), ptr(index), ptr(ws), nws,
+         stream_handle(dev))
+    return TokenOrder(keys=keys, index=index, rows=rows)
+
+
+def scaled_embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0
+                     ) -> torch.Tensor:
+    """out [N, C] = scale table[tokens] for a [V, C] table and tokens [N] int64
+    (mlcg_scaled_embedding); a token outside the table gives a zero row and sets
+    NUMERICS_TYPE_RANGE (check_numerics raises)."""
+    require_device(table, tokens)
+    dt = _chain_dtype(table, "scaled_embedding")
+    tokens = _check_tokens(tokens)
+    _check(table.dim() == 2 and 1 <= table.shape[0] < 2 ** 30
+           and 1 <= table.shape[1] <= MAX_RMS_WIDTH and tokens.device == table.device,
+           lambda: f"scaled_embedding takes a table of 1 .. {MAX_RMS_WIDTH} channels on the "
+                   f"tokens' device, got {tuple(table.shape)} on {table.device}")
+    table = table.contiguous()
+    out = torch.empty(tokens.shape[0], table.shape[1], dtype=table.dtype, device=table.device)
+    call("mlcg_scaled_embedding", ptr(table), table.shape[0], ptr(tokens), tokens.shape[0],
+         table.shape[1], dt, float(scale), ptr(out), stream_handle(table.device))
+    return out
+
+
+def scaled_embedding_backward(grad: torch.Tensor, order: TokenOrder, scale: float = 1.0
+                              ) -> torch.Tensor:
+    """grad table [V, C] = scale times the sums of grad's rows by token, in a
+    fixed order (mlcg_scaled_embedding_backward); order is token_order of the
+    tokens."""
+    require_device(grad)
+    dt = _chain_dtype(grad, "scaled_embedding_backward")
+    n = order.keys.shape[0]
+    _check(grad.dim() == 2 and grad.shape[0] == n and grad.device == order.keys.device
+           and 1 <= grad.shape[1] <= MAX_RMS_WIDTH,
+           lambda: f"grad must be [{n}, channels] on {order.keys.device}")
+    grad = grad.contiguous()
+    width, dev = grad.shape[1], grad.device
+    out = torch.empty(order.rows, width, dtype=grad.dtype, device=dev)
+    nws = int(_lib.load().mlcg_scaled_embedding_workspace_floats(n, width))
+    ws = torch.empty(nws, dtype=torch.float32, device=dev)
+    call("mlcg_scaled_embedding_backward", ptr(grad), ptr(order.keys), ptr(order.index), n,
+         order.rows, width, dt, float(scale), ptr(out), ptr(ws), nws, stream_handle(dev))
+    return out
