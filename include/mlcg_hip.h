@@ -1122,8 +1122,9 @@ int mlcg_dropout_add(const void* x, const void* residual, int64_t n, int dtype,
  * A bead that `keep` [beads] marks with 0 leaves the state as it is: its k, v,
  * decay and beta are not read as numbers; its q still reads the state.
  * q, k [beads, key_heads, dk] and v [beads, heads, dv] have the strides
- * {row, head} in elements; head h reads key head h / (heads / key_heads); dk and
- * dv lie in 1 .. 128.  decay, beta [beads, heads] are fp32, decay (the logarithm
+ * {row, head} in elements, row strides from 0 to below 2^22; head h reads key head h / (heads / key_heads); dk and
+ * dv are multiples of 8 up to 128 (of one bead, mlcg_gated_delta_step, any from
+ * 1): columns of zeros change nothing.  decay, beta [beads, heads] are fp32, decay (the logarithm
  * of the factor) at most 0 for a state that does not grow, -inf included.
  * state and last_state [chains, heads, dk, dv], fp32, may be NULL (zeros; not
  * wanted); last_state is not written for a chain without beads.
@@ -1140,8 +1141,8 @@ int mlcg_dropout_add(const void* x, const void* residual, int64_t n, int dtype,
  * and, unless grad_state is NULL, of state; grad_last_state may be NULL.
  * mlcg_gated_delta_step: one bead each for `batch` states [batch, heads, dk, dv];
  * next_state may be state. */
-int64_t mlcg_gated_delta_floats(int64_t beads, int64_t n_tiles, int64_t n_split,
-                                int heads, int dk, int dv, int dtype,
+int64_t mlcg_gated_delta_floats(int64_t n_tiles, int64_t n_split, int heads,
+                                int key_heads, int dk, int dv, int dtype,
                                 int which);
 int mlcg_gated_delta(const void* q, const int64_t* q_strides, const void* k,
                      const int64_t* k_strides, const void* v,

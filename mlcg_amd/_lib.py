@@ -163,7 +163,7 @@ _SIGNATURES = {
     "mlcg_group_norm_act_backward": [_P, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _P, _I64,
         _P, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P],
     "mlcg_dropout_add": [_P, _P, _I64, _I32, _I32, _U64, _P, _I64, _P, _P],
-    "mlcg_gated_delta_floats": [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32],
+    "mlcg_gated_delta_floats": [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32],
     "mlcg_gated_delta": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32,
         _P, _I64, _P, _I64, _P, _I64, _I32, _P, _P, _F32, _I32, _I32, _P, _P, _P, _I64, _I32,
         _P, _I64, _P],

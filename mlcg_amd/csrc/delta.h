@@ -27,7 +27,10 @@
 // Four kernels: delta_chunk forms T, P and the beads' factors of every chunk;
 // delta_scan carries the state along the chunks (16 columns of it a wave) and
 // gives u and o; delta_scan_back carries D; delta_grad gives the gradients of
-// q, k, beta and g of every chunk.
+// q, k, beta and g of every chunk.  Of few long chains the scans go over segments
+// of chunks at the same time: once from the state zero and from all unit vectors,
+// which gives the map of a segment, S -> M S + N; delta_join goes along these, and
+// the scan proper begins each segment at the state that it gives.
 //
 // The state, and all sums, are fp32.  Products are on the bf16 matrix
 // instructions with operands in pieces, x = x0 + x1 + ..., each the rounding
@@ -39,16 +42,20 @@
 // A result of the 16 x 16 x 32 instruction has 4 rows of one column in a lane,
 // which is half of what the next product wants of its right operand if its
 // sum's index runs in the order 4 g + j, 16 + 4 g + j (g the lane's quarter): the
-// chains K S -> T (..) -> K^T (..) stay in registers, and the left operands are
-// read in that order, rows as they are or, by the transposing read, columns.
+// chains K S -> T (..) -> K^T (..) stay in registers.  k, q, T and P lie in memory
+// and in LDS as the left operands that they are, in blocks of 16 rows x 32 columns:
+// lane (g, c) has row c's elements 4 g .. and 16 + 4 g .. in the 16 bytes of slot
+// 16 g + (c ^ 8 (g / 2)).  delta_chunk writes them so, absent beads and rows past
+// the end as zeros, and every later copy is one of memory to LDS as it stands.
+// The exchange of c spreads what the transposing read takes over more banks.
 #pragma once
 
 #include "chain.h"
 
 constexpr int kDeltaRows = 64;       // beads of a chunk
-constexpr int kDeltaThreads = 256;
+constexpr int kDeltaThreads = 256;   // of delta_chunk and delta_grad
 constexpr int kDeltaFactors = 8;     // arrays of factors of a chunk and head
-constexpr int kDeltaPlane = kDeltaRows * kDeltaRows;
+constexpr int kDeltaLower = 6;       // blocks of a lower triangle, 16 x 32
 
 // a chunk's factors, [kDeltaFactors][64] for each (chunk, head)
 enum {
@@ -70,32 +77,32 @@ struct DeltaArgs {
   int64_t beads;
   int heads, keys, group, dk, dv, dvp;  // dvp: dv rounded up to 16
   float scale;
-  int normalize, reverse, vec;  // vec: rows of q and k in 16-byte loads
+  int normalize, reverse;
   const int4* tiles;            // (chain's first row, its length, tile's first row in it, chain)
   int n_tiles;
   const int4* segs;             // (chain, first tile, tiles, 1 first of its chain | 2 last)
   const int* seg_first;         // [chains with beads + 1]
   int n_segs, n_whole;          // segments; chains with beads
   float* fac;
-  __bf16 *T, *P;
-  float *U, *S0;  // [heads, beads, dvp], [tile, heads, DK, dvp]
+  float4 *K, *Q;                // operands, [tile, keys, pieces, 4, DK / 32, 64 slots]
+  float4 *T, *P;                // [tile, heads, pieces, 6, 64 slots]
+  float *U, *S0;                // [tile, heads, 64, dvp], [tile, heads, DK, dvp]
 };
 
 struct DeltaBack {
   const void* grad;       // [beads, heads, dv]
-  const float* grad_state;
   void *dq, *dk, *dv;
   float *ddecay, *dbeta, *dstate;
-  float *D, *dR;          // [tile, heads, DK, dvp], [heads, beads, dvp]
+  float *D, *dR;          // as S0 and U
 };
 
 // where a scan begins and ends
 struct DeltaEnds {
-  const float* init;  // the caller's states [chain, heads, dk, dv], or of segments, or NULL
-  float* last;        // the caller's
+  const float* init;      // the caller's states [chain, heads, dk, dv], or NULL
+  float* last;            // the caller's
   const float* seg_init;  // [seg, heads, DK, dvp]
   float* seg_last;        // [seg, heads, DK, dvp]: the segments alone, from zero
-  float* seg_map;         // [seg, heads, DK, DK]: what they make of a state
+  float4* seg_map;        // the transpose of what they make of a state, as operands
 };
 
 template <typename T>
@@ -112,10 +119,13 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
 
 // pieces of the arrays' elements and of what is computed from them
 template <typename T> struct Pieces;
@@ -128,13 +138,26 @@ struct Frag {
   bf16x8 p[N];
 };
 
+// What a piece leaves is x - 1 x0 + 0 x0', one instruction on the pair that the
+// rounding gave (exact: x0 is the rounding of x).
 template <int N>
 __device__ __forceinline__ Frag<N> split8(f32x8 x) {
+  // (-1, 0) and (0, -1), from registers: as a constant in the instruction -1.0 is
+  // taken by the hardware in another half than the compiler means
+  uint32_t c0 = 0x0000BF80u, c1 = 0xBF800000u;
+  asm("" : "+v"(c0), "+v"(c1));
+  const bf16x2 first = __builtin_bit_cast(bf16x2, c0), second = __builtin_bit_cast(bf16x2, c1);
   Frag<N> f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     f.p[i] = __builtin_convertvector(x, bf16x8);
-    if (i + 1 < N) x -= __builtin_convertvector(f.p[i], f32x8);
+    if (i + 1 < N)
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const bf16x2 h = {f.p[i][j], f.p[i][j + 1]};
+        x[j] = __builtin_amdgcn_fdot2_f32_bf16(h, first, x[j], false);
+        x[j + 1] = __builtin_amdgcn_fdot2_f32_bf16(h, second, x[j + 1], false);
+      }
   }
   return f;
 }
@@ -152,6 +175,19 @@ __device__ __forceinline__ Frag<N> split_raw(v8<T> x) {
     return split8<N>(__builtin_convertvector(x, f32x8));
   }
 }
+// the sum of the pieces
+template <int N>
+__device__ __forceinline__ f32x8 whole(const Frag<N>& f) {
+  f32x8 x = __builtin_convertvector(f.p[N - 1], f32x8);
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) x += __builtin_convertvector(f.p[i], f32x8);
+  return x;
+}
+template <int HALF>
+__device__ __forceinline__ f32x4 half_of(f32x8 x) {
+  return HALF ? __builtin_shufflevector(x, x, 4, 5, 6, 7)
+              : __builtin_shufflevector(x, x, 0, 1, 2, 3);
+}
 
 // c += a b to the accuracy of the operand with more pieces
 template <int NA, int NB>
@@ -167,129 +203,155 @@ __device__ __forceinline__ void mma(f32x4& c, const Frag<NA>& a, const Frag<NB>&
     }
 }
 
-__device__ __forceinline__ int wave_number() {
-  return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// a value that all lanes have, as the one that it is
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int4 uniform(int4 x) {
+  return make_int4(uniform(x.x), uniform(x.y), uniform(x.z), uniform(x.w));
+}
+__device__ __forceinline__ int wave_number() { return uniform(threadIdx.x >> 6); }
+
+// A barrier for what the workgroup shares in LDS: loads and stores of memory stay
+// on their way across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// A tile of 64 rows of LEN elements in LDS, in N planes.  A row's stride of 16
-// more bytes moves it by four banks: the 16 rows x 16 bytes of half a wave of
-// the reads below fall on all banks.
-template <int N, int LEN>
-struct Tile {
-  static constexpr int stride = LEN + 8, plane = kDeltaRows * stride;
-  __bf16 x[N * plane];
+// Operands in LDS: N planes of NB blocks.
+template <int N, int NB>
+struct Image {
+  static constexpr int units = N * NB;  // of 1 KB
+  float4 x[units * 64];
 
-  // left operand: row `row`, its elements 32 kk + 4 g .. and 32 kk + 16 + 4 g ..
-  __device__ __forceinline__ Frag<N> rows(int row, int kk) const {
-    const int g = mlcg_lane() >> 4;
+  __device__ static __forceinline__ int slot() {
+    const int g = mlcg_lane() >> 4, c = mlcg_lane() & 15;
+    return 16 * g + (c ^ (8 * (g >> 1)));
+  }
+  // a block as a left operand
+  __device__ __forceinline__ Frag<N> rows(int block) const {
     Frag<N> f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const __bf16* p = x + i * plane + row * stride + 32 * kk + 4 * g;
-      const bf16x4 lo = *reinterpret_cast<const bf16x4*>(p);
-      const bf16x4 hi = *reinterpret_cast<const bf16x4*>(p + 16);
-      f.p[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
+    for (int i = 0; i < N; ++i)
+      f.p[i] = __builtin_bit_cast(bf16x8, x[(i * NB + block) * 64 + slot()]);
     return f;
   }
-  // left operand: column 16 m + (lane & 15), its rows 32 kk + 4 g .. and 32 kk + 16 + 4 g ..
-  __device__ __forceinline__ Frag<N> columns(int m, int kk) const {
-    const int lane = mlcg_lane(), g = lane >> 4;
+  // the transpose of blocks b0 and b1 (32 rows): columns 16 HALF .. of them
+  template <int HALF>
+  __device__ __forceinline__ Frag<N> columns(int b0, int b1) const {
     // 16 lanes give the places of 4 rows x 16 columns, lane i those of row
     // i / 4, and get a column's 4 rows each
-    const int row = 32 * kk + 4 * g + ((lane & 15) >> 2), el = 16 * m + 4 * (lane & 3);
+    const int lane = mlcg_lane(), s = lane & 3, r = 4 * (lane >> 4) + ((lane & 15) >> 2);
+    const int at = 16 * s + (r ^ (8 * (s >> 1)));
     Frag<N> f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      s16x4 r[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        r[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4*)(x + i * plane + (row + 16 * h) * stride + el));
-      f.p[i] = __builtin_bit_cast(bf16x8,
-                                  __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      const char* const p0 = reinterpret_cast<const char*>(&x[(i * NB + b0) * 64 + at]);
+      const char* const p1 = reinterpret_cast<const char*>(&x[(i * NB + b1) * 64 + at]);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 8 * HALF));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p1 + 8 * HALF));
+      f.p[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return f;
   }
 };
+
+// UNITS x 1 KB from memory to LDS, on their way when this returns
+template <int UNITS, int WAVES>
+__device__ __forceinline__ void send_to_lds(float4* lds, const float4* src) {
+  const int w = wave_number(), lane = mlcg_lane();
+#pragma unroll
+  for (int u = 0; u < (UNITS + WAVES - 1) / WAVES; ++u) {
+    const int unit = u * WAVES + w;
+    if ((u + 1) * WAVES <= UNITS || unit < UNITS)
+      __builtin_amdgcn_global_load_lds((global_void*)(src + 64 * unit + lane),
+                                       (lds_void*)(lds + 64 * unit), 16, 0, 0);
+  }
+}
+__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Where the beads of a chunk are.
 struct Chunk {
   int64_t base;  // bead of row 0
   int n, step;   // rows, and +1 or -1
+  Chunk() = default;
   __device__ __forceinline__ Chunk(const DeltaArgs& a, int tile) {
-    const int4 t = a.tiles[tile];
+    const int4 t = uniform(a.tiles[tile]);
     n = min(kDeltaRows, t.y - t.z);
     base = (int64_t)t.x + (a.reverse ? t.y - 1 - t.z : t.z);
     step = a.reverse ? -1 : 1;
   }
   __device__ __forceinline__ int64_t bead(int row) const { return base + (int64_t)row * step; }
+  // elements from row 0 to a row, rows past the end taken as the last one
+  __device__ __forceinline__ int offset(int row, int stride) const {
+    return min(row, n - 1) * step * stride;
+  }
 };
 
-// 8 elements of a row from el on, zeros past `len`
+// The rows r + l of a whole chunk, r the same for all lanes and l of 0 .. most by
+// lane, of an array of rows: an address that is the same for all lanes and an
+// offset, not negative, that is the same for all r.
+struct Lines {
+  char* at;
+  int stride;  // bytes
+  uint32_t lane;
+  __device__ __forceinline__ Lines(void* p, int64_t base, int step, int row_bytes, int l, int most,
+                                   int column_bytes) {
+    at = reinterpret_cast<char*>(p) + (step > 0 ? base : base - most) * row_bytes;
+    stride = step * row_bytes;
+    lane = (uint32_t)((step > 0 ? l : most - l) * row_bytes + column_bytes);
+    // not known to be the same from chunk to chunk: its multiples would be kept
+    asm volatile("" : "+s"(stride));
+  }
+  template <typename T>
+  __device__ __forceinline__ T& row(int r) const {
+    return *reinterpret_cast<T*>(at + r * stride + lane);
+  }
+};
+
+// The chunks of a segment one after the other, without looking them up.
+struct Walk {
+  int first, len, at;  // the chain's first bead and length, the chunk's first row in it
+  __device__ __forceinline__ Walk(const DeltaArgs& a, int tile) {
+    const int4 t = uniform(a.tiles[tile]);
+    first = t.x;
+    len = t.y;
+    at = t.z;
+  }
+  __device__ __forceinline__ Chunk chunk(const DeltaArgs& a, int rows_on) const {
+    Chunk c;
+    const int from = at + rows_on;
+    c.n = min(kDeltaRows, len - from);
+    c.base = (int64_t)first + (a.reverse ? len - 1 - from : from);
+    c.step = a.reverse ? -1 : 1;
+    return c;
+  }
+};
+
+// elements that are aligned as one
+template <typename T, int N>
+struct loose {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+// 8 and 4 elements of a row of len (a multiple of 8) from el on, zeros past its
+// end: without a branch, so that loads are not waited for one by one
 template <typename T>
-__device__ __forceinline__ v8<T> load8(const T* row, int el, int len, bool vec) {
-  v8<T> x{};
-  if (vec) {
-    if (el < len) x = *reinterpret_cast<const v8<T>*>(row + el);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (el + j < len) x[j] = row[el + j];
-  }
-  return x;
+__device__ __forceinline__ v8<T> load8(const T* row, int el, int len) {
+  const v8<T> x = *reinterpret_cast<const typename loose<T, 8>::type*>(row + min(el, len - 8));
+  return el < len ? x : v8<T>{};
 }
-
-// A chunk's rows of q or k on their way to LDS.
-template <typename T, int DK, int N>
-struct StageRows {
-  static constexpr int per_row = DK / 8, per = kDeltaRows * per_row / kDeltaThreads;
-  v8<T> x[per];
-  __device__ __forceinline__ void load(const DeltaArgs& a, const Chunk& c, const T* src,
-                                       int64_t row_stride, bool masked) {
-#pragma unroll
-    for (int p = 0; p < per; ++p) {
-      const int i = threadIdx.x + p * kDeltaThreads, row = i / per_row;
-      x[p] = v8<T>{};
-      if (row < c.n) {
-        const int64_t bead = c.bead(row);
-        if (!masked || !a.keep || a.keep[bead])
-          x[p] = load8<T>(src + bead * row_stride, 8 * (i % per_row), a.dk, a.vec);
-      }
-    }
-  }
-  __device__ __forceinline__ void put(Tile<N, DK>& t) const {
-#pragma unroll
-    for (int p = 0; p < per; ++p) {
-      const int i = threadIdx.x + p * kDeltaThreads;
-      const Frag<N> f = split_raw<N, T>(x[p]);
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        *reinterpret_cast<bf16x8*>(t.x + j * t.plane + i / per_row * t.stride +
-                                   8 * (i % per_row)) = f.p[j];
-    }
-  }
-};
-
-// A chunk's T or P, planes of 64 x 64, on their way to LDS.
-template <int N>
-struct StageMatrix {
-  static constexpr int per = N * kDeltaPlane / 8 / kDeltaThreads;
-  bf16x8 x[per];
-  __device__ __forceinline__ void load(const __bf16* src) {
-#pragma unroll
-    for (int p = 0; p < per; ++p)
-      x[p] = *reinterpret_cast<const bf16x8*>(src + 8 * (threadIdx.x + p * kDeltaThreads));
-  }
-  __device__ __forceinline__ void put(Tile<N, kDeltaRows>& t) const {
-#pragma unroll
-    for (int p = 0; p < per; ++p) {
-      const int i = threadIdx.x + p * kDeltaThreads, j = i / (kDeltaPlane / 8),
-                r = i % (kDeltaPlane / 8);
-      *reinterpret_cast<bf16x8*>(t.x + j * t.plane + r / 8 * t.stride + 8 * (r % 8)) = x[p];
-    }
-  }
-};
+template <typename T>
+__device__ __forceinline__ v4<T> load4(const T* row, int el, int len) {
+  const v4<T> x = *reinterpret_cast<const typename loose<T, 4>::type*>(row + min(el, len - 4));
+  return el < len ? x : v4<T>{};
+}
+// 4 values to a row of len (a multiple of 8) from el on
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int el, int len, f32x4 x) {
+  typedef typename loose<T, 4>::type vec;
+  if (el < len) *reinterpret_cast<vec*>(row + el) = __builtin_convertvector(x, vec);
+}
 
 __device__ __forceinline__ float exp2_of(float hi, float lo) {
   return __builtin_amdgcn_exp2f(hi + lo);
@@ -302,66 +364,86 @@ __device__ __forceinline__ float quarter_sum(float v) {
 }
 
 // ---------------------------------------------------------------------------
-// T, P and the factors of a chunk, for the heads of one key head.
+// T, P and the factors of a chunk, for the heads of one key head, and k and q as
+// operands.
+
+template <typename T, int DK>
+struct ChunkTiles {
+  Image<Pieces<T>::in, DK / 8> k;
+  float A[kDeltaRows][kDeltaRows + 4];
+  float diag[4][16][20];  // inverses of the diagonal blocks
+  float ghi[kDeltaRows], glo[kDeltaRows], rk[kDeltaRows], rq[kDeltaRows], be[kDeltaRows];
+};
 
 template <typename T, int DK>
 __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
-  constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32;
-  constexpr int LD = kDeltaRows + 4;
-  __shared__ __align__(16) float A[kDeltaRows][LD];
-  __shared__ __align__(16) float diag[4][16][20];  // inverses of the diagonal blocks
-  __shared__ float ghi[kDeltaRows], glo[kDeltaRows], rk[kDeltaRows], rq[kDeltaRows],
-      be[kDeltaRows];
+  constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32, NB = 4 * KS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  ChunkTiles<T, DK>& sh = *reinterpret_cast<ChunkTiles<T, DK>*>(smem);
+  auto& A = sh.A;
   const int tile = blockIdx.x, kh = blockIdx.y;
   const int w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
+  const int slot = sh.k.slot();
   const Chunk ch(a, tile);
-  const T* const q = (const T*)a.q + kh * a.q_head;
-  const T* const k = (const T*)a.k + kh * a.k_head;
+  const int row = 16 * w + c;
+  const bool in = row < ch.n;
+  const int64_t bead = ch.bead(min(row, ch.n - 1));
+  const bool there = in && (!a.keep || a.keep[bead]);
 
-  // products of this wave's 16 beads (columns) with those up to them (rows)
+  // this wave's 16 beads, as columns
   Frag<NI> kb[KS], qb[KS];
   float nk = 0.0f, nq = 0.0f;
-  const int row = 16 * w + c;
-  bool there = false;
   {
-    const bool in = row < ch.n;
-    const int64_t bead = in ? ch.bead(row) : 0;
-    there = in && (!a.keep || a.keep[bead]);
+    const T* const q = (const T*)a.q + kh * a.q_head + bead * a.q_row;
+    const T* const k = (const T*)a.k + kh * a.k_head + bead * a.k_row;
+    v4<T> x[KS][2], y[KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[s][j] = load4<T>(k, 32 * s + 16 * j + 4 * g, a.dk);
+        y[s][j] = load4<T>(q, 32 * s + 16 * j + 4 * g, a.dk);
+      }
+    const int64_t at = ((int64_t)tile * a.keys + kh) * (NI * NB * 64) + w * KS * 64 + slot;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      v8<T> x{}, y{};
-      if (there) x = load8<T>(k + bead * a.k_row, 32 * s + 8 * g, a.dk, a.vec);
-      if (in) y = load8<T>(q + bead * a.q_row, 32 * s + 8 * g, a.dk, a.vec);
+      v8<T> u = __builtin_shufflevector(x[s][0], x[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      v8<T> v = __builtin_shufflevector(y[s][0], y[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if (!there) u = v8<T>{};
+      if (!in) v = v8<T>{};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        nk = fmaf((float)x[j], (float)x[j], nk);
-        nq = fmaf((float)y[j], (float)y[j], nq);
+        nk = fmaf((float)u[j], (float)u[j], nk);
+        nq = fmaf((float)v[j], (float)v[j], nq);
       }
-      kb[s] = split_raw<NI, T>(x);
-      qb[s] = split_raw<NI, T>(y);
+      kb[s] = split_raw<NI, T>(u);
+      qb[s] = split_raw<NI, T>(v);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const float4 f = __builtin_bit_cast(float4, kb[s].p[i]);
+        sh.k.x[(i * NB + w * KS + s) * 64 + slot] = f;
+        a.K[at + (i * NB + s) * 64] = f;
+        a.Q[at + (i * NB + s) * 64] = __builtin_bit_cast(float4, qb[s].p[i]);
+      }
     }
   }
   nk = quarter_sum(nk);
   nq = quarter_sum(nq);
   if (g == 0) {
-    rk[row] = !there ? 0.0f : a.normalize ? 1.0f / sqrtf(nk + 1e-6f) : 1.0f;
-    rq[row] = a.normalize ? 1.0f / sqrtf(nq + 1e-6f) : 1.0f;
+    sh.rk[row] = !there ? 0.0f : a.normalize ? 1.0f / sqrtf(nk + 1e-6f) : 1.0f;
+    sh.rq[row] = a.normalize ? 1.0f / sqrtf(nq + 1e-6f) : 1.0f;
   }
+  __syncthreads();
+  // products with the beads up to them
   f32x4 kk[4], qk[4];
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     kk[m] = f32x4{};
     qk[m] = f32x4{};
     if (m > w) continue;
-    const int r = 16 * m + c;
-    const bool in = r < ch.n;
-    const int64_t bead = in ? ch.bead(r) : 0;
-    const bool here = in && (!a.keep || a.keep[bead]);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      v8<T> x{};
-      if (here) x = load8<T>(k + bead * a.k_row, 32 * s + 8 * g, a.dk, a.vec);
-      const Frag<NI> f = split_raw<NI, T>(x);
+      const Frag<NI> f = sh.k.rows(m * KS + s);
       mma(kk[m], f, kb[s]);
       mma(qk[m], f, qb[s]);
     }
@@ -369,13 +451,12 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
 
   for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
     const int64_t at = (int64_t)tile * a.heads + h;
-    __syncthreads();  // rk, rq; the last head's A has been read
     if (w == 0) {
-      const bool in = lane < ch.n;
-      const int64_t bead = in ? ch.bead(lane) : 0;
-      const bool here = in && (!a.keep || a.keep[bead]);
-      float d = here ? a.decay[bead * a.heads + h] : 0.0f;
-      const float b = here ? a.beta[bead * a.heads + h] : 0.0f;
+      const bool here = lane < ch.n && (!a.keep || a.keep[ch.bead(lane)]);
+      const int64_t x = ch.bead(min(lane, ch.n - 1)) * a.heads + h;
+      float d = a.decay[x], b = a.beta[x];
+      d = here ? d : 0.0f;
+      b = here ? b : 0.0f;
       if (d < -256.0f) d = -256.0f;  // e^g is 0 all the same, and -inf - -inf no number
       double G = (double)d * 1.4426950408889634;
 #pragma unroll
@@ -385,41 +466,45 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
       }
       const float hi = (float)G, lo = (float)(G - (double)hi);
       const float hc = __shfl(hi, 63, MLCG_WAVE), lc = __shfl(lo, 63, MLCG_WAVE);
-      ghi[lane] = hi;
-      glo[lane] = lo;
-      be[lane] = b;
-      const float e = exp2_of(hi, lo);
+      sh.ghi[lane] = hi;
+      sh.glo[lane] = lo;
+      sh.be[lane] = b;
+      const float e = exp2_of(hi, lo), rk = sh.rk[lane], rq = sh.rq[lane];
       float* const f = a.fac + at * (kDeltaFactors * kDeltaRows) + lane;
-      f[kFacRead * kDeltaRows] = e * rk[lane];
-      f[kFacWrite * kDeltaRows] = exp2_of(hc - hi, lc - lo) * rk[lane];
+      f[kFacRead * kDeltaRows] = e * rk;
+      f[kFacWrite * kDeltaRows] = exp2_of(hc - hi, lc - lo) * rk;
       f[kFacBeta * kDeltaRows] = b;
-      f[kFacOut * kDeltaRows] = a.scale * e * rq[lane];
+      f[kFacOut * kDeltaRows] = a.scale * e * rq;
       f[kFacHi * kDeltaRows] = hi;
       f[kFacLo * kDeltaRows] = lo;
-      f[kFacK * kDeltaRows] = rk[lane];
-      f[kFacQ * kDeltaRows] = rq[lane];
+      f[kFacK * kDeltaRows] = rk;
+      f[kFacQ * kDeltaRows] = rq;
     }
     __syncthreads();
     // rows s = 16 m + 4 g + i, column t = 16 w + c
-    const float th = ghi[row], tl = glo[row], bt = be[row] * rk[row], qt = a.scale * rq[row];
+    const float th = sh.ghi[row], tl = sh.glo[row];
+    const float bt = sh.be[row] * sh.rk[row], qt = a.scale * sh.rq[row];
+    f32x4 y[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      f32x4 x, y;
+      f32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int s = 16 * m + 4 * g + i;
-        const float e = s <= row ? exp2_of(th - ghi[s], tl - glo[s]) * rk[s] : 0.0f;
+        const float e = s <= row ? exp2_of(th - sh.ghi[s], tl - sh.glo[s]) * sh.rk[s] : 0.0f;
         x[i] = s < row ? bt * e * kk[m][i] : 0.0f;
-        y[i] = s <= row ? qt * e * qk[m][i] : 0.0f;
+        y[m][i] = s <= row ? qt * e * qk[m][i] : 0.0f;
       }
-      *reinterpret_cast<f32x4*>(&A[row][16 * m + 4 * g]) = x;
-      __bf16* p = a.P + at * (NM * kDeltaPlane) + row * kDeltaRows + 16 * m + 4 * g;
+      if (m <= w) *reinterpret_cast<f32x4*>(&A[row][16 * m + 4 * g]) = x;
+    }
 #pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        const bf16x4 z = __builtin_convertvector(y, bf16x4);
-        *reinterpret_cast<bf16x4*>(p + i * kDeltaPlane) = z;
-        y -= __builtin_convertvector(z, f32x4);
-      }
+    for (int j = 0; j < 2; ++j) {
+      if (j > w / 2) continue;
+      const Frag<NM> f = split44<NM>(y[2 * j], y[2 * j + 1]);
+#pragma unroll
+      for (int i = 0; i < NM; ++i)
+        a.P[((at * NM + i) * kDeltaLower + w + (w == 3) + j) * 64 + slot] =
+            __builtin_bit_cast(float4, f.p[i]);
     }
     __syncthreads();
     // (1 + A)^-1: column c of the inverse of this wave's diagonal block, by
@@ -434,18 +519,17 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
     }
     if (g == 0)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) diag[w][r][c] = z[r];
+      for (int r = 0; r < 16; ++r) sh.diag[w][r][c] = z[r];
     __syncthreads();
     // ... and the blocks below it, T_i = -T_ii sum_j A_ij T_j, in fp32
     f32x4 t[4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) t[m] = f32x4{};
-#pragma unroll
     for (int i = 0; i < 4; ++i) {
+      t[i] = f32x4{};
       if (i < w) continue;
       if (i == w) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[i][e] = diag[w][4 * g + e][c];
+        for (int e = 0; e < 4; ++e) t[i][e] = sh.diag[w][4 * g + e][c];
         continue;
       }
       f32x4 s{};
@@ -457,7 +541,7 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
         for (int e = 0; e < 4; ++e)
           s = __builtin_amdgcn_mfma_f32_16x16x4f32(l[e], t[j][e], s, 0, 0, 0);
       }
-      const f32x4 l = *reinterpret_cast<const f32x4*>(&diag[i][c][4 * g]);
+      const f32x4 l = *reinterpret_cast<const f32x4*>(&sh.diag[i][c][4 * g]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         t[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[e], s[e], t[i], 0, 0, 0);
@@ -468,114 +552,239 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) A[16 * i + 4 * g + e][16 * w + c] = t[i][e];
     __syncthreads();
+    for (int u = w; u < kDeltaLower; u += 4) {
+      const int b = u < 2 ? u : 2 + (u - 2) / 2, j = u < 2 ? 0 : u % 2;
+      const Frag<NM> f =
+          split44<NM>(*reinterpret_cast<const f32x4*>(&A[16 * b + c][32 * j + 4 * g]),
+                      *reinterpret_cast<const f32x4*>(&A[16 * b + c][32 * j + 16 + 4 * g]));
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int i = threadIdx.x + p * kDeltaThreads, r = i / 8, s = 8 * (i % 8);
-      const Frag<NM> f = split44<NM>(*reinterpret_cast<const f32x4*>(&A[r][s]),
-                                     *reinterpret_cast<const f32x4*>(&A[r][s + 4]));
-#pragma unroll
-      for (int j = 0; j < NM; ++j)
-        *reinterpret_cast<bf16x8*>(a.T + (at * NM + j) * kDeltaPlane + r * kDeltaRows + s) =
-            f.p[j];
+      for (int i = 0; i < NM; ++i)
+        a.T[((at * NM + i) * kDeltaLower + u) * 64 + slot] = __builtin_bit_cast(float4, f.p[i]);
     }
+    __syncthreads();  // A and the gates have been read
   }
 }
 
 // ---------------------------------------------------------------------------
-// The state along the chunks of a segment: 16 columns a wave, 64 a workgroup.
+// The state along the chunks of a segment: 16 columns a wave, all a workgroup.
 
-// a head's 16 x 4 rows of a column of v, do: rows 16 b + 4 g + i
-template <typename T>
-__device__ __forceinline__ void load_column(f32x4 (&x)[4], const Chunk& ch, const T* src,
-                                            int64_t stride, bool in) {
-  const int g = mlcg_lane() >> 4;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * b + 4 * g + i;
-      x[b][i] = in && r < ch.n ? (float)src[ch.bead(r) * stride] : 0.0f;
-    }
-}
-
+// what a chunk's step needs in LDS, the last two for outputs and backward
 template <typename T, int DK>
 struct ScanTiles {
   static constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid;
-  Tile<NI, DK> k, q;
-  Tile<NM, kDeltaRows> t, p;
+  Image<NI, DK / 8> k;
+  Image<NM, kDeltaLower> t;
   float fac[4][kDeltaRows];  // the first four
-  float decay;               // e^G_C
+  Image<NI, DK / 8> q;
+  Image<NM, kDeltaLower> p;
+  static constexpr size_t bytes(bool out) {
+    return out ? sizeof(ScanTiles)
+               : (NI * (DK / 8) + NM * kDeltaLower) * 1024 + 4 * kDeltaRows * sizeof(float);
+  }
+  template <int WAVES, bool OUT>
+  __device__ __forceinline__ void send(const DeltaArgs& a, int tile, int h) {
+    const int64_t at = (int64_t)tile * a.heads + h;
+    const int64_t kat = ((int64_t)tile * a.keys + h / a.group) * (k.units * 64);
+    send_to_lds<Image<NI, DK / 8>::units, WAVES>(k.x, a.K + kat);
+    send_to_lds<Image<NM, kDeltaLower>::units, WAVES>(t.x, a.T + at * (t.units * 64));
+    send_to_lds<1, WAVES>(reinterpret_cast<float4*>(fac),
+                          reinterpret_cast<const float4*>(
+                              a.fac + at * (kDeltaFactors * kDeltaRows)));
+    if (OUT) {
+      send_to_lds<Image<NI, DK / 8>::units, WAVES>(q.x, a.Q + kat);
+      send_to_lds<Image<NM, kDeltaLower>::units, WAVES>(p.x, a.P + at * (p.units * 64));
+    }
+  }
 };
 
-// a chunk's tiles on their way to LDS
-template <typename T, int DK>
-struct ScanStage {
-  StageRows<T, DK, Pieces<T>::in> k, q;
-  StageMatrix<Pieces<T>::mid> t, p;
-  float fac, hi, lo;
+// The parts of G_C of a chunk, on their way.
+struct ChunkEnd {
+  float hi, lo;
   __device__ __forceinline__ void load(const DeltaArgs& a, int tile, int h) {
-    const Chunk ch(a, tile);
-    const int64_t at = (int64_t)tile * a.heads + h;
-    k.load(a, ch, (const T*)a.k + h / a.group * a.k_head, a.k_row, true);
-    q.load(a, ch, (const T*)a.q + h / a.group * a.q_head, a.q_row, false);
-    t.load(a.T + at * (Pieces<T>::mid * kDeltaPlane));
-    p.load(a.P + at * (Pieces<T>::mid * kDeltaPlane));
-    const float* f = a.fac + at * (kDeltaFactors * kDeltaRows);
-    fac = f[threadIdx.x];
-    hi = f[kFacHi * kDeltaRows + 63];
-    lo = f[kFacLo * kDeltaRows + 63];
-  }
-  __device__ __forceinline__ void put(ScanTiles<T, DK>& s) const {
-    k.put(s.k);
-    q.put(s.q);
-    t.put(s.t);
-    p.put(s.p);
-    s.fac[threadIdx.x / kDeltaRows][threadIdx.x % kDeltaRows] = fac;
-    if (threadIdx.x == 0) s.decay = exp2_of(hi, lo);
+    const float* const f =
+        a.fac + ((int64_t)tile * a.heads + h) * (kDeltaFactors * kDeltaRows) + kDeltaRows - 1;
+    hi = f[kFacHi * kDeltaRows];
+    lo = f[kFacLo * kDeltaRows];
   }
 };
+
+// 16 x 4 rows of a lane's column of v or do on their way: rows 16 b + 4 g + i
+template <typename T>
+struct Columns {
+  T x[16];
+  // src: the first column; col: the lane's, one that is there
+  __device__ __forceinline__ void load(const Chunk& ch, const T* src, int stride, int col) {
+    const int g = mlcg_lane() >> 4;
+    if (ch.n == kDeltaRows) {
+      const Lines l(const_cast<T*>(src), ch.base, ch.step, stride * (int)sizeof(T), 4 * g, 12,
+                    col * (int)sizeof(T));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = l.row<const T>(16 * (r / 4) + r % 4);
+    } else {
+      const T* const p = src + ch.base * stride + col;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = p[ch.offset(16 * (r / 4) + 4 * g + r % 4, stride)];
+    }
+  }
+  // the four rows of block b
+  __device__ __forceinline__ f32x4 rows(int b) const {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)x[4 * b + i];
+    return v;
+  }
+};
+
+// the same rows of a column to a chunk's 64 rows of ld floats
+__device__ __forceinline__ void store_column(float* at, int ld, const f32x4 (&x)[4]) {
+  const Lines l(at, 0, 1, 4 * ld, 4 * (mlcg_lane() >> 4), 12, 4 * (mlcg_lane() & 15));
+#pragma unroll
+  for (int r = 0; r < 16; ++r) l.row<float>(16 * (r / 4) + r % 4) = x[r / 4][r % 4];
+}
 
 // a state's 16 columns from `at` on: rows 16 b + 4 g + i, column c of them
-template <int DK>
-__device__ __forceinline__ void load_state(f32x4 (&s)[DK / 16], const float* at, int ld, int rows,
+template <int B>
+__device__ __forceinline__ void load_state(f32x4 (&s)[B], const float* at, int ld, int rows,
                                            bool in) {
   const int g = mlcg_lane() >> 4, c = mlcg_lane() & 15;
 #pragma unroll
-  for (int b = 0; b < DK / 16; ++b)
+  for (int b = 0; b < B; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * b + 4 * g + i;
-      s[b][i] = in && r < rows ? at[(int64_t)r * ld + c] : 0.0f;
+      s[b][i] = in && r < rows ? at[r * ld + c] : 0.0f;
     }
 }
-template <int DK>
-__device__ __forceinline__ void store_state(const f32x4 (&s)[DK / 16], float* at, int ld, int rows,
+template <int B>
+__device__ __forceinline__ void store_state(const f32x4 (&s)[B], float* at, int ld, int rows,
                                             bool in) {
   const int g = mlcg_lane() >> 4, c = mlcg_lane() & 15;
+  if (!in) return;
 #pragma unroll
-  for (int b = 0; b < DK / 16; ++b)
+  for (int b = 0; b < B; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * b + 4 * g + i;
-      if (in && r < rows) at[(int64_t)r * ld + c] = s[b][i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (16 * b + 4 * g + i < rows) at[(16 * b + 4 * g + i) * ld + c] = s[b][i];
+}
+// ... all rows of a padded one
+template <int B>
+__device__ __forceinline__ void store_padded(const f32x4 (&s)[B], float* at, int ld) {
+  const Lines l(at, 0, 1, 4 * ld, 4 * (mlcg_lane() >> 4), 12, 4 * (mlcg_lane() & 15));
+#pragma unroll
+  for (int b = 0; b < B; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l.row<float>(16 * b + i) = s[b][i];
 }
 
-// Alone: what a segment makes of the state zero (columns of v) and, in the
-// workgroups past those, of every unit vector; no outputs.
-template <typename T, int DK, bool ALONE>
-__global__ __launch_bounds__(kDeltaThreads) void delta_scan(DeltaArgs a, DeltaEnds e, T* out) {
+// The products of a chunk with a wave's columns: the left operands of several
+// matrix instructions are sent for before the first of them.  y[b]: rows 16 b ..
+// of the image times s, or, FLIP, the transpose of that.
+template <bool FLIP, int N, int NB, int M, int KS>
+__device__ __forceinline__ void rows_product(f32x4 (&y)[4], const Image<N, NB>& t,
+                                             const Frag<M> (&s)[KS]) {
+  constexpr int G = KS * N <= 4 ? 4 : KS * N <= 8 ? 2 : 1;
+#pragma unroll
+  for (int b = 0; b < 4; b += G) {
+    Frag<N> f[G][KS];
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int i = 0; i < KS; ++i) f[j][i] = t.rows((b + j) * KS + i);
+#pragma unroll
+    for (int j = 0; j < G; ++j) y[b + j] = f32x4{};
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        if (FLIP)
+          mma(y[b + j], s[i], f[j][i]);
+        else
+          mma(y[b + j], f[j][i], s[i]);
+      }
+  }
+}
+// s += (columns of the image) x, the image of 32 R rows
+template <int B, int N, int NB, int M, int R>
+__device__ __forceinline__ void columns_product(f32x4 (&s)[B], const Image<N, NB>& t,
+                                                const Frag<M> (&x)[R]) {
+  constexpr int KS = B / 2;
+#pragma unroll
+  for (int b = 0; b < B; b += 2) {
+    Frag<N> f[2][R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      f[0][i] = t.template columns<0>(2 * i * KS + b / 2, (2 * i + 1) * KS + b / 2);
+      f[1][i] = t.template columns<1>(2 * i * KS + b / 2, (2 * i + 1) * KS + b / 2);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mma(s[b + j], f[j][i], x[i]);
+  }
+}
+// The blocks (b, i) of a lower triangle are 0 0, 1 0, 2 0, 2 1, 3 0, 3 1.
+__device__ __forceinline__ constexpr int lower(int b, int i) { return b + (b == 3) + i; }
+// y += (lower triangle) x, or, FLIP, the transpose of that
+template <bool FLIP, int N, int M>
+__device__ __forceinline__ void lower_product(f32x4 (&y)[4], const Image<N, kDeltaLower>& t,
+                                              const Frag<M> (&x)[2]) {
+  Frag<N> f[kDeltaLower];
+#pragma unroll
+  for (int u = 0; u < kDeltaLower; ++u) f[u] = t.rows(u);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int b = 2 * i; b < 4; ++b) {
+      if (FLIP)
+        mma(y[b], x[i], f[lower(b, i)]);
+      else
+        mma(y[b], f[lower(b, i)], x[i]);
+    }
+}
+// y += (lower triangle)^T x
+template <int N, int M>
+__device__ __forceinline__ void upper_product(f32x4 (&y)[4], const Image<N, kDeltaLower>& t,
+                                              const Frag<M> (&x)[2]) {
+  Frag<N> f[4][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int b = 0; b < 2 * i + 2; b += 2) {
+      f[b][i] = t.template columns<0>(lower(2 * i, b / 2), lower(2 * i + 1, b / 2));
+      f[b + 1][i] = t.template columns<1>(lower(2 * i, b / 2), lower(2 * i + 1, b / 2));
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int b = 0; b < 2 * i + 2; ++b) mma(y[b], f[b][i], x[i]);
+}
+// the 16 B rows of a wave's columns as right operands
+template <int N, int B>
+__device__ __forceinline__ void split_rows(Frag<N> (&x)[B / 2], const f32x4 (&y)[B]) {
+#pragma unroll
+  for (int i = 0; i < B / 2; ++i) x[i] = split44<N>(y[2 * i], y[2 * i + 1]);
+}
+// a factor of the rows 16 b + 4 g ..
+__device__ __forceinline__ f32x4 row_factor(const float* f, int b) {
+  return *reinterpret_cast<const f32x4*>(f + 16 * b + 4 * (mlcg_lane() >> 4));
+}
+
+// Alone: what a segment makes of the state zero (columns of v) and, in the second
+// workgroup, of every unit vector; no outputs.  Of two buffers the next chunk is
+// sent to one while the other is worked on; with one the next workgroup on the
+// compute unit works meanwhile.
+template <typename T, int DK, int WAVES, bool ALONE>
+__global__ __launch_bounds__(64 * WAVES) void delta_scan(DeltaArgs a, DeltaEnds e, T* out,
+                                                         int buffers) {
   constexpr int NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
-  ScanTiles<T, DK>& sh = *reinterpret_cast<ScanTiles<T, DK>*>(smem);
-  const int4 seg = a.segs[blockIdx.x];
+  typedef ScanTiles<T, DK> Tiles;
+  const int4 seg = uniform(a.segs[blockIdx.x]);
   const int h = blockIdx.y, w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
-  const int nz = (a.dv + 63) / 64;
-  const bool unit = ALONE && (int)blockIdx.z >= nz;
-  const int v0 = 64 * (unit ? blockIdx.z - nz : blockIdx.z) + 16 * w;
-  const bool live = v0 < (unit ? DK : a.dvp);   // wave-uniform
-  const bool in = !unit && v0 + c < a.dv;
-  const T* const v = (const T*)a.v + h * a.v_head + (in ? v0 + c : 0);
+  const bool unit = ALONE && blockIdx.z == 1;
+  const int v0 = 16 * w, col = min(v0 + c, a.dv - 1);
+  const bool live = v0 < (unit ? DK : a.dvp);  // wave-uniform
+  const T* const v = (const T*)a.v + h * a.v_head;
   f32x4 S[B];
   if (ALONE) {
 #pragma unroll
@@ -583,251 +792,282 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_scan(DeltaArgs a, DeltaEn
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[b][i] = unit && 16 * b + 4 * g + i == v0 + c ? 1.0f : 0.0f;
   } else if (e.seg_init) {
-    load_state<DK>(S, e.seg_init + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0, a.dvp,
-                   DK, live);
+    load_state<B>(S, e.seg_init + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0, a.dvp,
+                  DK, live);
   } else {
-    load_state<DK>(S, e.init + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
-                   a.dk, e.init && in);
+    load_state<B>(S, e.init + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
+                  a.dk, e.init && v0 + c < a.dv);
   }
-  ScanStage<T, DK> next;
-  f32x4 vn[4];
-  next.load(a, seg.y, h);
-  load_column<T>(vn, Chunk(a, seg.y), v, a.v_row, in);
+  const Walk walk(a, seg.y);
+  Columns<T> vn;
+  const auto tiles = [&](int n) {
+    return reinterpret_cast<Tiles*>(smem + (n % buffers) * Tiles::bytes(!ALONE));
+  };
+  ChunkEnd end;
+  end.load(a, seg.y, h);
+  if (buffers == 2) tiles(0)->template send<WAVES, !ALONE>(a, seg.y, h);
+  if (!unit) vn.load(walk.chunk(a, 0), v, (int)a.v_row, col);
   for (int n = 0; n < seg.z; ++n) {
     const int tile = seg.y + n;
-    next.put(sh);
-    f32x4 X[4], O[4];
+    Tiles& sh = *tiles(n);
+    if (buffers == 1) {
+      if (n > 0) lds_barrier();
+      sh.template send<WAVES, !ALONE>(a, tile, h);
+    }
+    wait_for_memory();
+    lds_barrier();
+    f32x4 X[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) X[b] = vn[b];
-    __syncthreads();
+    for (int b = 0; b < 4; ++b) X[b] = unit ? f32x4{} : vn.rows(b);
+    const float decay = exp2_of(end.hi, end.lo);
     if (n + 1 < seg.z) {
-      next.load(a, tile + 1, h);
-      load_column<T>(vn, Chunk(a, tile + 1), v, a.v_row, in);
+      end.load(a, tile + 1, h);
+      if (buffers == 2) tiles(n + 1)->template send<WAVES, !ALONE>(a, tile + 1, h);
+      if (!unit) vn.load(walk.chunk(a, kDeltaRows * (n + 1)), v, (int)a.v_row, col);
     }
-    if (live) {
-      const int64_t at = (int64_t)tile * a.heads + h;
-      if (!ALONE && a.S0) store_state<DK>(S, a.S0 + at * (DK * a.dvp) + v0, a.dvp, DK, true);
-      const Chunk ch(a, tile);
-      Frag<NM> s[KS];
+    if (!live) continue;
+    const int64_t at = (int64_t)tile * a.heads + h;
+    if (!ALONE && a.S0) store_padded<B>(S, a.S0 + at * (DK * a.dvp) + v0, a.dvp);
+    Frag<NM> s[KS], x[2];
+    split_rows<NM>(s, S);
+    f32x4 Y[4];
+    rows_product<false>(Y, sh.k, s);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s[i] = split44<NM>(S[2 * i], S[2 * i + 1]);
-      Frag<NM> x[2];
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 read = row_factor(sh.fac[kFacRead], b), beta = row_factor(sh.fac[kFacBeta], b);
+      X[b] = beta * (X[b] - read * Y[b]);
+      if (a.keep)  // v of an absent bead may be no number
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        f32x4 y{};
-        O[b] = f32x4{};
+        for (int i = 0; i < 4; ++i) X[b][i] = beta[i] == 0.0f ? 0.0f : X[b][i];
+    }
+    if (a.dv != a.dvp && !unit && v0 + c >= a.dv)  // columns that are none stay zeros
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          mma(y, sh.k.rows(16 * b + c, i), s[i]);
-          if (!ALONE) mma(O[b], sh.q.rows(16 * b + c, i), s[i]);
-        }
-        const f32x4 read = *reinterpret_cast<const f32x4*>(&sh.fac[kFacRead][16 * b + 4 * g]);
-        const f32x4 beta = *reinterpret_cast<const f32x4*>(&sh.fac[kFacBeta][16 * b + 4 * g]);
+      for (int b = 0; b < 4; ++b) X[b] = f32x4{};
+    split_rows<NM>(x, X);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)  // an absent bead's v may be no number
-          X[b][i] = beta[i] == 0.0f ? 0.0f : beta[i] * fmaf(-read[i], y[i], X[b][i]);
-      }
-      x[0] = split44<NM>(X[0], X[1]);
-      x[1] = split44<NM>(X[2], X[3]);
+    for (int b = 0; b < 4; ++b) X[b] = f32x4{};
+    lower_product<false>(X, sh.t, x);
+    if (!ALONE) {
+      split_rows<NM>(x, X);
+      // o^T: four columns of one bead in a lane
+      f32x4 O[4];
+      rows_product<true>(O, sh.q, s);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        X[b] = f32x4{};
+      for (int b = 0; b < 4; ++b) O[b] *= sh.fac[kFacOut][16 * b + c];
+      lower_product<true>(O, sh.p, x);
+      const Chunk ch = walk.chunk(a, kDeltaRows * n);
+      typedef typename loose<T, 4>::type vec;
+      const int el = v0 + 4 * g;
+      if (el < a.dv) {
+        if (ch.n == kDeltaRows) {
+          const Lines l(out, ch.base, ch.step, a.heads * a.dv * (int)sizeof(T), c, 15,
+                        (h * a.dv + el) * (int)sizeof(T));
 #pragma unroll
-        for (int i = 0; i <= b / 2; ++i) mma(X[b], sh.t.rows(16 * b + c, i), x[i]);
-      }
-      if (!ALONE) {
-        x[0] = split44<NM>(X[0], X[1]);
-        x[1] = split44<NM>(X[2], X[3]);
+          for (int b = 0; b < 4; ++b) l.row<vec>(16 * b) = __builtin_convertvector(O[b], vec);
+        } else {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          O[b] *= *reinterpret_cast<const f32x4*>(&sh.fac[kFacOut][16 * b + 4 * g]);
-#pragma unroll
-          for (int i = 0; i <= b / 2; ++i) mma(O[b], sh.p.rows(16 * b + c, i), x[i]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 16 * b + 4 * g + i;
-            if (r >= ch.n) continue;
-            const int64_t bead = ch.bead(r);
-            if (a.U) a.U[(h * a.beads + bead) * a.dvp + v0 + c] = X[b][i];
-            if (in) out[(bead * a.heads + h) * a.dv + v0 + c] = (T)O[b][i];
-          }
+          for (int b = 0; b < 4; ++b)
+            if (16 * b + c < ch.n)
+              store4<T>(out + (ch.bead(16 * b + c) * a.heads + h) * a.dv, el, a.dv, O[b]);
         }
       }
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        X[b] *= *reinterpret_cast<const f32x4*>(&sh.fac[kFacWrite][16 * b + 4 * g]);
-      x[0] = split44<NM>(X[0], X[1]);
-      x[1] = split44<NM>(X[2], X[3]);
-      const float decay = sh.decay;
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        S[b] *= decay;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) mma(S[b], sh.k.columns(b, i), x[i]);
-      }
+      if (a.U) store_column(a.U + at * (kDeltaRows * a.dvp) + v0, a.dvp, X);
     }
-    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; ++b) X[b] *= row_factor(sh.fac[kFacWrite], b);
+    split_rows<NM>(x, X);
+#pragma unroll
+    for (int b = 0; b < B; ++b) S[b] *= decay;
+    columns_product(S, sh.k, x);
   }
   if (!live) return;
-  if (ALONE) {
-    const int64_t at = (int64_t)blockIdx.x * a.heads + h;
-    if (unit)
-      store_state<DK>(S, e.seg_map + at * (DK * DK) + v0, DK, DK, true);
-    else
-      store_state<DK>(S, e.seg_last + at * (DK * a.dvp) + v0, a.dvp, DK, true);
+  const int64_t at = (int64_t)blockIdx.x * a.heads + h;
+  if (unit) {  // the map's transpose, as a left operand
+    Frag<NM> s[KS];
+    split_rows<NM>(s, S);
+    typedef Image<NM, B * KS> Map;
+    float4* const m = e.seg_map + at * (Map::units * 64);
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int j = 0; j < NM; ++j)
+        m[(j * (B * KS) + w * KS + i) * 64 + Map::slot()] = __builtin_bit_cast(float4, s[i].p[j]);
+  } else if (ALONE) {
+    store_padded<B>(S, e.seg_last + at * (DK * a.dvp) + v0, a.dvp);
   } else if (e.last && (seg.w & 2)) {
-    store_state<DK>(S, e.last + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
-                    a.dk, in);
+    store_state<B>(S, e.last + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
+                   a.dk, v0 + c < a.dv);
   }
 }
 
 // The states before the segments of a chain, one after the other: S <- M S + N.
 // Backward: after them, the last one first, S <- M^T S + N.
-template <int DK, bool BACK>
-__global__ __launch_bounds__(kDeltaThreads) void delta_join(DeltaArgs a, DeltaEnds e,
-                                                            float* seg_init) {
-  constexpr int B = DK / 16;
-  const int h = blockIdx.y, w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
-  const int v0 = 64 * blockIdx.z + 16 * w;
-  if (v0 >= a.dvp) return;
-  const int first = a.seg_first[blockIdx.x], n = a.seg_first[blockIdx.x + 1] - first;
-  const int chain = a.segs[first].x;
-  f32x4 S[B];
-  load_state<DK>(S, e.init + ((int64_t)chain * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
-                 a.dk, e.init && v0 + c < a.dv);
+template <typename T, int DK, int WAVES, bool BACK>
+__global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds e,
+                                                         float* seg_init, int buffers) {
+  constexpr int NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
+  typedef Image<NM, B * KS> Map;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Map* const maps = reinterpret_cast<Map*>(smem);  // one, or two in turn
+  const int h = blockIdx.y, c = mlcg_lane() & 15, v0 = 16 * wave_number();
+  const bool live = v0 < a.dvp;
+  const int first = uniform(a.seg_first[blockIdx.x]);
+  const int n = uniform(a.seg_first[blockIdx.x + 1]) - first;
+  const int chain = uniform(a.segs[first]).x;
+  f32x4 S[B], next[B];
+  load_state<B>(S, e.init + ((int64_t)chain * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
+                a.dk, e.init && v0 + c < a.dv);
+  const auto fetch = [&](int j) {
+    const int64_t at = (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
+    send_to_lds<Map::units, WAVES>(maps[j % buffers].x, e.seg_map + at * (Map::units * 64));
+    load_state<B>(next, e.seg_last + at * (DK * a.dvp) + v0, a.dvp, DK, live);
+  };
+  if (n > 1) fetch(0);
   for (int j = 0; j < n; ++j) {
-    const int seg = first + (BACK ? n - 1 - j : j);
-    const int64_t at = (int64_t)seg * a.heads + h;
-    store_state<DK>(S, seg_init + at * (DK * a.dvp) + v0, a.dvp, DK, true);
+    const int64_t at = (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
+    wait_for_memory();
+    lds_barrier();
+    Frag<NM> s[KS];
+    split_rows<NM>(s, S);
+    if (live) store_padded<B>(S, seg_init + at * (DK * a.dvp) + v0, a.dvp);
     if (j + 1 == n) break;
-    f32x4 next[B];
-    load_state<DK>(next, e.seg_last + at * (DK * a.dvp) + v0, a.dvp, DK, true);
-    const float* const M = e.seg_map + at * (DK * DK);
-#pragma unroll
-    for (int b = 0; b < B; ++b)
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        f32x4 l;
-        if (BACK) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) l[x] = M[(16 * i + 4 * g + x) * DK + 16 * b + c];
-        } else {
-          l = *reinterpret_cast<const f32x4*>(M + (16 * b + c) * DK + 16 * i + 4 * g);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          next[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[x], S[i][x], next[b], 0, 0, 0);
-      }
 #pragma unroll
     for (int b = 0; b < B; ++b) S[b] = next[b];
+    if (buffers == 2 && j + 2 < n) fetch(j + 1);
+    if (BACK) {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < KS; ++i) mma(S[b], maps[j % buffers].rows(b * KS + i), s[i]);
+    } else {
+      columns_product(S, maps[j % buffers], s);
+    }
+    if (buffers == 1 && j + 2 < n) {
+      lds_barrier();
+      fetch(j + 1);
+    }
   }
 }
 
 // The state's gradient along the chunks of a segment, the last one first.
-template <typename T, int DK, bool ALONE>
-__global__ __launch_bounds__(kDeltaThreads) void delta_scan_back(DeltaArgs a, DeltaBack o,
-                                                                 DeltaEnds e) {
+template <typename T, int DK, int WAVES, bool ALONE>
+__global__ __launch_bounds__(64 * WAVES) void delta_scan_back(DeltaArgs a, DeltaBack o,
+                                                              DeltaEnds e, int buffers) {
   constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
-  ScanTiles<T, DK>& sh = *reinterpret_cast<ScanTiles<T, DK>*>(smem);
-  const int4 seg = a.segs[blockIdx.x];
+  typedef ScanTiles<T, DK> Tiles;
+  const int4 seg = uniform(a.segs[blockIdx.x]);
   const int h = blockIdx.y, w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
-  const int v0 = 64 * blockIdx.z + 16 * w;
-  const bool live = v0 < a.dvp, in = v0 + c < a.dv;
-  const T* const grad = (const T*)o.grad + h * a.dv + (in ? v0 + c : 0);
-  const int64_t grad_row = (int64_t)a.heads * a.dv;
+  const int v0 = 16 * w, col = min(v0 + c, a.dv - 1);
+  const bool live = v0 < a.dvp;
+  const T* const grad = (const T*)o.grad + h * a.dv;
+  const int row = a.heads * a.dv;  // of do and dv
   f32x4 D[B];
   if (ALONE) {
 #pragma unroll
     for (int b = 0; b < B; ++b) D[b] = f32x4{};
   } else if (e.seg_init) {
-    load_state<DK>(D, e.seg_init + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0, a.dvp,
-                   DK, live);
+    load_state<B>(D, e.seg_init + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0, a.dvp,
+                  DK, live);
   } else {
-    load_state<DK>(D, e.init + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
-                   a.dk, e.init && in);
+    load_state<B>(D, e.init + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
+                  a.dk, e.init && v0 + c < a.dv);
   }
-  ScanStage<T, DK> next;
-  f32x4 gn[4];
-  next.load(a, seg.y + seg.z - 1, h);
-  load_column<T>(gn, Chunk(a, seg.y + seg.z - 1), grad, grad_row, in);
-  for (int n = seg.z - 1; n >= 0; --n) {
+  const Walk walk(a, seg.y);
+  Columns<T> gn;
+  const auto tiles = [&](int n) {
+    return reinterpret_cast<Tiles*>(smem + (n % buffers) * Tiles::bytes(true));
+  };
+  const int top = seg.z - 1;
+  ChunkEnd end;
+  end.load(a, seg.y + top, h);
+  if (buffers == 2) tiles(top)->template send<WAVES, true>(a, seg.y + top, h);
+  gn.load(walk.chunk(a, kDeltaRows * top), grad, row, col);
+  for (int n = top; n >= 0; --n) {
     const int tile = seg.y + n;
-    next.put(sh);
+    Tiles& sh = *tiles(n);
+    if (buffers == 1) {
+      if (n < top) lds_barrier();
+      sh.template send<WAVES, true>(a, tile, h);
+    }
+    wait_for_memory();
+    lds_barrier();
+    const Chunk ch = walk.chunk(a, kDeltaRows * n);
     f32x4 G[4], X[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) G[b] = gn[b];
-    __syncthreads();
+    for (int b = 0; b < 4; ++b) G[b] = gn.rows(b);
+    if (ch.n < kDeltaRows)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (16 * (r / 4) + 4 * g + r % 4 >= ch.n) G[r / 4][r % 4] = 0.0f;
+    if (a.dv != a.dvp && v0 + c >= a.dv)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) G[b] = f32x4{};
+    const float decay = exp2_of(end.hi, end.lo);
     if (n > 0) {
-      next.load(a, tile - 1, h);
-      load_column<T>(gn, Chunk(a, tile - 1), grad, grad_row, in);
+      end.load(a, tile - 1, h);
+      if (buffers == 2) tiles(n - 1)->template send<WAVES, true>(a, tile - 1, h);
+      gn.load(walk.chunk(a, kDeltaRows * (n - 1)), grad, row, col);
     }
-    if (live) {
-      const int64_t at = (int64_t)tile * a.heads + h;
-      if (!ALONE) store_state<DK>(D, o.D + at * (DK * a.dvp) + v0, a.dvp, DK, true);
-      const Chunk ch(a, tile);
+    if (!live) continue;
+    const int64_t at = (int64_t)tile * a.heads + h;
+    if (!ALONE) store_padded<B>(D, o.D + at * (DK * a.dvp) + v0, a.dvp);
+    Frag<NM> x[2];
+    {
       Frag<NM> d[KS];
+      split_rows<NM>(d, D);
+      rows_product<false>(X, sh.k, d);
+    }
+    // du
 #pragma unroll
-      for (int i = 0; i < KS; ++i) d[i] = split44<NM>(D[2 * i], D[2 * i + 1]);
-      const Frag<NI> go[2] = {split44<NI>(G[0], G[1]), split44<NI>(G[2], G[3])};
-      Frag<NM> x[2];
-      // du
+    for (int b = 0; b < 4; ++b) X[b] *= row_factor(sh.fac[kFacWrite], b);
+    {
+      Frag<NI> go[2];
+      split_rows<NI>(go, G);
+      upper_product(X, sh.p, go);
+    }
+    split_rows<NM>(x, X);
+    // dr
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        X[b] = f32x4{};
+    for (int b = 0; b < 4; ++b) X[b] = f32x4{};
+    upper_product(X, sh.t, x);
+    if (!ALONE) store_column(o.dR + at * (kDeltaRows * a.dvp) + v0, a.dvp, X);
 #pragma unroll
-        for (int i = 0; i < KS; ++i) mma(X[b], sh.k.rows(16 * b + c, i), d[i]);
-        X[b] *= *reinterpret_cast<const f32x4*>(&sh.fac[kFacWrite][16 * b + 4 * g]);
+    for (int b = 0; b < 4; ++b) X[b] *= row_factor(sh.fac[kFacBeta], b);
+    if (!ALONE && v0 + c < a.dv) {
+      if (ch.n == kDeltaRows) {
+        const Lines l(o.dv, ch.base, ch.step, row * (int)sizeof(T), 4 * g, 12,
+                      (h * a.dv + v0 + c) * (int)sizeof(T));
 #pragma unroll
-        for (int i = b / 2; i < 2; ++i) mma(X[b], sh.p.columns(b, i), go[i]);
-      }
-      x[0] = split44<NM>(X[0], X[1]);
-      x[1] = split44<NM>(X[2], X[3]);
-      // dr
+        for (int r = 0; r < 16; ++r) l.row<T>(16 * (r / 4) + r % 4) = (T)X[r / 4][r % 4];
+      } else {
+        T* const dv = (T*)o.dv + h * a.dv + v0 + c;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        X[b] = f32x4{};
-#pragma unroll
-        for (int i = b / 2; i < 2; ++i) mma(X[b], sh.t.columns(b, i), x[i]);
-        const f32x4 beta = *reinterpret_cast<const f32x4*>(&sh.fac[kFacBeta][16 * b + 4 * g]);
-        const f32x4 read = *reinterpret_cast<const f32x4*>(&sh.fac[kFacRead][16 * b + 4 * g]);
-        if (!ALONE) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 16 * b + 4 * g + i;
-            if (r >= ch.n) continue;
-            const int64_t bead = ch.bead(r);
-            o.dR[(h * a.beads + bead) * a.dvp + v0 + c] = X[b][i];
-            if (in) ((T*)o.dv)[(bead * a.heads + h) * a.dv + v0 + c] = (T)(beta[i] * X[b][i]);
-          }
-        }
-        X[b] *= -(beta * read);
-        G[b] *= *reinterpret_cast<const f32x4*>(&sh.fac[kFacOut][16 * b + 4 * g]);
-      }
-      x[0] = split44<NM>(X[0], X[1]);
-      x[1] = split44<NM>(X[2], X[3]);
-      const Frag<NM> gs[2] = {split44<NM>(G[0], G[1]), split44<NM>(G[2], G[3])};
-      const float decay = sh.decay;
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        D[b] *= decay;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma(D[b], sh.q.columns(b, i), gs[i]);
-          mma(D[b], sh.k.columns(b, i), x[i]);
+        for (int r = 0; r < 16; ++r) {
+          const int t = 16 * (r / 4) + 4 * g + r % 4;
+          if (t < ch.n) dv[ch.bead(t) * row] = (T)X[r / 4][r % 4];
         }
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      X[b] *= -row_factor(sh.fac[kFacRead], b);
+      G[b] *= row_factor(sh.fac[kFacOut], b);
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) D[b] *= decay;
+    split_rows<NM>(x, X);
+    columns_product(D, sh.k, x);
+    split_rows<NM>(x, G);
+    columns_product(D, sh.q, x);
   }
   if (!live) return;
-  if (ALONE) {
-    store_state<DK>(D, e.seg_last + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0, a.dvp,
-                    DK, true);
-  } else if (o.dstate && (seg.w & 1)) {
-    store_state<DK>(D, o.dstate + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0,
-                    a.dv, a.dk, in);
-  }
+  if (ALONE)
+    store_padded<B>(D, e.seg_last + ((int64_t)blockIdx.x * a.heads + h) * (DK * a.dvp) + v0,
+                    a.dvp);
+  else if (o.dstate && (seg.w & 1))
+    store_state<B>(D, o.dstate + ((int64_t)seg.x * a.heads + h) * ((int64_t)a.dk * a.dv) + v0,
+                   a.dv, a.dk, v0 + c < a.dv);
 }
 
 // ---------------------------------------------------------------------------
@@ -836,53 +1076,35 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_scan_back(DeltaArgs a, De
 
 template <typename T, int DK>
 struct GradTiles {
-  Tile<Pieces<T>::in, DK> k, q;
+  Image<Pieces<T>::in, DK / 8> k, q;
   float fac[kDeltaFactors][kDeltaRows];
   float dG[kDeltaRows];
   float ends[4];
 };
 
 // 8 floats of a padded row from el on, zeros past its end
-__device__ __forceinline__ f32x8 load_f8(const float* row, int el, int len, bool in) {
-  f32x8 x{};
-  if (in && el < len) x = *reinterpret_cast<const f32x8*>(row + el);
-  return x;
-}
-
-// 4 elements of a row from el on, as floats
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int el, int len, bool vec) {
-  f32x4 x{};
-  if (vec) {
-    if (el < len) x = __builtin_convertvector(*reinterpret_cast<const v4<T>*>(row + el), f32x4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (el + j < len) x[j] = (float)row[el + j];
-  }
-  return x;
+__device__ __forceinline__ f32x8 load_f8(const float* row, int el, int len) {
+  const f32x8 x = *reinterpret_cast<const f32x8*>(row + min(el, len - 8));
+  return el < len ? x : f32x8{};
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBack o, int gvec) {
-  constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, B = DK / 16;
+__global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBack o) {
+  constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, B = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   GradTiles<T, DK>& sh = *reinterpret_cast<GradTiles<T, DK>*>(smem);
   const int tile = blockIdx.x, kh = blockIdx.y;
   const int w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
   const Chunk ch(a, tile);
-  const T* const q = (const T*)a.q + kh * a.q_head;
-  const T* const k = (const T*)a.k + kh * a.k_head;
   {
-    StageRows<T, DK, NI> s;
-    s.load(a, ch, k, a.k_row, true);
-    s.put(sh.k);
-    s.load(a, ch, q, a.q_row, false);
-    s.put(sh.q);
+    constexpr int units = Image<NI, DK / 8>::units;
+    const int64_t at = ((int64_t)tile * a.keys + kh) * (units * 64);
+    send_to_lds<units, 4>(sh.k.x, a.K + at);
+    send_to_lds<units, 4>(sh.q.x, a.Q + at);
   }
   const int row = 16 * w + c;
   const bool in = row < ch.n;
-  const int64_t bead = in ? ch.bead(row) : 0;
+  const int64_t bead = ch.bead(min(row, ch.n - 1));
   const bool there = in && (!a.keep || a.keep[bead]);
   f32x4 dq[B], dk[B];
 #pragma unroll
@@ -891,12 +1113,14 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
 
   for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
     const int64_t at = (int64_t)tile * a.heads + h;
-    __syncthreads();  // sh.dG of the last head has been read
-    for (int i = threadIdx.x; i < kDeltaFactors * kDeltaRows; i += kDeltaThreads)
-      sh.fac[i / kDeltaRows][i % kDeltaRows] = a.fac[at * (kDeltaFactors * kDeltaRows) + i];
-    __syncthreads();
-    const float* const U = a.U + h * a.beads * a.dvp;
-    const float* const R = o.dR + h * a.beads * a.dvp;
+    if (h > kh * a.group) lds_barrier();  // what the last head left has been read
+    send_to_lds<2, 4>(reinterpret_cast<float4*>(sh.fac),
+                      reinterpret_cast<const float4*>(a.fac +
+                                                      at * (kDeltaFactors * kDeltaRows)));
+    wait_for_memory();
+    lds_barrier();
+    const float* const U = a.U + at * (kDeltaRows * a.dvp);
+    const float* const R = o.dR + at * (kDeltaRows * a.dvp);
     const T* const go = (const T*)o.grad + h * a.dv;
     const int64_t go_row = (int64_t)a.heads * a.dv;
     const float* const S0 = a.S0 + at * (DK * a.dvp);
@@ -912,11 +1136,12 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
     float rv = 0.0f, sd = 0.0f;  // dr.v;  this wave's part of <S0, D>
     for (int v0 = 0; v0 < a.dvp; v0 += 32) {
       const int el = v0 + 8 * g;
-      const f32x8 ur = load_f8(U + bead * a.dvp, el, a.dvp, in);
-      const f32x8 rr = load_f8(R + bead * a.dvp, el, a.dvp, in);
-      v8<T> gr{}, vr{};
-      if (in) gr = load8<T>(go + bead * go_row, el, a.dv, gvec & 1);
-      if (there) vr = load8<T>((const T*)a.v + bead * a.v_row + h * a.v_head, el, a.dv, gvec & 2);
+      const f32x8 ur = load_f8(U + row * a.dvp, el, a.dvp);
+      const f32x8 rr = load_f8(R + row * a.dvp, el, a.dvp);
+      v8<T> gr = load8<T>(go + bead * go_row, el, a.dv);
+      v8<T> vr = load8<T>((const T*)a.v + bead * a.v_row + h * a.v_head, el, a.dv);
+      if (!in) gr = v8<T>{};
+      if (!there) vr = v8<T>{};
 #pragma unroll
       for (int j = 0; j < 8; ++j) rv = fmaf(rr[j], (float)vr[j], rv);
       const Frag<NM> ub = split8<NM>(ur), rb = split8<NM>(rr);
@@ -924,26 +1149,22 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         const int r = 16 * m + c;
-        const bool rin = r < ch.n;
-        const int64_t rb_ = rin ? ch.bead(r) : 0;
         if (m <= w) {
-          const Frag<NM> f = split8<NM>(load_f8(U + rb_ * a.dvp, el, a.dvp, rin));
+          const Frag<NM> f = split8<NM>(load_f8(U + r * a.dvp, el, a.dvp));
           mma(ou0[m], f, gb);
           mma(ru0[m], f, rb);
         }
         if (m >= w) {
-          v8<T> x{};
-          if (rin) x = load8<T>(go + rb_ * go_row, el, a.dv, gvec & 1);
-          const Frag<NI> f = split_raw<NI, T>(x);
-          mma(ou1[m], f, ub);
-          const Frag<NM> f2 = split8<NM>(load_f8(R + rb_ * a.dvp, el, a.dvp, rin));
-          mma(ru1[m], f2, ub);
+          v8<T> x = load8<T>(go + ch.bead(min(r, ch.n - 1)) * go_row, el, a.dv);
+          if (r >= ch.n) x = v8<T>{};
+          mma(ou1[m], split_raw<NI, T>(x), ub);
+          mma(ru1[m], split8<NM>(load_f8(R + r * a.dvp, el, a.dvp)), ub);
         }
       }
 #pragma unroll
       for (int b = 0; b < B; ++b) {
-        const f32x8 s = load_f8(S0 + (16 * b + c) * a.dvp, el, a.dvp, true);
-        const f32x8 d = load_f8(D + (16 * b + c) * a.dvp, el, a.dvp, true);
+        const f32x8 s = load_f8(S0 + (16 * b + c) * a.dvp, el, a.dvp);
+        const f32x8 d = load_f8(D + (16 * b + c) * a.dvp, el, a.dvp);
         if (b % 4 == w)
 #pragma unroll
           for (int j = 0; j < 8; ++j) sd = fmaf(s[j], d[j], sd);
@@ -962,14 +1183,17 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
     rq = sh.fac[kFacQ][row];
     float kd = 0.0f;  // k.(e^(G_C - G) D u)
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      hq[b] *= first;
-      hr[b] *= -first;
-      hw[b] *= rest;
-      f32x4 x{};
-      if (there) x = load4<T>(k + bead * a.k_row, 16 * b + 4 * g, a.dk, a.vec);
+    for (int i = 0; i < KS; ++i) {
+      const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) kd = fmaf(rk * x[i], hw[b][i], kd);
+      for (int j = 0; j < 2; ++j) {
+        const int b = 2 * i + j;
+        hq[b] *= first;
+        hr[b] *= -first;
+        hw[b] *= rest;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) kd = fmaf(x[4 * j + y], hw[b][y], kd);
+      }
     }
     // inside the chunk
 #pragma unroll
@@ -993,26 +1217,38 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
       const Frag<NM> o1 = split44<NM>(ou1[2 * i], ou1[2 * i + 1]);
       const Frag<NM> r1 = split44<NM>(ru1[2 * i], ru1[2 * i + 1]);
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        const Frag<NI> kc = sh.k.columns(b, i), qc = sh.q.columns(b, i);
-        mma(hq[b], kc, o0);
-        mma(hr[b], kc, r0);
-        mma(hw[b], qc, o1);
-        mma(hw[b], kc, r1);
+      for (int b = 0; b < B; b += 2) {
+        const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
+        const Frag<NI> k0 = sh.k.template columns<0>(b0, b1), k1 = sh.k.template columns<1>(b0, b1);
+        const Frag<NI> q0 = sh.q.template columns<0>(b0, b1), q1 = sh.q.template columns<1>(b0, b1);
+        if (i <= w / 2) {  // beads up to this wave's
+          mma(hq[b], k0, o0);
+          mma(hq[b + 1], k1, o0);
+          mma(hr[b], k0, r0);
+          mma(hr[b + 1], k1, r0);
+        }
+        if (i >= w / 2) {
+          mma(hw[b], q0, o1);
+          mma(hw[b + 1], q1, o1);
+          mma(hw[b], k0, r1);
+          mma(hw[b + 1], k1, r1);
+        }
       }
     }
     float qd = 0.0f, kr = 0.0f, kw = 0.0f;
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      f32x4 x{}, y{};
-      if (there) x = load4<T>(k + bead * a.k_row, 16 * b + 4 * g, a.dk, a.vec);
-      if (in) y = load4<T>(q + bead * a.q_row, 16 * b + 4 * g, a.dk, a.vec);
+    for (int i = 0; i < KS; ++i) {
+      const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk, y = whole(sh.q.rows(w * KS + i)) * rq;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        qd = fmaf(rq * y[i], hq[b][i], qd);
-        kr = fmaf(rk * x[i], hr[b][i], kr);
-        kw = fmaf(rk * x[i], hw[b][i], kw);
+      for (int j = 0; j < 8; ++j) {
+        const int b = 2 * i + j / 4;
+        qd = fmaf(y[j], hq[b][j % 4], qd);
+        kr = fmaf(x[j], hr[b][j % 4], kr);
+        kw = fmaf(x[j], hw[b][j % 4], kw);
       }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
       dq[b] += hq[b];
       dk[b] += beta * hr[b] + hw[b];
     }
@@ -1027,7 +1263,7 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
     // <S, D> = e^G_C <S0, D> + sum k.(e^(G_C - G) D u)
     const float end = mlcg_wave_sum(fmaf(exp2_of(ch_hi, ch_lo), sd, kd));
     if (lane == 0) sh.ends[w] = end;
-    __syncthreads();
+    lds_barrier();
     if (w == 0) {
       double s = sh.dG[lane];
       if (lane == 63)
@@ -1047,16 +1283,13 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
   }
   // through the lengths of q and k
   float pq = 0.0f, pk = 0.0f;
-  f32x4 kx[B], qx[B];
 #pragma unroll
-  for (int b = 0; b < B; ++b) {
-    kx[b] = qx[b] = f32x4{};
-    if (there) kx[b] = load4<T>(k + bead * a.k_row, 16 * b + 4 * g, a.dk, a.vec) * rk;
-    if (in) qx[b] = load4<T>(q + bead * a.q_row, 16 * b + 4 * g, a.dk, a.vec) * rq;
+  for (int i = 0; i < KS; ++i) {
+    const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk, y = whole(sh.q.rows(w * KS + i)) * rq;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pq = fmaf(qx[b][i], dq[b][i], pq);
-      pk = fmaf(kx[b][i], dk[b][i], pk);
+    for (int j = 0; j < 8; ++j) {
+      pq = fmaf(y[j], dq[2 * i + j / 4][j % 4], pq);
+      pk = fmaf(x[j], dk[2 * i + j / 4][j % 4], pk);
     }
   }
   pq = quarter_sum(pq);
@@ -1065,23 +1298,15 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
   if (!in) return;
   T* const oq = (T*)o.dq + (bead * a.keys + kh) * a.dk;
   T* const ok = (T*)o.dk + (bead * a.keys + kh) * a.dk;
-  const bool wide = a.dk % 4 == 0;
 #pragma unroll
-  for (int b = 0; b < B; ++b) {
-    const int el = 16 * b + 4 * g;
-    if (el >= a.dk) continue;
-    const f32x4 x = (dq[b] - qx[b] * pq) * (a.scale * rq), y = (dk[b] - kx[b] * pk) * rk;
-    if (wide) {
-      *reinterpret_cast<v4<T>*>(oq + el) = __builtin_convertvector(x, v4<T>);
-      *reinterpret_cast<v4<T>*>(ok + el) = __builtin_convertvector(y, v4<T>);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (el + i < a.dk) {
-          oq[el + i] = (T)x[i];
-          ok[el + i] = (T)y[i];
-        }
-    }
+  for (int i = 0; i < KS; ++i) {
+    const f32x8 x = whole(sh.k.rows(w * KS + i)) * (rk * pk);
+    const f32x8 y = whole(sh.q.rows(w * KS + i)) * (rq * pq);
+    const int el = 32 * i + 4 * g;
+    store4<T>(oq, el, a.dk, (dq[2 * i] - half_of<0>(y)) * (a.scale * rq));
+    store4<T>(oq, el + 16, a.dk, (dq[2 * i + 1] - half_of<1>(y)) * (a.scale * rq));
+    store4<T>(ok, el, a.dk, (dk[2 * i] - half_of<0>(x)) * rk);
+    store4<T>(ok, el + 16, a.dk, (dk[2 * i + 1] - half_of<1>(x)) * rk);
   }
 }
 
@@ -1092,68 +1317,96 @@ inline bool lds_limit(const void* f, size_t bytes) {
          hipSuccess;
 }
 
-template <typename T, int DK>
-int forward_dk(const DeltaArgs& a, T* out, DeltaEnds e, float* ws, hipStream_t s) {
-  const size_t lds = sizeof(ScanTiles<T, DK>);
-  const unsigned nz = mlcg_div_up(a.dv, 64);
-  hipLaunchKernelGGL((delta_chunk<T, DK>), dim3(a.n_tiles, a.keys), dim3(kDeltaThreads), 0, s, a);
+// Two buffers of a chunk in LDS where there is room for them and no more
+// workgroups than compute units: 2 x 4099 beads, 8 heads of 64 in bf16, segments of
+// 6 chunks, 89 us forward against 93; 48 x 268, 8 heads of 16 in fp32, 75 against 61.
+constexpr size_t kDeltaLds = 160 * 1024;
+constexpr int kDeltaUnits = 256;
+inline int scan_buffers(size_t bytes, int64_t groups) {
+  return 2 * bytes <= kDeltaLds && groups <= kDeltaUnits ? 2 : 1;
+}
+
+template <typename T, int DK, int WAVES, bool BACK>
+int join(const DeltaArgs& a, const DeltaEnds& e, float* ws, hipStream_t s) {
+  const auto f = delta_join<T, DK, WAVES, BACK>;
+  const size_t one = sizeof(Image<Pieces<T>::mid, DK * DK / 512>);
+  const int buffers = 2 * one <= kDeltaLds ? 2 : 1;
+  if (!lds_limit(reinterpret_cast<const void*>(f), buffers * one)) return MLCG_ERR_LAUNCH;
+  hipLaunchKernelGGL(f, dim3(a.n_whole, a.heads), dim3(64 * WAVES), buffers * one, s, a, e, ws,
+                     buffers);
+  return MLCG_OK;
+}
+
+template <typename T, int DK, int WAVES>
+int forward_waves(const DeltaArgs& a, T* out, DeltaEnds e, float* ws, hipStream_t s) {
+  const auto chunk = delta_chunk<T, DK>;
+  if (!lds_limit(reinterpret_cast<const void*>(chunk), sizeof(ChunkTiles<T, DK>)))
+    return MLCG_ERR_LAUNCH;
+  hipLaunchKernelGGL(chunk, dim3(a.n_tiles, a.keys), dim3(kDeltaThreads),
+                     sizeof(ChunkTiles<T, DK>), s, a);
+  const int64_t groups = (int64_t)a.n_segs * a.heads;
   if (e.seg_last) {
-    const auto alone = delta_scan<T, DK, true>;
-    if (!lds_limit(reinterpret_cast<const void*>(alone), lds)) return MLCG_ERR_LAUNCH;
-    hipLaunchKernelGGL(alone, dim3(a.n_segs, a.heads, nz + mlcg_div_up(DK, 64)),
-                       dim3(kDeltaThreads), lds, s, a, e, out);
-    hipLaunchKernelGGL((delta_join<DK, false>), dim3(a.n_whole, a.heads, nz), dim3(kDeltaThreads),
-                       0, s, a, e, ws);
+    constexpr int W = 16 * WAVES < DK ? DK / 16 : WAVES;  // all unit vectors
+    const auto alone = delta_scan<T, DK, W, true>;
+    const size_t bytes = ScanTiles<T, DK>::bytes(false);
+    const int buffers = scan_buffers(bytes, 2 * groups);
+    if (!lds_limit(reinterpret_cast<const void*>(alone), buffers * bytes)) return MLCG_ERR_LAUNCH;
+    hipLaunchKernelGGL(alone, dim3(a.n_segs, a.heads, 2), dim3(64 * W), buffers * bytes, s, a, e,
+                       out, buffers);
+    const int status = join<T, DK, WAVES, false>(a, e, ws, s);
+    if (status != MLCG_OK) return status;
     e.seg_init = ws;
   }
-  const auto scan = delta_scan<T, DK, false>;
-  if (!lds_limit(reinterpret_cast<const void*>(scan), lds)) return MLCG_ERR_LAUNCH;
-  hipLaunchKernelGGL(scan, dim3(a.n_segs, a.heads, nz), dim3(kDeltaThreads), lds, s, a, e, out);
+  const auto scan = delta_scan<T, DK, WAVES, false>;
+  const size_t bytes = ScanTiles<T, DK>::bytes(true);
+  const int buffers = scan_buffers(bytes, groups);
+  if (!lds_limit(reinterpret_cast<const void*>(scan), buffers * bytes)) return MLCG_ERR_LAUNCH;
+  hipLaunchKernelGGL(scan, dim3(a.n_segs, a.heads), dim3(64 * WAVES), buffers * bytes, s, a, e, out,
+                     buffers);
   return mlcg_launch_status();
 }
 
-template <typename T, int DK>
-int backward_dk(const DeltaArgs& a, const DeltaBack& o, DeltaEnds e, float* ws, hipStream_t s) {
-  const size_t lds = sizeof(ScanTiles<T, DK>);
-  const unsigned nz = mlcg_div_up(a.dv, 64);
-  const dim3 grid(a.n_segs, a.heads, nz);
+template <typename T, int DK, int WAVES>
+int backward_waves(const DeltaArgs& a, const DeltaBack& o, DeltaEnds e, float* ws, hipStream_t s) {
+  const size_t bytes = ScanTiles<T, DK>::bytes(true);
+  const int buffers = scan_buffers(bytes, (int64_t)a.n_segs * a.heads);
+  const dim3 grid(a.n_segs, a.heads), block(64 * WAVES);
   if (e.seg_last) {
-    const auto alone = delta_scan_back<T, DK, true>;
-    if (!lds_limit(reinterpret_cast<const void*>(alone), lds)) return MLCG_ERR_LAUNCH;
-    hipLaunchKernelGGL(alone, grid, dim3(kDeltaThreads), lds, s, a, o, e);
-    hipLaunchKernelGGL((delta_join<DK, true>), dim3(a.n_whole, a.heads, nz), dim3(kDeltaThreads),
-                       0, s, a, e, ws);
+    const auto alone = delta_scan_back<T, DK, WAVES, true>;
+    if (!lds_limit(reinterpret_cast<const void*>(alone), buffers * bytes)) return MLCG_ERR_LAUNCH;
+    hipLaunchKernelGGL(alone, grid, block, buffers * bytes, s, a, o, e, buffers);
+    const int status = join<T, DK, WAVES, true>(a, e, ws, s);
+    if (status != MLCG_OK) return status;
     e.seg_init = ws;
   }
-  const auto scan = delta_scan_back<T, DK, false>;
-  if (!lds_limit(reinterpret_cast<const void*>(scan), lds)) return MLCG_ERR_LAUNCH;
-  hipLaunchKernelGGL(scan, grid, dim3(kDeltaThreads), lds, s, a, o, e);
-  const bool gv = a.dv % 8 == 0 && chain_aligned16(o.grad);
-  const bool vv = a.dv % 8 == 0 && chain_aligned16(a.v) && a.v_row * sizeof(T) % 16 == 0 &&
-                  a.v_head * sizeof(T) % 16 == 0;
+  const auto scan = delta_scan_back<T, DK, WAVES, false>;
+  if (!lds_limit(reinterpret_cast<const void*>(scan), buffers * bytes)) return MLCG_ERR_LAUNCH;
+  hipLaunchKernelGGL(scan, grid, block, buffers * bytes, s, a, o, e, buffers);
   const auto grad = delta_grad<T, DK>;
   const size_t glds = sizeof(GradTiles<T, DK>);
   if (!lds_limit(reinterpret_cast<const void*>(grad), glds)) return MLCG_ERR_LAUNCH;
-  hipLaunchKernelGGL(grad, dim3(a.n_tiles, a.keys), dim3(kDeltaThreads), glds, s, a, o,
-                     (gv ? 1 : 0) | (vv ? 2 : 0));
+  hipLaunchKernelGGL(grad, dim3(a.n_tiles, a.keys), dim3(kDeltaThreads), glds, s, a, o);
   return mlcg_launch_status();
 }
 
-template <typename T>
-DeltaArgs with_vec(DeltaArgs a) {
-  bool ok = a.dk % 8 == 0 && chain_aligned16(a.q) && chain_aligned16(a.k);
-  for (int64_t x : {a.q_row, a.q_head, a.k_row, a.k_head}) ok = ok && x * sizeof(T) % 16 == 0;
-  a.vec = ok;
-  return a;
+template <typename T, int DK>
+int forward_dk(const DeltaArgs& a, T* out, const DeltaEnds& e, float* ws, hipStream_t s) {
+  return a.dv <= 64 ? forward_waves<T, DK, 4>(a, out, e, ws, s)
+                    : forward_waves<T, DK, 8>(a, out, e, ws, s);
+}
+template <typename T, int DK>
+int backward_dk(const DeltaArgs& a, const DeltaBack& b, const DeltaEnds& e, float* ws,
+                hipStream_t s) {
+  return a.dv <= 64 ? backward_waves<T, DK, 4>(a, b, e, ws, s)
+                    : backward_waves<T, DK, 8>(a, b, e, ws, s);
 }
 
 }  // namespace
 
 template <>
-int delta_forward<MLCG_DELTA_TYPE>(const DeltaArgs& args, void* out, const DeltaEnds& e, float* ws,
+int delta_forward<MLCG_DELTA_TYPE>(const DeltaArgs& a, void* out, const DeltaEnds& e, float* ws,
                                    hipStream_t s) {
   typedef MLCG_DELTA_TYPE T;
-  const DeltaArgs a = with_vec<T>(args);
   switch (delta_dk(a.dk)) {
     case 32: return forward_dk<T, 32>(a, (T*)out, e, ws, s);
     case 64: return forward_dk<T, 64>(a, (T*)out, e, ws, s);
@@ -1162,10 +1415,9 @@ int delta_forward<MLCG_DELTA_TYPE>(const DeltaArgs& args, void* out, const Delta
 }
 
 template <>
-int delta_backward<MLCG_DELTA_TYPE>(const DeltaArgs& args, const DeltaBack& b, const DeltaEnds& e,
+int delta_backward<MLCG_DELTA_TYPE>(const DeltaArgs& a, const DeltaBack& b, const DeltaEnds& e,
                                     float* ws, hipStream_t s) {
   typedef MLCG_DELTA_TYPE T;
-  const DeltaArgs a = with_vec<T>(args);
   switch (delta_dk(a.dk)) {
     case 32: return backward_dk<T, 32>(a, b, e, ws, s);
     case 64: return backward_dk<T, 64>(a, b, e, ws, s);

@@ -147,36 +147,41 @@ int step_of(const StepArgs& a, int64_t batch, hipStream_t s) {
 
 // the parts of the buffers, in floats
 struct Parts {
-  int64_t fac, mats, u, s0, seg_state, seg_map;
+  int64_t fac, rows, mats, u, s0, seg_state, seg_map;
+  int64_t chunks() const { return fac + 2 * rows + 2 * mats + seg_map; }
 };
-Parts parts(int64_t beads, int64_t tiles, int64_t segs, int heads, int dk, int dv, int dtype) {
+Parts parts(int64_t tiles, int64_t segs, int heads, int keys, int dk, int dv, int dtype) {
   const int64_t DK = delta_dk(dk), dvp = (dv + 15) / 16 * 16;
-  const int64_t pieces = dtype == MLCG_DTYPE_F32 ? 3 : 2;
+  const int64_t in = dtype == MLCG_DTYPE_F32 ? 3 : dtype == MLCG_DTYPE_F16 ? 2 : 1;
+  const int64_t mid = dtype == MLCG_DTYPE_F32 ? 3 : 2;
   return Parts{tiles * heads * (kDeltaFactors * kDeltaRows),
-               tiles * heads * pieces * (kDeltaPlane / 2),
-               (beads * heads * dvp + 15) / 16 * 16,
+               tiles * keys * in * (DK / 8) * 256,
+               tiles * heads * mid * kDeltaLower * 256,
+               tiles * heads * kDeltaRows * dvp,
                tiles * heads * DK * dvp,
                segs * heads * DK * dvp,
-               segs * heads * DK * DK};
+               segs * heads * mid * (DK * DK / 2)};
 }
 
 bool delta_ok(const DeltaArgs& a, int dtype) {
+  for (int64_t row : {a.q_row, a.k_row, a.v_row})  // 64 rows are within 32 bits
+    if (row < 0 || row >= (int64_t(1) << 22)) return false;
   return a.beads >= 0 && a.beads < (int64_t(1) << 31) - 256 && a.heads >= 1 && a.heads <= 1024 &&
-         a.keys >= 1 && a.heads % a.keys == 0 && a.dk >= 1 && a.dk <= 128 && a.dv >= 1 &&
-         a.dv <= 128 && dtype >= MLCG_DTYPE_F32 && dtype <= MLCG_DTYPE_BF16;
+         a.keys >= 1 && a.heads % a.keys == 0 && a.dk >= 8 && a.dk <= 128 && a.dk % 8 == 0 &&
+         a.dv >= 8 && a.dv <= 128 && a.dv % 8 == 0 && dtype >= MLCG_DTYPE_F32 && dtype <= MLCG_DTYPE_BF16;
 }
 
 }  // namespace
 
-extern "C" int64_t mlcg_gated_delta_floats(int64_t beads, int64_t n_tiles, int64_t n_split,
-                                           int heads, int dk, int dv, int dtype, int which) {
-  if (beads < 0 || n_tiles < 0 || n_split < 0 || heads < 1 || dk < 1 || dk > 128 || dv < 1 ||
+extern "C" int64_t mlcg_gated_delta_floats(int64_t n_tiles, int64_t n_split, int heads,
+                                           int key_heads, int dk, int dv, int dtype, int which) {
+  if (n_tiles < 0 || n_split < 0 || heads < 1 || key_heads < 1 || dk < 1 || dk > 128 || dv < 1 ||
       dv > 128 || dtype < MLCG_DTYPE_F32 || dtype > MLCG_DTYPE_BF16)
     return -1;
-  const Parts p = parts(beads, n_tiles, n_split, heads, dk, dv, dtype);
+  const Parts p = parts(n_tiles, n_split, heads, key_heads, dk, dv, dtype);
   switch (which) {
-    case 0: return p.fac + 2 * p.mats + p.seg_map;
-    case 1: return p.fac + 2 * p.mats + p.seg_map + p.u + p.s0;
+    case 0: return p.chunks();
+    case 1: return p.chunks() + p.u + p.s0;
     case 2: return 2 * p.seg_state;
     case 3: return 2 * p.seg_state + p.u + p.s0;
     default: return -1;
@@ -185,13 +190,17 @@ extern "C" int64_t mlcg_gated_delta_floats(int64_t beads, int64_t n_tiles, int64
 
 namespace {
 
-// the arrays in `kept`: factors, T, P, the segments' maps, and u and S0
+// the arrays in `kept`: factors, k, q, T, P, the segments' maps, and u and S0
 void place(DeltaArgs& a, DeltaEnds& e, float* kept, const Parts& p, bool train, bool split) {
   a.fac = kept;
-  a.T = reinterpret_cast<__bf16*>(kept + p.fac);
-  a.P = reinterpret_cast<__bf16*>(kept + p.fac + p.mats);
-  float* at = kept + p.fac + 2 * p.mats;
-  e.seg_map = split ? at : nullptr;
+  float* at = kept + p.fac;
+  a.K = reinterpret_cast<float4*>(at);
+  a.Q = reinterpret_cast<float4*>(at + p.rows);
+  at += 2 * p.rows;
+  a.T = reinterpret_cast<float4*>(at);
+  a.P = reinterpret_cast<float4*>(at + p.mats);
+  at += 2 * p.mats;
+  e.seg_map = split ? reinterpret_cast<float4*>(at) : nullptr;
   at += p.seg_map;
   a.U = train ? at : nullptr;
   a.S0 = train ? at + p.u : nullptr;
@@ -212,16 +221,16 @@ extern "C" int mlcg_gated_delta(
                n_segments < (int64_t(1) << 31) && n_whole >= 0 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
-              (dv + 15) / 16 * 16, scale, normalize, reverse, 0,
+              (dv + 15) / 16 * 16, scale, normalize, reverse,
               reinterpret_cast<const int4*>(tiles), (int)n_tiles,
               reinterpret_cast<const int4*>(segments), segment_first, (int)n_segments,
-              (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr};
+              (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   MLCG_REQUIRE(delta_ok(a, dtype));
   if (beads == 0 || n_tiles == 0) return MLCG_OK;
   MLCG_REQUIRE(q && k && v && decay && beta && tiles && segments && segment_first && out && kept &&
                n_whole >= 1);
-  const Parts p = parts(beads, n_tiles, split ? n_segments : 0, heads, dk, dv, dtype);
-  MLCG_REQUIRE(kept_floats >= p.fac + 2 * p.mats + p.seg_map + (train ? p.u + p.s0 : 0) &&
+  const Parts p = parts(n_tiles, split ? n_segments : 0, heads, key_heads, dk, dv, dtype);
+  MLCG_REQUIRE(kept_floats >= p.chunks() + (train ? p.u + p.s0 : 0) &&
                workspace_floats >= 2 * p.seg_state && (!split || workspace));
   DeltaEnds e{state, last_state, nullptr, nullptr, nullptr};
   place(a, e, kept, p, train, split);
@@ -247,20 +256,20 @@ extern "C" int mlcg_gated_delta_backward(
                n_segments < (int64_t(1) << 31) && n_whole >= 1 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
-              (dv + 15) / 16 * 16, scale, normalize, reverse, 0,
+              (dv + 15) / 16 * 16, scale, normalize, reverse,
               reinterpret_cast<const int4*>(tiles), (int)n_tiles,
               reinterpret_cast<const int4*>(segments), segment_first, (int)n_segments,
-              (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr};
+              (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   MLCG_REQUIRE(delta_ok(a, dtype) && beads >= 1);
   MLCG_REQUIRE(q && k && v && decay && beta && tiles && segments && segment_first && kept &&
                grad_out && grad_q && grad_k && grad_v && grad_decay && grad_beta && workspace);
-  const Parts p = parts(beads, n_tiles, split ? n_segments : 0, heads, dk, dv, dtype);
-  MLCG_REQUIRE(kept_floats >= p.fac + 2 * p.mats + p.seg_map + p.u + p.s0 &&
+  const Parts p = parts(n_tiles, split ? n_segments : 0, heads, key_heads, dk, dv, dtype);
+  MLCG_REQUIRE(kept_floats >= p.chunks() + p.u + p.s0 &&
                workspace_floats >= 2 * p.seg_state + p.u + p.s0);
   DeltaEnds e{grad_last_state, nullptr, nullptr, nullptr, nullptr};
   place(a, e, const_cast<float*>(kept), p, true, split);
   float* at = workspace;
-  const DeltaBack b{grad_out, grad_last_state, grad_q, grad_k, grad_v, grad_decay, grad_beta,
+  const DeltaBack b{grad_out, grad_q, grad_k, grad_v, grad_decay, grad_beta,
                     grad_state, at, at + p.s0};
   at += p.s0 + p.u;
   if (split) e.seg_last = at;

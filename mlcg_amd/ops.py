@@ -2303,13 +2303,40 @@ class _DeltaPlan:
     split: int
 
 
-def _delta_segment_tiles(chains: ChainLayout, heads: int, dv: int) -> int:
-    """Chunks of a segment, 0 for whole chains."""
-    return 0
+def _delta_segment_tiles(chains: ChainLayout, heads: int) -> int:
+    """Chunks of a segment, 0 for whole chains: the smallest of the times that
+    these come to, in microseconds.  A workgroup takes about 2.9 a chunk; two go at
+    a time on each of 256 compute units; segments are gone through twice, and
+    joining them takes about 1.2 each, one after the other, and two launches more.
+    Measured, forward and backward: 2 x 4099 beads, 8 heads of 64 in bf16, whole
+    207 and 280, segments of 4, 6, 8 and 16 chunks 89 and 169, 78 and 164, 85 and
+    169, 110 and 200; 64 x 1000, 4 heads of 32, whole 98 and 242, of 8 126 and 264;
+    1 x 120001, 8 heads of 64, whole 5914, of 16, 32 and 64 817, 704 and 730."""
+    rows = chains.plans.get(("delta segment", heads))
+    if rows is None:
+        count = -(-np.asarray(chains.lengths, dtype=np.int64) // DELTA_ROWS)
+        count = count[count > 0]
+        rows = 0
+        if count.size:
+            longest = int(count.max())
+
+            def rounds(groups):
+                return -(-groups * heads // 512)
+
+            best = 2.9 * longest * rounds(count.size)
+            for step in (4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128):
+                if step >= longest:
+                    break
+                segs = -(-count // step)
+                cost = 5.8 * step * rounds(int(segs.sum())) + 1.2 * int(segs.max()) + 12.0
+                if cost < best:
+                    best, rows = cost, step
+        chains.plans[("delta segment", heads)] = rows
+    return rows
 
 
-def _delta_plan(chains: ChainLayout, heads: int, dv: int) -> _DeltaPlan:
-    rows = _delta_segment_tiles(chains, heads, dv)
+def _delta_plan(chains: ChainLayout, heads: int) -> _DeltaPlan:
+    rows = _delta_segment_tiles(chains, heads)
     plan = chains.plans.get(("delta", rows))
     if plan is None:
         lens = np.asarray(chains.lengths, dtype=np.int64)
@@ -2333,26 +2360,41 @@ def _delta_plan(chains: ChainLayout, heads: int, dv: int) -> _DeltaPlan:
     return plan
 
 
-def _delta_floats(chains: ChainLayout, plan: _DeltaPlan, heads, dk, dv, dt, which: int) -> int:
-    key = ("delta floats", plan.split, plan.segments.shape[0], heads, dk, dv, dt, which)
+def _delta_floats(chains: ChainLayout, plan: _DeltaPlan, heads, keys, dk, dv, dt,
+                  which: int) -> int:
+    key = ("delta floats", plan.split, plan.segments.shape[0], heads, keys, dk, dv, dt, which)
     n = chains.plans.get(key)
     if n is None:
         n = chains.plans[key] = int(_lib.load().mlcg_gated_delta_floats(
-            chains.n_beads, chains.tiles[DELTA_ROWS].shape[0],
-            plan.segments.shape[0] if plan.split else 0, heads, dk, dv, dt, which))
+            chains.tiles[DELTA_ROWS].shape[0], plan.segments.shape[0] if plan.split else 0, heads,
+            keys, dk, dv, dt, which))
     return n
+
+
+def _delta_pad(t: Optional[torch.Tensor], dk: int, dv: int) -> Optional[torch.Tensor]:
+    """States with rows and columns of zeros up to multiples of 8."""
+    if t is None or (dk % 8 == 0 and dv % 8 == 0):
+        return t
+    return torch.nn.functional.pad(t, (0, -dv % 8, 0, -dk % 8))
 
 
 def _delta_args(q, k, v, decay, beta, chains, scale, keep):
     _check(isinstance(chains, ChainLayout), "chains must be a ChainLayout")
+    _check(all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in (q, k, v)),
+           "q, k and v must be [beads, heads, dim]")
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    # the kernels take channels by eights: others are filled up with zeros, which
+    # change no product and no length
+    if q.shape[2] % 8 or v.shape[2] % 8:
+        q, k, v = (torch.nn.functional.pad(t, (0, -t.shape[2] % 8)) for t in (q, k, v))
     args = _delta_heads(q, k, v, decay, beta, chains.n_beads, "gated_delta")
-    dev, dk = args[0].device, args[10]
+    dev = args[0].device
     _check(chains.device == dev, "chains must be a ChainLayout on the rows' device")
     if keep is not None:
         _check(keep.shape == (chains.n_beads,) and keep.dtype == torch.bool
                and keep.device == dev, lambda: f"keep must be [{chains.n_beads}] bool on {dev}")
         keep = keep.contiguous()
-    return args, float(dk ** -0.5 if scale is None else scale), keep
+    return args, float(scale), keep
 
 
 def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
@@ -2375,20 +2417,23 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.
     it is, whatever its k, v, decay and beta hold; its q reads the state.  state
     [B, H, DK, DV] float32: where each chain begins (zeros by default); last is
     where it ends.  kept is what the backward pass takes (train=True)."""
+    own = q.shape[-1], v.shape[-1]
     (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
         q, k, v, decay, beta, chains, scale, keep)
     n, dev = chains.n_beads, q.device
-    state = _check_delta_state(state, "state", (chains.n_chains, heads, dk, dv), dev)
+    state = _check_delta_state(state, "state", (chains.n_chains, heads, *own), dev)
+    state = _delta_pad(state, *own)
     out = torch.empty(n, heads, dv, dtype=q.dtype, device=dev)
     last = torch.empty(chains.n_chains, heads, dk, dv, dtype=torch.float32, device=dev)
     if chains.whole.shape[0] < chains.n_chains:  # chains without beads end as they begin
         last.zero_() if state is None else last.copy_(state)
     if n == 0:
-        return out, last, torch.empty(0, dtype=torch.float32, device=dev)
-    plan = _delta_plan(chains, heads, dv)
-    size = _delta_floats(chains, plan, heads, dk, dv, dt, 1 if train else 0)
+        return (out[..., :own[1]], last[..., :own[0], :own[1]].contiguous(),
+                torch.empty(0, dtype=torch.float32, device=dev))
+    plan = _delta_plan(chains, heads)
+    size = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 1 if train else 0)
     kept = torch.empty(size, dtype=torch.float32, device=dev)
-    nws = _delta_floats(chains, plan, heads, dk, dv, dt, 2)
+    nws = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 2)
     ws = torch.empty(nws, dtype=torch.float32, device=dev) if nws > 0 else None
     tiles = chains.tiles[DELTA_ROWS]
     call("mlcg_gated_delta", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), n, heads,
@@ -2396,6 +2441,8 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.
          ptr(plan.first), plan.first.shape[0] - 1, plan.split, ptr(keep), ptr(state), scale,
          int(normalize), int(reverse), ptr(out), ptr(last), ptr(kept), size, int(train), ptr(ws),
          nws, stream_handle(dev))
+    if own != (dk, dv):
+        out, last = out[..., :own[1]].contiguous(), last[..., :own[0], :own[1]].contiguous()
     return out, last, kept
 
 
@@ -2406,14 +2453,18 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
     """(grad q, grad k, grad v, grad decay, grad beta, grad state | None) of
     gated_delta for the gradients of its outputs (mlcg_gated_delta_backward);
     kept is the forward's, with train=True.  Every sum has a fixed order."""
+    own = q.shape[-1], v.shape[-1]
     (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
         q, k, v, decay, beta, chains, scale, keep)
     n, dev = chains.n_beads, q.device
-    _check(grad.shape == (n, heads, dv) and grad.dtype == q.dtype and grad.device == dev,
-           lambda: f"grad must be [{n}, {heads}, {dv}] {q.dtype} on {dev}")
+    _check(grad.shape == (n, heads, own[1]) and grad.dtype == q.dtype and grad.device == dev,
+           lambda: f"grad must be [{n}, {heads}, {own[1]}] {q.dtype} on {dev}")
+    if own[1] != dv:
+        grad = torch.nn.functional.pad(grad, (0, dv - own[1]))
     grad = grad.contiguous()
     shape = (chains.n_chains, heads, dk, dv)
-    grad_last = _check_delta_state(grad_last, "grad_last", shape, dev)
+    grad_last = _check_delta_state(grad_last, "grad_last", (chains.n_chains, heads, *own), dev)
+    grad_last = _delta_pad(grad_last, *own)
     dq = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
     dkk = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
     dvv = torch.empty(n, heads, dv, dtype=q.dtype, device=dev)
@@ -2423,12 +2474,14 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
     if want_state and chains.whole.shape[0] < chains.n_chains:
         dstate.zero_() if grad_last is None else dstate.copy_(grad_last)
     if n == 0:
-        return dq, dkk, dvv, ddecay, dbeta, dstate
-    plan = _delta_plan(chains, heads, dv)
-    size = _delta_floats(chains, plan, heads, dk, dv, dt, 1)
+        if want_state:
+            dstate = dstate[..., :own[0], :own[1]].contiguous()
+        return dq[..., :own[0]], dkk[..., :own[0]], dvv[..., :own[1]], ddecay, dbeta, dstate
+    plan = _delta_plan(chains, heads)
+    size = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 1)
     _check(kept.shape == (size,) and kept.dtype == torch.float32 and kept.device == dev,
            "kept must be what gated_delta gave with train=True for the same chains")
-    nws = _delta_floats(chains, plan, heads, dk, dv, dt, 3)
+    nws = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 3)
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     tiles = chains.tiles[DELTA_ROWS]
     call("mlcg_gated_delta_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta),
@@ -2437,6 +2490,11 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
          scale, int(normalize), int(reverse), ptr(kept), size, ptr(grad), ptr(grad_last), ptr(dq),
          ptr(dkk), ptr(dvv), ptr(ddecay), ptr(dbeta), ptr(dstate), ptr(ws), nws,
          stream_handle(dev))
+    if own != (dk, dv):
+        dq, dkk, dvv = (t[..., :d].contiguous() for t, d in
+                        ((dq, own[0]), (dkk, own[0]), (dvv, own[1])))
+        if want_state:
+            dstate = dstate[..., :own[0], :own[1]].contiguous()
     return dq, dkk, dvv, ddecay, dbeta, dstate
 
 

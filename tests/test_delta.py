@@ -105,7 +105,7 @@ def test_segments(monkeypatch, lengths, chunks):
     marked."""
     monkeypatch.setattr(ops, "_delta_segment_tiles", lambda *a: chunks)
     c = ops.chain_layout(lengths, "cpu")
-    plan = ops._delta_plan(c, 4, 32)
+    plan = ops._delta_plan(c, 4)
     assert plan.split == (chunks > 0)
     segs, first = plan.segments.tolist(), plan.first.tolist()
     assert first[-1] == len(segs) and len(first) == 1 + sum(n > 0 for n in lengths)
