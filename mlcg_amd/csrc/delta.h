@@ -75,7 +75,7 @@ struct DeltaArgs {
   const float *decay, *beta;                            // [beads, heads]
   const uint8_t* keep;
   int64_t beads;
-  int heads, keys, group, dk, dv, dvp;  // dvp: dv rounded up to 16
+  int heads, keys, group, dk, dv, dvp;  // dvp: dv rounded up to 32
   float scale;
   int normalize, reverse;
   const int4* tiles;            // (chain's first row, its length, tile's first row in it, chain)
@@ -86,14 +86,14 @@ struct DeltaArgs {
   float* fac;
   float4 *K, *Q;                // operands, [tile, keys, pieces, 4, DK / 32, 64 slots]
   float4 *T, *P;                // [tile, heads, pieces, 6, 64 slots]
-  float *U, *S0;                // [tile, heads, 64, dvp], [tile, heads, DK, dvp]
+  float4 *U, *S0;               // operands: u, and the states' transposes, or NULL
 };
 
 struct DeltaBack {
   const void* grad;       // [beads, heads, dv]
   void *dq, *dk, *dv;
   float *ddecay, *dbeta, *dstate;
-  float *D, *dR;          // as S0 and U
+  float4 *D, *dR;         // as S0 and U
 };
 
 // where a scan begins and ends
@@ -568,6 +568,12 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
 // ---------------------------------------------------------------------------
 // The state along the chunks of a segment: 16 columns a wave, all a workgroup.
 
+// waves a SIMD of the scans: the registers are held to what so many leave
+template <typename T, int DK>
+constexpr int scan_waves() {
+  return DK == 128 ? 1 : sizeof(T) == 2 ? 3 : 2;
+}
+
 // what a chunk's step needs in LDS, the last two for outputs and backward
 template <typename T, int DK>
 struct ScanTiles {
@@ -635,11 +641,33 @@ struct Columns {
   }
 };
 
-// the same rows of a column to a chunk's 64 rows of ld floats
-__device__ __forceinline__ void store_column(float* at, int ld, const f32x4 (&x)[4]) {
-  const Lines l(at, 0, 1, 4 * ld, 4 * (mlcg_lane() >> 4), 12, 4 * (mlcg_lane() & 15));
+// A wave's right operands as they are to block row w of an image of `rows` of them:
+// read as rows they are the transpose of what the wave has.
+template <int N, int KS>
+__device__ __forceinline__ void store_operand(float4* images, int64_t at, int rows, int w,
+                                              const Frag<N> (&s)[KS]) {
+  float4* const p = images + at * ((int64_t)N * rows * KS * 64) + Image<N, KS>::slot();
 #pragma unroll
-  for (int r = 0; r < 16; ++r) l.row<float>(16 * (r / 4) + r % 4) = x[r / 4][r % 4];
+  for (int i = 0; i < KS; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      p[((j * rows + w) * KS + i) * 64] = __builtin_bit_cast(float4, s[i].p[j]);
+}
+// The transpose of a chunk's rows, 4 of the wave's 16 columns of row 16 b + c in a
+// lane, to an image of 64 rows and 32 kv columns: half of the blocks' elements.
+template <int N>
+__device__ __forceinline__ void store_half(float4* images, int64_t at, int kv, int w,
+                                           f32x4 (&y)[4]) {
+  bf16x4* const p = reinterpret_cast<bf16x4*>(images + at * ((int64_t)N * 4 * kv * 64) +
+                                              Image<N, 4>::slot()) + (w & 1);
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bf16x4 z = __builtin_convertvector(y[b], bf16x4);
+      p[((j * 4 + b) * kv + w / 2) * 128] = z;
+      if (j + 1 < N) y[b] -= __builtin_convertvector(z, f32x4);
+    }
 }
 
 // a state's 16 columns from `at` on: rows 16 b + 4 g + i, column c of them
@@ -741,8 +769,8 @@ __device__ __forceinline__ void lower_product(f32x4 (&y)[4], const Image<N, kDel
         mma(y[b], f[lower(b, i)], x[i]);
     }
 }
-// y += (lower triangle)^T x
-template <int N, int M>
+// y += (lower triangle)^T x, or, FLIP, the transpose of that
+template <bool FLIP, int N, int M>
 __device__ __forceinline__ void upper_product(f32x4 (&y)[4], const Image<N, kDeltaLower>& t,
                                               const Frag<M> (&x)[2]) {
   Frag<N> f[4][2];
@@ -756,7 +784,12 @@ __device__ __forceinline__ void upper_product(f32x4 (&y)[4], const Image<N, kDel
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int b = 0; b < 2 * i + 2; ++b) mma(y[b], f[b][i], x[i]);
+    for (int b = 0; b < 2 * i + 2; ++b) {
+      if (FLIP)
+        mma(y[b], x[i], f[b][i]);
+      else
+        mma(y[b], f[b][i], x[i]);
+    }
 }
 // the 16 B rows of a wave's columns as right operands
 template <int N, int B>
@@ -774,7 +807,7 @@ __device__ __forceinline__ f32x4 row_factor(const float* f, int b) {
 // sent to one while the other is worked on; with one the next workgroup on the
 // compute unit works meanwhile.
 template <typename T, int DK, int WAVES, bool ALONE>
-__global__ __launch_bounds__(64 * WAVES) void delta_scan(DeltaArgs a, DeltaEnds e, T* out,
+__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan(DeltaArgs a, DeltaEnds e, T* out,
                                                          int buffers) {
   constexpr int NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -827,9 +860,9 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan(DeltaArgs a, DeltaEnds 
     }
     if (!live) continue;
     const int64_t at = (int64_t)tile * a.heads + h;
-    if (!ALONE && a.S0) store_padded<B>(S, a.S0 + at * (DK * a.dvp) + v0, a.dvp);
     Frag<NM> s[KS], x[2];
     split_rows<NM>(s, S);
+    if (!ALONE && a.S0) store_operand<NM, KS>(a.S0, at, a.dvp / 16, w, s);
     f32x4 Y[4];
     rows_product<false>(Y, sh.k, s);
 #pragma unroll
@@ -843,10 +876,11 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan(DeltaArgs a, DeltaEnds 
     if (a.dv != a.dvp && !unit && v0 + c >= a.dv)  // columns that are none stay zeros
 #pragma unroll
       for (int b = 0; b < 4; ++b) X[b] = f32x4{};
-    split_rows<NM>(x, X);
+    Frag<NM> xu[2];
+    split_rows<NM>(xu, X);
 #pragma unroll
     for (int b = 0; b < 4; ++b) X[b] = f32x4{};
-    lower_product<false>(X, sh.t, x);
+    lower_product<false>(X, sh.t, xu);
     if (!ALONE) {
       split_rows<NM>(x, X);
       // o^T: four columns of one bead in a lane
@@ -871,7 +905,12 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan(DeltaArgs a, DeltaEnds 
               store4<T>(out + (ch.bead(16 * b + c) * a.heads + h) * a.dv, el, a.dv, O[b]);
         }
       }
-      if (a.U) store_column(a.U + at * (kDeltaRows * a.dvp) + v0, a.dvp, X);
+      if (a.U) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) O[b] = f32x4{};
+        lower_product<true>(O, sh.t, xu);
+        store_half<NM>(a.U, at, a.dvp / 32, w, O);
+      }
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) X[b] *= row_factor(sh.fac[kFacWrite], b);
@@ -951,7 +990,7 @@ __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds 
 
 // The state's gradient along the chunks of a segment, the last one first.
 template <typename T, int DK, int WAVES, bool ALONE>
-__global__ __launch_bounds__(64 * WAVES) void delta_scan_back(DeltaArgs a, DeltaBack o,
+__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan_back(DeltaArgs a, DeltaBack o,
                                                               DeltaEnds e, int buffers) {
   constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -1011,11 +1050,11 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_back(DeltaArgs a, Delta
     }
     if (!live) continue;
     const int64_t at = (int64_t)tile * a.heads + h;
-    if (!ALONE) store_padded<B>(D, o.D + at * (DK * a.dvp) + v0, a.dvp);
     Frag<NM> x[2];
     {
       Frag<NM> d[KS];
       split_rows<NM>(d, D);
+      if (!ALONE) store_operand<NM, KS>(o.D, at, a.dvp / 16, w, d);
       rows_product<false>(X, sh.k, d);
     }
     // du
@@ -1024,34 +1063,41 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_back(DeltaArgs a, Delta
     {
       Frag<NI> go[2];
       split_rows<NI>(go, G);
-      upper_product(X, sh.p, go);
+      upper_product<false>(X, sh.p, go);
     }
     split_rows<NM>(x, X);
     // dr
 #pragma unroll
     for (int b = 0; b < 4; ++b) X[b] = f32x4{};
-    upper_product(X, sh.t, x);
-    if (!ALONE) store_column(o.dR + at * (kDeltaRows * a.dvp) + v0, a.dvp, X);
+    upper_product<false>(X, sh.t, x);
+    if (!ALONE) {
+      // its transpose: four columns of one bead in a lane
+      f32x4 R[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) X[b] *= row_factor(sh.fac[kFacBeta], b);
-    if (!ALONE && v0 + c < a.dv) {
-      if (ch.n == kDeltaRows) {
-        const Lines l(o.dv, ch.base, ch.step, row * (int)sizeof(T), 4 * g, 12,
-                      (h * a.dv + v0 + c) * (int)sizeof(T));
+      for (int b = 0; b < 4; ++b) R[b] = f32x4{};
+      upper_product<true>(R, sh.t, x);
+      const int el = v0 + 4 * g;
+      if (el < a.dv) {
+        typedef typename loose<T, 4>::type vec;
+        if (ch.n == kDeltaRows) {
+          const Lines l(o.dv, ch.base, ch.step, row * (int)sizeof(T), c, 15,
+                        (h * a.dv + el) * (int)sizeof(T));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) l.row<T>(16 * (r / 4) + r % 4) = (T)X[r / 4][r % 4];
-      } else {
-        T* const dv = (T*)o.dv + h * a.dv + v0 + c;
+          for (int b = 0; b < 4; ++b)
+            l.row<vec>(16 * b) = __builtin_convertvector(R[b] * sh.fac[kFacBeta][16 * b + c], vec);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int t = 16 * (r / 4) + 4 * g + r % 4;
-          if (t < ch.n) dv[ch.bead(t) * row] = (T)X[r / 4][r % 4];
+          for (int b = 0; b < 4; ++b)
+            if (16 * b + c < ch.n)
+              store4<T>((T*)o.dv + ch.bead(16 * b + c) * row + h * a.dv, el, a.dv,
+                        R[b] * sh.fac[kFacBeta][16 * b + c]);
         }
       }
+      store_half<NM>(o.dR, at, a.dvp / 32, w, R);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      X[b] *= -row_factor(sh.fac[kFacRead], b);
+      X[b] *= row_factor(sh.fac[kFacBeta], b) * -row_factor(sh.fac[kFacRead], b);
       G[b] *= row_factor(sh.fac[kFacOut], b);
     }
 #pragma unroll
@@ -1074,34 +1120,52 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_back(DeltaArgs a, Delta
 // The gradients of q, k, beta and g of a chunk's beads, for the heads of one
 // key head; a wave has 16 beads, as columns.
 
-template <typename T, int DK>
+// What a chunk's gradients need in LDS, one after the other in one or two places:
+// u, dr and do; k and q; S0; D.
+template <typename T, int DK, int KV>
 struct GradTiles {
-  Image<Pieces<T>::in, DK / 8> k, q;
-  float fac[kDeltaFactors][kDeltaRows];
-  float dG[kDeltaRows];
-  float ends[4];
+  static constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid;
+  typedef Image<NM, 4 * KV> Rows;              // 64 beads x dv
+  typedef Image<NI, 4 * KV> Given;             // the same of do
+  typedef Image<NM, 2 * KV*(DK / 32)> State;   // dv x DK
+  typedef Image<NI, DK / 8> Keys;              // 64 beads x DK
+  static constexpr size_t rows = 2 * sizeof(Rows) + sizeof(Given);
+  static constexpr size_t keys = 2 * sizeof(Keys);
+  static constexpr size_t even = rows > sizeof(State) ? rows : sizeof(State);
+  static constexpr size_t odd = keys > sizeof(State) ? keys : sizeof(State);
+  static constexpr size_t bytes(int places) {
+    return places == 2 ? even + odd : even > odd ? even : odd;
+  }
+  struct Small {
+    float fac[kDeltaFactors][kDeltaRows];
+    float dG[kDeltaRows];
+    float ends[4];
+  };
 };
 
-// 8 floats of a padded row from el on, zeros past its end
-__device__ __forceinline__ f32x8 load_f8(const float* row, int el, int len) {
-  const f32x8 x = *reinterpret_cast<const f32x8*>(row + min(el, len - 8));
-  return el < len ? x : f32x8{};
+// waves a SIMD: two where the registers of half of it are enough
+template <typename T, int DK, int KV>
+constexpr int grad_waves() {
+  return sizeof(T) == 2 ? (DK <= 64 && KV <= 2 ? 2 : 1) : (DK == 32 && KV == 1 ? 2 : 1);
 }
 
-template <typename T, int DK>
-__global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBack o) {
+// MANY: several heads to a key head, whose gradients are summed
+template <typename T, int DK, int KV, bool MANY>
+__global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delta_grad(DeltaArgs a, DeltaBack o, int places) {
+  typedef GradTiles<T, DK, KV> Tiles;
+  typedef typename Tiles::Rows Rows;
+  typedef typename Tiles::Given Given;
+  typedef typename Tiles::State State;
+  typedef typename Tiles::Keys Keys;
   constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, B = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) unsigned char smem[];
-  GradTiles<T, DK>& sh = *reinterpret_cast<GradTiles<T, DK>*>(smem);
+  typename Tiles::Small& sh =
+      *reinterpret_cast<typename Tiles::Small*>(smem + Tiles::bytes(places));
+  unsigned char* const even = smem;
+  unsigned char* const odd = smem + (places - 1) * Tiles::even;
   const int tile = blockIdx.x, kh = blockIdx.y;
   const int w = wave_number(), lane = mlcg_lane(), c = lane & 15, g = lane >> 4;
   const Chunk ch(a, tile);
-  {
-    constexpr int units = Image<NI, DK / 8>::units;
-    const int64_t at = ((int64_t)tile * a.keys + kh) * (units * 64);
-    send_to_lds<units, 4>(sh.k.x, a.K + at);
-    send_to_lds<units, 4>(sh.q.x, a.Q + at);
-  }
   const int row = 16 * w + c;
   const bool in = row < ch.n;
   const int64_t bead = ch.bead(min(row, ch.n - 1));
@@ -1111,68 +1175,86 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
   for (int b = 0; b < B; ++b) dq[b] = dk[b] = f32x4{};
   float rq = 0.0f, rk = 0.0f;
 
+  const auto send_state = [&](unsigned char* to, const float4* from, int64_t at) {
+    send_to_lds<State::units, 4>(reinterpret_cast<float4*>(to), from + at * (State::units * 64));
+  };
+  const int64_t kat = ((int64_t)tile * a.keys + kh) * (Keys::units * 64);
+  const auto send_keys = [&](unsigned char* to) {
+    send_to_lds<Keys::units, 4>(reinterpret_cast<float4*>(to), a.K + kat);
+    send_to_lds<Keys::units, 4>(reinterpret_cast<float4*>(to + sizeof(Keys)), a.Q + kat);
+  };
+  // elements 32 i + 4 g .. and 32 i + 16 + 4 g .. of this wave's rows of k or q
+  const auto own_row = [&](const float4* from, int i) {
+    Frag<NI> f;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      f.p[j] = __builtin_bit_cast(
+          bf16x8, from[kat + (j * (DK / 8) + w * KS + i) * 64 + Keys::slot()]);
+    return whole(f);
+  };
+  // with one place, what comes next is sent for when all are done with the last
+  const auto wait_for = [&](auto send) {
+    if (places == 1) {
+      lds_barrier();
+      send();
+    }
+    wait_for_memory();
+    lds_barrier();
+  };
   for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
     const int64_t at = (int64_t)tile * a.heads + h;
     if (h > kh * a.group) lds_barrier();  // what the last head left has been read
+    Rows& U = *reinterpret_cast<Rows*>(even);
+    Rows& R = *reinterpret_cast<Rows*>(even + sizeof(Rows));
+    Given& G = *reinterpret_cast<Given*>(even + 2 * sizeof(Rows));
+    send_to_lds<Rows::units, 4>(U.x, a.U + at * (Rows::units * 64));
+    send_to_lds<Rows::units, 4>(R.x, o.dR + at * (Rows::units * 64));
     send_to_lds<2, 4>(reinterpret_cast<float4*>(sh.fac),
                       reinterpret_cast<const float4*>(a.fac +
                                                       at * (kDeltaFactors * kDeltaRows)));
+    // this wave's beads, as columns: do, and v for dr.v
+    Frag<NI> gb[KV];
+    f32x8 vr[KV];
+    {
+      const T* const go = (const T*)o.grad + (bead * a.heads + h) * a.dv;
+      const T* const v = (const T*)a.v + bead * a.v_row + h * a.v_head;
+#pragma unroll
+      for (int i = 0; i < KV; ++i) {
+        v4<T> x[2], y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          x[j] = load4<T>(go, 32 * i + 16 * j + 4 * g, a.dv);
+          y[j] = load4<T>(v, 32 * i + 16 * j + 4 * g, a.dv);
+        }
+        v8<T> u = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        v8<T> z = __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        if (!in) u = v8<T>{};
+        if (!there) z = v8<T>{};
+        gb[i] = split_raw<NI, T>(u);
+        vr[i] = __builtin_convertvector(z, f32x8);
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+          G.x[(j * (4 * KV) + w * KV + i) * 64 + G.slot()] =
+              __builtin_bit_cast(float4, gb[i].p[j]);
+      }
+    }
     wait_for_memory();
     lds_barrier();
-    const float* const U = a.U + at * (kDeltaRows * a.dvp);
-    const float* const R = o.dR + at * (kDeltaRows * a.dvp);
-    const T* const go = (const T*)o.grad + h * a.dv;
-    const int64_t go_row = (int64_t)a.heads * a.dv;
-    const float* const S0 = a.S0 + at * (DK * a.dvp);
-    const float* const D = o.D + at * (DK * a.dvp);
+    if (places == 2) send_keys(odd);
 
-    // [bead before][this wave's bead], and [bead after][this wave's bead]:
-    // ou, ru = do_t.u_s and dr_t.u_s
-    f32x4 ou0[4], ru0[4], ou1[4], ru1[4], hq[B], hr[B], hw[B];
+    // Products by beads with this wave's, s its row's or column's: of blocks before
+    // do_t.u_s and dr_t.u_s, [s][this wave's t]; of blocks behind the same, [t][this
+    // wave's s]; of its own both, the second apart.
+    Frag<NM> ub[KV], rb[KV];
+    f32x4 ou[4], ru[4], od{}, rd{};
+    float rv = 0.0f;  // dr.v
 #pragma unroll
-    for (int m = 0; m < 4; ++m) ou0[m] = ru0[m] = ou1[m] = ru1[m] = f32x4{};
+    for (int i = 0; i < KV; ++i) {
+      ub[i] = U.rows(w * KV + i);
+      rb[i] = R.rows(w * KV + i);
+      const f32x8 r = whole(rb[i]);
 #pragma unroll
-    for (int b = 0; b < B; ++b) hq[b] = hr[b] = hw[b] = f32x4{};
-    float rv = 0.0f, sd = 0.0f;  // dr.v;  this wave's part of <S0, D>
-    for (int v0 = 0; v0 < a.dvp; v0 += 32) {
-      const int el = v0 + 8 * g;
-      const f32x8 ur = load_f8(U + row * a.dvp, el, a.dvp);
-      const f32x8 rr = load_f8(R + row * a.dvp, el, a.dvp);
-      v8<T> gr = load8<T>(go + bead * go_row, el, a.dv);
-      v8<T> vr = load8<T>((const T*)a.v + bead * a.v_row + h * a.v_head, el, a.dv);
-      if (!in) gr = v8<T>{};
-      if (!there) vr = v8<T>{};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) rv = fmaf(rr[j], (float)vr[j], rv);
-      const Frag<NM> ub = split8<NM>(ur), rb = split8<NM>(rr);
-      const Frag<NI> gb = split_raw<NI, T>(gr);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int r = 16 * m + c;
-        if (m <= w) {
-          const Frag<NM> f = split8<NM>(load_f8(U + r * a.dvp, el, a.dvp));
-          mma(ou0[m], f, gb);
-          mma(ru0[m], f, rb);
-        }
-        if (m >= w) {
-          v8<T> x = load8<T>(go + ch.bead(min(r, ch.n - 1)) * go_row, el, a.dv);
-          if (r >= ch.n) x = v8<T>{};
-          mma(ou1[m], split_raw<NI, T>(x), ub);
-          mma(ru1[m], split8<NM>(load_f8(R + r * a.dvp, el, a.dvp)), ub);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        const f32x8 s = load_f8(S0 + (16 * b + c) * a.dvp, el, a.dvp);
-        const f32x8 d = load_f8(D + (16 * b + c) * a.dvp, el, a.dvp);
-        if (b % 4 == w)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sd = fmaf(s[j], d[j], sd);
-        const Frag<NM> f = split8<NM>(s);
-        mma(hq[b], f, gb);
-        mma(hr[b], f, rb);
-        mma(hw[b], split8<NM>(d), ub);
-      }
+      for (int j = 0; j < 8; ++j) rv = fmaf(r[j], vr[i][j], rv);
     }
     // factors of this wave's beads
     const float th = sh.fac[kFacHi][row], tl = sh.fac[kFacLo][row];
@@ -1181,64 +1263,158 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
     const float beta = sh.fac[kFacBeta][row];
     rk = sh.fac[kFacK][row];
     rq = sh.fac[kFacQ][row];
-    float kd = 0.0f;  // k.(e^(G_C - G) D u)
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk;
+    for (int m = 0; m < 4; ++m) {
+      const f32x4 hi = row_factor(sh.fac[kFacHi], m), lo = row_factor(sh.fac[kFacLo], m);
+      const f32x4 xk = row_factor(sh.fac[kFacK], m);
+      ou[m] = ru[m] = f32x4{};
+      if (m <= w) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int b = 2 * i + j;
-        hq[b] *= first;
-        hr[b] *= -first;
-        hw[b] *= rest;
+        for (int i = 0; i < KV; ++i) {
+          const Frag<NM> f = U.rows(m * KV + i);
+          mma(ou[m], f, gb[i]);
+          mma(ru[m], f, rb[i]);
+        }
 #pragma unroll
-        for (int y = 0; y < 4; ++y) kd = fmaf(x[4 * j + y], hw[b][y], kd);
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * m + 4 * g + i;
+          const float e = r <= row ? exp2_of(th - hi[i], tl - lo[i]) * xk[i] : 0.0f;
+          ou[m][i] = r <= row ? e * ou[m][i] : 0.0f;
+          ru[m][i] = r < row ? -e * ru[m][i] : 0.0f;
+        }
+      }
+      if (m >= w) {
+        const f32x4 xb = row_factor(sh.fac[kFacBeta], m), xq = row_factor(sh.fac[kFacQ], m);
+        f32x4 x{}, y{};
+#pragma unroll
+        for (int i = 0; i < KV; ++i) {
+          mma(x, G.rows(m * KV + i), ub[i]);
+          mma(y, R.rows(m * KV + i), ub[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * m + 4 * g + i;
+          const float e = r >= row ? exp2_of(hi[i] - th, lo[i] - tl) : 0.0f;
+          x[i] = r >= row ? e * xq[i] * a.scale * x[i] : 0.0f;
+          y[i] = r > row ? -e * xk[i] * xb[i] * y[i] : 0.0f;
+        }
+        if (m == w) {
+          od = x;
+          rd = y;
+        } else {
+          ou[m] = x;
+          ru[m] = y;
+        }
       }
     }
     // inside the chunk
+    f32x4 hq[B], hr[B], hw[B];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int b = 0; b < B; ++b) hq[b] = hr[b] = hw[b] = f32x4{};
+    wait_for([&] { send_keys(odd); });
+    if (places == 2) send_state(even, a.S0, at);
+    {
+      const Keys& K = *reinterpret_cast<const Keys*>(odd);
+      const Keys& Q = *reinterpret_cast<const Keys*>(odd + sizeof(Keys));
+      const f32x4 none{};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * m + 4 * g + i;
-        const float dh = th - sh.fac[kFacHi][r], dl = tl - sh.fac[kFacLo][r];
-        const float xk = sh.fac[kFacK][r];
-        const float e0 = r <= row ? exp2_of(dh, dl) * xk : 0.0f;
-        ou0[m][i] = r <= row ? e0 * ou0[m][i] : 0.0f;
-        ru0[m][i] = r < row ? -e0 * ru0[m][i] : 0.0f;
-        const float e1 = r >= row ? exp2_of(-dh, -dl) : 0.0f;
-        ou1[m][i] = r >= row ? e1 * sh.fac[kFacQ][r] * a.scale * ou1[m][i] : 0.0f;
-        ru1[m][i] = r > row ? -e1 * xk * sh.fac[kFacBeta][r] * ru1[m][i] : 0.0f;
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const Frag<NM> o0 = split44<NM>(ou0[2 * i], ou0[2 * i + 1]);
-      const Frag<NM> r0 = split44<NM>(ru0[2 * i], ru0[2 * i + 1]);
-      const Frag<NM> o1 = split44<NM>(ou1[2 * i], ou1[2 * i + 1]);
-      const Frag<NM> r1 = split44<NM>(ru1[2 * i], ru1[2 * i + 1]);
-#pragma unroll
-      for (int b = 0; b < B; b += 2) {
-        const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
-        const Frag<NI> k0 = sh.k.template columns<0>(b0, b1), k1 = sh.k.template columns<1>(b0, b1);
-        const Frag<NI> q0 = sh.q.template columns<0>(b0, b1), q1 = sh.q.template columns<1>(b0, b1);
+      for (int i = 0; i < 2; ++i) {
         if (i <= w / 2) {  // beads up to this wave's
-          mma(hq[b], k0, o0);
-          mma(hq[b + 1], k1, o0);
-          mma(hr[b], k0, r0);
-          mma(hr[b + 1], k1, r0);
+          const Frag<NM> of = split44<NM>(ou[2 * i], 2 * i + 1 <= w ? ou[2 * i + 1] : none);
+          const Frag<NM> rf = split44<NM>(ru[2 * i], 2 * i + 1 <= w ? ru[2 * i + 1] : none);
+#pragma unroll
+          for (int b = 0; b < B; b += 2) {
+            const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
+            const Frag<NI> k0 = K.template columns<0>(b0, b1), k1 = K.template columns<1>(b0, b1);
+            mma(hq[b], k0, of);
+            mma(hq[b + 1], k1, of);
+            mma(hr[b], k0, rf);
+            mma(hr[b + 1], k1, rf);
+          }
         }
         if (i >= w / 2) {
-          mma(hw[b], q0, o1);
-          mma(hw[b + 1], q1, o1);
-          mma(hw[b], k0, r1);
-          mma(hw[b + 1], k1, r1);
+          const f32x4 o0 = 2 * i == w ? od : 2 * i > w ? ou[2 * i] : none;
+          const f32x4 r0 = 2 * i == w ? rd : 2 * i > w ? ru[2 * i] : none;
+          const Frag<NM> of = split44<NM>(o0, 2 * i + 1 == w ? od : ou[2 * i + 1]);
+          const Frag<NM> rf = split44<NM>(r0, 2 * i + 1 == w ? rd : ru[2 * i + 1]);
+#pragma unroll
+          for (int b = 0; b < B; b += 2) {
+            const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
+            const Frag<NI> k0 = K.template columns<0>(b0, b1), k1 = K.template columns<1>(b0, b1);
+            const Frag<NI> q0 = Q.template columns<0>(b0, b1), q1 = Q.template columns<1>(b0, b1);
+            mma(hw[b], q0, of);
+            mma(hw[b + 1], q1, of);
+            mma(hw[b], k0, rf);
+            mma(hw[b + 1], k1, rf);
+          }
         }
+      }
+    }
+    // S0 do and S0 dr
+    wait_for([&] { send_state(even, a.S0, at); });
+    if (places == 2) send_state(odd, o.D, at);
+    {
+      const State& S = *reinterpret_cast<const State*>(even);
+#pragma unroll
+      for (int b = 0; b < B; b += 2) {
+        f32x4 q0{}, q1{}, r0{}, r1{};
+#pragma unroll
+        for (int i = 0; i < KV; ++i) {
+          const int b0 = 2 * i * KS + b / 2;
+          const Frag<NM> s0 = S.template columns<0>(b0, b0 + KS);
+          const Frag<NM> s1 = S.template columns<1>(b0, b0 + KS);
+          mma(q0, s0, gb[i]);
+          mma(r0, s0, rb[i]);
+          mma(q1, s1, gb[i]);
+          mma(r1, s1, rb[i]);
+        }
+        hq[b] += first * q0;
+        hq[b + 1] += first * q1;
+        hr[b] -= first * r0;
+        hr[b + 1] -= first * r1;
+      }
+    }
+    // D u, and this wave's part of <S0, D>
+    wait_for([&] { send_state(odd, o.D, at); });
+    float sd = 0.0f, kd = 0.0f;  // kd: k.(e^(G_C - G) D u)
+    {
+      const State& D = *reinterpret_cast<const State*>(odd);
+      const float4* const s0 = a.S0 + at * (State::units * 64) + State::slot();
+#pragma unroll
+      for (int u = 0; u < (2 * KV * KS + 3) / 4; ++u) {
+        const int block = 4 * u + w;
+        if (block >= 2 * KV * KS) continue;
+        Frag<NM> f;
+#pragma unroll
+        for (int j = 0; j < NM; ++j)
+          f.p[j] = __builtin_bit_cast(bf16x8, s0[(j * (2 * KV * KS) + block) * 64]);
+        const f32x8 x = whole(f), y = whole(D.rows(block));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sd = fmaf(x[j], y[j], sd);
+      }
+#pragma unroll
+      for (int b = 0; b < B; b += 2) {
+        const f32x8 x = own_row(a.K, b / 2) * (rk * rest);
+        f32x4 w0{}, w1{};
+#pragma unroll
+        for (int i = 0; i < KV; ++i) {
+          const int b0 = 2 * i * KS + b / 2;
+          mma(w0, D.template columns<0>(b0, b0 + KS), ub[i]);
+          mma(w1, D.template columns<1>(b0, b0 + KS), ub[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          kd = fmaf(x[j], w0[j], kd);
+          kd = fmaf(x[4 + j], w1[j], kd);
+        }
+        hw[b] += rest * w0;
+        hw[b + 1] += rest * w1;
       }
     }
     float qd = 0.0f, kr = 0.0f, kw = 0.0f;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk, y = whole(sh.q.rows(w * KS + i)) * rq;
+      const f32x8 x = own_row(a.K, i) * rk, y = own_row(a.Q, i) * rq;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int b = 2 * i + j / 4;
@@ -1249,8 +1425,13 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
     }
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      dq[b] += hq[b];
-      dk[b] += beta * hr[b] + hw[b];
+      if (MANY) {
+        dq[b] += hq[b];
+        dk[b] += beta * hr[b] + hw[b];
+      } else {
+        dq[b] = hq[b];
+        dk[b] = beta * hr[b] + hw[b];
+      }
     }
     qd = quarter_sum(qd);
     kr = quarter_sum(kr);
@@ -1285,7 +1466,7 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
   float pq = 0.0f, pk = 0.0f;
 #pragma unroll
   for (int i = 0; i < KS; ++i) {
-    const f32x8 x = whole(sh.k.rows(w * KS + i)) * rk, y = whole(sh.q.rows(w * KS + i)) * rq;
+    const f32x8 x = own_row(a.K, i) * rk, y = own_row(a.Q, i) * rq;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       pq = fmaf(y[j], dq[2 * i + j / 4][j % 4], pq);
@@ -1300,14 +1481,30 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_grad(DeltaArgs a, DeltaBa
   T* const ok = (T*)o.dk + (bead * a.keys + kh) * a.dk;
 #pragma unroll
   for (int i = 0; i < KS; ++i) {
-    const f32x8 x = whole(sh.k.rows(w * KS + i)) * (rk * pk);
-    const f32x8 y = whole(sh.q.rows(w * KS + i)) * (rq * pq);
+    const f32x8 x = own_row(a.K, i) * (rk * pk), y = own_row(a.Q, i) * (rq * pq);
     const int el = 32 * i + 4 * g;
     store4<T>(oq, el, a.dk, (dq[2 * i] - half_of<0>(y)) * (a.scale * rq));
     store4<T>(oq, el + 16, a.dk, (dq[2 * i + 1] - half_of<1>(y)) * (a.scale * rq));
     store4<T>(ok, el, a.dk, (dk[2 * i] - half_of<0>(x)) * rk);
     store4<T>(ok, el + 16, a.dk, (dk[2 * i + 1] - half_of<1>(x)) * rk);
   }
+}
+
+constexpr size_t kDeltaLds = 160 * 1024;
+constexpr int kDeltaUnits = 256;  // compute units
+
+template <typename T, int DK, int KV, bool MANY>
+int grad_kernel(const DeltaArgs& a, const DeltaBack& o, hipStream_t s) {
+  typedef GradTiles<T, DK, KV> Tiles;
+  constexpr size_t small = sizeof(typename Tiles::Small);
+  const int places = Tiles::bytes(2) + small <= kDeltaLds ? 2 : 1;
+  const size_t bytes = Tiles::bytes(places) + small;
+  const auto f = delta_grad<T, DK, KV, MANY>;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(f),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+    return MLCG_ERR_LAUNCH;
+  hipLaunchKernelGGL(f, dim3(a.n_tiles, a.keys), dim3(kDeltaThreads), bytes, s, a, o, places);
+  return mlcg_launch_status();
 }
 
 // ---------------------------------------------------------------------------
@@ -1320,8 +1517,6 @@ inline bool lds_limit(const void* f, size_t bytes) {
 // Two buffers of a chunk in LDS where there is room for them and no more
 // workgroups than compute units: 2 x 4099 beads, 8 heads of 64 in bf16, segments of
 // 6 chunks, 89 us forward against 93; 48 x 268, 8 heads of 16 in fp32, 75 against 61.
-constexpr size_t kDeltaLds = 160 * 1024;
-constexpr int kDeltaUnits = 256;
 inline int scan_buffers(size_t bytes, int64_t groups) {
   return 2 * bytes <= kDeltaLds && groups <= kDeltaUnits ? 2 : 1;
 }
@@ -1382,22 +1577,27 @@ int backward_waves(const DeltaArgs& a, const DeltaBack& o, DeltaEnds e, float* w
   const auto scan = delta_scan_back<T, DK, WAVES, false>;
   if (!lds_limit(reinterpret_cast<const void*>(scan), buffers * bytes)) return MLCG_ERR_LAUNCH;
   hipLaunchKernelGGL(scan, grid, block, buffers * bytes, s, a, o, e, buffers);
-  const auto grad = delta_grad<T, DK>;
-  const size_t glds = sizeof(GradTiles<T, DK>);
-  if (!lds_limit(reinterpret_cast<const void*>(grad), glds)) return MLCG_ERR_LAUNCH;
-  hipLaunchKernelGGL(grad, dim3(a.n_tiles, a.keys), dim3(kDeltaThreads), glds, s, a, o);
-  return mlcg_launch_status();
+  const int kv = a.dvp / 32;
+  if (a.group == 1)
+    return kv == 1   ? grad_kernel<T, DK, 1, false>(a, o, s)
+           : kv == 2 ? grad_kernel<T, DK, 2, false>(a, o, s)
+           : kv == 3 ? grad_kernel<T, DK, 3, false>(a, o, s)
+                     : grad_kernel<T, DK, 4, false>(a, o, s);
+  return kv == 1   ? grad_kernel<T, DK, 1, true>(a, o, s)
+         : kv == 2 ? grad_kernel<T, DK, 2, true>(a, o, s)
+         : kv == 3 ? grad_kernel<T, DK, 3, true>(a, o, s)
+                   : grad_kernel<T, DK, 4, true>(a, o, s);
 }
 
 template <typename T, int DK>
 int forward_dk(const DeltaArgs& a, T* out, const DeltaEnds& e, float* ws, hipStream_t s) {
-  return a.dv <= 64 ? forward_waves<T, DK, 4>(a, out, e, ws, s)
+  return a.dvp <= 64 ? forward_waves<T, DK, 4>(a, out, e, ws, s)
                     : forward_waves<T, DK, 8>(a, out, e, ws, s);
 }
 template <typename T, int DK>
 int backward_dk(const DeltaArgs& a, const DeltaBack& b, const DeltaEnds& e, float* ws,
                 hipStream_t s) {
-  return a.dv <= 64 ? backward_waves<T, DK, 4>(a, b, e, ws, s)
+  return a.dvp <= 64 ? backward_waves<T, DK, 4>(a, b, e, ws, s)
                     : backward_waves<T, DK, 8>(a, b, e, ws, s);
 }
 

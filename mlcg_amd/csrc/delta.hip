@@ -151,14 +151,14 @@ struct Parts {
   int64_t chunks() const { return fac + 2 * rows + 2 * mats + seg_map; }
 };
 Parts parts(int64_t tiles, int64_t segs, int heads, int keys, int dk, int dv, int dtype) {
-  const int64_t DK = delta_dk(dk), dvp = (dv + 15) / 16 * 16;
+  const int64_t DK = delta_dk(dk), dvp = (dv + 31) / 32 * 32;
   const int64_t in = dtype == MLCG_DTYPE_F32 ? 3 : dtype == MLCG_DTYPE_F16 ? 2 : 1;
   const int64_t mid = dtype == MLCG_DTYPE_F32 ? 3 : 2;
   return Parts{tiles * heads * (kDeltaFactors * kDeltaRows),
                tiles * keys * in * (DK / 8) * 256,
                tiles * heads * mid * kDeltaLower * 256,
-               tiles * heads * kDeltaRows * dvp,
-               tiles * heads * DK * dvp,
+               tiles * heads * mid * (dvp / 8) * 256,
+               tiles * heads * mid * (dvp / 16) * (DK / 32) * 256,
                segs * heads * DK * dvp,
                segs * heads * mid * (DK * DK / 2)};
 }
@@ -202,8 +202,8 @@ void place(DeltaArgs& a, DeltaEnds& e, float* kept, const Parts& p, bool train, 
   at += 2 * p.mats;
   e.seg_map = split ? reinterpret_cast<float4*>(at) : nullptr;
   at += p.seg_map;
-  a.U = train ? at : nullptr;
-  a.S0 = train ? at + p.u : nullptr;
+  a.U = train ? reinterpret_cast<float4*>(at) : nullptr;
+  a.S0 = train ? reinterpret_cast<float4*>(at + p.u) : nullptr;
 }
 
 }  // namespace
@@ -221,7 +221,7 @@ extern "C" int mlcg_gated_delta(
                n_segments < (int64_t(1) << 31) && n_whole >= 0 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
-              (dv + 15) / 16 * 16, scale, normalize, reverse,
+              (dv + 31) / 32 * 32, scale, normalize, reverse,
               reinterpret_cast<const int4*>(tiles), (int)n_tiles,
               reinterpret_cast<const int4*>(segments), segment_first, (int)n_segments,
               (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
@@ -256,7 +256,7 @@ extern "C" int mlcg_gated_delta_backward(
                n_segments < (int64_t(1) << 31) && n_whole >= 1 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
-              (dv + 15) / 16 * 16, scale, normalize, reverse,
+              (dv + 31) / 32 * 32, scale, normalize, reverse,
               reinterpret_cast<const int4*>(tiles), (int)n_tiles,
               reinterpret_cast<const int4*>(segments), segment_first, (int)n_segments,
               (int)n_whole, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
@@ -270,7 +270,7 @@ extern "C" int mlcg_gated_delta_backward(
   place(a, e, const_cast<float*>(kept), p, true, split);
   float* at = workspace;
   const DeltaBack b{grad_out, grad_q, grad_k, grad_v, grad_decay, grad_beta,
-                    grad_state, at, at + p.s0};
+                    grad_state, reinterpret_cast<float4*>(at), reinterpret_cast<float4*>(at + p.s0)};
   at += p.s0 + p.u;
   if (split) e.seg_last = at;
   float* const init = split ? at + p.seg_state : nullptr;
