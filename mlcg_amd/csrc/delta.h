@@ -376,7 +376,8 @@ struct ChunkTiles {
 };
 
 template <typename T, int DK>
-__global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
+__global__ __launch_bounds__(kDeltaThreads, (sizeof(T) == 4 && DK == 128 ? 2 : 4)) void delta_chunk(
+    DeltaArgs a) {
   constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32, NB = 4 * KS;
   extern __shared__ __align__(16) unsigned char smem[];
   ChunkTiles<T, DK>& sh = *reinterpret_cast<ChunkTiles<T, DK>*>(smem);
@@ -389,6 +390,18 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
   const bool in = row < ch.n;
   const int64_t bead = ch.bead(min(row, ch.n - 1));
   const bool there = in && (!a.keep || a.keep[bead]);
+
+  // the first wave makes a head's gates: what they are made of is sent for early
+  const int64_t gate = ch.bead(min(lane, ch.n - 1));
+  const bool gated = lane < ch.n && (!a.keep || a.keep[gate]);
+  float dn = 0.0f, bn = 0.0f;
+  const auto send_gates = [&](int h) {
+    if (w == 0) {
+      dn = a.decay[gate * a.heads + h];
+      bn = a.beta[gate * a.heads + h];
+    }
+  };
+  send_gates(kh * a.group);
 
   // this wave's 16 beads, as columns
   Frag<NI> kb[KS], qb[KS];
@@ -452,11 +465,9 @@ __global__ __launch_bounds__(kDeltaThreads) void delta_chunk(DeltaArgs a) {
   for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
     const int64_t at = (int64_t)tile * a.heads + h;
     if (w == 0) {
-      const bool here = lane < ch.n && (!a.keep || a.keep[ch.bead(lane)]);
-      const int64_t x = ch.bead(min(lane, ch.n - 1)) * a.heads + h;
-      float d = a.decay[x], b = a.beta[x];
-      d = here ? d : 0.0f;
-      b = here ? b : 0.0f;
+      float d = gated ? dn : 0.0f;
+      const float b = gated ? bn : 0.0f;
+      if (h + 1 < (kh + 1) * a.group) send_gates(h + 1);
       if (d < -256.0f) d = -256.0f;  // e^g is 0 all the same, and -inf - -inf no number
       double G = (double)d * 1.4426950408889634;
 #pragma unroll
