@@ -3,8 +3,9 @@
 //
 // The rows' order by token (stable: rows of one token stay in order) comes from
 // a radix sort, 8 bits of the token a pass, of three kernels: how many of each
-// digit a block of rows has; where each block's begin, by an exclusive sum over
-// (digit, block); every row to its place, ranked in its block by ballots.
+// digit a block of rows has; for every digit, by a workgroup of its own, the
+// exclusive sum over the blocks; every row to its place, ranked in its block by
+// ballots, after the digits before it.
 //
 // The gradient: slabs of the ordered rows, a row's channels over 8 to 64 lanes.
 // Runs of one token that begin and end in a slab are done there; of a longer one
@@ -20,8 +21,7 @@ constexpr int kEmbThreads = 256;
 constexpr int kEmbWaves = kEmbThreads / MLCG_WAVE;
 constexpr int kSortItems = 8;                           // a lane
 constexpr int kSortRows = kEmbThreads * kSortItems;     // a block
-constexpr int kScanThreads = 1024;
-constexpr int kSlabRows = 32;
+constexpr int kEmbRows = 4;                             // rows of a lane in the look-up
 constexpr int kEmbMaxWidth = 8192;
 
 template <typename T>
@@ -55,21 +55,30 @@ __device__ __forceinline__ void store_row8(T* row, int el, int width, f32x8 x) {
   }
 }
 
-// A row over `lanes` lanes; a token outside the table gives zeros and a flag.
+// kEmbRows rows over `lanes` lanes; a token outside the table gives zeros and a flag.
 template <typename T>
 __global__ __launch_bounds__(kEmbThreads) void embedding_forward(
     const T* __restrict__ table, int rows, const int64_t* __restrict__ tokens, int64_t n, int width,
     int lanes, float scale, T* __restrict__ out, unsigned* __restrict__ flags) {
   const int per = kEmbThreads / lanes, l = threadIdx.x % lanes;
-  const int64_t i = (int64_t)blockIdx.x * per + threadIdx.x / lanes;
-  if (i >= n) return;
-  const int64_t tok = tokens[i];
-  const bool bad = tok < 0 || tok >= rows;
+  const int64_t i0 = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * kEmbRows;
+  int64_t tok[kEmbRows];
+  bool ok[kEmbRows], bad = false;
+#pragma unroll
+  for (int r = 0; r < kEmbRows; ++r) {
+    tok[r] = i0 + r < n ? tokens[i0 + r] : 0;
+    ok[r] = tok[r] >= 0 && tok[r] < rows;
+    bad = bad || !ok[r];
+    if (!ok[r]) tok[r] = 0;
+  }
   if (bad && l == 0) atomicOr(flags, kFlagTypeRange);
   for (int el = 8 * l; el < width; el += 8 * lanes) {
-    f32x8 x{};
-    if (!bad) x = load_row8<T>(table + tok * width, el, width) * scale;
-    store_row8<T>(out + i * width, el, width, x);
+    f32x8 x[kEmbRows];
+#pragma unroll
+    for (int r = 0; r < kEmbRows; ++r) x[r] = load_row8<T>(table + tok[r] * width, el, width);
+#pragma unroll
+    for (int r = 0; r < kEmbRows; ++r)
+      if (i0 + r < n) store_row8<T>(out + (i0 + r) * width, el, width, ok[r] ? x[r] * scale : f32x8{});
   }
 }
 
@@ -107,18 +116,20 @@ __global__ __launch_bounds__(kEmbThreads) void sort_count(const int64_t* __restr
   counts[(int64_t)threadIdx.x * blocks + blockIdx.x] = hist[threadIdx.x];
 }
 
-// exclusive sum of m counts in place, by one workgroup
-__global__ __launch_bounds__(kScanThreads) void sort_scan(int* __restrict__ counts, int64_t m) {
-  __shared__ int sums[kScanThreads / MLCG_WAVE];
+// The exclusive sum of a digit's counts over the blocks, in place, and its total.
+__global__ __launch_bounds__(kEmbThreads) void sort_scan(int* __restrict__ counts, int blocks,
+                                                         int* __restrict__ totals) {
+  __shared__ int sums[kEmbWaves];
   constexpr int kItems = 4;
+  int* const row = counts + (int64_t)blockIdx.x * blocks;
   int carry = 0;
   const int l = mlcg_lane(), w = threadIdx.x / MLCG_WAVE;
-  for (int64_t b = 0; b < m; b += kScanThreads * kItems) {
+  for (int b = 0; b < blocks; b += kEmbThreads * kItems) {
     int v[kItems], own = 0;
-    const int64_t at = b + (int64_t)threadIdx.x * kItems;
+    const int at = b + threadIdx.x * kItems;
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
-      v[j] = at + j < m ? counts[at + j] : 0;
+      v[j] = at + j < blocks ? row[at + j] : 0;
       own += v[j];
     }
     int s = own;
@@ -129,28 +140,30 @@ __global__ __launch_bounds__(kScanThreads) void sort_scan(int* __restrict__ coun
     }
     if (l == MLCG_WAVE - 1) sums[w] = s;
     __syncthreads();
-    int before = carry, total = 0;
-    for (int j = 0; j < kScanThreads / MLCG_WAVE; ++j) {
+    int before = carry + s - own;
+#pragma unroll
+    for (int j = 0; j < kEmbWaves; ++j) {
       if (j < w) before += sums[j];
-      total += sums[j];
+      carry += sums[j];
     }
-    before += s - own;
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
-      if (at + j < m) counts[at + j] = before;
+      if (at + j < blocks) row[at + j] = before;
       before += v[j];
     }
-    carry += total;
     __syncthreads();
   }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
 // A wave has kSortItems x 64 rows in a row.
 __global__ __launch_bounds__(kEmbThreads) void sort_place(
     const int64_t* __restrict__ tokens, const int* __restrict__ keys,
     const int* __restrict__ index, int64_t n, int rows, int shift, int blocks,
-    const int* __restrict__ counts, int* __restrict__ keys_out, int* __restrict__ index_out) {
+    const int* __restrict__ counts, const int* __restrict__ totals, int* __restrict__ keys_out,
+    int* __restrict__ index_out) {
   __shared__ int seen[kEmbWaves][256];
+  __shared__ int sums[kEmbWaves];
   const int l = mlcg_lane(), w = threadIdx.x / MLCG_WAVE;
   for (int i = l; i < 256; i += MLCG_WAVE) seen[w][i] = 0;
   const uint64_t below = l == 0 ? 0ull : ~0ull >> (MLCG_WAVE - l);
@@ -179,9 +192,21 @@ __global__ __launch_bounds__(kEmbThreads) void sort_place(
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     rank[j] = before + __popcll(same & below);
   }
+  // rows of the digits before this thread's
+  const int own = totals[threadIdx.x];
+  int s = own;
+#pragma unroll
+  for (int o = 1; o < MLCG_WAVE; o <<= 1) {
+    const int up = __shfl_up(s, o, MLCG_WAVE);
+    if (l >= o) s += up;
+  }
+  if (l == MLCG_WAVE - 1) sums[w] = s;
   __syncthreads();
   {
-    int at = counts[(int64_t)threadIdx.x * blocks + blockIdx.x];
+    int at = counts[(int64_t)threadIdx.x * blocks + blockIdx.x] + s - own;
+#pragma unroll
+    for (int v = 0; v < kEmbWaves; ++v)
+      if (v < w) at += sums[v];
 #pragma unroll
     for (int v = 0; v < kEmbWaves; ++v) {
       const int c = seen[v][threadIdx.x];
@@ -216,46 +241,49 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_zero(T* __restrict__ ou
 
 // A slab's rows over `lanes` lanes and, on the grid's second axis, 8 lanes
 // channels each.  head[slab]: the sum of the rows of the run that comes from
-// before; tail[slab]: of the run that goes on behind and begins here.
-template <typename T>
+// before; tail[slab]: of the run that goes on behind and begins here.  The slabs'
+// keys and rows come to LDS first, so that the loads of rows wait for none.
+template <typename T, int SLAB>
 __global__ __launch_bounds__(kEmbThreads) void embedding_slab(
     const T* __restrict__ grad, const int* __restrict__ keys, const int* __restrict__ index,
     int64_t n, int rows, int width, int lanes, float scale, T* __restrict__ out,
     float* __restrict__ head, float* __restrict__ tail) {
-  const int per = kEmbThreads / lanes, l = threadIdx.x % lanes;
-  const int64_t slab = (int64_t)blockIdx.x * per + threadIdx.x / lanes;
-  const int64_t begin = slab * kSlabRows;
+  constexpr int kBatch = 8, kMost = kEmbThreads / 8 * SLAB;
+  __shared__ int key_of[kMost + 1], row_of[kMost];
+  const int per = kEmbThreads / lanes, l = threadIdx.x % lanes, p = threadIdx.x / lanes;
+  const int64_t base = (int64_t)blockIdx.x * per * SLAB;
+  for (int i = threadIdx.x; i <= per * SLAB; i += kEmbThreads) {
+    key_of[i] = base + i < n ? keys[base + i] : -1;
+    if (i < per * SLAB) row_of[i] = base + i < n ? index[base + i] : 0;
+  }
+  __syncthreads();
+  const int64_t slab = (int64_t)blockIdx.x * per + p, begin = slab * SLAB;
   const int el = 8 * (blockIdx.y * lanes + l);
   if (begin >= n || el >= width) return;
-  const int count = (int)min((int64_t)kSlabRows, n - begin);
-  const int before = begin > 0 ? keys[begin - 1] : -1;
-  const int after = begin + count < n ? keys[begin + count] : -1;
+  const int count = (int)min((int64_t)SLAB, n - begin);
+  const int* const key = key_of + p * SLAB;
+  const int* const row = row_of + p * SLAB;
+  // the run comes from the slab before
+  bool first = begin > 0 && keys[begin - 1] == key[0];
   f32x8 s{};
-  bool first = keys[begin] == before;  // the run comes from the slab before
-  constexpr int kBatch = 8;
   for (int r0 = 0; r0 < count; r0 += kBatch) {
-    int key[kBatch + 1];
     f32x8 x[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int64_t at = begin + min(r0 + j, count - 1);
-      key[j] = keys[at];
-      x[j] = load_row8<T>(grad + (int64_t)index[at] * width, el, width);
-    }
-    key[kBatch] = r0 + kBatch < count ? keys[begin + r0 + kBatch] : after;
+    for (int j = 0; j < kBatch; ++j)
+      x[j] = load_row8<T>(grad + (int64_t)row[min(r0 + j, count - 1)] * width, el, width);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (r0 + j >= count) break;
       s += x[j];
-      const int next = r0 + j + 1 < count ? key[j + 1] : after;
+      const int k = key[r0 + j], next = key[r0 + j + 1];  // -1 behind the last row
       const bool last = r0 + j + 1 == count;
-      if (key[j] == next && !last) continue;
+      if (k == next && !last) continue;
       if (first) {
         store_row8<float>(head + slab * width, el, width, s);
-      } else if (key[j] == next) {
+      } else if (k == next) {
         store_row8<float>(tail + slab * width, el, width, s);
-      } else if (key[j] < rows) {
-        store_row8<T>(out + (int64_t)key[j] * width, el, width, s * scale);
+      } else if (k < rows) {
+        store_row8<T>(out + (int64_t)k * width, el, width, s * scale);
       }
       first = false;
       s = f32x8{};
@@ -264,17 +292,17 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_slab(
 }
 
 // Runs over several slabs: the workgroup of the slab that one begins in.
-template <typename T>
+template <typename T, int SLAB>
 __global__ __launch_bounds__(kEmbThreads) void embedding_join(
     const int* __restrict__ keys, int64_t n, int rows, int width, int lanes, float scale,
     const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ out) {
-  const int64_t slab = blockIdx.x, slabs = (n + kSlabRows - 1) / kSlabRows;
-  const int64_t end = slab * kSlabRows + kSlabRows;
+  const int64_t slab = blockIdx.x, slabs = (n + SLAB - 1) / SLAB;
+  const int64_t end = slab * SLAB + SLAB;
   if (end >= n) return;
   const int key = keys[end - 1];
   if (key >= rows || keys[end] != key) return;  // ends here
   // begins here, not before this slab
-  const int64_t begin = slab * kSlabRows;
+  const int64_t begin = slab * SLAB;
   if (begin > 0 && keys[begin] == key && keys[begin - 1] == key) return;
   __shared__ int stop;
   __shared__ float sum[kEmbThreads * 8];
@@ -283,7 +311,7 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_join(
     if (threadIdx.x == 0) stop = kEmbThreads;
     __syncthreads();
     const int64_t s = s0 + threadIdx.x;
-    if (s >= slabs || keys[s * kSlabRows] != key) atomicMin(&stop, (int)threadIdx.x);
+    if (s >= slabs || keys[s * SLAB] != key) atomicMin(&stop, (int)threadIdx.x);
     __syncthreads();
     const int more = stop;
     __syncthreads();
@@ -329,30 +357,43 @@ template <typename T>
 int emb_forward(const void* table, int rows, const int64_t* tokens, int64_t n, int width,
                 float scale, void* out, unsigned* flags, hipStream_t s) {
   const int lanes = emb_lanes(width);
-  hipLaunchKernelGGL((embedding_forward<T>), dim3(mlcg_div_up(n, kEmbThreads / lanes)),
+  hipLaunchKernelGGL((embedding_forward<T>), dim3(mlcg_div_up(n, kEmbThreads / lanes * kEmbRows)),
                      dim3(kEmbThreads), 0, s, (const T*)table, rows, tokens, n, width, lanes, scale,
                      (T*)out, flags);
+  return mlcg_launch_status();
+}
+
+// Rows of a slab: long ones leave less to be joined, short ones more to do at the
+// same time.  548864 rows of 256 channels in bf16, 8000 tokens, slabs and joins
+// LONGTIMES; 17920 rows of 128 in fp32, 25 tokens, SHORTTIMES.
+int slab_rows(int64_t n) { return n >= (int64_t(1) << 17) ? 128 : 32; }
+
+template <typename T, int SLAB>
+int emb_sums(const void* grad, const int* keys, const int* index, int64_t n, int rows, int width,
+             float scale, void* out, float* ws, hipStream_t s) {
+  const int lanes = emb_lanes(width);
+  const int64_t slabs = (n + SLAB - 1) / SLAB;
+  const unsigned parts = mlcg_div_up(width, 8 * lanes);
+  float *head = ws, *tail = ws + slabs * width;
+  hipLaunchKernelGGL((embedding_slab<T, SLAB>), dim3(mlcg_div_up(slabs, kEmbThreads / lanes), parts),
+                     dim3(kEmbThreads), 0, s, (const T*)grad, keys, index, n, rows, width, lanes,
+                     scale, (T*)out, head, tail);
+  hipLaunchKernelGGL((embedding_join<T, SLAB>), dim3((unsigned)slabs, parts), dim3(kEmbThreads), 0, s,
+                     keys, n, rows, width, lanes, scale, head, tail, (T*)out);
   return mlcg_launch_status();
 }
 
 template <typename T>
 int emb_backward(const void* grad, const int* keys, const int* index, int64_t n, int rows,
                  int width, float scale, void* out, float* ws, hipStream_t s) {
-  const int lanes = emb_lanes(width);
-  const int64_t slabs = (n + kSlabRows - 1) / kSlabRows, total = (int64_t)rows * width;
-  const unsigned parts = mlcg_div_up(width, 8 * lanes);
+  const int64_t total = (int64_t)rows * width;
   hipLaunchKernelGGL((embedding_zero<T>),
                      dim3(mlcg_persistent_groups(mlcg_div_up(total, 16 * kEmbThreads), 8)),
                      dim3(kEmbThreads), 0, s, (T*)out, total);
-  if (n > 0) {
-    float *head = ws, *tail = ws + slabs * width;
-    hipLaunchKernelGGL((embedding_slab<T>), dim3(mlcg_div_up(slabs, kEmbThreads / lanes), parts),
-                       dim3(kEmbThreads), 0, s, (const T*)grad, keys, index, n, rows, width, lanes,
-                       scale, (T*)out, head, tail);
-    hipLaunchKernelGGL((embedding_join<T>), dim3((unsigned)slabs, parts), dim3(kEmbThreads), 0, s,
-                       keys, n, rows, width, lanes, scale, head, tail, (T*)out);
-  }
-  return mlcg_launch_status();
+  if (n == 0) return mlcg_launch_status();
+  return slab_rows(n) == 32
+             ? emb_sums<T, 32>(grad, keys, index, n, rows, width, scale, out, ws, s)
+             : emb_sums<T, 128>(grad, keys, index, n, rows, width, scale, out, ws, s);
 }
 
 bool emb_ok(int64_t rows, int64_t n, int width) {
@@ -384,7 +425,7 @@ extern "C" int mlcg_scaled_embedding(const void* table, int64_t rows, const int6
 
 extern "C" int64_t mlcg_token_order_workspace_ints(int64_t n, int64_t rows) {
   if (!emb_ok(rows, n, 1)) return -1;
-  return 2 * n + 256 * ((n + kSortRows - 1) / kSortRows);
+  return 2 * n + 256 + 256 * ((n + kSortRows - 1) / kSortRows);
 }
 
 extern "C" int mlcg_token_order(const int64_t* tokens, int64_t n, int64_t rows, int* keys,
@@ -400,16 +441,17 @@ extern "C" int mlcg_token_order(const int64_t* tokens, int64_t n, int64_t rows, 
   int bits = 1;  // of the largest key, `rows`
   while ((rows >> bits) != 0) ++bits;
   const int passes = (bits + 7) / 8;
-  int *keys2 = workspace, *index2 = workspace + n, *counts = workspace + 2 * n;
+  int *keys2 = workspace, *index2 = workspace + n, *totals = workspace + 2 * n;
+  int* const counts = totals + 256;
   const int *kin = nullptr, *iin = nullptr;
   for (int p = 0; p < passes; ++p) {
     const bool here = (passes - 1 - p) % 2 == 0;  // the last pass ends in the outputs
     int *ko = here ? keys : keys2, *io = here ? index : index2;
     hipLaunchKernelGGL(sort_count, dim3(blocks), dim3(kEmbThreads), 0, s, tokens, kin, n,
                        (int)rows, 8 * p, blocks, counts, flags);
-    hipLaunchKernelGGL(sort_scan, dim3(1), dim3(kScanThreads), 0, s, counts, (int64_t)256 * blocks);
+    hipLaunchKernelGGL(sort_scan, dim3(256), dim3(kEmbThreads), 0, s, counts, blocks, totals);
     hipLaunchKernelGGL(sort_place, dim3(blocks), dim3(kEmbThreads), 0, s, tokens, kin, iin, n,
-                       (int)rows, 8 * p, blocks, counts, ko, io);
+                       (int)rows, 8 * p, blocks, counts, totals, ko, io);
     kin = ko;
     iin = io;
   }
@@ -418,7 +460,8 @@ extern "C" int mlcg_token_order(const int64_t* tokens, int64_t n, int64_t rows, 
 
 extern "C" int64_t mlcg_scaled_embedding_workspace_floats(int64_t n, int width) {
   if (!emb_ok(1, n, width)) return -1;
-  return 2 * ((n + kSlabRows - 1) / kSlabRows) * width;
+  const int slab = slab_rows(n);
+  return 2 * ((n + slab - 1) / slab) * width;
 }
 
 extern "C" int mlcg_scaled_embedding_backward(const void* grad, const int* keys, const int* index,
