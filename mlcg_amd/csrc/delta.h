@@ -236,23 +236,66 @@ struct Image {
       f.p[i] = __builtin_bit_cast(bf16x8, x[(i * NB + block) * 64 + slot()]);
     return f;
   }
-  // the transpose of blocks b0 and b1 (32 rows): columns 16 HALF .. of them
-  template <int HALF>
-  __device__ __forceinline__ Frag<N> columns(int b0, int b1) const {
-    // 16 lanes give the places of 4 rows x 16 columns, lane i those of row
-    // i / 4, and get a column's 4 rows each
+  // The transposes of blocks b0 and b1 (32 rows), as left operands: columns 0 .. 15
+  // and 16 .. 31 of them, and with c0 and c1 those of a second pair.  16 lanes give
+  // the places of 4 rows x 16 columns, lane i those of row i / 4, and get a column's
+  // 4 rows each.  The reads and their wait are one piece of assembly: before its own
+  // form of this read (columns_now) the compiler waits for everything that is on its
+  // way from memory, the next chunk, too; but that leaves it more freedom, and
+  // delta_grad, whose registers are short, is faster with it (2 x 4099, 8 heads of 64
+  // on 4, 51 us against 59).
+  __device__ __forceinline__ lds_s16x4* column_place(int piece, int block) const {
     const int lane = mlcg_lane(), s = lane & 3, r = 4 * (lane >> 4) + ((lane & 15) >> 2);
-    const int at = 16 * s + (r ^ (8 * (s >> 1)));
-    Frag<N> f;
+    return (lds_s16x4*)&x[(piece * NB + block) * 64 + 16 * s + (r ^ (8 * (s >> 1)))];
+  }
+  __device__ __forceinline__ void columns_now(int b0, int b1, Frag<N> (&f)[2]) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const char* const p0 = reinterpret_cast<const char*>(&x[(i * NB + b0) * 64 + at]);
-      const char* const p1 = reinterpret_cast<const char*>(&x[(i * NB + b1) * 64 + at]);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0 + 8 * HALF));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p1 + 8 * HALF));
-      f.p[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      lds_s16x4 *const p0 = column_place(i, b0), *const p1 = column_place(i, b1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        f[j].p[i] = joined(__builtin_amdgcn_ds_read_tr16_b64_v4i16(p0 + j),
+                           __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1 + j));
     }
-    return f;
+  }
+  __device__ static __forceinline__ bf16x8 joined(s16x4 lo, s16x4 hi) {
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  __device__ __forceinline__ void columns(int b0, int b1, Frag<N> (&f)[2]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s16x4 r0, r1, r2, r3;
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\t"
+          "ds_read_b64_tr_b16 %2, %4 offset:8\n\tds_read_b64_tr_b16 %3, %5 offset:8\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+          : "v"(column_place(i, b0)), "v"(column_place(i, b1))
+          : "memory");
+      f[0].p[i] = joined(r0, r1);
+      f[1].p[i] = joined(r2, r3);
+    }
+  }
+  __device__ __forceinline__ void columns(int b0, int b1, int c0, int c1, Frag<N> (&f)[2],
+                                          Frag<N> (&g)[2]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s16x4 r0, r1, r2, r3, q0, q1, q2, q3;
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\t"
+          "ds_read_b64_tr_b16 %2, %8 offset:8\n\tds_read_b64_tr_b16 %3, %9 offset:8\n\t"
+          "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %11\n\t"
+          "ds_read_b64_tr_b16 %6, %10 offset:8\n\tds_read_b64_tr_b16 %7, %11 offset:8\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(q0), "=&v"(q1), "=&v"(q2), "=&v"(q3)
+          : "v"(column_place(i, b0)), "v"(column_place(i, b1)), "v"(column_place(i, c0)),
+            "v"(column_place(i, c1))
+          : "memory");
+      f[0].p[i] = joined(r0, r1);
+      f[1].p[i] = joined(r2, r3);
+      g[0].p[i] = joined(q0, q1);
+      g[1].p[i] = joined(q2, q3);
+    }
   }
 };
 
@@ -749,16 +792,20 @@ __device__ __forceinline__ void columns_product(f32x4 (&s)[B], const Image<N, NB
   constexpr int KS = B / 2;
 #pragma unroll
   for (int b = 0; b < B; b += 2) {
-    Frag<N> f[2][R];
+    Frag<N> f[R][2];
+    const int b0 = b / 2;
+    if constexpr (R == 1) {
+      t.columns(b0, KS + b0, f[0]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      f[0][i] = t.template columns<0>(2 * i * KS + b / 2, (2 * i + 1) * KS + b / 2);
-      f[1][i] = t.template columns<1>(2 * i * KS + b / 2, (2 * i + 1) * KS + b / 2);
+      for (int i = 0; i < R; i += 2)
+        t.columns(2 * i * KS + b0, (2 * i + 1) * KS + b0, (2 * i + 2) * KS + b0,
+                  (2 * i + 3) * KS + b0, f[i], f[i + 1]);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) mma(s[b + j], f[j][i], x[i]);
+      for (int j = 0; j < 2; ++j) mma(s[b + j], f[i][j], x[i]);
   }
 }
 // The blocks (b, i) of a lower triangle are 0 0, 1 0, 2 0, 2 1, 3 0, 3 1.
@@ -784,23 +831,21 @@ __device__ __forceinline__ void lower_product(f32x4 (&y)[4], const Image<N, kDel
 template <bool FLIP, int N, int M>
 __device__ __forceinline__ void upper_product(f32x4 (&y)[4], const Image<N, kDeltaLower>& t,
                                               const Frag<M> (&x)[2]) {
-  Frag<N> f[4][2];
+  Frag<N> f[2][2], g[2];  // rows 0 .. 31's columns 0 .. 31; rows 32 .. 63's 0 .. 31, 32 .. 63
+  t.columns(lower(0, 0), lower(1, 0), lower(2, 0), lower(3, 0), f[0], f[1]);
+  t.columns(lower(2, 1), lower(3, 1), g);
+  const auto product = [&](int b, const Frag<N>& l, const Frag<M>& r) {
+    if (FLIP)
+      mma(y[b], r, l);
+    else
+      mma(y[b], l, r);
+  };
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int b = 0; b < 2 * i + 2; b += 2) {
-      f[b][i] = t.template columns<0>(lower(2 * i, b / 2), lower(2 * i + 1, b / 2));
-      f[b + 1][i] = t.template columns<1>(lower(2 * i, b / 2), lower(2 * i + 1, b / 2));
-    }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int b = 0; b < 2 * i + 2; ++b) {
-      if (FLIP)
-        mma(y[b], x[i], f[b][i]);
-      else
-        mma(y[b], f[b][i], x[i]);
-    }
+  for (int b = 0; b < 2; ++b) {
+    product(b, f[0][b], x[0]);
+    product(b, f[1][b], x[1]);
+    product(b + 2, g[b], x[1]);
+  }
 }
 // the 16 B rows of a wave's columns as right operands
 template <int N, int B>
@@ -951,51 +996,66 @@ __global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan(
 }
 
 // The states before the segments of a chain, one after the other: S <- M S + N.
-// Backward: after them, the last one first, S <- M^T S + N.
+// Backward: after them, the last one first, S <- M^T S + N.  Bound by the latency of
+// memory: the maps, in three buffers, and N are sent for two steps ahead (with one
+// buffer, the widest maps in fp32, one).  What a wave sends arrives in order, so that
+// its part of a map is there when the N sent for behind it is.
 template <typename T, int DK, int WAVES, bool BACK>
 __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds e,
                                                          float* seg_init, int buffers) {
   constexpr int NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   typedef Image<NM, B * KS> Map;
   extern __shared__ __align__(16) unsigned char smem[];
-  Map* const maps = reinterpret_cast<Map*>(smem);  // one, or two in turn
+  Map* const maps = reinterpret_cast<Map*>(smem);
   const int h = blockIdx.y, c = mlcg_lane() & 15, v0 = 16 * wave_number();
   const bool live = v0 < a.dvp;
   const int first = uniform(a.seg_first[blockIdx.x]);
   const int n = uniform(a.seg_first[blockIdx.x + 1]) - first;
   const int chain = uniform(a.segs[first]).x;
-  f32x4 S[B], next[B];
+  f32x4 S[B], even[B], odd[B];
   load_state<B>(S, e.init + ((int64_t)chain * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
                 a.dk, e.init && v0 + c < a.dv);
-  const auto fetch = [&](int j) {
-    const int64_t at = (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
-    send_to_lds<Map::units, WAVES>(maps[j % buffers].x, e.seg_map + at * (Map::units * 64));
-    load_state<B>(next, e.seg_last + at * (DK * a.dvp) + v0, a.dvp, DK, live);
+  const auto seg_at = [&](int j) {
+    return (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
   };
-  if (n > 1) fetch(0);
-  for (int j = 0; j < n; ++j) {
-    const int64_t at = (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
-    wait_for_memory();
+  const auto fetch = [&](int j, f32x4 (&next)[B]) {
+    if (j + 1 >= n) return;  // nothing comes behind the last segment
+    const int64_t at = seg_at(j);
+    send_to_lds<Map::units, WAVES>(maps[j % buffers].x, e.seg_map + at * (Map::units * 64));
+    load_state<B>(next, e.seg_last + at * (DK * a.dvp) + (live ? v0 : 0), a.dvp, DK, true);
+  };
+  const auto step = [&](int j, f32x4 (&next)[B], f32x4 (&other)[B]) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) asm volatile("" : "+v"(next[b]));  // is there
     lds_barrier();
     Frag<NM> s[KS];
     split_rows<NM>(s, S);
-    if (live) store_padded<B>(S, seg_init + at * (DK * a.dvp) + v0, a.dvp);
-    if (j + 1 == n) break;
+    if (live) store_padded<B>(S, seg_init + seg_at(j) * (DK * a.dvp) + v0, a.dvp);
+    if (j + 1 >= n) return;
 #pragma unroll
     for (int b = 0; b < B; ++b) S[b] = next[b];
-    if (buffers == 2 && j + 2 < n) fetch(j + 1);
+    if (buffers > 1) fetch(j + 2, next);
+    const Map& m = maps[j % buffers];
     if (BACK) {
 #pragma unroll
       for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int i = 0; i < KS; ++i) mma(S[b], maps[j % buffers].rows(b * KS + i), s[i]);
+        for (int i = 0; i < KS; ++i) mma(S[b], m.rows(b * KS + i), s[i]);
     } else {
-      columns_product(S, maps[j % buffers], s);
+      columns_product(S, m, s);
     }
-    if (buffers == 1 && j + 2 < n) {
+    if (buffers == 1) {
       lds_barrier();
-      fetch(j + 1);
+      fetch(j + 1, other);
     }
+  };
+#pragma unroll
+  for (int b = 0; b < B; ++b) even[b] = odd[b] = f32x4{};
+  fetch(0, even);
+  if (buffers > 1) fetch(1, odd);
+  for (int j = 0; j < n; j += 2) {
+    step(j, even, odd);
+    if (j + 1 < n) step(j + 1, odd, even);
   }
 }
 
@@ -1336,11 +1396,13 @@ __global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delt
 #pragma unroll
           for (int b = 0; b < B; b += 2) {
             const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
-            const Frag<NI> k0 = K.template columns<0>(b0, b1), k1 = K.template columns<1>(b0, b1);
-            mma(hq[b], k0, of);
-            mma(hq[b + 1], k1, of);
-            mma(hr[b], k0, rf);
-            mma(hr[b + 1], k1, rf);
+            Frag<NI> k[2];
+            K.columns_now(b0, b1, k);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mma(hq[b + j], k[j], of);
+              mma(hr[b + j], k[j], rf);
+            }
           }
         }
         if (i >= w / 2) {
@@ -1351,12 +1413,14 @@ __global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delt
 #pragma unroll
           for (int b = 0; b < B; b += 2) {
             const int b0 = 2 * i * KS + b / 2, b1 = b0 + KS;
-            const Frag<NI> k0 = K.template columns<0>(b0, b1), k1 = K.template columns<1>(b0, b1);
-            const Frag<NI> q0 = Q.template columns<0>(b0, b1), q1 = Q.template columns<1>(b0, b1);
-            mma(hw[b], q0, of);
-            mma(hw[b + 1], q1, of);
-            mma(hw[b], k0, rf);
-            mma(hw[b + 1], k1, rf);
+            Frag<NI> k[2], q[2];
+            K.columns_now(b0, b1, k);
+            Q.columns_now(b0, b1, q);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mma(hw[b + j], q[j], of);
+              mma(hw[b + j], k[j], rf);
+            }
           }
         }
       }
@@ -1372,12 +1436,12 @@ __global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delt
 #pragma unroll
         for (int i = 0; i < KV; ++i) {
           const int b0 = 2 * i * KS + b / 2;
-          const Frag<NM> s0 = S.template columns<0>(b0, b0 + KS);
-          const Frag<NM> s1 = S.template columns<1>(b0, b0 + KS);
-          mma(q0, s0, gb[i]);
-          mma(r0, s0, rb[i]);
-          mma(q1, s1, gb[i]);
-          mma(r1, s1, rb[i]);
+          Frag<NM> s[2];
+          S.columns_now(b0, b0 + KS, s);
+          mma(q0, s[0], gb[i]);
+          mma(r0, s[0], rb[i]);
+          mma(q1, s[1], gb[i]);
+          mma(r1, s[1], rb[i]);
         }
         hq[b] += first * q0;
         hq[b + 1] += first * q1;
@@ -1410,8 +1474,10 @@ __global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delt
 #pragma unroll
         for (int i = 0; i < KV; ++i) {
           const int b0 = 2 * i * KS + b / 2;
-          mma(w0, D.template columns<0>(b0, b0 + KS), ub[i]);
-          mma(w1, D.template columns<1>(b0, b0 + KS), ub[i]);
+          Frag<NM> d[2];
+          D.columns_now(b0, b0 + KS, d);
+          mma(w0, d[0], ub[i]);
+          mma(w1, d[1], ub[i]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1536,7 +1602,7 @@ template <typename T, int DK, int WAVES, bool BACK>
 int join(const DeltaArgs& a, const DeltaEnds& e, float* ws, hipStream_t s) {
   const auto f = delta_join<T, DK, WAVES, BACK>;
   const size_t one = sizeof(Image<Pieces<T>::mid, DK * DK / 512>);
-  const int buffers = 2 * one <= kDeltaLds ? 2 : 1;
+  const int buffers = 3 * one <= kDeltaLds ? 3 : 1;
   if (!lds_limit(reinterpret_cast<const void*>(f), buffers * one)) return MLCG_ERR_LAUNCH;
   hipLaunchKernelGGL(f, dim3(a.n_whole, a.heads), dim3(64 * WAVES), buffers * one, s, a, e, ws,
                      buffers);
