@@ -35,9 +35,11 @@
 // The state, and all sums, are fp32.  Products are on the bf16 matrix
 // instructions with operands in pieces, x = x0 + x1 + ..., each the rounding
 // of what the ones before leave: one for bf16 arrays and two for fp16 (exact),
-// three for fp32 (2^-24); two for what is computed from 16-bit arrays (2^-17,
-// and bf16's range, so that gradients of any size keep their digits), three
-// from fp32.  Of the products of pieces those are taken that reach this far.
+// three for fp32 and for all that is computed (2^-24, and in bf16's range, so that
+// gradients of any size keep their digits).  Of the products of pieces those are
+// taken that reach this far.  Two pieces for what is computed from 16-bit arrays
+// would take a fifth to a third less time, but leave the states and the gradients
+// of decay and beta, which are fp32, 4e-6 to 1e-5 off.
 //
 // A result of the 16 x 16 x 32 instruction has 4 rows of one column in a lane,
 // which is half of what the next product wants of its right operand if its
@@ -129,8 +131,8 @@ typedef __attribute__((address_space(1))) const void global_void;
 
 // pieces of the arrays' elements and of what is computed from them
 template <typename T> struct Pieces;
-template <> struct Pieces<__bf16> { static constexpr int in = 1, mid = 2; };
-template <> struct Pieces<_Float16> { static constexpr int in = 2, mid = 2; };
+template <> struct Pieces<__bf16> { static constexpr int in = 1, mid = 3; };
+template <> struct Pieces<_Float16> { static constexpr int in = 2, mid = 3; };
 template <> struct Pieces<float> { static constexpr int in = 3, mid = 3; };
 
 template <int N>
@@ -625,7 +627,7 @@ __global__ __launch_bounds__(kDeltaThreads, (sizeof(T) == 4 && DK == 128 ? 2 : 4
 // waves a SIMD of the scans: the registers are held to what so many leave
 template <typename T, int DK>
 constexpr int scan_waves() {
-  return DK == 128 ? 1 : sizeof(T) == 2 ? 3 : 2;
+  return DK == 128 ? 1 : 2;
 }
 
 // what a chunk's step needs in LDS, the last two for outputs and backward
@@ -1192,7 +1194,7 @@ __global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan_
 // key head; a wave has 16 beads, as columns.
 
 // What a chunk's gradients need in LDS, one after the other in one or two places:
-// u, dr and do; k and q; S0; D.
+// u, dr (and do, in the other); k and q; S0; D.
 template <typename T, int DK, int KV>
 struct GradTiles {
   static constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid;
@@ -1200,12 +1202,15 @@ struct GradTiles {
   typedef Image<NI, 4 * KV> Given;             // the same of do
   typedef Image<NM, 2 * KV*(DK / 32)> State;   // dv x DK
   typedef Image<NI, DK / 8> Keys;              // 64 beads x DK
-  static constexpr size_t rows = 2 * sizeof(Rows) + sizeof(Given);
-  static constexpr size_t keys = 2 * sizeof(Keys);
+  static constexpr size_t rows = 2 * sizeof(Rows), keys = 2 * sizeof(Keys);
   static constexpr size_t even = rows > sizeof(State) ? rows : sizeof(State);
-  static constexpr size_t odd = keys > sizeof(State) ? keys : sizeof(State);
+  // k and q come to their place while do behind them is still read
+  static constexpr size_t behind = keys + sizeof(Given);
+  static constexpr size_t odd = behind > sizeof(State) ? behind : sizeof(State);
+  // in one place do lies behind u and dr
+  static constexpr size_t one = rows + sizeof(Given) > keys ? rows + sizeof(Given) : keys;
   static constexpr size_t bytes(int places) {
-    return places == 2 ? even + odd : even > odd ? even : odd;
+    return places == 2 ? even + odd : one > sizeof(State) ? one : sizeof(State);
   }
   struct Small {
     float fac[kDeltaFactors][kDeltaRows];
@@ -1277,7 +1282,7 @@ __global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delt
     if (h > kh * a.group) lds_barrier();  // what the last head left has been read
     Rows& U = *reinterpret_cast<Rows*>(even);
     Rows& R = *reinterpret_cast<Rows*>(even + sizeof(Rows));
-    Given& G = *reinterpret_cast<Given*>(even + 2 * sizeof(Rows));
+    Given& G = *reinterpret_cast<Given*>(places == 2 ? odd + Tiles::keys : even + Tiles::rows);
     send_to_lds<Rows::units, 4>(U.x, a.U + at * (Rows::units * 64));
     send_to_lds<Rows::units, 4>(R.x, o.dR + at * (Rows::units * 64));
     send_to_lds<2, 4>(reinterpret_cast<float4*>(sh.fac),

@@ -153,7 +153,7 @@ struct Parts {
 Parts parts(int64_t tiles, int64_t segs, int heads, int keys, int dk, int dv, int dtype) {
   const int64_t DK = delta_dk(dk), dvp = (dv + 31) / 32 * 32;
   const int64_t in = dtype == MLCG_DTYPE_F32 ? 3 : dtype == MLCG_DTYPE_F16 ? 2 : 1;
-  const int64_t mid = dtype == MLCG_DTYPE_F32 ? 3 : 2;
+  const int64_t mid = 3;  // pieces of what is computed
   return Parts{tiles * heads * (kDeltaFactors * kDeltaRows),
                tiles * keys * in * (DK / 8) * 256,
                tiles * heads * mid * kDeltaLower * 256,

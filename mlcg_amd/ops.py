@@ -2305,13 +2305,13 @@ class _DeltaPlan:
 
 def _delta_segment_tiles(chains: ChainLayout, heads: int) -> int:
     """Chunks of a segment, 0 for whole chains: the smallest of the times that
-    these come to, in microseconds.  A workgroup takes about 2.9 a chunk; two go at
-    a time on each of 256 compute units; segments are gone through twice, and
-    joining them takes about 1.2 each, one after the other, and two launches more.
-    Measured, forward and backward: 2 x 4099 beads, 8 heads of 64 in bf16, whole
-    207 and 280, segments of 4, 6, 8 and 16 chunks 89 and 169, 78 and 164, 85 and
-    169, 110 and 200; 64 x 1000, 4 heads of 32, whole 98 and 242, of 8 126 and 264;
-    1 x 120001, 8 heads of 64, whole 5914, of 16, 32 and 64 817, 704 and 730."""
+    these come to, in microseconds.  A workgroup takes about 4 a chunk; two go at a
+    time on each of 256 compute units; segments are gone through twice, and joining
+    them takes about 1.5 each, one after the other, and two launches more.  Measured,
+    forward and backward, in bf16: 2 x 4099 beads, 8 heads of 64, whole 284 and 429,
+    segments of 4, 6, 8 and 16 chunks 101 and 157, 93 and 152, 102 and 162, 136 and
+    222; 64 x 1000, 4 heads of 32, whole 112 and 186, of 8 131 and 219; 1 x 120001, 8
+    heads of 64, whole 8600, of 16 and 32 908 and 786 forward."""
     rows = chains.plans.get(("delta segment", heads))
     if rows is None:
         count = -(-np.asarray(chains.lengths, dtype=np.int64) // DELTA_ROWS)
@@ -2323,12 +2323,12 @@ def _delta_segment_tiles(chains: ChainLayout, heads: int) -> int:
             def rounds(groups):
                 return -(-groups * heads // 512)
 
-            best = 2.9 * longest * rounds(count.size)
+            best = 4.0 * longest * rounds(count.size)
             for step in (4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128):
                 if step >= longest:
                     break
                 segs = -(-count // step)
-                cost = 5.8 * step * rounds(int(segs.sum())) + 1.2 * int(segs.max()) + 12.0
+                cost = 8.0 * step * rounds(int(segs.sum())) + 1.5 * int(segs.max()) + 12.0
                 if cost < best:
                     best, rows = cost, step
         chains.plans[("delta segment", heads)] = rows
