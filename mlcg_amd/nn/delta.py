@@ -26,6 +26,17 @@ from .chain import CounterDropout, _needs_grad
 from .mlp import init_xavier_uniform
 
 
+def _once(backward):
+    """once_differentiable's refusal of second derivatives, entered only where they
+    are recorded: its wrapping takes about 5 us of a backward pass."""
+    recorded = once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return either
+
+
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, beta, state, chains, scale, keep, reverse, normalize):
@@ -37,7 +48,7 @@ class _GatedDelta(torch.autograd.Function):
         return out, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad, grad_last):
         if grad is None and grad_last is None:
             return (None,) * 11
@@ -73,14 +84,14 @@ class _RMSNormAdd(torch.autograd.Function):
         return y, t
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad, grad_t):
         t, weight, rstd = ctx.saved_tensors
         if grad is None and grad_t is None:
             return None, None, None, None
         if grad is None:
             grad = torch.zeros(t.shape, dtype=weight.dtype, device=t.device)
-        return (*ops.rms_norm_add_backward(grad, grad_t, t, weight, rstd), None)
+        return (*ops._rms_backward(grad, grad_t, t, weight, rstd), None)
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -91,10 +102,10 @@ class _RMSNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         x, weight, rstd = ctx.saved_tensors
-        dx, _, dw = ops.rms_norm_add_backward(grad, None, x, weight, rstd)
+        dx, _, dw = ops._rms_backward(grad, None, x, weight, rstd)
         return dx, dw, None
 
 
@@ -117,7 +128,7 @@ class _ScaledEmbedding(torch.autograd.Function):
         return ops.scaled_embedding(table, tokens, scale)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         tokens, = ctx.saved_tensors
         rows, scale = ctx.plan

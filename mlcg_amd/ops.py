@@ -9,6 +9,7 @@ torch's caching allocator and launches on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Tuple
@@ -2414,7 +2415,9 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.
     and head stride), decay (the factor's logarithm, at most 0 where states must
     not grow; -inf empties the state) and beta [S, H] in float32; scale defaults
     to 1 / sqrt(DK).  keep [S] bool: an absent bead (False) leaves the state as
-    it is, whatever its k, v, decay and beta hold; its q reads the state.  state
+    it is, whatever its k, v, decay and beta hold; its q reads the state.  A value
+    of a present bead that is no number spoils its chain's outputs from the start of
+    its chunk of 64 beads on, and the chain's gradients; no other chain's.  state
     [B, H, DK, DV] float32: where each chain begins (zeros by default); last is
     where it ends.  kept is what the backward pass takes (train=True)."""
     own = q.shape[-1], v.shape[-1]
@@ -2546,14 +2549,15 @@ def _rms_rows(t: torch.Tensor, width: int):
 def _rms_types(x, residual, weight):
     require_device(x, residual, weight)
     dt = _chain_dtype(x, "rms_norm_add")
-    _check(x.dim() == 2 and 1 <= x.shape[1] <= MAX_RMS_WIDTH and x.shape[0] < 2 ** 31,
-           lambda: f"x must be [rows, 1 .. {MAX_RMS_WIDTH} channels], got {tuple(x.shape)}")
-    _check(weight.shape == x.shape[1:] and weight.dtype == x.dtype and weight.device == x.device,
-           lambda: f"weight must be [{x.shape[1]}] {x.dtype} on {x.device}")
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    _check(len(shape) == 2 and 1 <= shape[1] <= MAX_RMS_WIDTH and shape[0] < 2 ** 31,
+           lambda: f"x must be [rows, 1 .. {MAX_RMS_WIDTH} channels], got {tuple(shape)}")
+    _check(weight.shape == shape[1:] and weight.dtype == dtype and weight.device == dev,
+           lambda: f"weight must be [{shape[1]}] {dtype} on {dev}")
     if residual is not None:
-        _check(residual.shape == x.shape and residual.device == x.device
-               and residual.dtype in (x.dtype, torch.float32),
-               lambda: f"residual must be {tuple(x.shape)} {x.dtype} or float32 on {x.device}, "
+        _check(residual.shape == shape and residual.device == dev
+               and residual.dtype in (dtype, torch.float32),
+               lambda: f"residual must be {tuple(shape)} {dtype} or float32 on {dev}, "
                        f"got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
     return dt
 
@@ -2597,19 +2601,33 @@ def rms_norm_add_backward(grad: torch.Tensor, grad_t: Optional[torch.Tensor], t:
     if grad_t is not None:
         _check(grad_t.shape == t.shape and grad_t.dtype == t.dtype and grad_t.device == dev,
                lambda: f"grad_t must be {tuple(t.shape)} {t.dtype} on {dev}")
+    return _rms_backward(grad, grad_t, t, weight, rstd.contiguous())
+
+
+@functools.lru_cache(maxsize=4096)
+def _rms_workspace(rows: int, width: int) -> int:
+    return int(_lib.load().mlcg_rms_norm_add_workspace_floats(rows, width))
+
+
+def _rms_backward(grad, grad_t, t, weight, rstd):
+    """rms_norm_add_backward of a forward pass's own arrays and of gradients whose
+    shapes, types and device autograd has made theirs: not checked again."""
+    n, width = t.shape
+    dev, dtype, t_dtype = t.device, grad.dtype, t.dtype
+    grad = grad.contiguous()
+    if grad_t is not None:
         grad_t = grad_t.contiguous()
-    grad, rstd = grad.contiguous(), rstd.contiguous()
     t, ld = _rms_rows(t, width)
-    dx = torch.empty(n, width, dtype=grad.dtype, device=dev)
-    dr = dx if t.dtype == grad.dtype else torch.empty(n, width, dtype=t.dtype, device=dev)
+    dx = torch.empty(n, width, dtype=dtype, device=dev)
+    dr = dx if t_dtype == dtype else torch.empty(n, width, dtype=t_dtype, device=dev)
     if n == 0:
         return dx, dr, torch.zeros_like(weight)
-    dw = torch.empty(width, dtype=weight.dtype, device=dev)
-    nws = int(_lib.load().mlcg_rms_norm_add_workspace_floats(n, width))
+    dw = torch.empty(width, dtype=dtype, device=dev)
+    nws = _rms_workspace(n, width)
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     call("mlcg_rms_norm_add_backward", ptr(grad), ptr(grad_t), ptr(t), ld,
-         ptr(weight.contiguous()), ptr(rstd), n, width, dt, DTYPE_IDS[t.dtype], ptr(dx),
-         None if dr is dx else ptr(dr), ptr(dw), ptr(ws), nws, stream_handle(dev))
+         ptr(weight.contiguous()), ptr(rstd), n, width, DTYPE_IDS[dtype], DTYPE_IDS[t_dtype],
+         ptr(dx), None if dr is dx else ptr(dr), ptr(dw), ptr(ws), nws, stream_handle(dev))
     return dx, dr, dw
 
 
