@@ -1,5 +1,6 @@
-// Helpers shared by the sequence encoder's kernels (attention.hip, norm.hip,
-// dropout.hip): element types, vectors of them and alignment.
+// Helpers shared by the sequence encoders' kernels (attention.hip, norm.hip,
+// dropout.hip, delta.h, rmsnorm.hip, embedding.hip): element types, vectors of
+// them and alignment.
 #pragma once
 
 #include "common.h"
@@ -15,6 +16,38 @@ using v4 = typename chain_vec<T>::v4;
 template <typename T>
 using v8 = typename chain_vec<T>::v8;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// 8 elements that are aligned as one, and 8 channels of a row from el on, in fp32
+template <typename T>
+struct loose8 {
+  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ f32x8 load_row8(const T* row, int el, int width) {
+  f32x8 x{};
+  if (el + 8 <= width) {
+    x = __builtin_convertvector(*reinterpret_cast<const typename loose8<T>::type*>(row + el),
+                                f32x8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (el + j < width) x[j] = (float)row[el + j];
+  }
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ void store_row8(T* row, int el, int width, f32x8 x) {
+  if (el + 8 <= width) {
+    *reinterpret_cast<typename loose8<T>::type*>(row + el) =
+        __builtin_convertvector(x, typename loose8<T>::type);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (el + j < width) row[el + j] = (T)x[j];
+  }
+}
 
 // true for NULL, too: an absent operand does not restrict the vector path
 static inline bool chain_aligned16(const void* p) {

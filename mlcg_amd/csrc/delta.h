@@ -123,7 +123,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
@@ -245,7 +244,8 @@ struct Image {
   // form of this read (columns_now) the compiler waits for everything that is on its
   // way from memory, the next chunk, too; but that leaves it more freedom, and
   // delta_grad, whose registers are short, is faster with it (2 x 4099, 8 heads of 64
-  // on 4, 51 us against 59).
+  // on 4 in bf16, 70 us against 76; 48 x 268, 8 heads of 16 in fp32, 37 against 41;
+  // 512 x 100, 8 heads of 32 in bf16, 71 against 67).
   __device__ __forceinline__ lds_s16x4* column_place(int piece, int block) const {
     const int lane = mlcg_lane(), s = lane & 3, r = 4 * (lane >> 4) + ((lane & 15) >> 2);
     return (lds_s16x4*)&x[(piece * NB + block) * 64 + 16 * s + (r ^ (8 * (s >> 1)))];
@@ -379,13 +379,7 @@ struct loose {
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
-// 8 and 4 elements of a row of len (a multiple of 8) from el on, zeros past its
-// end: without a branch, so that loads are not waited for one by one
-template <typename T>
-__device__ __forceinline__ v8<T> load8(const T* row, int el, int len) {
-  const v8<T> x = *reinterpret_cast<const typename loose<T, 8>::type*>(row + min(el, len - 8));
-  return el < len ? x : v8<T>{};
-}
+// 4 elements of a row of len (a multiple of 8) from el on, zeros past its end: without a branch, so that loads are not waited for one by one
 template <typename T>
 __device__ __forceinline__ v4<T> load4(const T* row, int el, int len) {
   const v4<T> x = *reinterpret_cast<const typename loose<T, 4>::type*>(row + min(el, len - 4));
@@ -1597,8 +1591,10 @@ inline bool lds_limit(const void* f, size_t bytes) {
 }
 
 // Two buffers of a chunk in LDS where there is room for them and no more
-// workgroups than compute units: 2 x 4099 beads, 8 heads of 64 in bf16, segments of
-// 6 chunks, 89 us forward against 93; 48 x 268, 8 heads of 16 in fp32, 75 against 61.
+// workgroups than compute units, which then have the LDS for one each.  Forward, 16 x
+// 500 beads, 8 heads of 64 in bf16: 53 us with two, 57 with one; 4 x 500: 46 and 50.
+// With more workgroups the scan alone, 512 x 100, 8 heads of 32: 68 and 50; 48 x 268,
+// 8 heads of 16 in fp32: 45 and 33.
 inline int scan_buffers(size_t bytes, int64_t groups) {
   return 2 * bytes <= kDeltaLds && groups <= kDeltaUnits ? 2 : 1;
 }

@@ -11,6 +11,13 @@
 // Runs of one token that begin and end in a slab are done there; of a longer one
 // every slab leaves its sum, which a workgroup at the run's first slab adds in
 // order.  No floating-point atomics: equal calls give equal bits.
+//
+// Both are bound by memory where there are many rows, by the latency of their
+// launches where there are few.  548864 rows of 256 channels in bf16, 8000 tokens:
+// the look-up 69 us (4.1 TB/s, nearly all of it written); the order 44 us in two
+// passes; the sums 121 us, of which the gradient's 281 MB are 58 at a copy's rate:
+// rows are read in the tokens' order, 512 bytes at a time.  17920 rows of 128 in
+// fp32, 25 tokens: 6 us, 14 us and 18 us.
 #include <type_traits>
 
 #include "chain.h"
@@ -23,37 +30,6 @@ constexpr int kSortItems = 8;                           // a lane
 constexpr int kSortRows = kEmbThreads * kSortItems;     // a block
 constexpr int kEmbRows = 4;                             // rows of a lane in the look-up
 constexpr int kEmbMaxWidth = 8192;
-
-template <typename T>
-struct loose8 {  // 8 elements that are aligned as one
-  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-};
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
-template <typename T>
-__device__ __forceinline__ f32x8 load_row8(const T* row, int el, int width) {
-  f32x8 x{};
-  if (el + 8 <= width) {
-    x = __builtin_convertvector(*reinterpret_cast<const typename loose8<T>::type*>(row + el),
-                                f32x8);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (el + j < width) x[j] = (float)row[el + j];
-  }
-  return x;
-}
-template <typename T>
-__device__ __forceinline__ void store_row8(T* row, int el, int width, f32x8 x) {
-  if (el + 8 <= width) {
-    *reinterpret_cast<typename loose8<T>::type*>(row + el) =
-        __builtin_convertvector(x, typename loose8<T>::type);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (el + j < width) row[el + j] = (T)x[j];
-  }
-}
 
 // kEmbRows rows over `lanes` lanes; a token outside the table gives zeros and a flag.
 template <typename T>
@@ -364,9 +340,10 @@ int emb_forward(const void* table, int rows, const int64_t* tokens, int64_t n, i
 }
 
 // Rows of a slab: long ones leave less to be joined, short ones more to do at the
-// same time.  548864 rows of 256 channels in bf16, 8000 tokens, slabs and joins
-// LONGTIMES; 17920 rows of 128 in fp32, 25 tokens, SHORTTIMES.
-int slab_rows(int64_t n) { return n >= (int64_t(1) << 17) ? 128 : 32; }
+// same time.  548864 rows of 256 channels in bf16, 8000 tokens, sums of the slabs
+// and their joins: 90 + 39 us with 32 rows, 88 + 33 with 64, 112 + 19 with 128.
+// 17920 rows of 128 in fp32, 25 tokens: 9.6 + 7.3, 16.0 + 6.3 and 28.0 + 5.7 us.
+int slab_rows(int64_t n) { return n >= (int64_t(1) << 17) ? 64 : 32; }
 
 template <typename T, int SLAB>
 int emb_sums(const void* grad, const int* keys, const int* index, int64_t n, int rows, int width,
@@ -393,7 +370,7 @@ int emb_backward(const void* grad, const int* keys, const int* index, int64_t n,
   if (n == 0) return mlcg_launch_status();
   return slab_rows(n) == 32
              ? emb_sums<T, 32>(grad, keys, index, n, rows, width, scale, out, ws, s)
-             : emb_sums<T, 128>(grad, keys, index, n, rows, width, scale, out, ws, s);
+             : emb_sums<T, 64>(grad, keys, index, n, rows, width, scale, out, ws, s);
 }
 
 bool emb_ok(int64_t rows, int64_t n, int width) {
