@@ -494,3 +494,75 @@ def test_other_stream():
     side.synchronize()
     for name, t in want.items():
         assert torch.equal(t, got[name]), name
+
+
+def test_other_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    from mlcg_amd import nn, ops
+
+    c = _case([5, 3], 4, 2, 16, 16, torch.float32, state=True, views=False)
+    names = ("q", "k", "v", "decay", "beta", "state")
+    for name in names:
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(c[name].clone(), torch.ones_like(c[name]))
+            args = dict({n: c[n] for n in names}, **{name: dual})
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                nn.gated_delta(chains=c["chains"], **args)
+        args = dict({n: c[n] for n in names}, **{name: c[name].clone().requires_grad_(True)})
+        out = nn.gated_delta(chains=c["chains"], **args)[0]
+        (d,) = torch.autograd.grad(out, args[name], torch.ones_like(out), create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.sum(), args[name])
+        with pytest.raises(RuntimeError, match="no gradients"):
+            ops.gated_delta_step(*[t[:8] for t in list(args.values())[:5]],
+                                 torch.zeros(8, 4, 16, 16, device="cuda",
+                                             requires_grad=name == "state"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_states_that_grow(dtype):
+    """Decays above zero: the rule as it is written, over one chunk."""
+    c = _case([64, 17], 2, 1, 32, 32, dtype, state=True)
+    c["decay"] = c["decay"].abs() / 8
+    _check(c)
+
+
+def test_elements_past_31_bits():
+    """Values, outputs, gradients and operands that lie past 2^31 elements: the last
+    chain's are those that it has alone."""
+    from mlcg_amd import ops
+
+    length, chains, heads = 101, 2600, 64  # 262600 beads x 64 heads x 128 > 2^31
+    n, g = length * chains, torch.Generator(device="cuda").manual_seed(3)
+    q, k = (torch.randn(n, 1, 32, device="cuda", generator=g).bfloat16() for _ in range(2))
+    v = torch.randn(n, heads, 128, device="cuda", dtype=torch.bfloat16, generator=g)
+    decay = -torch.rand(n, heads, device="cuda", generator=g)
+    beta = torch.rand(n, heads, device="cuda", generator=g)
+    results = []
+    for at, count in ((slice(0, n), chains), (slice(n - length, n), 1)):
+        args = [t[at] for t in (q, k, v, decay, beta)]
+        lay = ops.chain_layout([length] * count, "cuda")
+        out, last, kept = ops.gated_delta(*args, lay, train=True)
+        grads = ops.gated_delta_backward(*args, lay, kept, args[2], last)
+        results.append([t[-length:].clone() for t in (out, *grads[:5])] + [last[-1:].clone()])
+        del out, last, kept, grads
+    for name, a, b in zip(("out", "q", "k", "v", "decay", "beta", "last"), *results):
+        assert torch.equal(a, b), name
+
+
+def test_two_streams_at_once():
+    cases = [_case([300, 64, 1], 4, 2, 32, 32, torch.bfloat16, seed, state=True)
+             for seed in (0, 1)]
+    want = [_run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(_run(c))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for name in b:
+                assert torch.equal(a[name], b[name]), name

@@ -315,3 +315,105 @@ def test_recorded_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), i
+
+
+def test_other_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    from mlcg_amd import nn
+
+    tokens = torch.arange(6, device="cuda") % 4
+    w = torch.ones(16, device="cuda")
+    calls = [lambda t: nn.rms_norm_add(t, None, w)[0], lambda t: nn.rms_norm_add(w[None], t[:1], w)[0],
+             lambda t: nn.rms_norm_add(t, t * 2, w)[1], lambda t: nn.scaled_embedding(t, tokens, 2.0)]
+    for f in calls:
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.randn(4, 16, device="cuda"),
+                                        torch.randn(4, 16, device="cuda"))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f(dual)
+        leaf = torch.randn(4, 16, device="cuda", requires_grad=True)
+        out = f(leaf)
+        (d,) = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True,
+                                   allow_unused=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.sum(), leaf)
+
+
+def test_gradients_of_other_layouts():
+    """Gradients that autograd hands on as one number for all, or as a transpose."""
+    from mlcg_amd import nn
+
+    x, r, w, gy, gt = _rms_case(33, 40, torch.bfloat16, torch.float32)
+    table = torch.randn(5, 40, device="cuda")
+    tokens = torch.arange(33, device="cuda") % 5
+    for turn in (lambda g: torch.ones((), dtype=g.dtype, device="cuda").expand_as(g),
+                 lambda g: g.t().contiguous().t()):
+        grads = []
+        for how in (turn, lambda g: turn(g).contiguous()):
+            leaf = [t.detach().requires_grad_(True) for t in (x, r, w, table)]
+            y, t = nn.rms_norm_add(*leaf[:3])
+            e = nn.scaled_embedding(leaf[3], tokens, 3.0)
+            grads.append(torch.autograd.grad([y, t, e], leaf, [how(gy), how(gt), how(gt)]))
+        for a, b in zip(*grads):
+            assert torch.equal(a, b)
+
+
+def test_elements_past_31_bits():
+    """Rows whose elements lie past 2^31: their results are those of the rows alone
+    (of a row nothing depends on the others but the weight's gradient)."""
+    from mlcg_amd import ops
+
+    n, width = 2 ** 22 + 21, 512
+    x = torch.ones(n, width, dtype=torch.bfloat16, device="cuda")
+    last = slice(n - 21, n)
+    x[last].normal_()
+    w = torch.randn(width, device="cuda").bfloat16()
+    y, _, rstd = ops.rms_norm_add(x, None, w)
+    want = ops.rms_norm_add(x[last], None, w)
+    assert torch.equal(y[last], want[0]) and torch.equal(rstd[last], want[2])
+    dx = ops.rms_norm_add_backward(y, None, x, w, rstd)[0]
+    assert torch.equal(dx[last], ops.rms_norm_add_backward(y[last], None, x[last], w,
+                                                           rstd[last])[0])
+    del y, dx, rstd
+    tokens = torch.zeros(n, dtype=torch.int64, device="cuda")
+    tokens[last] = torch.arange(21, device="cuda") + 1
+    table = torch.randn(22, width, device="cuda").bfloat16()
+    out = ops.scaled_embedding(table, tokens, 2.0)
+    assert torch.equal(out[last], 2 * table[1:])
+    dt = ops.scaled_embedding_backward(x, ops.token_order(tokens, 22), 2.0)
+    assert torch.equal(dt[1:], 2 * x[last])
+    assert torch.equal(dt[0].float(), torch.full((width,), 2.0 ** 23, device="cuda"))
+    # a table whose rows lie past 2^31
+    del out, dt
+    tokens = torch.tensor([n - 1, 3, n - 21, n - 1], device="cuda")
+    assert torch.equal(ops.scaled_embedding(x, tokens, 0.5), 0.5 * x[tokens])
+    dt = ops.scaled_embedding_backward(x[:4].contiguous(), ops.token_order(tokens, n), 1.0)
+    assert torch.equal(dt[n - 1], x[0] + x[3]) and torch.equal(dt[n - 21], x[2])
+    assert not bool(dt[4:n - 21].any()) and not bool(dt[n - 20:n - 1].any())
+
+
+def test_two_streams_at_once():
+    from mlcg_amd import nn
+
+    cases = [_rms_case(20000, 128, torch.float32, torch.float32, seed) for seed in (0, 1)]
+    tokens = [torch.randint(0, 9, (20000,), device="cuda") for _ in cases]
+
+    def work(c, tok):
+        x, r, w, gy, gt = c
+        leaf = [t.detach().requires_grad_(True) for t in (x, r, w, x[:9])]
+        outs = [*nn.rms_norm_add(*leaf[:3]), nn.scaled_embedding(leaf[3], tok, 2.0)]
+        return [*outs, *torch.autograd.grad(outs, leaf, [gy, gt, gy])]
+
+    want = [work(c, t) for c, t in zip(cases, tokens)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, c, t in zip(streams, cases, tokens):
+            with torch.cuda.stream(s):
+                got.append(work(c, t))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for p, q in zip(a, b):
+                assert torch.equal(p, q)
