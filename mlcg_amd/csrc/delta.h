@@ -379,7 +379,8 @@ struct loose {
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
-// 4 elements of a row of len (a multiple of 8) from el on, zeros past its end: without a branch, so that loads are not waited for one by one
+// 4 elements of a row of len (a multiple of 8) from el on, zeros past its end: without
+// a branch, so that loads are not waited for one by one
 template <typename T>
 __device__ __forceinline__ v4<T> load4(const T* row, int el, int len) {
   const v4<T> x = *reinterpret_cast<const typename loose<T, 4>::type*>(row + min(el, len - 4));
@@ -859,8 +860,8 @@ __device__ __forceinline__ f32x4 row_factor(const float* f, int b) {
 // sent to one while the other is worked on; with one the next workgroup on the
 // compute unit works meanwhile.
 template <typename T, int DK, int WAVES, bool ALONE>
-__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan(DeltaArgs a, DeltaEnds e, T* out,
-                                                         int buffers) {
+__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan(
+    DeltaArgs a, DeltaEnds e, T* out, int buffers) {
   constexpr int NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
   typedef ScanTiles<T, DK> Tiles;
@@ -1057,8 +1058,8 @@ __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds 
 
 // The state's gradient along the chunks of a segment, the last one first.
 template <typename T, int DK, int WAVES, bool ALONE>
-__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan_back(DeltaArgs a, DeltaBack o,
-                                                              DeltaEnds e, int buffers) {
+__global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan_back(
+    DeltaArgs a, DeltaBack o, DeltaEnds e, int buffers) {
   constexpr int NI = Pieces<T>::in, NM = Pieces<T>::mid, KS = DK / 32, B = DK / 16;
   extern __shared__ __align__(16) unsigned char smem[];
   typedef ScanTiles<T, DK> Tiles;
@@ -1221,7 +1222,8 @@ constexpr int grad_waves() {
 
 // MANY: several heads to a key head, whose gradients are summed
 template <typename T, int DK, int KV, bool MANY>
-__global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delta_grad(DeltaArgs a, DeltaBack o, int places) {
+__global__ __launch_bounds__(kDeltaThreads, (grad_waves<T, DK, KV>())) void delta_grad(
+    DeltaArgs a, DeltaBack o, int places) {
   typedef GradTiles<T, DK, KV> Tiles;
   typedef typename Tiles::Rows Rows;
   typedef typename Tiles::Given Given;
@@ -1595,6 +1597,9 @@ inline bool lds_limit(const void* f, size_t bytes) {
 // 500 beads, 8 heads of 64 in bf16: 53 us with two, 57 with one; 4 x 500: 46 and 50.
 // With more workgroups the scan alone, 512 x 100, 8 heads of 32: 68 and 50; 48 x 268,
 // 8 heads of 16 in fp32: 45 and 33.
+// The limit that is set is that of two in either case: calls of several threads may
+// differ in it.
+inline size_t scan_most(size_t bytes) { return 2 * bytes <= kDeltaLds ? 2 * bytes : bytes; }
 inline int scan_buffers(size_t bytes, int64_t groups) {
   return 2 * bytes <= kDeltaLds && groups <= kDeltaUnits ? 2 : 1;
 }
@@ -1623,7 +1628,7 @@ int forward_waves(const DeltaArgs& a, T* out, DeltaEnds e, float* ws, hipStream_
     const auto alone = delta_scan<T, DK, W, true>;
     const size_t bytes = ScanTiles<T, DK>::bytes(false);
     const int buffers = scan_buffers(bytes, 2 * groups);
-    if (!lds_limit(reinterpret_cast<const void*>(alone), buffers * bytes)) return MLCG_ERR_LAUNCH;
+    if (!lds_limit(reinterpret_cast<const void*>(alone), scan_most(bytes))) return MLCG_ERR_LAUNCH;
     hipLaunchKernelGGL(alone, dim3(a.n_segs, a.heads, 2), dim3(64 * W), buffers * bytes, s, a, e,
                        out, buffers);
     const int status = join<T, DK, WAVES, false>(a, e, ws, s);
@@ -1633,7 +1638,7 @@ int forward_waves(const DeltaArgs& a, T* out, DeltaEnds e, float* ws, hipStream_
   const auto scan = delta_scan<T, DK, WAVES, false>;
   const size_t bytes = ScanTiles<T, DK>::bytes(true);
   const int buffers = scan_buffers(bytes, groups);
-  if (!lds_limit(reinterpret_cast<const void*>(scan), buffers * bytes)) return MLCG_ERR_LAUNCH;
+  if (!lds_limit(reinterpret_cast<const void*>(scan), scan_most(bytes))) return MLCG_ERR_LAUNCH;
   hipLaunchKernelGGL(scan, dim3(a.n_segs, a.heads), dim3(64 * WAVES), buffers * bytes, s, a, e, out,
                      buffers);
   return mlcg_launch_status();
@@ -1646,14 +1651,14 @@ int backward_waves(const DeltaArgs& a, const DeltaBack& o, DeltaEnds e, float* w
   const dim3 grid(a.n_segs, a.heads), block(64 * WAVES);
   if (e.seg_last) {
     const auto alone = delta_scan_back<T, DK, WAVES, true>;
-    if (!lds_limit(reinterpret_cast<const void*>(alone), buffers * bytes)) return MLCG_ERR_LAUNCH;
+    if (!lds_limit(reinterpret_cast<const void*>(alone), scan_most(bytes))) return MLCG_ERR_LAUNCH;
     hipLaunchKernelGGL(alone, grid, block, buffers * bytes, s, a, o, e, buffers);
     const int status = join<T, DK, WAVES, true>(a, e, ws, s);
     if (status != MLCG_OK) return status;
     e.seg_init = ws;
   }
   const auto scan = delta_scan_back<T, DK, WAVES, false>;
-  if (!lds_limit(reinterpret_cast<const void*>(scan), buffers * bytes)) return MLCG_ERR_LAUNCH;
+  if (!lds_limit(reinterpret_cast<const void*>(scan), scan_most(bytes))) return MLCG_ERR_LAUNCH;
   hipLaunchKernelGGL(scan, grid, block, buffers * bytes, s, a, o, e, buffers);
   const int kv = a.dvp / 32;
   if (a.group == 1)

@@ -54,7 +54,8 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_forward(
     for (int r = 0; r < kEmbRows; ++r) x[r] = load_row8<T>(table + tok[r] * width, el, width);
 #pragma unroll
     for (int r = 0; r < kEmbRows; ++r)
-      if (i0 + r < n) store_row8<T>(out + (i0 + r) * width, el, width, ok[r] ? x[r] * scale : f32x8{});
+      if (i0 + r < n)
+        store_row8<T>(out + (i0 + r) * width, el, width, ok[r] ? x[r] * scale : f32x8{});
   }
 }
 
@@ -352,11 +353,11 @@ int emb_sums(const void* grad, const int* keys, const int* index, int64_t n, int
   const int64_t slabs = (n + SLAB - 1) / SLAB;
   const unsigned parts = mlcg_div_up(width, 8 * lanes);
   float *head = ws, *tail = ws + slabs * width;
-  hipLaunchKernelGGL((embedding_slab<T, SLAB>), dim3(mlcg_div_up(slabs, kEmbThreads / lanes), parts),
-                     dim3(kEmbThreads), 0, s, (const T*)grad, keys, index, n, rows, width, lanes,
-                     scale, (T*)out, head, tail);
-  hipLaunchKernelGGL((embedding_join<T, SLAB>), dim3((unsigned)slabs, parts), dim3(kEmbThreads), 0, s,
-                     keys, n, rows, width, lanes, scale, head, tail, (T*)out);
+  hipLaunchKernelGGL((embedding_slab<T, SLAB>),
+                     dim3(mlcg_div_up(slabs, kEmbThreads / lanes), parts), dim3(kEmbThreads), 0, s,
+                     (const T*)grad, keys, index, n, rows, width, lanes, scale, (T*)out, head, tail);
+  hipLaunchKernelGGL((embedding_join<T, SLAB>), dim3((unsigned)slabs, parts), dim3(kEmbThreads),
+                     0, s, keys, n, rows, width, lanes, scale, head, tail, (T*)out);
   return mlcg_launch_status();
 }
 
