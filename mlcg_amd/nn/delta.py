@@ -40,10 +40,13 @@ def _once(backward):
 class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, beta, state, chains, scale, keep, reverse, normalize):
-        out, last, kept = ops.gated_delta(q, k, v, decay, beta, chains, scale, keep, state,
-                                          reverse, normalize, train=True)
+        args, scale, keep = ops._delta_args(q, k, v, decay, beta, chains, scale, keep)
+        own = q.shape[2], v.shape[2]
+        out, last, kept = ops._delta_forward(args, own, chains, scale, keep, state, reverse,
+                                             normalize, True)
+        q, qs, k, ks, v, vs, decay, beta, *dims = args
         ctx.save_for_backward(q, k, v, decay, beta, keep, kept)
-        ctx.plan = (chains, scale, reverse, normalize)
+        ctx.plan = (qs, ks, vs, dims, own, chains, scale, reverse, normalize)
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -53,12 +56,12 @@ class _GatedDelta(torch.autograd.Function):
         if grad is None and grad_last is None:
             return (None,) * 11
         q, k, v, decay, beta, keep, kept = ctx.saved_tensors
-        chains, scale, reverse, normalize = ctx.plan
+        qs, ks, vs, dims, own, chains, scale, reverse, normalize = ctx.plan
         if grad is None:
-            grad = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
-        grads = ops.gated_delta_backward(q, k, v, decay, beta, chains, kept, grad, grad_last,
-                                         scale, keep, reverse, normalize,
-                                         want_state=ctx.needs_input_grad[5])
+            grad = torch.zeros(*v.shape[:2], own[1], dtype=v.dtype, device=v.device)
+        grads = ops._delta_backward((q, qs, k, ks, v, vs, decay, beta, *dims), own, chains, kept,
+                                    grad, grad_last, scale, keep, reverse, normalize,
+                                    ctx.needs_input_grad[5])
         return (*grads, None, None, None, None, None)
 
 

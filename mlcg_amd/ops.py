@@ -2420,9 +2420,15 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.
     its chunk of 64 beads on, and the chain's gradients; no other chain's.  state
     [B, H, DK, DV] float32: where each chain begins (zeros by default); last is
     where it ends.  kept is what the backward pass takes (train=True)."""
-    own = q.shape[-1], v.shape[-1]
-    (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
-        q, k, v, decay, beta, chains, scale, keep)
+    args, scale, keep = _delta_args(q, k, v, decay, beta, chains, scale, keep)
+    return _delta_forward(args, (q.shape[2], v.shape[2]), chains, scale, keep, state, reverse,
+                          normalize, train)
+
+
+def _delta_forward(args, own, chains, scale, keep, state, reverse, normalize, train):
+    """gated_delta of what _delta_args gave; own: the channels before they were filled
+    up."""
+    q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = args
     n, dev = chains.n_beads, q.device
     state = _check_delta_state(state, "state", (chains.n_chains, heads, *own), dev)
     state = _delta_pad(state, *own)
@@ -2456,18 +2462,35 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
     """(grad q, grad k, grad v, grad decay, grad beta, grad state | None) of
     gated_delta for the gradients of its outputs (mlcg_gated_delta_backward);
     kept is the forward's, with train=True.  Every sum has a fixed order."""
-    own = q.shape[-1], v.shape[-1]
-    (q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt), scale, keep = _delta_args(
-        q, k, v, decay, beta, chains, scale, keep)
+    args, scale, keep = _delta_args(q, k, v, decay, beta, chains, scale, keep)
+    own, n, heads, dev = (q.shape[2], v.shape[2]), chains.n_beads, v.shape[1], q.device
+    _check(grad.shape == v.shape and grad.dtype == q.dtype and grad.device == dev,
+           lambda: f"grad must be {tuple(v.shape)} {q.dtype} on {dev}")
+    grad_last = _check_delta_state(grad_last, "grad_last", (chains.n_chains, heads, *own), dev)
+    _check(kept.dtype == torch.float32 and kept.device == dev and kept.is_contiguous()
+           and (n == 0 or kept.shape == (_delta_kept(args, chains),)),
+           "kept must be what gated_delta gave with train=True for the same chains")
+    return _delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, reverse,
+                           normalize, want_state)
+
+
+def _delta_kept(args, chains) -> int:
+    heads = args[8]
+    return _delta_floats(chains, _delta_plan(chains, heads), *args[8:], 1)
+
+
+def _delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, reverse, normalize,
+                    want_state):
+    """gated_delta_backward of a forward pass's own arrays and of gradients whose
+    shapes, types and device autograd has made theirs: not checked again."""
+    q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = args
     n, dev = chains.n_beads, q.device
-    _check(grad.shape == (n, heads, own[1]) and grad.dtype == q.dtype and grad.device == dev,
-           lambda: f"grad must be [{n}, {heads}, {own[1]}] {q.dtype} on {dev}")
     if own[1] != dv:
         grad = torch.nn.functional.pad(grad, (0, dv - own[1]))
     grad = grad.contiguous()
     shape = (chains.n_chains, heads, dk, dv)
-    grad_last = _check_delta_state(grad_last, "grad_last", (chains.n_chains, heads, *own), dev)
-    grad_last = _delta_pad(grad_last, *own)
+    if grad_last is not None:
+        grad_last = _delta_pad(grad_last.contiguous(), *own)
     dq = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
     dkk = torch.empty(n, keys, dk, dtype=q.dtype, device=dev)
     dvv = torch.empty(n, heads, dv, dtype=q.dtype, device=dev)
@@ -2481,17 +2504,14 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
             dstate = dstate[..., :own[0], :own[1]].contiguous()
         return dq[..., :own[0]], dkk[..., :own[0]], dvv[..., :own[1]], ddecay, dbeta, dstate
     plan = _delta_plan(chains, heads)
-    size = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 1)
-    _check(kept.shape == (size,) and kept.dtype == torch.float32 and kept.device == dev,
-           "kept must be what gated_delta gave with train=True for the same chains")
     nws = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 3)
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     tiles = chains.tiles[DELTA_ROWS]
     call("mlcg_gated_delta_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta),
          n, heads, keys, dk, dv, dt, ptr(tiles), tiles.shape[0], ptr(plan.segments),
          plan.segments.shape[0], ptr(plan.first), plan.first.shape[0] - 1, plan.split, ptr(keep),
-         scale, int(normalize), int(reverse), ptr(kept), size, ptr(grad), ptr(grad_last), ptr(dq),
-         ptr(dkk), ptr(dvv), ptr(ddecay), ptr(dbeta), ptr(dstate), ptr(ws), nws,
+         scale, int(normalize), int(reverse), ptr(kept), kept.shape[0], ptr(grad), ptr(grad_last),
+         ptr(dq), ptr(dkk), ptr(dvv), ptr(ddecay), ptr(dbeta), ptr(dstate), ptr(ws), nws,
          stream_handle(dev))
     if own != (dk, dv):
         dq, dkk, dvv = (t[..., :d].contiguous() for t, d in
