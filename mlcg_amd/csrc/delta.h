@@ -190,12 +190,13 @@ __device__ __forceinline__ f32x4 half_of(f32x8 x) {
               : __builtin_shufflevector(x, x, 0, 1, 2, 3);
 }
 
-// c += a b to the accuracy of the operand with more pieces
+// c += a b: products of pieces down to 2^-24 of the first (piece i is 2^-8i of its
+// operand or less), those of two exact operands of two pieces with them
 template <int NA, int NB>
 __device__ __forceinline__ void mma(f32x4& c, const Frag<NA>& a, const Frag<NB>& b) {
-  constexpr int most = NA > NB ? NA : NB;
+  constexpr int last = NA + NB < 4 ? NA + NB - 2 : 2;
 #pragma unroll
-  for (int o = most - 1; o >= 0; --o)  // the small products first
+  for (int o = last; o >= 0; --o)  // the small products first
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int j = o - i;

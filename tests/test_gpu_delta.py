@@ -566,3 +566,13 @@ def test_two_streams_at_once():
         for a, b in zip(got, want):
             for name in b:
                 assert torch.equal(a[name], b[name]), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,keys,d", [(4, 4, 16), (4, 2, 64), (2, 1, 128)])
+def test_sixteen_bit_arrays_keep_their_digits(monkeypatch, heads, keys, d, dtype):
+    """16-bit arrays are exact in one or two pieces, and what is computed from them
+    has three: states and the gates' gradients, which are fp32, are as far off as those
+    of fp32 arrays (p = 2^-24), the other outputs by their own rounding more."""
+    monkeypatch.setitem(P, dtype, 2.0 ** -24)
+    _check(_case([130, 64, 7], heads, keys, d, d, dtype, state=True))
