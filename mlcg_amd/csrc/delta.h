@@ -314,7 +314,13 @@ __device__ __forceinline__ void send_to_lds(float4* lds, const float4* src) {
                                        (lds_void*)(lds + 64 * unit), 16, 0, 0);
   }
 }
-__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// What this wave has sent for is there.  Memory is not touched across it in either
+// direction: the wait by itself says nothing of memory to the compiler.
+__device__ __forceinline__ void wait_for_memory() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  asm volatile("" ::: "memory");
+}
 
 // Where the beads of a chunk are.
 struct Chunk {
@@ -995,9 +1001,10 @@ __global__ __launch_bounds__(64 * WAVES, (scan_waves<T, DK>())) void delta_scan(
 
 // The states before the segments of a chain, one after the other: S <- M S + N.
 // Backward: after them, the last one first, S <- M^T S + N.  Bound by the latency of
-// memory: the maps, in three buffers, and N are sent for two steps ahead (with one
-// buffer, the widest maps in fp32, one).  What a wave sends arrives in order, so that
-// its part of a map is there when the N sent for behind it is.
+// memory: while a segment's map is worked on, the next one's map and N are on their
+// way, the map to the other of two buffers (with one, the maps of 128 channels, they
+// are sent for when all are done with the last).  Before the barrier every wave waits
+// for all that it sent, so that a map is whole and N there behind it.
 template <typename T, int DK, int WAVES, bool BACK>
 __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds e,
                                                          float* seg_init, int buffers) {
@@ -1010,21 +1017,23 @@ __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds 
   const int first = uniform(a.seg_first[blockIdx.x]);
   const int n = uniform(a.seg_first[blockIdx.x + 1]) - first;
   const int chain = uniform(a.segs[first]).x;
-  f32x4 S[B], even[B], odd[B];
+  f32x4 S[B], next[B];
   load_state<B>(S, e.init + ((int64_t)chain * a.heads + h) * ((int64_t)a.dk * a.dv) + v0, a.dv,
                 a.dk, e.init && v0 + c < a.dv);
   const auto seg_at = [&](int j) {
     return (int64_t)(first + (BACK ? n - 1 - j : j)) * a.heads + h;
   };
-  const auto fetch = [&](int j, f32x4 (&next)[B]) {
+  const auto fetch = [&](int j) {
     if (j + 1 >= n) return;  // nothing comes behind the last segment
     const int64_t at = seg_at(j);
     send_to_lds<Map::units, WAVES>(maps[j % buffers].x, e.seg_map + at * (Map::units * 64));
     load_state<B>(next, e.seg_last + at * (DK * a.dvp) + (live ? v0 : 0), a.dvp, DK, true);
   };
-  const auto step = [&](int j, f32x4 (&next)[B], f32x4 (&other)[B]) {
 #pragma unroll
-    for (int b = 0; b < B; ++b) asm volatile("" : "+v"(next[b]));  // is there
+  for (int b = 0; b < B; ++b) next[b] = f32x4{};
+  fetch(0);
+  for (int j = 0; j < n; ++j) {
+    wait_for_memory();
     lds_barrier();
     Frag<NM> s[KS];
     split_rows<NM>(s, S);
@@ -1032,7 +1041,8 @@ __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds 
     if (j + 1 >= n) return;
 #pragma unroll
     for (int b = 0; b < B; ++b) S[b] = next[b];
-    if (buffers > 1) fetch(j + 2, next);
+    // all have read the map of j - 1, which was in the place of that of j + 1
+    if (buffers == 2) fetch(j + 1);
     const Map& m = maps[j % buffers];
     if (BACK) {
 #pragma unroll
@@ -1044,16 +1054,8 @@ __global__ __launch_bounds__(64 * WAVES) void delta_join(DeltaArgs a, DeltaEnds 
     }
     if (buffers == 1) {
       lds_barrier();
-      fetch(j + 1, other);
+      fetch(j + 1);
     }
-  };
-#pragma unroll
-  for (int b = 0; b < B; ++b) even[b] = odd[b] = f32x4{};
-  fetch(0, even);
-  if (buffers > 1) fetch(1, odd);
-  for (int j = 0; j < n; j += 2) {
-    step(j, even, odd);
-    if (j + 1 < n) step(j + 1, odd, even);
   }
 }
 
@@ -1609,7 +1611,7 @@ template <typename T, int DK, int WAVES, bool BACK>
 int join(const DeltaArgs& a, const DeltaEnds& e, float* ws, hipStream_t s) {
   const auto f = delta_join<T, DK, WAVES, BACK>;
   const size_t one = sizeof(Image<Pieces<T>::mid, DK * DK / 512>);
-  const int buffers = 3 * one <= kDeltaLds ? 3 : 1;
+  const int buffers = 2 * one <= kDeltaLds ? 2 : 1;
   if (!lds_limit(reinterpret_cast<const void*>(f), buffers * one)) return MLCG_ERR_LAUNCH;
   hipLaunchKernelGGL(f, dim3(a.n_whole, a.heads), dim3(64 * WAVES), buffers * one, s, a, e, ws,
                      buffers);
