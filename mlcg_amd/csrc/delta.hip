@@ -146,6 +146,8 @@ int step_of(const StepArgs& a, int64_t batch, hipStream_t s) {
   return wide ? launch_step<T, 4>(a, batch, s) : launch_step<T, 1>(a, batch, s);
 }
 
+bool aligned32(const void* p) { return reinterpret_cast<uintptr_t>(p) % 32 == 0; }
+
 // the parts of the buffers, in floats
 struct Parts {
   int64_t fac, rows, mats, u, s0, seg_state, seg_map;
@@ -232,7 +234,8 @@ extern "C" int mlcg_gated_delta(
                n_whole >= 1);
   const Parts p = parts(n_tiles, split ? n_segments : 0, heads, key_heads, dk, dv, dtype);
   MLCG_REQUIRE(kept_floats >= p.chunks() + (train ? p.u + p.s0 : 0) &&
-               workspace_floats >= 2 * p.seg_state && (!split || workspace));
+               workspace_floats >= 2 * p.seg_state && (!split || workspace) && aligned32(kept) &&
+               aligned32(workspace));
   DeltaEnds e{state, last_state, nullptr, nullptr, nullptr};
   place(a, e, kept, p, train, split);
   if (split) e.seg_last = workspace;
@@ -266,7 +269,8 @@ extern "C" int mlcg_gated_delta_backward(
                grad_out && grad_q && grad_k && grad_v && grad_decay && grad_beta && workspace);
   const Parts p = parts(n_tiles, split ? n_segments : 0, heads, key_heads, dk, dv, dtype);
   MLCG_REQUIRE(kept_floats >= p.chunks() + p.u + p.s0 &&
-               workspace_floats >= 2 * p.seg_state + p.u + p.s0);
+               workspace_floats >= 2 * p.seg_state + p.u + p.s0 && aligned32(kept) &&
+               aligned32(workspace));
   DeltaEnds e{grad_last_state, nullptr, nullptr, nullptr, nullptr};
   place(a, e, const_cast<float*>(kept), p, true, split);
   float* at = workspace;

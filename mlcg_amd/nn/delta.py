@@ -44,9 +44,9 @@ class _GatedDelta(torch.autograd.Function):
         own = q.shape[2], v.shape[2]
         out, last, kept = ops._delta_forward(args, own, chains, scale, keep, state, reverse,
                                              normalize, True)
-        q, qs, k, ks, v, vs, decay, beta, *dims = args
+        q, _, k, _, v, _, decay, beta, *dims = args
         ctx.save_for_backward(q, k, v, decay, beta, keep, kept)
-        ctx.plan = (qs, ks, vs, dims, own, chains, scale, reverse, normalize)
+        ctx.plan = (dims, own, chains, scale, reverse, normalize)
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -55,13 +55,13 @@ class _GatedDelta(torch.autograd.Function):
     def backward(ctx, grad, grad_last):
         if grad is None and grad_last is None:
             return (None,) * 11
-        q, k, v, decay, beta, keep, kept = ctx.saved_tensors
-        qs, ks, vs, dims, own, chains, scale, reverse, normalize = ctx.plan
+        dims, own, chains, scale, reverse, normalize = ctx.plan
+        args, keep, kept = ops._delta_saved(*ctx.saved_tensors, dims, chains)
         if grad is None:
+            v = args[4]
             grad = torch.zeros(*v.shape[:2], own[1], dtype=v.dtype, device=v.device)
-        grads = ops._delta_backward((q, qs, k, ks, v, vs, decay, beta, *dims), own, chains, kept,
-                                    grad, grad_last, scale, keep, reverse, normalize,
-                                    ctx.needs_input_grad[5])
+        grads = ops._delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, reverse,
+                                    normalize, ctx.needs_input_grad[5])
         return (*grads, None, None, None, None, None)
 
 

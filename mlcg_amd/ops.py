@@ -2470,8 +2470,8 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
     _check(kept.dtype == torch.float32 and kept.device == dev and kept.is_contiguous()
            and (n == 0 or kept.shape == (_delta_kept(args, chains),)),
            "kept must be what gated_delta gave with train=True for the same chains")
-    return _delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, reverse,
-                           normalize, want_state)
+    return _delta_backward(args, own, chains, _delta_aligned(kept), grad, grad_last, scale, keep,
+                           reverse, normalize, want_state)
 
 
 def _delta_kept(args, chains) -> int:
@@ -2479,10 +2479,36 @@ def _delta_kept(args, chains) -> int:
     return _delta_floats(chains, _delta_plan(chains, heads), *args[8:], 1)
 
 
+def _delta_aligned(kept: torch.Tensor) -> torch.Tensor:
+    """kept where the kernels can read it: from a multiple of 32 bytes on."""
+    return kept.clone() if kept.data_ptr() % 32 else kept
+
+
+def _delta_saved(q, k, v, decay, beta, keep, kept, dims, chains):
+    """(args, keep, kept) from the arrays that a forward pass saved, as autograd's
+    hooks gave them back: the same values, but with strides and addresses of any
+    kind."""
+    heads, keys, dk, dv, dt = dims
+    n, dtype, dev = chains.n_beads, q.dtype, chains.device
+    q, qs = _attention_heads(q, "q", n, dtype, dev)
+    k, ks = _attention_heads(k, "k", n, dtype, dev)
+    v, vs = _attention_heads(v, "v", n, dtype, dev)
+    args = (q, qs, k, ks, v, vs, decay.contiguous(), beta.contiguous(), *dims)
+    gates, size = (n, heads), _delta_kept(args, chains) if n else 0
+    _check(DTYPE_IDS.get(dtype) == dt and q.shape == k.shape == (n, keys, dk)
+           and v.shape == (n, heads, dv) and decay.shape == beta.shape == gates
+           and decay.dtype == beta.dtype == kept.dtype == torch.float32
+           and kept.shape == (size,) and decay.device == beta.device == kept.device == dev
+           and (keep is None or (keep.shape == (n,) and keep.dtype == torch.bool
+                                 and keep.device == dev)),
+           "the arrays that gated_delta saved came back with another shape, type or device")
+    return args, None if keep is None else keep.contiguous(), _delta_aligned(kept.contiguous())
+
+
 def _delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, reverse, normalize,
                     want_state):
-    """gated_delta_backward of a forward pass's own arrays and of gradients whose
-    shapes, types and device autograd has made theirs: not checked again."""
+    """gated_delta_backward of checked arrays and of gradients whose shapes, types and
+    device autograd has made theirs: not checked again."""
     q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = args
     n, dev = chains.n_beads, q.device
     if own[1] != dv:
@@ -2621,7 +2647,7 @@ def rms_norm_add_backward(grad: torch.Tensor, grad_t: Optional[torch.Tensor], t:
     if grad_t is not None:
         _check(grad_t.shape == t.shape and grad_t.dtype == t.dtype and grad_t.device == dev,
                lambda: f"grad_t must be {tuple(t.shape)} {t.dtype} on {dev}")
-    return _rms_backward(grad, grad_t, t, weight, rstd.contiguous())
+    return _rms_backward(grad, grad_t, t, weight, rstd)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2630,11 +2656,16 @@ def _rms_workspace(rows: int, width: int) -> int:
 
 
 def _rms_backward(grad, grad_t, t, weight, rstd):
-    """rms_norm_add_backward of a forward pass's own arrays and of gradients whose
-    shapes, types and device autograd has made theirs: not checked again."""
+    """rms_norm_add_backward of a forward pass's own arrays, which autograd's hooks may
+    have put elsewhere, and of gradients whose shapes, types and device autograd has made
+    theirs."""
     n, width = t.shape
     dev, dtype, t_dtype = t.device, grad.dtype, t.dtype
-    grad = grad.contiguous()
+    _check(grad.shape == t.shape and weight.shape == (width,) and rstd.shape == (n,)
+           and weight.dtype == dtype and rstd.dtype == torch.float32
+           and weight.device == rstd.device == grad.device == dev,
+           "the arrays that rms_norm_add saved came back with another shape, type or device")
+    grad, rstd = grad.contiguous(), rstd.contiguous()
     if grad_t is not None:
         grad_t = grad_t.contiguous()
     t, ld = _rms_rows(t, width)

@@ -1,0 +1,94 @@
+"""Host side of calls of the encoder of linear cost's operators: what the entry
+points are handed, with the entry points themselves replaced."""
+
+import pytest
+import torch
+
+from mlcg_amd import nn, ops
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(name, arguments) of the entry points that CPU tensors are handed to."""
+    made = []
+    monkeypatch.setattr(ops, "call", lambda name, *args, **_: made.append((name, args)))
+    monkeypatch.setattr(ops, "require_device", lambda *tensors: None)
+    monkeypatch.setattr(ops, "stream_handle", lambda device=None: 0)
+    monkeypatch.setattr(ops, "_delta_floats", lambda *args: 64)
+    return made
+
+
+def _heads():
+    """q, k and v [8, 2 or 4, 16] as views of one projection, decay and beta."""
+    x = torch.randn(8, 2 * 2 * 16 + 4 * 16, requires_grad=True)
+    q, k, v = x.split([32, 32, 64], 1)
+    return (x, q.unflatten(1, (2, 16)), k.unflatten(1, (2, 16)), v.unflatten(1, (4, 16)),
+            -torch.rand(8, 4), torch.rand(8, 4))
+
+
+def _packed(t):
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _turned(t):
+    """The same values with the axes the other way round in memory."""
+    order = tuple(range(t.dim()))[::-1]
+    return t.permute(order).contiguous().permute(order)
+
+
+def _shifted(t):
+    """The same values from an address one element past an aligned one on."""
+    room = torch.zeros(t.numel() + 1, dtype=t.dtype)
+    return room[1:].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("how", [_packed, _turned, _shifted])
+def test_backward_takes_the_arrays_as_they_come_back(calls, how):
+    """Autograd's hooks may give a saved array back with other strides than it had:
+    those of the array that is read count."""
+    x, *args = _heads()
+    saved, given = [], []
+
+    def unpack(i):
+        given.append(how(saved[i]))
+        return given[-1]
+
+    def pack(t):
+        saved.append(t.detach())
+        return len(saved) - 1
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        out, _ = nn.gated_delta(*args, ops.chain_layout([5, 3], "cpu"))
+    torch.autograd.grad(out, x, torch.ones_like(out))
+    name, a = calls[-1]
+    assert name == "mlcg_gated_delta_backward"
+    arrays = {t.data_ptr(): t for t in given}
+    for i, t in enumerate(args[:3]):
+        assert a[2 * i + 1][1] >= 16 and a[2 * i + 1][0] >= t.shape[1] * 16
+        if a[2 * i] in arrays:  # not copied again
+            assert list(a[2 * i + 1]) == list(arrays[a[2 * i]].stride()[:2])
+            assert arrays[a[2 * i]].stride(2) == 1
+        else:
+            assert list(a[2 * i + 1]) == [t.shape[1] * 16, 16]
+    assert a[25] % 32 == 0 and a[26] == 64  # what the forward pass kept
+    if how is not _turned:
+        assert all(a[2 * i] in arrays for i in range(3))
+
+
+@pytest.mark.parametrize("change", [lambda t: t[..., :8], lambda t: t.double(),
+                                    lambda t: t.flatten()[:-1]])
+def test_backward_refuses_other_arrays(calls, change):
+    x, *args = _heads()
+    saved = []
+    for which in (0, 5):  # q; what the forward pass kept
+        del saved[:]
+
+        def pack(t):
+            saved.append(t.detach())
+            return len(saved) - 1
+
+        with torch.autograd.graph.saved_tensors_hooks(
+                pack, lambda i: change(saved[i]) if i == which else saved[i]):
+            out, _ = nn.gated_delta(*args, ops.chain_layout([5, 3], "cpu"))
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)

@@ -35,3 +35,75 @@ def test_many_segments(monkeypatch, dk, dv, reverse, dtype):
     first = base._check(c)
     for name, t in base._run(c).items():
         assert torch.equal(t, first[name]), name
+
+
+def _elsewhere(t):
+    """The same values from an address one element past an aligned one on, row after
+    row."""
+    room = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return room[1:].view(t.shape).copy_(t)
+
+
+def _turned(t):
+    order = tuple(range(t.dim()))[::-1]
+    return t.permute(order).contiguous().permute(order)
+
+
+HOOKS = {"packed": lambda t: t.clone(memory_format=torch.contiguous_format),
+         "elsewhere": _elsewhere, "turned": _turned}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("how", sorted(HOOKS) + ["host"])
+def test_saved_arrays_come_back_elsewhere(how, dtype):
+    """Autograd's hooks give the saved arrays back with other strides and addresses,
+    or from the host: the same gradients, bit for bit."""
+    from mlcg_amd import nn
+
+    print(f"delta hooks {how} {dtype}", flush=True)
+    hooks = (torch.autograd.graph.save_on_cpu() if how == "host" else
+             torch.autograd.graph.saved_tensors_hooks(HOOKS[how], lambda t: t))
+    g = torch.Generator().manual_seed(5)
+    table = torch.randn(7, 24, generator=g).to(dtype).cuda()
+    tokens = torch.randint(0, 7, (203,), generator=g).cuda()
+    wide = torch.randn(203, 48, generator=g).to(dtype).cuda()
+    gy = torch.randn(203, 24, generator=g).to(dtype).cuda()
+
+    def norms():
+        leaf = [t.detach().requires_grad_(True) for t in (table, wide, table[0])]
+        e = nn.scaled_embedding(leaf[0], tokens, 2.0)
+        y, t = nn.rms_norm_add(leaf[1][:, :24], e, leaf[2])
+        z = nn.rms_norm_add(leaf[1][:, 24:], None, leaf[2])[0]
+        return torch.autograd.grad([y, t, z], leaf, [gy, gy, gy])
+
+    for dk, dv in ((32, 32), (12, 20)):
+        c = base._case([130, 0, 73], 4, 2, dk, dv, dtype, keep=True, state=True)
+        want, others = base._run(c), norms()
+        with hooks:
+            got, again = base._run(c), norms()
+        for name, t in want.items():
+            assert torch.equal(t, got[name]), name
+        for a, b in zip(others, again):
+            assert torch.equal(a, b)
+
+
+def test_kept_from_an_odd_address():
+    from mlcg_amd import _lib, ops
+
+    c = base._case([70, 5], 2, 2, 16, 16, torch.float32)
+    args = [c[n] for n in ("q", "k", "v", "decay", "beta")]
+    _, _, kept = ops.gated_delta(*args, c["chains"], train=True)
+    want = ops.gated_delta_backward(*args, c["chains"], kept, c["grad"])
+    got = ops.gated_delta_backward(*args, c["chains"], _elsewhere(kept), c["grad"])
+    assert all(torch.equal(a, b) for a, b in zip(want[:5], got[:5]))
+    # the entry point itself refuses it
+    strides = ops._Strides(32, 16)
+    plan, tiles = ops._delta_plan(c["chains"], 2), c["chains"].tiles[ops.DELTA_ROWS]
+    odd = _elsewhere(kept)
+    out, p = torch.empty_like(c["v"]), _lib.ptr
+    with pytest.raises(RuntimeError, match="ARGUMENT"):
+        _lib.call("mlcg_gated_delta", p(args[0]), strides, p(args[1]), strides, p(args[2]),
+                  strides, p(args[3]), p(args[4]), 75, 2, 2, 16, 16, 0, p(tiles), tiles.shape[0],
+                  p(plan.segments), plan.segments.shape[0], p(plan.first),
+                  plan.first.shape[0] - 1, plan.split, None, None, 0.25, 1, 0, p(out), None,
+                  p(odd), odd.shape[0], 1, None, 0, _lib.stream_handle(out.device))
