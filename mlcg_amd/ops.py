@@ -16,6 +16,7 @@ from typing import List, Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, ptr, require_device, stream_handle
@@ -2553,6 +2554,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
             and second < first + a.numel() * a.element_size())
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation is on and one of these has a tangent."""
+    if forward_ad._current_level < 0:  # what unpack_dual asks first, once for all
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
                      beta: torch.Tensor, state: torch.Tensor, scale: Optional[float] = None,
                      normalize: bool = True, into: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2560,11 +2568,13 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     the rule of gated_delta on states that lie in memory: q and k [B, HK, DK], v
     [B, H, DV], decay and beta [B, H] float32, state [B, H, DK, DV] float32.  The
     new states take the old ones' place or, given `into`, go there.  No
-    gradients."""
+    derivatives: arrays that ask for one are refused."""
     _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [B, heads, dim]")
     _check(not (torch.is_grad_enabled()
                 and any(t.requires_grad for t in (q, k, v, decay, beta, state))),
            "gated_delta_step has no gradients: call it under torch.no_grad()")
+    _check(not _has_tangent(q, k, v, decay, beta, state, into),
+           "gated_delta_step has no forward-mode derivative")
     batch = q.shape[0]
     q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = _delta_heads(
         q, k, v, decay, beta, batch, "gated_delta_step")

@@ -92,3 +92,32 @@ def test_backward_refuses_other_arrays(calls, change):
             out, _ = nn.gated_delta(*args, ops.chain_layout([5, 3], "cpu"))
         with pytest.raises(RuntimeError):
             torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+
+
+def _step_args():
+    _, q, k, v, decay, beta = _heads()
+    return [q.detach(), k.detach(), v.detach(), decay, beta, torch.zeros(8, 4, 16, 16)]
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_step_refuses_tangents(calls, which):
+    """A forward-mode tangent is refused, not dropped: no_grad leaves that mode on."""
+    args = _step_args()
+    args.append(torch.zeros_like(args[5]))
+    with torch.autograd.forward_ad.dual_level():
+        args[which] = torch.autograd.forward_ad.make_dual(args[which],
+                                                          torch.ones_like(args[which]))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="derivative"):
+            ops.gated_delta_step(*args[:6], into=args[6])
+        assert not calls
+    with torch.no_grad():
+        ops.gated_delta_step(*_step_args())
+    assert len(calls) == 1
+
+
+def test_module_step_refuses_tangents(calls):
+    delta = nn.ChainDelta(32, 2, bidirectional=False)
+    with torch.autograd.forward_ad.dual_level():
+        x = torch.autograd.forward_ad.make_dual(torch.ones(3, 32), torch.ones(3, 32))
+        with pytest.raises(RuntimeError, match="derivative"):
+            delta.step(x, delta.new_state(3))
