@@ -2571,7 +2571,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     derivatives: arrays that ask for one are refused."""
     _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [B, heads, dim]")
     _check(not (torch.is_grad_enabled()
-                and any(t.requires_grad for t in (q, k, v, decay, beta, state))),
+                and any(t is not None and t.requires_grad
+                        for t in (q, k, v, decay, beta, state, into))),
            "gated_delta_step has no gradients: call it under torch.no_grad()")
     _check(not _has_tangent(q, k, v, decay, beta, state, into),
            "gated_delta_step has no forward-mode derivative")
@@ -2591,6 +2592,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     call("mlcg_gated_delta_step", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), batch,
          heads, keys, dk, dv, dt, ptr(state), float(dk ** -0.5 if scale is None else scale),
          int(normalize), ptr(out), ptr(into), stream_handle(dev))
+    torch.autograd.graph.increment_version(into)  # a graph that saved it is told
     return out
 
 

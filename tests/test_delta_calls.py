@@ -121,3 +121,29 @@ def test_module_step_refuses_tangents(calls):
         x = torch.autograd.forward_ad.make_dual(torch.ones(3, 32), torch.ones(3, 32))
         with pytest.raises(RuntimeError, match="derivative"):
             delta.step(x, delta.new_state(3))
+
+
+@pytest.mark.parametrize("own", [True, False])
+def test_step_moves_the_version_of_what_it_writes(calls, own):
+    """A state that a graph has saved cannot be written unseen."""
+    args = _step_args()
+    into = args[5] if own else torch.zeros_like(args[5])
+    scale = torch.ones((), requires_grad=True)
+    loss = (scale * into).sum()  # saves into
+    before = [t._version for t in args]
+    with torch.no_grad():
+        ops.gated_delta_step(*args, into=None if own else into)
+    assert [t._version for t in args[:5]] == before[:5]
+    assert args[5]._version == before[5] + own
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        ops.gated_delta_step(*_step_args())
+
+
+def test_step_into_a_leaf(calls):
+    args = _step_args()
+    into = torch.zeros_like(args[5]).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        ops.gated_delta_step(*args, into=into)
+    assert not calls

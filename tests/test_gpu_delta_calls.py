@@ -107,3 +107,26 @@ def test_kept_from_an_odd_address():
                   p(plan.segments), plan.segments.shape[0], p(plan.first),
                   plan.first.shape[0] - 1, plan.split, None, None, 0.25, 1, 0, p(out), None,
                   p(odd), odd.shape[0], 1, None, 0, _lib.stream_handle(out.device))
+
+
+def test_step_on_a_state_that_a_graph_saved():
+    """`last` of a training call in a loss that saved it, then steps on it: autograd
+    refuses the loss's gradient, as after any operation of torch in place."""
+    from mlcg_amd import nn, ops
+
+    c = base._case([70, 64], 2, 2, 16, 16, torch.float32, views=False)
+    v = c["v"].detach().requires_grad_(True)
+    args = [c["q"], c["k"], v, c["decay"], c["beta"]]
+    last = nn.gated_delta(*args, c["chains"])[1]
+    loss = last.square().sum()
+    row = [t.detach()[:2] for t in args]
+    with torch.no_grad():
+        ops.gated_delta_step(*row, last)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    last = nn.gated_delta(*args, c["chains"])[1]
+    loss = last.square().sum()
+    with torch.no_grad():
+        ops.gated_delta_step(*row, last, into=torch.empty_like(last))
+    loss.backward()
+    assert bool(v.grad.any())
