@@ -2632,6 +2632,7 @@ def rms_norm_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     n, width = x.shape
     dev = x.device
     x, ld = _rms_rows(x, width)
+    weight = weight.contiguous()
     y = torch.empty(n, width, dtype=x.dtype, device=dev)
     rstd = torch.empty(n, dtype=torch.float32, device=dev)
     t, rld, rdt = x, 0, dt
@@ -2639,7 +2640,7 @@ def rms_norm_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
         residual, rld = _rms_rows(residual, width)
         t = torch.empty(n, width, dtype=residual.dtype, device=dev)
         rdt = DTYPE_IDS[residual.dtype]
-    call("mlcg_rms_norm_add", ptr(x), ld, ptr(residual), rld, ptr(weight.contiguous()), n, width,
+    call("mlcg_rms_norm_add", ptr(x), ld, ptr(residual), rld, ptr(weight), n, width,
          dt, rdt, float(eps), ptr(y), None if residual is None else ptr(t), ptr(rstd),
          stream_handle(dev))
     return y, t, rstd
@@ -2677,7 +2678,7 @@ def _rms_backward(grad, grad_t, t, weight, rstd):
            and weight.dtype == dtype and rstd.dtype == torch.float32
            and weight.device == rstd.device == grad.device == dev,
            "the arrays that rms_norm_add saved came back with another shape, type or device")
-    grad, rstd = grad.contiguous(), rstd.contiguous()
+    grad, weight, rstd = grad.contiguous(), weight.contiguous(), rstd.contiguous()
     if grad_t is not None:
         grad_t = grad_t.contiguous()
     t, ld = _rms_rows(t, width)
@@ -2689,7 +2690,7 @@ def _rms_backward(grad, grad_t, t, weight, rstd):
     nws = _rms_workspace(n, width)
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     call("mlcg_rms_norm_add_backward", ptr(grad), ptr(grad_t), ptr(t), ld,
-         ptr(weight.contiguous()), ptr(rstd), n, width, DTYPE_IDS[dtype], DTYPE_IDS[t_dtype],
+         ptr(weight), ptr(rstd), n, width, DTYPE_IDS[dtype], DTYPE_IDS[t_dtype],
          ptr(dx), None if dr is dx else ptr(dr), ptr(dw), ptr(ws), nws, stream_handle(dev))
     return dx, dr, dw
 

@@ -130,3 +130,29 @@ def test_step_on_a_state_that_a_graph_saved():
         ops.gated_delta_step(*row, last, into=torch.empty_like(last))
     loss.backward()
     assert bool(v.grad.any())
+
+
+def test_copies_live_until_the_launch(monkeypatch):
+    """A weight with a stride is copied: the room of the copy is not given away before
+    the kernel that reads it has been launched."""
+    from mlcg_amd import ops
+
+    x = torch.randn(9, 40, device="cuda")
+    weight = torch.randn(40, 3, device="cuda")[:, 1]
+    want, t, rstd = ops.rms_norm_add(x, None, weight.contiguous())
+    grads = ops.rms_norm_add_backward(want, None, x, weight.contiguous(), rstd)
+    entry, seen = ops.call, []
+
+    def call(name, *args, **options):
+        taken = [torch.full((40,), float("nan"), device="cuda") for _ in range(4)]
+        seen.append(name)
+        entry(name, *args, **options)
+        del taken
+
+    monkeypatch.setattr(ops, "call", call)
+    y, _, r = ops.rms_norm_add(x, None, weight)
+    again = ops.rms_norm_add_backward(want, None, x, weight, rstd)
+    assert seen == ["mlcg_rms_norm_add", "mlcg_rms_norm_add_backward"]
+    assert torch.equal(y, want) and torch.equal(r, rstd)
+    for a, b in zip(grads, again):
+        assert torch.equal(a, b)
