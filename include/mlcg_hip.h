@@ -1128,7 +1128,7 @@ int mlcg_dropout_add(const void* x, const void* residual, int64_t n, int dtype,
  * of the factor) at most 0 for a state that does not grow, -inf included.
  * state and last_state [chains, heads, dk, dv], fp32, may be NULL (zeros; not
  * wanted); last_state is not written for a chain without beads.
- * `tiles` have 64 rows; segments [n_segments, 4]: (chain, its first tile there,
+ * `tiles` have 64 rows, fewer than 2^23 of them; segments [n_segments, 4]: (chain, its first tile there,
  * tiles, 1 for a chain's first | 2 for its last), those of a chain one after the
  * other; segment_first [n_whole + 1]: where the segments of each of the n_whole
  * chains with beads begin.  With split = 0 every chain is one segment; else the

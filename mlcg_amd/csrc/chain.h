@@ -49,6 +49,18 @@ __device__ __forceinline__ void store_row8(T* row, int el, int width, f32x8 x) {
   }
 }
 
+// A grid of `groups` x `parts` workgroups of 256 threads.  An axis holds fewer than
+// 2^32 threads and drops those above without an error: what is over goes on along z,
+// where workgroups past the last one do nothing.
+static inline dim3 chain_grid(int64_t groups, unsigned parts = 1) {
+  constexpr int64_t most = int64_t(1) << 23;
+  if (groups <= most) return dim3((unsigned)groups, parts);
+  return dim3((unsigned)most, parts, mlcg_div_up(groups, most));
+}
+__device__ __forceinline__ int64_t chain_group() {
+  return blockIdx.x + (int64_t)blockIdx.z * gridDim.x;
+}
+
 // true for NULL, too: an absent operand does not restrict the vector path
 static inline bool chain_aligned16(const void* p) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0;

@@ -17,6 +17,7 @@ struct StepArgs {
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   const float *decay, *beta, *state;
+  int64_t batch;
   int heads, group, dk, dv;
   float scale;
   int normalize;
@@ -32,7 +33,8 @@ __global__ __launch_bounds__(kStepThreads) void delta_step_kernel(StepArgs a, in
   __shared__ float norm[2];
   const int R = kStepThreads / cols;  // rows in flight; threads past R cols have none
   const int h = blockIdx.y;
-  const int64_t b = blockIdx.x, at = b * a.heads + h;
+  const int64_t b = chain_group(), at = b * a.heads + h;
+  if (b >= a.batch) return;
   const int r0 = threadIdx.x / cols, c0 = threadIdx.x % cols * W;
   const bool live = r0 < R;
   const float* const S = a.state + at * ((int64_t)a.dk * a.dv) + c0;
@@ -127,9 +129,9 @@ __global__ __launch_bounds__(kStepThreads) void delta_step_kernel(StepArgs a, in
 }
 
 template <typename T, int W>
-int launch_step(const StepArgs& a, int64_t batch, hipStream_t s) {
+int launch_step(const StepArgs& a, hipStream_t s) {
   const int cols = a.dv / W, R = kStepThreads / cols;
-  const dim3 grid((unsigned)batch, a.heads), block(kStepThreads);
+  const dim3 grid = chain_grid(a.batch, a.heads), block(kStepThreads);
   const int rows = (a.dk + R - 1) / R;
   if (rows <= 4)
     hipLaunchKernelGGL((delta_step_kernel<T, W, 4>), grid, block, 0, s, a, cols);
@@ -141,10 +143,13 @@ int launch_step(const StepArgs& a, int64_t batch, hipStream_t s) {
 }
 
 template <typename T>
-int step_of(const StepArgs& a, int64_t batch, hipStream_t s) {
+int step_of(const StepArgs& a, hipStream_t s) {
   const bool wide = a.dv % 4 == 0 && chain_aligned16(a.state) && chain_aligned16(a.next);
-  return wide ? launch_step<T, 4>(a, batch, s) : launch_step<T, 1>(a, batch, s);
+  return wide ? launch_step<T, 4>(a, s) : launch_step<T, 1>(a, s);
 }
+
+// workgroups of up to 512 threads along one axis; `kept` of so many takes 370 GB
+constexpr int64_t kMostTiles = int64_t(1) << 23;
 
 bool aligned32(const void* p) { return reinterpret_cast<uintptr_t>(p) % 32 == 0; }
 
@@ -220,8 +225,8 @@ extern "C" int mlcg_gated_delta(
     void* out, float* last_state, float* kept, int64_t kept_floats, int train, float* workspace,
     int64_t workspace_floats, void* stream) {
   MLCG_REQUIRE(q_strides && k_strides && v_strides && key_heads >= 1 && n_tiles >= 0 &&
-               n_tiles < (int64_t(1) << 31) && n_segments >= 0 &&
-               n_segments < (int64_t(1) << 31) && n_whole >= 0 && n_whole <= n_segments);
+               n_tiles < kMostTiles && n_segments >= 0 && n_segments < kMostTiles &&
+               n_whole >= 0 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
               (dv + 31) / 32 * 32, scale, normalize, reverse,
@@ -256,8 +261,8 @@ extern "C" int mlcg_gated_delta_backward(
     void* grad_k, void* grad_v, float* grad_decay, float* grad_beta, float* grad_state,
     float* workspace, int64_t workspace_floats, void* stream) {
   MLCG_REQUIRE(q_strides && k_strides && v_strides && key_heads >= 1 && n_tiles >= 1 &&
-               n_tiles < (int64_t(1) << 31) && n_segments >= 1 &&
-               n_segments < (int64_t(1) << 31) && n_whole >= 1 && n_whole <= n_segments);
+               n_tiles < kMostTiles && n_segments >= 1 && n_segments < kMostTiles &&
+               n_whole >= 1 && n_whole <= n_segments);
   DeltaArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
               v_strides[1], decay, beta, keep, beads, heads, key_heads, heads / key_heads, dk, dv,
               (dv + 31) / 32 * 32, scale, normalize, reverse,
@@ -297,13 +302,13 @@ extern "C" int mlcg_gated_delta_step(const void* q, const int64_t* q_strides, co
   if (batch == 0) return MLCG_OK;
   MLCG_REQUIRE(q && k && v && decay && beta && state && out && next_state);
   const StepArgs a{q, k, v, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0],
-                   v_strides[1], decay, beta, state, heads, heads / key_heads, dk, dv, scale,
+                   v_strides[1], decay, beta, state, batch, heads, heads / key_heads, dk, dv, scale,
                    normalize, next_state, out};
   hipStream_t s = mlcg_stream(stream);
   switch (dtype) {
-    case MLCG_DTYPE_F32: return step_of<float>(a, batch, s);
-    case MLCG_DTYPE_F16: return step_of<_Float16>(a, batch, s);
-    case MLCG_DTYPE_BF16: return step_of<__bf16>(a, batch, s);
+    case MLCG_DTYPE_F32: return step_of<float>(a, s);
+    case MLCG_DTYPE_F16: return step_of<_Float16>(a, s);
+    case MLCG_DTYPE_BF16: return step_of<__bf16>(a, s);
     default: return MLCG_ERR_ARGUMENT;
   }
 }

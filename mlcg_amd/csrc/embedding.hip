@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_forward(
     const T* __restrict__ table, int rows, const int64_t* __restrict__ tokens, int64_t n, int width,
     int lanes, float scale, T* __restrict__ out, unsigned* __restrict__ flags) {
   const int per = kEmbThreads / lanes, l = threadIdx.x % lanes;
-  const int64_t i0 = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * kEmbRows;
+  const int64_t i0 = (chain_group() * per + threadIdx.x / lanes) * kEmbRows;
   int64_t tok[kEmbRows];
   bool ok[kEmbRows], bad = false;
 #pragma unroll
@@ -228,13 +228,13 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_slab(
   constexpr int kBatch = 8, kMost = kEmbThreads / 8 * SLAB;
   __shared__ int key_of[kMost + 1], row_of[kMost];
   const int per = kEmbThreads / lanes, l = threadIdx.x % lanes, p = threadIdx.x / lanes;
-  const int64_t base = (int64_t)blockIdx.x * per * SLAB;
+  const int64_t base = chain_group() * per * SLAB;
   for (int i = threadIdx.x; i <= per * SLAB; i += kEmbThreads) {
     key_of[i] = base + i < n ? keys[base + i] : -1;
     if (i < per * SLAB) row_of[i] = base + i < n ? index[base + i] : 0;
   }
   __syncthreads();
-  const int64_t slab = (int64_t)blockIdx.x * per + p, begin = slab * SLAB;
+  const int64_t slab = chain_group() * per + p, begin = slab * SLAB;
   const int el = 8 * (blockIdx.y * lanes + l);
   if (begin >= n || el >= width) return;
   const int count = (int)min((int64_t)SLAB, n - begin);
@@ -273,7 +273,7 @@ template <typename T, int SLAB>
 __global__ __launch_bounds__(kEmbThreads) void embedding_join(
     const int* __restrict__ keys, int64_t n, int rows, int width, int lanes, float scale,
     const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ out) {
-  const int64_t slab = blockIdx.x, slabs = (n + SLAB - 1) / SLAB;
+  const int64_t slab = chain_group(), slabs = (n + SLAB - 1) / SLAB;
   const int64_t end = slab * SLAB + SLAB;
   if (end >= n) return;
   const int key = keys[end - 1];
@@ -334,9 +334,9 @@ template <typename T>
 int emb_forward(const void* table, int rows, const int64_t* tokens, int64_t n, int width,
                 float scale, void* out, unsigned* flags, hipStream_t s) {
   const int lanes = emb_lanes(width);
-  hipLaunchKernelGGL((embedding_forward<T>), dim3(mlcg_div_up(n, kEmbThreads / lanes * kEmbRows)),
-                     dim3(kEmbThreads), 0, s, (const T*)table, rows, tokens, n, width, lanes, scale,
-                     (T*)out, flags);
+  const dim3 grid = chain_grid(mlcg_div_up(n, kEmbThreads / lanes * kEmbRows));
+  hipLaunchKernelGGL((embedding_forward<T>), grid, dim3(kEmbThreads), 0, s, (const T*)table, rows,
+                     tokens, n, width, lanes, scale, (T*)out, flags);
   return mlcg_launch_status();
 }
 
@@ -354,10 +354,11 @@ int emb_sums(const void* grad, const int* keys, const int* index, int64_t n, int
   const unsigned parts = mlcg_div_up(width, 8 * lanes);
   float *head = ws, *tail = ws + slabs * width;
   hipLaunchKernelGGL((embedding_slab<T, SLAB>),
-                     dim3(mlcg_div_up(slabs, kEmbThreads / lanes), parts), dim3(kEmbThreads), 0, s,
-                     (const T*)grad, keys, index, n, rows, width, lanes, scale, (T*)out, head, tail);
-  hipLaunchKernelGGL((embedding_join<T, SLAB>), dim3((unsigned)slabs, parts), dim3(kEmbThreads),
-                     0, s, keys, n, rows, width, lanes, scale, head, tail, (T*)out);
+                     chain_grid(mlcg_div_up(slabs, kEmbThreads / lanes), parts), dim3(kEmbThreads),
+                     0, s, (const T*)grad, keys, index, n, rows, width, lanes, scale, (T*)out,
+                     head, tail);
+  hipLaunchKernelGGL((embedding_join<T, SLAB>), chain_grid(slabs, parts), dim3(kEmbThreads), 0, s,
+                     keys, n, rows, width, lanes, scale, head, tail, (T*)out);
   return mlcg_launch_status();
 }
 

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kRmsThreads) void rms_forward(
     const T* __restrict__ weight, int64_t rows, int width, int lanes, float eps,
     T* __restrict__ y, R* __restrict__ t, float* __restrict__ rstd) {
   const int per = kRmsThreads / lanes;
-  const int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / lanes;
+  const int64_t row = chain_group() * per + threadIdx.x / lanes;
   const int l = threadIdx.x % lanes;
   const bool in = row < rows;
   f32x8 v[NV];
@@ -188,10 +188,10 @@ int rms_launch(const RmsCall& a, bool backward, hipStream_t s) {
   const RmsShape sh(a.width);
   const dim3 block(kRmsThreads);
   if (!backward) {
-    hipLaunchKernelGGL((rms_forward<T, R, NV>), dim3(mlcg_div_up(a.rows, kRmsThreads / sh.lanes)),
-                       block, 0, s, (const T*)a.x, a.x_ld, (const R*)a.residual, a.r_ld,
-                       (const T*)a.weight, a.rows, a.width, sh.lanes, a.eps, (T*)a.y, (R*)a.t,
-                       a.rstd);
+    const dim3 grid = chain_grid(mlcg_div_up(a.rows, kRmsThreads / sh.lanes));
+    hipLaunchKernelGGL((rms_forward<T, R, NV>), grid, block, 0, s, (const T*)a.x, a.x_ld,
+                       (const R*)a.residual, a.r_ld, (const T*)a.weight, a.rows, a.width, sh.lanes,
+                       a.eps, (T*)a.y, (R*)a.t, a.rstd);
     return mlcg_launch_status();
   }
   const unsigned n = rms_groups(a.rows, a.width);

@@ -156,3 +156,76 @@ def test_copies_live_until_the_launch(monkeypatch):
     assert torch.equal(y, want) and torch.equal(r, rstd)
     for a, b in zip(grads, again):
         assert torch.equal(a, b)
+
+
+# Rows, tokens and sequences that take 2^32 threads and more: a launch holds fewer along
+# one axis.  (What is compared is made outside of the assertions, which would print it.)
+
+def test_norm_of_more_rows_than_one_axis_holds():
+    from mlcg_amd import ops
+
+    n = 2 ** 29 + 5  # 32 a workgroup
+    x = torch.full((n, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    x[-7:] = -3.0
+    y, _, rstd = ops.rms_norm_add(x, None, torch.ones(1, dtype=torch.bfloat16, device="cuda"))
+    right = [bool(t.all()) for t in (y[:-7] == 1, y[-7:] == -1, rstd[:-7] == rstd[0],
+                                     rstd[-7:] < 0.34)]
+    assert right == [True] * 4
+
+
+def test_step_of_more_sequences_than_one_axis_holds():
+    """Of one channel: S <- e^g S + beta k (v - k S), four roundings of terms of the
+    size below; out = S q."""
+    from mlcg_amd import ops
+
+    n = 2 ** 24 + 3  # one a workgroup
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, state = (torch.randn(n, 1, 1, device="cuda", generator=g) for _ in range(4))
+    decay = -torch.rand(n, 1, device="cuda", generator=g)
+    beta = torch.rand(n, 1, device="cuda", generator=g)
+    q8, k8, v8, want = (t[:, 0, 0].double() for t in (q, k, v, state))
+    want = torch.exp(decay[:, 0].double()) * want
+    want = want + beta[:, 0].double() * k8 * (v8 - k8 * want)
+    state = state[..., None].contiguous()
+    out = ops.gated_delta_step(q, k, v, decay, beta, state, scale=1.0, normalize=False)
+    got = state.view(-1).double()
+    size = 1 + float(k8.abs().max() ** 2 * want.abs().max())
+    off = [float((got - want).abs().max()), float((out[:, 0, 0].double() - got * q8).abs().max())]
+    assert off[0] <= 8 * 2.0 ** -24 * size and off[1] <= 2.0 ** -23 * float((got * q8).abs().max())
+
+
+def test_embedding_gradient_of_more_tokens_than_one_axis_holds():
+    from mlcg_amd import ops
+
+    n = 2 ** 30 + 71  # slabs of 64, one a workgroup
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tokens = torch.arange(n, device="cuda").remainder_(3)
+    table = torch.tensor([[3.0], [-1.0], [2.0]], device="cuda")
+    out = ops.scaled_embedding(table, tokens, 0.5)
+    right = [bool((out[i::3] == 0.5 * table[i]).all()) for i in range(3)]
+    del out
+    grad = torch.zeros(n, 1, device="cuda")
+    at = torch.randint(0, n, (1000,), device="cuda", generator=g)
+    at = torch.cat([at, torch.arange(n - 70, n, device="cuda")]).unique()
+    grad[at] = 1.0
+    got = ops.scaled_embedding_backward(grad, ops.token_order(tokens, 3), 2.0)
+    want = 2.0 * torch.bincount(at % 3, minlength=3).float()
+    assert right == [True] * 3 and torch.equal(got[:, 0], want)
+
+
+def test_look_up_of_more_wide_rows_than_one_axis_holds():
+    from mlcg_amd import ops
+
+    n, width = 2 ** 28 + 21, 257  # 16 a workgroup
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2.2 * n * width:
+        pytest.skip("the output takes 138 GB")
+    tokens = torch.arange(n, device="cuda").remainder_(5)
+    table = torch.randn(5, width, device="cuda").bfloat16()
+    out = ops.scaled_embedding(table, tokens, 2.0)
+    right = [torch.equal(out[at], 2 * table[tokens[at]])
+             for at in (slice(0, 1000), slice(2 ** 27, 2 ** 27 + 1000), slice(n - 1000, n))]
+    right += [torch.equal(out[:, c], (2 * table[:, c])[tokens]) for c in (0, 255, 256)]
+    del out
+    torch.cuda.empty_cache()
+    assert right == [True] * 6
