@@ -44,9 +44,10 @@ class _GatedDelta(torch.autograd.Function):
         own = q.shape[2], v.shape[2]
         out, last, kept = ops._delta_forward(args, own, chains, scale, keep, state, reverse,
                                              normalize, True)
-        q, _, k, _, v, _, decay, beta, *dims = args
+        q, qs, k, ks, v, vs, decay, beta, *dims = args
         ctx.save_for_backward(q, k, v, decay, beta, keep, kept)
-        ctx.plan = (dims, own, chains, scale, reverse, normalize)
+        ctx.arrays = (dims, kept.shape, (q.stride(), k.stride(), v.stride()), (qs, ks, vs))
+        ctx.plan = (own, chains, scale, reverse, normalize)
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -55,8 +56,8 @@ class _GatedDelta(torch.autograd.Function):
     def backward(ctx, grad, grad_last):
         if grad is None and grad_last is None:
             return (None,) * 11
-        dims, own, chains, scale, reverse, normalize = ctx.plan
-        args, keep, kept = ops._delta_saved(*ctx.saved_tensors, dims, chains)
+        own, chains, scale, reverse, normalize = ctx.plan
+        args, keep, kept = ops._delta_saved(ctx.saved_tensors, ctx.arrays, chains)
         if grad is None:
             v = args[4]
             grad = torch.zeros(*v.shape[:2], own[1], dtype=v.dtype, device=v.device)

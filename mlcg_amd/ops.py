@@ -2270,21 +2270,23 @@ def _delta_heads(q, k, v, decay, beta, n: int, what: str):
     """The checked arguments that gated_delta and its step share."""
     require_device(q, k, v, decay, beta)
     dt = _chain_dtype(q, what)
-    dev = q.device
-    q, qs = _attention_heads(q, "q", n, q.dtype, dev)
-    k, ks = _attention_heads(k, "k", n, q.dtype, dev)
-    v, vs = _attention_heads(v, "v", n, q.dtype, dev)
-    keys, dk, heads, dv = q.shape[1], q.shape[2], v.shape[1], v.shape[2]
-    _check(k.shape == q.shape, lambda: f"k must be {tuple(q.shape)} like q, got {tuple(k.shape)}")
+    dev, dtype = q.device, q.dtype
+    q, qs = _attention_heads(q, "q", n, dtype, dev)
+    k, ks = _attention_heads(k, "k", n, dtype, dev)
+    v, vs = _attention_heads(v, "v", n, dtype, dev)
+    shape = q.shape
+    (_, keys, dk), (_, heads, dv) = shape, v.shape
+    _check(k.shape == shape, lambda: f"k must be {tuple(q.shape)} like q, got {tuple(k.shape)}")
     _check(1 <= dk <= MAX_DELTA_DIM and 1 <= dv <= MAX_DELTA_DIM,
            lambda: f"{what} takes heads of 1 .. {MAX_DELTA_DIM} channels, got {dk} and {dv}")
     _check(1 <= keys <= heads <= 1024 and heads % keys == 0,
            lambda: f"the heads of v must be a multiple of those of q and k and at most 1024, got "
                    f"{heads} and {keys}")
-    for t, name in ((decay, "decay"), (beta, "beta")):
-        _check(t.shape == (n, heads) and t.dtype == torch.float32 and t.device == dev,
-               lambda: f"{name} must be [{n}, {heads}] float32 on {dev}, got {tuple(t.shape)} "
-                       f"{t.dtype} on {t.device}")
+    _check(decay.shape == beta.shape == (n, heads) and decay.dtype == beta.dtype == torch.float32
+           and decay.device == beta.device == dev,
+           lambda: f"decay and beta must be [{n}, {heads}] float32 on {dev}, got "
+                   f"{tuple(decay.shape)} {decay.dtype} on {decay.device} and {tuple(beta.shape)} "
+                   f"{beta.dtype} on {beta.device}")
     return (q, qs, k, ks, v, vs, decay.contiguous(), beta.contiguous(), heads, keys, dk, dv, dt)
 
 
@@ -2364,13 +2366,21 @@ def _delta_plan(chains: ChainLayout, heads: int) -> _DeltaPlan:
 
 def _delta_floats(chains: ChainLayout, plan: _DeltaPlan, heads, keys, dk, dv, dt,
                   which: int) -> int:
-    key = ("delta floats", plan.split, plan.segments.shape[0], heads, keys, dk, dv, dt, which)
-    n = chains.plans.get(key)
-    if n is None:
-        n = chains.plans[key] = int(_lib.load().mlcg_gated_delta_floats(
-            chains.tiles[DELTA_ROWS].shape[0], plan.segments.shape[0] if plan.split else 0, heads,
-            keys, dk, dv, dt, which))
-    return n
+    return int(_lib.load().mlcg_gated_delta_floats(
+        chains.tiles[DELTA_ROWS].shape[0], plan.segments.shape[0] if plan.split else 0, heads,
+        keys, dk, dv, dt, which))
+
+
+def _delta_sizes(chains: ChainLayout, *dims):
+    """(plan, floats of kept, of kept with train, of the workspaces of the forward and
+    the backward pass) for (heads, keys, dk, dv, dtype)."""
+    key = ("delta sizes", dims)
+    sizes = chains.plans.get(key)
+    if sizes is None:
+        plan = _delta_plan(chains, dims[0])
+        sizes = chains.plans[key] = (plan, *(_delta_floats(chains, plan, *dims, which)
+                                             for which in range(4)))
+    return sizes
 
 
 def _delta_pad(t: Optional[torch.Tensor], dk: int, dv: int) -> Optional[torch.Tensor]:
@@ -2440,10 +2450,9 @@ def _delta_forward(args, own, chains, scale, keep, state, reverse, normalize, tr
     if n == 0:
         return (out[..., :own[1]], last[..., :own[0], :own[1]].contiguous(),
                 torch.empty(0, dtype=torch.float32, device=dev))
-    plan = _delta_plan(chains, heads)
-    size = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 1 if train else 0)
+    plan, alone, with_train, nws, _ = _delta_sizes(chains, heads, keys, dk, dv, dt)
+    size = with_train if train else alone
     kept = torch.empty(size, dtype=torch.float32, device=dev)
-    nws = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 2)
     ws = torch.empty(nws, dtype=torch.float32, device=dev) if nws > 0 else None
     tiles = chains.tiles[DELTA_ROWS]
     call("mlcg_gated_delta", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), n, heads,
@@ -2469,15 +2478,10 @@ def gated_delta_backward(q, k, v, decay, beta, chains: ChainLayout, kept: torch.
            lambda: f"grad must be {tuple(v.shape)} {q.dtype} on {dev}")
     grad_last = _check_delta_state(grad_last, "grad_last", (chains.n_chains, heads, *own), dev)
     _check(kept.dtype == torch.float32 and kept.device == dev and kept.is_contiguous()
-           and (n == 0 or kept.shape == (_delta_kept(args, chains),)),
+           and (n == 0 or kept.shape == (_delta_sizes(chains, *args[8:])[2],)),
            "kept must be what gated_delta gave with train=True for the same chains")
     return _delta_backward(args, own, chains, _delta_aligned(kept), grad, grad_last, scale, keep,
                            reverse, normalize, want_state)
-
-
-def _delta_kept(args, chains) -> int:
-    heads = args[8]
-    return _delta_floats(chains, _delta_plan(chains, heads), *args[8:], 1)
 
 
 def _delta_aligned(kept: torch.Tensor) -> torch.Tensor:
@@ -2485,24 +2489,27 @@ def _delta_aligned(kept: torch.Tensor) -> torch.Tensor:
     return kept.clone() if kept.data_ptr() % 32 else kept
 
 
-def _delta_saved(q, k, v, decay, beta, keep, kept, dims, chains):
+def _delta_saved(saved, plan, chains):
     """(args, keep, kept) from the arrays that a forward pass saved, as autograd's
     hooks gave them back: the same values, but with strides and addresses of any
-    kind."""
+    kind.  plan: (dims, the size of kept, the forward's strides of q, k and v, the
+    same for the kernels)."""
+    q, k, v, decay, beta, keep, kept = saved
+    dims, size, strides, (qs, ks, vs) = plan
     heads, keys, dk, dv, dt = dims
     n, dtype, dev = chains.n_beads, q.dtype, chains.device
-    q, qs = _attention_heads(q, "q", n, dtype, dev)
-    k, ks = _attention_heads(k, "k", n, dtype, dev)
-    v, vs = _attention_heads(v, "v", n, dtype, dev)
-    args = (q, qs, k, ks, v, vs, decay.contiguous(), beta.contiguous(), *dims)
-    gates, size = (n, heads), _delta_kept(args, chains) if n else 0
-    _check(DTYPE_IDS.get(dtype) == dt and q.shape == k.shape == (n, keys, dk)
-           and v.shape == (n, heads, dv) and decay.shape == beta.shape == gates
+    rows, gates = (n, keys, dk), (n, heads)
+    _check(q.shape == rows and k.shape == rows and v.shape == (n, heads, dv)
+           and decay.shape == gates and beta.shape == gates and kept.shape == size
+           and DTYPE_IDS.get(dtype) == dt and k.dtype == dtype and v.dtype == dtype
            and decay.dtype == beta.dtype == kept.dtype == torch.float32
-           and kept.shape == (size,) and decay.device == beta.device == kept.device == dev
-           and (keep is None or (keep.shape == (n,) and keep.dtype == torch.bool
-                                 and keep.device == dev)),
+           and q.device == k.device == v.device == decay.device == beta.device == kept.device
+           == dev and (keep is None or (keep.shape == (n,) and keep.dtype == torch.bool
+                                        and keep.device == dev)),
            "the arrays that gated_delta saved came back with another shape, type or device")
+    if (q.stride(), k.stride(), v.stride()) != strides:
+        (q, qs), (k, ks), (v, vs) = (_attention_heads(t, "", n, dtype, dev) for t in (q, k, v))
+    args = (q, qs, k, ks, v, vs, decay.contiguous(), beta.contiguous(), *dims)
     return args, None if keep is None else keep.contiguous(), _delta_aligned(kept.contiguous())
 
 
@@ -2530,8 +2537,7 @@ def _delta_backward(args, own, chains, kept, grad, grad_last, scale, keep, rever
         if want_state:
             dstate = dstate[..., :own[0], :own[1]].contiguous()
         return dq[..., :own[0]], dkk[..., :own[0]], dvv[..., :own[1]], ddecay, dbeta, dstate
-    plan = _delta_plan(chains, heads)
-    nws = _delta_floats(chains, plan, heads, keys, dk, dv, dt, 3)
+    plan, _, _, _, nws = _delta_sizes(chains, heads, keys, dk, dv, dt)
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     tiles = chains.tiles[DELTA_ROWS]
     call("mlcg_gated_delta_backward", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta),
@@ -2554,11 +2560,11 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
             and second < first + a.numel() * a.element_size())
 
 
-def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+def _has_tangent(*tensors: torch.Tensor) -> bool:
     """Whether forward-mode differentiation is on and one of these has a tangent."""
     if forward_ad._current_level < 0:  # what unpack_dual asks first, once for all
         return False
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
@@ -2570,23 +2576,22 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     new states take the old ones' place or, given `into`, go there.  No
     derivatives: arrays that ask for one are refused."""
     _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [B, heads, dim]")
-    _check(not (torch.is_grad_enabled()
-                and any(t is not None and t.requires_grad
-                        for t in (q, k, v, decay, beta, state, into))),
+    arrays = (q, k, v, decay, beta, state, state if into is None else into)
+    _check(not (torch.is_grad_enabled() and any([t.requires_grad for t in arrays])),
            "gated_delta_step has no gradients: call it under torch.no_grad()")
-    _check(not _has_tangent(q, k, v, decay, beta, state, into),
+    _check(not _has_tangent(*arrays),
            "gated_delta_step has no forward-mode derivative")
     batch = q.shape[0]
     q, qs, k, ks, v, vs, decay, beta, heads, keys, dk, dv, dt = _delta_heads(
         q, k, v, decay, beta, batch, "gated_delta_step")
     dev, shape = q.device, (batch, heads, dk, dv)
     into = state if into is None else into
-    for t, name in ((state, "state"), (into, "into")):
+    for t, name in ((state, "state"), (into, "into"))[:1 if into is state else 2]:
         require_device(t)
         _check(t.shape == shape and t.dtype == torch.float32 and t.device == dev
                and t.is_contiguous(),
                lambda: f"{name} must be a contiguous {shape} float32 on {dev}")
-    _check(state.data_ptr() == into.data_ptr() or not _overlap(state, into),
+    _check(into is state or state.data_ptr() == into.data_ptr() or not _overlap(state, into),
            "into must be the state itself or not overlap it")
     out = torch.empty(batch, heads, dv, dtype=q.dtype, device=dev)
     call("mlcg_gated_delta_step", ptr(q), qs, ptr(k), ks, ptr(v), vs, ptr(decay), ptr(beta), batch,
