@@ -2339,10 +2339,17 @@ def _delta_segment_tiles(chains: ChainLayout, heads: int) -> int:
     return rows
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 def _delta_plan(chains: ChainLayout, heads: int) -> _DeltaPlan:
     rows = _delta_segment_tiles(chains, heads)
     plan = chains.plans.get(("delta", rows))
     if plan is None:
+        _check(not _capturing(chains.device),
+               "the first gated_delta of a ChainLayout for a number of heads copies its plan "
+               "from the host: make one call like this before the capture")
         lens = np.asarray(chains.lengths, dtype=np.int64)
         order = np.argsort(-lens, kind="stable")
         order = order[lens[order] > 0]
@@ -2430,7 +2437,9 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.
     of a present bead that is no number spoils its chain's outputs from the start of
     its chunk of 64 beads on, and the chain's gradients; no other chain's.  state
     [B, H, DK, DV] float32: where each chain begins (zeros by default); last is
-    where it ends.  kept is what the backward pass takes (train=True)."""
+    where it ends.  kept is what the backward pass takes (train=True).
+    The first call with a layout for a number of heads makes its plan, which cannot be
+    recorded: call once before a capture."""
     args, scale, keep = _delta_args(q, k, v, decay, beta, chains, scale, keep)
     return _delta_forward(args, (q.shape[2], v.shape[2]), chains, scale, keep, state, reverse,
                           normalize, train)

@@ -147,3 +147,17 @@ def test_step_into_a_leaf(calls):
     with pytest.raises(RuntimeError, match="no_grad"):
         ops.gated_delta_step(*args, into=into)
     assert not calls
+
+
+def test_plan_is_not_made_inside_a_capture(monkeypatch, calls):
+    """A plan is copied from the host: a first call inside a capture is refused before
+    anything is recorded, later ones have it."""
+    chains = ops.chain_layout([70, 3], "cpu")
+    monkeypatch.setattr(ops, "_capturing", lambda device: True)
+    _, q, k, v, decay, beta = _heads()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        ops._delta_plan(chains, 4)
+    monkeypatch.undo()
+    plan = ops._delta_plan(chains, 4)
+    monkeypatch.setattr(ops, "_capturing", lambda device: True)
+    assert ops._delta_plan(chains, 4) is plan

@@ -229,3 +229,33 @@ def test_look_up_of_more_wide_rows_than_one_axis_holds():
     del out
     torch.cuda.empty_cache()
     assert right == [True] * 6
+
+
+def test_first_call_inside_a_capture():
+    """Refused with nothing recorded, so that the capture goes on; the same call is
+    recorded after one outside."""
+    from mlcg_amd import ops
+
+    c = base._case([70, 200], 2, 2, 16, 16, torch.float32)
+    args = [c[n] for n in ("q", "k", "v", "decay", "beta")]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first, stream=side):
+            twice = 2 * c["v"]
+            with pytest.raises(RuntimeError, match="before the capture"):
+                ops.gated_delta(*args, c["chains"])
+        first.replay()
+        want = ops.gated_delta(*args, c["chains"])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = ops.gated_delta(*args, c["chains"])
+    torch.cuda.synchronize()
+    assert torch.equal(twice, 2 * c["v"])
+    for _ in range(3):
+        for t in got[:2]:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
