@@ -279,6 +279,8 @@ class ChainEmbedding(torch.nn.Module):
     The table is made anew in every forward pass, as training needs it;
     ``as_embedding()`` gives it as a plain Embedding for simulations."""
 
+    scale: Optional[float] = None  # of modules that were saved before it was theirs
+
     def __init__(self, embedding_size: int, width: int, encoder: torch.nn.Module, types, lengths,
                  keep=None, positions=None, scale: Optional[float] = None):
         super().__init__()

@@ -161,3 +161,17 @@ def test_plan_is_not_made_inside_a_capture(monkeypatch, calls):
     plan = ops._delta_plan(chains, 4)
     monkeypatch.setattr(ops, "_capturing", lambda device: True)
     assert ops._delta_plan(chains, 4) is plan
+
+
+def test_embedding_pickled_without_a_factor():
+    """A ChainEmbedding saved whole before it had a factor is one without."""
+    class Same(torch.nn.Module):
+        def forward(self, x, chains, keep=None, positions=None):
+            return x
+
+    made = nn.ChainEmbedding(4, 8, Same(), [0, 1, 3, 1], (3, 1))
+    state = made.__getstate__()
+    state.pop("scale", None)
+    old = nn.ChainEmbedding.__new__(nn.ChainEmbedding)
+    old.__setstate__(state)
+    assert torch.equal(old.table(), made.table())
