@@ -259,3 +259,78 @@ def test_first_call_inside_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# 16-bit arrays are exact in one or two pieces and what is computed from them has three:
+# the cases of test_gpu_delta.py at p = 2^-24.
+
+SIXTEEN = [torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("lengths", sorted(base.LENGTHS))
+def test_digits_of_lengths(lengths, dtype):
+    base.test_lengths(lengths, dtype)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("dk,dv", [(5, 16), (16, 5), (24, 40), (32, 128), (33, 17), (64, 64),
+                                   (96, 100), (127, 33), (128, 128)])
+def test_digits_of_head_dims(dk, dv, dtype):
+    base.test_head_dims(dk, dv, dtype)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("heads,keys", [(4, 4), (6, 1), (8, 2)])
+def test_digits_of_shared_heads(heads, keys, dtype):
+    base.test_shared_heads(heads, keys, dtype)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("keep", [False, True])
+def test_digits_of_options(keep, normalize, reverse, dtype):
+    base.test_options(keep, normalize, reverse, dtype)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("chunks", [1, 2, 3])
+def test_digits_of_segments(monkeypatch, chunks, dtype):
+    base.test_segments(monkeypatch, chunks, dtype)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+def test_digits_of_other_values(monkeypatch, dtype):
+    base.test_wide_segments(monkeypatch, dtype)
+    base.test_absent_beads(dtype)
+    base.test_equal_keys(dtype)
+    base.test_states_that_grow(dtype)
+
+
+def test_digits_of_decays():
+    base.test_decays(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("scale", [2.0 ** -18, 2.0 ** 8])
+def test_digits_of_gradients_of_any_size(scale, dtype):
+    """Gradients near fp16's smallest and largest numbers: all that they give is as
+    exact as of ordinary ones.  A decay's gradient sums D S: twice |D|_F |S|_F, with D
+    and S taken where a chain begins and ends."""
+    c = base._case([150, 20], 2, 2, 32, 32, dtype, state=True)
+    c["grad_last"] *= 0.0
+    c["grad"] = (c["grad"].float() * scale).to(dtype)
+    got, ref = base._run(c), base._oracle(c)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for name in ("q", "k", "v", "beta", "state", "decay"):
+        size = None
+        if name == "decay":
+            size = 2 * float(ref["state"].flatten(2).norm(dim=2).max()) * max(
+                float(x.flatten(2).norm(dim=2).max())
+                for x in (ref["last"], c["state"].cpu().double()))
+        elif name in ("q", "k"):
+            size = max(float(ref[name].abs().max()), ref[name + "_size"])
+        own = got[name].dtype == dtype
+        base._within(got[name], ref[name], name, base.U[dtype] if own else 2.0 ** -24, 2.0 ** -24,
+                     size, tiny if own else 0.0)
