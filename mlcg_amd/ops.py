@@ -32,6 +32,13 @@ def _check(cond: bool, msg) -> None:
         raise RuntimeError(msg() if callable(msg) else msg)
 
 
+def _rows_of(*tensors: Optional[torch.Tensor]):
+    """The tensors as rows without gaps.  A copy is made here and held by the caller
+    until its launch: one that only the call's argument held would be let go of before
+    the next argument is made, which could be given the same room."""
+    return [None if t is None else t.contiguous() for t in tensors]
+
+
 def _as_i64(t: torch.Tensor) -> torch.Tensor:
     return t.to(torch.int64).contiguous()
 
@@ -826,10 +833,10 @@ def out_forward(x: torch.Tensor, W0: torch.Tensor, b0: Optional[torch.Tensor],
     if seed is not None:
         seed = seed.contiguous().to(torch.float32)
         _check(seed.numel() == n, "seed must have one entry per node")
-    call("mlcg_out_forward", ptr(x), n, NUM_FILTERS, hh, ptr(W0.contiguous()),
-         ptr(None if b0 is None else b0.contiguous()), ptr(w1.contiguous().view(-1)),
-         ptr(None if b1 is None else b1.contiguous()), int(act), int(reverse), ptr(seed),
-         ptr(o), ptr(oz), ptr(os_), ptr(xbar), stream_handle(dev))
+    W0, b0, w1, b1 = _rows_of(W0, b0, w1, b1)
+    call("mlcg_out_forward", ptr(x), n, NUM_FILTERS, hh, ptr(W0), ptr(b0), ptr(w1), ptr(b1),
+         int(act), int(reverse), ptr(seed), ptr(o), ptr(oz), ptr(os_), ptr(xbar),
+         stream_handle(dev))
     return o, oz, os_, xbar
 
 
@@ -843,8 +850,7 @@ def out_rev2(x: torch.Tensor, xdot: Optional[torch.Tensor], W0: torch.Tensor,
     hh = W0.shape[0]
     n = x.shape[0]
     dev = x.device
-    c = lambda t: None if t is None else t.contiguous()  # noqa: E731
-    x, xdot, oz, os_, tw, pw = map(c, (x, xdot, oz, os_, tw, pw))
+    x, xdot, oz, os_, tw, pw, W0, w1 = _rows_of(x, xdot, oz, os_, tw, pw, W0, w1)
     _check(os_ is not None and tuple(os_.shape) == (n, hh), "os must be [N, HH]")
     _check(xdot is None or xdot.shape == x.shape, "xdot must match x")
     _check(not want_odot or xdot is not None, "odot needs a tangent direction")
@@ -856,10 +862,9 @@ def out_rev2(x: torch.Tensor, xdot: Optional[torch.Tensor], W0: torch.Tensor,
     gb1 = torch.empty(1, dtype=torch.float32, device=dev) if has_b1 else None
     nws = int(_lib.load().mlcg_out_rev2_workspace_floats(n, hh))
     ws = torch.empty(max(nws, 1), dtype=torch.float32, device=dev)
-    call("mlcg_out_rev2", ptr(x), ptr(xdot), n, NUM_FILTERS, hh, ptr(W0.contiguous()),
-         ptr(w1.contiguous().view(-1)), ptr(oz), ptr(os_), int(act), ptr(tw), ptr(pw),
-         ptr(odot), ptr(xbar2), ptr(gW0), ptr(gb0), ptr(gW1), ptr(gb1), ptr(ws), nws,
-         stream_handle(dev))
+    call("mlcg_out_rev2", ptr(x), ptr(xdot), n, NUM_FILTERS, hh, ptr(W0), ptr(w1), ptr(oz),
+         ptr(os_), int(act), ptr(tw), ptr(pw), ptr(odot), ptr(xbar2), ptr(gW0), ptr(gb0),
+         ptr(gW1), ptr(gb1), ptr(ws), nws, stream_handle(dev))
     return odot, xbar2, gW0, gb0, gW1, gb1
 
 
@@ -1011,10 +1016,11 @@ def filter_bwd(pos: torch.Tensor, graph: PairGraph, spec: FilterSpec, W1: torch.
     dW1, db1, dW2 = _filter_grads(F, K, dev)
     W1c, b1c, W2c = (t.detach().float().contiguous() for t in (W1, b1, W2))
     ab, adb = _pair_adjoint_outputs(pair_adjoints, cap, F, dev)
+    Wbar, Wdbar = _rows_of(Wbar, Wdbar)
     call("mlcg_filter_bwd", ptr(pos), ptr(graph.pair_ij), cap, ptr(graph.n_pairs_dev), cap,
          *spec.basis_args(), K, spec.rbf_cut_kind, spec.rbf_lo, spec.rbf_hi,
          spec.conv_cut_kind, spec.conv_lo, spec.conv_hi, spec.act, ptr(W1c), ptr(b1c),
-         ptr(W2c), F, ptr(Wbar.contiguous()), ptr(Wdbar.contiguous()), ptr(dW1), ptr(db1),
+         ptr(W2c), F, ptr(Wbar), ptr(Wdbar), ptr(dW1), ptr(db1),
          ptr(dW2), ptr(ab), ptr(adb), ptr(ws), nws, int(strict_fp32), stream_handle(dev))
     if pair_adjoints:
         return dW1, db1, dW2, ab, adb
@@ -1040,12 +1046,12 @@ def filter_bwd_cfconv(pos: torch.Tensor, graph: PairGraph, spec: FilterSpec,
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
     dW1, db1, dW2 = _filter_grads(F, K, dev)
     W1c, b1c, W2c = (t.detach().float().contiguous() for t in (W1, b1, W2))
-    c = lambda t: None if t is None else t.contiguous()  # noqa: E731
+    gagg2, y, gagg1, ydot = _rows_of(gagg2, y, gagg1, ydot)
     ab, adb = _pair_adjoint_outputs(pair_adjoints, cap, F, dev)
     call("mlcg_filter_bwd_cfconv", ptr(pos), ptr(graph.pair_ij), cap, ptr(graph.n_pairs_dev),
          cap, *spec.basis_args(), K, spec.rbf_cut_kind, spec.rbf_lo, spec.rbf_hi,
          spec.conv_cut_kind, spec.conv_lo, spec.conv_hi, spec.act, ptr(W1c), ptr(b1c),
-         ptr(W2c), F, ptr(c(gagg2)), ptr(c(y)), ptr(c(gagg1)), ptr(c(ydot)), ptr(ddot),
+         ptr(W2c), F, ptr(gagg2), ptr(y), ptr(gagg1), ptr(ydot), ptr(ddot),
          ptr(dW1), ptr(db1), ptr(dW2), ptr(ab), ptr(adb), ptr(ws), nws, int(strict_fp32),
          stream_handle(dev))
     if pair_adjoints:
@@ -1076,9 +1082,10 @@ def rbf_param_grad(dist: torch.Tensor, graph: PairGraph, spec: FilterSpec, W1: t
         out = (torch.empty(K, dtype=torch.float32, device=dev),
                torch.empty(K, dtype=torch.float32, device=dev))
     W1c = W1.detach().float().contiguous()
+    abar, adbar = _rows_of(abar, adbar)
     args = (ptr(dist), ptr(graph.n_pairs_dev), cap, *spec.basis_args(), K,
             spec.rbf_cut_kind, spec.rbf_lo, spec.rbf_hi, ptr(W1c), NUM_FILTERS,
-            ptr(abar.contiguous()), ptr(adbar.contiguous()), int(accumulate), ptr(out[0]),
+            ptr(abar), ptr(adbar), int(accumulate), ptr(out[0]),
             ptr(out[1]), ptr(ws), nws)
     if gate is None:
         call("mlcg_rbf_param_grad", *args, stream_handle(dev))
@@ -1485,8 +1492,9 @@ def cfconv_gather(src: torch.Tensor, W: torch.Tensor, graph: PairGraph) -> torch
     if src.dtype == torch.float64:
         _check(W.dtype == torch.float64 and W.shape[1] == src.shape[1],
                "a float64 gather takes float64 filters of the source's width")
-        call("mlcg_cfconv_gather_f64", ptr(src), ptr(W.contiguous()), ptr(graph.rowptr),
-             ptr(graph.col), ptr(graph.eid2pair), graph.num_nodes, src.shape[1], ptr(out),
+        W = W.contiguous()
+        call("mlcg_cfconv_gather_f64", ptr(src), ptr(W), ptr(graph.rowptr), ptr(graph.col),
+             ptr(graph.eid2pair), graph.num_nodes, src.shape[1], ptr(out),
              stream_handle(src.device))
         return out
     wp, wf16 = _wptr(W)
@@ -1502,10 +1510,10 @@ def cfconv_gather_bwd(gagg: torch.Tensor, y: torch.Tensor, W: torch.Tensor, Wd: 
     """ybar = gather(gagg, W); dbar[p] += <Wd_p, gagg_i y_j + gagg_j y_i> in
     place (dbar[p] = ... with accumulate=False: dbar may be uninitialised).
     want_ybar=False: dbar only (the same values), returns None."""
-    gagg = gagg.contiguous()
+    gagg, y = _rows_of(gagg, y)
     ybar = torch.empty_like(gagg) if want_ybar else None
     wp, wf16 = _wptr(W)
-    call("mlcg_cfconv_gather_bwd", ptr(gagg), ptr(y.contiguous()), wp, ptr(Wd), wf16,
+    call("mlcg_cfconv_gather_bwd", ptr(gagg), ptr(y), wp, ptr(Wd), wf16,
          ptr(graph.rowptr), ptr(graph.col), ptr(graph.eid2pair), graph.num_nodes,
          gagg.shape[1], ptr(ybar), ptr(dbar), int(accumulate), stream_handle(gagg.device))
     return ybar
@@ -1513,11 +1521,11 @@ def cfconv_gather_bwd(gagg: torch.Tensor, y: torch.Tensor, W: torch.Tensor, Wd: 
 
 def cfconv_gather_tangent(ydot: Optional[torch.Tensor], y: torch.Tensor, W: torch.Tensor,
                           Wd: torch.Tensor, ddot: torch.Tensor, graph: PairGraph) -> torch.Tensor:
-    y = y.contiguous()
+    y, ydot = _rows_of(y, ydot)
     out = torch.empty_like(y)
-    call("mlcg_cfconv_gather_tangent", ptr(None if ydot is None else ydot.contiguous()),
-         ptr(y), ptr(W), ptr(Wd), ptr(ddot), ptr(graph.rowptr), ptr(graph.col),
-         ptr(graph.eid2pair), graph.num_nodes, y.shape[1], ptr(out), stream_handle(y.device))
+    call("mlcg_cfconv_gather_tangent", ptr(ydot), ptr(y), ptr(W), ptr(Wd), ptr(ddot),
+         ptr(graph.rowptr), ptr(graph.col), ptr(graph.eid2pair), graph.num_nodes, y.shape[1],
+         ptr(out), stream_handle(y.device))
     return out
 
 
@@ -1526,7 +1534,7 @@ def cfconv_gather_rev2(gagg2: torch.Tensor, gagg1: Optional[torch.Tensor], y: to
                        ddot: Optional[torch.Tensor], graph: PairGraph,
                        pair_adjoints: bool = True):
     """ybar2 and (with pair_adjoints) the [P, F] adjoints Wbar, Wdbar."""
-    gagg2 = gagg2.contiguous()
+    gagg2, gagg1, y, ydot = _rows_of(gagg2, gagg1, y, ydot)
     F = gagg2.shape[1]
     ybar2 = torch.empty_like(gagg2)
     cap = graph.pair_capacity
@@ -1534,10 +1542,8 @@ def cfconv_gather_rev2(gagg2: torch.Tensor, gagg1: Optional[torch.Tensor], y: to
     if pair_adjoints:
         Wbar = torch.empty(cap, F, dtype=torch.float32, device=gagg2.device)
         Wdbar = torch.empty(cap, F, dtype=torch.float32, device=gagg2.device)
-    call("mlcg_cfconv_gather_rev2", ptr(gagg2),
-         ptr(None if gagg1 is None else gagg1.contiguous()), ptr(y.contiguous()),
-         ptr(None if ydot is None else ydot.contiguous()), ptr(W), ptr(Wd), ptr(ddot),
-         ptr(graph.rowptr), ptr(graph.col), ptr(graph.eid2pair), graph.num_nodes, F,
+    call("mlcg_cfconv_gather_rev2", ptr(gagg2), ptr(gagg1), ptr(y), ptr(ydot), ptr(W), ptr(Wd),
+         ptr(ddot), ptr(graph.rowptr), ptr(graph.col), ptr(graph.eid2pair), graph.num_nodes, F,
          ptr(ybar2), ptr(Wbar), ptr(Wdbar), stream_handle(gagg2.device))
     return ybar2, Wbar, Wdbar
 
@@ -1546,9 +1552,10 @@ def pair_ddot(pos: torch.Tensor, dist: torch.Tensor, graph: PairGraph,
               u: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """ddot[p] = scale * rhat_p . (u[j] - u[i]) over the graph's pairs."""
     cap = graph.pair_capacity
+    u = u.contiguous()
     ddot = torch.empty(cap, dtype=torch.float32, device=pos.device)
     call("mlcg_pair_ddot", ptr(pos), ptr(dist), ptr(graph.pair_ij), cap,
-         ptr(graph.n_pairs_dev), cap, ptr(u.contiguous()), float(scale), ptr(ddot),
+         ptr(graph.n_pairs_dev), cap, ptr(u), float(scale), ptr(ddot),
          stream_handle(pos.device))
     return ddot
 
@@ -1749,9 +1756,9 @@ def langevin_baoa(pos: torch.Tensor, vel: torch.Tensor, forces: torch.Tensor,
         noise = noise.contiguous()
     if step is not None:
         _check(step.dtype == torch.int64 and step.numel() == 1, "step must be one int64")
+    masses, beta_mass_ratio = _rows_of(masses.to(dt_), beta_mass_ratio.to(dt_))
     call("mlcg_langevin_baoa_f64" if dt_ == torch.float64 else "mlcg_langevin_baoa", ptr(pos),
-         ptr(vel), ptr(forces), ptr(masses.to(dt_).contiguous()),
-         ptr(beta_mass_ratio.to(dt_).contiguous()), n, float(dt), float(vscale),
+         ptr(vel), ptr(forces), ptr(masses), ptr(beta_mass_ratio), n, float(dt), float(vscale),
          float(noisescale), int(seed) & ((1 << 64) - 1), ptr(step), ptr(noise),
          stream_handle(pos.device))
 
@@ -1762,12 +1769,13 @@ def langevin_b(vel: torch.Tensor, forces: torch.Tensor, masses: torch.Tensor, dt
     require_device(vel, forces, masses)
     if vel.dtype == torch.float64:
         _check(forces.dtype == torch.float64, "forces must be float64 with float64 velocities")
-        call("mlcg_langevin_b_f64", ptr(vel), ptr(forces),
-             ptr(masses.to(torch.float64).contiguous()), vel.shape[0], float(dt), ptr(step),
-             stream_handle(vel.device))
+        masses = masses.to(torch.float64).contiguous()
+        call("mlcg_langevin_b_f64", ptr(vel), ptr(forces), ptr(masses), vel.shape[0], float(dt),
+             ptr(step), stream_handle(vel.device))
         return
-    call("mlcg_langevin_b", ptr(vel), ptr(forces), ptr(masses.to(torch.float32).contiguous()),
-         vel.shape[0], float(dt), ptr(step), stream_handle(vel.device))
+    masses = masses.to(torch.float32).contiguous()
+    call("mlcg_langevin_b", ptr(vel), ptr(forces), ptr(masses), vel.shape[0], float(dt),
+         ptr(step), stream_handle(vel.device))
 
 
 def philox_normals(seed: int, step: int, n: int, device) -> torch.Tensor:
