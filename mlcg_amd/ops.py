@@ -2784,11 +2784,15 @@ def scaled_embedding_backward(grad: torch.Tensor, order: TokenOrder, scale: floa
     _check(grad.dim() == 2 and grad.shape[0] == n and grad.device == order.keys.device
            and 1 <= grad.shape[1] <= MAX_RMS_WIDTH,
            lambda: f"grad must be [{n}, channels] on {order.keys.device}")
+    keys, index = order.keys, order.index
+    _check(keys.shape == index.shape == (n,) and keys.dtype == index.dtype == torch.int32
+           and index.device == keys.device and keys.is_contiguous() and index.is_contiguous()
+           and 1 <= order.rows < 2 ** 30, "order must be what token_order gave")
     grad = grad.contiguous()
     width, dev = grad.shape[1], grad.device
     out = torch.empty(order.rows, width, dtype=grad.dtype, device=dev)
     nws = int(_lib.load().mlcg_scaled_embedding_workspace_floats(n, width))
     ws = torch.empty(nws, dtype=torch.float32, device=dev)
-    call("mlcg_scaled_embedding_backward", ptr(grad), ptr(order.keys), ptr(order.index), n,
+    call("mlcg_scaled_embedding_backward", ptr(grad), ptr(keys), ptr(index), n,
          order.rows, width, dt, float(scale), ptr(out), ptr(ws), nws, stream_handle(dev))
     return out

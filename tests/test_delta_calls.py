@@ -175,3 +175,19 @@ def test_embedding_pickled_without_a_factor():
     old = nn.ChainEmbedding.__new__(nn.ChainEmbedding)
     old.__setstate__(state)
     assert torch.equal(old.table(), made.table())
+
+
+def test_orders_that_token_order_did_not_make(calls):
+    """The gradient reads the rows that an order names: arrays that cannot be one are
+    refused."""
+    order = ops.token_order(torch.tensor([1, 0, 1]), 2)
+    grad = torch.zeros(3, 4)
+    short, wide = order.index[:2], order.index.long()
+    for keys, index, rows in ((order.keys, short, 2), (order.keys, wide, 2),
+                              (order.keys.long(), order.index, 2),
+                              (order.keys, order.index.new_zeros(3, 2)[:, 0], 2),
+                              (order.keys, order.index, 0), (order.keys, order.index, 2 ** 30)):
+        with pytest.raises(RuntimeError):
+            ops.scaled_embedding_backward(grad, ops.TokenOrder(keys, index, rows))
+    assert [name for name, _ in calls] == ["mlcg_token_order"]
+    ops.scaled_embedding_backward(grad, order)
