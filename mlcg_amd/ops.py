@@ -2315,35 +2315,43 @@ class _DeltaPlan:
     split: int
 
 
-def _delta_segment_tiles(chains: ChainLayout, heads: int) -> int:
-    """Chunks of a segment, 0 for whole chains: the smallest of the times that
-    these come to, in microseconds.  A workgroup takes about 4 a chunk; two go at a
-    time on each of 256 compute units; segments are gone through twice, and joining
-    them takes about 1.5 each, one after the other, and two launches more.  Measured,
-    forward and backward, in bf16: 2 x 4099 beads, 8 heads of 64, whole 284 and 429,
-    segments of 4, 6, 8 and 16 chunks 101 and 157, 93 and 152, 102 and 162, 136 and
-    222; 64 x 1000, 4 heads of 32, whole 112 and 186, of 8 131 and 219; 1 x 120001, 8
-    heads of 64, whole 8600, of 16 and 32 908 and 786 forward."""
-    rows = chains.plans.get(("delta segment", heads))
+def _delta_segment_tiles(chains: ChainLayout, heads: int, dk: int) -> int:
+    """Chunks of a segment, 0 for whole chains: the smallest of the costs that these
+    come to.  256 workgroups, a chain's or a segment's head each, have a compute unit to
+    themselves; more take turns.  A whole chain's chunk costs 5.6 (4.6 of more than 64
+    key channels); a segment's 9.8, since segments are gone through twice; a join, one
+    after the other, 1.1 (4.1, where maps have one buffer); the launches more 15.  The
+    costs are fitted to the times of both passes, in fp32 and bf16, with which the choice
+    is 1 % slower than the best at 23 sizes in the mean and 10 % at most.  Measured,
+    forward + backward, in us, the choice first: 2 x 4099 beads, 8 heads of 64, bf16,
+    segments of 6 chunks 89 + 127, of 4 and 8 95 + 134 and 97 + 137, whole 249 + 339; the
+    same in fp32, 6 114 + 200, 4 135 + 234, whole 361 + 545; 4 heads of 128, bf16, 6
+    164 + 262, 4 208 + 278, whole 427 + 559; 16 x 1000, 8 heads of 64, fp32, whole 145 +
+    288, 8 155 + 298; 64 x 1000, 4 heads of 32, bf16, whole 103 + 174, 8 126 + 213; 1 x
+    120001, 8 heads of 64, bf16, 64 734 + 1315, 32 791 + 1281; 32 x 2000, 4 heads of 32,
+    bf16, 16 149 + 232, where 8 take 130 + 215."""
+    key = ("delta segment", heads, dk > 64)
+    rows = chains.plans.get(key)
     if rows is None:
         count = -(-np.asarray(chains.lengths, dtype=np.int64) // DELTA_ROWS)
         count = count[count > 0]
         rows = 0
         if count.size:
             longest = int(count.max())
+            chunk, join = (4.6, 4.1) if dk > 64 else (5.6, 1.1)
 
             def rounds(groups):
-                return -(-groups * heads // 512)
+                return -(-groups * heads // 256)
 
-            best = 4.0 * longest * rounds(count.size)
+            best = chunk * longest * rounds(count.size)
             for step in (4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128):
                 if step >= longest:
                     break
                 segs = -(-count // step)
-                cost = 8.0 * step * rounds(int(segs.sum())) + 1.5 * int(segs.max()) + 12.0
+                cost = 9.8 * step * rounds(int(segs.sum())) + join * int(segs.max()) + 15.0
                 if cost < best:
                     best, rows = cost, step
-        chains.plans[("delta segment", heads)] = rows
+        chains.plans[key] = rows
     return rows
 
 
@@ -2351,8 +2359,8 @@ def _capturing(device: torch.device) -> bool:
     return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
-def _delta_plan(chains: ChainLayout, heads: int) -> _DeltaPlan:
-    rows = _delta_segment_tiles(chains, heads)
+def _delta_plan(chains: ChainLayout, heads: int, dk: int = 64) -> _DeltaPlan:
+    rows = _delta_segment_tiles(chains, heads, dk)
     plan = chains.plans.get(("delta", rows))
     if plan is None:
         _check(not _capturing(chains.device),
@@ -2392,7 +2400,7 @@ def _delta_sizes(chains: ChainLayout, *dims):
     key = ("delta sizes", dims)
     sizes = chains.plans.get(key)
     if sizes is None:
-        plan = _delta_plan(chains, dims[0])
+        plan = _delta_plan(chains, dims[0], dims[2])
         sizes = chains.plans[key] = (plan, *(_delta_floats(chains, plan, *dims, which)
                                              for which in range(4)))
     return sizes

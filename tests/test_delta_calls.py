@@ -191,3 +191,13 @@ def test_orders_that_token_order_did_not_make(calls):
             ops.scaled_embedding_backward(grad, ops.TokenOrder(keys, index, rows))
     assert [name for name, _ in calls] == ["mlcg_token_order"]
     ops.scaled_embedding_backward(grad, order)
+
+
+@pytest.mark.parametrize("lengths,heads,dk,best", [
+    ([4099] * 2, 8, 64, 6), ([4099] * 2, 4, 128, 6), ([4099] * 8, 8, 64, 6), ([20000], 8, 128, 12),
+    ([20000], 4, 32, 6), ([2000], 4, 32, 4), ([120001], 8, 64, 64), ([1000] * 64, 4, 32, 0),
+    ([1000] * 16, 8, 64, 0), ([500], 4, 32, 0), ([35], 4, 32, 0), ([0, 0], 1, 1, 0)])
+def test_segments_that_measured_best(lengths, heads, dk, best):
+    """The choice is what was measured fastest (forward and backward together) or within
+    2 % of it."""
+    assert ops._delta_segment_tiles(ops.chain_layout(lengths, "cpu"), heads, dk) == best
