@@ -341,10 +341,16 @@ int emb_forward(const void* table, int rows, const int64_t* tokens, int64_t n, i
 }
 
 // Rows of a slab: long ones leave less to be joined, short ones more to do at the
-// same time.  548864 rows of 256 channels in bf16, 8000 tokens, sums of the slabs
-// and their joins: 90 + 39 us with 32 rows, 88 + 33 with 64, 112 + 19 with 128.
-// 17920 rows of 128 in fp32, 25 tokens: 9.6 + 7.3, 16.0 + 6.3 and 28.0 + 5.7 us.
-int slab_rows(int64_t n) { return n >= (int64_t(1) << 17) ? 64 : 32; }
+// same time: 64 where the gradient has 24 Mi elements in fp32, 96 Mi in 16 bits.  Sums
+// and joins with 32 and 64 rows, us, 25 and 8000 tokens: fp32, 65536 x 128 19 and 26
+// against 26 and 31; 262144 x 64 (16 Mi) 30 and 49 against 32 and 44; 262144 x 128 39 and
+// 57 against 36 and 45; 131072 x 512 59 and 68 against 52 and 60; bf16, 131072 x 256 31
+// and 40 against 43 and 47; 262144 x 256 (64 Mi) 42 and 57 against 48 and 56; 548864 x
+// 128 50 and 66 against 53 and 71; 548864 x 256 89 and 106 against 74 and 97.  128 rows
+// (548864 x 256) took 112 + 19 us, sums and joins, where 64 took 88 + 33.
+int slab_rows(int64_t n, int width, bool fp32) {
+  return n * width >= (int64_t(fp32 ? 24 : 96) << 20) ? 64 : 32;
+}
 
 template <typename T, int SLAB>
 int emb_sums(const void* grad, const int* keys, const int* index, int64_t n, int rows, int width,
@@ -370,7 +376,7 @@ int emb_backward(const void* grad, const int* keys, const int* index, int64_t n,
                      dim3(mlcg_persistent_groups(mlcg_div_up(total, 16 * kEmbThreads), 8)),
                      dim3(kEmbThreads), 0, s, (T*)out, total);
   if (n == 0) return mlcg_launch_status();
-  return slab_rows(n) == 32
+  return slab_rows(n, width, sizeof(T) == 4) == 32
              ? emb_sums<T, 32>(grad, keys, index, n, rows, width, scale, out, ws, s)
              : emb_sums<T, 64>(grad, keys, index, n, rows, width, scale, out, ws, s);
 }
@@ -439,7 +445,7 @@ extern "C" int mlcg_token_order(const int64_t* tokens, int64_t n, int64_t rows, 
 
 extern "C" int64_t mlcg_scaled_embedding_workspace_floats(int64_t n, int width) {
   if (!emb_ok(1, n, width)) return -1;
-  const int slab = slab_rows(n);
+  const int slab = slab_rows(n, width, false);  // the shorter of both types'
   return 2 * ((n + slab - 1) / slab) * width;
 }
 

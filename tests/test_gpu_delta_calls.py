@@ -334,3 +334,28 @@ def test_digits_of_gradients_of_any_size(scale, dtype):
         own = got[name].dtype == dtype
         base._within(got[name], ref[name], name, base.U[dtype] if own else 2.0 ** -24, 2.0 ** -24,
                      size, tiny if own else 0.0)
+
+
+@pytest.mark.parametrize("dtype,width,n", [
+    (torch.float32, 128, 24 * 2 ** 13), (torch.float32, 128, 24 * 2 ** 13 - 1),
+    (torch.float32, 77, 24 * 2 ** 20 // 77 + 40), (torch.bfloat16, 512, 96 * 2 ** 11),
+    (torch.float16, 512, 96 * 2 ** 11 - 1), (torch.bfloat16, 64, 2 ** 17 + 33)])
+def test_embedding_gradient_where_slabs_change(dtype, width, n):
+    """Either side of where slabs of the sorted rows become longer, in runs of all
+    lengths: 8 parts of 2^-24 of the sum of sizes, as in test_gpu_rms_embedding.py, and one
+    rounding."""
+    from mlcg_amd import ops
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    tokens = (torch.rand(n, device="cuda", generator=g) ** 4 * 300).long()
+    grad = torch.randn(n, width, device="cuda", generator=g).to(dtype)
+    got = ops.scaled_embedding_backward(grad, ops.token_order(tokens, 301), 2.0)
+    want, size = (torch.zeros(301, width, dtype=torch.float64, device="cuda") for _ in range(2))
+    for at in range(0, n, 2 ** 16):
+        part = slice(at, at + 2 ** 16)
+        want.index_add_(0, tokens[part], grad[part].double())
+        size.index_add_(0, tokens[part], grad[part].double().abs())
+    off = (got.double() - 2 * want).abs()
+    bound = base.U[dtype] * (2 * want).abs() + 16 * 2.0 ** -24 * size
+    assert bool((off <= bound).all()), float((off / bound.clamp_min(1e-300)).max())
+    assert not bool(got[300].any())
