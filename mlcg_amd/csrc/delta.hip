@@ -4,7 +4,7 @@
 //   S <- e^g S,  u = beta (v - S^T k),  S <- S + k u^T,  o = scale S^T q,
 // reads it once and writes it once; both sums over Dk go through LDS, in a fixed
 // order.  Bound by memory: the states' bytes.  1024 sequences, 8 heads of 64 x 128,
-// bf16: 108 us, 5.0 TB/s; 16 sequences, 4 heads of 32 x 32 in fp32: 6 us, a launch.
+// bf16: 109 us, 5.0 TB/s; 16 sequences, 4 heads of 32 x 32 in fp32: 6 us, a launch.
 #include <type_traits>
 
 #include "delta.h"

@@ -14,10 +14,10 @@
 //
 // Both are bound by memory where there are many rows, by the latency of their
 // launches where there are few.  548864 rows of 256 channels in bf16, 8000 tokens:
-// the look-up 69 us (4.1 TB/s, nearly all of it written); the order 44 us in two
-// passes; the sums 121 us, of which the gradient's 281 MB are 58 at a copy's rate:
+// the look-up 70 us (4.1 TB/s, nearly all of it written); the order 45 us in two
+// passes; the sums 118 us, of which the gradient's 281 MB are 58 at a copy's rate:
 // rows are read in the tokens' order, 512 bytes at a time.  17920 rows of 128 in
-// fp32, 25 tokens: 6 us, 14 us and 18 us.
+// fp32, 25 tokens: 6 us, 14 us and 17 us.
 #include <type_traits>
 
 #include "chain.h"

@@ -15,9 +15,9 @@
 // a fixed order.
 //
 // Bound by memory: x, the residual, y and t once each, dy, dt, t and dx once each.
-// 262144 rows of 512 channels, bf16 beside an fp32 residual: 271 us forward (5.9
+// 262144 rows of 512 channels, bf16 beside an fp32 residual: 267 us forward (6.0
 // TB/s), 412 us backward (4.6 TB/s: three streams read, two written); 17920 rows of
-// 128 in fp32, 10.4 and 10.2 + 4.2 us.
+// 128 in fp32, 9.2 and 9.3 + 4.3 us.
 #include <type_traits>
 
 #include "chain.h"
